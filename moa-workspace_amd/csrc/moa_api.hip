@@ -90,6 +90,8 @@ DevCtx* device_context(hipError_t* err) {
     const size_t t_rflag = carve(sizeof(uint64_t) * kRowsFlagWords);
     const size_t t_attn = carve(sizeof(float) * kAttnPartFloats);
     const size_t t_fattn = carve(sizeof(float) * kFattnPartFloats);
+    const size_t t_plist = carve(sizeof(int32_t) * (2 * (size_t)kPagedMaxPages + 16));
+    const size_t t_ppart = carve(sizeof(float) * kPagedPartFloats);
     int cus = 0;
     *err = hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev);
     if (*err != hipSuccess) return nullptr;
@@ -119,6 +121,8 @@ DevCtx* device_context(hipError_t* err) {
     c.rows_flag = reinterpret_cast<uint64_t*>(b + t_rflag);
     c.attn_part = reinterpret_cast<float*>(b + t_attn);
     c.fattn_part = reinterpret_cast<float*>(b + t_fattn);
+    c.paged_list = reinterpret_cast<int32_t*>(b + t_plist);
+    c.paged_part = reinterpret_cast<float*>(b + t_ppart);
     c.base = base;
     return &c;
 }
@@ -194,6 +198,19 @@ DevCtx* noalloc_context(int* code) {
 }
 }  // namespace
 
+DevCtx* call_context(int* code) {
+    if (g_tripped[current_device_or_0()].load()) { *code = tripped_fail(current_device_or_0()); return nullptr; }
+    hipError_t e;
+    DevCtx* c = device_context(&e);
+    if (!c) *code = hip_fail(e, "allocating the per-device scratch");
+    return c;
+}
+
+int call_result(hipError_t e, const char* what) {
+    if (e != hipSuccess) return hip_fail(e, what);
+    return MOA_SUCCESS;
+}
+
 }  // namespace moa
 
 using namespace moa;
@@ -223,18 +240,9 @@ struct Check {
     }
 };
 
-DevCtx* ctx_or_fail(int* code) {
-    if (g_tripped[current_device_or_0()].load()) { *code = tripped_fail(current_device_or_0()); return nullptr; }
-    hipError_t e;
-    DevCtx* c = device_context(&e);
-    if (!c) *code = hip_fail(e, "allocating the per-device scratch");
-    return c;
-}
+DevCtx* ctx_or_fail(int* code) { return call_context(code); }
 
-int finish(hipError_t e, const char* what) {
-    if (e != hipSuccess) return hip_fail(e, what);
-    return MOA_SUCCESS;
-}
+int finish(hipError_t e, const char* what) { return call_result(e, what); }
 
 int qkv_common(const QkvParams& p, int M, void* stream) {
     Check c;

@@ -70,10 +70,17 @@ constexpr int kOfnCopies = 8;  // copies of O's post-norm words in the single-la
 // one per block of down partial sums, one per normalised row.
 constexpr int kRowsFlagWords = 512;
 
+// The paged cache (moa_paged.hip): page lists and moves, and the split attention's records, f32
+// [16 or 128 query rows][max, sum, out[head_dim]] each: 72 MB, room for 274 records of 128 rows of 512 dims.
+constexpr int kPagedMaxPages = 1 << 20;
+constexpr int kPagedMaxSequences = 1 << 16;
+constexpr size_t kPagedPartFloats = 18 << 20;
+
 // Device-side error bits (OR-ed by kernels; read back by moa_device_errors()).
 constexpr uint32_t kErrRopeOffset = 1u;
 constexpr uint32_t kErrKvOffset = 2u;
 constexpr uint32_t kErrSpinTimeout = 4u;
+constexpr uint32_t kErrPaged = 8u;
 constexpr int kErrTakeOvers = 1;  // err[1]: waits of the one-token kernels that took work over (tests)
 
 // Per-device persistent scratch, allocated once on first use (never per call).
@@ -93,6 +100,8 @@ struct DevCtx {
     uint64_t* rows_flag = nullptr; // tagged flags of the one-launch rows FFN (kRowsFlagWords)
     float* attn_part = nullptr;   // sliding_attention split partials (kAttnPartFloats)
     float* fattn_part = nullptr;  // full-attention page partials (kFattnPartFloats)
+    int32_t* paged_list = nullptr;  // 2 * kPagedMaxPages + 16: page lists of a cache call, its result word
+    float* paged_part = nullptr;    // paged attention's split records (kPagedPartFloats)
     void* base = nullptr;
     int cus = 0;                  // compute units of the device
     int8_t ffn_fused[6] = {-1, -1, -1, -1, -1, -1};  // per (format, scale kind): grid fits resident? (-1 unknown)
@@ -106,6 +115,12 @@ struct DevCtx {
 
 // Returns the context of the current device, allocating it on first use. nullptr on failure.
 DevCtx* device_context(hipError_t* err);
+
+// The context of the current device for a call that computes on it; nullptr, with *code set and the
+// error recorded, where there is none or its state is tripped.
+DevCtx* call_context(int* code);
+// MOA_SUCCESS, or MOA_ERROR_HIP with the reason recorded.
+int call_result(hipError_t e, const char* what);
 
 // Records `msg` as this thread's last error (moa_last_error_string) and returns `code`.
 int set_error(int code, const char* msg);

@@ -1,0 +1,616 @@
+// moa_paged.hip -- the paged KV cache (include/moa_paged.h): argument checks, the calls that change its
+// state (reserve, fork, free, compact), the append of new rows, and the copies of pages.
+//
+// State changes are planned by one workgroup that reads the lengths and the reference counts, checks the whole
+// call, and only then writes: that makes a call all or nothing and its result independent of any order between
+// workgroups. Pages are copied by a second launch over the plan's list of moves.
+#include <string>
+
+#include "../../include/moa_paged.h"
+#include "moa_device.h"
+#include "moa_paged.h"
+
+namespace moa {
+namespace {
+
+constexpr int kPlanBlock = 1024;
+constexpr int kPlanWaves = kPlanBlock / kWave;
+
+// ------------------------------------------------------------------ one workgroup's sums and ranks
+
+// The sum of v over the workgroup, in every thread.
+__device__ uint64_t block_sum(uint64_t v, uint64_t* lds) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, kWave);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+    __syncthreads();
+    uint64_t t = 0;
+#pragma unroll
+    for (int w = 0; w < kPlanWaves; ++w) t += lds[w];
+    return t;
+}
+
+// The sum of v over the threads before this one; *total: over all of them.
+__device__ int block_before(int v, int* lds, int* total) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int x = v;
+#pragma unroll
+    for (int o = 1; o < kWave; o <<= 1) {
+        const int y = __shfl_up(x, o, kWave);
+        if (lane >= o) x += y;
+    }
+    __syncthreads();
+    if (lane == 63) lds[wave] = x;
+    __syncthreads();
+    int before = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < kPlanWaves; ++w) {
+        before += w < wave ? lds[w] : 0;
+        all += lds[w];
+    }
+    *total = all;
+    return before + x - v;
+}
+
+// Calls f(page, rank) for the pages of [from, to) that are free (want_free) or live, in ascending order of rank, until
+// `most` of them; returns how many there were. kPer pages a thread and step, one ballot each, so that a step's loads
+// go out together.
+constexpr int kPer = 8;
+template <class F>
+__device__ int each_page(const int32_t* refs, int from, int to, bool want_free, int most, int* lds, F f) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int found = 0;
+    for (int base = from; base < to && found < most; base += kPlanBlock * kPer) {
+        uint64_t b[kPer];
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+            const int p = base + j * kPlanBlock + (int)threadIdx.x;
+            const bool live = p < to && refs[p] > 0;
+            b[j] = __ballot(p < to && live != want_free);
+        }
+        __syncthreads();  // the step before has read the counts
+        if (lane < kPer) {
+            uint64_t mine = b[0];
+#pragma unroll
+            for (int j = 1; j < kPer; ++j) mine = lane == j ? b[j] : mine;
+            lds[lane * kPlanWaves + wave] = __popcll(mine);
+        }
+        __syncthreads();
+        // every wave scans the step's kPer * kPlanWaves = 128 counts, two a lane
+        const int c0 = lds[2 * lane], c1 = lds[2 * lane + 1];
+        int x = c0 + c1;
+#pragma unroll
+        for (int o = 1; o < kWave; o <<= 1) {
+            const int y = __shfl_up(x, o, kWave);
+            if (lane >= o) x += y;
+        }
+        const int all = __shfl(x, 63, kWave);
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+            const int at = j * kPlanWaves + wave;  // counts before it: the scan of the lane that holds it
+            const int upto = __shfl(x, at >> 1, kWave), odd = __shfl(c1, at >> 1, kWave), even = __shfl(c0, at >> 1, kWave);
+            const int before = upto - odd - ((at & 1) ? 0 : even);
+            const int rank = found + before + __popcll(b[j] & ((1ull << lane) - 1));
+            if ((b[j] >> lane & 1) && rank < most) f(base + j * kPlanBlock + (int)threadIdx.x, rank);
+        }
+        found += all;
+    }
+    __syncthreads();  // what f wrote is seen by the workgroup
+    return min(found, most);
+}
+static_assert(kPer * kPlanWaves == 2 * kWave, "each_page scans two counts a lane");
+
+__device__ __forceinline__ int pages_of(const PagedView& c, int n) { return (int)page_of(c, (uint32_t)(n + (int)c.slots - 1)); }
+
+__device__ __forceinline__ void raise(const PagedView& c) { atomicOr(c.err, kErrPaged); }
+
+// ------------------------------------------------------------------------------------------ reserve
+
+// Thread t takes sequences t, t + 1024, ...: a first pass checks them and counts the pages they need, then the lowest
+// free pages are listed, and a second pass hands them out by the prefix sums of the needs.
+__global__ __launch_bounds__(kPlanBlock) void paged_reserve_kernel(PagedView c, const int32_t* fresh, int32_t* list) {
+    __shared__ uint64_t sums[kPlanWaves];
+    __shared__ int lds[2 * kWave];
+    const int cap = paged_capacity(c);
+    uint64_t need = 0;
+    bool bad = false;
+    for (int s = threadIdx.x; s < c.sequences; s += kPlanBlock) {
+        const int len = c.lens[s], n = fresh[s];
+        if (n < 0 || len < 0 || len > cap || n > cap - len) bad = true;
+        else need += pages_of(c, len + n) - pages_of(c, len);
+    }
+    bad = __syncthreads_or(bad);
+    need = block_sum(need, sums);
+    if (bad || need > (uint64_t)c.pages) {
+        if (threadIdx.x == 0) raise(c);
+        return;
+    }
+    if (each_page(c.refs, 0, c.pages, true, (int)need, lds, [&](int p, int rank) { list[rank] = p; }) < (int)need) {
+        if (threadIdx.x == 0) raise(c);
+        return;
+    }
+    int given = 0;
+    for (int base = 0; base < c.sequences; base += kPlanBlock) {
+        const int s = base + (int)threadIdx.x;
+        const int len = s < c.sequences ? c.lens[s] : 0, n = s < c.sequences ? fresh[s] : 0;
+        const int had = pages_of(c, len), has = pages_of(c, len + n);
+        int all = 0;
+        const int at = given + block_before(has - had, lds, &all);
+        for (int i = had; i < has; ++i) {
+            const int p = list[at + i - had];
+            c.table[s * c.table_stride + i] = p;
+            c.refs[p] = 1;
+        }
+        if (n > 0) c.lens[s] = len + n;
+        given += all;
+    }
+}
+
+// --------------------------------------------------------------------------------------- page copies
+
+// Moves (source page, target page) of every layer's K and V; a negative source is no move. A unit of work is up to
+// kCopyBytes of one page of one tensor: 256 threads, four 16-byte loads each before the first store, so a workgroup
+// has 16 KB in flight.
+constexpr int kCopyBlock = 256;
+constexpr int kCopyBytes = kCopyBlock * 16 * 4;
+
+// Where 16-byte chunk i of a page lies. Dense: slots and heads fill the page without gaps, in either order.
+__device__ __forceinline__ int64_t chunk_at(bool dense, uint32_t i, uint32_t per_row, uint32_t heads, int64_t slot, int64_t head) {
+    if (dense) return (int64_t)i * 16;
+    const uint32_t row = i / per_row, in = i - row * per_row, s = row / heads, h = row - s * heads;
+    return s * slot + h * head + in * 16;
+}
+
+__device__ void copy_pages(const PagedView& c, const int32_t* src, const int32_t* dst, int moves, int elem, int dense_k,
+                           int dense_v, int wg, int wgs) {
+    const uint32_t per_row = (uint32_t)(c.head_dim * elem / 16), chunks = c.slots * (uint32_t)c.kv_heads * per_row;
+    const uint32_t parts = (chunks + kCopyBytes / 16 - 1) / (kCopyBytes / 16);
+    const uint64_t per_move = (uint64_t)parts * 2 * c.layers;
+    for (uint64_t u = wg; u < per_move * moves; u += wgs) {
+        const int m = (int)(u / per_move);
+        const uint32_t r = (uint32_t)(u - m * per_move), tensor = r / parts, part = r - tensor * parts;
+        const int from = src[m], to = dst[m];
+        if (from < 0) continue;
+        const bool v = tensor & 1;
+        uint8_t* base = v ? c.v + (int64_t)(tensor >> 1) * c.v_layer : c.k + (int64_t)(tensor >> 1) * c.k_layer;
+        const int64_t page = v ? c.v_page : c.k_page, slot = v ? c.v_slot : c.k_slot, head = v ? c.v_head : c.k_head;
+        const uint8_t* a = base + from * page;
+        uint8_t* b = base + to * page;
+        const bool dense = v ? dense_v : dense_k;
+        const uint32_t i0 = part * (kCopyBytes / 16) + threadIdx.x;
+        uint4 w[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (i0 + j * kCopyBlock < chunks)
+                w[j] = ld16(a + chunk_at(dense, i0 + j * kCopyBlock, per_row, c.kv_heads, slot, head));
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (i0 + j * kCopyBlock < chunks)
+                *reinterpret_cast<uint4*>(b + chunk_at(dense, i0 + j * kCopyBlock, per_row, c.kv_heads, slot, head)) = w[j];
+    }
+}
+
+// --------------------------------------------------------------------------------------------- fork
+
+// Checks the whole call, then hands out the pages of the partly filled last pages. list: per fork the page to copy (-1:
+// none) and its copy; result: the number of forks, 0 if the call is refused.
+__global__ __launch_bounds__(kPlanBlock) void paged_fork_plan_kernel(PagedView c, const int32_t* parents, const int32_t* children,
+                                                                     int count, int32_t* src, int32_t* dst, int32_t* result) {
+    __shared__ int lds[2 * kWave];
+    __shared__ uint32_t child[kPagedMaxSequences / 32];
+    const int cap = paged_capacity(c);
+    if (threadIdx.x == 0) *result = 0;
+    for (int i = threadIdx.x; i < kPagedMaxSequences / 32; i += kPlanBlock) child[i] = 0;
+    __syncthreads();
+    bool bad = false;
+    for (int f = threadIdx.x; f < count; f += kPlanBlock) {
+        const int s = children[f];
+        if (s < 0 || s >= c.sequences || c.lens[s] != 0) bad = true;
+        else bad |= (atomicOr(&child[s >> 5], 1u << (s & 31)) >> (s & 31) & 1) != 0;
+    }
+    bad = __syncthreads_or(bad);
+    int need = 0;
+    if (!bad) {
+        for (int f = threadIdx.x; f < count; f += kPlanBlock) {
+            const int s = parents[f];
+            if (s < 0 || s >= c.sequences || (child[s >> 5] >> (s & 31) & 1)) { bad = true; continue; }
+            const int len = c.lens[s], full = len < 0 ? 0 : (int)page_of(c, len);
+            if (len < 0 || len > cap) { bad = true; continue; }
+            if (full * (int)c.slots < len) {
+                const int p = c.table[s * c.table_stride + full];
+                if (p < 0 || p >= c.pages) bad = true;
+                ++need;
+            }
+        }
+        bad = __syncthreads_or(bad);
+    }
+    int total = 0;
+    (void)block_before(need, lds, &total);
+    if (bad || total > c.pages ||
+        each_page(c.refs, 0, c.pages, true, total, lds, [&](int p, int rank) { dst[kPagedMaxSequences + rank] = p; }) < total) {
+        if (threadIdx.x == 0) raise(c);
+        return;
+    }
+    int given = 0;
+    for (int base = 0; base < count; base += kPlanBlock) {
+        const int f = base + (int)threadIdx.x;
+        const int s = f < count ? parents[f] : 0, len = f < count ? c.lens[s] : 0, full = (int)page_of(c, len);
+        const bool part = full * (int)c.slots < len;
+        int all = 0;
+        const int at = given + block_before(part, lds, &all);
+        if (f < count) {
+            src[f] = -1;
+            if (part) {
+                const int p = dst[kPagedMaxSequences + at];
+                src[f] = c.table[s * c.table_stride + full];
+                dst[f] = p;
+                c.table[children[f] * c.table_stride + full] = p;
+                c.refs[p] = 1;
+            }
+            c.lens[children[f]] = len;
+        }
+        given += all;
+    }
+    if (threadIdx.x == 0) *result = count;
+}
+
+// The first `count` workgroups each copy one child's table row and count its references; all of them copy pages.
+__global__ __launch_bounds__(kCopyBlock) void paged_fork_kernel(PagedView c, const int32_t* parents, const int32_t* children,
+                                                                const int32_t* src, const int32_t* dst, const int32_t* result,
+                                                                int elem, int dense_k, int dense_v) {
+    const int count = *result;
+    for (int f = blockIdx.x; f < count; f += gridDim.x) {
+        const int s = parents[f], ch = children[f], full = (int)page_of(c, c.lens[ch]);
+        for (int i = threadIdx.x; i < full; i += kCopyBlock) {
+            const int p = c.table[s * c.table_stride + i];
+            c.table[ch * c.table_stride + i] = p;
+            if (p >= 0 && p < c.pages) atomicAdd(c.refs + p, 1);
+            else raise(c);
+        }
+    }
+    copy_pages(c, src, dst, count, elem, dense_k, dense_v, blockIdx.x, gridDim.x);
+}
+
+// --------------------------------------------------------------------------------------------- free
+
+// One workgroup per listed sequence; the first to take its length (an exchange) gives its pages back.
+__global__ __launch_bounds__(kCopyBlock) void paged_free_kernel(PagedView c, const int32_t* sequences, int count) {
+    __shared__ int had;
+    for (int f = blockIdx.x; f < count; f += gridDim.x) {
+        const int s = sequences[f];
+        const bool in = s >= 0 && s < c.sequences;
+        __syncthreads();
+        if (threadIdx.x == 0) had = in ? atomicExch(c.lens + s, 0) : -1;
+        __syncthreads();
+        const int len = had;
+        if (len < 0 || len > paged_capacity(c)) {
+            if (threadIdx.x == 0) raise(c);
+            continue;
+        }
+        for (int i = threadIdx.x; i < pages_of(c, len); i += kCopyBlock) {
+            const int p = c.table[s * c.table_stride + i];
+            if (p < 0 || p >= c.pages) raise(c);
+            else if (atomicSub(c.refs + p, 1) <= 0) {  // the count was wrong: a free page stays at 0
+                atomicAdd(c.refs + p, 1);
+                raise(c);
+            }
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------- compact
+
+// list: place[p] for every page from the number of live pages on (where page p goes, itself if it does not move), and
+// behind kPagedMaxPages the targets and sources of the moves; result: the number of live pages, and of moves.
+__global__ __launch_bounds__(kPlanBlock) void paged_compact_plan_kernel(PagedView c, int32_t* place, int32_t* src, int32_t* dst,
+                                                                        int32_t* result) {
+    __shared__ uint64_t sums[kPlanWaves];
+    __shared__ int lds[2 * kWave];
+    uint64_t n = 0;
+    for (int p = threadIdx.x; p < c.pages; p += kPlanBlock) n += c.refs[p] > 0;
+    const int live = (int)block_sum(n, sums);
+    for (int p = live + (int)threadIdx.x; p < c.pages; p += kPlanBlock) place[p] = p;
+    const int moves = each_page(c.refs, 0, live, true, live, lds, [&](int p, int rank) { dst[rank] = p; });
+    // as many live pages lie behind `live` as free ones before it
+    each_page(c.refs, live, c.pages, false, moves, lds, [&](int p, int rank) {
+        const int to = dst[rank];
+        src[rank] = p;
+        place[p] = to;
+        c.refs[to] = c.refs[p];
+    });
+    for (int i = threadIdx.x; i < moves; i += kPlanBlock) c.refs[src[i]] = 0;
+    if (threadIdx.x == 0) {
+        result[0] = live;
+        result[1] = moves;
+    }
+}
+
+__global__ __launch_bounds__(kCopyBlock) void paged_compact_kernel(PagedView c, const int32_t* place, const int32_t* src,
+                                                                   const int32_t* dst, const int32_t* result, int elem,
+                                                                   int dense_k, int dense_v) {
+    const int live = result[0], moves = result[1];
+    if (!moves) return;
+    for (int s = blockIdx.x; s < c.sequences; s += gridDim.x) {
+        const int len = c.lens[s];
+        if (len < 0 || len > paged_capacity(c)) {
+            if (threadIdx.x == 0) raise(c);
+            continue;
+        }
+        for (int i = threadIdx.x; i < pages_of(c, len); i += kCopyBlock) {
+            const int p = c.table[s * c.table_stride + i];
+            if (p < 0 || p >= c.pages) raise(c);
+            else if (p >= live) c.table[s * c.table_stride + i] = place[p];
+        }
+    }
+    copy_pages(c, src, dst, moves, elem, dense_k, dense_v, blockIdx.x, gridDim.x);
+}
+
+// -------------------------------------------------------------------------------------------- append
+
+// One wave per row: it finds the row's sequence, then moves K and V, 8 elements a lane and step.
+template <bool E4M3>
+__global__ __launch_bounds__(256) void paged_append_kernel(PagedView c, const uint16_t* k, int64_t k_row, const uint16_t* v,
+                                                           int64_t v_row, const int32_t* starts, int rows) {
+    const int lane = threadIdx.x & 63, m = blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (m >= rows) return;
+    const int s = sequence_of(starts, c.sequences, m);
+    if (s < 0 || s >= c.sequences) return;
+    const int end = starts[s + 1], len = c.lens[s], cap = paged_capacity(c);
+    const int t = len - (end - m);
+    if (end <= m) return;  // starts that descend
+    if (end > rows || len < 0 || len > cap || t < 0) {
+        if (lane == 0) raise(c);
+        return;
+    }
+    const uint32_t i = page_of(c, t), slot = t - i * c.slots;
+    const int p = c.table[s * c.table_stride + i];
+    if (p < 0 || p >= c.pages) {
+        if (lane == 0) raise(c);
+        return;
+    }
+    const int per_head = c.head_dim / 8, chunks = c.kv_heads * per_head;
+    uint8_t* kp = c.k + p * c.k_page + slot * c.k_slot;
+    uint8_t* vp = c.v + p * c.v_page + slot * c.v_slot;
+    for (int x = lane; x < 2 * chunks; x += 64) {
+        const bool is_v = x >= chunks;
+        const int y = is_v ? x - chunks : x, h = y / per_head, at = (y - h * per_head) * 8;
+        const uint4 w = ld16((is_v ? v + m * v_row : k + m * k_row) + (int64_t)y * 8);
+        uint8_t* to = is_v ? vp + h * c.v_head : kp + h * c.k_head;
+        if (!E4M3) {
+            *reinterpret_cast<uint4*>(to + at * 2) = w;
+        } else {
+            const float f = is_v ? c.v_scale[h] : c.k_scale[h];
+            float e[8];
+            bf16x8_to_f32(w, e);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                e[j] = __fdiv_rn(e[j], f);
+                e[j] = e[j] > 448.0f ? 448.0f : (e[j] < -448.0f ? -448.0f : e[j]);  // a NaN stays one
+            }
+            uint32_t lo = __builtin_amdgcn_cvt_pk_fp8_f32(e[0], e[1], 0, false);
+            lo = __builtin_amdgcn_cvt_pk_fp8_f32(e[2], e[3], lo, true);
+            uint32_t hi = __builtin_amdgcn_cvt_pk_fp8_f32(e[4], e[5], 0, false);
+            hi = __builtin_amdgcn_cvt_pk_fp8_f32(e[6], e[7], hi, true);
+            *reinterpret_cast<uint2*>(to + at) = make_uint2(lo, hi);
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------ host: the checks
+
+int bad_value(const std::string& msg) { return set_error(MOA_ERROR_INVALID_VALUE, msg.c_str()); }
+
+int check_ptr(const void* p, const char* name, size_t align) {
+    if (!p) return bad_value(std::string(name) + " is NULL");
+    if (reinterpret_cast<uintptr_t>(p) % align)
+        return set_error(MOA_ERROR_MISALIGNED, (std::string(name) + " is not " + std::to_string(align) + "-byte aligned").c_str());
+    return MOA_SUCCESS;
+}
+
+int check_range(int v, int lo, int hi, const char* name) {
+    if (v >= lo && v <= hi) return MOA_SUCCESS;
+    return bad_value(std::string(name) + " must be in [" + std::to_string(lo) + ", " + std::to_string(hi) + "], got " + std::to_string(v));
+}
+
+int elem_bytes(const moa_paged_cache* c) { return c->element == MOA_PAGES_BF16 ? 2 : 1; }
+
+// Strides of one tensor: multiples of 16 bytes, at least a head, within 2^46 elements over the whole tensor.
+int check_strides(const int64_t* st, const moa_paged_cache* c, const char* name) {
+    static const char* dims[4] = {"layer", "page", "slot", "head"};
+    const int64_t size[4] = {c->layers, c->pages, c->slots, c->kv_heads};
+    for (int i = 0; i < 4; ++i) {
+        if (size[i] == 1) continue;
+        if (st[i] < c->head_dim || st[i] % (16 / elem_bytes(c)) || st[i] > (int64_t(1) << 46) / size[i])
+            return bad_value(std::string(name) + ": the " + dims[i] + " stride must be a multiple of 16 bytes, at least head_dim, got " +
+                             std::to_string(st[i]) + " elements");
+    }
+    return MOA_SUCCESS;
+}
+
+// The checks of a cache and, with the call's layer, the view its kernels get.
+int cache_view(const moa_paged_cache* c, int layer, PagedView* v) {
+    if (!c) return bad_value("cache is NULL");
+    int e;
+    if ((e = check_range(c->layers, 1, 1024, "layers")) || (e = check_range(c->pages, 1, kPagedMaxPages, "pages")) ||
+        (e = check_range(c->slots, 1, 65536, "slots")) || (e = check_range(c->kv_heads, 1, 256, "kv_heads")) ||
+        (e = check_range(c->element, MOA_PAGES_BF16, MOA_PAGES_E4M3, "element")) ||
+        (e = check_range(c->sequences, 1, kPagedMaxSequences, "sequences")) ||
+        (e = check_range(c->columns, 1, 1 << 20, "columns")) || (e = check_range(layer, 0, c->layers - 1, "layer")))
+        return e;
+    if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256 && c->head_dim != 512)
+        return bad_value("head_dim must be 64, 128, 256 or 512, got " + std::to_string(c->head_dim));
+    if ((int64_t)c->columns * c->slots > (1 << 30)) return bad_value("columns * slots must be at most 2^30");
+    if (c->table_stride < c->columns || c->table_stride > (int64_t(1) << 40))
+        return bad_value("table_stride must be at least columns, got " + std::to_string(c->table_stride));
+    if ((e = check_ptr(c->k_pages, "k_pages", 16)) || (e = check_ptr(c->v_pages, "v_pages", 16)) ||
+        (e = check_ptr(c->page_table, "page_table", 4)) || (e = check_ptr(c->seq_lens, "seq_lens", 4)) ||
+        (e = check_ptr(c->ref_counts, "ref_counts", 4)))
+        return e;
+    if (c->element == MOA_PAGES_E4M3) {
+        if ((e = check_ptr(c->k_scale, "k_scale", 4)) || (e = check_ptr(c->v_scale, "v_scale", 4))) return e;
+    } else if (c->k_scale || c->v_scale) {
+        return bad_value("bf16 pages have no scales: k_scale and v_scale must be NULL");
+    }
+    if ((e = check_strides(c->k_stride, c, "k_pages")) || (e = check_strides(c->v_stride, c, "v_pages"))) return e;
+    const int b = elem_bytes(c);
+    const bool e4 = c->element == MOA_PAGES_E4M3;
+    v->k_layer = c->k_stride[0] * b, v->k_page = c->k_stride[1] * b, v->k_slot = c->k_stride[2] * b, v->k_head = c->k_stride[3] * b;
+    v->v_layer = c->v_stride[0] * b, v->v_page = c->v_stride[1] * b, v->v_slot = c->v_stride[2] * b, v->v_head = c->v_stride[3] * b;
+    v->k = static_cast<uint8_t*>(c->k_pages) + layer * v->k_layer;
+    v->v = static_cast<uint8_t*>(c->v_pages) + layer * v->v_layer;
+    v->k_scale = e4 ? c->k_scale + (size_t)layer * c->kv_heads : nullptr;
+    v->v_scale = e4 ? c->v_scale + (size_t)layer * c->kv_heads : nullptr;
+    v->table = c->page_table, v->lens = c->seq_lens, v->refs = c->ref_counts;
+    v->table_stride = c->table_stride;
+    v->slots = (uint32_t)c->slots;
+    uint32_t log = 0;
+    while ((1 << log) < c->slots) ++log;
+    v->shift = 31 + log;
+    v->magic = (uint32_t)((uint64_t(1) << v->shift) / (uint32_t)c->slots + 1);
+    v->layers = c->layers, v->pages = c->pages, v->kv_heads = c->kv_heads, v->head_dim = c->head_dim;
+    v->sequences = c->sequences, v->columns = c->columns;
+    v->err = nullptr;
+    return MOA_SUCCESS;
+}
+
+// Whether a page's rows fill it without gaps, slots outside heads or heads outside slots.
+int dense_page(const moa_paged_cache* c, const int64_t* st) {
+    const int64_t d = c->head_dim;
+    const int64_t slot = c->slots == 1 ? c->kv_heads * d : st[2], head = c->kv_heads == 1 ? d : st[3];
+    return (head == d && slot == c->kv_heads * d) || (slot == d && st[3] == c->slots * d);
+}
+
+int64_t copy_units(const moa_paged_cache* c, int64_t moves) {
+    const int64_t bytes = (int64_t)c->slots * c->kv_heads * c->head_dim * elem_bytes(c);
+    return moves * ((bytes + kCopyBytes - 1) / kCopyBytes) * 2 * c->layers;
+}
+
+// Workgroups of a copy launch: one per unit of work, up to the eight of 256 threads that a CU holds; more would
+// only wait.
+int copy_grid(int64_t units, int cus) {
+    const int64_t most = (int64_t)cus * 8;
+    return (int)(units < 1 ? 1 : (units < most ? units : most));
+}
+
+}  // namespace
+}  // namespace moa
+
+using namespace moa;
+
+extern "C" {
+
+int moa_paged_cache_reserve(const moa_paged_cache* cache, const int32_t* new_tokens, void* stream) {
+    PagedView v;
+    int e;
+    if ((e = cache_view(cache, 0, &v)) || (e = check_ptr(new_tokens, "new_tokens", 4))) return e;
+    DevCtx* ctx = call_context(&e);
+    if (!ctx) return e;
+    v.err = ctx->err;
+    hipLaunchKernelGGL(paged_reserve_kernel, dim3(1), dim3(kPlanBlock), 0, static_cast<hipStream_t>(stream), v, new_tokens,
+                       ctx->paged_list);
+    return call_result(hipGetLastError(), "paged_cache_reserve launch");
+}
+
+int moa_paged_cache_append(const moa_paged_cache* cache, const uint16_t* k, int64_t k_row_stride, const uint16_t* v_rows,
+                           int64_t v_row_stride, const int32_t* row_starts, int rows, int layer, void* stream) {
+    PagedView v;
+    int e;
+    if ((e = cache_view(cache, layer, &v)) || (e = check_range(rows, 0, 1 << 20, "rows"))) return e;
+    if (rows == 0) return MOA_SUCCESS;
+    if ((e = check_ptr(k, "k", 16)) || (e = check_ptr(v_rows, "v", 16)) || (e = check_ptr(row_starts, "row_starts", 4))) return e;
+    const int64_t width = (int64_t)v.kv_heads * v.head_dim;
+    for (const int64_t st : {k_row_stride, v_row_stride})
+        if (rows > 1 && (st < width || st % 8 || st > (int64_t(1) << 40)))
+            return bad_value("k and v row strides must be multiples of 8 elements and at least kv_heads * head_dim, got " + std::to_string(st));
+    DevCtx* ctx = call_context(&e);
+    if (!ctx) return e;
+    v.err = ctx->err;
+    auto* f = cache->element == MOA_PAGES_E4M3 ? paged_append_kernel<true> : paged_append_kernel<false>;
+    hipLaunchKernelGGL(f, dim3((rows + 3) / 4), dim3(256), 0, static_cast<hipStream_t>(stream), v, k, k_row_stride, v_rows,
+                       v_row_stride, row_starts, rows);
+    return call_result(hipGetLastError(), "paged_cache_append launch");
+}
+
+int moa_paged_cache_fork(const moa_paged_cache* cache, const int32_t* parents, const int32_t* children, int count, void* stream) {
+    PagedView v;
+    int e;
+    if ((e = cache_view(cache, 0, &v)) || (e = check_range(count, 0, kPagedMaxSequences, "count"))) return e;
+    if (count == 0) return MOA_SUCCESS;
+    if ((e = check_ptr(parents, "parents", 4)) || (e = check_ptr(children, "children", 4))) return e;
+    DevCtx* ctx = call_context(&e);
+    if (!ctx) return e;
+    v.err = ctx->err;
+    int32_t *src = ctx->paged_list, *dst = src + kPagedMaxPages, *result = dst + kPagedMaxPages;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    hipLaunchKernelGGL(paged_fork_plan_kernel, dim3(1), dim3(kPlanBlock), 0, s, v, parents, children, count, src, dst, result);
+    e = call_result(hipGetLastError(), "paged_cache_fork launch");
+    if (e) return e;
+    hipLaunchKernelGGL(paged_fork_kernel, dim3(copy_grid(copy_units(cache, count), ctx->cus)), dim3(kCopyBlock), 0, s, v, parents,
+                       children, src, dst, result, elem_bytes(cache), dense_page(cache, cache->k_stride),
+                       dense_page(cache, cache->v_stride));
+    return call_result(hipGetLastError(), "paged_cache_fork launch");
+}
+
+int moa_paged_cache_free(const moa_paged_cache* cache, const int32_t* sequences, int count, void* stream) {
+    PagedView v;
+    int e;
+    if ((e = cache_view(cache, 0, &v)) || (e = check_range(count, 0, 1 << 20, "count"))) return e;
+    if (count == 0) return MOA_SUCCESS;
+    if ((e = check_ptr(sequences, "sequences", 4))) return e;
+    DevCtx* ctx = call_context(&e);
+    if (!ctx) return e;
+    v.err = ctx->err;
+    hipLaunchKernelGGL(paged_free_kernel, dim3(count < 4096 ? count : 4096), dim3(kCopyBlock), 0, static_cast<hipStream_t>(stream), v,
+                       sequences, count);
+    return call_result(hipGetLastError(), "paged_cache_free launch");
+}
+
+int moa_paged_cache_compact(const moa_paged_cache* cache, void* stream) {
+    PagedView v;
+    int e;
+    if ((e = cache_view(cache, 0, &v))) return e;
+    DevCtx* ctx = call_context(&e);
+    if (!ctx) return e;
+    v.err = ctx->err;
+    // at most half of the pages move: their sources and targets share the second list
+    int32_t *place = ctx->paged_list, *src = place + kPagedMaxPages, *dst = src + kPagedMaxPages / 2, *result = src + kPagedMaxPages;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    hipLaunchKernelGGL(paged_compact_plan_kernel, dim3(1), dim3(kPlanBlock), 0, s, v, place, src, dst, result);
+    e = call_result(hipGetLastError(), "paged_cache_compact launch");
+    if (e) return e;
+    const int64_t units = copy_units(cache, cache->pages / 2);
+    hipLaunchKernelGGL(paged_compact_kernel, dim3(copy_grid(units < cache->sequences ? cache->sequences : units, ctx->cus)),
+                       dim3(kCopyBlock), 0, s, v, place, src, dst, result, elem_bytes(cache), dense_page(cache, cache->k_stride),
+                       dense_page(cache, cache->v_stride));
+    return call_result(hipGetLastError(), "paged_cache_compact launch");
+}
+
+int moa_paged_attention(const uint16_t* q, int64_t q_row_stride, const moa_paged_cache* cache, const int32_t* row_starts,
+                        uint16_t* out, int64_t out_row_stride, int rows, int q_heads, int layer, int window, float scale,
+                        int max_rows, void* stream) {
+    PagedView v;
+    int e;
+    if ((e = cache_view(cache, layer, &v)) || (e = check_range(rows, 0, 1 << 20, "rows")) ||
+        (e = check_range(q_heads, 1, 1 << 15, "q_heads")) || (e = check_range(window, 0, 1 << 30, "window")))
+        return e;
+    if (q_heads % v.kv_heads || q_heads / v.kv_heads > 128)
+        return bad_value("q_heads must be kv_heads times 1 .. 128, got " + std::to_string(q_heads) + " and " + std::to_string(v.kv_heads));
+    if (!(scale > -1e30f && scale < 1e30f)) return bad_value("scale must be finite and below 1e30");
+    if (rows == 0) return MOA_SUCCESS;
+    if ((e = check_range(max_rows, 1, rows, "max_rows")) || (e = check_ptr(q, "q", 16)) || (e = check_ptr(out, "out", 16)) ||
+        (e = check_ptr(row_starts, "row_starts", 4)))
+        return e;
+    const int64_t width = (int64_t)q_heads * v.head_dim;
+    for (const int64_t st : {q_row_stride, out_row_stride})
+        if (rows > 1 && (st < width || st % 8 || st > (int64_t(1) << 40)))
+            return bad_value("q and out row strides must be multiples of 8 elements and at least q_heads * head_dim, got " + std::to_string(st));
+    DevCtx* ctx = call_context(&e);
+    if (!ctx) return e;
+    v.err = ctx->err;
+    const PagedAttentionCall a{q, out, q_row_stride, out_row_stride, row_starts, rows, q_heads, q_heads / v.kv_heads,
+                               window, max_rows, scale * 1.4426950408889634f};
+    return call_result(launch_paged_attention(v, a, static_cast<hipStream_t>(stream), ctx), "paged_attention launch");
+}
+
+}  // extern "C"

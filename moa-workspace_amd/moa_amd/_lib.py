@@ -1,4 +1,4 @@
-"""ctypes binding of libmoa_gfx950.so (declarations mirror include/moa_ops.h and include/moa_ckpt.h).
+"""ctypes binding of libmoa_gfx950.so (declarations mirror include/moa_ops.h, moa_paged.h and moa_ckpt.h).
 
 Loading fails loudly when the library is missing: there is no CPU fallback.
 """
@@ -25,6 +25,7 @@ ERRORS = {
 DEVERR_ROPE_OFFSET = 1
 DEVERR_KV_OFFSET = 2
 DEVERR_SPIN_TIMEOUT = 4
+DEVERR_PAGED = 8
 
 
 class MoaError(RuntimeError):
@@ -85,6 +86,13 @@ SIGNATURES = {
     "moa_test_scratch_state": [U32P],
     "moa_test_trip_device_state": [I32],
     "moa_clear_device_state": [I32],
+    # include/moa_paged.h
+    "moa_paged_cache_reserve": [P, P, P],
+    "moa_paged_cache_append": [P, P, I64, P, I64, P, I32, I32, P],
+    "moa_paged_cache_fork": [P, P, P, I32, P],
+    "moa_paged_cache_free": [P, P, I32, P],
+    "moa_paged_cache_compact": [P, P],
+    "moa_paged_attention": [P, I64, P, P, P, I64, I32, I32, I32, I32, C.c_float, I32, P],
     # include/moa_bench.h
     "moa_bench_stream_read": [P, U64, I32, I32, P, P],
 }

@@ -18,6 +18,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 
 import torch
 
@@ -39,7 +40,8 @@ def _call(name: str, *args) -> None:
         bits = device_errors()
         if bits:
             raise _lib.MoaError(-5, f"{name}: device error bits {bits:#x} (1 rope offset, 2 kv offset, "
-                                    f"4 expired wait: the device state is now tripped, see clear_device_state)")
+                                    f"4 expired wait: the device state is now tripped, see clear_device_state; "
+                                    f"8 paged-cache argument)")
 
 H, L, NS, GS, DS, QS, PS, TS, E, W = 3840, 15360, 8, 2, 256, 4096, 2048, 1024, 32768, 262144
 
@@ -341,6 +343,160 @@ def sliding_attention_output_feedforward_mxfp4(x, post_attn_rms_weight, o_weight
         _ptr(post_ff_rms_weight, "post_ff_rms_weight", _BF16, H), _ptr(layer_scalar, "layer_scalar", _BF16, 8),
     ]
     _call("moa_sliding_attention_output_feedforward_mxfp4", *args, M, _stream(x))
+
+
+# ---- the paged KV cache (include/moa_paged.h; no counterpart in the reference, which serves one sequence)
+
+_PAGED_STRUCT = struct.Struct("=7Q9q8i")  # moa_paged_cache
+
+
+class PagedCache:
+    """Many sequences' K and V over one pool of pages, as the paged_* operators take it. The tensors stay the
+    caller's; this handle checks them once and holds them.
+
+      k_pages, v_pages    bf16, or E4M3 codes (float8_e4m3fn / uint8) [layers, pages, slots, kv_heads, head_dim], or
+                          without the layers; head_dim 64, 128, 256 or 512, dense; other strides multiples of 16 bytes
+      page_table          int32 [sequences, columns], dense rows: position t of sequence s lies in page
+                          page_table[s, t // slots] at slot t % slots
+      seq_lens            int32 [sequences]: positions of each sequence (0: a free one)
+      ref_counts          int32 [pages]: the table entries in use that name the page (0: a free page)
+      k_scale, v_scale    with E4M3 pages: f32 [layers, kv_heads] (or [kv_heads]), a value is code * scale
+
+    A new cache has seq_lens and ref_counts zero. Calls that find a bad value in the state or in an index tensor
+    leave it out and raise bit 8 of device_errors() (each operator says what is left out)."""
+
+    def __init__(self, k_pages, v_pages, page_table, seq_lens, ref_counts, k_scale=None, v_scale=None):
+        for t, name in ((k_pages, "k_pages"), (v_pages, "v_pages"), (page_table, "page_table"), (seq_lens, "seq_lens"),
+                        (ref_counts, "ref_counts")):
+            if not isinstance(t, torch.Tensor):
+                raise TypeError(f"{name} must be a torch.Tensor")
+        k_pages, v_pages = (t.detach()[None] if t.dim() == 4 else t.detach() for t in (k_pages, v_pages))
+        if k_pages.dim() != 5 or k_pages.shape != v_pages.shape:
+            raise ValueError(f"k_pages and v_pages must both be [layers, pages, slots, kv_heads, head_dim], got "
+                             f"{tuple(k_pages.shape)} and {tuple(v_pages.shape)}")
+        if 0 in k_pages.shape:
+            raise ValueError(f"k_pages and v_pages must not be empty, got {tuple(k_pages.shape)}")
+        e4m3 = k_pages.dtype in _U8
+        if k_pages.dtype not in _BF16 + _U8 or (v_pages.dtype in _U8) != e4m3 or v_pages.dtype not in _BF16 + _U8:
+            raise TypeError(f"k_pages and v_pages must both be bf16 or both be E4M3, got {k_pages.dtype} and {v_pages.dtype}")
+        for t, name in ((k_pages, "k_pages"), (v_pages, "v_pages")):
+            if not t.is_cuda:
+                raise ValueError(f"{name} must live on a ROCm device, got {t.device}")
+            if t.stride(4) != 1:
+                raise ValueError(f"{name}: head_dim must be dense")
+        layers, pages, slots, heads, dim = k_pages.shape
+        if page_table.dim() != 2 or page_table.dtype != torch.int32 or (page_table.shape[1] > 1 and page_table.stride(1) != 1):
+            raise ValueError("page_table must be int32 [sequences, columns] with dense rows")
+        if not page_table.is_cuda:
+            raise ValueError(f"page_table must live on a ROCm device, got {page_table.device}")
+        seqs, columns = page_table.shape
+        table_stride = page_table.stride(0) if seqs > 1 else columns
+        self._keep = [k_pages, v_pages, page_table.detach(), seq_lens.detach(), ref_counts.detach()]
+        ptrs = [k_pages.data_ptr(), v_pages.data_ptr()]
+        for t, name in ((k_scale, "k_scale"), (v_scale, "v_scale")):
+            if e4m3 and t is None:
+                raise ValueError(f"E4M3 pages need {name}")
+            if not e4m3 and t is not None:
+                raise ValueError(f"bf16 pages have no scales: {name} must be None")
+            ptrs.append(_ptr(t, name, _F32, layers * heads) or 0)
+            self._keep.append(t if t is None else t.detach())
+        ptrs += [page_table.data_ptr(), _ptr(seq_lens, "seq_lens", _I32, seqs), _ptr(ref_counts, "ref_counts", _I32, pages)]
+        device = k_pages.get_device()
+        if any(t is not None and t.get_device() != device for t in self._keep):
+            raise ValueError("the cache's tensors must live on one device")
+        self.layers, self.pages, self.slots, self.kv_heads, self.head_dim = layers, pages, slots, heads, dim
+        self.sequences, self.columns, self.device_index = seqs, columns, device
+        self._struct = _PAGED_STRUCT.pack(*ptrs, *k_pages.stride()[:4], *v_pages.stride()[:4], table_stride, layers, pages,
+                                          slots, heads, dim, int(e4m3), seqs, columns)
+
+
+def _paged(cache, *indexes):
+    """The stream of a call on `cache`, after the checks of its index tensors (tensor, name, elements or None)."""
+    if not isinstance(cache, PagedCache):
+        raise TypeError("cache must be a PagedCache")
+    ptrs = [_ptr(t, name, _I32, n) for t, name, n in indexes]
+    dev = cache.device_index
+    for t, name, _ in indexes:
+        if t.get_device() != dev:
+            raise ValueError(f"{name} lives on cuda:{t.get_device()}, the cache on cuda:{dev}")
+    return _stream(cache._keep[0]), *ptrs
+
+
+def _row_tensor(t, name, cache, heads):
+    """Address, row stride and rows of a bf16 [rows, heads, head_dim] tensor whose rows may lie apart."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    dev = t.get_device()
+    if dev != cache.device_index:
+        raise ValueError(f"{name} must live on cuda:{cache.device_index} as the cache does, got {t.device}")
+    if t.dtype not in _BF16:
+        raise TypeError(f"{name}: dtype {t.dtype} not in {_BF16}")
+    if t.dim() != 3 or t.shape[2] != cache.head_dim or (heads is not None and t.shape[1] != heads):
+        raise ValueError(f"{name} must be [rows, {heads or 'heads'}, {cache.head_dim}], got {tuple(t.shape)}")
+    rows, h, d = t.shape
+    row, head, one = t.stride()
+    if (one != 1 and d > 1) or (head != d and h > 1):
+        raise ValueError(f"{name}: heads and head_dim must be dense")
+    return t.data_ptr(), (row if rows > 1 else h * d), rows
+
+
+def paged_cache_reserve(cache, new_tokens) -> None:
+    """Grows every sequence s by new_tokens[s] positions (int32 [sequences]): the lowest free pages, in the order of the
+    sequences. All or nothing: where it cannot be served whole the state stays and bit 8 is raised."""
+    s, p = _paged(cache, (new_tokens, "new_tokens", cache.sequences if isinstance(cache, PagedCache) else None))
+    _call("moa_paged_cache_reserve", cache._struct, p, s)
+
+
+def paged_cache_append(cache, k, v, row_starts, layer=0) -> None:
+    """Writes one layer's K and V rows of a step's new tokens: k, v bf16 [rows, kv_heads, head_dim] (rows may lie apart).
+    Rows row_starts[s] .. row_starts[s + 1] - 1 (int32 [sequences + 1]) are the last positions of sequence s, so reserve
+    first. E4M3 pages take the nearest code of x / scale, at most +-448. A row whose position or page is out of range is
+    not written (bit 8)."""
+    s, p = _paged(cache, (row_starts, "row_starts", cache.sequences + 1 if isinstance(cache, PagedCache) else None))
+    kp, kr, rows = _row_tensor(k, "k", cache, cache.kv_heads)
+    vp, vr, vrows = _row_tensor(v, "v", cache, cache.kv_heads)
+    if vrows != rows:
+        raise ValueError(f"v: expected {rows} rows, got {vrows}")
+    _call("moa_paged_cache_append", cache._struct, kp, kr, vp, vr, p, rows, layer, s)
+
+
+def paged_cache_fork(cache, parents, children) -> None:
+    """Makes the empty sequences children[i] copies of parents[i] (int32 [count]): full pages are shared, the partly
+    filled last page of every layer is copied to the lowest free page. All or nothing (bit 8): see moa_paged.h."""
+    n = children.numel() if isinstance(children, torch.Tensor) else None
+    s, p, c = _paged(cache, (parents, "parents", n), (children, "children", n))
+    _call("moa_paged_cache_fork", cache._struct, p, c, n, s)
+
+
+def paged_cache_free(cache, sequences) -> None:
+    """Ends the listed sequences (int32 [count]): their length becomes 0 and their pages lose a reference. Empty and
+    repeated ones change nothing; an index out of range is left out (bit 8)."""
+    s, p = _paged(cache, (sequences, "sequences", None))
+    _call("moa_paged_cache_free", cache._struct, p, sequences.numel(), s)
+
+
+def paged_cache_compact(cache) -> None:
+    """Moves the n live pages to pages 0 .. n - 1 in every layer, page table and reference counts with them: those at n
+    and beyond go, in order, to the free pages below n."""
+    s, = _paged(cache)
+    _call("moa_paged_cache_compact", cache._struct, s)
+
+
+def paged_attention(q, cache, row_starts, out, layer=0, window=0, scale=1.0, max_rows=None) -> None:
+    """Attention of a batch's new rows over one layer of a paged cache, their own positions included (append first).
+    q, out bf16 [rows, q_heads, head_dim] (rows may lie apart; out may be q). Rows row_starts[s] .. row_starts[s + 1] - 1
+    (int32 [sequences + 1]) are the last tokens of sequence s: row i of n stands at position seq_lens[s] - n + i and sees
+    the positions up to its own, the last `window` of them if window > 0. A row that sees nothing gives zeros, rows of no
+    sequence are left as they were. max_rows: the most rows a sequence has in this call (default: all rows; the
+    right number makes the call faster). A sequence with a bad length, bad row starts or more rows than max_rows is left
+    out, and so is at least every row that sees a page outside the pool (bit 8)."""
+    s, p = _paged(cache, (row_starts, "row_starts", cache.sequences + 1 if isinstance(cache, PagedCache) else None))
+    qp, qr, rows = _row_tensor(q, "q", cache, None)
+    op, orow, orows = _row_tensor(out, "out", cache, q.shape[1])
+    if orows != rows:
+        raise ValueError(f"out: expected {rows} rows, got {orows}")
+    _call("moa_paged_attention", qp, qr, cache._struct, p, op, orow, rows, q.shape[1], layer, window, scale,
+          rows if max_rows is None else max_rows, s)
 
 
 def fp8_scaled_projection(x, w, scale, out) -> None:

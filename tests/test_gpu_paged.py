@@ -1,0 +1,723 @@
+"""The paged KV cache on the GPU: attention of new rows against a float64 evaluation, the append's bits, the calls that
+change the cache's state against a plain model, and runs of them together."""
+import itertools
+import random
+
+import pytest
+
+import paged_model as pm
+from gpu_util import need_gpu, say, torch
+from moa_amd import _lib, ops
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+def i32(v):
+    return torch.tensor(v, dtype=torch.int32, device=DEV)
+
+
+def pool(layers, pages, slots, heads, dim, dtype, layout):
+    """K and V views [layers, pages, slots, heads, dim] of a layout: nhd (dense), hnd (heads outside slots), pairs (K
+    and V pages side by side in one allocation), slots (K and V side by side in every slot)."""
+    if layout == "nhd":
+        return tuple(torch.zeros((layers, pages, slots, heads, dim), dtype=dtype, device=DEV) for _ in range(2))
+    if layout == "hnd":
+        return tuple(torch.zeros((layers, pages, heads, slots, dim), dtype=dtype, device=DEV).transpose(2, 3) for _ in range(2))
+    if layout == "pairs":
+        t = torch.zeros((layers, pages, 2, slots, heads, dim), dtype=dtype, device=DEV)
+        return t[:, :, 0], t[:, :, 1]
+    t = torch.zeros((layers, pages, slots, 2, heads, dim), dtype=dtype, device=DEV)
+    return t[:, :, :, 0], t[:, :, :, 1]
+
+
+class Setup:
+    """A cache with sequences of the given lengths in shuffled pages, and its plain state."""
+
+    def __init__(self, lens, slots, heads, dim, fmt="bf16", layers=1, seed=0, spare=3, columns=None, layout="nhd", poison=False):
+        g = torch.Generator().manual_seed(seed)
+        self.fmt, self.slots, self.heads, self.dim, self.layers = fmt, slots, heads, dim, layers
+        used = [pm.pages_of(n, slots) for n in lens]
+        pages, columns = sum(used) + spare, columns or max(used + [1])
+        order = torch.randperm(pages, generator=g).tolist()
+        table, refs = [], [0] * pages
+        for n in used:
+            table.append([order.pop() for _ in range(n)] + [-7] * (columns - n))
+            for p in table[-1][:n]:
+                refs[p] = 1
+        self.state = pm.State(table, lens, refs, slots)
+        self.table, self.lens, self.refs = i32(table), i32(lens), i32(refs)
+        dtype = torch.bfloat16 if fmt == "bf16" else torch.float8_e4m3fn
+        self.k, self.v = pool(layers, pages, slots, heads, dim, dtype, layout)
+        gd = torch.Generator(device=DEV).manual_seed(seed + 1)
+        for t in (self.k, self.v):
+            x = torch.randn(t.shape, generator=gd, device=DEV)
+            t.copy_(x.to(torch.bfloat16) if fmt == "bf16" else (x * 60).clamp(-448, 448).to(dtype))
+        self.k_scale = self.v_scale = None
+        if fmt == "e4m3":
+            self.k_scale, self.v_scale = ((torch.rand((layers, heads), generator=gd, device=DEV) + 0.5) / 60 for _ in range(2))
+        if poison:  # every slot that no position occupies holds NaN
+            hold = torch.zeros((pages, slots), dtype=torch.bool)
+            for s, n in enumerate(lens):
+                for t in range(n):
+                    hold[table[s][t // slots], t % slots] = True
+            bad = ~hold.to(DEV)
+            for t in (self.k, self.v):
+                b = t if fmt == "bf16" else t.view(torch.uint8)
+                b[:, bad] = float("nan") if fmt == "bf16" else 0x7F
+        self.cache = ops.PagedCache(self.k, self.v, self.table, self.lens, self.refs, self.k_scale, self.v_scale)
+
+    def values(self, layer=0):
+        return self.k[layer].float(), self.v[layer].float()
+
+    def check_state(self):
+        """Everything in use: lengths, reference counts, and the table up to each sequence's pages."""
+        assert self.lens.tolist() == self.state.lens
+        assert self.refs.tolist() == self.state.refs
+        for s, row in enumerate(self.table.tolist()):
+            n = pm.pages_of(self.state.lens[s], self.slots)
+            assert row[:n] == self.state.table[s][:n], f"sequence {s}"
+
+
+def queries(rows, heads, dim, seed, spread=2.0):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    return (torch.randn((rows, heads, dim), generator=g, device=DEV) * spread / dim ** 0.5).to(torch.bfloat16)
+
+
+def starts_of(rows, first=0):
+    return [first] + list(itertools.accumulate(rows, initial=first))[1:]
+
+
+def check_rows(got, want, a, d, dim, rows=None):
+    """|got - want| within: half a bf16 step of the result (2^-8 relative); weights rounded to bf16, at most 2^-8 of each,
+    which moves the result by at most 2^-8 a; scores rounded as f32 sums of `dim` products (dim + 4 roundings of 2^-24
+    relative to sum |q k|), which moves every weight and the sum by that much: twice; exponentials, sums and the
+    division in f32: 2^-18 of a covers them (exp2 of a rounded argument below 2^7, sums of up to 2^15 weights)."""
+    sel = slice(None) if rows is None else rows
+    got, want, a, d = got.double()[sel], want[sel], a[sel], d[sel]
+    assert torch.isfinite(got).all()
+    tol = 2.0 ** -8 * want.abs() + (1 + 2.0 ** -8) * a * (2.0 ** -8 + 2.0 ** -18 + 2 * (dim + 4) * 2.0 ** -24 * d[..., None]) + 1e-30
+    over = ((got - want).abs() - tol).max().item() if got.numel() else 0.0
+    assert over <= 0, f"beyond the tolerance by {over}; worst |d| {(got - want).abs().max().item()}"
+
+
+def attend(st, rows, heads, window=0, scale=1.0, seed=5, first=0, tail=0, max_rows=None, layer=0, q=None, out=None):
+    """One call on a Setup; checks every row, and that rows outside the sequences keep what they held."""
+    starts = starts_of(rows, first)
+    R = starts[-1] + tail
+    q = queries(R, heads, st.dim, seed, 2.0 / scale) if q is None else q
+    out = torch.full((R, heads, st.dim), 123.0, dtype=torch.bfloat16, device=DEV) if out is None else out
+    qc = q.clone()
+    ops.paged_attention(q, st.cache, i32(starts), out, layer=layer, window=window, scale=scale, max_rows=max_rows)
+    assert ops.device_errors() == 0
+    k, v = st.values(layer)
+    sc = (None, None) if st.k_scale is None else (st.k_scale[layer], st.v_scale[layer])
+    want, a, d = pm.attention(qc, k, v, st.state.table, st.state.lens, starts, st.slots, window, scale, *sc)
+    inside = slice(first, starts[-1])
+    check_rows(out, want, a, d, st.dim, inside)
+    for t in (out[:first], out[starts[-1]:]):
+        assert out.data_ptr() == q.data_ptr() or (t == 123.0).all()
+    return out
+
+
+LAYOUTS = [(2, 8, 256), (16, 1, 512), (4, 8, 128), (1, 3, 64), (7, 2, 128), (12, 2, 64), (1, 2, 512), (5, 1, 256), (40, 1, 64)]
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "e4m3"])
+@pytest.mark.parametrize("group,heads,dim", LAYOUTS)
+def test_single_tokens_of_ragged_sequences(group, heads, dim, fmt):
+    need_gpu()
+    say(f"paged attention tokens G{group} x {heads} x {dim} {fmt}")
+    lens = [1, 2, 31, 32, 33, 127, 128, 129, 700, 0, 2051]
+    st = Setup(lens, 24, heads, dim, fmt, seed=1, poison=True)
+    attend(st, [1] * len(lens), group * heads, max_rows=1)
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "e4m3"])
+@pytest.mark.parametrize("group,heads,dim", LAYOUTS)
+def test_chunks_beside_tokens(group, heads, dim, fmt):
+    need_gpu()
+    say(f"paged attention mixed G{group} x {heads} x {dim} {fmt}")
+    rows = [1, 130, 0, 3, 64, 1, 17]
+    lens = [600, 130, 50, 3, 371, 1, 16]  # the last has a row before position 0
+    st = Setup(lens, 40, heads, dim, fmt, seed=2, poison=True)
+    attend(st, rows, group * heads, first=2, tail=3)
+
+
+@pytest.mark.parametrize("window", [1, 16, 100, 129, 1024])
+@pytest.mark.parametrize("fmt", ["bf16", "e4m3"])
+def test_window(window, fmt):
+    need_gpu()
+    say(f"paged attention window {window} {fmt}")
+    rows, lens = [1, 2, 150, 0, 1, 77], [1500, 2, 900, 5, 0, 77]
+    st = Setup(lens, 48, 8, 256, fmt, seed=3, poison=True)
+    attend(st, rows, 16, window=window)
+
+
+@pytest.mark.parametrize("slots", [1, 7, 16, 32, 64, 100, 512])
+@pytest.mark.parametrize("layout", ["nhd", "hnd", "pairs", "slots"])
+def test_page_sizes_and_layouts(slots, layout):
+    need_gpu()
+    say(f"paged attention pages of {slots}, {layout}")
+    for fmt, dim in (("bf16", 128), ("e4m3", 256)):
+        rows, lens = [1, 90, 4], [333, 290, 64]
+        st = Setup(lens, slots, 2, dim, fmt, layers=2, seed=4, layout=layout, poison=True)
+        attend(st, rows, 8, layer=1)
+
+
+@pytest.mark.parametrize("group,heads,dim,fmt", [(16, 1, 512, "bf16"), (2, 8, 256, "e4m3"), (4, 2, 128, "bf16")])
+def test_long_sequences_split(group, heads, dim, fmt):
+    need_gpu()
+    say(f"paged attention long G{group} x {heads} x {dim} {fmt}")
+    for rows, lens in (([1], [32768]), ([4, 1], [20000, 3]), ([70], [9000]), ([300, 1, 2], [5000, 8001, 1])):
+        st = Setup(lens, 512, heads, dim, fmt, seed=6)
+        attend(st, rows, group * heads, max_rows=max(rows))
+
+
+def test_many_sequences():
+    need_gpu()
+    say("paged attention of 700 sequences, most without rows")
+    r = random.Random(1)
+    lens = [r.randrange(0, 90) for _ in range(700)]
+    rows = [r.choice([0, 0, 0, 1, 1, 2, 30]) if n else 0 for n in lens]
+    rows = [min(n, x) for n, x in zip(lens, rows)]
+    st = Setup(lens, 16, 2, 64, seed=7, poison=True)
+    attend(st, rows, 8)
+
+
+def test_rows_apart_and_in_place():
+    need_gpu()
+    say("paged attention with strided q and out, and out = q")
+    rows, lens = [3, 1, 60], [100, 50, 200]
+    st = Setup(lens, 32, 2, 128, seed=8)
+    big = queries(64, 12, 128, 9)
+    q = big[:, 2:10]
+    out = torch.full((64, 3, 8, 128), 9.0, dtype=torch.bfloat16, device=DEV)[:, 1]
+    attend(st, rows, 8, q=q, out=out)
+    q2 = queries(64, 8, 128, 9)
+    attend(st, rows, 8, q=q2, out=q2)
+
+
+def test_scale_and_large_scores():
+    need_gpu()
+    say("paged attention with scores of some hundreds, and a negative scale")
+    st = Setup([400, 90], 32, 2, 128, seed=10)
+    for scale in (1.0, -0.5, 0.0883):
+        attend(st, [1, 50], 8, scale=scale, q=queries(51, 8, 128, 11, 60.0))
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "e4m3"])
+@pytest.mark.parametrize("rows", [[4], [100], [1]])
+@pytest.mark.parametrize("window", [0, 40])
+def test_values_of_positions_that_a_row_does_not_see_never_reach_it(rows, window, fmt):
+    """K and V of every new token are infinite or NaN: rows before it are unharmed."""
+    need_gpu()
+    n = rows[0]
+    say(f"paged attention, non-finite later tokens, {n} rows window {window} {fmt}")
+    st = Setup([300], 16, 2, 128, fmt, seed=12)
+    clean_k, clean_v = (t.clone() for t in st.values())
+    last = 299
+    page, slot = st.state.table[0][last // 16], last % 16
+    for t, x in ((st.k, float("inf")), (st.v, float("nan"))):
+        if fmt == "bf16":
+            t[0, page, slot] = x
+        else:
+            t.view(torch.uint8)[0, page, slot] = 0x7F
+    if window and n < 300 - window:  # and what the window has left behind
+        old = 300 - n - window
+        page, slot = st.state.table[0][old // 16], old % 16
+        (st.v if fmt == "bf16" else st.v.view(torch.uint8))[0, page, slot] = float("nan") if fmt == "bf16" else 0x7F
+    q = queries(n, 8, 128, 13)
+    out = torch.zeros_like(q)
+    ops.paged_attention(q, st.cache, i32([0, n]), out, window=window)
+    assert ops.device_errors() == 0
+    sc = (None, None) if st.k_scale is None else (st.k_scale[0], st.v_scale[0])
+    want, a, d = pm.attention(q, clean_k, clean_v, st.state.table, [300], [0, n], 16, window, 1.0, *sc)
+    check_rows(out, want, a, d, 128, slice(0, n - 1))
+    assert torch.isnan(out[n - 1].float()).any()
+
+
+def test_offsets_past_32_bits():
+    need_gpu()
+    say("paged attention and append in a pool of 5.4 GB")
+    slots, heads, dim, pages = 64, 8, 256, 20500
+    k = torch.empty((1, pages, slots, heads, dim), dtype=torch.bfloat16, device=DEV)
+    v = torch.empty_like(k)
+    assert k.numel() * 2 > 1 << 32
+    table = [[pages - 1, 0, pages - 2, 17000]]
+    st = pm.State(table, [250], [0] * pages, slots)
+    for p in table[0]:
+        k[0, p], v[0, p] = queries(slots, heads, dim, p, 16.0), queries(slots, heads, dim, p + 1, 16.0)
+    cache = ops.PagedCache(k, v, i32(table), i32([250]), i32(st.refs))
+    nk, nv = queries(40, heads, dim, 3, 16.0), queries(40, heads, dim, 4, 16.0)
+    ops.paged_cache_append(cache, nk, nv, i32([0, 40]))
+    for i in range(40):
+        t = 210 + i
+        assert torch.equal(k[0, table[0][t // slots], t % slots], nk[i]) and torch.equal(v[0, table[0][t // slots], t % slots], nv[i])
+    for n in (1, 40):
+        q = queries(n, 16, dim, 5)
+        out = torch.empty_like(q)
+        ops.paged_attention(q, cache, i32([0, n]), out)
+        assert ops.device_errors() == 0
+        low = i32(sorted(set(table[0]))).long()
+        small = {int(p): i for i, p in enumerate(low)}
+        want, a, d = pm.attention(q, k[0, low].float(), v[0, low].float(), [[small[p] for p in table[0]]], [250], [0, n], slots, 0, 1.0)
+        check_rows(out, want, a, d, dim)
+
+
+# ------------------------------------------------------------------------------- bad device arguments
+
+@pytest.mark.parametrize("n", [1, 90])
+@pytest.mark.parametrize("bad", ["page_high", "page_negative", "len_negative", "len_long", "rows_over", "row_end"])
+def test_bad_sequences_are_left_out(bad, n):
+    need_gpu()
+    say(f"paged attention, {bad}, {n} rows")
+    st = Setup([200, 210, 220], 16, 2, 128, seed=14, columns=14)
+    table, lens, starts, max_rows = [list(r) for r in st.state.table], list(st.state.lens), [0, n, 2 * n, 3 * n], n
+    if bad == "page_high":
+        table[1][2] = len(st.state.refs)
+    elif bad == "page_negative":
+        table[1][2] = -1
+    elif bad == "len_negative":
+        lens[1] = -3
+    elif bad == "len_long":
+        lens[1] = 14 * 16 + 1
+    elif bad == "rows_over":
+        starts, max_rows = [0, n, 3 * n + 1, 4 * n + 1], 2 * n
+    elif bad == "row_end":
+        starts = [0, n, 2 * n, 9 * n]
+    st.table.copy_(i32(table))
+    st.lens.copy_(i32(lens))
+    R = 4 * n + 1
+    q = queries(R, 8, 128, 15)
+    out = torch.full_like(q, 123.0)
+    ops.paged_attention(q, st.cache, i32(starts), out, max_rows=max_rows)
+    assert ops.device_errors() == _lib.DEVERR_PAGED
+    k, v = st.values()
+    left = 2 if bad == "row_end" else 1
+    ok_lens = [st.state.lens[s] for s in range(3)]
+    ok_starts = [min(x, R) for x in starts]
+    want, a, d = pm.attention(q, k, v, st.state.table, ok_lens, ok_starts, 16, 0, 1.0)
+    for s in range(3):
+        rows = slice(ok_starts[s], ok_starts[s + 1])
+        if s == left:
+            assert (out[rows] == 123.0).all()
+        else:
+            check_rows(out, want, a, d, 128, rows)
+    assert (out[ok_starts[3]:] == 123.0).all()
+
+
+def test_append_leaves_out_bad_rows():
+    need_gpu()
+    say("append: positions and pages out of range")
+    st = Setup([20, 3, 40], 16, 2, 64, seed=16, columns=3)
+    st.table[2, 2] = 1 << 30
+    before_k, before_v = st.k.clone(), st.v.clone()
+    k, v = queries(19, 2, 64, 1, 8.0), queries(19, 2, 64, 2, 8.0)
+    ops.paged_cache_append(st.cache, k, v, i32([1, 3, 8, 18]))  # 5 rows of a 3-long sequence; the third's end in a bad page
+    assert ops.device_errors() == _lib.DEVERR_PAGED
+    for m, s, t in pm.positions([1, 3, 8, 18], [20, 3, 40]):
+        if t >= 0 and not (s == 2 and t >= 32):
+            p = st.state.table[s][t // 16]
+            before_k[0, p, t % 16], before_v[0, p, t % 16] = k[m], v[m]
+    assert torch.equal(st.k, before_k) and torch.equal(st.v, before_v)
+
+
+# ------------------------------------------------------------------------------------------- append
+
+@pytest.mark.parametrize("layout", ["nhd", "hnd", "slots"])
+@pytest.mark.parametrize("heads,dim", [(8, 256), (1, 512), (3, 64), (5, 128)])
+def test_append_bits(heads, dim, layout):
+    need_gpu()
+    say(f"append {heads} x {dim} {layout}")
+    rows, lens = [1, 70, 0, 5], [33, 70, 12, 300]
+    starts = starts_of(rows)
+    for fmt in ("bf16", "e4m3"):
+        st = Setup(lens, 24, heads, dim, fmt, layers=2, seed=17, layout=layout)
+        want_k, want_v = st.k.clone(), st.v.clone()
+        wide = queries(starts[-1], 2 * heads + 1, dim, 18, dim ** 0.5)
+        k, v = wide[:, 1:1 + heads], wide[:, 1 + heads:]
+        if fmt == "e4m3":  # values over the largest code, ties, signed zeros, infinities and NaN
+            special = torch.tensor([1e9, -1e9, 0.0, -0.0, float("inf"), float("-inf"), float("nan"), 2.0 ** -30], device=DEV)
+            wide[2].view(-1)[:8 * ((2 * heads + 1) * dim // 8)] = special.repeat((2 * heads + 1) * dim // 8).to(torch.bfloat16)
+        ops.paged_cache_append(st.cache, k, v, i32(starts), layer=1)
+        assert ops.device_errors() == 0
+        for x, want, scale in ((k, want_k, st.k_scale), (v, want_v, st.v_scale)):
+            if fmt == "e4m3":
+                x = (x.float() / scale[1][:, None]).clamp(-448, 448).to(torch.float8_e4m3fn).view(torch.uint8)
+                want = want.view(torch.uint8)
+            for m, s, t in pm.positions(starts, lens):
+                want[1, st.state.table[s][t // 24], t % 24] = x[m]
+        for got, want in ((st.k, want_k), (st.v, want_v)):
+            if fmt == "e4m3":
+                got, want = got.view(torch.uint8), want.view(torch.uint8)
+                nan = (want & 0x7F) == 0x7F  # a NaN's sign is free
+                assert torch.equal((got & 0x7F) == 0x7F, nan) and torch.equal(got[~nan], want[~nan])
+            else:
+                assert torch.equal(got.view(torch.int16), want.view(torch.int16))
+
+
+# ------------------------------------------------------------------------------------- state changes
+
+def move_pages(st, k, v):
+    for a, b in st.state.moves:
+        k[:, b], v[:, b] = k[:, a].clone(), v[:, a].clone()
+
+
+def raw(t):
+    return t.view(torch.int16) if t.dtype == torch.bfloat16 else t.view(torch.uint8)
+
+
+def test_reserve_takes_the_lowest_free_pages():
+    need_gpu()
+    say("reserve")
+    st = Setup([10, 0, 33, 16], 16, 1, 64, seed=19, spare=40, columns=30)
+    for new in ([1, 1, 1, 1], [0, 0, 0, 0], [0, 100, 0, 300], [6, 0, 14, 0]):
+        ops.paged_cache_reserve(st.cache, i32(new))
+        assert st.state.reserve(new) and ops.device_errors() == 0
+        st.check_state()
+
+
+@pytest.mark.parametrize("new", [[0, 0, -1, 0], [0, 0, 0, 30 * 16], [16 * 20, 16 * 20, 16 * 20, 0], [2 ** 31 - 1, 0, 0, 0]])
+def test_reserve_is_all_or_nothing(new):
+    need_gpu()
+    say(f"reserve refused {new}")
+    st = Setup([10, 0, 33, 16], 16, 1, 64, seed=19, spare=40, columns=30)
+    before = st.table.clone()
+    ops.paged_cache_reserve(st.cache, i32(new))
+    assert ops.device_errors() == _lib.DEVERR_PAGED and not st.state.reserve(new)
+    st.check_state()
+    assert torch.equal(st.table, before)
+
+
+@pytest.mark.parametrize("layout", ["nhd", "hnd", "pairs", "slots"])
+@pytest.mark.parametrize("fmt", ["bf16", "e4m3"])
+def test_fork_shares_full_pages_and_copies_the_last(layout, fmt):
+    need_gpu()
+    say(f"fork {layout} {fmt}")
+    st = Setup([70, 48, 5, 0, 0, 0, 0, 0, 0], 16, 2, 64, fmt, layers=3, seed=20, spare=9, layout=layout)
+    k, v = raw(st.k).clone(), raw(st.v).clone()
+    parents, children = [0, 0, 1, 2, 3], [8, 4, 5, 6, 7]
+    ops.paged_cache_fork(st.cache, i32(parents), i32(children))
+    assert ops.device_errors() == 0 and st.state.fork(parents, children)
+    st.check_state()
+    move_pages(st, k, v)
+    assert torch.equal(raw(st.k), k) and torch.equal(raw(st.v), v)
+    attend(st, [1 if n else 0 for n in st.state.lens], 4, layer=2)
+    # the parents and the children grow apart
+    new = [3, 0, 0, 0, 3, 16, 20, 0, 1]
+    ops.paged_cache_reserve(st.cache, i32(new))
+    assert st.state.reserve(new)
+    st.check_state()
+
+
+@pytest.mark.parametrize("parents,children", [([0], [9]), ([-1], [3]), ([0], [1]), ([0, 0], [4, 4]), ([3, 0], [4, 3]),
+                                              ([0, 2, 2, 0], [3, 4, 5, 6]), ([3], [3])])
+def test_fork_is_all_or_nothing(parents, children):
+    need_gpu()
+    say(f"fork refused {parents} {children}")
+    st = Setup([70, 48, 5, 0, 0, 0, 0, 0, 0], 16, 2, 64, layers=2, seed=21, spare=3)
+    k, table = st.k.clone(), st.table.clone()
+    ops.paged_cache_fork(st.cache, i32(parents), i32(children))
+    assert ops.device_errors() == _lib.DEVERR_PAGED and not st.state.fork(parents, children)
+    st.check_state()
+    assert torch.equal(st.k, k) and torch.equal(st.table, table)
+
+
+def test_free_counts_shared_pages_once_per_sequence():
+    need_gpu()
+    say("free")
+    st = Setup([70, 48, 0, 5, 0], 16, 1, 64, seed=22, spare=9)
+    ops.paged_cache_fork(st.cache, i32([0, 0]), i32([2, 4]))
+    assert st.state.fork([0, 0], [2, 4])
+    for seqs in ([0], [2, 2, 1], [2], [4, 3, 4, 3]):
+        ops.paged_cache_free(st.cache, i32(seqs))
+        st.state.free(list(dict.fromkeys(seqs)))
+        assert ops.device_errors() == 0
+        st.check_state()
+    assert not any(st.refs.tolist())
+    ops.paged_cache_free(st.cache, i32([5, -1, 1]))
+    assert ops.device_errors() == _lib.DEVERR_PAGED
+    st.check_state()
+
+
+def test_free_keeps_a_wrong_count_at_zero():
+    need_gpu()
+    say("free of pages whose count is wrong")
+    st = Setup([40], 16, 1, 64, seed=23)
+    st.refs[st.state.table[0][1]] = 0
+    ops.paged_cache_free(st.cache, i32([0]))
+    assert ops.device_errors() == _lib.DEVERR_PAGED
+    assert not any(st.refs.tolist()) and st.lens.tolist() == [0]
+
+
+@pytest.mark.parametrize("layout", ["nhd", "hnd", "pairs", "slots"])
+@pytest.mark.parametrize("fmt", ["bf16", "e4m3"])
+def test_compact(layout, fmt):
+    need_gpu()
+    say(f"compact {layout} {fmt}")
+    st = Setup([70, 48, 5, 0, 200, 31], 16, 2, 64, fmt, layers=2, seed=24, spare=30, layout=layout)
+    ops.paged_cache_fork(st.cache, i32([4]), i32([3]))
+    assert st.state.fork([4], [3])
+    for gone in ([0], [4], [], [3, 2], [1, 5]):
+        k, v = raw(st.k).clone(), raw(st.v).clone()
+        if gone:
+            ops.paged_cache_free(st.cache, i32(gone))
+            st.state.free(gone)
+        ops.paged_cache_compact(st.cache)
+        st.state.compact()
+        assert ops.device_errors() == 0
+        st.check_state()
+        move_pages(st, k, v)
+        assert torch.equal(raw(st.k), k) and torch.equal(raw(st.v), v)
+
+
+def test_compact_of_many_pages():
+    need_gpu()
+    say("compact 40000 pages of one slot")
+    r = random.Random(2)
+    st = Setup([r.randrange(0, 800) for _ in range(90)], 1, 1, 64, seed=25, spare=9000)
+    gone = r.sample(range(90), 40)
+    k, v = st.k.clone(), st.v.clone()
+    ops.paged_cache_free(st.cache, i32(gone))
+    ops.paged_cache_compact(st.cache)
+    st.state.free(gone)
+    st.state.compact()
+    assert ops.device_errors() == 0
+    st.check_state()
+    k[:, [b for _, b in st.state.moves]] = k[:, [a for a, _ in st.state.moves]]
+    v[:, [b for _, b in st.state.moves]] = v[:, [a for a, _ in st.state.moves]]
+    assert torch.equal(st.k, k) and torch.equal(st.v, v)
+    new = [50] * 90
+    ops.paged_cache_reserve(st.cache, i32(new))
+    done = st.state.reserve(new)
+    assert ops.device_errors() == (0 if done else _lib.DEVERR_PAGED)
+    st.check_state()
+
+
+@pytest.mark.parametrize("seed", range(4))
+def test_a_run_of_calls_in_any_order(seed):
+    """A cache lives through 60 random calls, refused ones among them; the model follows, and the attention of every
+    sequence's last rows reads the values that were appended."""
+    need_gpu()
+    say(f"paged cache, random calls, seed {seed}")
+    r = random.Random(seed)
+    S, slots, heads, dim = 9, 16, 2, 64
+    st = Setup([0] * S, slots, heads, dim, layers=2, seed=seed, spare=60, columns=20)
+    k, v = st.k.clone(), st.v.clone()
+    for step in range(60):
+        what = r.choice(["grow", "grow", "fork", "free", "compact"])
+        err, st.state.moves = True, []
+        if what == "grow":
+            new = [r.choice([0, 1, 1, 7, 40]) for _ in range(S)]
+            ops.paged_cache_reserve(st.cache, i32(new))
+            if not st.state.reserve(new):
+                new = [0] * S
+                err = False
+            starts = starts_of(new)
+            nk, nv = queries(starts[-1], heads, dim, step, 8.0), queries(starts[-1], heads, dim, step + 99, 8.0)
+            for layer in range(2):
+                ops.paged_cache_append(st.cache, nk, nv, i32(starts), layer=layer)
+            for m, s, t in pm.positions(starts, st.state.lens):
+                p = st.state.table[s][t // slots]
+                k[:, p, t % slots], v[:, p, t % slots] = nk[m], nv[m]
+        elif what == "fork":
+            p, c = [r.randrange(S) for _ in range(2)], [r.randrange(S) for _ in range(2)]
+            ops.paged_cache_fork(st.cache, i32(p), i32(c))
+            err = st.state.fork(p, c)
+            move_pages(st, k, v)
+        elif what == "free":
+            gone = r.sample(range(S), 2)
+            ops.paged_cache_free(st.cache, i32(gone))
+            st.state.free(gone)
+        else:
+            ops.paged_cache_compact(st.cache)
+            st.state.compact()
+            move_pages(st, k, v)
+        assert ops.device_errors() == (0 if err else _lib.DEVERR_PAGED), what
+        st.check_state()
+        assert torch.equal(st.k, k) and torch.equal(st.v, v), what
+    attend(st, [min(n, 3) for n in st.state.lens], 4, layer=1)
+
+
+# ------------------------------------------------------------------- streams, graphs, the whole step
+
+def test_a_captured_step_replays():
+    """Reserve, append and attention captured once; each replay grows the sequences by one token and gives the eager
+    results, with eager work between the replays."""
+    need_gpu()
+    say("paged step in a graph")
+    ops.init(0)
+    a = Setup([100, 7, 900], 16, 2, 128, seed=30, spare=40, columns=70)
+    b = Setup([100, 7, 900], 16, 2, 128, seed=30, spare=40, columns=70)
+    q, k, v = queries(3, 8, 128, 1), queries(3, 2, 128, 2, 11.0), queries(3, 2, 128, 3, 11.0)
+    one, starts = i32([1, 1, 1]), i32([0, 1, 2, 3])
+    out_a, out_b = torch.empty_like(q), torch.empty_like(q)
+
+    def step(st, out):
+        ops.paged_cache_reserve(st.cache, one)
+        ops.paged_cache_append(st.cache, k, v, starts)
+        ops.paged_attention(q, st.cache, starts, out, max_rows=1)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        step(a, out_a)
+    for i in range(5):
+        q.copy_(queries(3, 8, 128, 40 + i))
+        k.copy_(queries(3, 2, 128, 50 + i, 11.0))
+        graph.replay()
+        step(b, out_b)
+        assert b.state.reserve([1, 1, 1])
+        torch.cuda.synchronize()
+        assert torch.equal(out_a, out_b) and torch.equal(a.lens, b.lens) and torch.equal(a.table, b.table)
+        assert torch.equal(a.k, b.k) and torch.equal(a.refs, b.refs)
+        attend(b, [30, 7, 100], 8, seed=i)  # the same scratch between the replays
+    assert ops.device_errors() == 0
+
+
+def test_a_captured_chunk_and_state_calls_replay():
+    need_gpu()
+    say("paged chunk attention, fork, free and compact in a graph")
+    ops.init(0)
+    st = Setup([500, 0, 300], 16, 2, 128, seed=31, spare=50, columns=40)
+    start = [t.clone() for t in (st.table, st.lens, st.refs, st.k, st.v)]
+    q = queries(260, 8, 128, 1)
+    out = torch.empty_like(q)
+    parents, children, gone, starts = i32([0]), i32([1]), i32([0]), i32([0, 0, 200, 260])
+
+    def step():
+        for t, x in zip((st.table, st.lens, st.refs, st.k, st.v), start):
+            t.copy_(x)
+        ops.paged_cache_fork(st.cache, parents, children)
+        ops.paged_cache_free(st.cache, gone)
+        ops.paged_cache_compact(st.cache)
+        ops.paged_attention(q, st.cache, starts, out, max_rows=200)
+
+    step()
+    assert st.state.fork([0], [1])
+    st.state.free([0])
+    st.state.compact()
+    st.check_state()
+    want = [t.clone() for t in (out, st.table, st.lens, st.refs)]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for _ in range(4):
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        for t, x in zip((out, st.table, st.lens, st.refs), want):
+            assert torch.equal(t, x)
+        attend(st, [0, 20, 1], 8)
+    assert ops.device_errors() == 0
+
+
+def test_calls_follow_the_current_stream():
+    need_gpu()
+    say("paged calls on a side stream")
+    st = Setup([100, 40], 16, 2, 128, seed=32, spare=10, columns=20)
+    side = torch.cuda.Stream()
+    big = torch.randn((4096, 4096), device=DEV)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        for _ in range(20):
+            big = big @ big
+            big = big / big.norm()
+        nk = (queries(2, 2, 128, 1, 11.0).float() + big[0, 0] * 0).to(torch.bfloat16)
+        ops.paged_cache_reserve(st.cache, i32([1, 1]))
+        ops.paged_cache_append(st.cache, nk, nk, i32([0, 1, 2]))
+        assert st.state.reserve([1, 1])
+        attend(st, [1, 1], 8)
+    st.check_state()
+
+
+def test_a_sliding_layer_over_pages_gives_what_the_ring_gives():
+    """QKV of two sequences into scratch rings, their rows appended to the cache, attention and O: the ring's own
+    attention of the same tokens gives the same result within both calls' rounding."""
+    need_gpu()
+    say("sliding layer: QKV -> append -> paged attention -> O, against the ring")
+    from gpu_util import dev, dev_zeros
+    from moa_amd import synth
+    lens, M = [40, 9], [40, 9]
+    st = Setup([0, 0], 64, 8, 256, seed=40, spare=4, columns=2)
+    ops.paged_cache_reserve(st.cache, i32(M))
+    st.state.reserve(M)
+    layers, ring, q_all = [], [], []
+    for s, m in enumerate(M):
+        d = synth.cfg_qkv(seed=3, M=m, pos=0)
+        kc, vc, q = dev_zeros(1024 * 2048), dev_zeros(1024 * 2048), dev_zeros(m * 4096)
+        ops.sliding_project_qkv(*[dev(d[n]) for n in ("x", "q_weight", "k_weight", "v_weight", "q_weight_scale", "k_weight_scale",
+                                                      "v_weight_scale", "input_rms_weight", "q_rms_weight", "k_rms_weight")],
+                                i32([0]), i32([0]), dev(d["cos"]), dev(d["sin"]), kc, vc, q)
+        mask = (torch.arange(1024, device=DEV)[None] <= torch.arange(m, device=DEV)[:, None]).float()
+        o = dev_zeros(m * 4096)
+        ops.sliding_attention(q, kc, vc, mask, o)
+        ring.append(o.view(torch.bfloat16).view(m, 16, 256))
+        layers.append([t.view(torch.bfloat16).view(1024, 8, 256)[:m] for t in (kc, vc)])
+        q_all.append(q.view(torch.bfloat16).view(m, 16, 256))
+    starts = i32(starts_of(M))
+    k, v, q = torch.cat([a for a, _ in layers]), torch.cat([b for _, b in layers]), torch.cat(q_all)
+    ops.paged_cache_append(st.cache, k, v, starts)
+    out = torch.empty_like(q)
+    ops.paged_attention(q, st.cache, starts, out, window=1024, max_rows=max(M))
+    assert ops.device_errors() == 0
+    kk, vv = st.values()
+    want, a, d = pm.attention(q, kk, vv, st.state.table, lens, starts_of(M), 64, 1024, 1.0)
+    check_rows(out, want, a, d, 256)
+    check_rows(torch.cat(ring), want, a, d, 256)
+    o = synth.cfg_o(seed=4, M=sum(M))
+    res = [dev(o["residual"]) for _ in range(2)]
+    for r, x in zip(res, (out, torch.cat(ring))):
+        ops.sliding_attention_output(x.reshape(sum(M), 4096), dev(o["post_attn_rms_weight"]), dev(o["o_weight"]), dev(o["o_weight_scale"]), r)
+    a, b = (r.view(torch.bfloat16).float() for r in res)
+    assert torch.isfinite(a).all() and (a - b).abs().max() <= 0.05 * b.abs().max()
+
+
+def test_a_full_layers_pages_are_pages_of_the_cache():
+    """full_project_qkv writes into the cache's own page; paged_attention then gives full_attention's out / sum."""
+    need_gpu()
+    say("full layer: QKV into a page of the cache, paged attention against full_attention")
+    from gpu_util import dev, dev_zeros
+    from moa_amd import synth
+    d = synth.cfg_full_qkv(seed=5, M=3, pos=700)
+    st = Setup([703], 512, 1, 512, seed=41, layers=1)
+    page = st.state.table[0][1]
+    q = dev_zeros(3 * 8192)
+    ops.full_project_qkv(dev(d["x"]), dev(d["q_weight"]), dev(d["k_weight"]), dev(d["q_weight_scale"]), dev(d["k_weight_scale"]),
+                         dev(d["input_rms_weight"]), dev(d["q_rms_weight"]), dev(d["k_rms_weight"]), i32([d["kv_offset"]]),
+                         i32([d["rope_offset"]]), dev(d["cos"]), dev(d["sin"]), st.k[0, page].view(torch.int16),
+                         st.v[0, page].view(torch.int16), q)
+    q = q.view(torch.bfloat16).view(3, 16, 512)
+    out = torch.empty_like(q)
+    ops.paged_attention(q, st.cache, i32([0, 3]), out)
+    assert ops.device_errors() == 0
+    k, v = st.values()
+    want, a, dd = pm.attention(q, k, v, st.state.table, [703], [0, 3], 512, 0, 1.0)
+    check_rows(out, want, a, dd, 512)
+    pages = torch.tensor(st.state.table[0], device=DEV)
+    masks = torch.stack([(torch.arange(512, device=DEV)[None] + 512 * p <= 700 + torch.arange(3, device=DEV)[:, None]).float() for p in range(2)])
+    mx, sm, o = torch.empty(48, device=DEV), torch.empty(48, device=DEV), torch.empty_like(q)
+    ops.full_attention(q, st.k[0, pages].contiguous(), st.v[0, pages].contiguous(), masks.contiguous(), mx, sm, o)
+    check_rows(o.double() / sm.view(3, 16, 1).double(), want, a, dd, 512)
+    # full_attention_output divides by the running sum: with a normalised row it is one
+    w = synth.cfg_full_o(seed=6, M=3)
+    res = [dev(w["residual"]) for _ in range(2)]
+    for r, x, total in zip(res, (out, o), (torch.ones(48, device=DEV), sm)):
+        ops.full_attention_output(x, total, dev(w["post_attn_rms_weight"]), dev(w["o_weight"]), dev(w["o_weight_scale"]), r)
+    a, b = (r.view(torch.bfloat16).float() for r in res)
+    assert torch.isfinite(a).all() and (a - b).abs().max() <= 0.05 * b.abs().max()
+
+
+def test_calls_of_one_process_repeat_their_bits():
+    need_gpu()
+    say("paged attention twice, the same bits")
+    st = Setup([3000, 70, 1200], 48, 1, 512, seed=33)
+    for rows in ([1, 1, 1], [200, 1, 40]):
+        q = queries(sum(rows), 16, 512, 2)
+        outs = [torch.empty_like(q) for _ in range(2)]
+        for o in outs:
+            ops.paged_attention(q, st.cache, i32(starts_of(rows)), o, max_rows=max(rows))
+            attend(st, [1, 0, 0], 16)
+        assert torch.equal(*outs)
