@@ -2,21 +2,569 @@
 //
 // Row i of a sequence's n new rows stands at p = len - n + i and sees positions max(0, p - window + 1) .. p. With
 // x_t = scale (q . k_t) it gives sum_t e^(x_t - m) v_t / sum_t e^(x_t - m), m the largest x_t, in one pass over the
-// positions with a running m and sum. E4M3 pages: k_t and v_t are codes times the head's scale; K's joins the
-// factor of x_t, V's the last division.
+// positions with a running m and sum (in base 2: x log2 e). E4M3 pages: k_t and v_t are codes times the head's scale;
+// K's joins the factor of x_t, V's the last division.
+//
+// The query heads of a KV head are rows beside each other: row r of a sequence is token r / group, head r % group of
+// the KV head, so one pass over K and V serves them all. Sequences with at most 16 such rows go to the token kernel,
+// the others to the chunk kernel; each finds its work from the row starts and lengths on the device.
+#include <algorithm>
+
 #include "moa_device.h"
 #include "moa_paged.h"
 
 namespace moa {
 namespace {
 
-constexpr int kMaxDim = 512;
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
-// One row (m, head h) by one wave, any type and shape: 64 positions at a time, a lane each for the scores; then the lanes
-// hold head_dim / 64 dims each and take the 64 weights in turn. Positions outside the row's range are never used.
+constexpr int kTokenRows = 16;   // rows of a token-kernel item
+constexpr int kTokenUnit = 128;  // positions that a split is a multiple of: one or two steps of four waves
+// Weights are 2^(x - reference), the reference at most this far below the row's largest x so far: the output is
+// rescaled only when the maximum has grown by more.
+constexpr float kSlack = 8.0f;
+
+__device__ __forceinline__ bf16x8 as_bf16x8(const uint4& v) { return __builtin_bit_cast(bf16x8, v); }
+
+// ------------------------------------------------------------------------------------ who does what
+
+// How a call's sequences are split into items, the same in every kernel of the call. A sequence of r = n * group rows has
+// ceil(r / bm) tiles, each split over ceil(units / c) items, where units covers the positions a tile can see in steps of
+// `unit`, and c is chosen so that all sequences together have at most `items` items per KV head.
+struct PlanArgs {
+    int bm, unit, items;
+    bool tokens;  // the token kernel's sequences (at most kTokenRows rows) or the others
+};
+
+struct Piece {  // an item, or a row of the merge
+    int s, row0, n, len;    // its sequence: first row of the call, new rows, length
+    int tile, split, splits, units_per;
+    int record;             // the first record of its tile
+    int row;                // the merge: row of the sequence
+};
+
+struct SeqWork { int row0, n, len, tiles, units; };
+
+__device__ __forceinline__ SeqWork seq_work(const PagedView& c, const PagedAttentionCall& a, const PlanArgs& p, int s, bool* bad) {
+    SeqWork w = {0, 0, 0, 0, 0};
+    if (s >= c.sequences) return w;
+    w.row0 = a.starts[s];
+    const int end = a.starts[s + 1];
+    w.len = c.lens[s];
+    w.n = end - w.row0;
+    if (w.n == 0) return w;
+    if (w.row0 < 0 || w.n < 0 || end > a.rows || w.n > a.max_rows || w.len < 0 || w.len > paged_capacity(c)) {
+        *bad = true;
+        return w;
+    }
+    const int64_t rows = (int64_t)w.n * a.group;
+    if ((rows <= kTokenRows) != p.tokens) return w;
+    w.tiles = (int)((rows + p.bm - 1) / p.bm);
+    // positions that a tile's rows see: all, or the window and the tile's tokens, from a multiple of the unit on
+    const int span = p.tokens ? w.n : min(w.n, (p.bm + a.group - 1) / a.group + 1);
+    const int seen = a.window ? min(w.len, a.window + span - 1 + p.unit) : w.len;
+    w.units = max(1, (seen + p.unit - 1) / p.unit);
+    return w;
+}
+
+// Finds piece `want` of KV head-independent work by one wave: of items (merge = false) or of rows whose tiles are split
+// (merge = true). False: there are not that many.
+__device__ bool find_piece(const PagedView& c, const PagedAttentionCall& a, const PlanArgs& p, bool merge, int64_t want, Piece* out) {
+    const int lane = threadIdx.x & 63;
+    uint64_t tiles = 0, units = 0;
+    bool bad = false;
+    SeqWork w = {};
+    for (int base = 0; base < c.sequences; base += 64) {
+        w = seq_work(c, a, p, base + lane, &bad);
+        tiles += w.tiles;
+        units += (uint64_t)w.tiles * w.units;
+    }
+    if (__any(bad) && blockIdx.x == 0 && lane == 0) atomicOr(c.err, kErrPaged);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        tiles += __shfl_xor(tiles, o, kWave);
+        units += __shfl_xor(units, o, kWave);
+    }
+    // sum of ceil(units / c) <= units / c + tiles <= items
+    const uint64_t room = tiles < (uint64_t)p.items ? p.items - tiles : 0;
+    const uint64_t per64 = room ? (units + room - 1) / room : 1u << 30;
+    const int per = (int)(per64 < 1 ? 1 : (per64 > (1u << 30) ? 1u << 30 : per64));
+    int64_t items_before = 0, rows_before = 0;
+    for (int base = 0; base < c.sequences; base += 64) {
+        if (c.sequences > 64) w = seq_work(c, a, p, base + lane, &bad);
+        const int splits = w.tiles ? (w.units + per - 1) / per : 0;
+        const int64_t items = (int64_t)w.tiles * splits, rows = splits > 1 ? (int64_t)w.n * a.group : 0;
+        int64_t xi = items, xr = rows;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int64_t yi = __shfl_up(xi, o, kWave);
+            if (lane >= o) xi += yi;
+        }
+        if (merge) {
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) {
+                const int64_t yr = __shfl_up(xr, o, kWave);
+                if (lane >= o) xr += yr;
+            }
+        }
+        const int64_t mine = merge ? rows_before + xr : items_before + xi;
+        const uint64_t hit = __ballot(mine > want);
+        if (hit) {
+            const int l = __builtin_ctzll(hit);
+            auto get = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
+            out->s = base + l;
+            out->row0 = get(w.row0), out->n = get(w.n), out->len = get(w.len);
+            out->splits = get(splits), out->units_per = per;
+            const int first_item = get((int)(items_before + xi - items));
+            if (merge) {
+                out->row = (int)(want - __shfl(mine - rows, l, kWave));
+                out->tile = out->row / p.bm;
+                out->split = 0;
+            } else {
+                const int k = (int)(want - __shfl(mine - items, l, kWave));
+                out->tile = k / out->splits;
+                out->split = k - out->tile * out->splits;
+                out->row = 0;
+            }
+            out->record = first_item + out->tile * out->splits;
+            return true;
+        }
+        items_before += __shfl(xi, 63, kWave);
+        rows_before += __shfl(xr, 63, kWave);
+    }
+    return false;
+}
+
+// Records of split tiles: per tile and split bm maxima, bm sums, out [bm][dim], f32. A record whose keys include a page
+// outside the pool has NaN maxima: its rows are not written.
+__device__ __forceinline__ int64_t record_floats(int bm, int dim) { return (int64_t)bm * (2 + dim); }
+
+// One row by one wave over positions [lo, hi), nothing outside them used: 64 positions at a time, a lane each for the
+// scores; then lane l holds dims l * dim / 64 .. and takes the weights in turn. The kernels fall back to it where a value that
+// their rows do not all see is infinite or NaN (zero times that is NaN). Pages are in range here.
+template <bool E4M3>
+__device__ void careful_row(const PagedView& c, const uint16_t* q, int s, int kvh, float factor, int lo, int hi, float* mx_out,
+                            float* sum_out, float (&o)[8]) {
+    const int lane = threadIdx.x & 63, d = c.head_dim, per = d / 64;
+    float mx = -INFINITY, sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] = 0.0f;
+    for (int t0 = lo; t0 < hi; t0 += 64) {
+        const int t = min(t0 + lane, hi - 1);
+        const uint32_t i = page_of(c, t);
+        const int slot = t - i * c.slots, page = c.table[s * c.table_stride + i];
+        const uint8_t* kp = c.k + page * c.k_page + slot * c.k_slot + kvh * c.k_head;
+        float x = 0.0f;
+        for (int j = 0; j < d; j += 8) {
+            float e[8], f[8];
+            bf16x8_to_f32(ld16(q + j), f);
+            if (E4M3) {
+                const uint2 w = *reinterpret_cast<const uint2*>(kp + j);
+                fp8x4_to_f32(w.x, e);
+                fp8x4_to_f32(w.y, e + 4);
+            } else {
+                bf16x8_to_f32(ld16(kp + 2 * j), e);
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k) x = fmaf(e[k], f[k], x);
+        }
+        x = t0 + lane < hi ? x * factor : -INFINITY;
+        float mn = x;
+#pragma unroll
+        for (int w = 32; w > 0; w >>= 1) mn = fmaxf(mn, __shfl_xor(mn, w, kWave));
+        mn = fmaxf(mn, mx);
+        const float f = mx == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mx - mn);
+        const float w = t0 + lane < hi ? __builtin_amdgcn_exp2f(x - mn) : 0.0f;
+        mx = mn;
+        sum = fmaf(sum, f, wave_sum(w));
+#pragma unroll
+        for (int k = 0; k < 8; ++k) o[k] *= f;
+        for (int j = 0; j < min(64, hi - t0); ++j) {
+            const float wj = __shfl(w, j, kWave);
+            const uint8_t* vp = c.v + __shfl(page, j, kWave) * c.v_page + __shfl(slot, j, kWave) * c.v_slot + kvh * c.v_head;
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (k < per)
+                    o[k] = fmaf(wj, E4M3 ? e4m3_to_f32(vp[lane * per + k]) : bf2f(reinterpret_cast<const uint16_t*>(vp)[lane * per + k]), o[k]);
+        }
+    }
+    *mx_out = mx;
+    *sum_out = sum;
+}
+
+// Row r of a sequence: where it lies in the call, and the positions it sees.
+struct Row {
+    int64_t m;      // row of the call
+    int h, lo, hi;  // query head; positions [lo, hi)
+};
+__device__ __forceinline__ Row row_of(const PagedAttentionCall& a, const Piece& t, int kvh, int r) {
+    Row x;
+    const int i = r / a.group, p = t.len - t.n + i;
+    x.m = t.row0 + i;
+    x.h = kvh * a.group + (r - i * a.group);
+    x.hi = p + 1;
+    x.lo = a.window && p >= a.window ? p - a.window + 1 : 0;
+    return x;
+}
+
+// The careful path for a piece's rows [r0, r0 + nr) over positions [lo, hi), waves taking rows in turn.
+template <bool E4M3>
+__device__ void careful_piece(const PagedView& c, const PagedAttentionCall& a, const Piece& t, int kvh, int r0, int nr, int lo, int hi,
+                              float* rec, int bm) {
+    const int lane = threadIdx.x & 63, per = c.head_dim / 64;
+    for (int r = threadIdx.x >> 6; r < nr; r += blockDim.x >> 6) {
+        const Row x = row_of(a, t, kvh, r0 + r);
+        float o[8], mx, sum;
+        careful_row<E4M3>(c, a.q + x.m * a.q_row + x.h * c.head_dim, t.s, kvh, E4M3 ? c.k_scale[kvh] * a.scale_log2 : a.scale_log2,
+                          max(lo, x.lo), min(hi, x.hi), &mx, &sum, o);
+        if (rec) {
+            if (lane == 0) rec[r] = mx, rec[bm + r] = sum;
+            for (int k = 0; k < per; ++k) rec[2 * bm + (int64_t)r * c.head_dim + lane * per + k] = o[k];
+        } else {
+            const float inv = sum == 0.0f ? 0.0f : (E4M3 ? c.v_scale[kvh] : 1.0f) / sum;
+            for (int k = 0; k < per; ++k) a.out[x.m * a.out_row + x.h * c.head_dim + lane * per + k] = (uint16_t)f2bf(o[k] * inv);
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------ the token kernel
+
+// Up to 16 rows of a sequence over a span of positions: bound by the bytes of K and V, which go from memory to
+// registers and never through LDS. Four waves take a tile of 16 or 32 positions each in turn. Scores are K times Q^T
+// (16 x 16 x 32 MFMAs): lane (c = lane % 16, g = lane / 16) then holds, for row c, positions 4 g .. 4 g + 3 of each 16,
+// which are just the positions it supplies as A of P times V when V's lanes take the same ones: P moves between no
+// lanes. V's lane (c, g) loads kVD dims of each of its positions, and v_perm pairs two positions of a dim; MFMA (b, d)
+// then covers dims 16 kVD b + kVD c + d of all c. P enters as two bf16 parts, high and rest (what is lost is 2^-16 of a
+// weight): tiles of 16 positions put both into one MFMA, beside the same V twice, tiles of 32 take two. This
+// tile's V and the next tile's K are in flight during the arithmetic.
+template <int D, bool E4M3>
+struct TokenShape {
+    static constexpr int kElem = E4M3 ? 1 : 2;
+    static constexpr int kSub = D * kElem >= 512 ? 1 : 2;                       // 16 positions each: K and V of a tile in 128 registers
+    static constexpr int kTile = 16 * kSub;
+    static constexpr int kWavesPerSimd = D == 512 ? 1 : (D == 256 ? 2 : 3);
+    static constexpr int kKLoads = D * kElem / 64;                              // 16-byte loads of a K row per lane
+    static constexpr int kVD = (E4M3 ? 16 : 8) < D / 16 ? (E4M3 ? 16 : 8) : D / 16;  // dims per V load
+    static constexpr int kVB = D / (16 * kVD);                                  // V loads of a row per lane
+    static constexpr int kVWords = kVD * kElem / 4;
+    static constexpr int kQStride = D + 8;                                      // LDS row of Q: 16 rows start on 16 bank groups
+    static constexpr int kLds = 16 * kQStride * 2 + 4 * kTokenRows * D * 4;
+};
+
+template <int W>
+struct Words { uint32_t w[W]; };
+
+template <int W>
+__device__ __forceinline__ Words<W> ld_words(const uint8_t* p) {
+    Words<W> r;
+    if constexpr (W == 4) {
+        const uint4 v = ld16(p);
+        r.w[0] = v.x, r.w[1] = v.y, r.w[2] = v.z, r.w[3] = v.w;
+    } else if constexpr (W == 2) {
+        const uint2 v = *reinterpret_cast<const uint2*>(p);
+        r.w[0] = v.x, r.w[1] = v.y;
+    } else {
+        r.w[0] = *reinterpret_cast<const uint32_t*>(p);
+    }
+    return r;
+}
+
+__device__ __forceinline__ uint32_t bf16_pair_of_fp8(uint32_t two) {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(two, 1.0f, false));
+}
+
+template <int D, bool E4M3>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(TokenShape<D, E4M3>::kWavesPerSimd))) void paged_token_kernel(
+    PagedView c, PagedAttentionCall a, PlanArgs plan, float* part) {
+    using T = TokenShape<D, E4M3>;
+    constexpr int NT = T::kSub;
+    __shared__ __attribute__((aligned(16))) uint16_t qs[16 * T::kQStride];
+    __shared__ __attribute__((aligned(16))) float os[4 * kTokenRows * D];
+    __shared__ float ms[4][kTokenRows], ls[4][kTokenRows];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l16 = lane & 15, g = lane >> 4;
+    const int kvh = blockIdx.x % c.kv_heads;
+    const float factor = E4M3 ? c.k_scale[kvh] * a.scale_log2 : a.scale_log2;
+    Piece t;
+    for (int64_t item = blockIdx.x / c.kv_heads; find_piece(c, a, plan, false, item, &t); item += gridDim.x / c.kv_heads) {
+        const int nr = t.n * a.group;
+        // the item's positions, from a multiple of the tile on
+        const int first = a.window ? max(0, t.len - t.n + 1 - a.window) / T::kTile * T::kTile : 0;
+        const int lo = first + min((int64_t)t.split * t.units_per * kTokenUnit, (int64_t)1 << 30);
+        const int hi = (int)min((int64_t)lo + (int64_t)t.units_per * kTokenUnit, (int64_t)t.len);
+        __syncthreads();  // the item before has been written out
+        for (int i = threadIdx.x; i < 16 * D / 8; i += 256) {
+            const int r = i / (D / 8), j = i - r * (D / 8);
+            const Row x = row_of(a, t, kvh, min(r, nr - 1));
+            *reinterpret_cast<uint4*>(qs + r * T::kQStride + 8 * j) = ld16(a.q + x.m * a.q_row + x.h * D + 8 * j);
+        }
+        const Row mine = row_of(a, t, kvh, min(l16, nr - 1));
+        const int see_lo = l16 < nr ? mine.lo : 0, see_hi = l16 < nr ? mine.hi : 0;
+        __syncthreads();
+
+        f32x4 o[T::kVB][T::kVD];
+#pragma unroll
+        for (int b = 0; b < T::kVB; ++b)
+#pragma unroll
+            for (int d = 0; d < T::kVD; ++d) o[b][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        float m_run = -INFINITY, m_ref = -INFINITY, l_run = 0.0f;
+        bool bad = false;
+
+        const int32_t* table = c.table + t.s * c.table_stride;
+        // lane l looks after position t0 + l % kTile: its page (the next tile's is asked for a tile ahead)
+        auto page_at = [&](int t0) { return t0 < hi ? table[page_of(c, min(t0 + lane % T::kTile, hi - 1))] : 0; };
+        uint4 kf[NT][T::kKLoads];
+        Words<T::kVWords> vf[T::kVB][4 * NT];
+        int64_t koff = 0, voff = 0;
+        auto place = [&](int page, int t0) {  // offsets of the lane's position; a bad page becomes page 0, and is remembered
+            if (t0 >= hi) return;
+            const int p = min(t0 + lane % T::kTile, hi - 1);
+            const bool in = page >= 0 && page < c.pages;
+            bad |= !in;
+            page = in ? page : 0;
+            const uint32_t slot = p - page_of(c, p) * c.slots;
+            koff = page * c.k_page + slot * c.k_slot;
+            voff = page * c.v_page + slot * c.v_slot;
+        };
+        const uint8_t* kbase = c.k + kvh * c.k_head + 16 * g;
+        const uint8_t* vbase = c.v + kvh * c.v_head + l16 * T::kVD * T::kElem;
+        auto load_k = [&] {
+#pragma unroll
+            for (int i = 0; i < NT; ++i) {
+                const uint8_t* p = kbase + __shfl(koff, 16 * i + l16, kWave);
+#pragma unroll
+                for (int j = 0; j < T::kKLoads; ++j) kf[i][j] = ld16(p + 64 * j);
+            }
+        };
+        auto load_v = [&] {
+#pragma unroll
+            for (int i = 0; i < 4 * NT; ++i) {
+                const uint8_t* p = vbase + __shfl(voff, 16 * (i >> 2) + 4 * g + (i & 3), kWave);
+#pragma unroll
+                for (int b = 0; b < T::kVB; ++b) vf[b][i] = ld_words<T::kVWords>(p + 16 * T::kVD * T::kElem * b);
+            }
+        };
+
+        int t0 = lo + wave * T::kTile;
+        constexpr int kStep = 4 * T::kTile;
+        int page = page_at(t0), page1 = page_at(t0 + kStep);
+        place(page, t0);
+        if (t0 < hi) load_k();
+        for (; t0 < hi; t0 += kStep) {
+            load_v();
+            if constexpr (D == 512) __asm__ volatile("" ::: "memory");  // Q is read from LDS again: no registers for it
+            f32x4 sc[NT];
+#pragma unroll
+            for (int i = 0; i < NT; ++i) sc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            // Q's dims follow the order K's 16-byte loads have: bf16 dims 32 j + 8 g, E4M3 dims 64 j + 16 g, two steps a load
+#pragma unroll
+            for (int j = 0; j < T::kKLoads; ++j) {
+                if constexpr (E4M3) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const bf16x8 qf = as_bf16x8(ld16(qs + l16 * T::kQStride + 64 * j + 16 * g + 8 * h));
+#pragma unroll
+                        for (int i = 0; i < NT; ++i) {
+                            const uint32_t w0 = h ? kf[i][j].z : kf[i][j].x, w1 = h ? kf[i][j].w : kf[i][j].y;
+                            const uint4 kb = make_uint4(bf16_pair_of_fp8(w0), bf16_pair_of_fp8(w0 >> 16), bf16_pair_of_fp8(w1),
+                                                        bf16_pair_of_fp8(w1 >> 16));
+                            sc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(kb), qf, sc[i], 0, 0, 0);
+                        }
+                    }
+                } else {
+                    const bf16x8 qf = as_bf16x8(ld16(qs + l16 * T::kQStride + 32 * j + 8 * g));
+#pragma unroll
+                    for (int i = 0; i < NT; ++i) sc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(kf[i][j]), qf, sc[i], 0, 0, 0);
+                }
+            }
+            // the next tile's K
+            page = page1;
+            page1 = page_at(t0 + 2 * kStep);
+            place(page, t0 + kStep);
+            if (t0 + kStep < hi) load_k();
+
+            // weights of row l16 at positions t0 + 16 i + 4 g + e
+            float x[NT][4], mx = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < NT; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int p = t0 + 16 * i + 4 * g + e;
+                    x[i][e] = p >= see_lo && p < see_hi ? sc[i][e] * factor : -INFINITY;
+                    mx = fmaxf(mx, x[i][e]);
+                }
+            mx = fmaxf(mx, __shfl_xor(mx, 16));
+            mx = fmaxf(mx, __shfl_xor(mx, 32));
+            m_run = fmaxf(m_run, mx);
+            float scale = 1.0f;
+            if (m_run > m_ref + kSlack) {
+                scale = m_ref == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m_ref - m_run);  // -inf: sum and out are zero
+                m_ref = m_run;
+            }
+            if (__any(scale != 1.0f)) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float f = __shfl(scale, 4 * g + e, kWave);
+#pragma unroll
+                    for (int b = 0; b < T::kVB; ++b)
+#pragma unroll
+                        for (int d = 0; d < T::kVD; ++d) o[b][d][e] *= f;
+                }
+            }
+            const float mu = m_ref == -INFINITY ? 0.0f : m_ref;
+            float sum = 0.0f;
+            uint32_t ph[2 * NT], pl[2 * NT];
+#pragma unroll
+            for (int i = 0; i < NT; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; e += 2) {
+                    const float p0 = __builtin_amdgcn_exp2f(x[i][e] - mu), p1 = __builtin_amdgcn_exp2f(x[i][e + 1] - mu);
+                    sum += p0 + p1;
+                    const uint32_t w = pk_bf16(p0, p1);
+                    ph[2 * i + e / 2] = w;
+                    pl[2 * i + e / 2] = pk_bf16(p0 - bf2f(w & 0xffffu), p1 - bf2f(w >> 16));
+                }
+            l_run = fmaf(l_run, scale, sum);
+#pragma unroll
+            for (int b = 0; b < T::kVB; ++b)
+#pragma unroll
+                for (int d = 0; d < T::kVD; ++d) {
+                    uint32_t w[2 * NT];
+#pragma unroll
+                    for (int i = 0; i < 2 * NT; ++i) {
+                        if constexpr (E4M3)
+                            w[i] = bf16_pair_of_fp8(__builtin_amdgcn_perm(vf[b][2 * i + 1].w[d / 4], vf[b][2 * i].w[d / 4],
+                                                                          0x0c0c0000u | (4 + d % 4) << 8 | d % 4));
+                        else
+                            w[i] = __builtin_amdgcn_perm(vf[b][2 * i + 1].w[d / 2], vf[b][2 * i].w[d / 2], d & 1 ? 0x07060302u : 0x05040100u);
+                    }
+                    if constexpr (NT == 1) {
+                        o[b][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(make_uint4(ph[0], ph[1], pl[0], pl[1])),
+                                                                          as_bf16x8(make_uint4(w[0], w[1], w[0], w[1])), o[b][d], 0, 0, 0);
+                    } else {
+                        const bf16x8 vb = as_bf16x8(make_uint4(w[0], w[1], w[2], w[3]));
+                        o[b][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(make_uint4(ph[0], ph[1], ph[2], ph[3])), vb, o[b][d], 0, 0, 0);
+                        o[b][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(make_uint4(pl[0], pl[1], pl[2], pl[3])), vb, o[b][d], 0, 0, 0);
+                    }
+                }
+        }
+
+        // the four waves' states into one
+        l_run += __shfl_xor(l_run, 16);
+        l_run += __shfl_xor(l_run, 32);
+        if (g == 0) ms[wave][l16] = m_ref, ls[wave][l16] = l_run;
+#pragma unroll
+        for (int b = 0; b < T::kVB; ++b)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+                for (int d = 0; d < T::kVD; d += 4)
+                    *reinterpret_cast<float4*>(os + ((wave * kTokenRows + 4 * g + e) * D + 16 * T::kVD * b + T::kVD * l16 + d)) =
+                        make_float4(o[b][d][e], o[b][d + 1][e], o[b][d + 2][e], o[b][d + 3][e]);
+        bad = __syncthreads_or(bad);
+        float* rec = t.splits > 1 ? part + ((int64_t)kvh * plan.items + t.record + t.split) * record_floats(kTokenRows, D) : nullptr;
+        bool odd = false;
+        const float vs = E4M3 ? c.v_scale[kvh] : 1.0f;
+        for (int i = threadIdx.x; i < nr * (D / 4); i += 256) {
+            const int r = i / (D / 4), d = 4 * (i - r * (D / 4));
+            const float m = fmaxf(fmaxf(ms[0][r], ms[1][r]), fmaxf(ms[2][r], ms[3][r]));
+            float l = 0.0f, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const float f = ms[w][r] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ms[w][r] - m);
+                const float4 y = *reinterpret_cast<const float4*>(os + (w * kTokenRows + r) * D + d);
+                l = fmaf(f, ls[w][r], l);
+                v[0] = fmaf(f, y.x, v[0]), v[1] = fmaf(f, y.y, v[1]), v[2] = fmaf(f, y.z, v[2]), v[3] = fmaf(f, y.w, v[3]);
+            }
+            odd |= !(fabsf(v[0]) + fabsf(v[1]) + fabsf(v[2]) + fabsf(v[3]) < INFINITY);
+            if (rec) {
+                if (d == 0) rec[r] = bad ? NAN : m, rec[kTokenRows + r] = l;
+                *reinterpret_cast<float4*>(rec + 2 * kTokenRows + r * D + d) = make_float4(v[0], v[1], v[2], v[3]);
+            } else if (!bad) {
+                const Row x = row_of(a, t, kvh, r);
+                const float inv = l == 0.0f ? 0.0f : vs / l;
+                *reinterpret_cast<uint2*>(a.out + x.m * a.out_row + x.h * D + d) =
+                    make_uint2(pk_bf16(v[0] * inv, v[1] * inv), pk_bf16(v[2] * inv, v[3] * inv));
+            }
+        }
+        odd = __syncthreads_or(odd);
+        if (bad && threadIdx.x == 0) atomicOr(c.err, kErrPaged);
+        if (odd && !bad) careful_piece<E4M3>(c, a, t, kvh, 0, nr, lo, hi, rec, kTokenRows);
+    }
+}
+
+// ------------------------------------------------------------------------------------------- the merge
+
+// Rows of split tiles: a workgroup takes a row's dims in blocks of kMergeDims, its threads the records in turn.
+constexpr int kMergeDims = 128;
+
+template <int D, bool E4M3>
+__global__ __launch_bounds__(256) void paged_merge_kernel(PagedView c, PagedAttentionCall a, PlanArgs plan, const float* part) {
+    constexpr int DB = D < kMergeDims ? D : kMergeDims, kBlocks = D / DB, kCols = DB / 4, kGroups = 256 / kCols;
+    __shared__ float4 ov[kGroups][kCols];
+    const int lane = threadIdx.x & 63, col = threadIdx.x % kCols, grp = threadIdx.x / kCols;
+    const int kvh = blockIdx.x % c.kv_heads;
+    Piece t;
+    for (int64_t u = blockIdx.x / c.kv_heads;; u += gridDim.x / c.kv_heads) {
+        const int64_t row = u / kBlocks;
+        const int d = (int)(u - row * kBlocks) * DB + 4 * col;
+        if (!find_piece(c, a, plan, true, row, &t)) return;
+        const int r = t.row - t.tile * plan.bm;
+        const int64_t size = record_floats(plan.bm, D);
+        const float* rec = part + ((int64_t)kvh * plan.items + t.record) * size;
+        float m = -INFINITY, l = 0.0f;
+        bool bad = false;
+        for (int j = lane; j < t.splits; j += 64) {
+            const float x = rec[j * size + r];
+            bad |= x != x;
+            m = fmaxf(m, x);
+        }
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, kWave));
+        for (int j = lane; j < t.splits; j += 64) {
+            const float x = rec[j * size + r];
+            l += x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x - m) * rec[j * size + plan.bm + r];
+        }
+        l = wave_sum(l);
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        const float* rv = rec + 2 * plan.bm + (int64_t)r * D + d;
+        constexpr int kAhead = 4;
+        for (int j0 = grp; j0 < t.splits; j0 += kGroups * kAhead) {
+            float f[kAhead];
+            float4 y[kAhead];
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) {
+                const int j = min(j0 + k * kGroups, t.splits - 1);
+                const float x = rec[j * size + r];
+                y[k] = *reinterpret_cast<const float4*>(rv + j * size);
+                f[k] = j0 + k * kGroups >= t.splits || x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x - m);
+            }
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k)
+                if (f[k] != 0.0f) {
+                    v.x = fmaf(f[k], y[k].x, v.x), v.y = fmaf(f[k], y[k].y, v.y);
+                    v.z = fmaf(f[k], y[k].z, v.z), v.w = fmaf(f[k], y[k].w, v.w);
+                }
+        }
+        ov[grp][col] = v;
+        __syncthreads();
+        if (grp == 0 && !__any(bad)) {
+#pragma unroll
+            for (int k = 1; k < kGroups; ++k) {
+                const float4 y = ov[k][col];
+                v.x += y.x, v.y += y.y, v.z += y.z, v.w += y.w;
+            }
+            const Row x = row_of(a, t, kvh, t.row);
+            const float inv = l == 0.0f ? 0.0f : (E4M3 ? c.v_scale[kvh] : 1.0f) / l;
+            *reinterpret_cast<uint2*>(a.out + x.m * a.out_row + x.h * D + d) = make_uint2(pk_bf16(v.x * inv, v.y * inv), pk_bf16(v.z * inv, v.w * inv));
+        }
+        __syncthreads();
+    }
+}
+
+// ---------------------------------------------------------------------- rows of longer sequences, one wave each
+
 template <bool E4M3>
 __global__ __launch_bounds__(256) void paged_attention_row_kernel(PagedView c, PagedAttentionCall a) {
-    __shared__ float qs[4][kMaxDim];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t unit = (int64_t)blockIdx.x * 4 + wave;
     const int m = (int)(unit / a.q_heads), h = (int)(unit - (int64_t)m * a.q_heads), kvh = h / a.group;
@@ -24,84 +572,75 @@ __global__ __launch_bounds__(256) void paged_attention_row_kernel(PagedView c, P
     const int s = sequence_of(a.starts, c.sequences, m);
     if (s < 0 || s >= c.sequences) return;
     const int start = a.starts[s], end = a.starts[s + 1], len = c.lens[s];
-    if (end <= m) return;
+    if (end <= m || (int64_t)(end - start) * a.group <= kTokenRows) return;
     if (start < 0 || end > a.rows || end - start > a.max_rows || len < 0 || len > paged_capacity(c)) {
         if (lane == 0) atomicOr(c.err, kErrPaged);
         return;
     }
-    const int p = len - (end - m), lo = a.window && p >= a.window ? p - a.window + 1 : 0;
-    const int d = c.head_dim;
-    for (int i = lane; i < d; i += 64) qs[wave][i] = bf2f(a.q[m * a.q_row + h * d + i]);
-    const float ks = E4M3 ? c.k_scale[kvh] * a.scale_log2 : a.scale_log2;
-    const int per = d / 64;
-    float o[kMaxDim / 64] = {}, mx = -INFINITY, sum = 0.0f;
+    Piece t = {s, start, end - start, len, 0, 0, 1, 0, 0, 0};
+    const int r = (m - start) * a.group + (h - kvh * a.group);
+    const Row x = row_of(a, t, kvh, r);
     bool bad = false;
-    for (int t0 = lo; t0 <= p; t0 += 64) {
-        const int t = t0 + lane;
-        int page = 0, slot = 0;
-        float x = -INFINITY;
-        if (t <= p) {
-            const uint32_t i = page_of(c, t);
-            slot = t - i * c.slots;
-            page = c.table[s * c.table_stride + i];
-            if (page < 0 || page >= c.pages) bad = true;
-            else {
-                const uint8_t* kp = c.k + page * c.k_page + slot * c.k_slot + kvh * c.k_head;
-                float acc = 0.0f;
-                for (int j = 0; j < d; j += 8) {
-                    float e[8];
-                    if (E4M3) {
-                        const uint2 w = *reinterpret_cast<const uint2*>(kp + j);
-                        fp8x4_to_f32(w.x, e);
-                        fp8x4_to_f32(w.y, e + 4);
-                    } else {
-                        bf16x8_to_f32(ld16(kp + 2 * j), e);
-                    }
-#pragma unroll
-                    for (int i2 = 0; i2 < 8; ++i2) acc = fmaf(e[i2], qs[wave][j + i2], acc);
-                }
-                x = acc * ks;
-            }
-        }
-        if (__any(bad)) break;
-        float mn = x;
-#pragma unroll
-        for (int o2 = 32; o2 > 0; o2 >>= 1) mn = fmaxf(mn, __shfl_xor(mn, o2, kWave));
-        mn = fmaxf(mn, mx);
-        const float f = mx == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mx - mn);
-        const float w = t <= p && mn != -INFINITY ? __builtin_amdgcn_exp2f(x - mn) : 0.0f;
-        mx = mn;
-        sum = fmaf(sum, f, wave_sum(w));
-#pragma unroll
-        for (int i = 0; i < kMaxDim / 64; ++i) o[i] *= f;
-        const int n = min(64, p - t0 + 1);
-        for (int j = 0; j < n; ++j) {
-            const float wj = __shfl(w, j, kWave);
-            const uint8_t* vp = c.v + __shfl(page, j, kWave) * c.v_page + __shfl(slot, j, kWave) * c.v_slot + kvh * c.v_head;
-#pragma unroll
-            for (int i = 0; i < kMaxDim / 64; ++i)
-                if (i < per)
-                    o[i] = fmaf(wj, E4M3 ? e4m3_to_f32(vp[lane * per + i]) : bf2f(reinterpret_cast<const uint16_t*>(vp)[lane * per + i]), o[i]);
-        }
+    for (int i = lane; x.hi > x.lo && i <= (int)page_of(c, x.hi - 1); i += 64) {
+        const int p = c.table[s * c.table_stride + i];
+        bad |= i >= (int)page_of(c, x.lo) && (p < 0 || p >= c.pages);
     }
     if (__any(bad)) {
         if (lane == 0) atomicOr(c.err, kErrPaged);
         return;
     }
-    const float vs = E4M3 ? c.v_scale[kvh] : 1.0f;
-    const float inv = sum == 0.0f ? 0.0f : vs / sum;
-#pragma unroll
-    for (int i = 0; i < kMaxDim / 64; ++i)
-        if (i < per) a.out[m * a.out_row + h * d + lane * per + i] = (uint16_t)f2bf(o[i] * inv);
+    float o[8], mx, sum;
+    careful_row<E4M3>(c, a.q + x.m * a.q_row + x.h * c.head_dim, s, kvh, E4M3 ? c.k_scale[kvh] * a.scale_log2 : a.scale_log2, x.lo, x.hi,
+                      &mx, &sum, o);
+    const float inv = sum == 0.0f ? 0.0f : (E4M3 ? c.v_scale[kvh] : 1.0f) / sum;
+    const int per = c.head_dim / 64;
+    for (int k = 0; k < per; ++k) a.out[x.m * a.out_row + x.h * c.head_dim + lane * per + k] = (uint16_t)f2bf(o[k] * inv);
+}
+
+int64_t clamp64(int64_t v, int64_t lo, int64_t hi) { return v < lo ? lo : (v > hi ? hi : v); }
+
+template <int D, bool E4M3>
+hipError_t launch(const PagedView& c, const PagedAttentionCall& a, hipStream_t s, DevCtx* ctx) {
+    using T = TokenShape<D, E4M3>;
+    const int64_t capacity = (int64_t)c.columns * c.slots;
+    // token kernel: about four items per workgroup that the device holds, and one more for every sequence
+    const int resident = ctx->cus * T::kWavesPerSimd;
+    const int64_t records = (int64_t)kPagedPartFloats / (kTokenRows * (2 + D)) / c.kv_heads;
+    const PlanArgs plan{kTokenRows, kTokenUnit, (int)clamp64(4 * (int64_t)resident / c.kv_heads + c.sequences, 1, records), true};
+    const int64_t most_units = (a.window ? std::min<int64_t>(capacity, (int64_t)a.window + a.max_rows + kTokenUnit) : capacity) / kTokenUnit + 1;
+    const int64_t items = std::min<int64_t>(plan.items, c.sequences * most_units);
+    hipLaunchKernelGGL((paged_token_kernel<D, E4M3>), dim3((uint32_t)(items * c.kv_heads)), dim3(256), 0, s, c, a, plan, ctx->paged_part);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    if (most_units > 1) {
+        const int64_t rows = std::min<int64_t>((int64_t)a.rows * a.group, (int64_t)c.sequences * kTokenRows) * ((D + kMergeDims - 1) / kMergeDims);
+        hipLaunchKernelGGL((paged_merge_kernel<D, E4M3>), dim3((uint32_t)(std::min<int64_t>(rows, std::max(1, 2048 / c.kv_heads)) * c.kv_heads)),
+                           dim3(256), 0, s, c, a, plan, ctx->paged_part);
+        e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    if ((int64_t)a.max_rows * a.group > kTokenRows) {
+        const int64_t units = (int64_t)a.rows * a.q_heads;
+        hipLaunchKernelGGL(paged_attention_row_kernel<E4M3>, dim3((uint32_t)((units + 3) / 4)), dim3(256), 0, s, c, a);
+        e = hipGetLastError();
+    }
+    return e;
+}
+
+template <int D>
+hipError_t launch_type(const PagedView& c, const PagedAttentionCall& a, hipStream_t s, DevCtx* ctx) {
+    return c.k_scale ? launch<D, true>(c, a, s, ctx) : launch<D, false>(c, a, s, ctx);
 }
 
 }  // namespace
 
-hipError_t launch_paged_attention(const PagedView& c, const PagedAttentionCall& a, hipStream_t s, DevCtx*) {
-    const int64_t units = (int64_t)a.rows * a.q_heads;
-    auto* f = c.k_scale ? paged_attention_row_kernel<true> : paged_attention_row_kernel<false>;
-    hipLaunchKernelGGL(f, dim3((uint32_t)((units + 3) / 4)), dim3(256), 0, s, c, a);
-    return hipGetLastError();
+hipError_t launch_paged_attention(const PagedView& c, const PagedAttentionCall& a, hipStream_t s, DevCtx* ctx) {
+    switch (c.head_dim) {
+        case 64: return launch_type<64>(c, a, s, ctx);
+        case 128: return launch_type<128>(c, a, s, ctx);
+        case 256: return launch_type<256>(c, a, s, ctx);
+        default: return launch_type<512>(c, a, s, ctx);
+    }
 }
 
 }  // namespace moa
