@@ -30,15 +30,16 @@ __device__ __forceinline__ bf16x8 as_bf16x8(const uint4& v) { return __builtin_b
 
 // How a call's sequences are split into items, the same in every kernel of the call. A sequence of r = n * group rows has
 // ceil(r / bm) tiles, each split over ceil(units / c) items, where units covers the positions a tile can see in steps of
-// `unit`, and c is chosen so that all sequences together have at most `items` items per KV head.
+// `unit`, and c, at least min_units, is chosen so that all sequences together have at most `items` items per KV head (a
+// call with more tiles than that splits none). The last tiles of a sequence, which see the most, come first.
 struct PlanArgs {
-    int bm, unit, items;
+    int bm, unit, items, min_units;
     bool tokens;  // the token kernel's sequences (at most kTokenRows rows) or the others
 };
 
 struct Piece {  // an item, or a row of the merge
     int s, row0, n, len;    // its sequence: first row of the call, new rows, length
-    int tile, split, splits, units_per;
+    int tile, split, splits;
     int record;             // the first record of its tile
     int row;                // the merge: row of the sequence
 };
@@ -88,7 +89,7 @@ __device__ bool find_piece(const PagedView& c, const PagedAttentionCall& a, cons
     // sum of ceil(units / c) <= units / c + tiles <= items
     const uint64_t room = tiles < (uint64_t)p.items ? p.items - tiles : 0;
     const uint64_t per64 = room ? (units + room - 1) / room : 1u << 30;
-    const int per = (int)(per64 < 1 ? 1 : (per64 > (1u << 30) ? 1u << 30 : per64));
+    const int per = (int)(per64 < (uint64_t)p.min_units ? p.min_units : (per64 > (1u << 30) ? 1u << 30 : per64));
     int64_t items_before = 0, rows_before = 0;
     for (int base = 0; base < c.sequences; base += 64) {
         if (c.sequences > 64) w = seq_work(c, a, p, base + lane, &bad);
@@ -114,19 +115,22 @@ __device__ bool find_piece(const PagedView& c, const PagedAttentionCall& a, cons
             auto get = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
             out->s = base + l;
             out->row0 = get(w.row0), out->n = get(w.n), out->len = get(w.len);
-            out->splits = get(splits), out->units_per = per;
+            out->splits = get(splits);
+            const int tiles_here = get(w.tiles);
             const int first_item = get((int)(items_before + xi - items));
             if (merge) {
                 out->row = (int)(want - __shfl(mine - rows, l, kWave));
                 out->tile = out->row / p.bm;
                 out->split = 0;
+                out->record = first_item + (tiles_here - 1 - out->tile) * out->splits;
             } else {
                 const int k = (int)(want - __shfl(mine - items, l, kWave));
-                out->tile = k / out->splits;
-                out->split = k - out->tile * out->splits;
+                const int j = k / out->splits;
+                out->tile = tiles_here - 1 - j;
+                out->split = k - j * out->splits;
                 out->row = 0;
+                out->record = first_item + j * out->splits;
             }
-            out->record = first_item + out->tile * out->splits;
             return true;
         }
         items_before += __shfl(xi, 63, kWave);
@@ -137,7 +141,7 @@ __device__ bool find_piece(const PagedView& c, const PagedAttentionCall& a, cons
 
 // Records of split tiles: per tile and split bm maxima, bm sums, out [bm][dim], f32. A record whose keys include a page
 // outside the pool has NaN maxima: its rows are not written.
-__device__ __forceinline__ int64_t record_floats(int bm, int dim) { return (int64_t)bm * (2 + dim); }
+__host__ __device__ inline int64_t record_floats(int bm, int dim) { return (int64_t)bm * (2 + dim); }
 
 // One row by one wave over positions [lo, hi), nothing outside them used: 64 positions at a time, a lane each for the
 // scores; then lane l holds dims l * dim / 64 .. and takes the weights in turn. The kernels fall back to it where a value that
@@ -205,6 +209,17 @@ __device__ __forceinline__ Row row_of(const PagedAttentionCall& a, const Piece& 
     x.hi = p + 1;
     x.lo = a.window && p >= a.window ? p - a.window + 1 : 0;
     return x;
+}
+
+// The positions [lo, hi) of a piece's split: what rows r0 .. r1 of its sequence see, from a multiple of `align` on, in even
+// parts of whole units.
+struct Span { int lo, hi; };
+__device__ __forceinline__ Span span_of(const PagedAttentionCall& a, const Piece& t, int r0, int r1, int unit, int align) {
+    const int p0 = t.len - t.n + r0 / a.group, p1 = t.len - t.n + r1 / a.group;
+    const int lo = a.window && p0 >= a.window ? (p0 - a.window + 1) / align * align : 0, hi = max(p1 + 1, lo);
+    const int units = (hi - lo + unit - 1) / unit, per = (units + t.splits - 1) / t.splits;
+    const int64_t from = (int64_t)t.split * per * unit, to = from + (int64_t)per * unit;
+    return {(int)min((int64_t)hi, lo + from), (int)min((int64_t)hi, lo + to)};
 }
 
 // The careful path for a piece's rows [r0, r0 + nr) over positions [lo, hi), waves taking rows in turn.
@@ -287,10 +302,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(TokenShape<
     Piece t;
     for (int64_t item = blockIdx.x / c.kv_heads; find_piece(c, a, plan, false, item, &t); item += gridDim.x / c.kv_heads) {
         const int nr = t.n * a.group;
-        // the item's positions, from a multiple of the tile on
-        const int first = a.window ? max(0, t.len - t.n + 1 - a.window) / T::kTile * T::kTile : 0;
-        const int lo = first + min((int64_t)t.split * t.units_per * kTokenUnit, (int64_t)1 << 30);
-        const int hi = (int)min((int64_t)lo + (int64_t)t.units_per * kTokenUnit, (int64_t)t.len);
+        const Span span = span_of(a, t, 0, nr - 1, kTokenUnit, T::kTile);
+        const int lo = span.lo, hi = span.hi;
         __syncthreads();  // the item before has been written out
         for (int i = threadIdx.x; i < 16 * D / 8; i += 256) {
             const int r = i / (D / 8), j = i - r * (D / 8);
@@ -561,40 +574,293 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedView c, PagedAtte
     }
 }
 
-// ---------------------------------------------------------------------- rows of longer sequences, one wave each
+// ------------------------------------------------------------------------------------ the chunk kernel
 
-template <bool E4M3>
-__global__ __launch_bounds__(256) void paged_attention_row_kernel(PagedView c, PagedAttentionCall a) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t unit = (int64_t)blockIdx.x * 4 + wave;
-    const int m = (int)(unit / a.q_heads), h = (int)(unit - (int64_t)m * a.q_heads), kvh = h / a.group;
-    if (m >= a.rows) return;
-    const int s = sequence_of(a.starts, c.sequences, m);
-    if (s < 0 || s >= c.sequences) return;
-    const int start = a.starts[s], end = a.starts[s + 1], len = c.lens[s];
-    if (end <= m || (int64_t)(end - start) * a.group <= kTokenRows) return;
-    if (start < 0 || end > a.rows || end - start > a.max_rows || len < 0 || len > paged_capacity(c)) {
-        if (lane == 0) atomicOr(c.err, kErrPaged);
-        return;
+// 128 rows of a sequence (four waves of 32) over the positions they see: bound by the matrix cores and LDS. K and V tiles
+// of kTile positions go through LDS, two buffers, the next tile loading while this one is used (bf16: loads straight into
+// LDS; E4M3: through registers, widened to bf16 once for all waves). Scores are K times Q^T (32 x 32 x 16 MFMAs):
+// lane (c = lane % 32, hf = lane / 32) holds, for row c, positions 8 (e / 4) + 4 hf + e % 4 of 32, and 8 of them in a
+// row are what it supplies as B of V^T times P^T when V's transposing LDS reads fetch the same positions: P moves
+// between no lanes, and a row's maximum, sum and rescaling stay in its lane. P enters as bf16, each weight off by at most
+// 2^-8 of itself: a second part, as in the token kernel, would add half as much matrix work again for a result that
+// is rounded to bf16 anyway. The sum adds the unrounded weights in f32.
+constexpr int kChunkRows = 128;
+template <int D, bool E4M3>
+struct ChunkShape {
+    static constexpr int kTile = D >= 256 ? 32 : 64;
+    static constexpr int kSub = kTile / 32;
+    static constexpr int kWavesPerSimd = D == 512 ? 1 : 2;
+    static constexpr int kRowBytes = 2 * D;                     // LDS row of a position
+    static constexpr int kRowsPerLoad = 1024 / kRowBytes;       // positions a wave's load into LDS covers
+    static constexpr int kLoads = kTile / 4 / kRowsPerLoad;     // loads of K (and of V) per wave and tile
+    static constexpr int kCodeLoads = kTile * D / 16 / 256;     // E4M3: 16-byte loads of K (and V) per thread and tile
+};
+constexpr int kChunkUnit = 64;      // positions that a split is a multiple of
+constexpr int kChunkMinUnits = 4;   // and the fewest of them
+
+// 16-byte chunk c of LDS row r lies in chunk c ^ swizzle(r): sixteen rows' reads of one chunk, and four rows' reads of four
+// chunks, then meet on no bank. Rows of 128 bytes (64 dims) pair up: two rows span the banks.
+template <int D>
+__host__ __device__ constexpr int chunk_swizzle(int r) {
+    return D == 64 ? ((r >> 1 & 1) << 2 | (r >> 2 & 3)) : ((r & 3) << 2 | (r >> 2 & 3));
+}
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef __attribute__((address_space(3))) void lds_void;
+typedef __attribute__((address_space(1))) const void global_void;
+
+// Four transposing reads per dim tile and 32 positions, waited for here: the compiler would wait for every load into LDS
+// first. r[2 k + y]: positions 16 k + 8 y + 4 hf .. + 3 of the lane's dim.
+template <int ROW>
+__device__ __forceinline__ void read_v8(uint32_t a0, uint32_t a1, uint32_t b0, uint32_t b1, uint2 (&r)[8]) {
+    __asm__ volatile(
+        "ds_read_b64_tr_b16 %0, %8\n\t"
+        "ds_read_b64_tr_b16 %1, %9 offset:%12\n\t"
+        "ds_read_b64_tr_b16 %4, %10\n\t"
+        "ds_read_b64_tr_b16 %5, %11 offset:%12\n\t"
+        "ds_read_b64_tr_b16 %2, %8 offset:%13\n\t"
+        "ds_read_b64_tr_b16 %3, %9 offset:%14\n\t"
+        "ds_read_b64_tr_b16 %6, %10 offset:%13\n\t"
+        "ds_read_b64_tr_b16 %7, %11 offset:%14\n\t"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3]), "=&v"(r[4]), "=&v"(r[5]), "=&v"(r[6]), "=&v"(r[7])
+        : "v"(a0), "v"(a1), "v"(b0), "v"(b1), "n"(8 * ROW), "n"(16 * ROW), "n"(24 * ROW)
+        : "memory");
+}
+
+template <int N>
+struct Buf { static constexpr int n = N; };
+
+template <int D, bool E4M3>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(ChunkShape<D, E4M3>::kWavesPerSimd))) void paged_chunk_kernel(
+    PagedView c, PagedAttentionCall a, PlanArgs plan, float* part) {
+    using T = ChunkShape<D, E4M3>;
+    constexpr int kTile = T::kTile, kSteps = D / 16, kDims = D / 32;
+    __shared__ __attribute__((aligned(1024))) uint16_t k0[kTile * D], k1[kTile * D], v0[kTile * D], v1[kTile * D];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int l32 = lane & 31, hf = lane >> 5, l16 = lane & 15;
+    const int kvh = blockIdx.x % c.kv_heads;
+    const float factor = E4M3 ? c.k_scale[kvh] * a.scale_log2 : a.scale_log2;
+    // LDS byte addresses: K rows l32, chunk 2 s + hf; V's transposing reads (see read_v8), dim tile 0
+    const int ka = l32 * T::kRowBytes + (hf ^ chunk_swizzle<D>(l32)) * 16;
+    const int vrow = 4 * hf + (l16 >> 2);
+    const int va = vrow * T::kRowBytes + ((2 * (lane >> 4 & 1) + (l16 >> 1 & 1)) ^ chunk_swizzle<D>(vrow)) * 16 + (l16 & 1) * 8;
+    Piece t;
+    for (int64_t item = blockIdx.x / c.kv_heads; find_piece(c, a, plan, false, item, &t); item += gridDim.x / c.kv_heads) {
+        const int r0 = t.tile * kChunkRows, nr = (int)min((int64_t)kChunkRows, (int64_t)t.n * a.group - r0);
+        const Span span = span_of(a, t, r0, r0 + nr - 1, kChunkUnit, kTile);
+        const int lo = span.lo, hi = span.hi;
+        const int wrow = 32 * wave + l32;  // the lane's row of the tile
+        const Row mine = row_of(a, t, kvh, r0 + min(wrow, nr - 1));
+        const int see_lo = wrow < nr ? mine.lo : 0, see_hi = wrow < nr ? mine.hi : 0;
+        // positions that all of the wave's rows see, and that any does
+        int all_lo = mine.lo, all_hi = mine.hi, any_lo = mine.lo, any_hi = mine.hi;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            all_lo = max(all_lo, __shfl_xor(all_lo, o)), all_hi = min(all_hi, __shfl_xor(all_hi, o));
+            any_lo = min(any_lo, __shfl_xor(any_lo, o)), any_hi = max(any_hi, __shfl_xor(any_hi, o));
+        }
+        all_lo = __builtin_amdgcn_readfirstlane(all_lo), all_hi = __builtin_amdgcn_readfirstlane(all_hi);
+        any_lo = __builtin_amdgcn_readfirstlane(any_lo), any_hi = __builtin_amdgcn_readfirstlane(any_hi);
+        if (32 * wave >= nr) any_hi = 0;  // no rows
+
+        uint4 qf[kSteps];
+        {
+            const uint16_t* qp = a.q + mine.m * a.q_row + mine.h * D + 8 * hf;
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s) qf[s] = ld16(qp + 16 * s);
+        }
+        f32x16 o[kDims];
+#pragma unroll
+        for (int d = 0; d < kDims; ++d)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[d][e] = 0.0f;
+        float m_run = -INFINITY, m_ref = -INFINITY, l_run = 0.0f;
+        bool bad = false;
+
+        const int32_t* table = c.table + t.s * c.table_stride;
+        const uint8_t *kbase = c.k + kvh * c.k_head, *vbase = c.v + kvh * c.v_head;
+        // lane l looks after position t0 + l % kTile, its page a tile ahead of its use
+        auto page_at = [&](int t0) { return t0 < hi ? table[page_of(c, min(t0 + lane % kTile, hi - 1))] : 0; };
+        int64_t koff = 0, voff = 0;
+        auto place = [&](int page, int t0) {
+            const int p = min(t0 + lane % kTile, hi - 1);
+            const bool in = page >= 0 && page < c.pages;
+            bad |= !in;
+            page = in ? page : 0;
+            const uint32_t slot = p - page_of(c, p) * c.slots;
+            koff = page * c.k_page + slot * c.k_slot;
+            voff = page * c.v_page + slot * c.v_slot;
+        };
+        auto load_tile = [&](uint16_t* kd, uint16_t* vd) {  // bf16: this wave's quarter of the tile, straight into LDS
+#pragma unroll
+            for (int i = 0; i < T::kLoads; ++i) {
+                const int row = wave * (kTile / 4) + i * T::kRowsPerLoad, mr = row + lane / (64 / T::kRowsPerLoad);
+                const int at = ((lane % (64 / T::kRowsPerLoad)) ^ chunk_swizzle<D>(mr)) * 16;
+                __builtin_amdgcn_global_load_lds((global_void*)(kbase + __shfl(koff, mr, kWave) + at), (lds_void*)(kd + row * D), 16, 0, 0);
+                __builtin_amdgcn_global_load_lds((global_void*)(vbase + __shfl(voff, mr, kWave) + at), (lds_void*)(vd + row * D), 16, 0, 0);
+            }
+        };
+        // E4M3: thread i of 256 takes 16 codes of row 256 j / (D / 16) + i / (D / 16)
+        uint4 kc[T::kCodeLoads], vc[T::kCodeLoads];
+        auto load_codes = [&] {
+#pragma unroll
+            for (int j = 0; j < T::kCodeLoads; ++j) {
+                const int x = 256 * j + (int)threadIdx.x, row = x / (D / 16), at = x % (D / 16) * 16;
+                kc[j] = ld16(kbase + __shfl(koff, row, kWave) + at);
+                vc[j] = ld16(vbase + __shfl(voff, row, kWave) + at);
+            }
+        };
+        auto store_codes = [&](uint16_t* kd, uint16_t* vd) {
+            auto put = [&](uint16_t* d, const uint4& w, int row, int col) {
+                const uint4 lo8 = make_uint4(bf16_pair_of_fp8(w.x), bf16_pair_of_fp8(w.x >> 16), bf16_pair_of_fp8(w.y), bf16_pair_of_fp8(w.y >> 16));
+                const uint4 hi8 = make_uint4(bf16_pair_of_fp8(w.z), bf16_pair_of_fp8(w.z >> 16), bf16_pair_of_fp8(w.w), bf16_pair_of_fp8(w.w >> 16));
+                *reinterpret_cast<uint4*>(d + row * D + ((2 * col) ^ chunk_swizzle<D>(row)) * 8) = lo8;
+                *reinterpret_cast<uint4*>(d + row * D + ((2 * col + 1) ^ chunk_swizzle<D>(row)) * 8) = hi8;
+            };
+#pragma unroll
+            for (int j = 0; j < T::kCodeLoads; ++j) {
+                const int x = 256 * j + (int)threadIdx.x, row = x / (D / 16), col = x % (D / 16);
+                put(kd, kc[j], row, col);
+                put(vd, vc[j], row, col);
+            }
+        };
+
+        auto compute = [&](const uint16_t* ks, const uint16_t* vs, int t0) __attribute__((always_inline)) {
+            if (t0 >= any_hi || t0 + kTile <= any_lo) return;
+            f32x16 sc[T::kSub];
+#pragma unroll
+            for (int b = 0; b < T::kSub; ++b)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) sc[b][e] = 0.0f;
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+                for (int b = 0; b < T::kSub; ++b) {
+                    const bf16x8 kf = *reinterpret_cast<const bf16x8*>(reinterpret_cast<const uint8_t*>(ks) + (ka ^ (32 * (s & 7))) +
+                                                                       256 * (s >> 3) + b * 32 * T::kRowBytes);
+                    sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, as_bf16x8(qf[s]), sc[b], 0, 0, 0);
+                }
+            const bool whole = t0 >= all_lo && t0 + kTile <= all_hi;
+            float mx = -INFINITY;
+#pragma unroll
+            for (int b = 0; b < T::kSub; ++b)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const int p = t0 + 32 * b + 8 * (e >> 2) + 4 * hf + (e & 3);
+                    sc[b][e] *= factor;
+                    if (!whole) sc[b][e] = p >= see_lo && p < see_hi ? sc[b][e] : -INFINITY;
+                    mx = fmaxf(mx, sc[b][e]);
+                }
+            mx = fmaxf(mx, __shfl_xor(mx, 32));
+            m_run = fmaxf(m_run, mx);
+            float scale = 1.0f;
+            if (m_run > m_ref + kSlack) {
+                scale = m_ref == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m_ref - m_run);
+                m_ref = m_run;
+            }
+            if (__any(scale != 1.0f)) {
+#pragma unroll
+                for (int d = 0; d < kDims; ++d)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) o[d][e] *= scale;
+            }
+            const float mu = m_ref == -INFINITY ? 0.0f : m_ref;
+            uint32_t pw[T::kSub][8];
+            float sum = 0.0f;
+#pragma unroll
+            for (int b = 0; b < T::kSub; ++b)
+#pragma unroll
+                for (int e = 0; e < 16; e += 2) {
+                    const float p0 = __builtin_amdgcn_exp2f(sc[b][e] - mu), p1 = __builtin_amdgcn_exp2f(sc[b][e + 1] - mu);
+                    sum += p0 + p1;
+                    pw[b][e / 2] = pk_bf16(p0, p1);
+                }
+            l_run = fmaf(l_run, scale, sum);
+            const uint32_t vb = (uint32_t)(uintptr_t)(lds_void*)vs + va;
+#pragma unroll
+            for (int b = 0; b < T::kSub; ++b) {
+                const bf16x8 p0 = as_bf16x8(make_uint4(pw[b][0], pw[b][1], pw[b][2], pw[b][3]));
+                const bf16x8 p1 = as_bf16x8(make_uint4(pw[b][4], pw[b][5], pw[b][6], pw[b][7]));
+#pragma unroll
+                for (int d = 0; d < kDims; d += 2) {
+                    uint2 r[8];
+                    const uint32_t at = vb + b * 32 * T::kRowBytes;
+                    // the second eight positions' swizzle differs in bit 1 of the chunk (rows of 128 bytes: bit 1 too)
+                    const uint32_t x0 = (at ^ (64 * (d & 3))) + 256 * (d >> 2), x1 = (at ^ (64 * ((d + 1) & 3))) + 256 * ((d + 1) >> 2);
+                    read_v8<T::kRowBytes>(x0, x0 ^ 32, x1, x1 ^ 32, r);
+                    auto frag = [&](int i) { return as_bf16x8(make_uint4(r[i].x, r[i].y, r[i + 1].x, r[i + 1].y)); };
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag(0), p0, o[d], 0, 0, 0);
+                    o[d + 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag(4), p0, o[d + 1], 0, 0, 0);
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag(2), p1, o[d], 0, 0, 0);
+                    o[d + 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag(6), p1, o[d + 1], 0, 0, 0);
+                }
+            }
+        };
+        // this wave's loads into LDS are done, and then everybody's; and everybody has read the other buffer
+        auto ready = [&] {
+            __asm__ volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            __asm__ volatile("" ::: "memory");
+        };
+
+        __syncthreads();  // the item before has read its last tile
+        int t0 = lo, page = 0;
+        if (t0 < hi) {
+            place(page_at(t0), t0);
+            page = page_at(t0 + kTile);
+            if constexpr (E4M3) {
+                load_codes();
+                store_codes(k0, v0);
+            } else {
+                load_tile(k0, v0);
+            }
+        }
+        auto step = [&](auto buf) __attribute__((always_inline)) {
+            constexpr int n = decltype(buf)::n;
+            uint16_t *kn = n ? k0 : k1, *vn = n ? v0 : v1;
+            ready();
+            const bool more = t0 + kTile < hi;
+            if (more) {
+                place(page, t0 + kTile);
+                page = page_at(t0 + 2 * kTile);
+                if constexpr (E4M3) load_codes();
+                else load_tile(kn, vn);
+            }
+            compute(n ? k1 : k0, n ? v1 : v0, t0);
+            if (E4M3 && more) store_codes(kn, vn);
+            t0 += kTile;
+        };
+        while (t0 < hi) {
+            step(Buf<0>{});
+            if (t0 >= hi) break;
+            step(Buf<1>{});
+        }
+
+        l_run += __shfl_xor(l_run, 32);
+        bad = __syncthreads_or(bad);
+        float* rec = t.splits > 1 ? part + ((int64_t)kvh * plan.items + t.record + t.split) * record_floats(kChunkRows, D) : nullptr;
+        const float inv = l_run == 0.0f ? 0.0f : (E4M3 ? c.v_scale[kvh] : 1.0f) / l_run;
+        bool odd = false;
+        if (wrow < nr) {
+#pragma unroll
+            for (int d = 0; d < kDims; ++d)
+#pragma unroll
+                for (int e = 0; e < 16; e += 4) {
+                    const float x = o[d][e], y = o[d][e + 1], z = o[d][e + 2], w = o[d][e + 3];
+                    odd |= !(fabsf(x) + fabsf(y) + fabsf(z) + fabsf(w) < INFINITY);
+                    const int dim = 32 * d + 2 * e + 4 * hf;
+                    if (rec) *reinterpret_cast<float4*>(rec + 2 * kChunkRows + wrow * D + dim) = make_float4(x, y, z, w);
+                    else if (!bad)
+                        *reinterpret_cast<uint2*>(a.out + mine.m * a.out_row + mine.h * D + dim) =
+                            make_uint2(pk_bf16(x * inv, y * inv), pk_bf16(z * inv, w * inv));
+                }
+            if (rec && hf == 0) rec[wrow] = bad ? NAN : m_ref, rec[kChunkRows + wrow] = l_run;
+        }
+        odd = __syncthreads_or(odd);
+        if (bad && threadIdx.x == 0) atomicOr(c.err, kErrPaged);
+        if (odd && !bad) careful_piece<E4M3>(c, a, t, kvh, r0, nr, lo, hi, rec, kChunkRows);
     }
-    Piece t = {s, start, end - start, len, 0, 0, 1, 0, 0, 0};
-    const int r = (m - start) * a.group + (h - kvh * a.group);
-    const Row x = row_of(a, t, kvh, r);
-    bool bad = false;
-    for (int i = lane; x.hi > x.lo && i <= (int)page_of(c, x.hi - 1); i += 64) {
-        const int p = c.table[s * c.table_stride + i];
-        bad |= i >= (int)page_of(c, x.lo) && (p < 0 || p >= c.pages);
-    }
-    if (__any(bad)) {
-        if (lane == 0) atomicOr(c.err, kErrPaged);
-        return;
-    }
-    float o[8], mx, sum;
-    careful_row<E4M3>(c, a.q + x.m * a.q_row + x.h * c.head_dim, s, kvh, E4M3 ? c.k_scale[kvh] * a.scale_log2 : a.scale_log2, x.lo, x.hi,
-                      &mx, &sum, o);
-    const float inv = sum == 0.0f ? 0.0f : (E4M3 ? c.v_scale[kvh] : 1.0f) / sum;
-    const int per = c.head_dim / 64;
-    for (int k = 0; k < per; ++k) a.out[x.m * a.out_row + x.h * c.head_dim + lane * per + k] = (uint16_t)f2bf(o[k] * inv);
 }
 
 int64_t clamp64(int64_t v, int64_t lo, int64_t hi) { return v < lo ? lo : (v > hi ? hi : v); }
@@ -606,7 +872,7 @@ hipError_t launch(const PagedView& c, const PagedAttentionCall& a, hipStream_t s
     // token kernel: about four items per workgroup that the device holds, and one more for every sequence
     const int resident = ctx->cus * T::kWavesPerSimd;
     const int64_t records = (int64_t)kPagedPartFloats / (kTokenRows * (2 + D)) / c.kv_heads;
-    const PlanArgs plan{kTokenRows, kTokenUnit, (int)clamp64(4 * (int64_t)resident / c.kv_heads + c.sequences, 1, records), true};
+    const PlanArgs plan{kTokenRows, kTokenUnit, (int)clamp64(4 * (int64_t)resident / c.kv_heads + c.sequences, 1, records), 1, true};
     const int64_t most_units = (a.window ? std::min<int64_t>(capacity, (int64_t)a.window + a.max_rows + kTokenUnit) : capacity) / kTokenUnit + 1;
     const int64_t items = std::min<int64_t>(plan.items, c.sequences * most_units);
     hipLaunchKernelGGL((paged_token_kernel<D, E4M3>), dim3((uint32_t)(items * c.kv_heads)), dim3(256), 0, s, c, a, plan, ctx->paged_part);
@@ -619,11 +885,20 @@ hipError_t launch(const PagedView& c, const PagedAttentionCall& a, hipStream_t s
         e = hipGetLastError();
         if (e != hipSuccess) return e;
     }
-    if ((int64_t)a.max_rows * a.group > kTokenRows) {
-        const int64_t units = (int64_t)a.rows * a.q_heads;
-        hipLaunchKernelGGL(paged_attention_row_kernel<E4M3>, dim3((uint32_t)((units + 3) / 4)), dim3(256), 0, s, c, a);
-        e = hipGetLastError();
-    }
+    if ((int64_t)a.max_rows * a.group <= kTokenRows) return e;
+    // chunk kernel: about two items per workgroup that the device holds
+    const int64_t held = 2 * (int64_t)ctx->cus * ChunkShape<D, E4M3>::kWavesPerSimd / c.kv_heads;
+    const PlanArgs chunks{kChunkRows, kChunkUnit, (int)clamp64(held, 1, (int64_t)kPagedPartFloats / record_floats(kChunkRows, D) / c.kv_heads),
+                          kChunkMinUnits, false};
+    const int64_t tiles = (int64_t)a.rows * a.group / kChunkRows + std::min(c.sequences, a.rows);
+    const int64_t grid = std::max<int64_t>(chunks.items, std::min<int64_t>(tiles, 65536 / c.kv_heads));
+    hipLaunchKernelGGL((paged_chunk_kernel<D, E4M3>), dim3((uint32_t)(grid * c.kv_heads)), dim3(256), 0, s, c, a, chunks, ctx->paged_part);
+    e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    const int64_t rows = (int64_t)a.rows * a.group * ((D + kMergeDims - 1) / kMergeDims);
+    hipLaunchKernelGGL((paged_merge_kernel<D, E4M3>), dim3((uint32_t)(std::min<int64_t>(rows, std::max(1, 2048 / c.kv_heads)) * c.kv_heads)),
+                       dim3(256), 0, s, c, a, chunks, ctx->paged_part);
+    e = hipGetLastError();
     return e;
 }
 
