@@ -9,6 +9,7 @@
 // the KV head, so one pass over K and V serves them all. Sequences with at most 16 such rows go to the token kernel,
 // the others to the chunk kernel; each finds its work from the row starts and lengths on the device.
 #include <algorithm>
+#include <type_traits>
 
 #include "moa_device.h"
 #include "moa_paged.h"
@@ -576,7 +577,7 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedView c, PagedAtte
 
 // ------------------------------------------------------------------------------------ the chunk kernel
 
-// 128 rows of a sequence (four waves of 32) over the positions they see: bound by the matrix cores and LDS. K and V tiles
+// 128 rows of a sequence (32 per wave) over the positions they see: bound by the matrix cores and LDS. K and V tiles
 // of kTile positions go through LDS, two buffers, the next tile loading while this one is used (bf16: loads straight into
 // LDS; E4M3: through registers, widened to bf16 once for all waves). Scores are K times Q^T (32 x 32 x 16 MFMAs):
 // lane (c = lane % 32, hf = lane / 32) holds, for row c, positions 8 (e / 4) + 4 hf + e % 4 of 32, and 8 of them in a
@@ -584,16 +585,20 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedView c, PagedAtte
 // between no lanes, and a row's maximum, sum and rescaling stay in its lane. P enters as bf16, each weight off by at most
 // 2^-8 of itself: a second part, as in the token kernel, would add half as much matrix work again for a result that
 // is rounded to bf16 anyway. The sum adds the unrounded weights in f32.
+// 512 dims: a row's Q and out do not fit beside each other in a wave's registers, so two waves share 32 rows, each with
+// half of the dims: they add the halves of the scores through LDS, and both weigh them.
 constexpr int kChunkRows = 128;
 template <int D, bool E4M3>
 struct ChunkShape {
     static constexpr int kTile = D >= 256 ? 32 : 64;
     static constexpr int kSub = kTile / 32;
-    static constexpr int kWavesPerSimd = D == 512 ? 1 : 2;
+    static constexpr int kPair = D == 512 ? 2 : 1;              // waves that share 32 rows
+    static constexpr int kThreads = 256 * kPair;
+    static constexpr int kHeld = D == 512 ? 1 : 2;              // workgroups on a CU: two waves per SIMD
     static constexpr int kRowBytes = 2 * D;                     // LDS row of a position
     static constexpr int kRowsPerLoad = 1024 / kRowBytes;       // positions a wave's load into LDS covers
-    static constexpr int kLoads = kTile / 4 / kRowsPerLoad;     // loads of K (and of V) per wave and tile
-    static constexpr int kCodeLoads = kTile * D / 16 / 256;     // E4M3: 16-byte loads of K (and V) per thread and tile
+    static constexpr int kLoads = kTile / (4 * kPair) / kRowsPerLoad;     // loads of K (and of V) per wave and tile
+    static constexpr int kCodeLoads = kTile * D / 16 / kThreads;     // E4M3: 16-byte loads of K (and V) per thread and tile
 };
 constexpr int kChunkUnit = 64;      // positions that a split is a multiple of
 constexpr int kChunkMinUnits = 4;   // and the fewest of them
@@ -628,19 +633,70 @@ __device__ __forceinline__ void read_v8(uint32_t a0, uint32_t a1, uint32_t b0, u
         : "memory");
 }
 
-template <int N>
-struct Buf { static constexpr int n = N; };
+// K's fragments of four 16-dim steps, of 32 (read_k4) or 64 positions (read_k8, r[4 + i]: the second 32), likewise.
+template <int OFF>
+__device__ __forceinline__ void read_k4(uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, bf16x8 (&r)[4]) {
+    __asm__ volatile(
+        "ds_read_b128 %0, %4 offset:%8\n\t"
+        "ds_read_b128 %1, %5 offset:%8\n\t"
+        "ds_read_b128 %2, %6 offset:%8\n\t"
+        "ds_read_b128 %3, %7 offset:%8\n\t"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3])
+        : "v"(a0), "v"(a1), "v"(a2), "v"(a3), "n"(OFF)
+        : "memory");
+}
+template <int OFF, int SUB>
+__device__ __forceinline__ void read_k8(uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, bf16x8 (&r)[8]) {
+    __asm__ volatile(
+        "ds_read_b128 %0, %8 offset:%12\n\t"
+        "ds_read_b128 %4, %8 offset:%13\n\t"
+        "ds_read_b128 %1, %9 offset:%12\n\t"
+        "ds_read_b128 %5, %9 offset:%13\n\t"
+        "ds_read_b128 %2, %10 offset:%12\n\t"
+        "ds_read_b128 %6, %10 offset:%13\n\t"
+        "ds_read_b128 %3, %11 offset:%12\n\t"
+        "ds_read_b128 %7, %11 offset:%13\n\t"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3]), "=&v"(r[4]), "=&v"(r[5]), "=&v"(r[6]), "=&v"(r[7])
+        : "v"(a0), "v"(a1), "v"(a2), "v"(a3), "n"(OFF), "n"(OFF + SUB)
+        : "memory");
+}
+
+// v, opaque to the compiler: what is computed from it in a loop is not kept in registers across the loop.
+__device__ __forceinline__ int in_loop(int v) {
+    __asm__ volatile("" : "+v"(v));
+    return v;
+}
 
 template <int D, bool E4M3>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(ChunkShape<D, E4M3>::kWavesPerSimd))) void paged_chunk_kernel(
+__global__ __launch_bounds__((ChunkShape<D, E4M3>::kThreads)) __attribute__((amdgpu_waves_per_eu(2))) void paged_chunk_kernel(
     PagedView c, PagedAttentionCall a, PlanArgs plan, float* part) {
     using T = ChunkShape<D, E4M3>;
-    constexpr int kTile = T::kTile, kSteps = D / 16, kDims = D / 32;
-    __shared__ __attribute__((aligned(1024))) uint16_t k0[kTile * D], k1[kTile * D], v0[kTile * D], v1[kTile * D];
+    constexpr int kTile = T::kTile, kPair = T::kPair, kWaves = 4 * kPair, kMine = D / kPair;  // dims of a wave
+    constexpr int kSteps = kMine / 16, kDims = kMine / 32;
+    constexpr int kTileBytes = kTile * T::kRowBytes;
+    __shared__ __attribute__((aligned(1024))) uint8_t tiles[4 * kTileBytes];  // two buffers of K and V
+    __shared__ float4 xs[kPair == 2 ? 8 * 4 * 64 : 16];  // pairs: the other wave's half of the scores; flags of the waves
+    auto any_wave = [&](bool x) {  // whether x holds in any thread; a barrier on both sides
+        uint32_t* f = reinterpret_cast<uint32_t*>(xs);
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) f[threadIdx.x >> 6] = 0;
+        if (__any(x)) f[threadIdx.x >> 6] = 1;
+        __syncthreads();
+        uint32_t r = 0;
+        for (int w = 0; w < kWaves; ++w) r |= f[w];
+        return r != 0;
+    };
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int l32 = lane & 31, hf = lane >> 5, l16 = lane & 15;
+    const int rg = wave & 3, half = wave >> 2;  // rows 32 rg .., dims half * kMine ..
     const int kvh = blockIdx.x % c.kv_heads;
-    const float factor = E4M3 ? c.k_scale[kvh] * a.scale_log2 : a.scale_log2;
+    // x = factor (q . k): a negative factor's sign goes to q, so that the largest product is the largest x; and a factor of
+    // zero stays above it, so that a product of -inf (a position that a row does not see) stays -inf
+    const float signed_factor = E4M3 ? c.k_scale[kvh] * a.scale_log2 : a.scale_log2;
+    const float factor = fmaxf(fabsf(signed_factor), 1.2e-38f);
+    const uint32_t flip = signed_factor < 0.0f ? 0x80008000u : 0u;
     // LDS byte addresses: K rows l32, chunk 2 s + hf; V's transposing reads (see read_v8), dim tile 0
     const int ka = l32 * T::kRowBytes + (hf ^ chunk_swizzle<D>(l32)) * 16;
     const int vrow = 4 * hf + (l16 >> 2);
@@ -650,7 +706,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(ChunkShape<
         const int r0 = t.tile * kChunkRows, nr = (int)min((int64_t)kChunkRows, (int64_t)t.n * a.group - r0);
         const Span span = span_of(a, t, r0, r0 + nr - 1, kChunkUnit, kTile);
         const int lo = span.lo, hi = span.hi;
-        const int wrow = 32 * wave + l32;  // the lane's row of the tile
+        const int wrow = 32 * rg + l32;  // the lane's row of the tile
         const Row mine = row_of(a, t, kvh, r0 + min(wrow, nr - 1));
         const int see_lo = wrow < nr ? mine.lo : 0, see_hi = wrow < nr ? mine.hi : 0;
         // positions that all of the wave's rows see, and that any does
@@ -662,13 +718,16 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(ChunkShape<
         }
         all_lo = __builtin_amdgcn_readfirstlane(all_lo), all_hi = __builtin_amdgcn_readfirstlane(all_hi);
         any_lo = __builtin_amdgcn_readfirstlane(any_lo), any_hi = __builtin_amdgcn_readfirstlane(any_hi);
-        if (32 * wave >= nr) any_hi = 0;  // no rows
+        if (32 * rg >= nr) any_hi = 0;  // no rows
 
         uint4 qf[kSteps];
         {
-            const uint16_t* qp = a.q + mine.m * a.q_row + mine.h * D + 8 * hf;
+            const uint16_t* qp = a.q + mine.m * a.q_row + mine.h * D + half * kMine + 8 * hf;
 #pragma unroll
-            for (int s = 0; s < kSteps; ++s) qf[s] = ld16(qp + 16 * s);
+            for (int s = 0; s < kSteps; ++s) {
+                qf[s] = ld16(qp + 16 * s);
+                qf[s] = make_uint4(qf[s].x ^ flip, qf[s].y ^ flip, qf[s].z ^ flip, qf[s].w ^ flip);
+            }
         }
         f32x16 o[kDims];
 #pragma unroll
@@ -692,68 +751,103 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(ChunkShape<
             koff = page * c.k_page + slot * c.k_slot;
             voff = page * c.v_page + slot * c.v_slot;
         };
-        auto load_tile = [&](uint16_t* kd, uint16_t* vd) {  // bf16: this wave's quarter of the tile, straight into LDS
+        auto load_tile = [&](uint8_t* kd) {  // bf16: this wave's quarter of the tile, straight into LDS
+            const int ln = in_loop(lane);
 #pragma unroll
             for (int i = 0; i < T::kLoads; ++i) {
-                const int row = wave * (kTile / 4) + i * T::kRowsPerLoad, mr = row + lane / (64 / T::kRowsPerLoad);
-                const int at = ((lane % (64 / T::kRowsPerLoad)) ^ chunk_swizzle<D>(mr)) * 16;
-                __builtin_amdgcn_global_load_lds((global_void*)(kbase + __shfl(koff, mr, kWave) + at), (lds_void*)(kd + row * D), 16, 0, 0);
-                __builtin_amdgcn_global_load_lds((global_void*)(vbase + __shfl(voff, mr, kWave) + at), (lds_void*)(vd + row * D), 16, 0, 0);
+                const int row = wave * (kTile / kWaves) + i * T::kRowsPerLoad, mr = row + ln / (64 / T::kRowsPerLoad);
+                const int at = ((ln % (64 / T::kRowsPerLoad)) ^ chunk_swizzle<D>(mr)) * 16;
+                __builtin_amdgcn_global_load_lds((global_void*)(kbase + __shfl(koff, mr, kWave) + at), (lds_void*)(kd + row * T::kRowBytes), 16, 0, 0);
+                __builtin_amdgcn_global_load_lds((global_void*)(vbase + __shfl(voff, mr, kWave) + at), (lds_void*)(kd + kTileBytes + row * T::kRowBytes), 16, 0, 0);
             }
         };
-        // E4M3: thread i of 256 takes 16 codes of row 256 j / (D / 16) + i / (D / 16)
+        // E4M3: thread i takes 16 codes a load, D / 16 threads a row
         uint4 kc[T::kCodeLoads], vc[T::kCodeLoads];
         auto load_codes = [&] {
+            const int tid = in_loop(threadIdx.x);
 #pragma unroll
             for (int j = 0; j < T::kCodeLoads; ++j) {
-                const int x = 256 * j + (int)threadIdx.x, row = x / (D / 16), at = x % (D / 16) * 16;
+                const int x = T::kThreads * j + tid, row = x / (D / 16), at = x % (D / 16) * 16;
                 kc[j] = ld16(kbase + __shfl(koff, row, kWave) + at);
                 vc[j] = ld16(vbase + __shfl(voff, row, kWave) + at);
             }
         };
-        auto store_codes = [&](uint16_t* kd, uint16_t* vd) {
-            auto put = [&](uint16_t* d, const uint4& w, int row, int col) {
+        auto store_codes = [&](uint8_t* kd) {
+            auto put = [&](uint8_t* d, const uint4& w, int row, int col) {
                 const uint4 lo8 = make_uint4(bf16_pair_of_fp8(w.x), bf16_pair_of_fp8(w.x >> 16), bf16_pair_of_fp8(w.y), bf16_pair_of_fp8(w.y >> 16));
                 const uint4 hi8 = make_uint4(bf16_pair_of_fp8(w.z), bf16_pair_of_fp8(w.z >> 16), bf16_pair_of_fp8(w.w), bf16_pair_of_fp8(w.w >> 16));
-                *reinterpret_cast<uint4*>(d + row * D + ((2 * col) ^ chunk_swizzle<D>(row)) * 8) = lo8;
-                *reinterpret_cast<uint4*>(d + row * D + ((2 * col + 1) ^ chunk_swizzle<D>(row)) * 8) = hi8;
+                *reinterpret_cast<uint4*>(d + row * T::kRowBytes + ((2 * col) ^ chunk_swizzle<D>(row)) * 16) = lo8;
+                *reinterpret_cast<uint4*>(d + row * T::kRowBytes + ((2 * col + 1) ^ chunk_swizzle<D>(row)) * 16) = hi8;
             };
+            const int tid = in_loop(threadIdx.x);
 #pragma unroll
             for (int j = 0; j < T::kCodeLoads; ++j) {
-                const int x = 256 * j + (int)threadIdx.x, row = x / (D / 16), col = x % (D / 16);
+                const int x = T::kThreads * j + tid, row = x / (D / 16), col = x % (D / 16);
                 put(kd, kc[j], row, col);
-                put(vd, vc[j], row, col);
+                put(kd + kTileBytes, vc[j], row, col);
             }
         };
 
-        auto compute = [&](const uint16_t* ks, const uint16_t* vs, int t0) __attribute__((always_inline)) {
-            if (t0 >= any_hi || t0 + kTile <= any_lo) return;
+        auto compute = [&](uint32_t tile, int t0) __attribute__((always_inline)) {  // tile: LDS address of the buffer
+            const bool sees = t0 < any_hi && t0 + kTile > any_lo;
+            if (kPair == 1 && !sees) return;
             f32x16 sc[T::kSub];
 #pragma unroll
             for (int b = 0; b < T::kSub; ++b)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) sc[b][e] = 0.0f;
+            {
+                const uint32_t kx = tile + half * kMine * 2 + in_loop(ka);
+                auto steps = [&](auto off) __attribute__((always_inline)) {  // four steps
+                    constexpr int s = decltype(off)::value;
+                    constexpr int x = 32 * (s & 7), at = 256 * (s >> 3);
+                    bf16x8 kf[4 * T::kSub];
+                    if constexpr (T::kSub == 1) read_k4<at>(kx ^ x, kx ^ (x + 32), kx ^ (x + 64), kx ^ (x + 96), kf);
+                    else read_k8<at, 32 * T::kRowBytes>(kx ^ x, kx ^ (x + 32), kx ^ (x + 64), kx ^ (x + 96), kf);
 #pragma unroll
-            for (int s = 0; s < kSteps; ++s)
+                    for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int b = 0; b < T::kSub; ++b) {
-                    const bf16x8 kf = *reinterpret_cast<const bf16x8*>(reinterpret_cast<const uint8_t*>(ks) + (ka ^ (32 * (s & 7))) +
-                                                                       256 * (s >> 3) + b * 32 * T::kRowBytes);
-                    sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, as_bf16x8(qf[s]), sc[b], 0, 0, 0);
+                        for (int b = 0; b < T::kSub; ++b)
+                            sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[4 * b + i], as_bf16x8(qf[s + i]), sc[b], 0, 0, 0);
+                };
+                steps(std::integral_constant<int, 0>{});
+                if constexpr (kSteps > 4) steps(std::integral_constant<int, 4>{});
+                if constexpr (kSteps > 8) {
+                    steps(std::integral_constant<int, 8>{});
+                    steps(std::integral_constant<int, 12>{});
                 }
-            const bool whole = t0 >= all_lo && t0 + kTile <= all_hi;
+            }
+            if constexpr (kPair == 2) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    xs[(wave * 4 + e) * 64 + lane] = make_float4(sc[0][4 * e], sc[0][4 * e + 1], sc[0][4 * e + 2], sc[0][4 * e + 3]);
+                __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                __builtin_amdgcn_s_barrier();
+                __asm__ volatile("" ::: "memory");
+                if (!sees) return;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float4 y = xs[((wave ^ 4) * 4 + e) * 64 + lane];
+                    sc[0][4 * e] += y.x, sc[0][4 * e + 1] += y.y, sc[0][4 * e + 2] += y.z, sc[0][4 * e + 3] += y.w;
+                }
+            }
+            if (t0 < all_lo || t0 + kTile > all_hi) {  // some row does not see all of it
+                const int from = in_loop(see_lo - t0 - 4 * hf), to = in_loop(see_hi - t0 - 4 * hf);
+#pragma unroll
+                for (int b = 0; b < T::kSub; ++b)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const int p = 32 * b + 8 * (e >> 2) + (e & 3);
+                        sc[b][e] = p >= from && p < to ? sc[b][e] : -INFINITY;
+                    }
+            }
             float mx = -INFINITY;
 #pragma unroll
             for (int b = 0; b < T::kSub; ++b)
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const int p = t0 + 32 * b + 8 * (e >> 2) + 4 * hf + (e & 3);
-                    sc[b][e] *= factor;
-                    if (!whole) sc[b][e] = p >= see_lo && p < see_hi ? sc[b][e] : -INFINITY;
-                    mx = fmaxf(mx, sc[b][e]);
-                }
+                for (int e = 0; e < 16; ++e) mx = fmaxf(mx, sc[b][e]);
             mx = fmaxf(mx, __shfl_xor(mx, 32));
-            m_run = fmaxf(m_run, mx);
+            m_run = fmaxf(m_run, mx * factor);
             float scale = 1.0f;
             if (m_run > m_ref + kSlack) {
                 scale = m_ref == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m_ref - m_run);
@@ -772,12 +866,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(ChunkShape<
             for (int b = 0; b < T::kSub; ++b)
 #pragma unroll
                 for (int e = 0; e < 16; e += 2) {
-                    const float p0 = __builtin_amdgcn_exp2f(sc[b][e] - mu), p1 = __builtin_amdgcn_exp2f(sc[b][e + 1] - mu);
+                    const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[b][e], factor, -mu));
+                    const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[b][e + 1], factor, -mu));
                     sum += p0 + p1;
                     pw[b][e / 2] = pk_bf16(p0, p1);
                 }
             l_run = fmaf(l_run, scale, sum);
-            const uint32_t vb = (uint32_t)(uintptr_t)(lds_void*)vs + va;
+            const uint32_t vb = tile + kTileBytes + half * kMine * 2 + in_loop(va);
 #pragma unroll
             for (int b = 0; b < T::kSub; ++b) {
                 const bf16x8 p0 = as_bf16x8(make_uint4(pw[b][0], pw[b][1], pw[b][2], pw[b][3]));
@@ -786,7 +881,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(ChunkShape<
                 for (int d = 0; d < kDims; d += 2) {
                     uint2 r[8];
                     const uint32_t at = vb + b * 32 * T::kRowBytes;
-                    // the second eight positions' swizzle differs in bit 1 of the chunk (rows of 128 bytes: bit 1 too)
+                    // the second eight positions' swizzle differs in bit 1 of the chunk
                     const uint32_t x0 = (at ^ (64 * (d & 3))) + 256 * (d >> 2), x1 = (at ^ (64 * ((d + 1) & 3))) + 256 * ((d + 1) >> 2);
                     read_v8<T::kRowBytes>(x0, x0 ^ 32, x1, x1 ^ 32, r);
                     auto frag = [&](int i) { return as_bf16x8(make_uint4(r[i].x, r[i].y, r[i + 1].x, r[i + 1].y)); };
@@ -805,59 +900,66 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(ChunkShape<
         };
 
         __syncthreads();  // the item before has read its last tile
-        int t0 = lo, page = 0;
-        if (t0 < hi) {
-            place(page_at(t0), t0);
-            page = page_at(t0 + kTile);
+        int page = 0;
+        if (lo < hi) {
+            place(page_at(lo), lo);
+            page = page_at(lo + kTile);
             if constexpr (E4M3) {
                 load_codes();
-                store_codes(k0, v0);
+                store_codes(tiles);
             } else {
-                load_tile(k0, v0);
+                load_tile(tiles);
             }
         }
-        auto step = [&](auto buf) __attribute__((always_inline)) {
-            constexpr int n = decltype(buf)::n;
-            uint16_t *kn = n ? k0 : k1, *vn = n ? v0 : v1;
+        const uint32_t lds = (uint32_t)(uintptr_t)(lds_void*)tiles;
+        uint32_t at = 0;  // the buffer in use
+        for (int t0 = lo; t0 < hi; t0 += kTile) {
             ready();
+            const uint32_t next = at ^ (2 * kTileBytes);
             const bool more = t0 + kTile < hi;
             if (more) {
                 place(page, t0 + kTile);
                 page = page_at(t0 + 2 * kTile);
                 if constexpr (E4M3) load_codes();
-                else load_tile(kn, vn);
+                else load_tile(tiles + next);
             }
-            compute(n ? k1 : k0, n ? v1 : v0, t0);
-            if (E4M3 && more) store_codes(kn, vn);
-            t0 += kTile;
-        };
-        while (t0 < hi) {
-            step(Buf<0>{});
-            if (t0 >= hi) break;
-            step(Buf<1>{});
+            compute(lds + at, t0);
+            if (E4M3 && more) store_codes(tiles + next);
+            at = next;
         }
 
         l_run += __shfl_xor(l_run, 32);
-        bad = __syncthreads_or(bad);
+        bad = any_wave(bad);
         float* rec = t.splits > 1 ? part + ((int64_t)kvh * plan.items + t.record + t.split) * record_floats(kChunkRows, D) : nullptr;
         const float inv = l_run == 0.0f ? 0.0f : (E4M3 ? c.v_scale[kvh] : 1.0f) / l_run;
         bool odd = false;
         if (wrow < nr) {
+            float most = 0.0f;
 #pragma unroll
             for (int d = 0; d < kDims; ++d)
 #pragma unroll
-                for (int e = 0; e < 16; e += 4) {
-                    const float x = o[d][e], y = o[d][e + 1], z = o[d][e + 2], w = o[d][e + 3];
-                    odd |= !(fabsf(x) + fabsf(y) + fabsf(z) + fabsf(w) < INFINITY);
-                    const int dim = 32 * d + 2 * e + 4 * hf;
-                    if (rec) *reinterpret_cast<float4*>(rec + 2 * kChunkRows + wrow * D + dim) = make_float4(x, y, z, w);
-                    else if (!bad)
-                        *reinterpret_cast<uint2*>(a.out + mine.m * a.out_row + mine.h * D + dim) =
-                            make_uint2(pk_bf16(x * inv, y * inv), pk_bf16(z * inv, w * inv));
-                }
-            if (rec && hf == 0) rec[wrow] = bad ? NAN : m_ref, rec[kChunkRows + wrow] = l_run;
+                for (int e = 0; e < 16; ++e) most += fabsf(o[d][e]);
+            odd = !(most < INFINITY);
+            const int first = half * kMine + 4 * hf;  // of the lane's dims: first + 32 d + 2 e .. + 3
+            if (rec) {
+                float* to = rec + 2 * kChunkRows + wrow * D + first;
+#pragma unroll
+                for (int d = 0; d < kDims; ++d)
+#pragma unroll
+                    for (int e = 0; e < 16; e += 4)
+                        *reinterpret_cast<float4*>(to + 32 * d + 2 * e) = make_float4(o[d][e], o[d][e + 1], o[d][e + 2], o[d][e + 3]);
+            } else if (!bad) {
+                uint16_t* to = a.out + mine.m * a.out_row + mine.h * D + first;
+#pragma unroll
+                for (int d = 0; d < kDims; ++d)
+#pragma unroll
+                    for (int e = 0; e < 16; e += 4)
+                        *reinterpret_cast<uint2*>(to + 32 * d + 2 * e) =
+                            make_uint2(pk_bf16(o[d][e] * inv, o[d][e + 1] * inv), pk_bf16(o[d][e + 2] * inv, o[d][e + 3] * inv));
+            }
+            if (rec && hf == 0 && half == 0) rec[wrow] = bad ? NAN : m_ref, rec[kChunkRows + wrow] = l_run;
         }
-        odd = __syncthreads_or(odd);
+        odd = any_wave(odd);
         if (bad && threadIdx.x == 0) atomicOr(c.err, kErrPaged);
         if (odd && !bad) careful_piece<E4M3>(c, a, t, kvh, r0, nr, lo, hi, rec, kChunkRows);
     }
@@ -887,12 +989,12 @@ hipError_t launch(const PagedView& c, const PagedAttentionCall& a, hipStream_t s
     }
     if ((int64_t)a.max_rows * a.group <= kTokenRows) return e;
     // chunk kernel: about two items per workgroup that the device holds
-    const int64_t held = 2 * (int64_t)ctx->cus * ChunkShape<D, E4M3>::kWavesPerSimd / c.kv_heads;
+    const int64_t held = 2 * (int64_t)ctx->cus * ChunkShape<D, E4M3>::kHeld / c.kv_heads;
     const PlanArgs chunks{kChunkRows, kChunkUnit, (int)clamp64(held, 1, (int64_t)kPagedPartFloats / record_floats(kChunkRows, D) / c.kv_heads),
                           kChunkMinUnits, false};
     const int64_t tiles = (int64_t)a.rows * a.group / kChunkRows + std::min(c.sequences, a.rows);
     const int64_t grid = std::max<int64_t>(chunks.items, std::min<int64_t>(tiles, 65536 / c.kv_heads));
-    hipLaunchKernelGGL((paged_chunk_kernel<D, E4M3>), dim3((uint32_t)(grid * c.kv_heads)), dim3(256), 0, s, c, a, chunks, ctx->paged_part);
+    hipLaunchKernelGGL((paged_chunk_kernel<D, E4M3>), dim3((uint32_t)(grid * c.kv_heads)), dim3(ChunkShape<D, E4M3>::kThreads), 0, s, c, a, chunks, ctx->paged_part);
     e = hipGetLastError();
     if (e != hipSuccess) return e;
     const int64_t rows = (int64_t)a.rows * a.group * ((D + kMergeDims - 1) / kMergeDims);
