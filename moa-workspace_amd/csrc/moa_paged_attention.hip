@@ -584,7 +584,7 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedView c, PagedAtte
 // row are what it supplies as B of V^T times P^T when V's transposing LDS reads fetch the same positions: P moves
 // between no lanes, and a row's maximum, sum and rescaling stay in its lane. P enters as bf16, each weight off by at most
 // 2^-8 of itself: a second part, as in the token kernel, would add half as much matrix work again for a result that
-// is rounded to bf16 anyway. The sum adds the unrounded weights in f32.
+// is rounded to bf16 anyway. The sum adds the weights as they enter, in f32: their roundings then cancel in part.
 // 512 dims: a row's Q and out do not fit beside each other in a wave's registers, so two waves share 32 rows, each with
 // half of the dims: they add the halves of the scores through LDS, and both weigh them.
 constexpr int kChunkRows = 128;
@@ -612,55 +612,14 @@ __host__ __device__ constexpr int chunk_swizzle(int r) {
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef __attribute__((address_space(3))) void lds_void;
-typedef __attribute__((address_space(1))) const void global_void;
 
-// Four transposing reads per dim tile and 32 positions, waited for here: the compiler would wait for every load into LDS
-// first. r[2 k + y]: positions 16 k + 8 y + 4 hf .. + 3 of the lane's dim.
-template <int ROW>
-__device__ __forceinline__ void read_v8(uint32_t a0, uint32_t a1, uint32_t b0, uint32_t b1, uint2 (&r)[8]) {
-    __asm__ volatile(
-        "ds_read_b64_tr_b16 %0, %8\n\t"
-        "ds_read_b64_tr_b16 %1, %9 offset:%12\n\t"
-        "ds_read_b64_tr_b16 %4, %10\n\t"
-        "ds_read_b64_tr_b16 %5, %11 offset:%12\n\t"
-        "ds_read_b64_tr_b16 %2, %8 offset:%13\n\t"
-        "ds_read_b64_tr_b16 %3, %9 offset:%14\n\t"
-        "ds_read_b64_tr_b16 %6, %10 offset:%13\n\t"
-        "ds_read_b64_tr_b16 %7, %11 offset:%14\n\t"
-        "s_waitcnt lgkmcnt(0)"
-        : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3]), "=&v"(r[4]), "=&v"(r[5]), "=&v"(r[6]), "=&v"(r[7])
-        : "v"(a0), "v"(a1), "v"(b0), "v"(b1), "n"(8 * ROW), "n"(16 * ROW), "n"(24 * ROW)
-        : "memory");
-}
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
-// K's fragments of four 16-dim steps, of 32 (read_k4) or 64 positions (read_k8, r[4 + i]: the second 32), likewise.
-template <int OFF>
-__device__ __forceinline__ void read_k4(uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, bf16x8 (&r)[4]) {
-    __asm__ volatile(
-        "ds_read_b128 %0, %4 offset:%8\n\t"
-        "ds_read_b128 %1, %5 offset:%8\n\t"
-        "ds_read_b128 %2, %6 offset:%8\n\t"
-        "ds_read_b128 %3, %7 offset:%8\n\t"
-        "s_waitcnt lgkmcnt(0)"
-        : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3])
-        : "v"(a0), "v"(a1), "v"(a2), "v"(a3), "n"(OFF)
-        : "memory");
-}
-template <int OFF, int SUB>
-__device__ __forceinline__ void read_k8(uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, bf16x8 (&r)[8]) {
-    __asm__ volatile(
-        "ds_read_b128 %0, %8 offset:%12\n\t"
-        "ds_read_b128 %4, %8 offset:%13\n\t"
-        "ds_read_b128 %1, %9 offset:%12\n\t"
-        "ds_read_b128 %5, %9 offset:%13\n\t"
-        "ds_read_b128 %2, %10 offset:%12\n\t"
-        "ds_read_b128 %6, %10 offset:%13\n\t"
-        "ds_read_b128 %3, %11 offset:%12\n\t"
-        "ds_read_b128 %7, %11 offset:%13\n\t"
-        "s_waitcnt lgkmcnt(0)"
-        : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3]), "=&v"(r[4]), "=&v"(r[5]), "=&v"(r[6]), "=&v"(r[7])
-        : "v"(a0), "v"(a1), "v"(a2), "v"(a3), "n"(OFF), "n"(OFF + SUB)
-        : "memory");
+// 16 bytes per lane from global memory into LDS, lane l's at lds + 16 l. In asm, since the compiler would let no LDS read
+// pass before all such loads are done; `ready` waits for them. (One wait state between the write of m0 and its use.)
+__device__ __forceinline__ void load_to_lds(const void* from, uint32_t lds) {
+    __asm__ volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "{m0}"(lds) : "memory");
 }
 
 // v, opaque to the compiler: what is computed from it in a loop is not kept in registers across the loop.
@@ -751,14 +710,14 @@ __global__ __launch_bounds__((ChunkShape<D, E4M3>::kThreads)) __attribute__((amd
             koff = page * c.k_page + slot * c.k_slot;
             voff = page * c.v_page + slot * c.v_slot;
         };
-        auto load_tile = [&](uint8_t* kd) {  // bf16: this wave's quarter of the tile, straight into LDS
+        auto load_tile = [&](uint32_t tile) {  // bf16: this wave's quarter of the tile, straight into LDS
             const int ln = in_loop(lane);
 #pragma unroll
             for (int i = 0; i < T::kLoads; ++i) {
                 const int row = wave * (kTile / kWaves) + i * T::kRowsPerLoad, mr = row + ln / (64 / T::kRowsPerLoad);
                 const int at = ((ln % (64 / T::kRowsPerLoad)) ^ chunk_swizzle<D>(mr)) * 16;
-                __builtin_amdgcn_global_load_lds((global_void*)(kbase + __shfl(koff, mr, kWave) + at), (lds_void*)(kd + row * T::kRowBytes), 16, 0, 0);
-                __builtin_amdgcn_global_load_lds((global_void*)(vbase + __shfl(voff, mr, kWave) + at), (lds_void*)(kd + kTileBytes + row * T::kRowBytes), 16, 0, 0);
+                load_to_lds(kbase + __shfl(koff, mr, kWave) + at, tile + row * T::kRowBytes);
+                load_to_lds(vbase + __shfl(voff, mr, kWave) + at, tile + kTileBytes + row * T::kRowBytes);
             }
         };
         // E4M3: thread i takes 16 codes a load, D / 16 threads a row
@@ -788,7 +747,7 @@ __global__ __launch_bounds__((ChunkShape<D, E4M3>::kThreads)) __attribute__((amd
             }
         };
 
-        auto compute = [&](uint32_t tile, int t0) __attribute__((always_inline)) {  // tile: LDS address of the buffer
+        auto compute = [&](uint32_t tile, int t0) __attribute__((always_inline)) {  // tile: the buffer's place in `tiles`
             const bool sees = t0 < any_hi && t0 + kTile > any_lo;
             if (kPair == 1 && !sees) return;
             f32x16 sc[T::kSub];
@@ -796,25 +755,26 @@ __global__ __launch_bounds__((ChunkShape<D, E4M3>::kThreads)) __attribute__((amd
             for (int b = 0; b < T::kSub; ++b)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) sc[b][e] = 0.0f;
+            // fragments are read kAhead steps before their MFMAs, and no further: the registers belong to Q and out
             {
-                const uint32_t kx = tile + half * kMine * 2 + in_loop(ka);
-                auto steps = [&](auto off) __attribute__((always_inline)) {  // four steps
-                    constexpr int s = decltype(off)::value;
-                    constexpr int x = 32 * (s & 7), at = 256 * (s >> 3);
-                    bf16x8 kf[4 * T::kSub];
-                    if constexpr (T::kSub == 1) read_k4<at>(kx ^ x, kx ^ (x + 32), kx ^ (x + 64), kx ^ (x + 96), kf);
-                    else read_k8<at, 32 * T::kRowBytes>(kx ^ x, kx ^ (x + 32), kx ^ (x + 64), kx ^ (x + 96), kf);
+                constexpr int kAhead = T::kSub == 2 ? 2 : 3;
+                const uint8_t* kt = tiles + tile + half * kMine * 2;
+                const int kx = in_loop(ka);
+                bf16x8 kf[kAhead][T::kSub];
+                auto read_k = [&](int s) __attribute__((always_inline)) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-#pragma unroll
-                        for (int b = 0; b < T::kSub; ++b)
-                            sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[4 * b + i], as_bf16x8(qf[s + i]), sc[b], 0, 0, 0);
+                    for (int b = 0; b < T::kSub; ++b)
+                        kf[s % kAhead][b] = *reinterpret_cast<const bf16x8*>(kt + (kx ^ (32 * (s & 7))) + 256 * (s >> 3) + b * 32 * T::kRowBytes);
                 };
-                steps(std::integral_constant<int, 0>{});
-                if constexpr (kSteps > 4) steps(std::integral_constant<int, 4>{});
-                if constexpr (kSteps > 8) {
-                    steps(std::integral_constant<int, 8>{});
-                    steps(std::integral_constant<int, 12>{});
+#pragma unroll
+                for (int s = 0; s < kAhead; ++s) read_k(s);
+#pragma unroll
+                for (int s = 0; s < kSteps; ++s) {
+#pragma unroll
+                    for (int b = 0; b < T::kSub; ++b)
+                        sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[s % kAhead][b], as_bf16x8(qf[s]), sc[b], 0, 0, 0);
+                    if (s + kAhead < kSteps) read_k(s + kAhead);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
             }
             if constexpr (kPair == 2) {
@@ -862,33 +822,43 @@ __global__ __launch_bounds__((ChunkShape<D, E4M3>::kThreads)) __attribute__((amd
             const float mu = m_ref == -INFINITY ? 0.0f : m_ref;
             uint32_t pw[T::kSub][8];
             float sum = 0.0f;
+            const bf16x2 ones = {(__bf16)1.0f, (__bf16)1.0f};
 #pragma unroll
             for (int b = 0; b < T::kSub; ++b)
 #pragma unroll
                 for (int e = 0; e < 16; e += 2) {
                     const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[b][e], factor, -mu));
                     const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[b][e + 1], factor, -mu));
-                    sum += p0 + p1;
                     pw[b][e / 2] = pk_bf16(p0, p1);
+                    sum = dot2_bf16(pw[b][e / 2], ones, sum);
                 }
             l_run = fmaf(l_run, scale, sum);
-            const uint32_t vb = tile + kTileBytes + half * kMine * 2 + in_loop(va);
+            {
+                constexpr int kAhead = 2, kN = T::kSub * kDims;  // step n: 32 positions n / kDims, dim tile n % kDims
+                uint8_t* vt = tiles + tile + kTileBytes + half * kMine * 2;
+                const int vx = in_loop(va);
+                s16x4 vr[kAhead][4];
+                auto read_v = [&](int n) __attribute__((always_inline)) {
+                    const int d = n % kDims, b = n / kDims;
 #pragma unroll
-            for (int b = 0; b < T::kSub; ++b) {
-                const bf16x8 p0 = as_bf16x8(make_uint4(pw[b][0], pw[b][1], pw[b][2], pw[b][3]));
-                const bf16x8 p1 = as_bf16x8(make_uint4(pw[b][4], pw[b][5], pw[b][6], pw[b][7]));
+                    for (int i = 0; i < 4; ++i)  // positions 8 i + 4 hf ..; an odd i's swizzle differs in bit 1 of the chunk
+                        vr[n % kAhead][i] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                            (lds_s16x4*)(vt + (vx ^ (64 * (d & 3) + 32 * (i & 1))) + 256 * (d >> 2) + (32 * b + 8 * i) * T::kRowBytes));
+                };
+                auto frag = [&](int n, int i) __attribute__((always_inline)) {
+                    return __builtin_bit_cast(bf16x8, __builtin_shufflevector(vr[n % kAhead][2 * i], vr[n % kAhead][2 * i + 1], 0, 1, 2, 3, 4, 5, 6, 7));
+                };
 #pragma unroll
-                for (int d = 0; d < kDims; d += 2) {
-                    uint2 r[8];
-                    const uint32_t at = vb + b * 32 * T::kRowBytes;
-                    // the second eight positions' swizzle differs in bit 1 of the chunk
-                    const uint32_t x0 = (at ^ (64 * (d & 3))) + 256 * (d >> 2), x1 = (at ^ (64 * ((d + 1) & 3))) + 256 * ((d + 1) >> 2);
-                    read_v8<T::kRowBytes>(x0, x0 ^ 32, x1, x1 ^ 32, r);
-                    auto frag = [&](int i) { return as_bf16x8(make_uint4(r[i].x, r[i].y, r[i + 1].x, r[i + 1].y)); };
-                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag(0), p0, o[d], 0, 0, 0);
-                    o[d + 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag(4), p0, o[d + 1], 0, 0, 0);
-                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag(2), p1, o[d], 0, 0, 0);
-                    o[d + 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag(6), p1, o[d + 1], 0, 0, 0);
+                for (int n = 0; n < kAhead; ++n) read_v(n);
+#pragma unroll
+                for (int n = 0; n < kN; ++n) {
+                    const int d = n % kDims, b = n / kDims;
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+                        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+                            frag(n, i), as_bf16x8(make_uint4(pw[b][4 * i], pw[b][4 * i + 1], pw[b][4 * i + 2], pw[b][4 * i + 3])), o[d], 0, 0, 0);
+                    if (n + kAhead < kN) read_v(n + kAhead);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
             }
         };
@@ -900,6 +870,7 @@ __global__ __launch_bounds__((ChunkShape<D, E4M3>::kThreads)) __attribute__((amd
         };
 
         __syncthreads();  // the item before has read its last tile
+        const uint32_t lds = (uint32_t)(uintptr_t)(lds_void*)tiles;
         int page = 0;
         if (lo < hi) {
             place(page_at(lo), lo);
@@ -908,10 +879,9 @@ __global__ __launch_bounds__((ChunkShape<D, E4M3>::kThreads)) __attribute__((amd
                 load_codes();
                 store_codes(tiles);
             } else {
-                load_tile(tiles);
+                load_tile(lds);
             }
         }
-        const uint32_t lds = (uint32_t)(uintptr_t)(lds_void*)tiles;
         uint32_t at = 0;  // the buffer in use
         for (int t0 = lo; t0 < hi; t0 += kTile) {
             ready();
@@ -921,9 +891,9 @@ __global__ __launch_bounds__((ChunkShape<D, E4M3>::kThreads)) __attribute__((amd
                 place(page, t0 + kTile);
                 page = page_at(t0 + 2 * kTile);
                 if constexpr (E4M3) load_codes();
-                else load_tile(tiles + next);
+                else load_tile(lds + next);
             }
-            compute(lds + at, t0);
+            compute(at, t0);
             if (E4M3 && more) store_codes(tiles + next);
             at = next;
         }
