@@ -71,10 +71,11 @@ constexpr int kOfnCopies = 8;  // copies of O's post-norm words in the single-la
 constexpr int kRowsFlagWords = 512;
 
 // The paged cache (moa_paged.hip): page lists and moves, and the split attention's records, f32
-// [16 or 128 query rows][max, sum, out[head_dim]] each: 72 MB, room for 274 records of 128 rows of 512 dims.
+// [16 or 128 query rows][max, sum, out[head_dim]] each: 160 MB, half of it for each kernel of a call that has both,
+// room for 318 records of 128 rows of 512 dims.
 constexpr int kPagedMaxPages = 1 << 20;
 constexpr int kPagedMaxSequences = 1 << 16;
-constexpr size_t kPagedPartFloats = 18 << 20;
+constexpr size_t kPagedPartFloats = 40 << 20;
 
 // Device-side error bits (OR-ed by kernels; read back by moa_device_errors()).
 constexpr uint32_t kErrRopeOffset = 1u;

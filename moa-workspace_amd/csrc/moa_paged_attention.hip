@@ -42,7 +42,7 @@ struct Piece {  // an item, or a row of the merge
     int s, row0, n, len;    // its sequence: first row of the call, new rows, length
     int tile, split, splits;
     int record;             // the first record of its tile
-    int row;                // the merge: row of the sequence
+    int row;                // the merge: first row of the block, in its sequence
 };
 
 struct SeqWork { int row0, n, len, tiles, units; };
@@ -59,9 +59,9 @@ __device__ __forceinline__ SeqWork seq_work(const PagedView& c, const PagedAtten
         *bad = true;
         return w;
     }
-    const int64_t rows = (int64_t)w.n * a.group;
+    const int rows = w.n * a.group;  // at most 2^20 * 128
     if ((rows <= kTokenRows) != p.tokens) return w;
-    w.tiles = (int)((rows + p.bm - 1) / p.bm);
+    w.tiles = (rows + p.bm - 1) / p.bm;
     // positions that a tile's rows see: all, or the window and the tile's tokens, from a multiple of the unit on
     const int span = p.tokens ? w.n : min(w.n, (p.bm + a.group - 1) / a.group + 1);
     const int seen = a.window ? min(w.len, a.window + span - 1 + p.unit) : w.len;
@@ -69,73 +69,73 @@ __device__ __forceinline__ SeqWork seq_work(const PagedView& c, const PagedAtten
     return w;
 }
 
-// Finds piece `want` of KV head-independent work by one wave: of items (merge = false) or of rows whose tiles are split
-// (merge = true). False: there are not that many.
-__device__ bool find_piece(const PagedView& c, const PagedAttentionCall& a, const PlanArgs& p, bool merge, int64_t want, Piece* out) {
+// Inclusive sum over the wave's lanes: four shifts within rows of 16, then the rows' last lanes (DPP: no LDS on the way).
+__device__ __forceinline__ int scan_sum(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);
+    return x;
+}
+__device__ __forceinline__ int wave_total(int x) { return __builtin_amdgcn_readlane(scan_sum(x), 63); }
+
+// Finds piece `want` by one wave: an item (merge_rows = 0), or block `want` of merge_rows rows of the tiles that are split.
+// False: there are not that many.
+__device__ bool find_piece(const PagedView& c, const PagedAttentionCall& a, const PlanArgs& p, int merge_rows, int want, Piece* out) {
     const int lane = threadIdx.x & 63;
-    uint64_t tiles = 0, units = 0;
+    int tiles = 0;
+    float units = 0.0f;
     bool bad = false;
     SeqWork w = {};
     for (int base = 0; base < c.sequences; base += 64) {
         w = seq_work(c, a, p, base + lane, &bad);
         tiles += w.tiles;
-        units += (uint64_t)w.tiles * w.units;
+        units += (float)w.tiles * (float)w.units;
     }
     if (__any(bad) && blockIdx.x == 0 && lane == 0) atomicOr(c.err, kErrPaged);
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        tiles += __shfl_xor(tiles, o, kWave);
-        units += __shfl_xor(units, o, kWave);
-    }
-    // sum of ceil(units / c) <= units / c + tiles <= items
-    const uint64_t room = tiles < (uint64_t)p.items ? p.items - tiles : 0;
-    const uint64_t per64 = room ? (units + room - 1) / room : 1u << 30;
-    const int per = (int)(per64 < (uint64_t)p.min_units ? p.min_units : (per64 > (1u << 30) ? 1u << 30 : per64));
-    int64_t items_before = 0, rows_before = 0;
+    tiles = wave_total(tiles);  // at most 2^20 rows * 128 heads / bm, and one per sequence
+    if (tiles == 0) return false;
+    // sum of ceil(units / per) <= units / per + tiles <= items. The float sum is rounded the same in every wave, and
+    // short by at most 1024 + 8 roundings of 2^-24: a part in ten thousand more covers them.
+    units = wave_sum(units);
+    int per = 1 << 30;
+    if (tiles < p.items) per = max(p.min_units, (int)fminf(units * 1.0001f / (float)(p.items - tiles) + 1.0f, 1e9f));
+    int items_before = 0, blocks_before = 0;
     for (int base = 0; base < c.sequences; base += 64) {
         if (c.sequences > 64) w = seq_work(c, a, p, base + lane, &bad);
-        const int splits = w.tiles ? (w.units + per - 1) / per : 0;
-        const int64_t items = (int64_t)w.tiles * splits, rows = splits > 1 ? (int64_t)w.n * a.group : 0;
-        int64_t xi = items, xr = rows;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int64_t yi = __shfl_up(xi, o, kWave);
-            if (lane >= o) xi += yi;
-        }
-        if (merge) {
-#pragma unroll
-            for (int o = 1; o < 64; o <<= 1) {
-                const int64_t yr = __shfl_up(xr, o, kWave);
-                if (lane >= o) xr += yr;
-            }
-        }
-        const int64_t mine = merge ? rows_before + xr : items_before + xi;
-        const uint64_t hit = __ballot(mine > want);
+        const int splits = w.tiles ? (w.units + per - 1) / per : 0, items = w.tiles * splits;
+        const int rows = w.n * a.group, tile_blocks = merge_rows ? p.bm / merge_rows : 0;
+        const int blocks = merge_rows && splits > 1 ? (rows + merge_rows - 1) / merge_rows : 0;
+        const int xi = scan_sum(items), xb = merge_rows ? scan_sum(blocks) : 0;
+        const uint64_t hit = __ballot((merge_rows ? blocks_before + xb : items_before + xi) > want);
         if (hit) {
             const int l = __builtin_ctzll(hit);
             auto get = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
             out->s = base + l;
             out->row0 = get(w.row0), out->n = get(w.n), out->len = get(w.len);
             out->splits = get(splits);
-            const int tiles_here = get(w.tiles);
-            const int first_item = get((int)(items_before + xi - items));
-            if (merge) {
-                out->row = (int)(want - __shfl(mine - rows, l, kWave));
-                out->tile = out->row / p.bm;
+            const int last = get(w.tiles) - 1, first_item = items_before + get(xi - items);
+            int j;  // the tile's place, the last tile first
+            if (merge_rows) {
+                const int k = want - blocks_before - get(xb - blocks);
+                out->tile = k / tile_blocks;
                 out->split = 0;
-                out->record = first_item + (tiles_here - 1 - out->tile) * out->splits;
+                out->row = k * merge_rows;
+                j = last - out->tile;
             } else {
-                const int k = (int)(want - __shfl(mine - items, l, kWave));
-                const int j = k / out->splits;
-                out->tile = tiles_here - 1 - j;
+                const int k = want - items_before - get(xi - items);
+                j = k / out->splits;
+                out->tile = last - j;
                 out->split = k - j * out->splits;
                 out->row = 0;
-                out->record = first_item + j * out->splits;
             }
+            out->record = first_item + j * out->splits;
             return true;
         }
-        items_before += __shfl(xi, 63, kWave);
-        rows_before += __shfl(xr, 63, kWave);
+        items_before += __builtin_amdgcn_readlane(xi, 63);
+        blocks_before += __builtin_amdgcn_readlane(xb, 63);
     }
     return false;
 }
@@ -301,7 +301,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(TokenShape<
     const int kvh = blockIdx.x % c.kv_heads;
     const float factor = E4M3 ? c.k_scale[kvh] * a.scale_log2 : a.scale_log2;
     Piece t;
-    for (int64_t item = blockIdx.x / c.kv_heads; find_piece(c, a, plan, false, item, &t); item += gridDim.x / c.kv_heads) {
+    for (int item = blockIdx.x / c.kv_heads; find_piece(c, a, plan, 0, item, &t); item += gridDim.x / c.kv_heads) {
         const int nr = t.n * a.group;
         const Span span = span_of(a, t, 0, nr - 1, kTokenUnit, T::kTile);
         const int lo = span.lo, hi = span.hi;
@@ -506,75 +506,6 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(TokenShape<
     }
 }
 
-// ------------------------------------------------------------------------------------------- the merge
-
-// Rows of split tiles: a workgroup takes a row's dims in blocks of kMergeDims, its threads the records in turn.
-constexpr int kMergeDims = 128;
-
-template <int D, bool E4M3>
-__global__ __launch_bounds__(256) void paged_merge_kernel(PagedView c, PagedAttentionCall a, PlanArgs plan, const float* part) {
-    constexpr int DB = D < kMergeDims ? D : kMergeDims, kBlocks = D / DB, kCols = DB / 4, kGroups = 256 / kCols;
-    __shared__ float4 ov[kGroups][kCols];
-    const int lane = threadIdx.x & 63, col = threadIdx.x % kCols, grp = threadIdx.x / kCols;
-    const int kvh = blockIdx.x % c.kv_heads;
-    Piece t;
-    for (int64_t u = blockIdx.x / c.kv_heads;; u += gridDim.x / c.kv_heads) {
-        const int64_t row = u / kBlocks;
-        const int d = (int)(u - row * kBlocks) * DB + 4 * col;
-        if (!find_piece(c, a, plan, true, row, &t)) return;
-        const int r = t.row - t.tile * plan.bm;
-        const int64_t size = record_floats(plan.bm, D);
-        const float* rec = part + ((int64_t)kvh * plan.items + t.record) * size;
-        float m = -INFINITY, l = 0.0f;
-        bool bad = false;
-        for (int j = lane; j < t.splits; j += 64) {
-            const float x = rec[j * size + r];
-            bad |= x != x;
-            m = fmaxf(m, x);
-        }
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, kWave));
-        for (int j = lane; j < t.splits; j += 64) {
-            const float x = rec[j * size + r];
-            l += x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x - m) * rec[j * size + plan.bm + r];
-        }
-        l = wave_sum(l);
-        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        const float* rv = rec + 2 * plan.bm + (int64_t)r * D + d;
-        constexpr int kAhead = 4;
-        for (int j0 = grp; j0 < t.splits; j0 += kGroups * kAhead) {
-            float f[kAhead];
-            float4 y[kAhead];
-#pragma unroll
-            for (int k = 0; k < kAhead; ++k) {
-                const int j = min(j0 + k * kGroups, t.splits - 1);
-                const float x = rec[j * size + r];
-                y[k] = *reinterpret_cast<const float4*>(rv + j * size);
-                f[k] = j0 + k * kGroups >= t.splits || x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x - m);
-            }
-#pragma unroll
-            for (int k = 0; k < kAhead; ++k)
-                if (f[k] != 0.0f) {
-                    v.x = fmaf(f[k], y[k].x, v.x), v.y = fmaf(f[k], y[k].y, v.y);
-                    v.z = fmaf(f[k], y[k].z, v.z), v.w = fmaf(f[k], y[k].w, v.w);
-                }
-        }
-        ov[grp][col] = v;
-        __syncthreads();
-        if (grp == 0 && !__any(bad)) {
-#pragma unroll
-            for (int k = 1; k < kGroups; ++k) {
-                const float4 y = ov[k][col];
-                v.x += y.x, v.y += y.y, v.z += y.z, v.w += y.w;
-            }
-            const Row x = row_of(a, t, kvh, t.row);
-            const float inv = l == 0.0f ? 0.0f : (E4M3 ? c.v_scale[kvh] : 1.0f) / l;
-            *reinterpret_cast<uint2*>(a.out + x.m * a.out_row + x.h * D + d) = make_uint2(pk_bf16(v.x * inv, v.y * inv), pk_bf16(v.z * inv, v.w * inv));
-        }
-        __syncthreads();
-    }
-}
-
 // ------------------------------------------------------------------------------------ the chunk kernel
 
 // 128 rows of a sequence (32 per wave) over the positions they see: bound by the matrix cores and LDS. K and V tiles
@@ -661,7 +592,7 @@ __global__ __launch_bounds__((ChunkShape<D, E4M3>::kThreads)) __attribute__((amd
     const int vrow = 4 * hf + (l16 >> 2);
     const int va = vrow * T::kRowBytes + ((2 * (lane >> 4 & 1) + (l16 >> 1 & 1)) ^ chunk_swizzle<D>(vrow)) * 16 + (l16 & 1) * 8;
     Piece t;
-    for (int64_t item = blockIdx.x / c.kv_heads; find_piece(c, a, plan, false, item, &t); item += gridDim.x / c.kv_heads) {
+    for (int item = blockIdx.x / c.kv_heads; find_piece(c, a, plan, 0, item, &t); item += gridDim.x / c.kv_heads) {
         const int r0 = t.tile * kChunkRows, nr = (int)min((int64_t)kChunkRows, (int64_t)t.n * a.group - r0);
         const Span span = span_of(a, t, r0, r0 + nr - 1, kChunkUnit, kTile);
         const int lo = span.lo, hi = span.hi;
@@ -935,43 +866,173 @@ __global__ __launch_bounds__((ChunkShape<D, E4M3>::kThreads)) __attribute__((amd
     }
 }
 
+// ------------------------------------------------------------------------------------------- the merge
+
+// Rows of split tiles, both kernels' in one launch. A workgroup takes kMergeRows rows of a tile: with many splits and few
+// rows (tokens) one row and 128 of its dims, its threads in groups that take the records in turn; else (chunks)
+// eight rows, a wave per row at a time, its lanes across the dims.
+constexpr int kMergeDims = 128;
+constexpr int kMergeChunkRows = 8;
+
+template <int D, bool E4M3>
+__device__ void merge_tokens(const PagedView& c, const PagedAttentionCall& a, const PlanArgs& plan, const float* part, int kvh, int first,
+                             int stride) {
+    constexpr int DB = D < kMergeDims ? D : kMergeDims, kBlocks = D / DB, kCols = DB / 4, kGroups = 256 / kCols, kAhead = 4;
+    __shared__ float4 ov[kGroups][kCols];
+    const int lane = threadIdx.x & 63, col = threadIdx.x % kCols, grp = threadIdx.x / kCols;
+    const int64_t size = record_floats(kTokenRows, D);
+    Piece t;
+    for (int u = first; find_piece(c, a, plan, 1, u / kBlocks, &t); u += stride) {
+        const int d = u % kBlocks * DB + 4 * col, r = t.row;  // one tile a sequence
+        const float* rec = part + ((int64_t)kvh * plan.items + t.record) * size;
+        float m = -INFINITY, l = 0.0f;
+        bool bad = false;
+        for (int j = lane; j < t.splits; j += 64) {
+            const float x = rec[j * size + r];
+            bad |= x != x;
+            m = fmaxf(m, x);
+        }
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, kWave));
+        for (int j = lane; j < t.splits; j += 64) {
+            const float x = rec[j * size + r];
+            l += x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x - m) * rec[j * size + kTokenRows + r];
+        }
+        l = wave_sum(l);
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        const float* rv = rec + 2 * kTokenRows + r * D + d;
+        for (int j0 = grp; j0 < t.splits; j0 += kGroups * kAhead) {
+            float f[kAhead];
+            float4 y[kAhead];
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) {
+                const int j = min(j0 + k * kGroups, t.splits - 1);
+                const float x = rec[j * size + r];
+                y[k] = *reinterpret_cast<const float4*>(rv + j * size);
+                f[k] = j0 + k * kGroups >= t.splits || x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x - m);
+            }
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k)
+                if (f[k] != 0.0f) {
+                    v.x = fmaf(f[k], y[k].x, v.x), v.y = fmaf(f[k], y[k].y, v.y);
+                    v.z = fmaf(f[k], y[k].z, v.z), v.w = fmaf(f[k], y[k].w, v.w);
+                }
+        }
+        ov[grp][col] = v;
+        __syncthreads();
+        if (grp == 0 && !__any(bad)) {
+#pragma unroll
+            for (int k = 1; k < kGroups; ++k) {
+                const float4 y = ov[k][col];
+                v.x += y.x, v.y += y.y, v.z += y.z, v.w += y.w;
+            }
+            const Row x = row_of(a, t, kvh, r);
+            const float inv = l == 0.0f ? 0.0f : (E4M3 ? c.v_scale[kvh] : 1.0f) / l;
+            *reinterpret_cast<uint2*>(a.out + x.m * a.out_row + x.h * D + d) = make_uint2(pk_bf16(v.x * inv, v.y * inv), pk_bf16(v.z * inv, v.w * inv));
+        }
+        __syncthreads();
+    }
+}
+
+template <int D, bool E4M3>
+__device__ void merge_chunks(const PagedView& c, const PagedAttentionCall& a, const PlanArgs& plan, const float* part, int kvh, int first,
+                             int stride) {
+    constexpr int kPer = D / 64;  // dims of a lane
+    const int lane = threadIdx.x & 63;
+    const int64_t size = record_floats(kChunkRows, D);
+    Piece t;
+    for (int u = first; find_piece(c, a, plan, kMergeChunkRows, u, &t); u += stride) {
+        const float* rec = part + ((int64_t)kvh * plan.items + t.record) * size;
+        const int r0 = t.row - t.tile * kChunkRows, rows = min(kMergeChunkRows, t.n * a.group - t.row);
+#pragma unroll 2
+        for (int i = threadIdx.x >> 6; i < rows; i += 4) {
+            const int r = r0 + i;
+            float m = -INFINITY, l = 0.0f, v[kPer] = {};
+            bool bad = false;
+            for (int j = 0; j < t.splits; ++j) {
+                const float x = rec[j * size + r];
+                bad |= x != x;
+                m = fmaxf(m, x);
+            }
+            for (int j = 0; j < t.splits; ++j) {
+                const float x = rec[j * size + r], y = rec[j * size + kChunkRows + r];
+                const float* o = rec + j * size + 2 * kChunkRows + r * D + lane * kPer;
+                float w[kPer];
+#pragma unroll
+                for (int k = 0; k < kPer; ++k) w[k] = o[k];
+                const float f = x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x - m);
+                if (f == 0.0f) continue;  // its sums may be anything
+                l = fmaf(f, y, l);
+#pragma unroll
+                for (int k = 0; k < kPer; ++k) v[k] = fmaf(f, w[k], v[k]);
+            }
+            if (bad) continue;
+            const Row x = row_of(a, t, kvh, t.row + i);
+            const float inv = l == 0.0f ? 0.0f : (E4M3 ? c.v_scale[kvh] : 1.0f) / l;
+            uint16_t* to = a.out + x.m * a.out_row + x.h * D + lane * kPer;
+            if constexpr (kPer == 1) {
+                *to = (uint16_t)f2bf(v[0] * inv);
+            } else {
+#pragma unroll
+                for (int k = 0; k < kPer; k += 2) reinterpret_cast<uint32_t*>(to)[k / 2] = pk_bf16(v[k] * inv, v[k + 1] * inv);
+            }
+        }
+    }
+}
+
+// The first token_groups workgroups of a KV head merge tokens, the others chunks.
+template <int D, bool E4M3>
+__global__ __launch_bounds__(256) void paged_merge_kernel(PagedView c, PagedAttentionCall a, PlanArgs tokens, PlanArgs chunks, int token_groups,
+                                                          const float* token_part, const float* chunk_part) {
+    const int kvh = blockIdx.x % c.kv_heads, g = blockIdx.x / c.kv_heads, groups = gridDim.x / c.kv_heads;
+    if (g < token_groups) merge_tokens<D, E4M3>(c, a, tokens, token_part, kvh, g, token_groups);
+    else merge_chunks<D, E4M3>(c, a, chunks, chunk_part, kvh, g - token_groups, groups - token_groups);
+}
+
 int64_t clamp64(int64_t v, int64_t lo, int64_t hi) { return v < lo ? lo : (v > hi ? hi : v); }
 
 template <int D, bool E4M3>
 hipError_t launch(const PagedView& c, const PagedAttentionCall& a, hipStream_t s, DevCtx* ctx) {
     using T = TokenShape<D, E4M3>;
+    const int heads = c.kv_heads;
+    const bool chunks_too = (int64_t)a.max_rows * a.group > kTokenRows;
     const int64_t capacity = (int64_t)c.columns * c.slots;
-    // token kernel: about four items per workgroup that the device holds, and one more for every sequence
-    const int resident = ctx->cus * T::kWavesPerSimd;
-    const int64_t records = (int64_t)kPagedPartFloats / (kTokenRows * (2 + D)) / c.kv_heads;
-    const PlanArgs plan{kTokenRows, kTokenUnit, (int)clamp64(4 * (int64_t)resident / c.kv_heads + c.sequences, 1, records), 1, true};
-    const int64_t most_units = (a.window ? std::min<int64_t>(capacity, (int64_t)a.window + a.max_rows + kTokenUnit) : capacity) / kTokenUnit + 1;
-    const int64_t items = std::min<int64_t>(plan.items, c.sequences * most_units);
-    hipLaunchKernelGGL((paged_token_kernel<D, E4M3>), dim3((uint32_t)(items * c.kv_heads)), dim3(256), 0, s, c, a, plan, ctx->paged_part);
+    // Records of both kernels, which one merge reads: the chunk kernel's behind the token kernel's.
+    const int64_t floats = chunks_too ? kPagedPartFloats / 2 : kPagedPartFloats;
+    // Tokens: about four items per workgroup that the device holds, and one more for every sequence. Beside chunks the grid is
+    // one round: a call without short sequences then loses little.
+    const int64_t resident = (int64_t)ctx->cus * T::kWavesPerSimd;
+    const PlanArgs tokens{kTokenRows, kTokenUnit, (int)clamp64(4 * resident / heads + c.sequences, 1, floats / record_floats(kTokenRows, D) / heads),
+                          1, true};
+    const int64_t units = (a.window ? std::min<int64_t>(capacity, (int64_t)a.window + a.max_rows + kTokenUnit) : capacity) / kTokenUnit + 1;
+    const int64_t items = std::min<int64_t>({(int64_t)tokens.items, c.sequences * units, chunks_too ? std::max<int64_t>(1, resident / heads) : tokens.items});
+    hipLaunchKernelGGL((paged_token_kernel<D, E4M3>), dim3((uint32_t)(items * heads)), dim3(256), 0, s, c, a, tokens, ctx->paged_part);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    if (most_units > 1) {
-        const int64_t rows = std::min<int64_t>((int64_t)a.rows * a.group, (int64_t)c.sequences * kTokenRows) * ((D + kMergeDims - 1) / kMergeDims);
-        hipLaunchKernelGGL((paged_merge_kernel<D, E4M3>), dim3((uint32_t)(std::min<int64_t>(rows, std::max(1, 2048 / c.kv_heads)) * c.kv_heads)),
-                           dim3(256), 0, s, c, a, plan, ctx->paged_part);
+    // rows of split tiles to merge, tokens': at most
+    int64_t merge_tokens = units > 1 ? std::min<int64_t>((int64_t)a.rows * a.group, (int64_t)c.sequences * kTokenRows) * std::max(1, D / kMergeDims) : 0;
+    merge_tokens = std::min<int64_t>(merge_tokens, std::max(1, (chunks_too ? 512 : 2048) / heads));
+    int64_t merge_chunks = 0;
+    PlanArgs chunks{};
+    float* chunk_part = ctx->paged_part + kPagedPartFloats / 2;
+    if (chunks_too) {
+        // about two items per workgroup that the device holds
+        const int64_t held = 2 * (int64_t)ctx->cus * ChunkShape<D, E4M3>::kHeld / heads;
+        chunks = {kChunkRows, kChunkUnit, (int)clamp64(held, 1, (int64_t)(kPagedPartFloats / 2) / record_floats(kChunkRows, D) / heads), kChunkMinUnits,
+                  false};
+        const int64_t tiles = (int64_t)a.rows * a.group / kChunkRows + std::min(c.sequences, a.rows);
+        const int64_t grid = std::max<int64_t>(chunks.items, std::min<int64_t>(tiles, std::max(1, 65536 / heads)));
+        hipLaunchKernelGGL((paged_chunk_kernel<D, E4M3>), dim3((uint32_t)(grid * heads)), dim3(ChunkShape<D, E4M3>::kThreads), 0, s, c, a, chunks,
+                           chunk_part);
         e = hipGetLastError();
         if (e != hipSuccess) return e;
+        // a tile that is split has at least one other item: no more split tiles than items / 2
+        merge_chunks = std::min<int64_t>((int64_t)chunks.items / 2 * (kChunkRows / kMergeChunkRows), std::max(1, 2048 / heads));
     }
-    if ((int64_t)a.max_rows * a.group <= kTokenRows) return e;
-    // chunk kernel: about two items per workgroup that the device holds
-    const int64_t held = 2 * (int64_t)ctx->cus * ChunkShape<D, E4M3>::kHeld / c.kv_heads;
-    const PlanArgs chunks{kChunkRows, kChunkUnit, (int)clamp64(held, 1, (int64_t)kPagedPartFloats / record_floats(kChunkRows, D) / c.kv_heads),
-                          kChunkMinUnits, false};
-    const int64_t tiles = (int64_t)a.rows * a.group / kChunkRows + std::min(c.sequences, a.rows);
-    const int64_t grid = std::max<int64_t>(chunks.items, std::min<int64_t>(tiles, 65536 / c.kv_heads));
-    hipLaunchKernelGGL((paged_chunk_kernel<D, E4M3>), dim3((uint32_t)(grid * c.kv_heads)), dim3(ChunkShape<D, E4M3>::kThreads), 0, s, c, a, chunks, ctx->paged_part);
-    e = hipGetLastError();
-    if (e != hipSuccess) return e;
-    const int64_t rows = (int64_t)a.rows * a.group * ((D + kMergeDims - 1) / kMergeDims);
-    hipLaunchKernelGGL((paged_merge_kernel<D, E4M3>), dim3((uint32_t)(std::min<int64_t>(rows, std::max(1, 2048 / c.kv_heads)) * c.kv_heads)),
-                       dim3(256), 0, s, c, a, chunks, ctx->paged_part);
-    e = hipGetLastError();
-    return e;
+    if (merge_tokens + merge_chunks == 0) return e;
+    hipLaunchKernelGGL((paged_merge_kernel<D, E4M3>), dim3((uint32_t)((merge_tokens + merge_chunks) * heads)), dim3(256), 0, s, c, a, tokens, chunks,
+                       (int)merge_tokens, ctx->paged_part, chunk_part);
+    return hipGetLastError();
 }
 
 template <int D>
