@@ -18,6 +18,8 @@ struct PagedView {
     int64_t table_stride;
     uint32_t slots, magic, shift;         // t / slots = t * magic >> shift, for t < 2^31
     int32_t layers, pages, kv_heads, head_dim, sequences, columns;
+    bool near;                            // every offset within a layer's K, and V, is below 2^32 bytes
+    bool alike;                           // K's and V's pages and slots have the same strides
     uint32_t* err;
 };
 

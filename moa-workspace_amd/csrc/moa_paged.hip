@@ -470,6 +470,11 @@ int cache_view(const moa_paged_cache* c, int layer, PagedView* v) {
     v->magic = (uint32_t)((uint64_t(1) << v->shift) / (uint32_t)c->slots + 1);
     v->layers = c->layers, v->pages = c->pages, v->kv_heads = c->kv_heads, v->head_dim = c->head_dim;
     v->sequences = c->sequences, v->columns = c->columns;
+    auto reach = [&](const int64_t* st) {  // bytes from the first element of a layer to behind its last
+        return ((c->pages - 1) * st[1] + (c->slots - 1) * st[2] + (c->kv_heads - 1) * st[3] + c->head_dim) * b;
+    };
+    v->near = reach(c->k_stride) < (int64_t(1) << 32) && reach(c->v_stride) < (int64_t(1) << 32);
+    v->alike = v->k_page == v->v_page && v->k_slot == v->v_slot;
     v->err = nullptr;
     return MOA_SUCCESS;
 }

@@ -528,8 +528,10 @@ struct ChunkShape {
     static constexpr int kHeld = D == 512 ? 1 : 2;              // workgroups on a CU: two waves per SIMD
     static constexpr int kRowBytes = 2 * D;                     // LDS row of a position
     static constexpr int kRowsPerLoad = 1024 / kRowBytes;       // positions a wave's load into LDS covers
-    static constexpr int kLoads = kTile / (4 * kPair) / kRowsPerLoad;     // loads of K (and of V) per wave and tile
+    static constexpr int kWaveRows = kTile / (4 * kPair);       // positions of a tile that a wave loads
+    static constexpr int kLoads = kWaveRows / kRowsPerLoad;     // loads of K (and of V) per wave and tile
     static constexpr int kCodeLoads = kTile * D / 16 / kThreads;     // E4M3: 16-byte loads of K (and V) per thread and tile
+    static constexpr int kGroup = 64 / kWaveRows;               // tiles whose positions a wave's lanes look up at once
 };
 constexpr int kChunkUnit = 64;      // positions that a split is a multiple of
 constexpr int kChunkMinUnits = 4;   // and the fewest of them
@@ -548,9 +550,13 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
 // 16 bytes per lane from global memory into LDS, lane l's at lds + 16 l. In asm, since the compiler would let no LDS read
-// pass before all such loads are done; `ready` waits for them. (One wait state between the write of m0 and its use.)
+// pass before all such loads are done; `ready` waits for them. (One wait state between the
+// write of m0 and its use, five between a vector instruction's write of a scalar register and its use.)
 __device__ __forceinline__ void load_to_lds(const void* from, uint32_t lds) {
     __asm__ volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "{m0}"(lds) : "memory");
+}
+__device__ __forceinline__ void load_to_lds(const void* base, uint32_t offset, uint32_t lds) {
+    __asm__ volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(base), "{m0}"(lds) : "memory");
 }
 
 // v, opaque to the compiler: what is computed from it in a loop is not kept in registers across the loop.
@@ -587,7 +593,7 @@ __global__ __launch_bounds__((ChunkShape<D, E4M3>::kThreads)) __attribute__((amd
     const float signed_factor = E4M3 ? c.k_scale[kvh] * a.scale_log2 : a.scale_log2;
     const float factor = fmaxf(fabsf(signed_factor), 1.2e-38f);
     const uint32_t flip = signed_factor < 0.0f ? 0x80008000u : 0u;
-    // LDS byte addresses: K rows l32, chunk 2 s + hf; V's transposing reads (see read_v8), dim tile 0
+    // LDS byte addresses: K rows l32, chunk 2 s + hf; V's transposing reads, dim tile 0
     const int ka = l32 * T::kRowBytes + (hf ^ chunk_swizzle<D>(l32)) * 16;
     const int vrow = 4 * hf + (l16 >> 2);
     const int va = vrow * T::kRowBytes + ((2 * (lane >> 4 & 1) + (l16 >> 1 & 1)) ^ chunk_swizzle<D>(vrow)) * 16 + (l16 & 1) * 8;
@@ -629,11 +635,13 @@ __global__ __launch_bounds__((ChunkShape<D, E4M3>::kThreads)) __attribute__((amd
 
         const int32_t* table = c.table + t.s * c.table_stride;
         const uint8_t *kbase = c.k + kvh * c.k_head, *vbase = c.v + kvh * c.v_head;
-        // lane l looks after position t0 + l % kTile, its page a tile ahead of its use
-        auto page_at = [&](int t0) { return t0 < hi ? table[page_of(c, min(t0 + lane % kTile, hi - 1))] : 0; };
+        // Lane l looks after position l % kWaveRows of the wave's part of tile l / kWaveRows, kGroup tiles at once; the next
+        // group's pages are asked for a group ahead.
+        const int own = lane / T::kWaveRows * kTile + wave * T::kWaveRows + lane % T::kWaveRows;
+        auto page_at = [&](int t0) { return t0 < hi ? table[page_of(c, min(t0 + own, hi - 1))] : 0; };
         int64_t koff = 0, voff = 0;
         auto place = [&](int page, int t0) {
-            const int p = min(t0 + lane % kTile, hi - 1);
+            const int p = min(t0 + own, hi - 1);
             const bool in = page >= 0 && page < c.pages;
             bad |= !in;
             page = in ? page : 0;
@@ -641,38 +649,49 @@ __global__ __launch_bounds__((ChunkShape<D, E4M3>::kThreads)) __attribute__((amd
             koff = page * c.k_page + slot * c.k_slot;
             voff = page * c.v_page + slot * c.v_slot;
         };
-        auto load_tile = [&](uint32_t tile) {  // bf16: this wave's quarter of the tile, straight into LDS
-            const int ln = in_loop(lane);
+        // bf16: the wave's part of tile `ti` of the group, straight into LDS
+        auto load_tile = [&](uint32_t tile, int ti) __attribute__((always_inline)) {
+            constexpr int kLanes = 64 / T::kRowsPerLoad;  // lanes of a row
+            const int ln = in_loop(lane), from = ti * T::kWaveRows + ln / kLanes;
 #pragma unroll
             for (int i = 0; i < T::kLoads; ++i) {
-                const int row = wave * (kTile / kWaves) + i * T::kRowsPerLoad, mr = row + ln / (64 / T::kRowsPerLoad);
-                const int at = ((ln % (64 / T::kRowsPerLoad)) ^ chunk_swizzle<D>(mr)) * 16;
-                load_to_lds(kbase + __shfl(koff, mr, kWave) + at, tile + row * T::kRowBytes);
-                load_to_lds(vbase + __shfl(voff, mr, kWave) + at, tile + kTileBytes + row * T::kRowBytes);
+                const int row = wave * T::kWaveRows + i * T::kRowsPerLoad;
+                const int at = ((ln % kLanes) ^ chunk_swizzle<D>(row + ln / kLanes)) * 16, src = from + i * T::kRowsPerLoad;
+                const uint32_t kd = tile + row * T::kRowBytes, vd = kd + kTileBytes;
+                if (c.near) {
+                    const uint32_t ko = (uint32_t)__shfl((int)koff, src, kWave);
+                    const uint32_t vo = c.alike ? ko : (uint32_t)__shfl((int)voff, src, kWave);
+                    load_to_lds(kbase, ko + at, kd);
+                    load_to_lds(vbase, vo + at, vd);
+                } else {
+                    load_to_lds(kbase + __shfl(koff, src, kWave) + at, kd);
+                    load_to_lds(vbase + __shfl(voff, src, kWave) + at, vd);
+                }
             }
         };
-        // E4M3: thread i takes 16 codes a load, D / 16 threads a row
+        // E4M3: the same positions' codes into registers, 16 a load, and from there into LDS as bf16
+        constexpr int kCodeLanes = D / 16;
         uint4 kc[T::kCodeLoads], vc[T::kCodeLoads];
-        auto load_codes = [&] {
-            const int tid = in_loop(threadIdx.x);
+        auto load_codes = [&](int ti) __attribute__((always_inline)) {
+            const int ln = in_loop(lane);
 #pragma unroll
             for (int j = 0; j < T::kCodeLoads; ++j) {
-                const int x = T::kThreads * j + tid, row = x / (D / 16), at = x % (D / 16) * 16;
-                kc[j] = ld16(kbase + __shfl(koff, row, kWave) + at);
-                vc[j] = ld16(vbase + __shfl(voff, row, kWave) + at);
+                const int src = ti * T::kWaveRows + j * (64 / kCodeLanes) + ln / kCodeLanes, at = ln % kCodeLanes * 16;
+                kc[j] = ld16(kbase + __shfl(koff, src, kWave) + at);
+                vc[j] = ld16(vbase + __shfl(voff, src, kWave) + at);
             }
         };
-        auto store_codes = [&](uint8_t* kd) {
+        auto store_codes = [&](uint8_t* kd) __attribute__((always_inline)) {
             auto put = [&](uint8_t* d, const uint4& w, int row, int col) {
                 const uint4 lo8 = make_uint4(bf16_pair_of_fp8(w.x), bf16_pair_of_fp8(w.x >> 16), bf16_pair_of_fp8(w.y), bf16_pair_of_fp8(w.y >> 16));
                 const uint4 hi8 = make_uint4(bf16_pair_of_fp8(w.z), bf16_pair_of_fp8(w.z >> 16), bf16_pair_of_fp8(w.w), bf16_pair_of_fp8(w.w >> 16));
                 *reinterpret_cast<uint4*>(d + row * T::kRowBytes + ((2 * col) ^ chunk_swizzle<D>(row)) * 16) = lo8;
                 *reinterpret_cast<uint4*>(d + row * T::kRowBytes + ((2 * col + 1) ^ chunk_swizzle<D>(row)) * 16) = hi8;
             };
-            const int tid = in_loop(threadIdx.x);
+            const int ln = in_loop(lane);
 #pragma unroll
             for (int j = 0; j < T::kCodeLoads; ++j) {
-                const int x = T::kThreads * j + tid, row = x / (D / 16), col = x % (D / 16);
+                const int row = wave * T::kWaveRows + j * (64 / kCodeLanes) + ln / kCodeLanes, col = ln % kCodeLanes;
                 put(kd, kc[j], row, col);
                 put(kd + kTileBytes, vc[j], row, col);
             }
@@ -802,15 +821,16 @@ __global__ __launch_bounds__((ChunkShape<D, E4M3>::kThreads)) __attribute__((amd
 
         __syncthreads();  // the item before has read its last tile
         const uint32_t lds = (uint32_t)(uintptr_t)(lds_void*)tiles;
-        int page = 0;
+        constexpr int kGroupStep = T::kGroup * kTile;
+        int page = 0, ti = 0;  // the next group's pages; the tile's place in its group
         if (lo < hi) {
             place(page_at(lo), lo);
-            page = page_at(lo + kTile);
+            page = page_at(lo + kGroupStep);
             if constexpr (E4M3) {
-                load_codes();
+                load_codes(0);
                 store_codes(tiles);
             } else {
-                load_tile(lds);
+                load_tile(lds, 0);
             }
         }
         uint32_t at = 0;  // the buffer in use
@@ -819,10 +839,13 @@ __global__ __launch_bounds__((ChunkShape<D, E4M3>::kThreads)) __attribute__((amd
             const uint32_t next = at ^ (2 * kTileBytes);
             const bool more = t0 + kTile < hi;
             if (more) {
-                place(page, t0 + kTile);
-                page = page_at(t0 + 2 * kTile);
-                if constexpr (E4M3) load_codes();
-                else load_tile(lds + next);
+                if (++ti == T::kGroup) {
+                    ti = 0;
+                    place(page, t0 + kTile);
+                    page = page_at(t0 + kTile + kGroupStep);
+                }
+                if constexpr (E4M3) load_codes(ti);
+                else load_tile(lds + next, ti);
             }
             compute(at, t0);
             if (E4M3 && more) store_codes(tiles + next);
