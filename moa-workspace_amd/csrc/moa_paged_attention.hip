@@ -32,9 +32,12 @@ __device__ __forceinline__ bf16x8 as_bf16x8(const uint4& v) { return __builtin_b
 // How a call's sequences are split into items, the same in every kernel of the call. A sequence of r = n * group rows has
 // ceil(r / bm) tiles, each split over ceil(units / c) items, where units covers the positions a tile can see in steps of
 // `unit`, and c, at least min_units, is chosen so that all sequences together have at most `items` items per KV head (a
-// call with more tiles than that splits none). The last tiles of a sequence, which see the most, come first.
+// call with `enough` tiles splits none). The last tiles of a sequence, which see the most, come first.
 struct PlanArgs {
     int bm, unit, items, min_units;
+    int enough;   // with this many tiles or more, none is split
+    int most;     // no call has more items than this
+    int most_blocks;  // nor more blocks of rows to merge
     bool tokens;  // the token kernel's sequences (at most kTokenRows rows) or the others
 };
 
@@ -101,7 +104,7 @@ __device__ bool find_piece(const PagedView& c, const PagedAttentionCall& a, cons
     // short by at most 1024 + 8 roundings of 2^-24: a part in ten thousand more covers them.
     units = wave_sum(units);
     int per = 1 << 30;
-    if (tiles < p.items) per = max(p.min_units, (int)fminf(units * 1.0001f / (float)(p.items - tiles) + 1.0f, 1e9f));
+    if (tiles < p.enough) per = max(p.min_units, (int)fminf(units * 1.0001f / (float)(p.items - tiles) + 1.0f, 1e9f));
     int items_before = 0, blocks_before = 0;
     for (int base = 0; base < c.sequences; base += 64) {
         if (c.sequences > 64) w = seq_work(c, a, p, base + lane, &bad);
@@ -301,7 +304,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(TokenShape<
     const int kvh = blockIdx.x % c.kv_heads;
     const float factor = E4M3 ? c.k_scale[kvh] * a.scale_log2 : a.scale_log2;
     Piece t;
-    for (int item = blockIdx.x / c.kv_heads; find_piece(c, a, plan, 0, item, &t); item += gridDim.x / c.kv_heads) {
+    for (int item = blockIdx.x / c.kv_heads; item < plan.most && find_piece(c, a, plan, 0, item, &t); item += gridDim.x / c.kv_heads) {
         const int nr = t.n * a.group;
         const Span span = span_of(a, t, 0, nr - 1, kTokenUnit, T::kTile);
         const int lo = span.lo, hi = span.hi;
@@ -564,6 +567,13 @@ __device__ __forceinline__ int in_loop(int v) {
     __asm__ volatile("" : "+v"(v));
     return v;
 }
+// The lane, computed where it is used: registers that the chunk kernel's loop reloaded from scratch memory would wait for every
+// load into LDS before them (512 dims, 1000 rows over 15800 positions: 758 us with three such reloads a tile, 734 without).
+__device__ __forceinline__ int lane_here() {
+    int v;
+    __asm__ volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(v));
+    return v;
+}
 
 template <int D, bool E4M3>
 __global__ __launch_bounds__((ChunkShape<D, E4M3>::kThreads)) __attribute__((amdgpu_waves_per_eu(2))) void paged_chunk_kernel(
@@ -585,7 +595,7 @@ __global__ __launch_bounds__((ChunkShape<D, E4M3>::kThreads)) __attribute__((amd
         return r != 0;
     };
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int l32 = lane & 31, hf = lane >> 5, l16 = lane & 15;
+    const int l32 = lane & 31, hf = lane >> 5;
     const int rg = wave & 3, half = wave >> 2;  // rows 32 rg .., dims half * kMine ..
     const int kvh = blockIdx.x % c.kv_heads;
     // x = factor (q . k): a negative factor's sign goes to q, so that the largest product is the largest x; and a factor of
@@ -593,12 +603,17 @@ __global__ __launch_bounds__((ChunkShape<D, E4M3>::kThreads)) __attribute__((amd
     const float signed_factor = E4M3 ? c.k_scale[kvh] * a.scale_log2 : a.scale_log2;
     const float factor = fmaxf(fabsf(signed_factor), 1.2e-38f);
     const uint32_t flip = signed_factor < 0.0f ? 0x80008000u : 0u;
-    // LDS byte addresses: K rows l32, chunk 2 s + hf; V's transposing reads, dim tile 0
-    const int ka = l32 * T::kRowBytes + (hf ^ chunk_swizzle<D>(l32)) * 16;
-    const int vrow = 4 * hf + (l16 >> 2);
-    const int va = vrow * T::kRowBytes + ((2 * (lane >> 4 & 1) + (l16 >> 1 & 1)) ^ chunk_swizzle<D>(vrow)) * 16 + (l16 & 1) * 8;
+    // LDS byte addresses of a lane: K rows lane % 32, chunk 2 s + lane / 32; V's transposing reads, dim tile 0
+    auto k_address = [&] {
+        const int ln = lane_here(), r = ln & 31;
+        return r * T::kRowBytes + ((ln >> 5) ^ chunk_swizzle<D>(r)) * 16;
+    };
+    auto v_address = [&] {
+        const int ln = lane_here(), r = 4 * (ln >> 5) + (ln >> 2 & 3);
+        return r * T::kRowBytes + ((2 * (ln >> 4 & 1) + (ln >> 1 & 1)) ^ chunk_swizzle<D>(r)) * 16 + (ln & 1) * 8;
+    };
     Piece t;
-    for (int item = blockIdx.x / c.kv_heads; find_piece(c, a, plan, 0, item, &t); item += gridDim.x / c.kv_heads) {
+    for (int item = blockIdx.x / c.kv_heads; item < plan.most && find_piece(c, a, plan, 0, item, &t); item += gridDim.x / c.kv_heads) {
         const int r0 = t.tile * kChunkRows, nr = (int)min((int64_t)kChunkRows, (int64_t)t.n * a.group - r0);
         const Span span = span_of(a, t, r0, r0 + nr - 1, kChunkUnit, kTile);
         const int lo = span.lo, hi = span.hi;
@@ -652,7 +667,7 @@ __global__ __launch_bounds__((ChunkShape<D, E4M3>::kThreads)) __attribute__((amd
         // bf16: the wave's part of tile `ti` of the group, straight into LDS
         auto load_tile = [&](uint32_t tile, int ti) __attribute__((always_inline)) {
             constexpr int kLanes = 64 / T::kRowsPerLoad;  // lanes of a row
-            const int ln = in_loop(lane), from = ti * T::kWaveRows + ln / kLanes;
+            const int ln = lane_here(), from = ti * T::kWaveRows + ln / kLanes;
 #pragma unroll
             for (int i = 0; i < T::kLoads; ++i) {
                 const int row = wave * T::kWaveRows + i * T::kRowsPerLoad;
@@ -673,7 +688,7 @@ __global__ __launch_bounds__((ChunkShape<D, E4M3>::kThreads)) __attribute__((amd
         constexpr int kCodeLanes = D / 16;
         uint4 kc[T::kCodeLoads], vc[T::kCodeLoads];
         auto load_codes = [&](int ti) __attribute__((always_inline)) {
-            const int ln = in_loop(lane);
+            const int ln = lane_here();
 #pragma unroll
             for (int j = 0; j < T::kCodeLoads; ++j) {
                 const int src = ti * T::kWaveRows + j * (64 / kCodeLanes) + ln / kCodeLanes, at = ln % kCodeLanes * 16;
@@ -688,7 +703,7 @@ __global__ __launch_bounds__((ChunkShape<D, E4M3>::kThreads)) __attribute__((amd
                 *reinterpret_cast<uint4*>(d + row * T::kRowBytes + ((2 * col) ^ chunk_swizzle<D>(row)) * 16) = lo8;
                 *reinterpret_cast<uint4*>(d + row * T::kRowBytes + ((2 * col + 1) ^ chunk_swizzle<D>(row)) * 16) = hi8;
             };
-            const int ln = in_loop(lane);
+            const int ln = lane_here();
 #pragma unroll
             for (int j = 0; j < T::kCodeLoads; ++j) {
                 const int row = wave * T::kWaveRows + j * (64 / kCodeLanes) + ln / kCodeLanes, col = ln % kCodeLanes;
@@ -709,7 +724,7 @@ __global__ __launch_bounds__((ChunkShape<D, E4M3>::kThreads)) __attribute__((amd
             {
                 constexpr int kAhead = T::kSub == 2 ? 2 : 3;
                 const uint8_t* kt = tiles + tile + half * kMine * 2;
-                const int kx = in_loop(ka);
+                const int kx = k_address();
                 bf16x8 kf[kAhead][T::kSub];
                 auto read_k = [&](int s) __attribute__((always_inline)) {
 #pragma unroll
@@ -728,16 +743,17 @@ __global__ __launch_bounds__((ChunkShape<D, E4M3>::kThreads)) __attribute__((amd
                 }
             }
             if constexpr (kPair == 2) {
+                const int ln = lane_here();
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    xs[(wave * 4 + e) * 64 + lane] = make_float4(sc[0][4 * e], sc[0][4 * e + 1], sc[0][4 * e + 2], sc[0][4 * e + 3]);
+                    xs[(wave * 4 + e) * 64 + ln] = make_float4(sc[0][4 * e], sc[0][4 * e + 1], sc[0][4 * e + 2], sc[0][4 * e + 3]);
                 __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
                 __builtin_amdgcn_s_barrier();
                 __asm__ volatile("" ::: "memory");
                 if (!sees) return;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const float4 y = xs[((wave ^ 4) * 4 + e) * 64 + lane];
+                    const float4 y = xs[((wave ^ 4) * 4 + e) * 64 + ln];
                     sc[0][4 * e] += y.x, sc[0][4 * e + 1] += y.y, sc[0][4 * e + 2] += y.z, sc[0][4 * e + 3] += y.w;
                 }
             }
@@ -786,7 +802,7 @@ __global__ __launch_bounds__((ChunkShape<D, E4M3>::kThreads)) __attribute__((amd
             {
                 constexpr int kAhead = 2, kN = T::kSub * kDims;  // step n: 32 positions n / kDims, dim tile n % kDims
                 uint8_t* vt = tiles + tile + kTileBytes + half * kMine * 2;
-                const int vx = in_loop(va);
+                const int vx = v_address();
                 s16x4 vr[kAhead][4];
                 auto read_v = [&](int n) __attribute__((always_inline)) {
                     const int d = n % kDims, b = n / kDims;
@@ -905,7 +921,7 @@ __device__ void merge_tokens(const PagedView& c, const PagedAttentionCall& a, co
     const int lane = threadIdx.x & 63, col = threadIdx.x % kCols, grp = threadIdx.x / kCols;
     const int64_t size = record_floats(kTokenRows, D);
     Piece t;
-    for (int u = first; find_piece(c, a, plan, 1, u / kBlocks, &t); u += stride) {
+    for (int u = first; u < plan.most_blocks * kBlocks && find_piece(c, a, plan, 1, u / kBlocks, &t); u += stride) {
         const int d = u % kBlocks * DB + 4 * col, r = t.row;  // one tile a sequence
         const float* rec = part + ((int64_t)kvh * plan.items + t.record) * size;
         float m = -INFINITY, l = 0.0f;
@@ -964,7 +980,7 @@ __device__ void merge_chunks(const PagedView& c, const PagedAttentionCall& a, co
     const int lane = threadIdx.x & 63;
     const int64_t size = record_floats(kChunkRows, D);
     Piece t;
-    for (int u = first; find_piece(c, a, plan, kMergeChunkRows, u, &t); u += stride) {
+    for (int u = first; u < plan.most_blocks && find_piece(c, a, plan, kMergeChunkRows, u, &t); u += stride) {
         const float* rec = part + ((int64_t)kvh * plan.items + t.record) * size;
         const int r0 = t.row - t.tile * kChunkRows, rows = min(kMergeChunkRows, t.n * a.group - t.row);
 #pragma unroll 2
@@ -1022,35 +1038,42 @@ hipError_t launch(const PagedView& c, const PagedAttentionCall& a, hipStream_t s
     const int64_t capacity = (int64_t)c.columns * c.slots;
     // Records of both kernels, which one merge reads: the chunk kernel's behind the token kernel's.
     const int64_t floats = chunks_too ? kPagedPartFloats / 2 : kPagedPartFloats;
-    // Tokens: about four items per workgroup that the device holds, and one more for every sequence. Beside chunks the grid is
-    // one round: a call without short sequences then loses little.
+    // Tokens: about four items per CU, and one more for every sequence: fewer leave CUs without work behind the longest (48 ragged
+    // sequences of 16 x 512: 381 us with two, 353), more cost records and starts (64 of 32 x 128, E4M3: 203 us with twelve, 192
+    // with six). Beside chunks the grid is one round: a call without short sequences then loses little.
     const int64_t resident = (int64_t)ctx->cus * T::kWavesPerSimd;
-    const PlanArgs tokens{kTokenRows, kTokenUnit, (int)clamp64(4 * resident / heads + c.sequences, 1, floats / record_floats(kTokenRows, D) / heads),
-                          1, true};
+    PlanArgs tokens{kTokenRows, kTokenUnit, (int)clamp64(4 * ctx->cus / heads + c.sequences, 1, floats / record_floats(kTokenRows, D) / heads),
+                    1, 0, 0, 0, true};
+    tokens.enough = tokens.items;
     const int64_t units = (a.window ? std::min<int64_t>(capacity, (int64_t)a.window + a.max_rows + kTokenUnit) : capacity) / kTokenUnit + 1;
-    const int64_t items = std::min<int64_t>({(int64_t)tokens.items, c.sequences * units, chunks_too ? std::max<int64_t>(1, resident / heads) : tokens.items});
+    const int64_t sequences = std::min(c.sequences, a.rows);  // with rows
+    // unsplit, an item a sequence; split, within the plan's items
+    tokens.most = (int)std::min<int64_t>(sequences * units, std::max<int64_t>(tokens.items, sequences));
+    tokens.most_blocks = (int)(units > 1 ? std::min<int64_t>((int64_t)a.rows * a.group, sequences * kTokenRows) : 0);
+    const int64_t items = std::min<int64_t>(tokens.most, chunks_too ? std::max<int64_t>(1, resident / heads) : tokens.items);
     hipLaunchKernelGGL((paged_token_kernel<D, E4M3>), dim3((uint32_t)(items * heads)), dim3(256), 0, s, c, a, tokens, ctx->paged_part);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    // rows of split tiles to merge, tokens': at most
-    int64_t merge_tokens = units > 1 ? std::min<int64_t>((int64_t)a.rows * a.group, (int64_t)c.sequences * kTokenRows) * std::max(1, D / kMergeDims) : 0;
-    merge_tokens = std::min<int64_t>(merge_tokens, std::max(1, (chunks_too ? 512 : 2048) / heads));
+    const int64_t merge_tokens = std::min<int64_t>((int64_t)tokens.most_blocks * std::max(1, D / kMergeDims), std::max(1, (chunks_too ? 512 : 2048) / heads));
     int64_t merge_chunks = 0;
     PlanArgs chunks{};
     float* chunk_part = ctx->paged_part + kPagedPartFloats / 2;
     if (chunks_too) {
-        // about two items per workgroup that the device holds
-        const int64_t held = 2 * (int64_t)ctx->cus * ChunkShape<D, E4M3>::kHeld / heads;
-        chunks = {kChunkRows, kChunkUnit, (int)clamp64(held, 1, (int64_t)(kPagedPartFloats / 2) / record_floats(kChunkRows, D) / heads), kChunkMinUnits,
-                  false};
-        const int64_t tiles = (int64_t)a.rows * a.group / kChunkRows + std::min(c.sequences, a.rows);
-        const int64_t grid = std::max<int64_t>(chunks.items, std::min<int64_t>(tiles, std::max(1, 65536 / heads)));
+        // Tiles are split where they leave CUs without work, into about an item per workgroup that the device holds: a split's
+        // records cost a write and a read of its rows (35 tiles of 8 heads of 256, window 1024: 193 us in three parts, 167 whole).
+        const int64_t records = (int64_t)(kPagedPartFloats / 2) / record_floats(kChunkRows, D) / heads;
+        const int64_t tiles = (int64_t)a.rows * a.group / kChunkRows + sequences;
+        chunks = {kChunkRows, kChunkUnit, (int)clamp64((int64_t)ctx->cus * ChunkShape<D, E4M3>::kHeld / heads, 1, records), kChunkMinUnits, 0, 0, 0, false};
+        chunks.enough = std::min<int>(chunks.items, std::max(1, ctx->cus * 3 / 4 / heads));
+        chunks.most = (int)std::max<int64_t>(chunks.items, tiles);
+        // a tile that is split has at least one other item: no more split tiles than items / 2
+        chunks.most_blocks = chunks.items / 2 * (kChunkRows / kMergeChunkRows);
+        const int64_t grid = std::min<int64_t>(chunks.most, std::max(1, 65536 / heads));
         hipLaunchKernelGGL((paged_chunk_kernel<D, E4M3>), dim3((uint32_t)(grid * heads)), dim3(ChunkShape<D, E4M3>::kThreads), 0, s, c, a, chunks,
                            chunk_part);
         e = hipGetLastError();
         if (e != hipSuccess) return e;
-        // a tile that is split has at least one other item: no more split tiles than items / 2
-        merge_chunks = std::min<int64_t>((int64_t)chunks.items / 2 * (kChunkRows / kMergeChunkRows), std::max(1, 2048 / heads));
+        merge_chunks = std::min<int64_t>(chunks.most_blocks, std::max(1, 2048 / heads));
     }
     if (merge_tokens + merge_chunks == 0) return e;
     hipLaunchKernelGGL((paged_merge_kernel<D, E4M3>), dim3((uint32_t)((merge_tokens + merge_chunks) * heads)), dim3(256), 0, s, c, a, tokens, chunks,
