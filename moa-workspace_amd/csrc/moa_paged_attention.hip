@@ -907,11 +907,60 @@ __global__ __launch_bounds__((ChunkShape<D, E4M3>::kThreads)) __attribute__((amd
 
 // ------------------------------------------------------------------------------------------- the merge
 
-// Rows of split tiles, both kernels' in one launch. A workgroup takes kMergeRows rows of a tile: with many splits and few
-// rows (tokens) one row and 128 of its dims, its threads in groups that take the records in turn; else (chunks)
-// eight rows, a wave per row at a time, its lanes across the dims.
+// Rows of split tiles, both kernels' in one launch. A workgroup takes a block of rows of a tile and finds it once. Few
+// splits: a wave per row, its lanes across the dims. More (long sequences of few rows): the workgroup takes 128 dims of a
+// row, its threads in groups that take the records in turn.
 constexpr int kMergeDims = 128;
+constexpr int kMergeTokenRows = 2;
 constexpr int kMergeChunkRows = 8;
+constexpr int kMergeWaveSplits = 16;
+
+// Row r of the tile (rec: its first record, bm rows each), row `row` of its sequence, by one wave.
+template <int D, bool E4M3>
+__device__ __forceinline__ void merge_row(const PagedView& c, const PagedAttentionCall& a, const Piece& t, int kvh, const float* rec, int bm, int r, int row) {
+    constexpr int kPer = D / 64, kAhead = 4;  // dims of a lane, records in flight
+    const int lane = threadIdx.x & 63;
+    const int64_t size = record_floats(bm, D);
+    float m = -INFINITY, l = 0.0f, v[kPer] = {};
+    bool bad = false;
+    for (int j = lane; j < t.splits; j += 64) {
+        const float x = rec[j * size + r];
+        bad |= x != x;
+        m = fmaxf(m, x);
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, kWave));
+    if (__any(bad)) return;
+    for (int j0 = 0; j0 < t.splits; j0 += kAhead) {
+        float x[kAhead], y[kAhead], w[kAhead][kPer];
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+            const float* at = rec + min(j0 + k, t.splits - 1) * size;
+            x[k] = j0 + k < t.splits ? at[r] : -INFINITY;
+            y[k] = at[bm + r];
+            const float* o = at + 2 * bm + r * D + lane * kPer;
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) w[k][i] = o[i];
+        }
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+            const float f = x[k] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x[k] - m);
+            if (f == 0.0f) continue;  // its sums may be anything
+            l = fmaf(f, y[k], l);
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) v[i] = fmaf(f, w[k][i], v[i]);
+        }
+    }
+    const Row x = row_of(a, t, kvh, row);
+    const float inv = l == 0.0f ? 0.0f : (E4M3 ? c.v_scale[kvh] : 1.0f) / l;
+    uint16_t* to = a.out + x.m * a.out_row + x.h * D + lane * kPer;
+    if constexpr (kPer == 1) {
+        *to = (uint16_t)f2bf(v[0] * inv);
+    } else {
+#pragma unroll
+        for (int k = 0; k < kPer; k += 2) reinterpret_cast<uint32_t*>(to)[k / 2] = pk_bf16(v[k] * inv, v[k + 1] * inv);
+    }
+}
 
 template <int D, bool E4M3>
 __device__ void merge_tokens(const PagedView& c, const PagedAttentionCall& a, const PlanArgs& plan, const float* part, int kvh, int first,
@@ -921,101 +970,76 @@ __device__ void merge_tokens(const PagedView& c, const PagedAttentionCall& a, co
     const int lane = threadIdx.x & 63, col = threadIdx.x % kCols, grp = threadIdx.x / kCols;
     const int64_t size = record_floats(kTokenRows, D);
     Piece t;
-    for (int u = first; u < plan.most_blocks * kBlocks && find_piece(c, a, plan, 1, u / kBlocks, &t); u += stride) {
-        const int d = u % kBlocks * DB + 4 * col, r = t.row;  // one tile a sequence
+    // blocks of kMergeTokenRows rows; the dims of one are dealt out too where its records are many
+    for (int u = first; u < plan.most_blocks * kBlocks && find_piece(c, a, plan, kMergeTokenRows, u / kBlocks, &t); u += stride) {
+        const int d = u % kBlocks * DB + 4 * col, nr = min(kMergeTokenRows, t.n * a.group - t.row);  // one tile a sequence
         const float* rec = part + ((int64_t)kvh * plan.items + t.record) * size;
-        float m = -INFINITY, l = 0.0f;
-        bool bad = false;
-        for (int j = lane; j < t.splits; j += 64) {
-            const float x = rec[j * size + r];
-            bad |= x != x;
-            m = fmaxf(m, x);
+        if (t.splits <= kMergeWaveSplits) {
+            const int i = threadIdx.x >> 6;
+            if (u % kBlocks == 0 && i < nr) merge_row<D, E4M3>(c, a, t, kvh, rec, kTokenRows, t.row + i, t.row + i);
+            continue;
         }
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, kWave));
-        for (int j = lane; j < t.splits; j += 64) {
-            const float x = rec[j * size + r];
-            l += x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x - m) * rec[j * size + kTokenRows + r];
-        }
-        l = wave_sum(l);
-        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        const float* rv = rec + 2 * kTokenRows + r * D + d;
-        for (int j0 = grp; j0 < t.splits; j0 += kGroups * kAhead) {
-            float f[kAhead];
-            float4 y[kAhead];
-#pragma unroll
-            for (int k = 0; k < kAhead; ++k) {
-                const int j = min(j0 + k * kGroups, t.splits - 1);
+        for (int r = t.row; r < t.row + nr; ++r) {
+            float m = -INFINITY, l = 0.0f;
+            bool bad = false;
+            for (int j = lane; j < t.splits; j += 64) {
                 const float x = rec[j * size + r];
-                y[k] = *reinterpret_cast<const float4*>(rv + j * size);
-                f[k] = j0 + k * kGroups >= t.splits || x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x - m);
+                bad |= x != x;
+                m = fmaxf(m, x);
             }
 #pragma unroll
-            for (int k = 0; k < kAhead; ++k)
-                if (f[k] != 0.0f) {
-                    v.x = fmaf(f[k], y[k].x, v.x), v.y = fmaf(f[k], y[k].y, v.y);
-                    v.z = fmaf(f[k], y[k].z, v.z), v.w = fmaf(f[k], y[k].w, v.w);
+            for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, kWave));
+            for (int j = lane; j < t.splits; j += 64) {
+                const float x = rec[j * size + r];
+                l += x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x - m) * rec[j * size + kTokenRows + r];
+            }
+            l = wave_sum(l);
+            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            const float* rv = rec + 2 * kTokenRows + r * D + d;
+            for (int j0 = grp; j0 < t.splits; j0 += kGroups * kAhead) {
+                float f[kAhead];
+                float4 y[kAhead];
+#pragma unroll
+                for (int k = 0; k < kAhead; ++k) {
+                    const int j = min(j0 + k * kGroups, t.splits - 1);
+                    const float x = rec[j * size + r];
+                    y[k] = *reinterpret_cast<const float4*>(rv + j * size);
+                    f[k] = j0 + k * kGroups >= t.splits || x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x - m);
                 }
-        }
-        ov[grp][col] = v;
-        __syncthreads();
-        if (grp == 0 && !__any(bad)) {
 #pragma unroll
-            for (int k = 1; k < kGroups; ++k) {
-                const float4 y = ov[k][col];
-                v.x += y.x, v.y += y.y, v.z += y.z, v.w += y.w;
+                for (int k = 0; k < kAhead; ++k)
+                    if (f[k] != 0.0f) {
+                        v.x = fmaf(f[k], y[k].x, v.x), v.y = fmaf(f[k], y[k].y, v.y);
+                        v.z = fmaf(f[k], y[k].z, v.z), v.w = fmaf(f[k], y[k].w, v.w);
+                    }
             }
-            const Row x = row_of(a, t, kvh, r);
-            const float inv = l == 0.0f ? 0.0f : (E4M3 ? c.v_scale[kvh] : 1.0f) / l;
-            *reinterpret_cast<uint2*>(a.out + x.m * a.out_row + x.h * D + d) = make_uint2(pk_bf16(v.x * inv, v.y * inv), pk_bf16(v.z * inv, v.w * inv));
+            ov[grp][col] = v;
+            __syncthreads();
+            if (grp == 0 && !__any(bad)) {
+#pragma unroll
+                for (int k = 1; k < kGroups; ++k) {
+                    const float4 y = ov[k][col];
+                    v.x += y.x, v.y += y.y, v.z += y.z, v.w += y.w;
+                }
+                const Row x = row_of(a, t, kvh, r);
+                const float inv = l == 0.0f ? 0.0f : (E4M3 ? c.v_scale[kvh] : 1.0f) / l;
+                *reinterpret_cast<uint2*>(a.out + x.m * a.out_row + x.h * D + d) =
+                    make_uint2(pk_bf16(v.x * inv, v.y * inv), pk_bf16(v.z * inv, v.w * inv));
+            }
+            __syncthreads();
         }
-        __syncthreads();
     }
 }
 
 template <int D, bool E4M3>
 __device__ void merge_chunks(const PagedView& c, const PagedAttentionCall& a, const PlanArgs& plan, const float* part, int kvh, int first,
                              int stride) {
-    constexpr int kPer = D / 64;  // dims of a lane
-    const int lane = threadIdx.x & 63;
-    const int64_t size = record_floats(kChunkRows, D);
     Piece t;
     for (int u = first; u < plan.most_blocks && find_piece(c, a, plan, kMergeChunkRows, u, &t); u += stride) {
-        const float* rec = part + ((int64_t)kvh * plan.items + t.record) * size;
-        const int r0 = t.row - t.tile * kChunkRows, rows = min(kMergeChunkRows, t.n * a.group - t.row);
-#pragma unroll 2
-        for (int i = threadIdx.x >> 6; i < rows; i += 4) {
-            const int r = r0 + i;
-            float m = -INFINITY, l = 0.0f, v[kPer] = {};
-            bool bad = false;
-            for (int j = 0; j < t.splits; ++j) {
-                const float x = rec[j * size + r];
-                bad |= x != x;
-                m = fmaxf(m, x);
-            }
-            for (int j = 0; j < t.splits; ++j) {
-                const float x = rec[j * size + r], y = rec[j * size + kChunkRows + r];
-                const float* o = rec + j * size + 2 * kChunkRows + r * D + lane * kPer;
-                float w[kPer];
-#pragma unroll
-                for (int k = 0; k < kPer; ++k) w[k] = o[k];
-                const float f = x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x - m);
-                if (f == 0.0f) continue;  // its sums may be anything
-                l = fmaf(f, y, l);
-#pragma unroll
-                for (int k = 0; k < kPer; ++k) v[k] = fmaf(f, w[k], v[k]);
-            }
-            if (bad) continue;
-            const Row x = row_of(a, t, kvh, t.row + i);
-            const float inv = l == 0.0f ? 0.0f : (E4M3 ? c.v_scale[kvh] : 1.0f) / l;
-            uint16_t* to = a.out + x.m * a.out_row + x.h * D + lane * kPer;
-            if constexpr (kPer == 1) {
-                *to = (uint16_t)f2bf(v[0] * inv);
-            } else {
-#pragma unroll
-                for (int k = 0; k < kPer; k += 2) reinterpret_cast<uint32_t*>(to)[k / 2] = pk_bf16(v[k] * inv, v[k + 1] * inv);
-            }
-        }
+        const float* rec = part + ((int64_t)kvh * plan.items + t.record) * record_floats(kChunkRows, D);
+        const int rows = min(kMergeChunkRows, t.n * a.group - t.row);
+        for (int i = threadIdx.x >> 6; i < rows; i += 4)
+            merge_row<D, E4M3>(c, a, t, kvh, rec, kChunkRows, t.row - t.tile * kChunkRows + i, t.row + i);
     }
 }
 
@@ -1049,7 +1073,9 @@ hipError_t launch(const PagedView& c, const PagedAttentionCall& a, hipStream_t s
     const int64_t sequences = std::min(c.sequences, a.rows);  // with rows
     // unsplit, an item a sequence; split, within the plan's items
     tokens.most = (int)std::min<int64_t>(sequences * units, std::max<int64_t>(tokens.items, sequences));
-    tokens.most_blocks = (int)(units > 1 ? std::min<int64_t>((int64_t)a.rows * a.group, sequences * kTokenRows) : 0);
+    tokens.most_blocks = (int)(units > 1 ? std::min<int64_t>((int64_t)a.rows * a.group / kMergeTokenRows + sequences,
+                                                             sequences * std::min<int64_t>(kTokenRows / kMergeTokenRows, (int64_t)a.max_rows * a.group))
+                                         : 0);
     const int64_t items = std::min<int64_t>(tokens.most, chunks_too ? std::max<int64_t>(1, resident / heads) : tokens.items);
     hipLaunchKernelGGL((paged_token_kernel<D, E4M3>), dim3((uint32_t)(items * heads)), dim3(256), 0, s, c, a, tokens, ctx->paged_part);
     hipError_t e = hipGetLastError();

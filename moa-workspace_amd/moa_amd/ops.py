@@ -410,32 +410,42 @@ class PagedCache:
                                           slots, heads, dim, int(e4m3), seqs, columns)
 
 
-def _paged(cache, *indexes):
-    """The stream of a call on `cache`, after the checks of its index tensors (tensor, name, elements or None)."""
+def _index(t, name, cache, numel):
+    """The address of an int32 index tensor of a call on `cache` (numel: None for any number)."""
     if not isinstance(cache, PagedCache):
         raise TypeError("cache must be a PagedCache")
-    ptrs = [_ptr(t, name, _I32, n) for t, name, n in indexes]
-    dev = cache.device_index
-    for t, name, _ in indexes:
-        if t.get_device() != dev:
-            raise ValueError(f"{name} lives on cuda:{t.get_device()}, the cache on cuda:{dev}")
-    return _stream(cache._keep[0]), *ptrs
+    p = _ptr(t, name, _I32, numel if numel is None else getattr(cache, numel[0]) + numel[1])
+    if p is None:
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if t.get_device() != cache.device_index:
+        raise ValueError(f"{name} lives on cuda:{t.get_device()}, the cache on cuda:{cache.device_index}")
+    return p
+
+
+def _cache_stream(cache) -> int:
+    """The current stream of the cache's device, which must be the current one (as _stream)."""
+    cur = torch.cuda.current_device()
+    if cache.device_index != cur:
+        raise ValueError(f"the cache lives on cuda:{cache.device_index} but the current device is cuda:{cur}; "
+                         f"call it under torch.cuda.device({cache.device_index})")
+    return torch._C._cuda_getCurrentRawStream(cur)
 
 
 def _row_tensor(t, name, cache, heads):
-    """Address, row stride and rows of a bf16 [rows, heads, head_dim] tensor whose rows may lie apart."""
+    """Address, row stride and rows of a bf16 [rows, heads, head_dim] tensor whose rows may lie apart. (Tuples are unpacked
+    and compared whole: every call runs this for each of its tensors.)"""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
-    dev = t.get_device()
-    if dev != cache.device_index:
+    if t.get_device() != cache.device_index:
         raise ValueError(f"{name} must live on cuda:{cache.device_index} as the cache does, got {t.device}")
     if t.dtype not in _BF16:
         raise TypeError(f"{name}: dtype {t.dtype} not in {_BF16}")
-    if t.dim() != 3 or t.shape[2] != cache.head_dim or (heads is not None and t.shape[1] != heads):
-        raise ValueError(f"{name} must be [rows, {heads or 'heads'}, {cache.head_dim}], got {tuple(t.shape)}")
-    rows, h, d = t.shape
+    shape = t.shape
+    if len(shape) != 3 or shape[2] != cache.head_dim or (heads is not None and shape[1] != heads):
+        raise ValueError(f"{name} must be [rows, {heads or 'heads'}, {cache.head_dim}], got {tuple(shape)}")
+    rows, h, d = shape
     row, head, one = t.stride()
-    if (one != 1 and d > 1) or (head != d and h > 1):
+    if one != 1 or (head != d and h > 1):
         raise ValueError(f"{name}: heads and head_dim must be dense")
     return t.data_ptr(), (row if rows > 1 else h * d), rows
 
@@ -443,8 +453,8 @@ def _row_tensor(t, name, cache, heads):
 def paged_cache_reserve(cache, new_tokens) -> None:
     """Grows every sequence s by new_tokens[s] positions (int32 [sequences]): the lowest free pages, in the order of the
     sequences. All or nothing: where it cannot be served whole the state stays and bit 8 is raised."""
-    s, p = _paged(cache, (new_tokens, "new_tokens", cache.sequences if isinstance(cache, PagedCache) else None))
-    _call("moa_paged_cache_reserve", cache._struct, p, s)
+    p = _index(new_tokens, "new_tokens", cache, ("sequences", 0))
+    _call("moa_paged_cache_reserve", cache._struct, p, _cache_stream(cache))
 
 
 def paged_cache_append(cache, k, v, row_starts, layer=0) -> None:
@@ -452,34 +462,37 @@ def paged_cache_append(cache, k, v, row_starts, layer=0) -> None:
     Rows row_starts[s] .. row_starts[s + 1] - 1 (int32 [sequences + 1]) are the last positions of sequence s, so reserve
     first. E4M3 pages take the nearest code of x / scale, at most +-448. A row whose position or page is out of range is
     not written (bit 8)."""
-    s, p = _paged(cache, (row_starts, "row_starts", cache.sequences + 1 if isinstance(cache, PagedCache) else None))
+    p = _index(row_starts, "row_starts", cache, ("sequences", 1))
     kp, kr, rows = _row_tensor(k, "k", cache, cache.kv_heads)
     vp, vr, vrows = _row_tensor(v, "v", cache, cache.kv_heads)
     if vrows != rows:
         raise ValueError(f"v: expected {rows} rows, got {vrows}")
-    _call("moa_paged_cache_append", cache._struct, kp, kr, vp, vr, p, rows, layer, s)
+    _call("moa_paged_cache_append", cache._struct, kp, kr, vp, vr, p, rows, layer, _cache_stream(cache))
 
 
 def paged_cache_fork(cache, parents, children) -> None:
     """Makes the empty sequences children[i] copies of parents[i] (int32 [count]): full pages are shared, the partly
     filled last page of every layer is copied to the lowest free page. All or nothing (bit 8): see moa_paged.h."""
-    n = children.numel() if isinstance(children, torch.Tensor) else None
-    s, p, c = _paged(cache, (parents, "parents", n), (children, "children", n))
-    _call("moa_paged_cache_fork", cache._struct, p, c, n, s)
+    p, c = _index(parents, "parents", cache, None), _index(children, "children", cache, None)
+    n = children.numel()
+    if parents.numel() != n:
+        raise ValueError(f"parents: expected {n} elements, got {parents.numel()}")
+    _call("moa_paged_cache_fork", cache._struct, p, c, n, _cache_stream(cache))
 
 
 def paged_cache_free(cache, sequences) -> None:
     """Ends the listed sequences (int32 [count]): their length becomes 0 and their pages lose a reference. Empty and
     repeated ones change nothing; an index out of range is left out (bit 8)."""
-    s, p = _paged(cache, (sequences, "sequences", None))
-    _call("moa_paged_cache_free", cache._struct, p, sequences.numel(), s)
+    p = _index(sequences, "sequences", cache, None)
+    _call("moa_paged_cache_free", cache._struct, p, sequences.numel(), _cache_stream(cache))
 
 
 def paged_cache_compact(cache) -> None:
     """Moves the n live pages to pages 0 .. n - 1 in every layer, page table and reference counts with them: those at n
     and beyond go, in order, to the free pages below n."""
-    s, = _paged(cache)
-    _call("moa_paged_cache_compact", cache._struct, s)
+    if not isinstance(cache, PagedCache):
+        raise TypeError("cache must be a PagedCache")
+    _call("moa_paged_cache_compact", cache._struct, _cache_stream(cache))
 
 
 def paged_attention(q, cache, row_starts, out, layer=0, window=0, scale=1.0, max_rows=None) -> None:
@@ -490,13 +503,13 @@ def paged_attention(q, cache, row_starts, out, layer=0, window=0, scale=1.0, max
     sequence are left as they were. max_rows: the most rows a sequence has in this call (default: all rows; the
     right number makes the call faster). A sequence with a bad length, bad row starts or more rows than max_rows is left
     out, and so is at least every row that sees a page outside the pool (bit 8)."""
-    s, p = _paged(cache, (row_starts, "row_starts", cache.sequences + 1 if isinstance(cache, PagedCache) else None))
+    p = _index(row_starts, "row_starts", cache, ("sequences", 1))
     qp, qr, rows = _row_tensor(q, "q", cache, None)
     op, orow, orows = _row_tensor(out, "out", cache, q.shape[1])
     if orows != rows:
         raise ValueError(f"out: expected {rows} rows, got {orows}")
     _call("moa_paged_attention", qp, qr, cache._struct, p, op, orow, rows, q.shape[1], layer, window, scale,
-          rows if max_rows is None else max_rows, s)
+          rows if max_rows is None else max_rows, _cache_stream(cache))
 
 
 def fp8_scaled_projection(x, w, scale, out) -> None:
