@@ -20,7 +20,7 @@ namespace {
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kTokenRows = 16;   // rows of a token-kernel item
-constexpr int kTokenUnit = 128;  // positions that a split is a multiple of: one or two steps of four waves
+constexpr int kTokenUnit = 128;  // positions that work is dealt out by: one or two steps of four waves
 // Weights are 2^(x - reference), the reference at most this far below the row's largest x so far: the output is
 // rescaled only when the maximum has grown by more.
 constexpr float kSlack = 8.0f;
@@ -29,48 +29,36 @@ __device__ __forceinline__ bf16x8 as_bf16x8(const uint4& v) { return __builtin_b
 
 // ------------------------------------------------------------------------------------ who does what
 
-// How a call's sequences are split into items, the same in every kernel of the call. A sequence of r = n * group rows has
-// ceil(r / bm) tiles, each split over ceil(units / c) items, where units covers the positions a tile can see in steps of
-// `unit`, and c, at least min_units, is chosen so that all sequences together have at most `items` items per KV head (a
-// call with `enough` tiles splits none). The last tiles of a sequence, which see the most, come first.
-struct PlanArgs {
-    int bm, unit, items, min_units;
-    int enough;   // with this many tiles or more, none is split
-    int most;     // no call has more items than this
-    int most_blocks;  // nor more blocks of rows to merge
-    bool tokens;  // the token kernel's sequences (at most kTokenRows rows) or the others
-};
+// A sequence that takes part: its first row of the call, new rows and length. n = 0: it does not, or is bad.
+struct Seq { int row0, n, len; };
 
-struct Piece {  // an item, or a row of the merge
-    int s, row0, n, len;    // its sequence: first row of the call, new rows, length
-    int tile, split, splits;
-    int record;             // the first record of its tile
-    int row;                // the merge: first row of the block, in its sequence
-};
-
-struct SeqWork { int row0, n, len, tiles, units; };
-
-__device__ __forceinline__ SeqWork seq_work(const PagedView& c, const PagedAttentionCall& a, const PlanArgs& p, int s, bool* bad) {
-    SeqWork w = {0, 0, 0, 0, 0};
-    if (s >= c.sequences) return w;
-    w.row0 = a.starts[s];
+__device__ __forceinline__ Seq seq_of(const PagedView& c, const PagedAttentionCall& a, int s, bool tokens, bool* bad) {
+    Seq q = {0, 0, 0};
+    if (s >= c.sequences) return q;
+    q.row0 = a.starts[s];
     const int end = a.starts[s + 1];
-    w.len = c.lens[s];
-    w.n = end - w.row0;
-    if (w.n == 0) return w;
-    if (w.row0 < 0 || w.n < 0 || end > a.rows || w.n > a.max_rows || w.len < 0 || w.len > paged_capacity(c)) {
+    q.len = c.lens[s];
+    const int n = end - q.row0;
+    if (n == 0) return q;
+    if (q.row0 < 0 || n < 0 || end > a.rows || n > a.max_rows || q.len < 0 || q.len > paged_capacity(c)) {
         *bad = true;
-        return w;
+        return q;
     }
-    const int rows = w.n * a.group;  // at most 2^20 * 128
-    if ((rows <= kTokenRows) != p.tokens) return w;
-    w.tiles = (rows + p.bm - 1) / p.bm;
-    // positions that a tile's rows see: all, or the window and the tile's tokens, from a multiple of the unit on
-    const int span = p.tokens ? w.n : min(w.n, (p.bm + a.group - 1) / a.group + 1);
-    const int seen = a.window ? min(w.len, a.window + span - 1 + p.unit) : w.len;
-    w.units = max(1, (seen + p.unit - 1) / p.unit);
-    return w;
+    if ((n * a.group <= kTokenRows) == tokens) q.n = n;  // at most 2^20 * 128 rows
+    return q;
 }
+
+__device__ __forceinline__ void raise_bad(const PagedView& c, bool bad) {
+    if (__any(bad) && blockIdx.x == 0 && (threadIdx.x & 63) == 0) atomicOr(c.err, kErrPaged);
+}
+
+// Part of a sequence's rows and positions: what a workgroup works on.
+struct Piece {
+    int s, row0, n, len;        // its sequence
+    int tile, split, splits;    // the tile of rows, and which part of its positions
+    int record;                 // of the tile's first split
+    int row;                    // the merge: first row of the block, in its sequence
+};
 
 // Inclusive sum over the wave's lanes: four shifts within rows of 16, then the rows' last lanes (DPP: no LDS on the way).
 __device__ __forceinline__ int scan_sum(int x) {
@@ -84,55 +72,148 @@ __device__ __forceinline__ int scan_sum(int x) {
 }
 __device__ __forceinline__ int wave_total(int x) { return __builtin_amdgcn_readlane(scan_sum(x), 63); }
 
+// Token rows. The positions of all sequences, in units of kTokenUnit, are one row of U units, dealt out evenly: group w of
+// `groups` takes units [w q, (w + 1) q), q = ceil(U / groups), crossing from sequence to sequence. A part that is not its whole
+// sequence leaves a record for the merge: number 2 w where it begins inside its sequence, 2 w + 1 where it begins it, so
+// split j of a sequence that begins in group w0 is record 2 (w0 + j) + (j == 0).
+struct TokenWalk {
+    int64_t units, q;           // U, q
+    int base;                   // the 64 sequences looked at
+    int64_t before;             // units before them
+};
+
+// First position and units of a sequence's span: from a multiple of `align` on, at least one unit.
+__device__ __forceinline__ int token_first(const PagedAttentionCall& a, const Seq& q, int align) {
+    const int p0 = q.len - q.n;
+    return a.window && p0 >= a.window ? (p0 - a.window + 1) / align * align : 0;
+}
+__device__ __forceinline__ int token_units(const PagedAttentionCall& a, const Seq& q, int align) {
+    return q.n ? max(1, (q.len - token_first(a, q, align) + kTokenUnit - 1) / kTokenUnit) : 0;
+}
+
+__device__ TokenWalk token_walk(const PagedView& c, const PagedAttentionCall& a, int groups, int align) {
+    TokenWalk w = {0, 1, 0, 0};
+    bool bad = false;
+    for (int base = 0; base < c.sequences; base += 64)  // 64 sequences have at most 64 * 2^23 units
+        w.units += wave_total(token_units(a, seq_of(c, a, base + (threadIdx.x & 63), true, &bad), align));
+    raise_bad(c, bad);
+    // (a 64-bit quotient costs a microsecond; real calls have far fewer units)
+    w.q = w.units >> 31 ? (w.units + groups - 1) / groups : ((uint32_t)w.units + (uint32_t)groups - 1) / (uint32_t)groups;
+    w.q = w.q ? w.q : 1;
+    return w;
+}
+
+// The sequence that unit u (not before an earlier call's) belongs to, its units and the first of them. u < w.units.
+__device__ void token_at(const PagedView& c, const PagedAttentionCall& a, TokenWalk& w, int align, int64_t u, Piece* out, int* units,
+                         int64_t* first) {
+    const int lane = threadIdx.x & 63;
+    bool bad = false;
+    for (;; w.base += 64) {
+        const Seq q = seq_of(c, a, w.base + lane, true, &bad);
+        const int n = token_units(a, q, align), x = scan_sum(n), all = __builtin_amdgcn_readlane(x, 63);
+        if (w.base + 64 >= c.sequences || u - w.before < all) {
+            const int l = __builtin_ctzll(__ballot(x > (int)(u - w.before)) | 1ull << 63);
+            auto get = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
+            *out = {w.base + l, get(q.row0), get(q.n), get(q.len), 0, 0, 1, 0, 0};
+            *units = get(n);
+            *first = w.before + get(x - n);
+            return;
+        }
+        w.before += all;
+    }
+}
+
+// Block `want` of `rows` rows of the sequences that are split, for the merge; record: its first. False: there are not that many.
+__device__ bool token_block(const PagedView& c, const PagedAttentionCall& a, const TokenWalk& w, int align, int rows, int want, Piece* out) {
+    const int lane = threadIdx.x & 63;
+    bool bad = false;
+    int64_t before = 0;
+    int blocks_before = 0;
+    for (int base = 0; base < c.sequences; base += 64) {
+        const Seq q = seq_of(c, a, base + lane, true, &bad);
+        const int n = token_units(a, q, align), x = scan_sum(n);
+        const int64_t first = before + x - n, last = first + max(n, 1) - 1;
+        const int64_t w0 = w.units >> 31 ? first / w.q : (uint32_t)first / (uint32_t)w.q;
+        const int64_t w1 = w.units >> 31 ? last / w.q : (uint32_t)last / (uint32_t)w.q;
+        const int splits = n ? (int)(w1 - w0) + 1 : 0, blocks = splits > 1 ? (q.n * a.group + rows - 1) / rows : 0, xb = scan_sum(blocks);
+        const uint64_t hit = __ballot(blocks_before + xb > want);
+        if (hit) {
+            const int l = __builtin_ctzll(hit);
+            auto get = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
+            *out = {base + l, get(q.row0), get(q.n), get(q.len), 0, 0, get(splits), 2 * get((int)w0), (want - blocks_before - get(xb - blocks)) * rows};
+            return true;
+        }
+        before += __builtin_amdgcn_readlane(x, 63);
+        blocks_before += __builtin_amdgcn_readlane(xb, 63);
+    }
+    return false;
+}
+
+// Chunks: a sequence of r = n * group rows has ceil(r / kChunkRows) tiles, each split over ceil(units / c) items, where units
+// covers the positions a tile can see in steps of kChunkUnit, and c, at least kChunkMinUnits, is chosen so that all
+// sequences together have at most `items` items per KV head (a call with `enough` tiles splits none). The last tiles of
+// a sequence, which see the most, come first.
+constexpr int kChunkRows = 128;
+constexpr int kChunkUnit = 64;
+constexpr int kChunkMinUnits = 4;
+struct ChunkPlan {
+    int items;
+    int enough;       // with this many tiles or more, none is split
+    int most;         // no call has more items than this
+    int most_blocks;  // nor more blocks of rows to merge
+};
+
 // Finds piece `want` by one wave: an item (merge_rows = 0), or block `want` of merge_rows rows of the tiles that are split.
 // False: there are not that many.
-__device__ bool find_piece(const PagedView& c, const PagedAttentionCall& a, const PlanArgs& p, int merge_rows, int want, Piece* out) {
+__device__ bool find_piece(const PagedView& c, const PagedAttentionCall& a, const ChunkPlan& p, int merge_rows, int want, Piece* out) {
     const int lane = threadIdx.x & 63;
+    // tiles of a sequence, and the units that a tile's rows see: all, or the window and the tile's tokens
+    auto tiles_of = [&](const Seq& q) { return (q.n * a.group + kChunkRows - 1) / kChunkRows; };
+    auto units_of = [&](const Seq& q) {
+        const int span = min(q.n, (kChunkRows + a.group - 1) / a.group + 1);
+        const int seen = a.window ? min(q.len, a.window + span - 1 + kChunkUnit) : q.len;
+        return max(1, (seen + kChunkUnit - 1) / kChunkUnit);
+    };
     int tiles = 0;
     float units = 0.0f;
     bool bad = false;
-    SeqWork w = {};
+    Seq q = {};
     for (int base = 0; base < c.sequences; base += 64) {
-        w = seq_work(c, a, p, base + lane, &bad);
-        tiles += w.tiles;
-        units += (float)w.tiles * (float)w.units;
+        q = seq_of(c, a, base + lane, false, &bad);
+        tiles += tiles_of(q);
+        units += (float)tiles_of(q) * (float)units_of(q);
     }
-    if (__any(bad) && blockIdx.x == 0 && lane == 0) atomicOr(c.err, kErrPaged);
-    tiles = wave_total(tiles);  // at most 2^20 rows * 128 heads / bm, and one per sequence
+    raise_bad(c, bad);
+    tiles = wave_total(tiles);  // at most 2^20 rows * 128 heads / kChunkRows, and one per sequence
     if (tiles == 0) return false;
     // sum of ceil(units / per) <= units / per + tiles <= items. The float sum is rounded the same in every wave, and
     // short by at most 1024 + 8 roundings of 2^-24: a part in ten thousand more covers them.
     units = wave_sum(units);
     int per = 1 << 30;
-    if (tiles < p.enough) per = max(p.min_units, (int)fminf(units * 1.0001f / (float)(p.items - tiles) + 1.0f, 1e9f));
+    if (tiles < p.enough) per = max(kChunkMinUnits, (int)fminf(units * 1.0001f / (float)(p.items - tiles) + 1.0f, 1e9f));
     int items_before = 0, blocks_before = 0;
     for (int base = 0; base < c.sequences; base += 64) {
-        if (c.sequences > 64) w = seq_work(c, a, p, base + lane, &bad);
-        const int splits = w.tiles ? (w.units + per - 1) / per : 0, items = w.tiles * splits;
-        const int rows = w.n * a.group, tile_blocks = merge_rows ? p.bm / merge_rows : 0;
-        const int blocks = merge_rows && splits > 1 ? (rows + merge_rows - 1) / merge_rows : 0;
+        if (c.sequences > 64) q = seq_of(c, a, base + lane, false, &bad);
+        const int splits = q.n ? (units_of(q) + per - 1) / per : 0, items = tiles_of(q) * splits;
+        const int blocks = merge_rows && splits > 1 ? (q.n * a.group + merge_rows - 1) / merge_rows : 0;
         const int xi = scan_sum(items), xb = merge_rows ? scan_sum(blocks) : 0;
         const uint64_t hit = __ballot((merge_rows ? blocks_before + xb : items_before + xi) > want);
         if (hit) {
             const int l = __builtin_ctzll(hit);
             auto get = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
-            out->s = base + l;
-            out->row0 = get(w.row0), out->n = get(w.n), out->len = get(w.len);
-            out->splits = get(splits);
-            const int last = get(w.tiles) - 1, first_item = items_before + get(xi - items);
+            *out = {base + l, get(q.row0), get(q.n), get(q.len), 0, 0, get(splits), 0, 0};
+            const int last = get(tiles_of(q)) - 1, first_item = items_before + get(xi - items);
             int j;  // the tile's place, the last tile first
             if (merge_rows) {
                 const int k = want - blocks_before - get(xb - blocks);
-                out->tile = k / tile_blocks;
-                out->split = 0;
                 out->row = k * merge_rows;
+                out->tile = out->row / kChunkRows;
                 j = last - out->tile;
             } else {
                 const int k = want - items_before - get(xi - items);
                 j = k / out->splits;
                 out->tile = last - j;
                 out->split = k - j * out->splits;
-                out->row = 0;
             }
             out->record = first_item + j * out->splits;
             return true;
@@ -215,10 +296,11 @@ __device__ __forceinline__ Row row_of(const PagedAttentionCall& a, const Piece& 
     return x;
 }
 
-// The positions [lo, hi) of a piece's split: what rows r0 .. r1 of its sequence see, from a multiple of `align` on, in even
+// The positions [lo, hi) of a tile's split: what rows r0 .. r1 of its sequence see, from a multiple of `align` on, in even
 // parts of whole units.
 struct Span { int lo, hi; };
-__device__ __forceinline__ Span span_of(const PagedAttentionCall& a, const Piece& t, int r0, int r1, int unit, int align) {
+__device__ __forceinline__ Span span_of(const PagedAttentionCall& a, const Piece& t, int r0, int r1, int align) {
+    constexpr int unit = kChunkUnit;
     const int p0 = t.len - t.n + r0 / a.group, p1 = t.len - t.n + r1 / a.group;
     const int lo = a.window && p0 >= a.window ? (p0 - a.window + 1) / align * align : 0, hi = max(p1 + 1, lo);
     const int units = (hi - lo + unit - 1) / unit, per = (units + t.splits - 1) / t.splits;
@@ -248,7 +330,7 @@ __device__ void careful_piece(const PagedView& c, const PagedAttentionCall& a, c
 
 // ------------------------------------------------------------------------------------ the token kernel
 
-// Up to 16 rows of a sequence over a span of positions: bound by the bytes of K and V, which go from memory to
+// Up to 16 rows of a sequence over a part of its positions: bound by the bytes of K and V, which go from memory to
 // registers and never through LDS. Four waves take a tile of 16 or 32 positions each in turn. Scores are K times Q^T
 // (16 x 16 x 32 MFMAs): lane (c = lane % 16, g = lane / 16) then holds, for row c, positions 4 g .. 4 g + 3 of each 16,
 // which are just the positions it supplies as A of P times V when V's lanes take the same ones: P moves between no
@@ -261,7 +343,7 @@ struct TokenShape {
     static constexpr int kElem = E4M3 ? 1 : 2;
     static constexpr int kSub = D * kElem >= 512 ? 1 : 2;                       // 16 positions each: K and V of a tile in 128 registers
     static constexpr int kTile = 16 * kSub;
-    static constexpr int kWavesPerSimd = D == 512 ? 1 : (D == 256 ? 2 : 3);
+    static constexpr int kHeld = D == 512 ? 1 : (D == 256 ? 2 : 3);              // workgroups on a CU: waves per SIMD
     static constexpr int kKLoads = D * kElem / 64;                              // 16-byte loads of a K row per lane
     static constexpr int kVD = (E4M3 ? 16 : 8) < D / 16 ? (E4M3 ? 16 : 8) : D / 16;  // dims per V load
     static constexpr int kVB = D / (16 * kVD);                                  // V loads of a row per lane
@@ -293,8 +375,8 @@ __device__ __forceinline__ uint32_t bf16_pair_of_fp8(uint32_t two) {
 }
 
 template <int D, bool E4M3>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(TokenShape<D, E4M3>::kWavesPerSimd))) void paged_token_kernel(
-    PagedView c, PagedAttentionCall a, PlanArgs plan, float* part) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(TokenShape<D, E4M3>::kHeld))) void paged_token_kernel(
+    PagedView c, PagedAttentionCall a, float* part) {
     using T = TokenShape<D, E4M3>;
     constexpr int NT = T::kSub;
     __shared__ __attribute__((aligned(16))) uint16_t qs[16 * T::kQStride];
@@ -303,12 +385,20 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(TokenShape<
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l16 = lane & 15, g = lane >> 4;
     const int kvh = blockIdx.x % c.kv_heads;
     const float factor = E4M3 ? c.k_scale[kvh] * a.scale_log2 : a.scale_log2;
-    Piece t;
-    for (int item = blockIdx.x / c.kv_heads; item < plan.most && find_piece(c, a, plan, 0, item, &t); item += gridDim.x / c.kv_heads) {
-        const int nr = t.n * a.group;
-        const Span span = span_of(a, t, 0, nr - 1, kTokenUnit, T::kTile);
-        const int lo = span.lo, hi = span.hi;
-        __syncthreads();  // the item before has been written out
+    const int groups = gridDim.x / c.kv_heads, group = blockIdx.x / c.kv_heads;
+    TokenWalk walk = token_walk(c, a, groups, T::kTile);
+    const int64_t end = min(walk.units, (group + 1) * walk.q);
+    for (int64_t unit = group * walk.q; unit < end;) {
+        Piece t;
+        int units;
+        int64_t first;
+        token_at(c, a, walk, T::kTile, unit, &t, &units, &first);
+        const int off = (int)(unit - first), take = (int)min((int64_t)(units - off), end - unit);
+        const bool whole = off == 0 && take == units;
+        unit += take;
+        const int nr = t.n * a.group, from = token_first(a, Seq{t.row0, t.n, t.len}, T::kTile);
+        const int lo = from + off * kTokenUnit, hi = (int)min((int64_t)lo + (int64_t)take * kTokenUnit, (int64_t)t.len);
+        __syncthreads();  // the part before has been written out
         for (int i = threadIdx.x; i < 16 * D / 8; i += 256) {
             const int r = i / (D / 8), j = i - r * (D / 8);
             const Row x = row_of(a, t, kvh, min(r, nr - 1));
@@ -478,7 +568,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(TokenShape<
                     *reinterpret_cast<float4*>(os + ((wave * kTokenRows + 4 * g + e) * D + 16 * T::kVD * b + T::kVD * l16 + d)) =
                         make_float4(o[b][d][e], o[b][d + 1][e], o[b][d + 2][e], o[b][d + 3][e]);
         bad = __syncthreads_or(bad);
-        float* rec = t.splits > 1 ? part + ((int64_t)kvh * plan.items + t.record + t.split) * record_floats(kTokenRows, D) : nullptr;
+        float* rec = whole ? nullptr : part + ((int64_t)kvh * 2 * groups + 2 * group + (off == 0)) * record_floats(kTokenRows, D);
         bool odd = false;
         const float vs = E4M3 ? c.v_scale[kvh] : 1.0f;
         for (int i = threadIdx.x; i < nr * (D / 4); i += 256) {
@@ -521,7 +611,6 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(TokenShape<
 // is rounded to bf16 anyway. The sum adds the weights as they enter, in f32: their roundings then cancel in part.
 // 512 dims: a row's Q and out do not fit beside each other in a wave's registers, so two waves share 32 rows, each with
 // half of the dims: they add the halves of the scores through LDS, and both weigh them.
-constexpr int kChunkRows = 128;
 template <int D, bool E4M3>
 struct ChunkShape {
     static constexpr int kTile = D >= 256 ? 32 : 64;
@@ -536,8 +625,6 @@ struct ChunkShape {
     static constexpr int kCodeLoads = kTile * D / 16 / kThreads;     // E4M3: 16-byte loads of K (and V) per thread and tile
     static constexpr int kGroup = 64 / kWaveRows;               // tiles whose positions a wave's lanes look up at once
 };
-constexpr int kChunkUnit = 64;      // positions that a split is a multiple of
-constexpr int kChunkMinUnits = 4;   // and the fewest of them
 
 // 16-byte chunk c of LDS row r lies in chunk c ^ swizzle(r): sixteen rows' reads of one chunk, and four rows' reads of four
 // chunks, then meet on no bank. Rows of 128 bytes (64 dims) pair up: two rows span the banks.
@@ -577,7 +664,7 @@ __device__ __forceinline__ int lane_here() {
 
 template <int D, bool E4M3>
 __global__ __launch_bounds__((ChunkShape<D, E4M3>::kThreads)) __attribute__((amdgpu_waves_per_eu(2))) void paged_chunk_kernel(
-    PagedView c, PagedAttentionCall a, PlanArgs plan, float* part) {
+    PagedView c, PagedAttentionCall a, ChunkPlan plan, float* part) {
     using T = ChunkShape<D, E4M3>;
     constexpr int kTile = T::kTile, kPair = T::kPair, kWaves = 4 * kPair, kMine = D / kPair;  // dims of a wave
     constexpr int kSteps = kMine / 16, kDims = kMine / 32;
@@ -615,7 +702,7 @@ __global__ __launch_bounds__((ChunkShape<D, E4M3>::kThreads)) __attribute__((amd
     Piece t;
     for (int item = blockIdx.x / c.kv_heads; item < plan.most && find_piece(c, a, plan, 0, item, &t); item += gridDim.x / c.kv_heads) {
         const int r0 = t.tile * kChunkRows, nr = (int)min((int64_t)kChunkRows, (int64_t)t.n * a.group - r0);
-        const Span span = span_of(a, t, r0, r0 + nr - 1, kChunkUnit, kTile);
+        const Span span = span_of(a, t, r0, r0 + nr - 1, kTile);
         const int lo = span.lo, hi = span.hi;
         const int wrow = 32 * rg + l32;  // the lane's row of the tile
         const Row mine = row_of(a, t, kvh, r0 + min(wrow, nr - 1));
@@ -915,16 +1002,15 @@ constexpr int kMergeTokenRows = 2;
 constexpr int kMergeChunkRows = 8;
 constexpr int kMergeWaveSplits = 16;
 
-// Row r of the tile (rec: its first record, bm rows each), row `row` of its sequence, by one wave.
-template <int D, bool E4M3>
-__device__ __forceinline__ void merge_row(const PagedView& c, const PagedAttentionCall& a, const Piece& t, int kvh, const float* rec, int bm, int r, int row) {
+// Row r of the tile (rec(j): the record of split j, bm rows each), row `row` of its sequence, by one wave.
+template <int D, bool E4M3, class R>
+__device__ __forceinline__ void merge_row(const PagedView& c, const PagedAttentionCall& a, const Piece& t, int kvh, R rec, int bm, int r, int row) {
     constexpr int kPer = D / 64, kAhead = 4;  // dims of a lane, records in flight
     const int lane = threadIdx.x & 63;
-    const int64_t size = record_floats(bm, D);
     float m = -INFINITY, l = 0.0f, v[kPer] = {};
     bool bad = false;
     for (int j = lane; j < t.splits; j += 64) {
-        const float x = rec[j * size + r];
+        const float x = rec(j)[r];
         bad |= x != x;
         m = fmaxf(m, x);
     }
@@ -935,7 +1021,7 @@ __device__ __forceinline__ void merge_row(const PagedView& c, const PagedAttenti
         float x[kAhead], y[kAhead], w[kAhead][kPer];
 #pragma unroll
         for (int k = 0; k < kAhead; ++k) {
-            const float* at = rec + min(j0 + k, t.splits - 1) * size;
+            const float* at = rec(min(j0 + k, t.splits - 1));
             x[k] = j0 + k < t.splits ? at[r] : -INFINITY;
             y[k] = at[bm + r];
             const float* o = at + 2 * bm + r * D + lane * kPer;
@@ -963,17 +1049,20 @@ __device__ __forceinline__ void merge_row(const PagedView& c, const PagedAttenti
 }
 
 template <int D, bool E4M3>
-__device__ void merge_tokens(const PagedView& c, const PagedAttentionCall& a, const PlanArgs& plan, const float* part, int kvh, int first,
-                             int stride) {
+__device__ void merge_tokens(const PagedView& c, const PagedAttentionCall& a, int groups, int blocks, const float* part, int kvh,
+                             int first, int stride) {
     constexpr int DB = D < kMergeDims ? D : kMergeDims, kBlocks = D / DB, kCols = DB / 4, kGroups = 256 / kCols, kAhead = 4;
     __shared__ float4 ov[kGroups][kCols];
     const int lane = threadIdx.x & 63, col = threadIdx.x % kCols, grp = threadIdx.x / kCols;
+    constexpr int kAlign = TokenShape<D, E4M3>::kTile;
     const int64_t size = record_floats(kTokenRows, D);
+    const TokenWalk walk = token_walk(c, a, groups, kAlign);
     Piece t;
     // blocks of kMergeTokenRows rows; the dims of one are dealt out too where its records are many
-    for (int u = first; u < plan.most_blocks * kBlocks && find_piece(c, a, plan, kMergeTokenRows, u / kBlocks, &t); u += stride) {
+    for (int u = first; u < blocks * kBlocks && token_block(c, a, walk, kAlign, kMergeTokenRows, u / kBlocks, &t); u += stride) {
         const int d = u % kBlocks * DB + 4 * col, nr = min(kMergeTokenRows, t.n * a.group - t.row);  // one tile a sequence
-        const float* rec = part + ((int64_t)kvh * plan.items + t.record) * size;
+        const float* base = part + ((int64_t)kvh * 2 * groups + t.record) * size;
+        auto rec = [&](int j) { return base + (2 * j + (j == 0)) * size; };
         if (t.splits <= kMergeWaveSplits) {
             const int i = threadIdx.x >> 6;
             if (u % kBlocks == 0 && i < nr) merge_row<D, E4M3>(c, a, t, kvh, rec, kTokenRows, t.row + i, t.row + i);
@@ -983,27 +1072,27 @@ __device__ void merge_tokens(const PagedView& c, const PagedAttentionCall& a, co
             float m = -INFINITY, l = 0.0f;
             bool bad = false;
             for (int j = lane; j < t.splits; j += 64) {
-                const float x = rec[j * size + r];
+                const float x = rec(j)[r];
                 bad |= x != x;
                 m = fmaxf(m, x);
             }
 #pragma unroll
             for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, kWave));
             for (int j = lane; j < t.splits; j += 64) {
-                const float x = rec[j * size + r];
-                l += x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x - m) * rec[j * size + kTokenRows + r];
+                const float x = rec(j)[r];
+                l += x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x - m) * rec(j)[kTokenRows + r];
             }
             l = wave_sum(l);
             float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            const float* rv = rec + 2 * kTokenRows + r * D + d;
+            const int at = 2 * kTokenRows + r * D + d;
             for (int j0 = grp; j0 < t.splits; j0 += kGroups * kAhead) {
                 float f[kAhead];
                 float4 y[kAhead];
 #pragma unroll
                 for (int k = 0; k < kAhead; ++k) {
                     const int j = min(j0 + k * kGroups, t.splits - 1);
-                    const float x = rec[j * size + r];
-                    y[k] = *reinterpret_cast<const float4*>(rv + j * size);
+                    const float x = rec(j)[r];
+                    y[k] = *reinterpret_cast<const float4*>(rec(j) + at);
                     f[k] = j0 + k * kGroups >= t.splits || x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x - m);
                 }
 #pragma unroll
@@ -1032,24 +1121,26 @@ __device__ void merge_tokens(const PagedView& c, const PagedAttentionCall& a, co
 }
 
 template <int D, bool E4M3>
-__device__ void merge_chunks(const PagedView& c, const PagedAttentionCall& a, const PlanArgs& plan, const float* part, int kvh, int first,
+__device__ void merge_chunks(const PagedView& c, const PagedAttentionCall& a, const ChunkPlan& plan, const float* part, int kvh, int first,
                              int stride) {
     Piece t;
     for (int u = first; u < plan.most_blocks && find_piece(c, a, plan, kMergeChunkRows, u, &t); u += stride) {
-        const float* rec = part + ((int64_t)kvh * plan.items + t.record) * record_floats(kChunkRows, D);
+        const float* base = part + ((int64_t)kvh * plan.items + t.record) * record_floats(kChunkRows, D);
+        auto rec = [&](int j) { return base + j * record_floats(kChunkRows, D); };
         const int rows = min(kMergeChunkRows, t.n * a.group - t.row);
         for (int i = threadIdx.x >> 6; i < rows; i += 4)
             merge_row<D, E4M3>(c, a, t, kvh, rec, kChunkRows, t.row - t.tile * kChunkRows + i, t.row + i);
     }
 }
 
-// The first token_groups workgroups of a KV head merge tokens, the others chunks.
+// The first token_wgs workgroups of a KV head merge tokens (dealt out to token_groups groups, at most token_blocks blocks),
+// the others chunks.
 template <int D, bool E4M3>
-__global__ __launch_bounds__(256) void paged_merge_kernel(PagedView c, PagedAttentionCall a, PlanArgs tokens, PlanArgs chunks, int token_groups,
-                                                          const float* token_part, const float* chunk_part) {
-    const int kvh = blockIdx.x % c.kv_heads, g = blockIdx.x / c.kv_heads, groups = gridDim.x / c.kv_heads;
-    if (g < token_groups) merge_tokens<D, E4M3>(c, a, tokens, token_part, kvh, g, token_groups);
-    else merge_chunks<D, E4M3>(c, a, chunks, chunk_part, kvh, g - token_groups, groups - token_groups);
+__global__ __launch_bounds__(256) void paged_merge_kernel(PagedView c, PagedAttentionCall a, int token_groups, int token_blocks, int token_wgs,
+                                                          ChunkPlan chunks, const float* token_part, const float* chunk_part) {
+    const int kvh = blockIdx.x % c.kv_heads, g = blockIdx.x / c.kv_heads, wgs = gridDim.x / c.kv_heads;
+    if (g < token_wgs) merge_tokens<D, E4M3>(c, a, token_groups, token_blocks, token_part, kvh, g, token_wgs);
+    else merge_chunks<D, E4M3>(c, a, chunks, chunk_part, kvh, g - token_wgs, wgs - token_wgs);
 }
 
 int64_t clamp64(int64_t v, int64_t lo, int64_t hi) { return v < lo ? lo : (v > hi ? hi : v); }
@@ -1062,34 +1153,26 @@ hipError_t launch(const PagedView& c, const PagedAttentionCall& a, hipStream_t s
     const int64_t capacity = (int64_t)c.columns * c.slots;
     // Records of both kernels, which one merge reads: the chunk kernel's behind the token kernel's.
     const int64_t floats = chunks_too ? kPagedPartFloats / 2 : kPagedPartFloats;
-    // Tokens: about four items per CU, and one more for every sequence: fewer leave CUs without work behind the longest (48 ragged
-    // sequences of 16 x 512: 381 us with two, 353), more cost records and starts (64 of 32 x 128, E4M3: 203 us with twelve, 192
-    // with six). Beside chunks the grid is one round: a call without short sequences then loses little.
-    const int64_t resident = (int64_t)ctx->cus * T::kWavesPerSimd;
-    PlanArgs tokens{kTokenRows, kTokenUnit, (int)clamp64(4 * ctx->cus / heads + c.sequences, 1, floats / record_floats(kTokenRows, D) / heads),
-                    1, 0, 0, 0, true};
-    tokens.enough = tokens.items;
-    const int64_t units = (a.window ? std::min<int64_t>(capacity, (int64_t)a.window + a.max_rows + kTokenUnit) : capacity) / kTokenUnit + 1;
     const int64_t sequences = std::min(c.sequences, a.rows);  // with rows
-    // unsplit, an item a sequence; split, within the plan's items
-    tokens.most = (int)std::min<int64_t>(sequences * units, std::max<int64_t>(tokens.items, sequences));
-    tokens.most_blocks = (int)(units > 1 ? std::min<int64_t>((int64_t)a.rows * a.group / kMergeTokenRows + sequences,
-                                                             sequences * std::min<int64_t>(kTokenRows / kMergeTokenRows, (int64_t)a.max_rows * a.group))
-                                         : 0);
-    const int64_t items = std::min<int64_t>(tokens.most, chunks_too ? std::max<int64_t>(1, resident / heads) : tokens.items);
-    hipLaunchKernelGGL((paged_token_kernel<D, E4M3>), dim3((uint32_t)(items * heads)), dim3(256), 0, s, c, a, tokens, ctx->paged_part);
+    // Tokens: a group per workgroup that the device holds, units permitting, so that all end together.
+    const int64_t units = (a.window ? std::min<int64_t>(capacity, (int64_t)a.window + a.max_rows + kTokenUnit) : capacity) / kTokenUnit + 1;
+    const int groups = (int)clamp64(std::min<int64_t>((int64_t)ctx->cus * T::kHeld / heads, sequences * units), 1,
+                                    floats / record_floats(kTokenRows, D) / heads / 2);
+    hipLaunchKernelGGL((paged_token_kernel<D, E4M3>), dim3((uint32_t)(groups * heads)), dim3(256), 0, s, c, a, ctx->paged_part);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    const int64_t merge_tokens = std::min<int64_t>((int64_t)tokens.most_blocks * std::max(1, D / kMergeDims), std::max(1, (chunks_too ? 512 : 2048) / heads));
-    int64_t merge_chunks = 0;
-    PlanArgs chunks{};
+    // blocks of rows of split sequences, at most; each has another group's part
+    int64_t token_blocks = groups > 1 ? std::min<int64_t>((int64_t)a.rows * a.group / kMergeTokenRows + sequences, (int64_t)groups * (kTokenRows / kMergeTokenRows)) : 0;
+    const int64_t token_wgs = std::min<int64_t>(token_blocks * std::max(1, D / kMergeDims), std::max(1, (chunks_too ? 512 : 2048) / heads));
+    int64_t chunk_wgs = 0;
+    ChunkPlan chunks{};
     float* chunk_part = ctx->paged_part + kPagedPartFloats / 2;
     if (chunks_too) {
         // Tiles are split where they leave CUs without work, into about an item per workgroup that the device holds: a split's
         // records cost a write and a read of its rows (35 tiles of 8 heads of 256, window 1024: 193 us in three parts, 167 whole).
         const int64_t records = (int64_t)(kPagedPartFloats / 2) / record_floats(kChunkRows, D) / heads;
         const int64_t tiles = (int64_t)a.rows * a.group / kChunkRows + sequences;
-        chunks = {kChunkRows, kChunkUnit, (int)clamp64((int64_t)ctx->cus * ChunkShape<D, E4M3>::kHeld / heads, 1, records), kChunkMinUnits, 0, 0, 0, false};
+        chunks.items = (int)clamp64((int64_t)ctx->cus * ChunkShape<D, E4M3>::kHeld / heads, 1, records);
         chunks.enough = std::min<int>(chunks.items, std::max(1, ctx->cus * 3 / 4 / heads));
         chunks.most = (int)std::max<int64_t>(chunks.items, tiles);
         // a tile that is split has at least one other item: no more split tiles than items / 2
@@ -1099,11 +1182,11 @@ hipError_t launch(const PagedView& c, const PagedAttentionCall& a, hipStream_t s
                            chunk_part);
         e = hipGetLastError();
         if (e != hipSuccess) return e;
-        merge_chunks = std::min<int64_t>(chunks.most_blocks, std::max(1, 2048 / heads));
+        chunk_wgs = std::min<int64_t>(chunks.most_blocks, std::max(1, 2048 / heads));
     }
-    if (merge_tokens + merge_chunks == 0) return e;
-    hipLaunchKernelGGL((paged_merge_kernel<D, E4M3>), dim3((uint32_t)((merge_tokens + merge_chunks) * heads)), dim3(256), 0, s, c, a, tokens, chunks,
-                       (int)merge_tokens, ctx->paged_part, chunk_part);
+    if (token_wgs + chunk_wgs == 0) return e;
+    hipLaunchKernelGGL((paged_merge_kernel<D, E4M3>), dim3((uint32_t)((token_wgs + chunk_wgs) * heads)), dim3(256), 0, s, c, a, groups,
+                       (int)token_blocks, (int)token_wgs, chunks, ctx->paged_part, chunk_part);
     return hipGetLastError();
 }
 
