@@ -343,7 +343,7 @@ struct TokenShape {
     static constexpr int kElem = E4M3 ? 1 : 2;
     static constexpr int kSub = D * kElem >= 512 ? 1 : 2;                       // 16 positions each: K and V of a tile in 128 registers
     static constexpr int kTile = 16 * kSub;
-    static constexpr int kHeld = D == 512 ? 1 : (D == 256 ? 2 : 3);              // workgroups on a CU: waves per SIMD
+    static constexpr int kHeld = D == 512 ? 1 : 2;                              // workgroups on a CU: waves per SIMD
     static constexpr int kKLoads = D * kElem / 64;                              // 16-byte loads of a K row per lane
     static constexpr int kVD = (E4M3 ? 16 : 8) < D / 16 ? (E4M3 ? 16 : 8) : D / 16;  // dims per V load
     static constexpr int kVB = D / (16 * kVD);                                  // V loads of a row per lane
