@@ -349,7 +349,7 @@ struct TokenShape {
     static constexpr int kVB = D / (16 * kVD);                                  // V loads of a row per lane
     static constexpr int kVWords = kVD * kElem / 4;
     static constexpr int kQStride = D + 8;                                      // LDS row of Q: 16 rows start on 16 bank groups
-    static constexpr int kLds = 16 * kQStride * 2 + 4 * kTokenRows * D * 4;
+    static constexpr int kLds = 16 * kQStride * 2 + 4 * kTokenRows * D * 4 + 2 * 4 * kTokenRows * 4;
 };
 
 template <int W>
@@ -375,17 +375,16 @@ __device__ __forceinline__ uint32_t bf16_pair_of_fp8(uint32_t two) {
 }
 
 template <int D, bool E4M3>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(TokenShape<D, E4M3>::kHeld))) void paged_token_kernel(
-    PagedView c, PagedAttentionCall a, float* part) {
+__device__ __forceinline__ void token_part(const PagedView& c, const PagedAttentionCall& a, float* part, int kvh, int group, int groups,
+                                           uint8_t* lds) {
     using T = TokenShape<D, E4M3>;
     constexpr int NT = T::kSub;
-    __shared__ __attribute__((aligned(16))) uint16_t qs[16 * T::kQStride];
-    __shared__ __attribute__((aligned(16))) float os[4 * kTokenRows * D];
-    __shared__ float ms[4][kTokenRows], ls[4][kTokenRows];
+    uint16_t* qs = reinterpret_cast<uint16_t*>(lds);                           // [16][kQStride]
+    float* os = reinterpret_cast<float*>(lds + 16 * T::kQStride * 2);          // [4 waves][kTokenRows][D]
+    float(*ms)[kTokenRows] = reinterpret_cast<float(*)[kTokenRows]>(os + 4 * kTokenRows * D);
+    float(*ls)[kTokenRows] = ms + 4;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l16 = lane & 15, g = lane >> 4;
-    const int kvh = blockIdx.x % c.kv_heads;
     const float factor = E4M3 ? c.k_scale[kvh] * a.scale_log2 : a.scale_log2;
-    const int groups = gridDim.x / c.kv_heads, group = blockIdx.x / c.kv_heads;
     TokenWalk walk = token_walk(c, a, groups, T::kTile);
     const int64_t end = min(walk.units, (group + 1) * walk.q);
     for (int64_t unit = group * walk.q; unit < end;) {
@@ -599,6 +598,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(TokenShape<
     }
 }
 
+template <int D, bool E4M3>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(TokenShape<D, E4M3>::kHeld))) void paged_token_kernel(
+    PagedView c, PagedAttentionCall a, float* part) {
+    __shared__ __attribute__((aligned(16))) uint8_t lds[TokenShape<D, E4M3>::kLds];
+    token_part<D, E4M3>(c, a, part, blockIdx.x % c.kv_heads, blockIdx.x / c.kv_heads, gridDim.x / c.kv_heads, lds);
+}
+
 // ------------------------------------------------------------------------------------ the chunk kernel
 
 // 128 rows of a sequence (32 per wave) over the positions they see: bound by the matrix cores and LDS. K and V tiles
@@ -624,6 +630,8 @@ struct ChunkShape {
     static constexpr int kLoads = kWaveRows / kRowsPerLoad;     // loads of K (and of V) per wave and tile
     static constexpr int kCodeLoads = kTile * D / 16 / kThreads;     // E4M3: 16-byte loads of K (and V) per thread and tile
     static constexpr int kGroup = 64 / kWaveRows;               // tiles whose positions a wave's lanes look up at once
+    static constexpr int kTileBytes = kTile * kRowBytes;
+    static constexpr int kLds = 4 * kTileBytes + (kPair == 2 ? 8 * 4 * 64 * 16 : 256);
 };
 
 // 16-byte chunk c of LDS row r lies in chunk c ^ swizzle(r): sixteen rows' reads of one chunk, and four rows' reads of four
@@ -662,15 +670,16 @@ __device__ __forceinline__ int lane_here() {
     return v;
 }
 
+// Items first, first + stride, ... of KV head kvh. lds: T::kLds bytes at a multiple of 1024.
 template <int D, bool E4M3>
-__global__ __launch_bounds__((ChunkShape<D, E4M3>::kThreads)) __attribute__((amdgpu_waves_per_eu(2))) void paged_chunk_kernel(
-    PagedView c, PagedAttentionCall a, ChunkPlan plan, float* part) {
+__device__ __forceinline__ void chunk_part(const PagedView& c, const PagedAttentionCall& a, const ChunkPlan& plan, float* part, int kvh, int first,
+                                           int stride, uint8_t* lds_base) {
     using T = ChunkShape<D, E4M3>;
     constexpr int kTile = T::kTile, kPair = T::kPair, kWaves = 4 * kPair, kMine = D / kPair;  // dims of a wave
     constexpr int kSteps = kMine / 16, kDims = kMine / 32;
-    constexpr int kTileBytes = kTile * T::kRowBytes;
-    __shared__ __attribute__((aligned(1024))) uint8_t tiles[4 * kTileBytes];  // two buffers of K and V
-    __shared__ float4 xs[kPair == 2 ? 8 * 4 * 64 : 16];  // pairs: the other wave's half of the scores; flags of the waves
+    constexpr int kTileBytes = T::kTileBytes;
+    uint8_t* tiles = lds_base;                                            // two buffers of K and V
+    float4* xs = reinterpret_cast<float4*>(lds_base + 4 * kTileBytes);    // pairs: the other wave's half of the scores; flags of the waves
     auto any_wave = [&](bool x) {  // whether x holds in any thread; a barrier on both sides
         uint32_t* f = reinterpret_cast<uint32_t*>(xs);
         __syncthreads();
@@ -684,7 +693,6 @@ __global__ __launch_bounds__((ChunkShape<D, E4M3>::kThreads)) __attribute__((amd
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int l32 = lane & 31, hf = lane >> 5;
     const int rg = wave & 3, half = wave >> 2;  // rows 32 rg .., dims half * kMine ..
-    const int kvh = blockIdx.x % c.kv_heads;
     // x = factor (q . k): a negative factor's sign goes to q, so that the largest product is the largest x; and a factor of
     // zero stays above it, so that a product of -inf (a position that a row does not see) stays -inf
     const float signed_factor = E4M3 ? c.k_scale[kvh] * a.scale_log2 : a.scale_log2;
@@ -700,7 +708,7 @@ __global__ __launch_bounds__((ChunkShape<D, E4M3>::kThreads)) __attribute__((amd
         return r * T::kRowBytes + ((2 * (ln >> 4 & 1) + (ln >> 1 & 1)) ^ chunk_swizzle<D>(r)) * 16 + (ln & 1) * 8;
     };
     Piece t;
-    for (int item = blockIdx.x / c.kv_heads; item < plan.most && find_piece(c, a, plan, 0, item, &t); item += gridDim.x / c.kv_heads) {
+    for (int item = first; item < plan.most && find_piece(c, a, plan, 0, item, &t); item += stride) {
         const int r0 = t.tile * kChunkRows, nr = (int)min((int64_t)kChunkRows, (int64_t)t.n * a.group - r0);
         const Span span = span_of(a, t, r0, r0 + nr - 1, kTile);
         const int lo = span.lo, hi = span.hi;
@@ -992,6 +1000,29 @@ __global__ __launch_bounds__((ChunkShape<D, E4M3>::kThreads)) __attribute__((amd
     }
 }
 
+// Chunks, and up to 256 dims the token rows beside them: a workgroup of either kind fits a CU next to one of the other, the
+// one bound by memory, the other by arithmetic. `stripe` groups in a row (a KV head's share of one workgroup per CU) are
+// chunks', the next tokens', until the token groups are used up. (30 single tokens and 5 chunks of 8 heads of 256, window 1024:
+// XXX us in two launches, XXX in one.)
+template <int D, bool E4M3>
+__global__ __launch_bounds__((ChunkShape<D, E4M3>::kThreads)) __attribute__((amdgpu_waves_per_eu(2))) void paged_chunk_kernel(
+    PagedView c, PagedAttentionCall a, ChunkPlan plan, int token_groups, int stripe, float* token_records, float* chunk_records) {
+    using T = ChunkShape<D, E4M3>;
+    constexpr int kLds = T::kPair == 1 && TokenShape<D, E4M3>::kLds > T::kLds ? TokenShape<D, E4M3>::kLds : T::kLds;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[kLds];
+    const int kvh = blockIdx.x % c.kv_heads, g = blockIdx.x / c.kv_heads, groups = gridDim.x / c.kv_heads;
+    int tokens_before = 0;
+    if constexpr (T::kPair == 1) {
+        const int row = g / stripe, at = g - row * stripe, tokens = row / 2 * stripe + (row & 1 ? at : 0);
+        if ((row & 1) && tokens < token_groups) {
+            token_part<D, E4M3>(c, a, token_records, kvh, tokens, token_groups, lds);
+            return;
+        }
+        tokens_before = min(tokens, token_groups);
+    }
+    chunk_part<D, E4M3>(c, a, plan, chunk_records, kvh, g - tokens_before, groups - (T::kPair == 1 ? token_groups : 0), lds);
+}
+
 // ------------------------------------------------------------------------------------------- the merge
 
 // Rows of split tiles, both kernels' in one launch. A workgroup takes a block of rows of a tile and finds it once. Few
@@ -1154,19 +1185,24 @@ hipError_t launch(const PagedView& c, const PagedAttentionCall& a, hipStream_t s
     // Records of both kernels, which one merge reads: the chunk kernel's behind the token kernel's.
     const int64_t floats = chunks_too ? kPagedPartFloats / 2 : kPagedPartFloats;
     const int64_t sequences = std::min(c.sequences, a.rows);  // with rows
-    // Tokens: a group per workgroup that the device holds, units permitting, so that all end together.
+    // Tokens: a group per workgroup that the device holds (beside chunks in one launch: per CU), units permitting, so that all
+    // end together.
+    const bool one_launch = chunks_too && ChunkShape<D, E4M3>::kPair == 1;
     const int64_t units = (a.window ? std::min<int64_t>(capacity, (int64_t)a.window + a.max_rows + kTokenUnit) : capacity) / kTokenUnit + 1;
-    const int groups = (int)clamp64(std::min<int64_t>((int64_t)ctx->cus * T::kHeld / heads, sequences * units), 1,
+    const int groups = (int)clamp64(std::min<int64_t>((int64_t)ctx->cus * (one_launch ? 1 : T::kHeld) / heads, sequences * units), 1,
                                     floats / record_floats(kTokenRows, D) / heads / 2);
-    hipLaunchKernelGGL((paged_token_kernel<D, E4M3>), dim3((uint32_t)(groups * heads)), dim3(256), 0, s, c, a, ctx->paged_part);
-    hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
+    hipError_t e = hipSuccess;
+    if (!one_launch) {
+        hipLaunchKernelGGL((paged_token_kernel<D, E4M3>), dim3((uint32_t)(groups * heads)), dim3(256), 0, s, c, a, ctx->paged_part);
+        e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
     // blocks of rows of split sequences, at most; each has another group's part
     int64_t token_blocks = groups > 1 ? std::min<int64_t>((int64_t)a.rows * a.group / kMergeTokenRows + sequences, (int64_t)groups * (kTokenRows / kMergeTokenRows)) : 0;
     const int64_t token_wgs = std::min<int64_t>(token_blocks * std::max(1, D / kMergeDims), std::max(1, (chunks_too ? 512 : 2048) / heads));
     int64_t chunk_wgs = 0;
     ChunkPlan chunks{};
-    float* chunk_part = ctx->paged_part + kPagedPartFloats / 2;
+    float* chunk_records = ctx->paged_part + kPagedPartFloats / 2;
     if (chunks_too) {
         // Tiles are split where they leave CUs without work, into about an item per workgroup that the device holds: a split's
         // records cost a write and a read of its rows (35 tiles of 8 heads of 256, window 1024: 193 us in three parts, 167 whole).
@@ -1177,16 +1213,16 @@ hipError_t launch(const PagedView& c, const PagedAttentionCall& a, hipStream_t s
         chunks.most = (int)std::max<int64_t>(chunks.items, tiles);
         // a tile that is split has at least one other item: no more split tiles than items / 2
         chunks.most_blocks = chunks.items / 2 * (kChunkRows / kMergeChunkRows);
-        const int64_t grid = std::min<int64_t>(chunks.most, std::max(1, 65536 / heads));
+        const int64_t grid = std::min<int64_t>(chunks.most, std::max(1, 65536 / heads)) + (one_launch ? groups : 0);
         hipLaunchKernelGGL((paged_chunk_kernel<D, E4M3>), dim3((uint32_t)(grid * heads)), dim3(ChunkShape<D, E4M3>::kThreads), 0, s, c, a, chunks,
-                           chunk_part);
+                           groups, std::max(1, ctx->cus / heads), ctx->paged_part, chunk_records);
         e = hipGetLastError();
         if (e != hipSuccess) return e;
         chunk_wgs = std::min<int64_t>(chunks.most_blocks, std::max(1, 2048 / heads));
     }
     if (token_wgs + chunk_wgs == 0) return e;
     hipLaunchKernelGGL((paged_merge_kernel<D, E4M3>), dim3((uint32_t)((token_wgs + chunk_wgs) * heads)), dim3(256), 0, s, c, a, groups,
-                       (int)token_blocks, (int)token_wgs, chunks, ctx->paged_part, chunk_part);
+                       (int)token_blocks, (int)token_wgs, chunks, ctx->paged_part, chunk_records);
     return hipGetLastError();
 }
 
