@@ -149,16 +149,16 @@ __device__ bool token_block(const PagedView& c, const PagedAttentionCall& a, con
     return false;
 }
 
-// Chunks: a sequence of r = n * group rows has ceil(r / kChunkRows) tiles, each split over ceil(units / c) items, where units
-// covers the positions a tile can see in steps of kChunkUnit, and c, at least kChunkMinUnits, is chosen so that all
-// sequences together have at most `items` items per KV head (a call with `enough` tiles splits none). The last tiles of
-// a sequence, which see the most, come first.
+// Chunks: a sequence of r = n * group rows has ceil(r / kChunkRows) tiles; U is the sum over all tiles of the positions they
+// see, in units of kChunkUnit. A tile of more units than twice an even share, per = 2 U / items, but at least kChunkMinUnits, is
+// split into ceil(units / per) parts, which leave records for the merge: all split tiles together at most 2 U / per <= items
+// of them. (A part costs a write and a read of its rows: 35 tiles of 8 heads of 256, window 1024, took 193 us in three parts
+// each and 167 whole.) The last tiles of a sequence, which see the most, come first.
 constexpr int kChunkRows = 128;
 constexpr int kChunkUnit = 64;
 constexpr int kChunkMinUnits = 4;
 struct ChunkPlan {
-    int items;
-    int enough;       // with this many tiles or more, none is split
+    int items;        // per KV head: workgroups that the device holds; records
     int most;         // no call has more items than this
     int most_blocks;  // nor more blocks of rows to merge
 };
@@ -186,23 +186,23 @@ __device__ bool find_piece(const PagedView& c, const PagedAttentionCall& a, cons
     raise_bad(c, bad);
     tiles = wave_total(tiles);  // at most 2^20 rows * 128 heads / kChunkRows, and one per sequence
     if (tiles == 0) return false;
-    // sum of ceil(units / per) <= units / per + tiles <= items. The float sum is rounded the same in every wave, and
-    // short by at most 1024 + 8 roundings of 2^-24: a part in ten thousand more covers them.
+    // The float sum is rounded the same in every wave, and short by at most 1024 + 8 roundings of 2^-24: a part in ten
+    // thousand more covers them.
     units = wave_sum(units);
-    int per = 1 << 30;
-    if (tiles < p.enough) per = max(kChunkMinUnits, (int)fminf(units * 1.0001f / (float)(p.items - tiles) + 1.0f, 1e9f));
-    int items_before = 0, blocks_before = 0;
+    const int per = max(kChunkMinUnits, (int)fminf(2.0001f * units / (float)p.items + 1.0f, 1e9f));
+    int items_before = 0, blocks_before = 0, records_before = 0;
     for (int base = 0; base < c.sequences; base += 64) {
         if (c.sequences > 64) q = seq_of(c, a, base + lane, false, &bad);
         const int splits = q.n ? (units_of(q) + per - 1) / per : 0, items = tiles_of(q) * splits;
         const int blocks = merge_rows && splits > 1 ? (q.n * a.group + merge_rows - 1) / merge_rows : 0;
-        const int xi = scan_sum(items), xb = merge_rows ? scan_sum(blocks) : 0;
+        const int records = splits > 1 ? items : 0, xr = scan_sum(records);
+        const int xi = merge_rows ? 0 : scan_sum(items), xb = merge_rows ? scan_sum(blocks) : 0;
         const uint64_t hit = __ballot((merge_rows ? blocks_before + xb : items_before + xi) > want);
         if (hit) {
             const int l = __builtin_ctzll(hit);
             auto get = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
             *out = {base + l, get(q.row0), get(q.n), get(q.len), 0, 0, get(splits), 0, 0};
-            const int last = get(tiles_of(q)) - 1, first_item = items_before + get(xi - items);
+            const int last = get(tiles_of(q)) - 1;
             int j;  // the tile's place, the last tile first
             if (merge_rows) {
                 const int k = want - blocks_before - get(xb - blocks);
@@ -215,9 +215,10 @@ __device__ bool find_piece(const PagedView& c, const PagedAttentionCall& a, cons
                 out->tile = last - j;
                 out->split = k - j * out->splits;
             }
-            out->record = first_item + j * out->splits;
+            out->record = records_before + get(xr - records) + j * out->splits;
             return true;
         }
+        records_before += __builtin_amdgcn_readlane(xr, 63);
         items_before += __builtin_amdgcn_readlane(xi, 63);
         blocks_before += __builtin_amdgcn_readlane(xb, 63);
     }
@@ -1204,14 +1205,11 @@ hipError_t launch(const PagedView& c, const PagedAttentionCall& a, hipStream_t s
     ChunkPlan chunks{};
     float* chunk_records = ctx->paged_part + kPagedPartFloats / 2;
     if (chunks_too) {
-        // Tiles are split where they leave CUs without work, into about an item per workgroup that the device holds: a split's
-        // records cost a write and a read of its rows (35 tiles of 8 heads of 256, window 1024: 193 us in three parts, 167 whole).
         const int64_t records = (int64_t)(kPagedPartFloats / 2) / record_floats(kChunkRows, D) / heads;
         const int64_t tiles = (int64_t)a.rows * a.group / kChunkRows + sequences;
         chunks.items = (int)clamp64((int64_t)ctx->cus * ChunkShape<D, E4M3>::kHeld / heads, 1, records);
-        chunks.enough = std::min<int>(chunks.items, std::max(1, ctx->cus * 3 / 4 / heads));
-        chunks.most = (int)std::max<int64_t>(chunks.items, tiles);
-        // a tile that is split has at least one other item: no more split tiles than items / 2
+        chunks.most = (int)(tiles + chunks.items);
+        // a split tile has two records at least
         chunks.most_blocks = chunks.items / 2 * (kChunkRows / kMergeChunkRows);
         const int64_t grid = std::min<int64_t>(chunks.most, std::max(1, 65536 / heads)) + (one_launch ? groups : 0);
         hipLaunchKernelGGL((paged_chunk_kernel<D, E4M3>), dim3((uint32_t)(grid * heads)), dim3(ChunkShape<D, E4M3>::kThreads), 0, s, c, a, chunks,
