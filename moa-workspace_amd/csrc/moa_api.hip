@@ -91,7 +91,8 @@ DevCtx* device_context(hipError_t* err) {
     const size_t t_attn = carve(sizeof(float) * kAttnPartFloats);
     const size_t t_fattn = carve(sizeof(float) * kFattnPartFloats);
     const size_t t_plist = carve(sizeof(int32_t) * (2 * (size_t)kPagedMaxPages + 16));
-    const size_t t_ppart = carve(sizeof(float) * kPagedPartFloats);
+    const size_t t_ptok = carve(sizeof(float) * kPagedTokenFloats);
+    const size_t t_pchunk = carve(sizeof(float) * kPagedChunkFloats);
     int cus = 0;
     *err = hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev);
     if (*err != hipSuccess) return nullptr;
@@ -122,7 +123,8 @@ DevCtx* device_context(hipError_t* err) {
     c.attn_part = reinterpret_cast<float*>(b + t_attn);
     c.fattn_part = reinterpret_cast<float*>(b + t_fattn);
     c.paged_list = reinterpret_cast<int32_t*>(b + t_plist);
-    c.paged_part = reinterpret_cast<float*>(b + t_ppart);
+    c.paged_tokens = reinterpret_cast<float*>(b + t_ptok);
+    c.paged_chunks = reinterpret_cast<float*>(b + t_pchunk);
     c.base = base;
     return &c;
 }

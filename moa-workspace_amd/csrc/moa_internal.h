@@ -70,12 +70,13 @@ constexpr int kOfnCopies = 8;  // copies of O's post-norm words in the single-la
 // one per block of down partial sums, one per normalised row.
 constexpr int kRowsFlagWords = 512;
 
-// The paged cache (moa_paged.hip): page lists and moves, and the split attention's records, f32
-// [16 or 128 query rows][max, sum, out[head_dim]] each: 160 MB, half of it for each kernel of a call that has both,
-// room for 318 records of 128 rows of 512 dims.
+// The paged cache (moa_paged.hip): page lists and moves, and the split attention's records, f32 [16 or 128 query rows]
+// [max, sum, out[head_dim]] each. Tokens: two records per workgroup that the device holds (256 CUs: 17 MB with 256 or 512
+// dims); chunks: one (68 MB). Fewer fit where a CU count or head count asks for more: the work is then split less.
 constexpr int kPagedMaxPages = 1 << 20;
 constexpr int kPagedMaxSequences = 1 << 16;
-constexpr size_t kPagedPartFloats = 40 << 20;
+constexpr size_t kPagedTokenFloats = (size_t)9 << 19;   // 18.9 MB
+constexpr size_t kPagedChunkFloats = (size_t)17 << 20;  // 71.3 MB
 
 // Device-side error bits (OR-ed by kernels; read back by moa_device_errors()).
 constexpr uint32_t kErrRopeOffset = 1u;
@@ -102,7 +103,8 @@ struct DevCtx {
     float* attn_part = nullptr;   // sliding_attention split partials (kAttnPartFloats)
     float* fattn_part = nullptr;  // full-attention page partials (kFattnPartFloats)
     int32_t* paged_list = nullptr;  // 2 * kPagedMaxPages + 16: page lists of a cache call, its result word
-    float* paged_part = nullptr;    // paged attention's split records (kPagedPartFloats)
+    float* paged_tokens = nullptr;  // paged attention's split records (kPagedTokenFloats, kPagedChunkFloats)
+    float* paged_chunks = nullptr;
     void* base = nullptr;
     int cus = 0;                  // compute units of the device
     int8_t ffn_fused[6] = {-1, -1, -1, -1, -1, -1};  // per (format, scale kind): grid fits resident? (-1 unknown)

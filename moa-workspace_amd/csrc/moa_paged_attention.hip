@@ -94,9 +94,16 @@ __device__ __forceinline__ int token_units(const PagedAttentionCall& a, const Se
 __device__ TokenWalk token_walk(const PagedView& c, const PagedAttentionCall& a, int groups, int align) {
     TokenWalk w = {0, 1, 0, 0};
     bool bad = false;
-    for (int base = 0; base < c.sequences; base += 64)  // 64 sequences have at most 64 * 2^23 units
-        w.units += wave_total(token_units(a, seq_of(c, a, base + (threadIdx.x & 63), true, &bad), align));
+#pragma unroll 4
+    for (int base = 0; base < c.sequences; base += 64)
+        w.units += token_units(a, seq_of(c, a, base + (threadIdx.x & 63), true, &bad), align);
     raise_bad(c, bad);
+    if (c.sequences <= 64) {  // at most 64 * 2^23 units
+        w.units = wave_total((int)w.units);
+    } else {
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) w.units += __shfl_xor((long long)w.units, o, kWave);
+    }
     // (a 64-bit quotient costs a microsecond; real calls have far fewer units)
     w.q = w.units >> 31 ? (w.units + groups - 1) / groups : ((uint32_t)w.units + (uint32_t)groups - 1) / (uint32_t)groups;
     w.q = w.q ? w.q : 1;
@@ -1004,7 +1011,7 @@ __device__ __forceinline__ void chunk_part(const PagedView& c, const PagedAttent
 // Chunks, and up to 256 dims the token rows beside them: a workgroup of either kind fits a CU next to one of the other, the
 // one bound by memory, the other by arithmetic. `stripe` groups in a row (a KV head's share of one workgroup per CU) are
 // chunks', the next tokens', until the token groups are used up. (30 single tokens and 5 chunks of 8 heads of 256, window 1024:
-// XXX us in two launches, XXX in one.)
+// 144 us in two launches, 112 in one.)
 template <int D, bool E4M3>
 __global__ __launch_bounds__((ChunkShape<D, E4M3>::kThreads)) __attribute__((amdgpu_waves_per_eu(2))) void paged_chunk_kernel(
     PagedView c, PagedAttentionCall a, ChunkPlan plan, int token_groups, int stripe, float* token_records, float* chunk_records) {
@@ -1183,18 +1190,16 @@ hipError_t launch(const PagedView& c, const PagedAttentionCall& a, hipStream_t s
     const int heads = c.kv_heads;
     const bool chunks_too = (int64_t)a.max_rows * a.group > kTokenRows;
     const int64_t capacity = (int64_t)c.columns * c.slots;
-    // Records of both kernels, which one merge reads: the chunk kernel's behind the token kernel's.
-    const int64_t floats = chunks_too ? kPagedPartFloats / 2 : kPagedPartFloats;
     const int64_t sequences = std::min(c.sequences, a.rows);  // with rows
     // Tokens: a group per workgroup that the device holds (beside chunks in one launch: per CU), units permitting, so that all
     // end together.
     const bool one_launch = chunks_too && ChunkShape<D, E4M3>::kPair == 1;
     const int64_t units = (a.window ? std::min<int64_t>(capacity, (int64_t)a.window + a.max_rows + kTokenUnit) : capacity) / kTokenUnit + 1;
     const int groups = (int)clamp64(std::min<int64_t>((int64_t)ctx->cus * (one_launch ? 1 : T::kHeld) / heads, sequences * units), 1,
-                                    floats / record_floats(kTokenRows, D) / heads / 2);
+                                    (int64_t)kPagedTokenFloats / record_floats(kTokenRows, D) / heads / 2);
     hipError_t e = hipSuccess;
     if (!one_launch) {
-        hipLaunchKernelGGL((paged_token_kernel<D, E4M3>), dim3((uint32_t)(groups * heads)), dim3(256), 0, s, c, a, ctx->paged_part);
+        hipLaunchKernelGGL((paged_token_kernel<D, E4M3>), dim3((uint32_t)(groups * heads)), dim3(256), 0, s, c, a, ctx->paged_tokens);
         e = hipGetLastError();
         if (e != hipSuccess) return e;
     }
@@ -1203,9 +1208,8 @@ hipError_t launch(const PagedView& c, const PagedAttentionCall& a, hipStream_t s
     const int64_t token_wgs = std::min<int64_t>(token_blocks * std::max(1, D / kMergeDims), std::max(1, (chunks_too ? 512 : 2048) / heads));
     int64_t chunk_wgs = 0;
     ChunkPlan chunks{};
-    float* chunk_records = ctx->paged_part + kPagedPartFloats / 2;
     if (chunks_too) {
-        const int64_t records = (int64_t)(kPagedPartFloats / 2) / record_floats(kChunkRows, D) / heads;
+        const int64_t records = (int64_t)kPagedChunkFloats / record_floats(kChunkRows, D) / heads;
         const int64_t tiles = (int64_t)a.rows * a.group / kChunkRows + sequences;
         chunks.items = (int)clamp64((int64_t)ctx->cus * ChunkShape<D, E4M3>::kHeld / heads, 1, records);
         chunks.most = (int)(tiles + chunks.items);
@@ -1213,14 +1217,14 @@ hipError_t launch(const PagedView& c, const PagedAttentionCall& a, hipStream_t s
         chunks.most_blocks = chunks.items / 2 * (kChunkRows / kMergeChunkRows);
         const int64_t grid = std::min<int64_t>(chunks.most, std::max(1, 65536 / heads)) + (one_launch ? groups : 0);
         hipLaunchKernelGGL((paged_chunk_kernel<D, E4M3>), dim3((uint32_t)(grid * heads)), dim3(ChunkShape<D, E4M3>::kThreads), 0, s, c, a, chunks,
-                           groups, std::max(1, ctx->cus / heads), ctx->paged_part, chunk_records);
+                           groups, std::max(1, ctx->cus / heads), ctx->paged_tokens, ctx->paged_chunks);
         e = hipGetLastError();
         if (e != hipSuccess) return e;
         chunk_wgs = std::min<int64_t>(chunks.most_blocks, std::max(1, 2048 / heads));
     }
     if (token_wgs + chunk_wgs == 0) return e;
     hipLaunchKernelGGL((paged_merge_kernel<D, E4M3>), dim3((uint32_t)((token_wgs + chunk_wgs) * heads)), dim3(256), 0, s, c, a, groups,
-                       (int)token_blocks, (int)token_wgs, chunks, ctx->paged_part, chunk_records);
+                       (int)token_blocks, (int)token_wgs, chunks, ctx->paged_tokens, ctx->paged_chunks);
     return hipGetLastError();
 }
 
