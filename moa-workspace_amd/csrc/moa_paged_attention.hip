@@ -316,15 +316,16 @@ __device__ __forceinline__ Span span_of(const PagedAttentionCall& a, const Piece
     return {(int)min((int64_t)hi, lo + from), (int)min((int64_t)hi, lo + to)};
 }
 
-// The careful path for a piece's rows [r0, r0 + nr) over positions [lo, hi), waves taking rows in turn.
-template <bool E4M3>
-__device__ void careful_piece(const PagedView& c, const PagedAttentionCall& a, const Piece& t, int kvh, int r0, int nr, int lo, int hi,
+// The careful path for a piece's rows [r0, r0 + nr) over positions [lo, hi), waves taking rows in turn. q(r, row): where row
+// r0 + r's query lies, not in `out` once that is written (out may be q).
+template <bool E4M3, class Q>
+__device__ void careful_piece(const PagedView& c, const PagedAttentionCall& a, const Piece& t, int kvh, int r0, int nr, int lo, int hi, Q q,
                               float* rec, int bm) {
     const int lane = threadIdx.x & 63, per = c.head_dim / 64;
     for (int r = threadIdx.x >> 6; r < nr; r += blockDim.x >> 6) {
         const Row x = row_of(a, t, kvh, r0 + r);
         float o[8], mx, sum;
-        careful_row<E4M3>(c, a.q + x.m * a.q_row + x.h * c.head_dim, t.s, kvh, E4M3 ? c.k_scale[kvh] * a.scale_log2 : a.scale_log2,
+        careful_row<E4M3>(c, q(r, x), t.s, kvh, E4M3 ? c.k_scale[kvh] * a.scale_log2 : a.scale_log2,
                           max(lo, x.lo), min(hi, x.hi), &mx, &sum, o);
         if (rec) {
             if (lane == 0) rec[r] = mx, rec[bm + r] = sum;
@@ -602,7 +603,7 @@ __device__ __forceinline__ void token_part(const PagedView& c, const PagedAttent
         }
         odd = __syncthreads_or(odd);
         if (bad && threadIdx.x == 0) atomicOr(c.err, kErrPaged);
-        if (odd && !bad) careful_piece<E4M3>(c, a, t, kvh, 0, nr, lo, hi, rec, kTokenRows);
+        if (odd && !bad) careful_piece<E4M3>(c, a, t, kvh, 0, nr, lo, hi, [&](int r, const Row&) { return qs + r * T::kQStride; }, rec, kTokenRows);
     }
 }
 
@@ -688,15 +689,15 @@ __device__ __forceinline__ void chunk_part(const PagedView& c, const PagedAttent
     constexpr int kTileBytes = T::kTileBytes;
     uint8_t* tiles = lds_base;                                            // two buffers of K and V
     float4* xs = reinterpret_cast<float4*>(lds_base + 4 * kTileBytes);    // pairs: the other wave's half of the scores; flags of the waves
-    auto any_wave = [&](bool x) {  // whether x holds in any thread; a barrier on both sides
+    auto any_wave = [&](bool x, bool y) {  // bit 0: x holds in some thread of the workgroup, bit 1: y does
         uint32_t* f = reinterpret_cast<uint32_t*>(xs);
         __syncthreads();
-        if ((threadIdx.x & 63) == 0) f[threadIdx.x >> 6] = 0;
-        if (__any(x)) f[threadIdx.x >> 6] = 1;
+        const uint32_t mine = (__any(x) ? 1u : 0u) | (__any(y) ? 2u : 0u);
+        if ((threadIdx.x & 63) == 0) f[threadIdx.x >> 6] = mine;
         __syncthreads();
         uint32_t r = 0;
         for (int w = 0; w < kWaves; ++w) r |= f[w];
-        return r != 0;
+        return r;
     };
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int l32 = lane & 31, hf = lane >> 5;
@@ -972,17 +973,17 @@ __device__ __forceinline__ void chunk_part(const PagedView& c, const PagedAttent
         }
 
         l_run += __shfl_xor(l_run, 32);
-        bad = any_wave(bad);
+        float most = 0.0f;
+#pragma unroll
+        for (int d = 0; d < kDims; ++d)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) most += fabsf(o[d][e]);
+        const uint32_t flags = any_wave(bad, wrow < nr && !(most < INFINITY));
+        bad = flags & 1;
+        const bool odd = flags & 2;  // the careful path writes, and reads q, which may be out
         float* rec = t.splits > 1 ? part + ((int64_t)kvh * plan.items + t.record + t.split) * record_floats(kChunkRows, D) : nullptr;
         const float inv = l_run == 0.0f ? 0.0f : (E4M3 ? c.v_scale[kvh] : 1.0f) / l_run;
-        bool odd = false;
-        if (wrow < nr) {
-            float most = 0.0f;
-#pragma unroll
-            for (int d = 0; d < kDims; ++d)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) most += fabsf(o[d][e]);
-            odd = !(most < INFINITY);
+        if (wrow < nr && (bad || !odd)) {
             const int first = half * kMine + 4 * hf;  // of the lane's dims: first + 32 d + 2 e .. + 3
             if (rec) {
                 float* to = rec + 2 * kChunkRows + wrow * D + first;
@@ -1002,9 +1003,8 @@ __device__ __forceinline__ void chunk_part(const PagedView& c, const PagedAttent
             }
             if (rec && hf == 0 && half == 0) rec[wrow] = bad ? NAN : m_ref, rec[kChunkRows + wrow] = l_run;
         }
-        odd = any_wave(odd);
         if (bad && threadIdx.x == 0) atomicOr(c.err, kErrPaged);
-        if (odd && !bad) careful_piece<E4M3>(c, a, t, kvh, r0, nr, lo, hi, rec, kChunkRows);
+        if (odd && !bad) careful_piece<E4M3>(c, a, t, kvh, r0, nr, lo, hi, [&](int, const Row& x) { return a.q + x.m * a.q_row + x.h * D; }, rec, kChunkRows);
     }
 }
 
@@ -1061,7 +1061,7 @@ __device__ __forceinline__ void merge_row(const PagedView& c, const PagedAttenti
 #pragma unroll
         for (int k = 0; k < kAhead; ++k) {
             const float* at = rec(min(j0 + k, t.splits - 1));
-            x[k] = j0 + k < t.splits ? at[r] : -INFINITY;
+            x[k] = at[r];
             y[k] = at[bm + r];
             const float* o = at + 2 * bm + r * D + lane * kPer;
 #pragma unroll
@@ -1069,8 +1069,9 @@ __device__ __forceinline__ void merge_row(const PagedView& c, const PagedAttenti
         }
 #pragma unroll
         for (int k = 0; k < kAhead; ++k) {
+            if (j0 + k >= t.splits) continue;
+            // (a record of no weight counts too: sums that are NaN for a row's own values make the row NaN)
             const float f = x[k] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x[k] - m);
-            if (f == 0.0f) continue;  // its sums may be anything
             l = fmaf(f, y[k], l);
 #pragma unroll
             for (int i = 0; i < kPer; ++i) v[i] = fmaf(f, w[k][i], v[i]);
@@ -1119,7 +1120,7 @@ __device__ void merge_tokens(const PagedView& c, const PagedAttentionCall& a, in
             for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, kWave));
             for (int j = lane; j < t.splits; j += 64) {
                 const float x = rec(j)[r];
-                l += x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x - m) * rec(j)[kTokenRows + r];
+                l = fmaf(x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x - m), rec(j)[kTokenRows + r], l);
             }
             l = wave_sum(l);
             float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -1132,11 +1133,11 @@ __device__ void merge_tokens(const PagedView& c, const PagedAttentionCall& a, in
                     const int j = min(j0 + k * kGroups, t.splits - 1);
                     const float x = rec(j)[r];
                     y[k] = *reinterpret_cast<const float4*>(rec(j) + at);
-                    f[k] = j0 + k * kGroups >= t.splits || x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x - m);
+                    f[k] = x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x - m);
                 }
 #pragma unroll
                 for (int k = 0; k < kAhead; ++k)
-                    if (f[k] != 0.0f) {
+                    if (j0 + k * kGroups < t.splits) {
                         v.x = fmaf(f[k], y[k].x, v.x), v.y = fmaf(f[k], y[k].y, v.y);
                         v.z = fmaf(f[k], y[k].z, v.z), v.w = fmaf(f[k], y[k].w, v.w);
                     }

@@ -721,3 +721,54 @@ def test_calls_of_one_process_repeat_their_bits():
             ops.paged_attention(q, st.cache, i32(starts_of(rows)), o, max_rows=max(rows))
             attend(st, [1, 0, 0], 16)
         assert torch.equal(*outs)
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "e4m3"])
+@pytest.mark.parametrize("n,heads,dim", [(2, 8, 256), (4, 2, 128), (1, 1, 512), (90, 2, 128), (40, 1, 512)])
+def test_in_place_beside_values_that_a_row_does_not_see(n, heads, dim, fmt):
+    """out = q, one short sequence (nothing to merge), V of the last token NaN: the rows before it are right."""
+    need_gpu()
+    say(f"paged attention in place, non-finite last token, {n} rows of {heads} x {dim} {fmt}")
+    length = 100
+    st = Setup([length], 16, heads, dim, fmt, seed=21)
+    clean_k, clean_v = (t.clone() for t in st.values())
+    sc = (None, None) if st.k_scale is None else (st.k_scale[0], st.v_scale[0])
+    at = length if n == 1 else length - 1  # of a single token, what lies behind the sequence
+    page, slot = st.state.table[0][at // 16], at % 16
+    (st.v if fmt == "bf16" else st.v.view(torch.uint8))[0, page, slot] = float("nan") if fmt == "bf16" else 0x7F
+    q = queries(n, 4 * heads, dim, 22)
+    want, a, d = pm.attention(q, clean_k, clean_v, st.state.table, [length], [0, n], 16, 0, 1.0, *sc)
+    ops.paged_attention(q, st.cache, i32([0, n]), q)
+    assert ops.device_errors() == 0
+    check_rows(q, want, a, d, dim, slice(0, n - 1 if n > 1 else 1))
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "e4m3"])
+@pytest.mark.parametrize("n,length", [(1, 9000), (4, 9000), (90, 9000), (1, 120000), (40, 100), (3, 100)])
+def test_nan_that_a_row_sees_makes_it_nan(n, length, fmt):
+    """A query that is NaN gives a NaN row, and so does a visible key or value, split or not; other rows are unharmed."""
+    need_gpu()
+    say(f"paged attention, visible NaN, {n} rows over {length} positions {fmt}")
+    st = Setup([length], 64, 2, 128, fmt, seed=23)
+    sc = (None, None) if st.k_scale is None else (st.k_scale[0], st.v_scale[0])
+    q = queries(n, 8, 128, 24)
+    want, a, d = pm.attention(q, *st.values(), st.state.table, [length], [0, n], 64, 0, 1.0, *sc)
+    out = torch.zeros_like(q)
+    sick = q.clone()
+    sick[n // 2, 5] = float("nan")
+    ops.paged_attention(sick, st.cache, i32([0, n]), out)
+    assert ops.device_errors() == 0
+    assert torch.isnan(out[n // 2, 5].float()).all()
+    well = torch.ones((n, 8), dtype=torch.bool, device=DEV)
+    well[n // 2, 5] = False
+    check_rows(out[well], want[well], a[well], d[well], 128)
+    page, slot = st.state.table[0][17 // 64], 17
+    for t in (st.k, st.v):  # one position, far from where the largest scores may lie
+        view = t if fmt == "bf16" else t.view(torch.uint8)
+        old = view[0, page, slot].clone()
+        view[0, page, slot, 1, 3] = float("nan") if fmt == "bf16" else 0x7F
+        ops.paged_attention(q, st.cache, i32([0, n]), out)
+        assert ops.device_errors() == 0
+        assert torch.isnan(out[:, 4:, 3].float()).all(), "K" if t is st.k else "V"
+        check_rows(out[:, :4], want[:, :4], a[:, :4], d[:, :4], 128)
+        view[0, page, slot] = old
