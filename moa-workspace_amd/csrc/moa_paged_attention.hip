@@ -170,64 +170,75 @@ struct ChunkPlan {
     int most_blocks;  // nor more blocks of rows to merge
 };
 
-// Finds piece `want` by one wave: an item (merge_rows = 0), or block `want` of merge_rows rows of the tiles that are split.
-// False: there are not that many.
-__device__ bool find_piece(const PagedView& c, const PagedAttentionCall& a, const ChunkPlan& p, int merge_rows, int want, Piece* out) {
-    const int lane = threadIdx.x & 63;
-    // tiles of a sequence, and the units that a tile's rows see: all, or the window and the tile's tokens
-    auto tiles_of = [&](const Seq& q) { return (q.n * a.group + kChunkRows - 1) / kChunkRows; };
-    auto units_of = [&](const Seq& q) {
-        const int span = min(q.n, (kChunkRows + a.group - 1) / a.group + 1);
-        const int seen = a.window ? min(q.len, a.window + span - 1 + kChunkUnit) : q.len;
-        return max(1, (seen + kChunkUnit - 1) / kChunkUnit);
-    };
+// A walk over the sequences' pieces in ascending order, by one wave: items (merge_rows = 0), or blocks of merge_rows rows of the
+// tiles that are split.
+struct ChunkWalk {
+    int per;                          // units of a part; 0: the call has no chunks
+    int base, pieces, records;        // the 64 sequences looked at; pieces and records before them
+};
+
+// Tiles of a sequence, and the units that a tile's rows see: all, or the window and the tile's tokens.
+__device__ __forceinline__ int chunk_tiles(const PagedAttentionCall& a, const Seq& q) { return (q.n * a.group + kChunkRows - 1) / kChunkRows; }
+__device__ __forceinline__ int chunk_units(const PagedAttentionCall& a, const Seq& q) {
+    const int span = min(q.n, (kChunkRows + a.group - 1) / a.group + 1);
+    const int seen = a.window ? min(q.len, a.window + span - 1 + kChunkUnit) : q.len;
+    return max(1, (seen + kChunkUnit - 1) / kChunkUnit);
+}
+
+__device__ ChunkWalk chunk_walk(const PagedView& c, const PagedAttentionCall& a, const ChunkPlan& p) {
     int tiles = 0;
     float units = 0.0f;
     bool bad = false;
-    Seq q = {};
+#pragma unroll 4
     for (int base = 0; base < c.sequences; base += 64) {
-        q = seq_of(c, a, base + lane, false, &bad);
-        tiles += tiles_of(q);
-        units += (float)tiles_of(q) * (float)units_of(q);
+        const Seq q = seq_of(c, a, base + (threadIdx.x & 63), false, &bad);
+        const int n = chunk_tiles(a, q);
+        tiles = min(tiles + n, 1 << 24);
+        units += (float)n * (float)chunk_units(a, q);
     }
+    tiles = wave_total(tiles);
+    // More tiles than the call's rows can have: sequences whose rows overlap, by row starts that descend. None of them runs.
+    bad |= tiles > p.most - p.items;
     raise_bad(c, bad);
-    tiles = wave_total(tiles);  // at most 2^20 rows * 128 heads / kChunkRows, and one per sequence
-    if (tiles == 0) return false;
+    if (tiles == 0 || tiles > p.most - p.items) return {0, 0, 0, 0};
     // The float sum is rounded the same in every wave, and short by at most 1024 + 8 roundings of 2^-24: a part in ten
     // thousand more covers them.
     units = wave_sum(units);
-    const int per = max(kChunkMinUnits, (int)fminf(2.0001f * units / (float)p.items + 1.0f, 1e9f));
-    int items_before = 0, blocks_before = 0, records_before = 0;
-    for (int base = 0; base < c.sequences; base += 64) {
-        if (c.sequences > 64) q = seq_of(c, a, base + lane, false, &bad);
-        const int splits = q.n ? (units_of(q) + per - 1) / per : 0, items = tiles_of(q) * splits;
-        const int blocks = merge_rows && splits > 1 ? (q.n * a.group + merge_rows - 1) / merge_rows : 0;
+    const int per = (int)fminf(2.0001f * units / (float)p.items + 1.0f, 1e9f);
+    return {__builtin_amdgcn_readfirstlane(max(kChunkMinUnits, per)), 0, 0, 0};
+}
+
+// Piece `want`, not before an earlier call's. False: there are not that many.
+__device__ bool find_piece(const PagedView& c, const PagedAttentionCall& a, ChunkWalk& w, int merge_rows, int want, Piece* out) {
+    const int lane = threadIdx.x & 63;
+    bool bad = false;
+    if (w.per == 0) return false;
+    for (; w.base < c.sequences; w.base += 64) {
+        const Seq q = seq_of(c, a, w.base + lane, false, &bad);
+        const int tiles = chunk_tiles(a, q), splits = q.n ? (chunk_units(a, q) + w.per - 1) / w.per : 0, items = tiles * splits;
         const int records = splits > 1 ? items : 0, xr = scan_sum(records);
-        const int xi = merge_rows ? 0 : scan_sum(items), xb = merge_rows ? scan_sum(blocks) : 0;
-        const uint64_t hit = __ballot((merge_rows ? blocks_before + xb : items_before + xi) > want);
+        const int pieces = !merge_rows ? items : (splits > 1 ? (q.n * a.group + merge_rows - 1) / merge_rows : 0), x = scan_sum(pieces);
+        const uint64_t hit = __ballot(w.pieces + x > want);
         if (hit) {
             const int l = __builtin_ctzll(hit);
             auto get = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
-            *out = {base + l, get(q.row0), get(q.n), get(q.len), 0, 0, get(splits), 0, 0};
-            const int last = get(tiles_of(q)) - 1;
+            *out = {w.base + l, get(q.row0), get(q.n), get(q.len), 0, 0, get(splits), 0, 0};
+            const int last = get(tiles) - 1, k = want - w.pieces - get(x - pieces);
             int j;  // the tile's place, the last tile first
             if (merge_rows) {
-                const int k = want - blocks_before - get(xb - blocks);
                 out->row = k * merge_rows;
                 out->tile = out->row / kChunkRows;
                 j = last - out->tile;
             } else {
-                const int k = want - items_before - get(xi - items);
                 j = k / out->splits;
                 out->tile = last - j;
                 out->split = k - j * out->splits;
             }
-            out->record = records_before + get(xr - records) + j * out->splits;
+            out->record = w.records + get(xr - records) + j * out->splits;
             return true;
         }
-        records_before += __builtin_amdgcn_readlane(xr, 63);
-        items_before += __builtin_amdgcn_readlane(xi, 63);
-        blocks_before += __builtin_amdgcn_readlane(xb, 63);
+        w.pieces += __builtin_amdgcn_readlane(x, 63);
+        w.records += __builtin_amdgcn_readlane(xr, 63);
     }
     return false;
 }
@@ -716,8 +727,9 @@ __device__ __forceinline__ void chunk_part(const PagedView& c, const PagedAttent
         const int ln = lane_here(), r = 4 * (ln >> 5) + (ln >> 2 & 3);
         return r * T::kRowBytes + ((2 * (ln >> 4 & 1) + (ln >> 1 & 1)) ^ chunk_swizzle<D>(r)) * 16 + (ln & 1) * 8;
     };
+    ChunkWalk walk = chunk_walk(c, a, plan);
     Piece t;
-    for (int item = first; item < plan.most && find_piece(c, a, plan, 0, item, &t); item += stride) {
+    for (int item = first; item < plan.most && find_piece(c, a, walk, 0, item, &t); item += stride) {
         const int r0 = t.tile * kChunkRows, nr = (int)min((int64_t)kChunkRows, (int64_t)t.n * a.group - r0);
         const Span span = span_of(a, t, r0, r0 + nr - 1, kTile);
         const int lo = span.lo, hi = span.hi;
@@ -1118,6 +1130,7 @@ __device__ void merge_tokens(const PagedView& c, const PagedAttentionCall& a, in
             }
 #pragma unroll
             for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, kWave));
+            bad = __any(bad);  // of all lanes, before they part
             for (int j = lane; j < t.splits; j += 64) {
                 const float x = rec(j)[r];
                 l = fmaf(x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x - m), rec(j)[kTokenRows + r], l);
@@ -1144,7 +1157,7 @@ __device__ void merge_tokens(const PagedView& c, const PagedAttentionCall& a, in
             }
             ov[grp][col] = v;
             __syncthreads();
-            if (grp == 0 && !__any(bad)) {
+            if (grp == 0 && !bad) {
 #pragma unroll
                 for (int k = 1; k < kGroups; ++k) {
                     const float4 y = ov[k][col];
@@ -1163,8 +1176,9 @@ __device__ void merge_tokens(const PagedView& c, const PagedAttentionCall& a, in
 template <int D, bool E4M3>
 __device__ void merge_chunks(const PagedView& c, const PagedAttentionCall& a, const ChunkPlan& plan, const float* part, int kvh, int first,
                              int stride) {
+    ChunkWalk walk = chunk_walk(c, a, plan);
     Piece t;
-    for (int u = first; u < plan.most_blocks && find_piece(c, a, plan, kMergeChunkRows, u, &t); u += stride) {
+    for (int u = first; u < plan.most_blocks && find_piece(c, a, walk, kMergeChunkRows, u, &t); u += stride) {
         const float* base = part + ((int64_t)kvh * plan.items + t.record) * record_floats(kChunkRows, D);
         auto rec = [&](int j) { return base + j * record_floats(kChunkRows, D); };
         const int rows = min(kMergeChunkRows, t.n * a.group - t.row);

@@ -772,3 +772,227 @@ def test_nan_that_a_row_sees_makes_it_nan(n, length, fmt):
         assert torch.isnan(out[:, 4:, 3].float()).all(), "K" if t is st.k else "V"
         check_rows(out[:, :4], want[:, :4], a[:, :4], d[:, :4], 128)
         view[0, page, slot] = old
+
+
+# --------------------------------------------------------------------------------- ends of the ranges
+
+def test_overlapping_row_starts_are_found():
+    need_gpu()
+    say("paged attention, row starts that descend")
+    st = Setup([900, 900, 900, 900, 900], 32, 2, 64, seed=41)
+    q = queries(300, 16, 64, 42)
+    out = torch.full_like(q, 123.0)
+    ops.paged_attention(q, st.cache, i32([0, 300, 0, 300, 0, 300]), out)
+    assert ops.device_errors() == _lib.DEVERR_PAGED
+    assert (out == 123.0).all()
+    # 2^31 tiles by the starts' account
+    rows = S = 1 << 16
+    table = torch.zeros((S, 1), dtype=torch.int32, device=DEV)
+    pages = torch.zeros((1, 1, 1024, 1, 64), dtype=torch.bfloat16, device=DEV)
+    lens, refs = torch.full((S,), 8, dtype=torch.int32, device=DEV), i32([1])
+    cache = ops.PagedCache(pages, pages.clone(), table, lens, refs)
+    starts = torch.zeros(S + 1, dtype=torch.int32, device=DEV)
+    starts[1::2] = rows
+    q = torch.zeros((rows, 128, 64), dtype=torch.bfloat16, device=DEV)
+    out = torch.full_like(q, 123.0)
+    ops.paged_attention(q, cache, starts, out)
+    assert ops.device_errors() == _lib.DEVERR_PAGED
+    assert (out == 123.0).all()
+
+
+@pytest.mark.parametrize("S,base", [(1, 0), (65, 0), (1500, 2), (2300, 0)])
+def test_reserve_fork_free_of_many_sequences(S, base):
+    """More sequences and forks than a workgroup has threads."""
+    need_gpu()
+    say(f"reserve, fork, free of {S} sequences")
+    rng = random.Random(S)
+    lens = [rng.choice([0, 0, 1, 3, 4, 5, 11]) for _ in range(S)]
+    st = Setup(lens, 4, 1, 64, seed=43, spare=5 * S + 20, columns=6)
+    new = [rng.choice([0, 1, 2, 4, 9]) for _ in range(S)]
+    ops.paged_cache_reserve(st.cache, i32(new))
+    assert st.state.reserve(new) and ops.device_errors() == 0
+    st.check_state()
+    gone = [rng.randrange(S) for _ in range(S // 2 + 1)]  # some twice
+    ops.paged_cache_free(st.cache, i32(gone))
+    st.state.free(gone)
+    assert ops.device_errors() == 0
+    st.check_state()
+    children = [s for s in range(S) if st.state.lens[s] == 0]
+    rng.shuffle(children)
+    live = [s for s in range(S) if st.state.lens[s]]
+    if live and children:
+        parents = [rng.choice(live) for _ in children]
+        k = st.k.clone()
+        ops.paged_cache_fork(st.cache, i32(parents), i32(children))
+        assert st.state.fork(parents, children) and ops.device_errors() == 0
+        st.check_state()
+        for a, b in st.state.moves:
+            k[:, b] = k[:, a]
+        assert torch.equal(st.k, k)
+    ops.paged_cache_compact(st.cache)
+    st.state.compact()
+    assert ops.device_errors() == 0
+    st.check_state()
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "e4m3"])
+@pytest.mark.parametrize("heads,group,dim", [(256, 1, 64), (256, 1, 512), (200, 2, 256), (1, 128, 512), (2, 128, 64), (3, 17, 128)])
+def test_many_heads(heads, group, dim, fmt):
+    need_gpu()
+    say(f"paged attention, {heads} KV heads x {group} of {dim} {fmt}")
+    st = Setup([300, 5, 1100], 32, heads, dim, fmt, seed=44)
+    attend(st, [1, 1, 1], heads * group)
+    attend(st, [20, 1, 2], heads * group, window=200)
+
+
+@pytest.mark.parametrize("window", [0, 1000, 6000])
+@pytest.mark.parametrize("group,heads,dim,fmt", [(16, 1, 512, "bf16"), (2, 2, 256, "e4m3"), (4, 1, 128, "bf16"), (8, 1, 64, "e4m3")])
+def test_long_chunks_split(group, heads, dim, fmt, window):
+    need_gpu()
+    say(f"paged attention, split chunks of {heads} x {group} of {dim} {fmt} window {window}")
+    st = Setup([20011, 1, 9000, 300], 64, heads, dim, fmt, seed=45)
+    attend(st, [33, 1, 70, 1], heads * group, window=window)
+    attend(st, [1, 0, 17, 2], heads * group, window=window, max_rows=17)
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "e4m3"])
+@pytest.mark.parametrize("n,group,heads,dim", [(1, 4, 2, 128), (3, 1, 1, 512), (50, 4, 2, 128), (40, 8, 1, 512), (60, 2, 1, 64)])
+def test_a_bad_page_in_one_part_of_a_split_sequence(n, group, heads, dim, fmt):
+    need_gpu()
+    say(f"paged attention, a bad page of a split sequence, {n} rows of {heads} x {group} of {dim} {fmt}")
+    st = Setup([16000, 15000], 64, heads, dim, fmt, seed=46)
+    sc = (None, None) if st.k_scale is None else (st.k_scale[0], st.v_scale[0])
+    q = queries(2 * n, heads * group, dim, 47)
+    want, a, d = pm.attention(q, *st.values(), st.state.table, st.state.lens, [0, n, 2 * n], 64, 0, 1.0, *sc)
+    good = st.table.clone()
+    for at, p in ((3, -1), (100, 1 << 30), (249, len(st.state.refs))):  # the last page of sequence 0 is 249
+        st.table.copy_(good)
+        st.table[0, at] = p
+        out = torch.full_like(q, 123.0)
+        ops.paged_attention(q, st.cache, i32([0, n, 2 * n]), out)
+        assert ops.device_errors() == _lib.DEVERR_PAGED
+        check_rows(out, want, a, d, dim, slice(n, 2 * n))
+        assert (out[:n] == 123.0).all()
+
+
+@pytest.mark.parametrize("S", [64, 65, 1100])
+def test_tokens_and_chunks_of_many_sequences(S):
+    need_gpu()
+    say(f"paged attention, {S} sequences of one to forty rows")
+    rng = random.Random(S)
+    lens = [rng.choice([0, 1, 2, 40, 300]) for _ in range(S)]
+    lens[S // 2] = 5000
+    rows = [rng.choice([0, 1, 1, 1, 2, 9, 40]) if n else 0 for n in lens]
+    st = Setup(lens, 16, 2, 64, seed=48)
+    attend(st, rows, 8, first=3, tail=2)
+    attend(st, [min(r, 4) for r in rows], 8, max_rows=4)
+    attend(st, rows, 8, window=33, max_rows=40)
+
+
+def test_offsets_between_31_and_32_bits():
+    need_gpu()
+    say("paged attention in pools of 3 GB, K and V with other strides")
+    slots, heads, dim, pages = 64, 8, 128, 23000
+    k = torch.empty((1, pages, slots, heads, dim), dtype=torch.bfloat16, device=DEV)
+    v = torch.empty((1, pages, heads, slots, dim), dtype=torch.bfloat16, device=DEV).transpose(2, 3)
+    assert 1 << 31 < k.numel() * 2 < 1 << 32
+    table = [[pages - 1, 0, pages - 2, 17000]]
+    for p in table[0]:
+        k[0, p], v[0, p] = queries(slots, heads, dim, p, 11.0), queries(slots, heads, dim, p + 1, 11.0)
+    cache = ops.PagedCache(k, v, i32(table), i32([250]), torch.zeros(pages, dtype=torch.int32, device=DEV))
+    low = sorted(table[0])
+    for n in (1, 40):
+        q = queries(n, 16, dim, 5)
+        out = torch.empty_like(q)
+        ops.paged_attention(q, cache, i32([0, n]), out)
+        assert ops.device_errors() == 0
+        want, a, d = pm.attention(q, k[0, low].float(), v[0, low].float(), [[low.index(p) for p in table[0]]], [250], [0, n], slots, 0, 1.0)
+        check_rows(out, want, a, d, dim)
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "e4m3"])
+def test_layers_of_one_cache(fmt):
+    need_gpu()
+    say(f"paged append and attention of three layers {fmt}")
+    st = Setup([70, 3], 16, 2, 64, fmt, layers=3, seed=49)
+    before = raw(st.k).clone()
+    nk, nv = queries(5, 2, 64, 1, 8.0), queries(5, 2, 64, 2, 8.0)
+    ops.paged_cache_append(st.cache, nk, nv, i32([0, 3, 5]), layer=1)
+    after = raw(st.k)
+    assert torch.equal(after[0], before[0]) and torch.equal(after[2], before[2]) and not torch.equal(after[1], before[1])
+    for layer in range(3):
+        attend(st, [20, 3], 8, layer=layer)
+        attend(st, [1, 1], 8, layer=layer)
+
+
+@pytest.mark.parametrize("slots", [1, 3, 4097, 65536])
+def test_smallest_and_largest_pages(slots):
+    need_gpu()
+    say(f"paged cache of {slots} slots a page")
+    st = Setup([1, 0], slots, 1, 64, seed=50, spare=6, columns=4)
+    for new in ([1, 1], [2 * slots, 0], [0, slots]):
+        ops.paged_cache_reserve(st.cache, i32(new))
+        fits = st.state.reserve(new)
+        assert ops.device_errors() == (0 if fits else _lib.DEVERR_PAGED)
+        st.check_state()
+    attend(st, [1, 1], 4)
+    attend(st, [min(20, st.state.lens[0]), 1], 4, window=5)
+
+
+def test_calls_without_rows():
+    need_gpu()
+    say("paged calls of no rows and no sequences")
+    st = Setup([0], 16, 2, 128, seed=51, spare=1)
+    none = torch.empty((0, 8, 128), dtype=torch.bfloat16, device=DEV)
+    kv = torch.empty((0, 2, 128), dtype=torch.bfloat16, device=DEV)
+    ops.paged_attention(none, st.cache, i32([0, 0]), none.clone())
+    ops.paged_cache_append(st.cache, kv, kv, i32([0, 0]))
+    ops.paged_cache_fork(st.cache, i32([]), i32([]))
+    ops.paged_cache_free(st.cache, i32([]))
+    ops.paged_cache_reserve(st.cache, i32([0]))
+    ops.paged_cache_compact(st.cache)
+    attend(st, [0], 8, first=1, tail=2)
+    attend(st, [2], 8)  # rows of an empty sequence see nothing: zeros
+    assert ops.device_errors() == 0
+    st.check_state()
+
+
+def test_two_graphs_take_turns():
+    """Two captured calls share the library's scratch; replayed in turn, with eager calls between, each keeps its result."""
+    need_gpu()
+    say("two paged graphs in turn")
+    ops.init(0)
+    made = []
+    for i, (lens, rows, heads, dim) in enumerate([([9000, 40], [1, 1], 2, 128), ([5000, 300], [60, 1], 1, 512)]):
+        st = Setup(lens, 64, heads, dim, seed=52 + i)
+        q = queries(sum(rows), 8, dim, 54 + i)
+        out, want, starts = torch.empty_like(q), torch.empty_like(q), i32(starts_of(rows))
+        ops.paged_attention(q, st.cache, starts, want)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            ops.paged_attention(q, st.cache, starts, out)
+        made.append((graph, out, want, st, q, starts))  # what a graph reads stays alive
+    for _ in range(3):
+        for graph, out, want, *_ in made:
+            out.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, want)
+        attend(made[0][3], [30, 2], 8)
+    assert ops.device_errors() == 0
+
+
+@pytest.mark.parametrize("seed", range(12))
+def test_random_shapes(seed):
+    need_gpu()
+    rng = random.Random(1000 + seed)
+    dim, fmt, layout = rng.choice([64, 128, 256, 512]), rng.choice(["bf16", "e4m3"]), rng.choice(["nhd", "hnd", "pairs", "slots"])
+    heads, group, slots = rng.choice([1, 2, 3, 8]), rng.choice([1, 2, 3, 5, 8, 16, 30]), rng.choice([1, 5, 16, 48, 64, 256])
+    S = rng.choice([1, 3, 20, 70])
+    lens = [rng.choice([0, 1, rng.randrange(2, 400), rng.randrange(2, 3000)]) for _ in range(S)]
+    rows = [min(n, rng.choice([0, 1, 1, 2, 7, rng.randrange(1, 200)])) for n in lens]
+    window, scale = rng.choice([0, 0, 1, 31, 512]), rng.choice([1.0, 0.0625, -1.0])
+    say(f"paged attention {heads} x {group} of {dim} {fmt} {layout}, {slots} slots, rows {rows} of {lens}, window {window}, scale {scale}")
+    st = Setup(lens, slots, heads, dim, fmt, seed=seed, layout=layout, poison=True)
+    # poisoned slots are NaN: the oracle reads only the visible ones
+    attend(st, rows, heads * group, window=window, scale=scale, first=rng.choice([0, 2]), tail=rng.choice([0, 3]))
