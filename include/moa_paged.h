@@ -74,7 +74,8 @@ int moa_paged_cache_append(const moa_paged_cache* cache, const uint16_t* k, int6
 
 /* Makes sequence children[i] a copy of parents[i] (device int32 [count]) in every layer: it shares the
  * parent's full pages (reference count + 1) and gets a copy of its partly filled last page in the
- * lowest free page, handed out in the order of the list. A parent may be listed many times. All or
+ * lowest free page, handed out in the order of the list. A parent may be listed many times; append
+ * its reserved positions first, since an append to a shared page is seen by all that share it. All or
  * nothing: an index out of range, a child that is listed twice, that is also a parent or that has
  * positions, or too few free pages leave the state as it was (MOA_DEVERR_PAGED). count may be 0. */
 int moa_paged_cache_fork(const moa_paged_cache* cache, const int32_t* parents, const int32_t* children, int count,
@@ -100,7 +101,9 @@ int moa_paged_cache_compact(const moa_paged_cache* cache, void* stream);
  * query heads per KV head. max_rows: the most rows a sequence has in this call (it chooses the kernel
  * and its grid; rows itself is always right). Rows that belong to no sequence are left as they were.
  * A sequence whose rows or length are out of range, or that has more than max_rows rows, is left out; so
- * is at least every row that sees a page outside the pool (MOA_DEVERR_PAGED). rows may be 0. */
+ * is at least every row that sees a page outside the pool, and row starts that descend may leave out all
+ * (MOA_DEVERR_PAGED). Within one call a row's result does not depend on the other rows, but which kernel and which order
+ * of f32 sums it gets does: the last bits may differ between calls of other batches. rows may be 0. */
 int moa_paged_attention(const uint16_t* q, int64_t q_row_stride, const moa_paged_cache* cache,
                         const int32_t* row_starts, uint16_t* out, int64_t out_row_stride, int rows, int q_heads,
                         int layer, int window, float scale, int max_rows, void* stream);

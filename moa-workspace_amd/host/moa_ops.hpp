@@ -25,6 +25,7 @@
 
 #include <cstddef>
 #include <cstdint>
+#include <limits>
 #include <numeric>
 #include <stdexcept>
 #include <string>
@@ -33,6 +34,7 @@
 #include <vector>
 
 #include "moa_ops.h"
+#include "moa_paged.h"
 
 namespace moa {
 
@@ -194,7 +196,56 @@ inline const uint8_t* u8(const HbmTensor<T>& t) {
     return reinterpret_cast<const uint8_t*>(t.data());
 }
 inline const uint16_t* opt_u16(const HbmTensor<bf16>* t) { return t ? u16(*t) : nullptr; }
+inline int int_of(size_t n) {
+    if (n > static_cast<size_t>(std::numeric_limits<int>::max())) throw Error(MOA_ERROR_INVALID_VALUE, "a size past 2^31 - 1");
+    return static_cast<int>(n);
+}
 }  // namespace detail
+
+// Many sequences' K and V over one pool of pages (include/moa_paged.h; no counterpart in the reference, which serves one
+// sequence), as the paged operators take it. T: bf16, or f8e4m3 with scales. The tensors stay the caller's and outlive the cache:
+// k_pages, v_pages [layers, pages, slots, kv_heads, head_dim], page_table [sequences, columns], seq_lens [sequences] and
+// ref_counts [pages] (zero in a new cache), k_scale, v_scale [layers, kv_heads].
+template <class T>
+class PagedCache {
+    static_assert(std::is_same<T, bf16>::value || std::is_same<T, f8e4m3>::value, "pages hold bf16 or E4M3");
+
+  public:
+    PagedCache(HbmTensor<T>& k_pages, HbmTensor<T>& v_pages, HbmTensor<int32_t>& page_table, HbmTensor<int32_t>& seq_lens,
+               HbmTensor<int32_t>& ref_counts, const HbmTensor<float>* k_scale = nullptr, const HbmTensor<float>* v_scale = nullptr) {
+        using namespace detail;
+        const std::vector<size_t>& n = k_pages.shape();
+        if (n.size() != 5 || v_pages.shape() != n || page_table.shape().size() != 2)
+            throw Error(MOA_ERROR_INVALID_VALUE, "PagedCache: pages are [layers, pages, slots, kv_heads, head_dim], a table [sequences, columns]");
+        c_.k_pages = k_pages.data();
+        c_.v_pages = v_pages.data();
+        c_.layers = int_of(n[0]), c_.pages = int_of(n[1]), c_.slots = int_of(n[2]), c_.kv_heads = int_of(n[3]), c_.head_dim = int_of(n[4]);
+        c_.sequences = int_of(page_table.shape()[0]), c_.columns = int_of(page_table.shape()[1]);
+        c_.table_stride = c_.columns;
+        int64_t stride = c_.head_dim;
+        for (int i = 3; i >= 0; --i) {
+            c_.k_stride[i] = c_.v_stride[i] = stride;
+            stride *= static_cast<int64_t>(n[i]);
+        }
+        want(seq_lens, c_.sequences, "seq_lens");
+        want(ref_counts, c_.pages, "ref_counts");
+        c_.page_table = page_table.data();
+        c_.seq_lens = seq_lens.data();
+        c_.ref_counts = ref_counts.data();
+        c_.element = std::is_same<T, bf16>::value ? MOA_PAGES_BF16 : MOA_PAGES_E4M3;
+        if (k_scale) want(*k_scale, n[0] * n[3], "k_scale");
+        if (v_scale) want(*v_scale, n[0] * n[3], "v_scale");
+        c_.k_scale = k_scale ? k_scale->data() : nullptr;
+        c_.v_scale = v_scale ? v_scale->data() : nullptr;
+    }
+    const moa_paged_cache* get() const { return &c_; }
+    size_t sequences() const { return static_cast<size_t>(c_.sequences); }
+    size_t kv_heads() const { return static_cast<size_t>(c_.kv_heads); }
+    size_t head_dim() const { return static_cast<size_t>(c_.head_dim); }
+
+  private:
+    moa_paged_cache c_{};
+};
 
 namespace ops {
 
@@ -483,6 +534,66 @@ inline void final_norm_and_logits(const Device& device, const HbmTensor<bf16>& i
     device.make_current();
     check(moa_final_norm_and_logits(u16(input), u16(rms_weight), u16(lm_head_weight), u16(out), M, device.stream()),
           "final_norm_and_logits");
+}
+
+// The paged KV cache (include/moa_paged.h). A bad value in the state or in an index tensor is left out and raises
+// MOA_DEVERR_PAGED in Device::device_errors().
+template <class T>
+inline void paged_cache_reserve(const Device& device, PagedCache<T>& cache, const HbmTensor<int32_t>& new_tokens) {
+    detail::want(new_tokens, cache.sequences(), "new_tokens");
+    device.make_current();
+    check(moa_paged_cache_reserve(cache.get(), new_tokens.data(), device.stream()), "paged_cache_reserve");
+}
+
+// k, v [rows, kv_heads, head_dim]; row_starts [sequences + 1].
+template <class T>
+inline void paged_cache_append(const Device& device, PagedCache<T>& cache, const HbmTensor<bf16>& k, const HbmTensor<bf16>& v,
+                               const HbmTensor<int32_t>& row_starts, int layer = 0) {
+    using namespace detail;
+    const size_t width = cache.kv_heads() * cache.head_dim();
+    const int M = rows(k, width, "k");
+    want(v, M * width, "v"); want(row_starts, cache.sequences() + 1, "row_starts");
+    device.make_current();
+    check(moa_paged_cache_append(cache.get(), u16(k), width, u16(v), width, row_starts.data(), M, layer, device.stream()),
+          "paged_cache_append");
+}
+
+template <class T>
+inline void paged_cache_fork(const Device& device, PagedCache<T>& cache, const HbmTensor<int32_t>& parents,
+                             const HbmTensor<int32_t>& children) {
+    detail::want(children, parents.size(), "children");
+    device.make_current();
+    check(moa_paged_cache_fork(cache.get(), parents.data(), children.data(), detail::int_of(parents.size()), device.stream()),
+          "paged_cache_fork");
+}
+
+template <class T>
+inline void paged_cache_free(const Device& device, PagedCache<T>& cache, const HbmTensor<int32_t>& sequences) {
+    device.make_current();
+    check(moa_paged_cache_free(cache.get(), sequences.data(), detail::int_of(sequences.size()), device.stream()), "paged_cache_free");
+}
+
+template <class T>
+inline void paged_cache_compact(const Device& device, PagedCache<T>& cache) {
+    device.make_current();
+    check(moa_paged_cache_compact(cache.get(), device.stream()), "paged_cache_compact");
+}
+
+// q, out [rows, q_heads, head_dim] (out may be q); max_rows: the most rows a sequence has, 0: all.
+template <class T>
+inline void paged_attention(const Device& device, const HbmTensor<bf16>& q, const PagedCache<T>& cache,
+                            const HbmTensor<int32_t>& row_starts, HbmTensor<bf16>& out, int layer = 0, int window = 0,
+                            float scale = 1.0f, int max_rows = 0) {
+    using namespace detail;
+    if (q.shape().size() != 3 || q.shape()[2] != cache.head_dim() || q.size() == 0)
+        throw Error(MOA_ERROR_INVALID_VALUE, "q must be [rows, q_heads, head_dim]");
+    const int M = int_of(q.shape()[0]), heads = int_of(q.shape()[1]);
+    const int64_t width = static_cast<int64_t>(heads) * static_cast<int64_t>(cache.head_dim());
+    want(out, q.size(), "out"); want(row_starts, cache.sequences() + 1, "row_starts");
+    device.make_current();
+    check(moa_paged_attention(u16(q), width, cache.get(), row_starts.data(), u16(out), width, M, heads, layer, window, scale,
+                              max_rows ? max_rows : M, device.stream()),
+          "paged_attention");
 }
 
 }  // namespace ops
