@@ -53,21 +53,35 @@ __device__ int block_before(int v, int* lds, int* total) {
     return before + x - v;
 }
 
-// Calls f(page, rank) for the pages of [from, to) that are free (want_free) or live, in ascending order of rank, until
-// `most` of them; returns how many there were. kPer pages a thread and step, one ballot each, so that a step's loads
-// go out together.
+// kPer pages a thread and step, so that a step's loads go out together.
 constexpr int kPer = 8;
+constexpr int kStepPages = kPlanBlock * kPer;
+
+struct Counts { int32_t r[kPer]; };  // reference counts of the thread's pages of one step (0 behind the last)
+__device__ __forceinline__ Counts counts_at(const PagedView& c, int base) {
+    Counts v;
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+        const int p = base + j * kPlanBlock + (int)threadIdx.x;
+        v.r[j] = p < c.pages ? c.refs[p] : 0;
+    }
+    return v;
+}
+
+// Calls f(page, rank, count) for the pages of [from, to) that are free (want_free) or live, in ascending order of rank, until
+// `most` of them; returns how many there were. first: counts_at(c, 0), asked for ahead of the work that leads here.
 template <class F>
-__device__ int each_page(const int32_t* refs, int from, int to, bool want_free, int most, int* lds, F f) {
+__device__ int each_page(const PagedView& c, const Counts& first, int from, int to, bool want_free, int most, int* lds, F f) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     int found = 0;
-    for (int base = from; base < to && found < most; base += kPlanBlock * kPer) {
+    for (int base = from / kStepPages * kStepPages; base < to && found < most; base += kStepPages) {
+        Counts v = first;
+        if (base) v = counts_at(c, base);
         uint64_t b[kPer];
 #pragma unroll
         for (int j = 0; j < kPer; ++j) {
             const int p = base + j * kPlanBlock + (int)threadIdx.x;
-            const bool live = p < to && refs[p] > 0;
-            b[j] = __ballot(p < to && live != want_free);
+            b[j] = __ballot(p >= from && p < to && (v.r[j] > 0) != want_free);
         }
         __syncthreads();  // the step before has read the counts
         if (lane < kPer) {
@@ -92,7 +106,7 @@ __device__ int each_page(const int32_t* refs, int from, int to, bool want_free, 
             const int upto = __shfl(x, at >> 1, kWave), odd = __shfl(c1, at >> 1, kWave), even = __shfl(c0, at >> 1, kWave);
             const int before = upto - odd - ((at & 1) ? 0 : even);
             const int rank = found + before + __popcll(b[j] & ((1ull << lane) - 1));
-            if ((b[j] >> lane & 1) && rank < most) f(base + j * kPlanBlock + (int)threadIdx.x, rank);
+            if ((b[j] >> lane & 1) && rank < most) f(base + j * kPlanBlock + (int)threadIdx.x, rank, v.r[j]);
         }
         found += all;
     }
@@ -100,6 +114,17 @@ __device__ int each_page(const int32_t* refs, int from, int to, bool want_free, 
     return min(found, most);
 }
 static_assert(kPer * kPlanWaves == 2 * kWave, "each_page scans two counts a lane");
+
+// A list of pages by rank: the first kFew in LDS, the others in global memory.
+constexpr int kFew = 2 * kPlanBlock;
+struct PageList {
+    int *few; int32_t* more;
+    __device__ void put(int rank, int p) const {
+        if (rank < kFew) few[rank] = p;
+        else more[rank] = p;
+    }
+    __device__ int get(int rank) const { return rank < kFew ? few[rank] : more[rank]; }
+};
 
 __device__ __forceinline__ int pages_of(const PagedView& c, int n) { return (int)page_of(c, (uint32_t)(n + (int)c.slots - 1)); }
 
@@ -109,32 +134,33 @@ __device__ __forceinline__ void raise(const PagedView& c) { atomicOr(c.err, kErr
 
 // Thread t takes sequences t, t + 1024, ...: a first pass checks them and counts the pages they need, then the lowest
 // free pages are listed, and a second pass hands them out, 1024 sequences at a time: each thread takes pages by their rank and
-// finds their sequence among the prefix sums of the needs.
+// finds their sequence among the prefix sums of the needs. Bound by its chain of memory round trips and barriers (7.3 us with
+// lengths, counts and the list fetched one after the other, 6.7 with lengths and counts asked for at once and a short list in LDS).
 __global__ __launch_bounds__(kPlanBlock) void paged_reserve_kernel(PagedView c, const int32_t* fresh, int32_t* list) {
     __shared__ uint64_t sums[kPlanWaves];
-    __shared__ int lds[2 * kWave], before[kPlanBlock], old[kPlanBlock];
+    __shared__ int lds[2 * kWave], before[kPlanBlock], old[kPlanBlock], few[kFew];
+    const PageList free_pages = {few, list};
     const int cap = paged_capacity(c);
+    const Counts first = counts_at(c, 0);
+    const int len0 = (int)threadIdx.x < c.sequences ? c.lens[threadIdx.x] : 0, n0 = (int)threadIdx.x < c.sequences ? fresh[threadIdx.x] : 0;
     uint64_t need = 0;
     bool bad = false;
     for (int s = threadIdx.x; s < c.sequences; s += kPlanBlock) {
-        const int len = c.lens[s], n = fresh[s];
+        const int len = s < kPlanBlock ? len0 : c.lens[s], n = s < kPlanBlock ? n0 : fresh[s];
         if (n < 0 || len < 0 || len > cap || n > cap - len) bad = true;
         else need += pages_of(c, len + n) - pages_of(c, len);
     }
     bad = __syncthreads_or(bad);
     need = block_sum(need, sums);
-    if (bad || need > (uint64_t)c.pages) {
-        if (threadIdx.x == 0) raise(c);
-        return;
-    }
-    if (each_page(c.refs, 0, c.pages, true, (int)need, lds, [&](int p, int rank) { list[rank] = p; }) < (int)need) {
+    if (bad || need > (uint64_t)c.pages ||
+        each_page(c, first, 0, c.pages, true, (int)need, lds, [&](int p, int rank, int) { free_pages.put(rank, p); }) < (int)need) {
         if (threadIdx.x == 0) raise(c);
         return;
     }
     int given = 0;
     for (int base = 0; base < c.sequences; base += kPlanBlock) {
         const int s = base + (int)threadIdx.x, t = threadIdx.x;
-        const int len = s < c.sequences ? c.lens[s] : 0, n = s < c.sequences ? fresh[s] : 0;
+        const int len = base == 0 ? len0 : (s < c.sequences ? c.lens[s] : 0), n = base == 0 ? n0 : (s < c.sequences ? fresh[s] : 0);
         const int had = pages_of(c, len);
         int all = 0;
         before[t] = block_before(pages_of(c, len + n) - had, lds, &all);
@@ -146,7 +172,7 @@ __global__ __launch_bounds__(kPlanBlock) void paged_reserve_kernel(PagedView c, 
 #pragma unroll
             for (int step = kPlanBlock / 2; step > 0; step /= 2)
                 if (before[lo + step] <= r) lo += step;
-            const int p = list[given + r];
+            const int p = free_pages.get(given + r);
             c.table[(base + lo) * c.table_stride + old[lo] + r - before[lo]] = p;
             c.refs[p] = 1;
         }
@@ -201,33 +227,49 @@ __device__ void copy_pages(const PagedView& c, const int32_t* src, const int32_t
 
 // --------------------------------------------------------------------------------------------- fork
 
-// Checks the whole call, then hands out the pages of the partly filled last pages. list: per fork the page to copy (-1:
-// none) and its copy; result: the number of forks, 0 if the call is refused.
+// What the plan needs of fork f: lengths are -1 where an index is out of range.
+struct Fork { int parent, child, len, child_len, full, page; };
+__device__ __forceinline__ Fork fork_at(const PagedView& c, const int32_t* parents, const int32_t* children, int count, int f) {
+    Fork x = {-1, -1, -1, -1, 0, -1};
+    if (f >= count) return x;
+    x.parent = parents[f], x.child = children[f];
+    if (x.parent >= 0 && x.parent < c.sequences) x.len = c.lens[x.parent];
+    if (x.child >= 0 && x.child < c.sequences) x.child_len = c.lens[x.child];
+    if (x.len >= 0 && x.len <= paged_capacity(c)) {
+        x.full = (int)page_of(c, x.len);
+        if (x.full * (int)c.slots < x.len) x.page = c.table[x.parent * c.table_stride + x.full];
+    }
+    return x;
+}
+
+// Checks the whole call, then hands out the pages of the partly filled last pages. src, dst: per fork the page to copy (-1:
+// none) and its copy; result: the number of forks, 0 if the call is refused. Bound by its chain of memory round trips, as the
+// reserve plan: the first 1024 forks' values are fetched once (7.5 us with a fetch in each pass, 6.6 so).
 __global__ __launch_bounds__(kPlanBlock) void paged_fork_plan_kernel(PagedView c, const int32_t* parents, const int32_t* children,
                                                                      int count, int32_t* src, int32_t* dst, int32_t* result) {
-    __shared__ int lds[2 * kWave];
+    __shared__ int lds[2 * kWave], few[kFew];
     __shared__ uint32_t child[kPagedMaxSequences / 32];
-    const int cap = paged_capacity(c);
+    const PageList free_pages = {few, dst + kPagedMaxSequences};
+    const Counts first = counts_at(c, 0);
+    const Fork mine = fork_at(c, parents, children, count, threadIdx.x);
     if (threadIdx.x == 0) *result = 0;
-    for (int i = threadIdx.x; i < kPagedMaxSequences / 32; i += kPlanBlock) child[i] = 0;
+    for (int i = threadIdx.x; i < (c.sequences + 31) / 32; i += kPlanBlock) child[i] = 0;
     __syncthreads();
     bool bad = false;
     for (int f = threadIdx.x; f < count; f += kPlanBlock) {
-        const int s = children[f];
-        if (s < 0 || s >= c.sequences || c.lens[s] != 0) bad = true;
-        else bad |= (atomicOr(&child[s >> 5], 1u << (s & 31)) >> (s & 31) & 1) != 0;
+        const Fork x = f < kPlanBlock ? mine : fork_at(c, parents, children, count, f);
+        if (x.child_len != 0) bad = true;
+        else bad |= (atomicOr(&child[x.child >> 5], 1u << (x.child & 31)) >> (x.child & 31) & 1) != 0;
     }
     bad = __syncthreads_or(bad);
     int need = 0;
     if (!bad) {
         for (int f = threadIdx.x; f < count; f += kPlanBlock) {
-            const int s = parents[f];
-            if (s < 0 || s >= c.sequences || (child[s >> 5] >> (s & 31) & 1)) { bad = true; continue; }
-            const int len = c.lens[s], full = len < 0 ? 0 : (int)page_of(c, len);
-            if (len < 0 || len > cap) { bad = true; continue; }
-            if (full * (int)c.slots < len) {
-                const int p = c.table[s * c.table_stride + full];
-                if (p < 0 || p >= c.pages) bad = true;
+            const Fork x = f < kPlanBlock ? mine : fork_at(c, parents, children, count, f);
+            if (x.len < 0 || x.len > paged_capacity(c) || (child[x.parent >> 5] >> (x.parent & 31) & 1)) {
+                bad = true;
+            } else if (x.full * (int)c.slots < x.len) {
+                bad |= x.page < 0 || x.page >= c.pages;
                 ++need;
             }
         }
@@ -236,27 +278,27 @@ __global__ __launch_bounds__(kPlanBlock) void paged_fork_plan_kernel(PagedView c
     int total = 0;
     (void)block_before(need, lds, &total);
     if (bad || total > c.pages ||
-        each_page(c.refs, 0, c.pages, true, total, lds, [&](int p, int rank) { dst[kPagedMaxSequences + rank] = p; }) < total) {
+        each_page(c, first, 0, c.pages, true, total, lds, [&](int p, int rank, int) { free_pages.put(rank, p); }) < total) {
         if (threadIdx.x == 0) raise(c);
         return;
     }
     int given = 0;
     for (int base = 0; base < count; base += kPlanBlock) {
         const int f = base + (int)threadIdx.x;
-        const int s = f < count ? parents[f] : 0, len = f < count ? c.lens[s] : 0, full = (int)page_of(c, len);
-        const bool part = full * (int)c.slots < len;
+        const Fork x = base == 0 ? mine : fork_at(c, parents, children, count, f);
+        const bool part = f < count && x.full * (int)c.slots < x.len;
         int all = 0;
         const int at = given + block_before(part, lds, &all);
         if (f < count) {
             src[f] = -1;
             if (part) {
-                const int p = dst[kPagedMaxSequences + at];
-                src[f] = c.table[s * c.table_stride + full];
+                const int p = free_pages.get(at);
+                src[f] = x.page;
                 dst[f] = p;
-                c.table[children[f] * c.table_stride + full] = p;
+                c.table[x.child * c.table_stride + x.full] = p;
                 c.refs[p] = 1;
             }
-            c.lens[children[f]] = len;
+            c.lens[x.child] = x.len;
         }
         given += all;
     }
@@ -314,20 +356,30 @@ __global__ __launch_bounds__(kCopyBlock) void paged_free_kernel(PagedView c, con
 __global__ __launch_bounds__(kPlanBlock) void paged_compact_plan_kernel(PagedView c, int32_t* place, int32_t* src, int32_t* dst,
                                                                         int32_t* result) {
     __shared__ uint64_t sums[kPlanWaves];
-    __shared__ int lds[2 * kWave];
+    __shared__ int lds[2 * kWave], few[kFew];
+    const PageList targets = {few, dst};
+    const Counts first = counts_at(c, 0);
     uint64_t n = 0;
-    for (int p = threadIdx.x; p < c.pages; p += kPlanBlock) n += c.refs[p] > 0;
+    for (int base = 0; base < c.pages; base += kStepPages) {
+        Counts v = first;
+        if (base) v = counts_at(c, base);
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) n += v.r[j] > 0;
+    }
     const int live = (int)block_sum(n, sums);
     for (int p = live + (int)threadIdx.x; p < c.pages; p += kPlanBlock) place[p] = p;
-    const int moves = each_page(c.refs, 0, live, true, live, lds, [&](int p, int rank) { dst[rank] = p; });
+    const int moves = each_page(c, first, 0, live, true, live, lds, [&](int p, int rank, int) {
+        targets.put(rank, p);
+        if (rank < kFew) dst[rank] = p;
+    });
     // as many live pages lie behind `live` as free ones before it
-    each_page(c.refs, live, c.pages, false, moves, lds, [&](int p, int rank) {
-        const int to = dst[rank];
+    each_page(c, first, live, c.pages, false, moves, lds, [&](int p, int rank, int count) {
+        const int to = targets.get(rank);
         src[rank] = p;
         place[p] = to;
-        c.refs[to] = c.refs[p];
+        c.refs[to] = count;
+        c.refs[p] = 0;
     });
-    for (int i = threadIdx.x; i < moves; i += kPlanBlock) c.refs[src[i]] = 0;
     if (threadIdx.x == 0) {
         result[0] = live;
         result[1] = moves;

@@ -130,8 +130,11 @@ __device__ void token_at(const PagedView& c, const PagedAttentionCall& a, TokenW
     }
 }
 
-// Block `want` of `rows` rows of the sequences that are split, for the merge; record: its first. False: there are not that many.
-__device__ bool token_block(const PagedView& c, const PagedAttentionCall& a, const TokenWalk& w, int align, int rows, int want, Piece* out) {
+// Block `want` of the rows of the sequences that are split, for the merge: four rows, or one where the parts are many; record: the
+// sequence's first. False: there are not that many.
+constexpr int kMergeWaveSplits = 16;
+__device__ __forceinline__ int token_block_rows(int splits) { return splits > kMergeWaveSplits ? 1 : 4; }
+__device__ bool token_block(const PagedView& c, const PagedAttentionCall& a, const TokenWalk& w, int align, int want, Piece* out) {
     const int lane = threadIdx.x & 63;
     bool bad = false;
     int64_t before = 0;
@@ -142,12 +145,13 @@ __device__ bool token_block(const PagedView& c, const PagedAttentionCall& a, con
         const int64_t first = before + x - n, last = first + max(n, 1) - 1;
         const int64_t w0 = w.units >> 31 ? first / w.q : (uint32_t)first / (uint32_t)w.q;
         const int64_t w1 = w.units >> 31 ? last / w.q : (uint32_t)last / (uint32_t)w.q;
-        const int splits = n ? (int)(w1 - w0) + 1 : 0, blocks = splits > 1 ? (q.n * a.group + rows - 1) / rows : 0, xb = scan_sum(blocks);
+        const int splits = n ? (int)(w1 - w0) + 1 : 0, rows = token_block_rows(splits);
+        const int blocks = splits > 1 ? (q.n * a.group + rows - 1) / rows : 0, xb = scan_sum(blocks);
         const uint64_t hit = __ballot(blocks_before + xb > want);
         if (hit) {
             const int l = __builtin_ctzll(hit);
             auto get = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
-            *out = {base + l, get(q.row0), get(q.n), get(q.len), 0, 0, get(splits), 2 * get((int)w0), (want - blocks_before - get(xb - blocks)) * rows};
+            *out = {base + l, get(q.row0), get(q.n), get(q.len), 0, 0, get(splits), 2 * get((int)w0), (want - blocks_before - get(xb - blocks)) * get(rows)};
             return true;
         }
         before += __builtin_amdgcn_readlane(x, 63);
@@ -1047,31 +1051,25 @@ __global__ __launch_bounds__((ChunkShape<D, E4M3>::kThreads)) __attribute__((amd
 
 // Rows of split tiles, both kernels' in one launch. A workgroup takes a block of rows of a tile and finds it once. Few
 // splits: a wave per row, its lanes across the dims. More (long sequences of few rows): the workgroup takes 128 dims of a
-// row, its threads in groups that take the records in turn.
+// row, its threads in groups that take the records in turn. Bound by its chain of round trips where the records are few, so maxima,
+// sums and outputs are asked for at once. (250 records of 128 rows of 512: 15.8 us, 19.5 with the maxima first; 16 single tokens
+// of 8 heads of 128 in some 500 records: 8.4 and 10.6.)
 constexpr int kMergeDims = 128;
-constexpr int kMergeTokenRows = 2;
 constexpr int kMergeChunkRows = 8;
-constexpr int kMergeWaveSplits = 16;
 
 // Row r of the tile (rec(j): the record of split j, bm rows each), row `row` of its sequence, by one wave.
 template <int D, bool E4M3, class R>
 __device__ __forceinline__ void merge_row(const PagedView& c, const PagedAttentionCall& a, const Piece& t, int kvh, R rec, int bm, int r, int row) {
-    constexpr int kPer = D / 64, kAhead = 4;  // dims of a lane, records in flight
+    constexpr int kPer = D / 64;  // dims of a lane
     const int lane = threadIdx.x & 63;
     float m = -INFINITY, l = 0.0f, v[kPer] = {};
     bool bad = false;
-    for (int j = lane; j < t.splits; j += 64) {
-        const float x = rec(j)[r];
-        bad |= x != x;
-        m = fmaxf(m, x);
-    }
+    // records j0 .. of which `most` at once; find: they are all there are
+    auto take = [&](auto most, int j0, bool find) __attribute__((always_inline)) {
+        constexpr int K = decltype(most)::value;
+        float x[K], y[K], w[K][kPer];
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, kWave));
-    if (__any(bad)) return;
-    for (int j0 = 0; j0 < t.splits; j0 += kAhead) {
-        float x[kAhead], y[kAhead], w[kAhead][kPer];
-#pragma unroll
-        for (int k = 0; k < kAhead; ++k) {
+        for (int k = 0; k < K; ++k) {
             const float* at = rec(min(j0 + k, t.splits - 1));
             x[k] = at[r];
             y[k] = at[bm + r];
@@ -1079,8 +1077,12 @@ __device__ __forceinline__ void merge_row(const PagedView& c, const PagedAttenti
 #pragma unroll
             for (int i = 0; i < kPer; ++i) w[k][i] = o[i];
         }
+        if (find) {
 #pragma unroll
-        for (int k = 0; k < kAhead; ++k) {
+            for (int k = 0; k < K; ++k) bad |= x[k] != x[k], m = fmaxf(m, x[k]);
+        }
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
             if (j0 + k >= t.splits) continue;
             // (a record of no weight counts too: sums that are NaN for a row's own values make the row NaN)
             const float f = x[k] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x[k] - m);
@@ -1088,7 +1090,22 @@ __device__ __forceinline__ void merge_row(const PagedView& c, const PagedAttenti
 #pragma unroll
             for (int i = 0; i < kPer; ++i) v[i] = fmaf(f, w[k][i], v[i]);
         }
+    };
+    if (t.splits == 2) {
+        take(std::integral_constant<int, 2>{}, 0, true);
+    } else if (t.splits <= 4) {
+        take(std::integral_constant<int, 4>{}, 0, true);
+    } else {
+        for (int j = lane; j < t.splits; j += 64) {
+            const float x = rec(j)[r];
+            bad |= x != x;
+            m = fmaxf(m, x);
+        }
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, kWave));
+        for (int j0 = 0; j0 < t.splits; j0 += 4) take(std::integral_constant<int, 4>{}, j0, false);
     }
+    if (__any(bad)) return;
     const Row x = row_of(a, t, kvh, row);
     const float inv = l == 0.0f ? 0.0f : (E4M3 ? c.v_scale[kvh] : 1.0f) / l;
     uint16_t* to = a.out + x.m * a.out_row + x.h * D + lane * kPer;
@@ -1105,71 +1122,72 @@ __device__ void merge_tokens(const PagedView& c, const PagedAttentionCall& a, in
                              int first, int stride) {
     constexpr int DB = D < kMergeDims ? D : kMergeDims, kBlocks = D / DB, kCols = DB / 4, kGroups = 256 / kCols, kAhead = 4;
     __shared__ float4 ov[kGroups][kCols];
-    const int lane = threadIdx.x & 63, col = threadIdx.x % kCols, grp = threadIdx.x / kCols;
+    __shared__ float om[kGroups], ol[kGroups];
+    const int col = threadIdx.x % kCols, grp = threadIdx.x / kCols;
     constexpr int kAlign = TokenShape<D, E4M3>::kTile;
     const int64_t size = record_floats(kTokenRows, D);
     const TokenWalk walk = token_walk(c, a, groups, kAlign);
     Piece t;
-    // blocks of kMergeTokenRows rows; the dims of one are dealt out too where its records are many
-    for (int u = first; u < blocks * kBlocks && token_block(c, a, walk, kAlign, kMergeTokenRows, u / kBlocks, &t); u += stride) {
-        const int d = u % kBlocks * DB + 4 * col, nr = min(kMergeTokenRows, t.n * a.group - t.row);  // one tile a sequence
+    // the dims of a block are dealt out too where its records are many
+    for (int u = first; u < blocks * kBlocks && token_block(c, a, walk, kAlign, u / kBlocks, &t); u += stride) {
         const float* base = part + ((int64_t)kvh * 2 * groups + t.record) * size;
         auto rec = [&](int j) { return base + (2 * j + (j == 0)) * size; };
         if (t.splits <= kMergeWaveSplits) {
-            const int i = threadIdx.x >> 6;
-            if (u % kBlocks == 0 && i < nr) merge_row<D, E4M3>(c, a, t, kvh, rec, kTokenRows, t.row + i, t.row + i);
+            const int r = t.row + (threadIdx.x >> 6);
+            if (u % kBlocks == 0 && r < t.n * a.group) merge_row<D, E4M3>(c, a, t, kvh, rec, kTokenRows, r, r);
             continue;
         }
-        for (int r = t.row; r < t.row + nr; ++r) {
-            float m = -INFINITY, l = 0.0f;
-            bool bad = false;
-            for (int j = lane; j < t.splits; j += 64) {
-                const float x = rec(j)[r];
-                bad |= x != x;
-                m = fmaxf(m, x);
+        const int r = t.row, d = u % kBlocks * DB + 4 * col, at = 2 * kTokenRows + r * D + d;
+        // this group's records, with a running maximum (rescaled at most 512 / kGroups / kAhead times)
+        float m = -INFINITY, l = 0.0f;
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        bool bad = false;
+        for (int j0 = grp; j0 < t.splits; j0 += kGroups * kAhead) {
+            float x[kAhead], y[kAhead], most = m;
+            float4 w[kAhead];
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) {
+                const float* from = rec(min(j0 + k * kGroups, t.splits - 1));
+                x[k] = from[r];
+                y[k] = from[kTokenRows + r];
+                w[k] = *reinterpret_cast<const float4*>(from + at);
             }
 #pragma unroll
-            for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, kWave));
-            bad = __any(bad);  // of all lanes, before they part
-            for (int j = lane; j < t.splits; j += 64) {
-                const float x = rec(j)[r];
-                l = fmaf(x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x - m), rec(j)[kTokenRows + r], l);
+            for (int k = 0; k < kAhead; ++k) bad |= x[k] != x[k], most = fmaxf(most, x[k]);
+            const float g = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - most);
+            m = most;
+            l *= g, v.x *= g, v.y *= g, v.z *= g, v.w *= g;
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) {
+                if (j0 + k * kGroups >= t.splits) continue;
+                const float f = x[k] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x[k] - m);
+                l = fmaf(f, y[k], l);
+                v.x = fmaf(f, w[k].x, v.x), v.y = fmaf(f, w[k].y, v.y);
+                v.z = fmaf(f, w[k].z, v.z), v.w = fmaf(f, w[k].w, v.w);
             }
-            l = wave_sum(l);
-            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            const int at = 2 * kTokenRows + r * D + d;
-            for (int j0 = grp; j0 < t.splits; j0 += kGroups * kAhead) {
-                float f[kAhead];
-                float4 y[kAhead];
+        }
+        ov[grp][col] = v;
+        if (col == 0) om[grp] = bad ? NAN : m, ol[grp] = l;
+        __syncthreads();
+        if (grp == 0) {
+            m = -INFINITY, l = 0.0f, v = make_float4(0.0f, 0.0f, 0.0f, 0.0f), bad = false;
 #pragma unroll
-                for (int k = 0; k < kAhead; ++k) {
-                    const int j = min(j0 + k * kGroups, t.splits - 1);
-                    const float x = rec(j)[r];
-                    y[k] = *reinterpret_cast<const float4*>(rec(j) + at);
-                    f[k] = x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x - m);
-                }
+            for (int k = 0; k < kGroups; ++k) bad |= om[k] != om[k], m = fmaxf(m, om[k]);
 #pragma unroll
-                for (int k = 0; k < kAhead; ++k)
-                    if (j0 + k * kGroups < t.splits) {
-                        v.x = fmaf(f[k], y[k].x, v.x), v.y = fmaf(f[k], y[k].y, v.y);
-                        v.z = fmaf(f[k], y[k].z, v.z), v.w = fmaf(f[k], y[k].w, v.w);
-                    }
+            for (int k = 0; k < kGroups; ++k) {
+                const float f = om[k] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(om[k] - m);
+                const float4 y = ov[k][col];
+                l = fmaf(f, ol[k], l);
+                v.x = fmaf(f, y.x, v.x), v.y = fmaf(f, y.y, v.y), v.z = fmaf(f, y.z, v.z), v.w = fmaf(f, y.w, v.w);
             }
-            ov[grp][col] = v;
-            __syncthreads();
-            if (grp == 0 && !bad) {
-#pragma unroll
-                for (int k = 1; k < kGroups; ++k) {
-                    const float4 y = ov[k][col];
-                    v.x += y.x, v.y += y.y, v.z += y.z, v.w += y.w;
-                }
+            if (!bad) {
                 const Row x = row_of(a, t, kvh, r);
                 const float inv = l == 0.0f ? 0.0f : (E4M3 ? c.v_scale[kvh] : 1.0f) / l;
                 *reinterpret_cast<uint2*>(a.out + x.m * a.out_row + x.h * D + d) =
                     make_uint2(pk_bf16(v.x * inv, v.y * inv), pk_bf16(v.z * inv, v.w * inv));
             }
-            __syncthreads();
         }
+        __syncthreads();
     }
 }
 
@@ -1219,7 +1237,7 @@ hipError_t launch(const PagedView& c, const PagedAttentionCall& a, hipStream_t s
         if (e != hipSuccess) return e;
     }
     // blocks of rows of split sequences, at most; each has another group's part
-    int64_t token_blocks = groups > 1 ? std::min<int64_t>((int64_t)a.rows * a.group / kMergeTokenRows + sequences, (int64_t)groups * (kTokenRows / kMergeTokenRows)) : 0;
+    int64_t token_blocks = groups > 1 ? std::min<int64_t>((int64_t)a.rows * a.group, (int64_t)groups * kTokenRows) : 0;
     const int64_t token_wgs = std::min<int64_t>(token_blocks * std::max(1, D / kMergeDims), std::max(1, (chunks_too ? 512 : 2048) / heads));
     int64_t chunk_wgs = 0;
     ChunkPlan chunks{};
