@@ -640,7 +640,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(TokenShape<
 // 2^-8 of itself: a second part, as in the token kernel, would add half as much matrix work again for a result that
 // is rounded to bf16 anyway. The sum adds the weights as they enter, in f32: their roundings then cancel in part.
 // 512 dims: a row's Q and out do not fit beside each other in a wave's registers, so two waves share 32 rows, each with
-// half of the dims: they add the halves of the scores through LDS, and both weigh them.
+// half of the dims: they add the halves of the scores through LDS, and each weighs half of the positions for both (1000 rows of
+// 16 heads over 15800 positions: 672 us, 682 where both weigh all).
 template <int D, bool E4M3>
 struct ChunkShape {
     static constexpr int kTile = D >= 256 ? 32 : 64;
@@ -832,6 +833,12 @@ __device__ __forceinline__ void chunk_part(const PagedView& c, const PagedAttent
             }
         };
 
+        // pairs: what the waves of the workgroup wrote for each other is there; loads into LDS stay in flight
+        auto exchanged = [] {
+            __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            __asm__ volatile("" ::: "memory");
+        };
         auto compute = [&](uint32_t tile, int t0) __attribute__((always_inline)) {  // tile: the buffer's place in `tiles`
             const bool sees = t0 < any_hi && t0 + kTile > any_lo;
             if (kPair == 1 && !sees) return;
@@ -844,7 +851,7 @@ __device__ __forceinline__ void chunk_part(const PagedView& c, const PagedAttent
             {
                 constexpr int kAhead = T::kSub == 2 ? 2 : 3;
                 const uint8_t* kt = tiles + tile + half * kMine * 2;
-                const int kx = k_address();
+                const int kx = k_address() ^ (kPair == 2 ? half * 16 * T::kRowBytes : 0);  // pairs: own positions first
                 bf16x8 kf[kAhead][T::kSub];
                 auto read_k = [&](int s) __attribute__((always_inline)) {
 #pragma unroll
@@ -862,63 +869,116 @@ __device__ __forceinline__ void chunk_part(const PagedView& c, const PagedAttent
                     __builtin_amdgcn_sched_barrier(0);
                 }
             }
-            if constexpr (kPair == 2) {
-                const int ln = lane_here();
+            uint32_t pw[T::kSub][8];
+            if constexpr (kPair == 1) {
+                if (t0 < all_lo || t0 + kTile > all_hi) {  // some row does not see all of it
+                    const int from = in_loop(see_lo - t0 - 4 * hf), to = in_loop(see_hi - t0 - 4 * hf);
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    xs[(wave * 4 + e) * 64 + ln] = make_float4(sc[0][4 * e], sc[0][4 * e + 1], sc[0][4 * e + 2], sc[0][4 * e + 3]);
-                __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-                __builtin_amdgcn_s_barrier();
-                __asm__ volatile("" ::: "memory");
-                if (!sees) return;
+                    for (int b = 0; b < T::kSub; ++b)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float4 y = xs[((wave ^ 4) * 4 + e) * 64 + ln];
-                    sc[0][4 * e] += y.x, sc[0][4 * e + 1] += y.y, sc[0][4 * e + 2] += y.z, sc[0][4 * e + 3] += y.w;
+                        for (int e = 0; e < 16; ++e) {
+                            const int p = 32 * b + 8 * (e >> 2) + (e & 3);
+                            sc[b][e] = p >= from && p < to ? sc[b][e] : -INFINITY;
+                        }
                 }
-            }
-            if (t0 < all_lo || t0 + kTile > all_hi) {  // some row does not see all of it
-                const int from = in_loop(see_lo - t0 - 4 * hf), to = in_loop(see_hi - t0 - 4 * hf);
+                float mx = -INFINITY;
 #pragma unroll
                 for (int b = 0; b < T::kSub; ++b)
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        const int p = 32 * b + 8 * (e >> 2) + (e & 3);
-                        sc[b][e] = p >= from && p < to ? sc[b][e] : -INFINITY;
-                    }
-            }
-            float mx = -INFINITY;
-#pragma unroll
-            for (int b = 0; b < T::kSub; ++b)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) mx = fmaxf(mx, sc[b][e]);
-            mx = fmaxf(mx, __shfl_xor(mx, 32));
-            m_run = fmaxf(m_run, mx * factor);
-            float scale = 1.0f;
-            if (m_run > m_ref + kSlack) {
-                scale = m_ref == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m_ref - m_run);
-                m_ref = m_run;
-            }
-            if (__any(scale != 1.0f)) {
-#pragma unroll
-                for (int d = 0; d < kDims; ++d)
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) o[d][e] *= scale;
-            }
-            const float mu = m_ref == -INFINITY ? 0.0f : m_ref;
-            uint32_t pw[T::kSub][8];
-            float sum = 0.0f;
-            const bf16x2 ones = {(__bf16)1.0f, (__bf16)1.0f};
-#pragma unroll
-            for (int b = 0; b < T::kSub; ++b)
-#pragma unroll
-                for (int e = 0; e < 16; e += 2) {
-                    const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[b][e], factor, -mu));
-                    const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[b][e + 1], factor, -mu));
-                    pw[b][e / 2] = pk_bf16(p0, p1);
-                    sum = dot2_bf16(pw[b][e / 2], ones, sum);
+                    for (int e = 0; e < 16; ++e) mx = fmaxf(mx, sc[b][e]);
+                mx = fmaxf(mx, __shfl_xor(mx, 32));
+                m_run = fmaxf(m_run, mx * factor);
+                float scale = 1.0f;
+                if (m_run > m_ref + kSlack) {
+                    scale = m_ref == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m_ref - m_run);
+                    m_ref = m_run;
                 }
-            l_run = fmaf(l_run, scale, sum);
+                if (__any(scale != 1.0f)) {
+#pragma unroll
+                    for (int d = 0; d < kDims; ++d)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) o[d][e] *= scale;
+                }
+                const float mu = m_ref == -INFINITY ? 0.0f : m_ref;
+                float sum = 0.0f;
+                const bf16x2 ones = {(__bf16)1.0f, (__bf16)1.0f};
+#pragma unroll
+                for (int b = 0; b < T::kSub; ++b)
+#pragma unroll
+                    for (int e = 0; e < 16; e += 2) {
+                        const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[b][e], factor, -mu));
+                        const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[b][e + 1], factor, -mu));
+                        pw[b][e / 2] = pk_bf16(p0, p1);
+                        sum = dot2_bf16(pw[b][e / 2], ones, sum);
+                    }
+                l_run = fmaf(l_run, scale, sum);
+            } else {
+                // The positions of 16 a wave: the other's half of their scores comes through LDS, and the weights go back. A
+                // wave's weights stand against its own reference, a whole number, so that they move to the larger of the
+                // two exactly.
+                const int ln = lane_here();
+                float4 *out = xs + wave * 256 + ln, *in = xs + (wave ^ 4) * 256 + ln;  // two of scores, one of weights, references
+                out[0] = make_float4(sc[0][8], sc[0][9], sc[0][10], sc[0][11]);
+                out[64] = make_float4(sc[0][12], sc[0][13], sc[0][14], sc[0][15]);
+                exchanged();
+                if (!sees) {
+                    exchanged();
+                    return;
+                }
+                const float4 y0 = in[0], y1 = in[64];
+                float x[8] = {sc[0][0] + y0.x, sc[0][1] + y0.y, sc[0][2] + y0.z, sc[0][3] + y0.w,
+                              sc[0][4] + y1.x, sc[0][5] + y1.y, sc[0][6] + y1.z, sc[0][7] + y1.w};
+                if (t0 < all_lo || t0 + kTile > all_hi) {  // some row does not see all of it
+                    const int from = in_loop(see_lo - t0 - 4 * hf - 16 * half), to = in_loop(see_hi - t0 - 4 * hf - 16 * half);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const int p = 8 * (e >> 2) + (e & 3);
+                        x[e] = p >= from && p < to ? x[e] : -INFINITY;
+                    }
+                }
+                float mx = x[0];
+#pragma unroll
+                for (int e = 1; e < 8; ++e) mx = fmaxf(mx, x[e]);
+                mx = fmaxf(mx, __shfl_xor(mx, 32)) * factor;
+                const float r = mx > m_ref + kSlack ? ceilf(mx) : m_ref, mu = r == -INFINITY ? 0.0f : r;
+#pragma unroll
+                for (int e = 0; e < 8; e += 2)
+                    pw[0][e / 2] = pk_bf16(__builtin_amdgcn_exp2f(fmaf(x[e], factor, -mu)), __builtin_amdgcn_exp2f(fmaf(x[e + 1], factor, -mu)));
+                reinterpret_cast<uint4*>(out)[128] = make_uint4(pw[0][0], pw[0][1], pw[0][2], pw[0][3]);
+                reinterpret_cast<float*>(xs + wave * 256 + 192)[ln] = r;
+                exchanged();
+                const uint4 other = reinterpret_cast<const uint4*>(in)[128];
+                const float s = reinterpret_cast<const float*>(xs + (wave ^ 4) * 256 + 192)[ln], most = fmaxf(r, s);
+                const uint32_t theirs[4] = {other.x, other.y, other.z, other.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t own = pw[0][i];
+                    pw[0][i] = half ? theirs[i] : own;
+                    pw[0][4 + i] = half ? own : theirs[i];
+                }
+                const float scale = most == m_ref || m_ref == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m_ref - most);
+                const bool moved = __any(most != m_ref);
+                m_ref = most;
+                if (__any(scale != 1.0f)) {
+#pragma unroll
+                    for (int d = 0; d < kDims; ++d)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) o[d][e] *= scale;
+                }
+                if (moved) {
+                    const float f = r == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(r - most), g = s == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(s - most);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const float h = (i < 4) == (half == 0) ? f : g;
+                        pw[0][i] = pk_bf16(bf2f(pw[0][i] & 0xffffu) * h, bf2f(pw[0][i] >> 16) * h);
+                    }
+                }
+                const bf16x2 ones = {(__bf16)1.0f, (__bf16)1.0f};
+                float sum = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) sum = dot2_bf16(pw[0][i], ones, sum);
+                l_run = fmaf(l_run, scale, sum);
+            }
             {
                 constexpr int kAhead = 2, kN = T::kSub * kDims;  // step n: 32 positions n / kDims, dim tile n % kDims
                 uint8_t* vt = tiles + tile + kTileBytes + half * kMine * 2;
@@ -1052,8 +1112,8 @@ __global__ __launch_bounds__((ChunkShape<D, E4M3>::kThreads)) __attribute__((amd
 // Rows of split tiles, both kernels' in one launch. A workgroup takes a block of rows of a tile and finds it once. Few
 // splits: a wave per row, its lanes across the dims. More (long sequences of few rows): the workgroup takes 128 dims of a
 // row, its threads in groups that take the records in turn. Bound by its chain of round trips where the records are few, so maxima,
-// sums and outputs are asked for at once. (250 records of 128 rows of 512: 15.8 us, 19.5 with the maxima first; 16 single tokens
-// of 8 heads of 128 in some 500 records: 8.4 and 10.6.)
+// sums and outputs are asked for at once. (250 records of 128 rows of 512: 15.8 us, 19.5 with the maxima first; 64 times 16 rows of
+// 8 heads of 128: 8.4 and 10.6.)
 constexpr int kMergeDims = 128;
 constexpr int kMergeChunkRows = 8;
 
