@@ -189,17 +189,20 @@ __device__ __forceinline__ int chunk_units(const PagedAttentionCall& a, const Se
     return max(1, (seen + kChunkUnit - 1) / kChunkUnit);
 }
 
-__device__ ChunkWalk chunk_walk(const PagedView& c, const PagedAttentionCall& a, const ChunkPlan& p) {
+// last: the last 64 sequences' lanes, the only ones of most calls.
+__device__ ChunkWalk chunk_walk(const PagedView& c, const PagedAttentionCall& a, const ChunkPlan& p, Seq* last) {
     int tiles = 0;
     float units = 0.0f;
     bool bad = false;
+    Seq q = {};
 #pragma unroll 4
     for (int base = 0; base < c.sequences; base += 64) {
-        const Seq q = seq_of(c, a, base + (threadIdx.x & 63), false, &bad);
+        q = seq_of(c, a, base + (threadIdx.x & 63), false, &bad);
         const int n = chunk_tiles(a, q);
         tiles = min(tiles + n, 1 << 24);
         units += (float)n * (float)chunk_units(a, q);
     }
+    *last = q;
     tiles = wave_total(tiles);
     // More tiles than the call's rows can have: sequences whose rows overlap, by row starts that descend. None of them runs.
     bad |= tiles > p.most - p.items;
@@ -212,13 +215,16 @@ __device__ ChunkWalk chunk_walk(const PagedView& c, const PagedAttentionCall& a,
     return {__builtin_amdgcn_readfirstlane(max(kChunkMinUnits, per)), 0, 0, 0};
 }
 
-// Piece `want`, not before an earlier call's. False: there are not that many.
-__device__ bool find_piece(const PagedView& c, const PagedAttentionCall& a, ChunkWalk& w, int merge_rows, int want, Piece* out) {
+// Piece `want`, not before an earlier call's. False: there are not that many. have: the only 64 sequences' lanes, or nullptr.
+__device__ __forceinline__ bool find_piece(const PagedView& c, const PagedAttentionCall& a, ChunkWalk& w, int merge_rows, int want, const Seq* have,
+                                           Piece* out) {
     const int lane = threadIdx.x & 63;
     bool bad = false;
     if (w.per == 0) return false;
     for (; w.base < c.sequences; w.base += 64) {
-        const Seq q = seq_of(c, a, w.base + lane, false, &bad);
+        Seq q;
+        if (have && c.sequences <= 64) q = *have;
+        else q = seq_of(c, a, w.base + lane, false, &bad);
         const int tiles = chunk_tiles(a, q), splits = q.n ? (chunk_units(a, q) + w.per - 1) / w.per : 0, items = tiles * splits;
         const int records = splits > 1 ? items : 0, xr = scan_sum(records);
         const int pieces = !merge_rows ? items : (splits > 1 ? (q.n * a.group + merge_rows - 1) / merge_rows : 0), x = scan_sum(pieces);
@@ -732,9 +738,10 @@ __device__ __forceinline__ void chunk_part(const PagedView& c, const PagedAttent
         const int ln = lane_here(), r = 4 * (ln >> 5) + (ln >> 2 & 3);
         return r * T::kRowBytes + ((2 * (ln >> 4 & 1) + (ln >> 1 & 1)) ^ chunk_swizzle<D>(r)) * 16 + (ln & 1) * 8;
     };
-    ChunkWalk walk = chunk_walk(c, a, plan);
+    Seq seqs;
+    ChunkWalk walk = chunk_walk(c, a, plan, &seqs);
     Piece t;
-    for (int item = first; item < plan.most && find_piece(c, a, walk, 0, item, &t); item += stride) {
+    auto run = [&]() __attribute__((always_inline)) {
         const int r0 = t.tile * kChunkRows, nr = (int)min((int64_t)kChunkRows, (int64_t)t.n * a.group - r0);
         const Span span = span_of(a, t, r0, r0 + nr - 1, kTile);
         const int lo = span.lo, hi = span.hi;
@@ -1081,6 +1088,18 @@ __device__ __forceinline__ void chunk_part(const PagedView& c, const PagedAttent
         }
         if (bad && threadIdx.x == 0) atomicOr(c.err, kErrPaged);
         if (odd && !bad) careful_piece<E4M3>(c, a, t, kvh, r0, nr, lo, hi, [&](int, const Row& x) { return a.q + x.m * a.q_row + x.h * D; }, rec, kChunkRows);
+    };
+    // Few workgroups have a second item: the first takes the sequences that the walk has read (four prompts of 32 heads of 128,
+    // five items in turn on a place: 251 us, 254 with them read again; 512 dims: 683 and 675, for want of registers).
+    int item = first;
+    if constexpr (kPair == 1) {
+        if (item >= plan.most || !find_piece(c, a, walk, 0, item, &seqs, &t)) return;
+        do {
+            run();
+            item += stride;
+        } while (item < plan.most && find_piece(c, a, walk, 0, item, nullptr, &t));
+    } else {
+        for (; item < plan.most && find_piece(c, a, walk, 0, item, nullptr, &t); item += stride) run();
     }
 }
 
@@ -1254,9 +1273,10 @@ __device__ void merge_tokens(const PagedView& c, const PagedAttentionCall& a, in
 template <int D, bool E4M3>
 __device__ void merge_chunks(const PagedView& c, const PagedAttentionCall& a, const ChunkPlan& plan, const float* part, int kvh, int first,
                              int stride) {
-    ChunkWalk walk = chunk_walk(c, a, plan);
+    Seq seqs;
+    ChunkWalk walk = chunk_walk(c, a, plan, &seqs);
     Piece t;
-    for (int u = first; u < plan.most_blocks && find_piece(c, a, walk, kMergeChunkRows, u, &t); u += stride) {
+    for (int u = first; u < plan.most_blocks && find_piece(c, a, walk, kMergeChunkRows, u, &seqs, &t); u += stride) {
         const float* base = part + ((int64_t)kvh * plan.items + t.record) * record_floats(kChunkRows, D);
         auto rec = [&](int j) { return base + j * record_floats(kChunkRows, D); };
         const int rows = min(kMergeChunkRows, t.n * a.group - t.row);
