@@ -409,8 +409,8 @@ __global__ __launch_bounds__(kCopyBlock) void paged_compact_kernel(PagedView c, 
 // -------------------------------------------------------------------------------------------- append
 
 // One wave per row: it finds the row's sequence, then moves K and V, 8 elements a lane and step. Bound by memory: 10500
-// rows of 8 heads of 128 into E4M3 pages (65 MB) 18 us a layer, 3.6 TB/s; the other waves of a CU hide a wave's own steps
-// (loads sent ahead of the search: 19 us; a residual step in the division's place: 19).
+// rows of 8 heads of 128 into E4M3 pages (65 MB) 17 us a layer, 3.8 TB/s; the other waves of a CU hide a wave's own steps
+// (loads sent ahead of the search, or a residual step in the division's place: 1 us more).
 template <bool E4M3>
 __global__ __launch_bounds__(256) void paged_append_kernel(PagedView c, const uint16_t* k, int64_t k_row, const uint16_t* v,
                                                            int64_t v_row, const int32_t* starts, int rows) {
