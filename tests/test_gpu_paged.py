@@ -996,3 +996,69 @@ def test_random_shapes(seed):
     st = Setup(lens, slots, heads, dim, fmt, seed=seed, layout=layout, poison=True)
     # poisoned slots are NaN: the oracle reads only the visible ones
     attend(st, rows, heads * group, window=window, scale=scale, first=rng.choice([0, 2]), tail=rng.choice([0, 3]))
+
+
+def test_the_front_end_refuses():
+    """Tensors of a wrong type, shape, device or order never reach the library, and nothing is written."""
+    need_gpu()
+    say("paged front end refusals")
+    st = Setup([20, 3], 16, 2, 64, seed=60, spare=4)
+    before = [t.clone() for t in (st.k, st.v, st.table, st.lens, st.refs)]
+    q, out, kv = queries(4, 8, 64, 1), queries(4, 8, 64, 2), queries(4, 2, 64, 3)
+    starts, held = i32([0, 3, 4]), out.clone()
+    make = lambda **kw: ops.PagedCache(**{**dict(k_pages=st.k, v_pages=st.v, page_table=st.table, seq_lens=st.lens,  # noqa: E731
+                                                ref_counts=st.refs), **kw})
+    codes = st.k.to(torch.float8_e4m3fn)
+    scale = torch.ones((1, 2), device=DEV)
+    calls = {
+        "a page pool on the host": lambda: make(k_pages=st.k.cpu()),
+        "a table on the host": lambda: make(page_table=st.table.cpu()),
+        "pages of other shapes": lambda: make(v_pages=st.v[:, :-1]),
+        "pages of other types": lambda: make(v_pages=codes),
+        "f32 pages": lambda: make(k_pages=st.k.float(), v_pages=st.v.float()),
+        "head dims apart": lambda: make(k_pages=st.k.transpose(3, 4), v_pages=st.v.transpose(3, 4)),
+        "no pages": lambda: make(k_pages=st.k[:, :0], v_pages=st.v[:, :0]),
+        "codes without scales": lambda: make(k_pages=codes, v_pages=codes),
+        "codes with one scale": lambda: make(k_pages=codes, v_pages=codes, k_scale=scale),
+        "scales of another layer count": lambda: make(k_pages=codes, v_pages=codes, k_scale=scale[:, :1], v_scale=scale),
+        "scales with bf16": lambda: make(k_scale=scale, v_scale=scale),
+        "a table of int64": lambda: make(page_table=st.table.long()),
+        "a table with columns apart": lambda: make(page_table=st.table.t()),
+        "lengths of another number": lambda: make(seq_lens=i32([1, 2, 3])),
+        "counts of another number": lambda: make(ref_counts=st.refs[:-1]),
+        "lengths that are a list": lambda: make(seq_lens=[20, 3]),
+        "no cache": lambda: ops.paged_cache_compact(st),
+        "new tokens of another number": lambda: ops.paged_cache_reserve(st.cache, i32([1])),
+        "new tokens of int64": lambda: ops.paged_cache_reserve(st.cache, i32([1, 1]).long()),
+        "new tokens on the host": lambda: ops.paged_cache_reserve(st.cache, i32([1, 1]).cpu()),
+        "new tokens apart": lambda: ops.paged_cache_reserve(st.cache, i32([1, 0, 1, 0])[::2]),
+        "row starts of another number": lambda: ops.paged_cache_append(st.cache, kv, kv, i32([0, 4])),
+        "k of other heads": lambda: ops.paged_cache_append(st.cache, q, kv, starts),
+        "v of other rows": lambda: ops.paged_cache_append(st.cache, kv, kv[:3], starts),
+        "f32 rows": lambda: ops.paged_cache_append(st.cache, kv.float(), kv, starts),
+        "flat rows": lambda: ops.paged_cache_append(st.cache, kv.view(4, 128), kv, starts),
+        "heads apart": lambda: ops.paged_cache_append(st.cache, queries(4, 4, 64, 3)[:, ::2], kv, starts),
+        "dims apart": lambda: ops.paged_cache_append(st.cache, queries(4, 2, 128, 3)[:, :, ::2], kv, starts),
+        "rows on top of each other": lambda: ops.paged_cache_append(st.cache, kv[:1].expand(4, 2, 64), kv, starts),
+        "a layer behind the last": lambda: ops.paged_cache_append(st.cache, kv, kv, starts, layer=1),
+        "a negative layer": lambda: ops.paged_attention(q, st.cache, starts, out, layer=-1),
+        "q of other dims": lambda: ops.paged_attention(queries(4, 8, 128, 1), st.cache, starts, out),
+        "heads that are no multiple": lambda: ops.paged_attention(q[:, :7].contiguous(), st.cache, starts, out[:, :7].contiguous()),
+        "out of other rows": lambda: ops.paged_attention(q, st.cache, starts, out[:3]),
+        "out of other heads": lambda: ops.paged_attention(q, st.cache, starts, queries(4, 4, 64, 1)),
+        "q on the host": lambda: ops.paged_attention(q.cpu(), st.cache, starts, out),
+        "max_rows of zero": lambda: ops.paged_attention(q, st.cache, starts, out, max_rows=0),
+        "max_rows over the rows": lambda: ops.paged_attention(q, st.cache, starts, out, max_rows=5),
+        "a negative window": lambda: ops.paged_attention(q, st.cache, starts, out, window=-1),
+        "an infinite scale": lambda: ops.paged_attention(q, st.cache, starts, out, scale=float("inf")),
+        "q that is not aligned": lambda: ops.paged_attention(queries(5, 8, 64, 1).view(-1)[1:1 + q.numel()].view(q.shape), st.cache, starts, out),
+        "children of another number": lambda: ops.paged_cache_fork(st.cache, i32([0]), i32([0, 1])),
+        "sequences of int64": lambda: ops.paged_cache_free(st.cache, i32([0]).long()),
+    }
+    for name, call in calls.items():
+        with pytest.raises((TypeError, ValueError, _lib.MoaError)):
+            call()
+            pytest.fail(f"{name} was taken")
+    assert ops.device_errors() == 0 and torch.equal(out, held)
+    for t, old in zip((st.k, st.v, st.table, st.lens, st.refs), before):
+        assert torch.equal(t, old)
