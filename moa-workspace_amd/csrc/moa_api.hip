@@ -93,6 +93,7 @@ DevCtx* device_context(hipError_t* err) {
     const size_t t_plist = carve(sizeof(int32_t) * (2 * (size_t)kPagedMaxPages + 16));
     const size_t t_ptok = carve(sizeof(float) * kPagedTokenFloats);
     const size_t t_pchunk = carve(sizeof(float) * kPagedChunkFloats);
+    const size_t t_ptick = carve(sizeof(uint32_t) * kPagedTickets);
     int cus = 0;
     *err = hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev);
     if (*err != hipSuccess) return nullptr;
@@ -125,6 +126,7 @@ DevCtx* device_context(hipError_t* err) {
     c.paged_list = reinterpret_cast<int32_t*>(b + t_plist);
     c.paged_tokens = reinterpret_cast<float*>(b + t_ptok);
     c.paged_chunks = reinterpret_cast<float*>(b + t_pchunk);
+    c.paged_tickets = reinterpret_cast<uint32_t*>(b + t_ptick);
     c.base = base;
     return &c;
 }

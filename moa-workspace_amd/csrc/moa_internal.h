@@ -77,6 +77,7 @@ constexpr int kPagedMaxPages = 1 << 20;
 constexpr int kPagedMaxSequences = 1 << 16;
 constexpr size_t kPagedTokenFloats = (size_t)9 << 19;   // 18.9 MB
 constexpr size_t kPagedChunkFloats = (size_t)17 << 20;  // 71.3 MB
+constexpr int kPagedTickets = 2048;                     // arrivals at split sequences, zero between calls
 
 // Device-side error bits (OR-ed by kernels; read back by moa_device_errors()).
 constexpr uint32_t kErrRopeOffset = 1u;
@@ -105,6 +106,7 @@ struct DevCtx {
     int32_t* paged_list = nullptr;  // 2 * kPagedMaxPages + 16: page lists of a cache call, its result word
     float* paged_tokens = nullptr;  // paged attention's split records (kPagedTokenFloats, kPagedChunkFloats)
     float* paged_chunks = nullptr;
+    uint32_t* paged_tickets = nullptr;  // kPagedTickets
     void* base = nullptr;
     int cus = 0;                  // compute units of the device
     int8_t ffn_fused[6] = {-1, -1, -1, -1, -1, -1};  // per (format, scale kind): grid fits resident? (-1 unknown)

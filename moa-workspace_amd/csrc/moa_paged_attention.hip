@@ -20,6 +20,7 @@ namespace {
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kTokenRows = 16;   // rows of a token-kernel item
+constexpr int kJoinUnits = 16;   // units of a sequence up to which the token kernel joins its own records
 constexpr int kTokenUnit = 128;  // positions that work is dealt out by: one or two steps of four waves
 // Weights are 2^(x - reference), the reference at most this far below the row's largest x so far: the output is
 // rescaled only when the maximum has grown by more.
@@ -404,9 +405,54 @@ __device__ __forceinline__ uint32_t bf16_pair_of_fp8(uint32_t two) {
     return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(two, 1.0f, false));
 }
 
+// A split sequence's last workgroup, found by a counter per (KV head, group that begins it) that it sets back to zero, joins its
+// records: they are written and read past the XCDs' caches (agent scope).
 template <int D, bool E4M3>
+__device__ __forceinline__ void join_records(const PagedView& c, const PagedAttentionCall& a, const Piece& t, int kvh, const float* base, int splits) {
+    constexpr int kAhead = 4, kSize = kTokenRows * (2 + D) * 4;
+    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(base), 0, (uint32_t)(2 * splits * kSize), 0x00020000);
+    const float vs = E4M3 ? c.v_scale[kvh] : 1.0f;
+    const int nr = t.n * a.group;
+    for (int i = threadIdx.x; i < nr * (D / 4); i += 256) {
+        const int r = i / (D / 4), d = 4 * (i - r * (D / 4));
+        float m = -INFINITY, l = 0.0f;
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        bool bad = false;
+        for (int j0 = 0; j0 < splits; j0 += kAhead) {
+            float x[kAhead], y[kAhead], most = m;
+            float4 w[kAhead];
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) {
+                const int j = min(j0 + k, splits - 1), at = (2 * j + (j == 0)) * kSize;
+                x[k] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rs, at + 4 * r, 0, 16 /* sc1 */));
+                y[k] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rs, at + 4 * (kTokenRows + r), 0, 16));
+                w[k] = __builtin_bit_cast(float4, __builtin_amdgcn_raw_buffer_load_b128(rs, at + 4 * (2 * kTokenRows + r * D + d), 0, 16));
+            }
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) bad |= x[k] != x[k], most = fmaxf(most, x[k]);
+            const float g = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - most);
+            m = most;
+            l *= g, v.x *= g, v.y *= g, v.z *= g, v.w *= g;
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) {
+                if (j0 + k >= splits) continue;
+                const float f = x[k] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x[k] - m);
+                l = fmaf(f, y[k], l);
+                v.x = fmaf(f, w[k].x, v.x), v.y = fmaf(f, w[k].y, v.y);
+                v.z = fmaf(f, w[k].z, v.z), v.w = fmaf(f, w[k].w, v.w);
+            }
+        }
+        if (bad) continue;
+        const Row x = row_of(a, t, kvh, r);
+        const float inv = l == 0.0f ? 0.0f : vs / l;
+        *reinterpret_cast<uint2*>(a.out + x.m * a.out_row + x.h * D + d) = make_uint2(pk_bf16(v.x * inv, v.y * inv), pk_bf16(v.z * inv, v.w * inv));
+    }
+}
+
+// kJoin: the workgroups join their records (tickets [kv_heads][groups], zero); else the merge kernel does.
+template <int D, bool E4M3, bool kJoin = false>
 __device__ __forceinline__ void token_part(const PagedView& c, const PagedAttentionCall& a, float* part, int kvh, int group, int groups,
-                                           uint8_t* lds) {
+                                           uint8_t* lds, uint32_t* tickets = nullptr) {
     using T = TokenShape<D, E4M3>;
     constexpr int NT = T::kSub;
     uint16_t* qs = reinterpret_cast<uint16_t*>(lds);                           // [16][kQStride]
@@ -612,7 +658,19 @@ __device__ __forceinline__ void token_part(const PagedView& c, const PagedAttent
                 v[0] = fmaf(f, y.x, v[0]), v[1] = fmaf(f, y.y, v[1]), v[2] = fmaf(f, y.z, v[2]), v[3] = fmaf(f, y.w, v[3]);
             }
             odd |= !(fabsf(v[0]) + fabsf(v[1]) + fabsf(v[2]) + fabsf(v[3]) < INFINITY);
-            if (rec) {
+            if (rec && kJoin) {
+                const __amdgpu_buffer_rsrc_t rs =
+                    __builtin_amdgcn_make_buffer_rsrc(rec, 0, (uint32_t)(kTokenRows * (2 + D) * 4), 0x00020000);
+                const float most = bad ? NAN : m;
+                if (d == 0) {
+                    __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, most), rs, 4 * r, 0, 16 /* sc1 */);
+                    __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, l), rs, 4 * (kTokenRows + r), 0, 16);
+                }
+                typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+                const u32x4 w = {__builtin_bit_cast(uint32_t, v[0]), __builtin_bit_cast(uint32_t, v[1]), __builtin_bit_cast(uint32_t, v[2]),
+                                 __builtin_bit_cast(uint32_t, v[3])};
+                __builtin_amdgcn_raw_buffer_store_b128(w, rs, 4 * (2 * kTokenRows + r * D + d), 0, 16);
+            } else if (rec) {
                 if (d == 0) rec[r] = bad ? NAN : m, rec[kTokenRows + r] = l;
                 *reinterpret_cast<float4*>(rec + 2 * kTokenRows + r * D + d) = make_float4(v[0], v[1], v[2], v[3]);
             } else if (!bad) {
@@ -625,14 +683,31 @@ __device__ __forceinline__ void token_part(const PagedView& c, const PagedAttent
         odd = __syncthreads_or(odd);
         if (bad && threadIdx.x == 0) atomicOr(c.err, kErrPaged);
         if (odd && !bad) careful_piece<E4M3>(c, a, t, kvh, 0, nr, lo, hi, [&](int r, const Row&) { return qs + r * T::kQStride; }, rec, kTokenRows);
+        if constexpr (kJoin) {
+            if (rec) {
+                if (odd && !bad) __threadfence();  // the careful path's stores stop at the XCD's cache
+                __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                __syncthreads();
+                const int w0 = (int)((uint32_t)first / (uint32_t)walk.q), w1 = (int)((uint32_t)(first + units - 1) / (uint32_t)walk.q);
+                uint32_t* flag = reinterpret_cast<uint32_t*>(ms);
+                if (threadIdx.x == 0) {
+                    uint32_t* ticket = tickets + kvh * groups + w0;
+                    const bool last = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)(w1 - w0);
+                    if (last) __hip_atomic_store(ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                    *flag = last;
+                }
+                __syncthreads();
+                if (*flag) join_records<D, E4M3>(c, a, t, kvh, part + ((int64_t)kvh * 2 * groups + 2 * w0) * record_floats(kTokenRows, D), w1 - w0 + 1);
+            }
+        }
     }
 }
 
-template <int D, bool E4M3>
+template <int D, bool E4M3, bool kJoin>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(TokenShape<D, E4M3>::kHeld))) void paged_token_kernel(
-    PagedView c, PagedAttentionCall a, float* part) {
+    PagedView c, PagedAttentionCall a, float* part, uint32_t* tickets) {
     __shared__ __attribute__((aligned(16))) uint8_t lds[TokenShape<D, E4M3>::kLds];
-    token_part<D, E4M3>(c, a, part, blockIdx.x % c.kv_heads, blockIdx.x / c.kv_heads, gridDim.x / c.kv_heads, lds);
+    token_part<D, E4M3, kJoin>(c, a, part, blockIdx.x % c.kv_heads, blockIdx.x / c.kv_heads, gridDim.x / c.kv_heads, lds, tickets);
 }
 
 // ------------------------------------------------------------------------------------ the chunk kernel
@@ -1311,8 +1386,16 @@ hipError_t launch(const PagedView& c, const PagedAttentionCall& a, hipStream_t s
     const int groups = (int)clamp64(std::min<int64_t>((int64_t)ctx->cus * (one_launch ? 1 : T::kHeld) / heads, sequences * units), 1,
                                     (int64_t)kPagedTokenFloats / record_floats(kTokenRows, D) / heads / 2);
     hipError_t e = hipSuccess;
+    // Few parts of a sequence at most: the workgroup that ends last joins them, without a second launch.
+    const bool join = !chunks_too && units <= kJoinUnits && (int64_t)groups * heads <= kPagedTickets && sequences * units < (1 << 30);
+    if (join) {
+        hipLaunchKernelGGL((paged_token_kernel<D, E4M3, true>), dim3((uint32_t)(groups * heads)), dim3(256), 0, s, c, a, ctx->paged_tokens,
+                           ctx->paged_tickets);
+        return hipGetLastError();
+    }
     if (!one_launch) {
-        hipLaunchKernelGGL((paged_token_kernel<D, E4M3>), dim3((uint32_t)(groups * heads)), dim3(256), 0, s, c, a, ctx->paged_tokens);
+        hipLaunchKernelGGL((paged_token_kernel<D, E4M3, false>), dim3((uint32_t)(groups * heads)), dim3(256), 0, s, c, a, ctx->paged_tokens,
+                           ctx->paged_tickets);
         e = hipGetLastError();
         if (e != hipSuccess) return e;
     }
