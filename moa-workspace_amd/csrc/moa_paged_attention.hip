@@ -20,7 +20,6 @@ namespace {
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kTokenRows = 16;   // rows of a token-kernel item
-constexpr int kJoinUnits = 16;   // units of a sequence up to which the token kernel joins its own records
 constexpr int kTokenUnit = 128;  // positions that work is dealt out by: one or two steps of four waves
 // Weights are 2^(x - reference), the reference at most this far below the row's largest x so far: the output is
 // rescaled only when the maximum has grown by more.
@@ -406,47 +405,52 @@ __device__ __forceinline__ uint32_t bf16_pair_of_fp8(uint32_t two) {
 }
 
 // A split sequence's last workgroup, found by a counter per (KV head, group that begins it) that it sets back to zero, joins its
-// records: they are written and read past the XCDs' caches (agent scope).
+// records: they are written and read past the XCDs' caches (agent scope). A thread takes four dims of a row, so this is for
+// few rows, and for few parts, which it reads one batch after the other: rows * dims up to kJoinElements, up to kJoinUnits units
+// a sequence. One token of 8 x 2 heads of 256 over 700 positions: 11.8 us, 13.6 with a merge launch; 120 of them in a window of
+// 1024: 158 and 166. Beyond: 4 tokens (8 rows) over 700 to 1500 positions 16.7 and 14.4, one sequence of 16 rows of 512 38.9 and
+// 20.6, two tokens over 4000 to 5000 positions 27.7 and 24.4.
+constexpr int kJoinUnits = 16;
+constexpr int kJoinElements = 1024;
+
 template <int D, bool E4M3>
 __device__ __forceinline__ void join_records(const PagedView& c, const PagedAttentionCall& a, const Piece& t, int kvh, const float* base, int splits) {
-    constexpr int kAhead = 4, kSize = kTokenRows * (2 + D) * 4;
+    constexpr int kAhead = 8, kSize = kTokenRows * (2 + D) * 4;
     const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(base), 0, (uint32_t)(2 * splits * kSize), 0x00020000);
     const float vs = E4M3 ? c.v_scale[kvh] : 1.0f;
-    const int nr = t.n * a.group;
-    for (int i = threadIdx.x; i < nr * (D / 4); i += 256) {
-        const int r = i / (D / 4), d = 4 * (i - r * (D / 4));
-        float m = -INFINITY, l = 0.0f;
-        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        bool bad = false;
-        for (int j0 = 0; j0 < splits; j0 += kAhead) {
-            float x[kAhead], y[kAhead], most = m;
-            float4 w[kAhead];
+    const int r = threadIdx.x / (D / 4), d = 4 * (threadIdx.x - r * (D / 4));
+    if (r >= t.n * a.group) return;
+    float m = -INFINITY, l = 0.0f;
+    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    bool bad = false;
+    for (int j0 = 0; j0 < splits; j0 += kAhead) {
+        float x[kAhead], y[kAhead], most = m;
+        float4 w[kAhead];
 #pragma unroll
-            for (int k = 0; k < kAhead; ++k) {
-                const int j = min(j0 + k, splits - 1), at = (2 * j + (j == 0)) * kSize;
-                x[k] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rs, at + 4 * r, 0, 16 /* sc1 */));
-                y[k] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rs, at + 4 * (kTokenRows + r), 0, 16));
-                w[k] = __builtin_bit_cast(float4, __builtin_amdgcn_raw_buffer_load_b128(rs, at + 4 * (2 * kTokenRows + r * D + d), 0, 16));
-            }
-#pragma unroll
-            for (int k = 0; k < kAhead; ++k) bad |= x[k] != x[k], most = fmaxf(most, x[k]);
-            const float g = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - most);
-            m = most;
-            l *= g, v.x *= g, v.y *= g, v.z *= g, v.w *= g;
-#pragma unroll
-            for (int k = 0; k < kAhead; ++k) {
-                if (j0 + k >= splits) continue;
-                const float f = x[k] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x[k] - m);
-                l = fmaf(f, y[k], l);
-                v.x = fmaf(f, w[k].x, v.x), v.y = fmaf(f, w[k].y, v.y);
-                v.z = fmaf(f, w[k].z, v.z), v.w = fmaf(f, w[k].w, v.w);
-            }
+        for (int k = 0; k < kAhead; ++k) {
+            const int j = min(j0 + k, splits - 1), at = (2 * j + (j == 0)) * kSize;
+            x[k] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rs, at + 4 * r, 0, 16 /* sc1 */));
+            y[k] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rs, at + 4 * (kTokenRows + r), 0, 16));
+            w[k] = __builtin_bit_cast(float4, __builtin_amdgcn_raw_buffer_load_b128(rs, at + 4 * (2 * kTokenRows + r * D + d), 0, 16));
         }
-        if (bad) continue;
-        const Row x = row_of(a, t, kvh, r);
-        const float inv = l == 0.0f ? 0.0f : vs / l;
-        *reinterpret_cast<uint2*>(a.out + x.m * a.out_row + x.h * D + d) = make_uint2(pk_bf16(v.x * inv, v.y * inv), pk_bf16(v.z * inv, v.w * inv));
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) bad |= x[k] != x[k], most = fmaxf(most, x[k]);
+        const float g = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - most);
+        m = most;
+        l *= g, v.x *= g, v.y *= g, v.z *= g, v.w *= g;
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+            if (j0 + k >= splits) continue;
+            const float f = x[k] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x[k] - m);
+            l = fmaf(f, y[k], l);
+            v.x = fmaf(f, w[k].x, v.x), v.y = fmaf(f, w[k].y, v.y);
+            v.z = fmaf(f, w[k].z, v.z), v.w = fmaf(f, w[k].w, v.w);
+        }
     }
+    if (bad) return;
+    const Row x = row_of(a, t, kvh, r);
+    const float inv = l == 0.0f ? 0.0f : vs / l;
+    *reinterpret_cast<uint2*>(a.out + x.m * a.out_row + x.h * D + d) = make_uint2(pk_bf16(v.x * inv, v.y * inv), pk_bf16(v.z * inv, v.w * inv));
 }
 
 // kJoin: the workgroups join their records (tickets [kv_heads][groups], zero); else the merge kernel does.
@@ -1386,8 +1390,7 @@ hipError_t launch(const PagedView& c, const PagedAttentionCall& a, hipStream_t s
     const int groups = (int)clamp64(std::min<int64_t>((int64_t)ctx->cus * (one_launch ? 1 : T::kHeld) / heads, sequences * units), 1,
                                     (int64_t)kPagedTokenFloats / record_floats(kTokenRows, D) / heads / 2);
     hipError_t e = hipSuccess;
-    // Few parts of a sequence at most: the workgroup that ends last joins them, without a second launch.
-    const bool join = !chunks_too && units <= kJoinUnits && (int64_t)groups * heads <= kPagedTickets && sequences * units < (1 << 30);
+    const bool join = !chunks_too && units <= kJoinUnits && (int64_t)a.max_rows * a.group * D <= kJoinElements && (int64_t)groups * heads <= kPagedTickets;
     if (join) {
         hipLaunchKernelGGL((paged_token_kernel<D, E4M3, true>), dim3((uint32_t)(groups * heads)), dim3(256), 0, s, c, a, ctx->paged_tokens,
                            ctx->paged_tickets);

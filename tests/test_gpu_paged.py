@@ -1062,3 +1062,33 @@ def test_the_front_end_refuses():
     assert ops.device_errors() == 0 and torch.equal(out, held)
     for t, old in zip((st.k, st.v, st.table, st.lens, st.refs), before):
         assert torch.equal(t, old)
+
+
+def test_joined_records_leave_nothing_for_the_next_call():
+    """Single tokens in a window, whose parts are joined by their last workgroup: calls of other shapes, with bad pages and
+    with NaN between, and each result stays bit for bit what it was."""
+    need_gpu()
+    say("paged attention, joined records call after call")
+    made = []
+    for i, (lens, heads, group, dim, fmt, window) in enumerate([([700], 8, 2, 256, "bf16", 1024), ([1500, 9, 1100, 640], 8, 2, 256, "e4m3", 1024),
+                                                                ([300] * 70, 2, 4, 128, "bf16", 0), ([1900], 1, 2, 512, "bf16", 1500)]):
+        st = Setup(lens, 16, heads, dim, fmt, seed=70 + i)
+        q = queries(len(lens), heads * group, dim, 80 + i)
+        out = attend(st, [1] * len(lens), heads * group, window=window, q=q, max_rows=1)
+        made.append((st, q, out, i32(range(len(lens) + 1)), window))
+    for turn in range(6):
+        for st, q, want, starts, window in made:
+            got = torch.empty_like(q)
+            good = st.table.clone()
+            if turn in (1, 4):  # a bad page of the first sequence, inside its window
+                st.table[0, (st.state.lens[0] - 1) // 16 - 3 * turn] = -1
+            sick = q.clone()
+            if turn == 2:
+                sick[0, 0] = float("nan")
+            ops.paged_attention(sick, st.cache, starts, got, window=window, max_rows=1)
+            first = 1 if turn in (1, 2, 4) else 0
+            assert ops.device_errors() == (_lib.DEVERR_PAGED if turn in (1, 4) else 0)
+            assert torch.equal(got[first:], want[first:])
+            if turn == 2:
+                assert torch.isnan(got[0, 0].float()).all() and torch.equal(got[0, 1:], want[0, 1:])
+            st.table.copy_(good)
