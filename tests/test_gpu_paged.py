@@ -1092,3 +1092,25 @@ def test_joined_records_leave_nothing_for_the_next_call():
             if turn == 2:
                 assert torch.isnan(got[0, 0].float()).all() and torch.equal(got[0, 1:], want[0, 1:])
             st.table.copy_(good)
+
+
+@pytest.mark.parametrize("heads,group,dim,fmt", [(8, 2, 256, "bf16"), (8, 1, 128, "e4m3"), (1, 2, 512, "bf16"), (3, 4, 64, "e4m3"), (1, 16, 512, "bf16")])
+def test_a_value_before_the_window_never_reaches_a_joined_row(heads, group, dim, fmt):
+    """A NaN just before the window shares a tile with its first positions; the sequence is split, its first part is
+    computed again, and out is q."""
+    need_gpu()
+    say(f"paged attention, NaN before the window of a split token, {heads} x {group} of {dim} {fmt}")
+    st = Setup([1900, 1500], 16, heads, dim, fmt, seed=90)
+    clean = tuple(t.clone() for t in st.values())
+    sc = (None, None) if st.k_scale is None else (st.k_scale[0], st.v_scale[0])
+    for s, at in ((0, 897), (1, 499)):  # the windows begin at 900 and 500
+        page, slot = st.state.table[s][at // 16], at % 16
+        for t in (st.k, st.v):
+            (t if fmt == "bf16" else t.view(torch.uint8))[0, page, slot] = float("nan") if fmt == "bf16" else 0x7F
+    q = queries(2, heads * group, dim, 91)
+    want, a, d = pm.attention(q, *clean, st.state.table, st.state.lens, [0, 1, 2], 16, 1000, 1.0, *sc)
+    for _ in range(3):
+        out = q.clone()
+        ops.paged_attention(out, st.cache, i32([0, 1, 2]), out, window=1000, max_rows=1)
+        assert ops.device_errors() == 0
+        check_rows(out, want, a, d, dim)
