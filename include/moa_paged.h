@@ -103,7 +103,9 @@ int moa_paged_cache_compact(const moa_paged_cache* cache, void* stream);
  * A sequence whose rows or length are out of range, or that has more than max_rows rows, is left out; so
  * is at least every row that sees a page outside the pool, and row starts that descend may leave out all
  * (MOA_DEVERR_PAGED). The result is deterministic; how the positions are split, and with it the order of f32 sums,
- * follows the whole batch, so a row's last bits may differ between calls of other batches. rows may be 0. */
+ * follows the whole batch, so a row's last bits may differ between calls of other batches. Scores, maxima, sums and outputs are
+ * f32; a weight enters the product with V as two bf16 numbers, which hold it to 2^-16 of itself, in every row of every call; the
+ * result is rounded once. rows may be 0. */
 int moa_paged_attention(const uint16_t* q, int64_t q_row_stride, const moa_paged_cache* cache,
                         const int32_t* row_starts, uint16_t* out, int64_t out_row_stride, int rows, int q_heads,
                         int layer, int window, float scale, int max_rows, void* stream);

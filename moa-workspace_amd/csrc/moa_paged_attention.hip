@@ -27,6 +27,15 @@ constexpr float kSlack = 8.0f;
 
 __device__ __forceinline__ bf16x8 as_bf16x8(const uint4& v) { return __builtin_bit_cast(bf16x8, v); }
 
+// Two weights as two pairs of bf16, high parts and rests: what is lost is at most 2^-16 of a weight. (One part alone loses 2^-8,
+// which is more than what is left where values nearly cancel; a third, for the last 8 bits of f32, takes the chunk kernel another 24 %
+// and moves the result by less than the f32 rounding of its scores does.)
+constexpr int kParts = 2;
+__device__ __forceinline__ void split_weights(float p0, float p1, uint32_t (&w)[kParts]) {
+    w[0] = pk_bf16(p0, p1);
+    w[1] = pk_bf16(p0 - __uint_as_float(w[0] << 16), p1 - __uint_as_float(w[0] & 0xffff0000u));
+}
+
 // ------------------------------------------------------------------------------------ who does what
 
 // A sequence that takes part: its first row of the call, new rows and length. n = 0: it does not, or is bad.
@@ -365,8 +374,8 @@ __device__ void careful_piece(const PagedView& c, const PagedAttentionCall& a, c
 // (16 x 16 x 32 MFMAs): lane (c = lane % 16, g = lane / 16) then holds, for row c, positions 4 g .. 4 g + 3 of each 16,
 // which are just the positions it supplies as A of P times V when V's lanes take the same ones: P moves between no
 // lanes. V's lane (c, g) loads kVD dims of each of its positions, and v_perm pairs two positions of a dim; MFMA (b, d)
-// then covers dims 16 kVD b + kVD c + d of all c. P enters as two bf16 parts, high and rest (what is lost is 2^-16 of a
-// weight): tiles of 16 positions put both into one MFMA, beside the same V twice, tiles of 32 take two. This
+// then covers dims 16 kVD b + kVD c + d of all c. P enters as two bf16 parts: tiles of 16 positions put both into one
+// MFMA, beside the same V twice, tiles of 32 take two. This
 // tile's V and the next tile's K are in flight during the arithmetic. (48 sequences of 900 to 32000 positions, 16 heads of 512
 // over one: 1.8 GB in 312 us, 5.8 TB/s; 64 of 100 to 9000, 16 rows of 128 over each of 8 heads, E4M3: 0.63 GB in 146, 4.3.)
 template <int D, bool E4M3>
@@ -599,16 +608,14 @@ __device__ __forceinline__ void token_part(const PagedView& c, const PagedAttent
             }
             const float mu = m_ref == -INFINITY ? 0.0f : m_ref;
             float sum = 0.0f;
-            uint32_t ph[2 * NT], pl[2 * NT];
+            uint32_t pw[2 * NT][kParts];
 #pragma unroll
             for (int i = 0; i < NT; ++i)
 #pragma unroll
                 for (int e = 0; e < 4; e += 2) {
                     const float p0 = __builtin_amdgcn_exp2f(x[i][e] - mu), p1 = __builtin_amdgcn_exp2f(x[i][e + 1] - mu);
                     sum += p0 + p1;
-                    const uint32_t w = pk_bf16(p0, p1);
-                    ph[2 * i + e / 2] = w;
-                    pl[2 * i + e / 2] = pk_bf16(p0 - bf2f(w & 0xffffu), p1 - bf2f(w >> 16));
+                    split_weights(p0, p1, pw[2 * i + e / 2]);
                 }
             l_run = fmaf(l_run, scale, sum);
 #pragma unroll
@@ -625,12 +632,13 @@ __device__ __forceinline__ void token_part(const PagedView& c, const PagedAttent
                             w[i] = __builtin_amdgcn_perm(vf[b][2 * i + 1].w[d / 2], vf[b][2 * i].w[d / 2], d & 1 ? 0x07060302u : 0x05040100u);
                     }
                     if constexpr (NT == 1) {
-                        o[b][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(make_uint4(ph[0], ph[1], pl[0], pl[1])),
+                        o[b][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(make_uint4(pw[0][0], pw[1][0], pw[0][1], pw[1][1])),
                                                                           as_bf16x8(make_uint4(w[0], w[1], w[0], w[1])), o[b][d], 0, 0, 0);
                     } else {
-                        const bf16x8 vb = as_bf16x8(make_uint4(w[0], w[1], w[2], w[3]));
-                        o[b][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(make_uint4(ph[0], ph[1], ph[2], ph[3])), vb, o[b][d], 0, 0, 0);
-                        o[b][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(make_uint4(pl[0], pl[1], pl[2], pl[3])), vb, o[b][d], 0, 0, 0);
+#pragma unroll
+                        for (int p = 0; p < kParts; ++p)
+                            o[b][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(make_uint4(pw[0][p], pw[1][p], pw[2][p], pw[3][p])),
+                                                                              as_bf16x8(make_uint4(w[0], w[1], w[2], w[3])), o[b][d], 0, 0, 0);
                     }
                 }
         }
@@ -730,13 +738,12 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(TokenShape<
 // LDS; E4M3: through registers, widened to bf16 once for all waves). Scores are K times Q^T (32 x 32 x 16 MFMAs):
 // lane (c = lane % 32, hf = lane / 32) holds, for row c, positions 8 (e / 4) + 4 hf + e % 4 of 32, and 8 of them in a
 // row are what it supplies as B of V^T times P^T when V's transposing LDS reads fetch the same positions: P moves
-// between no lanes, and a row's maximum, sum and rescaling stay in its lane. P enters as bf16, each weight off by at most
-// 2^-8 of itself: a second part, as in the token kernel, would add half as much matrix work again for a result that
-// is rounded to bf16 anyway. The sum adds the weights as they enter, in f32: their roundings then cancel in part.
-// (Four prompts of 1100 to 4100 tokens, 32 heads of 128 over 8: 251 us, 0.7 PFLOP/s.)
+// between no lanes, and a row's maximum, sum and rescaling stay in its lane. P enters as two bf16 parts, which share V's
+// fragments, and up to 256 dims 16 positions are weighed beside the products of the 16 before them. (Four prompts of 1100 to 4100
+// tokens, 32 heads of 128 over 8: 301 us, 0.59 PFLOP/s of the products' own work; 318 with all weights first, 250 with one part.)
 // 512 dims: a row's Q and out do not fit beside each other in a wave's registers, so two waves share 32 rows, each with
 // half of the dims: they add the halves of the scores through LDS, and each weighs half of the positions for both (1000 rows of
-// 16 heads over 15800 positions: 672 us, 682 where both weigh all).
+// 16 heads over 15800 positions: 810 us; 677 with one part).
 template <int D, bool E4M3>
 struct ChunkShape {
     static constexpr int kTile = D >= 256 ? 32 : 64;
@@ -965,7 +972,7 @@ __device__ __forceinline__ void chunk_part(const PagedView& c, const PagedAttent
                     __builtin_amdgcn_sched_barrier(0);
                 }
             }
-            uint32_t pw[T::kSub][8];
+            uint32_t pw[T::kSub][8][kParts];
             if constexpr (kPair == 1) {
                 if (t0 < all_lo || t0 + kTile > all_hi) {  // some row does not see all of it
                     const int from = in_loop(see_lo - t0 - 4 * hf), to = in_loop(see_hi - t0 - 4 * hf);
@@ -995,33 +1002,22 @@ __device__ __forceinline__ void chunk_part(const PagedView& c, const PagedAttent
 #pragma unroll
                         for (int e = 0; e < 16; ++e) o[d][e] *= scale;
                 }
-                const float mu = m_ref == -INFINITY ? 0.0f : m_ref;
-                float sum = 0.0f;
-                const bf16x2 ones = {(__bf16)1.0f, (__bf16)1.0f};
-#pragma unroll
-                for (int b = 0; b < T::kSub; ++b)
-#pragma unroll
-                    for (int e = 0; e < 16; e += 2) {
-                        const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[b][e], factor, -mu));
-                        const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[b][e + 1], factor, -mu));
-                        pw[b][e / 2] = pk_bf16(p0, p1);
-                        sum = dot2_bf16(pw[b][e / 2], ones, sum);
-                    }
-                l_run = fmaf(l_run, scale, sum);
+                l_run *= scale;
             } else {
                 // The positions of 16 a wave: the other's half of their scores comes through LDS, and the weights go back. A
                 // wave's weights stand against its own reference, a whole number, so that they move to the larger of the
                 // two exactly.
                 const int ln = lane_here();
-                float4 *out = xs + wave * 256 + ln, *in = xs + (wave ^ 4) * 256 + ln;  // two of scores, one of weights, references
-                out[0] = make_float4(sc[0][8], sc[0][9], sc[0][10], sc[0][11]);
-                out[64] = make_float4(sc[0][12], sc[0][13], sc[0][14], sc[0][15]);
+                // `mine`: own scores, later the other's weights and reference; `theirs`: the reverse
+                float4 *mine = xs + wave * 256 + ln, *theirs = xs + (wave ^ 4) * 256 + ln;
+                mine[0] = make_float4(sc[0][8], sc[0][9], sc[0][10], sc[0][11]);
+                mine[64] = make_float4(sc[0][12], sc[0][13], sc[0][14], sc[0][15]);
                 exchanged();
                 if (!sees) {
                     exchanged();
                     return;
                 }
-                const float4 y0 = in[0], y1 = in[64];
+                const float4 y0 = theirs[0], y1 = theirs[64];
                 float x[8] = {sc[0][0] + y0.x, sc[0][1] + y0.y, sc[0][2] + y0.z, sc[0][3] + y0.w,
                               sc[0][4] + y1.x, sc[0][5] + y1.y, sc[0][6] + y1.z, sc[0][7] + y1.w};
                 if (t0 < all_lo || t0 + kTile > all_hi) {  // some row does not see all of it
@@ -1037,20 +1033,24 @@ __device__ __forceinline__ void chunk_part(const PagedView& c, const PagedAttent
                 for (int e = 1; e < 8; ++e) mx = fmaxf(mx, x[e]);
                 mx = fmaxf(mx, __shfl_xor(mx, 32)) * factor;
                 const float r = mx > m_ref + kSlack ? ceilf(mx) : m_ref, mu = r == -INFINITY ? 0.0f : r;
+                uint32_t own[4][kParts];
 #pragma unroll
                 for (int e = 0; e < 8; e += 2)
-                    pw[0][e / 2] = pk_bf16(__builtin_amdgcn_exp2f(fmaf(x[e], factor, -mu)), __builtin_amdgcn_exp2f(fmaf(x[e + 1], factor, -mu)));
-                reinterpret_cast<uint4*>(out)[128] = make_uint4(pw[0][0], pw[0][1], pw[0][2], pw[0][3]);
-                reinterpret_cast<float*>(xs + wave * 256 + 192)[ln] = r;
-                exchanged();
-                const uint4 other = reinterpret_cast<const uint4*>(in)[128];
-                const float s = reinterpret_cast<const float*>(xs + (wave ^ 4) * 256 + 192)[ln], most = fmaxf(r, s);
-                const uint32_t theirs[4] = {other.x, other.y, other.z, other.w};
+                    split_weights(__builtin_amdgcn_exp2f(fmaf(x[e], factor, -mu)), __builtin_amdgcn_exp2f(fmaf(x[e + 1], factor, -mu)), own[e / 2]);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const uint32_t own = pw[0][i];
-                    pw[0][i] = half ? theirs[i] : own;
-                    pw[0][4 + i] = half ? own : theirs[i];
+                for (int i = 0; i < kParts; ++i) reinterpret_cast<uint4*>(theirs)[64 * i] = make_uint4(own[0][i], own[1][i], own[2][i], own[3][i]);
+                *reinterpret_cast<float*>(theirs + 192) = r;
+                exchanged();
+                const float s = *reinterpret_cast<const float*>(mine + 192), most = fmaxf(r, s);
+#pragma unroll
+                for (int i = 0; i < kParts; ++i) {
+                    const uint4 w = reinterpret_cast<const uint4*>(mine)[64 * i];
+                    const uint32_t other[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        pw[0][j][i] = half ? other[j] : own[j][i];
+                        pw[0][4 + j][i] = half ? own[j][i] : other[j];
+                    }
                 }
                 const float scale = most == m_ref || m_ref == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m_ref - most);
                 const bool moved = __any(most != m_ref);
@@ -1064,44 +1064,68 @@ __device__ __forceinline__ void chunk_part(const PagedView& c, const PagedAttent
                 if (moved) {
                     const float f = r == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(r - most), g = s == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(s - most);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const float h = (i < 4) == (half == 0) ? f : g;
-                        pw[0][i] = pk_bf16(bf2f(pw[0][i] & 0xffffu) * h, bf2f(pw[0][i] >> 16) * h);
+                    for (int j = 0; j < 8; ++j) {
+                        const float h = (j < 4) == (half == 0) ? f : g;
+#pragma unroll
+                        for (int i = 0; i < kParts; ++i)
+                            pw[0][j][i] = pk_bf16(bf2f(pw[0][j][i] & 0xffffu) * h, bf2f(pw[0][j][i] >> 16) * h);
                     }
                 }
                 const bf16x2 ones = {(__bf16)1.0f, (__bf16)1.0f};
                 float sum = 0.0f;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) sum = dot2_bf16(pw[0][i], ones, sum);
+                for (int j = 0; j < 8; ++j)
+#pragma unroll
+                    for (int i = 0; i < kParts; ++i) sum = dot2_bf16(pw[0][j][i], ones, sum);
                 l_run = fmaf(l_run, scale, sum);
             }
             {
-                constexpr int kAhead = 2, kN = T::kSub * kDims;  // step n: 32 positions n / kDims, dim tile n % kDims
+                // step n: 16 positions n / kDims, dim tile n % kDims (the next 16 positions weighed beside it: see above). V is read kAhead
+                // steps ahead: four took 256 and 512 dims 172 and 886 us, three 152 and 810 (registers).
+                constexpr int kAhead = T::kSub == 2 ? 4 : 3, kUnits = 2 * T::kSub, kN = kUnits * kDims;
+                const float mu = m_ref == -INFINITY ? 0.0f : m_ref;
+                float sum = 0.0f;  // (pairs of waves have added theirs)
+                auto weigh = [&](int u, int j) __attribute__((always_inline)) {  // pair j of 4
+                    const int b = u / 2, e = 8 * (u & 1) + 2 * j;
+                    const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[b][e], factor, -mu)), p1 = __builtin_amdgcn_exp2f(fmaf(sc[b][e + 1], factor, -mu));
+                    split_weights(p0, p1, pw[b][e / 2]);
+                    sum += p0 + p1;
+                };
                 uint8_t* vt = tiles + tile + kTileBytes + half * kMine * 2;
                 const int vx = v_address();
-                s16x4 vr[kAhead][4];
+                s16x4 vr[kAhead][2];
                 auto read_v = [&](int n) __attribute__((always_inline)) {
-                    const int d = n % kDims, b = n / kDims;
+                    const int d = n % kDims, u = n / kDims;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)  // positions 8 i + 4 hf ..; an odd i's swizzle differs in bit 1 of the chunk
+                    for (int i = 0; i < 2; ++i)  // positions 8 i + 4 hf ..; an odd i's swizzle differs in bit 1 of the chunk
                         vr[n % kAhead][i] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                            (lds_s16x4*)(vt + (vx ^ (64 * (d & 3) + 32 * (i & 1))) + 256 * (d >> 2) + (32 * b + 8 * i) * T::kRowBytes));
-                };
-                auto frag = [&](int n, int i) __attribute__((always_inline)) {
-                    return __builtin_bit_cast(bf16x8, __builtin_shufflevector(vr[n % kAhead][2 * i], vr[n % kAhead][2 * i + 1], 0, 1, 2, 3, 4, 5, 6, 7));
+                            (lds_s16x4*)(vt + (vx ^ (64 * (d & 3) + 32 * i)) + 256 * (d >> 2) + (16 * u + 8 * i) * T::kRowBytes));
                 };
 #pragma unroll
                 for (int n = 0; n < kAhead; ++n) read_v(n);
+                if constexpr (kPair == 1) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) weigh(0, j);
+                }
 #pragma unroll
                 for (int n = 0; n < kN; ++n) {
-                    const int d = n % kDims, b = n / kDims;
+                    const int d = n % kDims, u = n / kDims, b = u / 2, i = u & 1;
+                    const bf16x8 vf = __builtin_bit_cast(bf16x8, __builtin_shufflevector(vr[n % kAhead][0], vr[n % kAhead][1], 0, 1, 2, 3, 4, 5, 6, 7));
 #pragma unroll
-                    for (int i = 0; i < 2; ++i)
+                    for (int p = 0; p < kParts; ++p)
                         o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-                            frag(n, i), as_bf16x8(make_uint4(pw[b][4 * i], pw[b][4 * i + 1], pw[b][4 * i + 2], pw[b][4 * i + 3])), o[d], 0, 0, 0);
+                            vf, as_bf16x8(make_uint4(pw[b][4 * i][p], pw[b][4 * i + 1][p], pw[b][4 * i + 2][p], pw[b][4 * i + 3][p])), o[d], 0, 0, 0);
                     if (n + kAhead < kN) read_v(n + kAhead);
+                    if constexpr (kPair == 1) {
+                        if (u + 1 < kUnits) {
+#pragma unroll
+                            for (int j = 0; j < 4; ++j)
+                                if (j * kDims / 4 == d) weigh(u + 1, j);
+                        }
+                    }
                     __builtin_amdgcn_sched_barrier(0);
                 }
+                l_run += sum;
             }
         };
         // this wave's loads into LDS are done, and then everybody's; and everybody has read the other buffer

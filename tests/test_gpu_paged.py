@@ -1114,3 +1114,50 @@ def test_a_value_before_the_window_never_reaches_a_joined_row(heads, group, dim,
         ops.paged_attention(out, st.cache, i32([0, 1, 2]), out, window=1000, max_rows=1)
         assert ops.device_errors() == 0
         check_rows(out, want, a, d, dim)
+
+
+# ------------------------------------------------------------------------- what the weights keep
+
+@pytest.mark.parametrize("n,heads,group,dim,fmt", [
+    # single tokens: 32 positions a tile, and 16 (256 dims of bf16, 512 of either type)
+    (1, 8, 2, 128, "bf16"), (1, 3, 5, 64, "e4m3"), (4, 2, 4, 256, "e4m3"), (1, 8, 2, 256, "bf16"), (1, 1, 16, 512, "bf16"), (2, 1, 8, 512, "e4m3"),
+    # chunks: a wave per 32 rows, and pairs of waves (512 dims)
+    (60, 2, 4, 128, "bf16"), (33, 1, 8, 64, "e4m3"), (50, 4, 2, 256, "bf16"), (20, 2, 2, 256, "e4m3"), (40, 1, 16, 512, "bf16"), (64, 1, 3, 512, "e4m3")])
+def test_values_that_nearly_cancel(n, heads, group, dim, fmt):
+    """Positions come in pairs of opposite values whose weights differ by 2^-10: what is left of a pair is far below the
+    rounding of a weight to one bf16 number (2^-8 of it), so every row would have wrong signs with such weights.
+
+    Tolerance, relative to a (the attention of |v|). A score is one product of bf16 numbers, so exact, and below 1: its
+    factor (three roundings), the product with it and the distance to the reference are off by at most 5 * 2^-23 together, the
+    exponential by 2^-22, which moves a weight by less than 2^-20 of it. Two bf16 parts hold a weight to (2^-8)^2 = 2^-16. The sums of at
+    most 64 products lose at most 2^-23 of a each time: 2^-17. The division and the last rounding are relative to the result."""
+    need_gpu()
+    say(f"paged attention, values that cancel, {n} rows of {heads} x {group} of {dim} {fmt}")
+    length = 64
+    st = Setup([length], 16, heads, dim, fmt, seed=95)
+    g = torch.Generator(device=DEV).manual_seed(96)
+    even, step, q0 = (1 + torch.randint(0, 60, (length // 2, heads), generator=g, device=DEV) / 64, 2.0 ** -7, 2.0 ** -3)
+    if fmt == "e4m3":
+        even, step, q0 = 1 + torch.randint(0, 7, (length // 2, heads), generator=g, device=DEV) / 8, 2.0 ** -3, 2.0 ** -7
+        st.k_scale.fill_(1.0)
+    sign = torch.randint(0, 2, (length // 2, heads), generator=g, device=DEV) * 2 - 1  # which of a pair weighs more
+    k = torch.stack([even, even + step], 1)
+    k = torch.where(sign[:, None] > 0, k, k.flip(1)).reshape(length, heads)
+    v = torch.randn((length // 2, 1, heads, dim), generator=g, device=DEV).clamp(-3, 3) * (60 if fmt == "e4m3" else 1)
+    v = torch.cat([v, -v], 1).reshape(length, heads, dim)
+    table = torch.tensor(st.state.table[0], device=DEV)
+    t = torch.arange(length, device=DEV)
+    kv = torch.zeros((length, heads, dim), device=DEV)
+    kv[:, :, dim - 1] = k
+    st.k[0, table[t // 16], t % 16] = kv.to(st.k.dtype)
+    st.v[0, table[t // 16], t % 16] = v.to(st.v.dtype)
+    q = torch.zeros((n, heads * group, dim), dtype=torch.bfloat16, device=DEV)
+    q[:, :, dim - 1] = q0
+    sc = (None, None) if st.k_scale is None else (st.k_scale[0], st.v_scale[0])
+    want, a, _ = pm.attention(q, *st.values(), st.state.table, [length], [0, n], 16, 0, 1.0, *sc)
+    out = torch.empty_like(q)
+    ops.paged_attention(q, st.cache, i32([0, n]), out)
+    assert ops.device_errors() == 0
+    assert (want[-1].abs() < 2.0 ** -9 * a[-1]).float().mean() > 0.9  # they do cancel
+    over = ((out.double() - want).abs() - 2.0 ** -8 * want.abs() - a * (2.0 ** -16 + 2.0 ** -17 + 2.0 ** -20)).max().item()
+    assert over <= 0, f"beyond the tolerance by {over}, relative to a: {((out.double() - want).abs() / a).max().item()}"
