@@ -6,6 +6,7 @@
 #include <stdint.h>
 
 #include "moa_internal.h"
+#include "moa_paged_plan.h"
 
 namespace moa {
 

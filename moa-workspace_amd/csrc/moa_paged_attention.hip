@@ -47,12 +47,12 @@ __device__ __forceinline__ Seq seq_of(const PagedView& c, const PagedAttentionCa
     q.row0 = a.starts[s];
     const int end = a.starts[s + 1];
     q.len = c.lens[s];
-    const int n = end - q.row0;
-    if (n == 0) return q;
-    if (q.row0 < 0 || n < 0 || end > a.rows || n > a.max_rows || q.len < 0 || q.len > paged_capacity(c)) {
+    if (end == q.row0) return q;
+    if (!rows_in_range(q.row0, end, a.rows, a.max_rows) || q.len < 0 || q.len > paged_capacity(c)) {
         *bad = true;
         return q;
     }
+    const int n = end - q.row0;
     if ((n * a.group <= kTokenRows) == tokens) q.n = n;  // at most 2^20 * 128 rows
     return q;
 }

@@ -1,0 +1,18 @@
+// moa_paged_plan.h -- decisions of the paged cache's kernels in plain arithmetic, for the device and for host tests.
+#pragma once
+
+#ifdef __HIPCC__
+#define MOA_PLAN_FN __host__ __device__ __forceinline__
+#else
+#define MOA_PLAN_FN inline
+#endif
+
+namespace moa {
+
+// Whether a sequence's rows [row0, end) lie within a call's `rows`, at most max_rows of them. Row starts are device memory and
+// may hold anything: the difference is taken only of values that are in range, since elsewhere it can pass 32 bits and look small.
+MOA_PLAN_FN bool rows_in_range(int row0, int end, int rows, int max_rows) {
+    return row0 >= 0 && row0 <= end && end <= rows && end - row0 <= max_rows;
+}
+
+}  // namespace moa

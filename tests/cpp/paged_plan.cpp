@@ -1,0 +1,6 @@
+// The paged cache's decisions (moa-workspace_amd/csrc/moa_paged_plan.h) for host tests, by C names.
+#include "moa_paged_plan.h"
+
+extern "C" {
+int rows_in_range(int row0, int end, int rows, int max_rows) { return moa::rows_in_range(row0, end, rows, max_rows); }
+}

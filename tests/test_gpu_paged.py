@@ -1161,3 +1161,24 @@ def test_values_that_nearly_cancel(n, heads, group, dim, fmt):
     assert (want[-1].abs() < 2.0 ** -9 * a[-1]).float().mean() > 0.9  # they do cancel
     over = ((out.double() - want).abs() - 2.0 ** -8 * want.abs() - a * (2.0 ** -16 + 2.0 ** -17 + 2.0 ** -20)).max().item()
     assert over <= 0, f"beyond the tolerance by {over}, relative to a: {((out.double() - want).abs() / a).max().item()}"
+
+
+# ---------------------------------------------------------------------------- bad row starts and states
+
+@pytest.mark.parametrize("n", [1, 90])
+@pytest.mark.parametrize("bad", [[2 ** 31 - 1, -2 ** 31], [2 ** 31 - 1, -2 ** 31 + 2], [-2 ** 31, 2 ** 31 - 1], [2 ** 30, 2 ** 30 + 1], [-1, 0], [2 ** 31 - 1, 2 ** 31 - 1]])
+def test_row_starts_at_the_ends_of_int32(bad, n):
+    """Starts whose difference passes 32 bits, or that lie outside the call's rows, in the middle of a call's sequences: those
+    sequences are left out, the others' rows are right, and nothing else is written."""
+    need_gpu()
+    say(f"paged attention, row starts {bad}, {n} rows")
+    st = Setup([200, 210, 220, 230, 240], 16, 2, 128, seed=97)
+    q = queries(3 * n, 8, 128, 98)
+    out = torch.full_like(q, 123.0)
+    ops.paged_attention(q, st.cache, i32([0, n, *bad, 2 * n, 3 * n]), out, max_rows=n)
+    assert ops.device_errors() == _lib.DEVERR_PAGED
+    k, v = st.values()
+    for s, rows in ((0, slice(0, n)), (4, slice(2 * n, 3 * n))):
+        want, a, d = pm.attention(q[rows], k, v, [st.state.table[s]], [st.state.lens[s]], [0, n], 16, 0, 1.0)
+        check_rows(out[rows], want, a, d, 128)
+    assert (out[n:2 * n] == 123.0).all()
