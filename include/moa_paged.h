@@ -68,7 +68,7 @@ int moa_paged_cache_reserve(const moa_paged_cache* cache, const int32_t* new_tok
  * dense, rows k_row_stride / v_row_stride elements apart, 16-byte aligned). E4M3 pages take the
  * nearest code of x / scale, ties to even, at most +-448. Rows before row_starts[0] or from
  * row_starts[sequences] on belong to no sequence and are not read. A row whose position or page is out of
- * range is not written (MOA_DEVERR_PAGED). rows may be 0. */
+ * range, or whose sequence's starts descend, is not written (MOA_DEVERR_PAGED). rows may be 0. */
 int moa_paged_cache_append(const moa_paged_cache* cache, const uint16_t* k, int64_t k_row_stride, const uint16_t* v,
                            int64_t v_row_stride, const int32_t* row_starts, int rows, int layer, void* stream);
 

@@ -419,9 +419,9 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedView c, const ui
     const int s = sequence_of(starts, c.sequences, m);
     if (s < 0 || s >= c.sequences) return;
     const int end = starts[s + 1], len = c.lens[s], cap = paged_capacity(c);
-    const int t = len - (end - m);
-    if (end <= m) return;  // starts that descend
-    if (end > rows || len < 0 || len > cap || t < 0) {
+    // (end <= m: starts that descend. Only then is the difference sure to fit.)
+    const int t = end > m && end <= rows && len >= 0 && len <= cap ? len - (end - m) : -1;
+    if (t < 0) {
         if (lane == 0) raise(c);
         return;
     }

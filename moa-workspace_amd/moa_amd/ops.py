@@ -460,8 +460,8 @@ def paged_cache_reserve(cache, new_tokens) -> None:
 def paged_cache_append(cache, k, v, row_starts, layer=0) -> None:
     """Writes one layer's K and V rows of a step's new tokens: k, v bf16 [rows, kv_heads, head_dim] (rows may lie apart).
     Rows row_starts[s] .. row_starts[s + 1] - 1 (int32 [sequences + 1]) are the last positions of sequence s, so reserve
-    first. E4M3 pages take the nearest code of x / scale, at most +-448. A row whose position or page is out of range is
-    not written (bit 8)."""
+    first. E4M3 pages take the nearest code of x / scale, at most +-448. A row whose position or page is out of range, or
+    whose sequence's starts descend, is not written (bit 8)."""
     p = _index(row_starts, "row_starts", cache, ("sequences", 1))
     kp, kr, rows = _row_tensor(k, "k", cache, cache.kv_heads)
     vp, vr, vrows = _row_tensor(v, "v", cache, cache.kv_heads)

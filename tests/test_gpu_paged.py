@@ -1182,3 +1182,20 @@ def test_row_starts_at_the_ends_of_int32(bad, n):
         want, a, d = pm.attention(q[rows], k, v, [st.state.table[s]], [st.state.lens[s]], [0, n], 16, 0, 1.0)
         check_rows(out[rows], want, a, d, 128)
     assert (out[n:2 * n] == 123.0).all()
+
+
+@pytest.mark.parametrize("starts,written", [([0, 5, 3, 8], {0: (0, 3), 2: (5, 8)}), ([0, 2, -2 ** 31, 8], {2: (2, 8)}), ([0, 2, 2 ** 31 - 1, 8], {0: (0, 2)})])
+def test_append_with_row_starts_that_are_out_of_order(starts, written):
+    """Rows whose sequence's starts descend or end past the call's rows raise the bit and are not written; those of the others are."""
+    need_gpu()
+    say(f"append, row starts {starts}")
+    st = Setup([40, 50, 60], 16, 2, 64, seed=99)
+    want = st.k.clone()
+    k = queries(8, 2, 64, 1, 8.0)
+    ops.paged_cache_append(st.cache, k, k, i32(starts))
+    assert ops.device_errors() == _lib.DEVERR_PAGED
+    for s, (m0, m1) in written.items():
+        for m in range(m0, m1):
+            t = st.state.lens[s] - (starts[s + 1] - m)
+            want[0, st.state.table[s][t // 16], t % 16] = k[m]
+    assert torch.equal(raw(st.k), raw(want))
