@@ -414,13 +414,14 @@ __device__ __forceinline__ uint32_t bf16_pair_of_fp8(uint32_t two) {
     return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(two, 1.0f, false));
 }
 
-// A split sequence's last workgroup, found by a counter per (KV head, group that begins it) that it sets back to zero, joins its
+// A split sequence's last workgroup, found by a counter per (KV head, group that begins it: one split sequence at most), joins its
 // records: they are written and read past the XCDs' caches (agent scope). A thread takes four dims of a row, so this is for
 // few rows, and for few parts, which it reads one batch after the other: rows * dims up to kJoinElements, up to kJoinUnits units
 // a sequence. One token of 8 x 2 heads of 256 over 700 positions: 11.8 us, 13.6 with a merge launch; 120 of them in a window of
 // 1024: 158 and 166. Beyond: 4 tokens (8 rows) over 700 to 1500 positions 16.7 and 14.4, one sequence of 16 rows of 512 38.9 and
 // 20.6, two tokens over 4000 to 5000 positions 27.7 and 24.4.
 constexpr int kJoinUnits = 16;
+static_assert(kJoinUnits < (int)kJoinTurn, "a sequence's parts are fewer than a turn of its counter");
 constexpr int kJoinElements = 1024;
 
 template <int D, bool E4M3>
@@ -463,7 +464,7 @@ __device__ __forceinline__ void join_records(const PagedView& c, const PagedAtte
     *reinterpret_cast<uint2*>(a.out + x.m * a.out_row + x.h * D + d) = make_uint2(pk_bf16(v.x * inv, v.y * inv), pk_bf16(v.z * inv, v.w * inv));
 }
 
-// kJoin: the workgroups join their records (tickets [kv_heads][groups], zero); else the merge kernel does.
+// kJoin: the workgroups join their records (tickets [kv_heads][groups], multiples of kJoinTurn); else the merge kernel does.
 template <int D, bool E4M3, bool kJoin = false>
 __device__ __forceinline__ void token_part(const PagedView& c, const PagedAttentionCall& a, float* part, int kvh, int group, int groups,
                                            uint8_t* lds, uint32_t* tickets = nullptr) {
@@ -705,9 +706,8 @@ __device__ __forceinline__ void token_part(const PagedView& c, const PagedAttent
                 uint32_t* flag = reinterpret_cast<uint32_t*>(ms);
                 if (threadIdx.x == 0) {
                     uint32_t* ticket = tickets + kvh * groups + w0;
-                    const bool last = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)(w1 - w0);
-                    if (last) __hip_atomic_store(ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                    *flag = last;
+                    const uint32_t share = join_share(off == 0, w1 - w0 + 1);
+                    *flag = join_last(__hip_atomic_fetch_add(ticket, share, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT), share);
                 }
                 __syncthreads();
                 if (*flag) join_records<D, E4M3>(c, a, t, kvh, part + ((int64_t)kvh * 2 * groups + 2 * w0) * record_floats(kTokenRows, D), w1 - w0 + 1);

@@ -15,4 +15,11 @@ MOA_PLAN_FN bool rows_in_range(int row0, int end, int rows, int max_rows) {
     return row0 >= 0 && row0 <= end && end <= rows && end - row0 <= max_rows;
 }
 
+// A counter that the parts of a split sequence arrive at: a launch adds kJoinTurn in all (the first part what the others leave), so
+// the arrival that completes a turn is the last one, nothing is set back, and the counter stands at a multiple of kJoinTurn after
+// every launch, whatever it held: calls that overlapped against the contract spoil their own results and no later call's.
+constexpr unsigned kJoinTurn = 32;
+MOA_PLAN_FN unsigned join_share(bool first, int parts) { return first ? kJoinTurn + 1 - (unsigned)parts : 1; }
+MOA_PLAN_FN bool join_last(unsigned before, unsigned share) { return (before + share) % kJoinTurn == 0; }
+
 }  // namespace moa

@@ -3,4 +3,7 @@
 
 extern "C" {
 int rows_in_range(int row0, int end, int rows, int max_rows) { return moa::rows_in_range(row0, end, rows, max_rows); }
+unsigned join_turn() { return moa::kJoinTurn; }
+unsigned join_share(int first, int parts) { return moa::join_share(first != 0, parts); }
+int join_last(unsigned before, unsigned share) { return moa::join_last(before, share); }
 }

@@ -2,6 +2,7 @@
 host with the device's arithmetic (integers wrap)."""
 import ctypes as C
 import itertools
+import random
 import shutil
 import subprocess
 from pathlib import Path
@@ -30,3 +31,40 @@ def test_rows_in_range_at_the_ends_of_int32(plan, rows, max_rows):
     for row0, end in itertools.product(ENDS, ENDS):
         want = 0 <= row0 <= end <= rows and end - row0 <= max_rows
         assert bool(plan.rows_in_range(row0, end, rows, max_rows)) == want, (row0, end)
+
+
+def arrive(plan, counter, order):
+    """The parts of `order`, (first, parts) each, arrive at a counter in turn: its new value, and which arrivals were told to join."""
+    joins = []
+    for i, (first, parts) in enumerate(order):
+        share = plan.join_share(first, parts)
+        if plan.join_last(counter, share):
+            joins.append(i)
+        counter = (counter + share) % 2 ** 32
+    return counter, joins
+
+
+@pytest.mark.parametrize("held", [0, 32, 2 ** 32 - 32])
+def test_a_split_sequence_is_joined_by_its_last_part(plan, held):
+    rng = random.Random(held)
+    for parts in range(2, 17):
+        for _ in range(40):
+            order = [(i == 0, parts) for i in range(parts)]
+            rng.shuffle(order)
+            after, joins = arrive(plan, held, order)
+            assert joins == [parts - 1] and after % plan.join_turn() == 0
+
+
+def test_counters_heal_after_calls_that_overlapped(plan):
+    """Two launches whose parts arrive at one counter in any order: the next launch joins once, by its last part."""
+    rng = random.Random(3)
+    for _ in range(500):
+        both = []
+        for parts in (rng.randrange(2, 17), rng.randrange(2, 17)):
+            both += [(i == 0, parts) for i in range(parts)]
+        rng.shuffle(both)
+        counter, _ = arrive(plan, 32 * rng.randrange(2 ** 27), both)
+        parts = rng.randrange(2, 17)
+        order = [(i == 0, parts) for i in range(parts)]
+        rng.shuffle(order)
+        assert arrive(plan, counter, order)[1] == [parts - 1]
