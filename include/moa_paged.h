@@ -82,8 +82,8 @@ int moa_paged_cache_fork(const moa_paged_cache* cache, const int32_t* parents, c
                          void* stream);
 
 /* Ends the listed sequences (device int32 [count]): length 0, and one reference fewer on each of their
- * pages. A sequence that is empty or listed again changes nothing; an index out of range is left out
- * (MOA_DEVERR_PAGED). count may be 0. */
+ * pages. A sequence that is empty or listed again changes nothing; an index out of range and a sequence whose length is out of
+ * range are left out, and so is a table entry outside the pool or a page whose count is zero (MOA_DEVERR_PAGED). count may be 0. */
 int moa_paged_cache_free(const moa_paged_cache* cache, const int32_t* sequences, int count, void* stream);
 
 /* Moves the live pages (reference count > 0; n of them) to pages 0 .. n - 1: those at n and beyond go,

@@ -324,20 +324,20 @@ __global__ __launch_bounds__(kCopyBlock) void paged_fork_kernel(PagedView c, con
 
 // --------------------------------------------------------------------------------------------- free
 
-// One workgroup per listed sequence; the first to take its length (an exchange) gives its pages back.
+// One workgroup per listed sequence; the first to take its length (an exchange with 0 of what it has checked) gives its pages back.
 __global__ __launch_bounds__(kCopyBlock) void paged_free_kernel(PagedView c, const int32_t* sequences, int count) {
     __shared__ int had;
     for (int f = blockIdx.x; f < count; f += gridDim.x) {
         const int s = sequences[f];
-        const bool in = s >= 0 && s < c.sequences;
         __syncthreads();
-        if (threadIdx.x == 0) had = in ? atomicExch(c.lens + s, 0) : -1;
+        if (threadIdx.x == 0) {
+            const int len = s >= 0 && s < c.sequences ? c.lens[s] : -1;
+            const bool bad = len < 0 || len > paged_capacity(c);
+            if (bad) raise(c);
+            had = bad || atomicCAS(c.lens + s, len, 0) != len ? 0 : len;  // taken by an equal entry: nothing is left
+        }
         __syncthreads();
         const int len = had;
-        if (len < 0 || len > paged_capacity(c)) {
-            if (threadIdx.x == 0) raise(c);
-            continue;
-        }
         for (int i = threadIdx.x; i < pages_of(c, len); i += kCopyBlock) {
             const int p = c.table[s * c.table_stride + i];
             if (p < 0 || p >= c.pages) raise(c);

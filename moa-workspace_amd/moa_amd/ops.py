@@ -482,7 +482,7 @@ def paged_cache_fork(cache, parents, children) -> None:
 
 def paged_cache_free(cache, sequences) -> None:
     """Ends the listed sequences (int32 [count]): their length becomes 0 and their pages lose a reference. Empty and
-    repeated ones change nothing; an index out of range is left out (bit 8)."""
+    repeated ones change nothing; an index or a length out of range is left out (bit 8)."""
     p = _index(sequences, "sequences", cache, None)
     _call("moa_paged_cache_free", cache._struct, p, sequences.numel(), _cache_stream(cache))
 

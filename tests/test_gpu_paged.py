@@ -1199,3 +1199,24 @@ def test_append_with_row_starts_that_are_out_of_order(starts, written):
             t = st.state.lens[s] - (starts[s + 1] - m)
             want[0, st.state.table[s][t // 16], t % 16] = k[m]
     assert torch.equal(raw(st.k), raw(want))
+
+
+@pytest.mark.parametrize("length", [-1, -2 ** 31, 6 * 16 + 1, 2 ** 31 - 1])
+def test_free_leaves_a_sequence_with_a_bad_length(length):
+    """Its length, its pages' counts and its table stay, so that the caller can put the length right; the others are freed."""
+    need_gpu()
+    say(f"free, a length of {length}")
+    st = Setup([70, 48, 5], 16, 1, 64, seed=100, columns=6)
+    table = st.table.clone()
+    st.lens[1] = length
+    ops.paged_cache_free(st.cache, i32([0, 1, 2, 1]))
+    assert ops.device_errors() == _lib.DEVERR_PAGED
+    assert st.lens.tolist() == [0, length, 0]
+    st.lens[1] = 48
+    st.state.free([0, 2])
+    st.check_state()
+    assert torch.equal(st.table, table)
+    ops.paged_cache_free(st.cache, i32([1, 1]))
+    st.state.free([1])
+    assert ops.device_errors() == 0
+    st.check_state()
