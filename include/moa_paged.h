@@ -77,7 +77,8 @@ int moa_paged_cache_append(const moa_paged_cache* cache, const uint16_t* k, int6
  * lowest free page, handed out in the order of the list. A parent may be listed many times; append
  * its reserved positions first, since an append to a shared page is seen by all that share it. All or
  * nothing: an index out of range, a child that is listed twice, that is also a parent or that has
- * positions, or too few free pages leave the state as it was (MOA_DEVERR_PAGED). count may be 0. */
+ * positions, a parent whose length or whose pages are out of range, or too few free pages leave the state as it was
+ * (MOA_DEVERR_PAGED). count may be 0. */
 int moa_paged_cache_fork(const moa_paged_cache* cache, const int32_t* parents, const int32_t* children, int count,
                          void* stream);
 

@@ -53,6 +53,15 @@ __device__ int block_before(int v, int* lds, int* total) {
     return before + x - v;
 }
 
+// The last of kPlanBlock ascending numbers, the first of which is 0, that is at most r.
+__device__ __forceinline__ int last_at_most(const int* numbers, int r) {
+    int lo = 0;
+#pragma unroll
+    for (int step = kPlanBlock / 2; step > 0; step /= 2)
+        if (numbers[lo + step] <= r) lo += step;
+    return lo;
+}
+
 // kPer pages a thread and step, so that a step's loads go out together.
 constexpr int kPer = 8;
 constexpr int kStepPages = kPlanBlock * kPer;
@@ -168,10 +177,7 @@ __global__ __launch_bounds__(kPlanBlock) void paged_reserve_kernel(PagedView c, 
         if (n > 0) c.lens[s] = len + n;
         __syncthreads();
         for (int r = t; r < all; r += kPlanBlock) {
-            int lo = 0;  // the last sequence whose pages start at or before rank r: one with pages
-#pragma unroll
-            for (int step = kPlanBlock / 2; step > 0; step /= 2)
-                if (before[lo + step] <= r) lo += step;
+            const int lo = last_at_most(before, r);  // the sequence whose pages start at or before rank r: one with pages
             const int p = free_pages.get(given + r);
             c.table[(base + lo) * c.table_stride + old[lo] + r - before[lo]] = p;
             c.refs[p] = 1;
@@ -242,18 +248,19 @@ __device__ __forceinline__ Fork fork_at(const PagedView& c, const int32_t* paren
     return x;
 }
 
-// Checks the whole call, then hands out the pages of the partly filled last pages. src, dst: per fork the page to copy (-1:
-// none) and its copy; result: the number of forks, 0 if the call is refused. Bound by its chain of memory round trips, as the
-// reserve plan: the first 1024 forks' values are fetched once (7.5 us with a fetch in each pass, 6.6 so).
+// Checks the whole call, the tables of the parents included (each parent's once, 1024 forks' entries at a time dealt out to the
+// threads, as the reserve plan deals out pages), then hands out the pages of the partly filled last pages. src, dst: per fork the
+// page to copy (-1: none) and its copy; result: the number of forks, 0 if the call is refused. Bound by its chain of memory round
+// trips, as the reserve plan: the first 1024 forks' values are fetched once (7.5 us with a fetch in each pass, 6.6 so).
 __global__ __launch_bounds__(kPlanBlock) void paged_fork_plan_kernel(PagedView c, const int32_t* parents, const int32_t* children,
                                                                      int count, int32_t* src, int32_t* dst, int32_t* result) {
-    __shared__ int lds[2 * kWave], few[kFew];
-    __shared__ uint32_t child[kPagedMaxSequences / 32];
+    __shared__ int lds[2 * kWave], few[kFew], before[kPlanBlock], row[kPlanBlock];
+    __shared__ uint32_t child[kPagedMaxSequences / 32], parent[kPagedMaxSequences / 32];
     const PageList free_pages = {few, dst + kPagedMaxSequences};
     const Counts first = counts_at(c, 0);
     const Fork mine = fork_at(c, parents, children, count, threadIdx.x);
     if (threadIdx.x == 0) *result = 0;
-    for (int i = threadIdx.x; i < (c.sequences + 31) / 32; i += kPlanBlock) child[i] = 0;
+    for (int i = threadIdx.x; i < (c.sequences + 31) / 32; i += kPlanBlock) child[i] = 0, parent[i] = 0;
     __syncthreads();
     bool bad = false;
     for (int f = threadIdx.x; f < count; f += kPlanBlock) {
@@ -272,6 +279,26 @@ __global__ __launch_bounds__(kPlanBlock) void paged_fork_plan_kernel(PagedView c
                 bad |= x.page < 0 || x.page >= c.pages;
                 ++need;
             }
+        }
+        bad = __syncthreads_or(bad);
+    }
+    if (!bad) {
+        const int t = threadIdx.x;
+        for (int base = 0; base < count; base += kPlanBlock) {
+            const int f = base + t;
+            const Fork x = base == 0 ? mine : fork_at(c, parents, children, count, f);
+            const bool first_of = f < count && !(atomicOr(&parent[x.parent >> 5], 1u << (x.parent & 31)) >> (x.parent & 31) & 1);
+            int all = 0;
+            before[t] = block_before(first_of ? x.full : 0, lds, &all);  // at most 2^20 a fork
+            row[t] = x.parent;
+            __syncthreads();
+#pragma unroll 4
+            for (int r = t; r < all; r += kPlanBlock) {
+                const int lo = last_at_most(before, r);
+                const int p = c.table[row[lo] * c.table_stride + r - before[lo]];
+                bad |= p < 0 || p >= c.pages;
+            }
+            __syncthreads();  // the next forks' entries
         }
         bad = __syncthreads_or(bad);
     }
@@ -313,10 +340,9 @@ __global__ __launch_bounds__(kCopyBlock) void paged_fork_kernel(PagedView c, con
     for (int f = blockIdx.x; f < count; f += gridDim.x) {
         const int s = parents[f], ch = children[f], full = (int)page_of(c, c.lens[ch]);
         for (int i = threadIdx.x; i < full; i += kCopyBlock) {
-            const int p = c.table[s * c.table_stride + i];
+            const int p = c.table[s * c.table_stride + i];  // the plan has checked it
             c.table[ch * c.table_stride + i] = p;
-            if (p >= 0 && p < c.pages) atomicAdd(c.refs + p, 1);
-            else raise(c);
+            atomicAdd(c.refs + p, 1);
         }
     }
     copy_pages(c, src, dst, count, elem, dense_k, dense_v, blockIdx.x, gridDim.x);

@@ -1220,3 +1220,29 @@ def test_free_leaves_a_sequence_with_a_bad_length(length):
     st.state.free([1])
     assert ops.device_errors() == 0
     st.check_state()
+
+
+@pytest.mark.parametrize("what", ["first page", "last full page", "partly filled page", "negative page", "length", "negative length", "parent of the last fork"])
+def test_fork_of_a_broken_parent_changes_nothing(what):
+    need_gpu()
+    say(f"fork refused: {what}")
+    S = 1200  # more forks than a workgroup has threads
+    st = Setup([70, 48, 5, 64] + [0] * S, 16, 2, 64, layers=2, seed=101, spare=2 * S, columns=6)
+    parents, children = [0, 1, 3] + [0] * (S - 4) + [2], list(range(4, 4 + S))
+    at, value = {"first page": ((0, 0), len(st.state.refs)), "last full page": ((3, 3), 1 << 30), "partly filled page": ((0, 4), 1 << 29),
+                 "negative page": ((1, 2), -1), "parent of the last fork": ((2, 0), -5)}.get(what, (None, None))
+    good_table, good_lens = st.table.clone(), st.lens.clone()
+    if at:
+        st.table[at] = value
+    else:
+        st.lens[1] = 6 * 16 + 1 if what == "length" else -1
+    before = [t.clone() for t in (st.table, st.lens, st.refs, st.k, st.v)]
+    ops.paged_cache_fork(st.cache, i32(parents), i32(children))
+    assert ops.device_errors() == _lib.DEVERR_PAGED
+    for t, x in zip((st.table, st.lens, st.refs, st.k, st.v), before):
+        assert torch.equal(t, x)
+    st.table.copy_(good_table)  # put right, the same call goes through
+    st.lens.copy_(good_lens)
+    ops.paged_cache_fork(st.cache, i32(parents), i32(children))
+    assert ops.device_errors() == 0 and st.state.fork(parents, children)
+    st.check_state()
