@@ -89,7 +89,8 @@ int moa_paged_cache_free(const moa_paged_cache* cache, const int32_t* sequences,
 
 /* Moves the live pages (reference count > 0; n of them) to pages 0 .. n - 1: those at n and beyond go,
  * in ascending order, to the free pages below n, in ascending order, in every layer. The page table
- * and the reference counts follow. */
+ * and the reference counts follow. A length out of range leaves the state as it was; a table entry outside the pool is
+ * left as it is (MOA_DEVERR_PAGED for both, for an entry only where some page moves). */
 int moa_paged_cache_compact(const moa_paged_cache* cache, void* stream);
 
 /* Attention of a batch's new rows over one layer of the cache, their own positions included (append

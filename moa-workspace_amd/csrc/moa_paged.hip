@@ -378,19 +378,29 @@ __global__ __launch_bounds__(kCopyBlock) void paged_free_kernel(PagedView c, con
 // ------------------------------------------------------------------------------------------- compact
 
 // list: place[p] for every page from the number of live pages on (where page p goes, itself if it does not move), and
-// behind kPagedMaxPages the targets and sources of the moves; result: the number of live pages, and of moves.
+// behind kPagedMaxPages the targets and sources of the moves; result: the number of live pages, and of moves. A length that is
+// out of range refuses the call: nobody could say which entries of that table follow their pages.
 __global__ __launch_bounds__(kPlanBlock) void paged_compact_plan_kernel(PagedView c, int32_t* place, int32_t* src, int32_t* dst,
                                                                         int32_t* result) {
     __shared__ uint64_t sums[kPlanWaves];
     __shared__ int lds[2 * kWave], few[kFew];
     const PageList targets = {few, dst};
     const Counts first = counts_at(c, 0);
+    bool bad = false;
+    for (int s = threadIdx.x; s < c.sequences; s += kPlanBlock) bad |= c.lens[s] < 0 || c.lens[s] > paged_capacity(c);
     uint64_t n = 0;
     for (int base = 0; base < c.pages; base += kStepPages) {
         Counts v = first;
         if (base) v = counts_at(c, base);
 #pragma unroll
         for (int j = 0; j < kPer; ++j) n += v.r[j] > 0;
+    }
+    if (__syncthreads_or(bad)) {
+        if (threadIdx.x == 0) {
+            result[1] = 0;
+            raise(c);
+        }
+        return;
     }
     const int live = (int)block_sum(n, sums);
     for (int p = live + (int)threadIdx.x; p < c.pages; p += kPlanBlock) place[p] = p;
@@ -418,12 +428,8 @@ __global__ __launch_bounds__(kCopyBlock) void paged_compact_kernel(PagedView c, 
     const int live = result[0], moves = result[1];
     if (!moves) return;
     for (int s = blockIdx.x; s < c.sequences; s += gridDim.x) {
-        const int len = c.lens[s];
-        if (len < 0 || len > paged_capacity(c)) {
-            if (threadIdx.x == 0) raise(c);
-            continue;
-        }
-        for (int i = threadIdx.x; i < pages_of(c, len); i += kCopyBlock) {
+        const int pages = pages_of(c, c.lens[s]);
+        for (int i = threadIdx.x; i < pages; i += kCopyBlock) {
             const int p = c.table[s * c.table_stride + i];
             if (p < 0 || p >= c.pages) raise(c);
             else if (p >= live) c.table[s * c.table_stride + i] = place[p];

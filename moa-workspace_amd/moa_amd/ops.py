@@ -489,7 +489,8 @@ def paged_cache_free(cache, sequences) -> None:
 
 def paged_cache_compact(cache) -> None:
     """Moves the n live pages to pages 0 .. n - 1 in every layer, page table and reference counts with them: those at n
-    and beyond go, in order, to the free pages below n."""
+    and beyond go, in order, to the free pages below n. A length out of range leaves all as it was, a table entry outside the
+    pool stays (bit 8)."""
     if not isinstance(cache, PagedCache):
         raise TypeError("cache must be a PagedCache")
     _call("moa_paged_cache_compact", cache._struct, _cache_stream(cache))

@@ -1246,3 +1246,38 @@ def test_fork_of_a_broken_parent_changes_nothing(what):
     ops.paged_cache_fork(st.cache, i32(parents), i32(children))
     assert ops.device_errors() == 0 and st.state.fork(parents, children)
     st.check_state()
+
+
+@pytest.mark.parametrize("at,length", [(1, -1), (1, 6 * 16 + 1), (0, 2 ** 31 - 1), (1499, -2 ** 31)])
+def test_compact_with_a_bad_length_changes_nothing(at, length):
+    need_gpu()
+    say(f"compact, sequence {at} of length {length}")
+    st = Setup([70, 48, 5, 96] + [0, 3] * 748, 16, 1, 64, layers=2, seed=102, spare=40, columns=6)
+    ops.paged_cache_free(st.cache, i32([2, 0]))
+    st.state.free([2, 0])
+    st.lens[at] = length
+    before = [t.clone() for t in (st.table, st.lens, st.refs, st.k, st.v)]
+    ops.paged_cache_compact(st.cache)
+    assert ops.device_errors() == _lib.DEVERR_PAGED
+    for t, x in zip((st.table, st.lens, st.refs, st.k, st.v), before):
+        assert torch.equal(t, x)
+    st.lens[at] = st.state.lens[at]
+    ops.paged_cache_compact(st.cache)
+    st.state.compact()
+    assert ops.device_errors() == 0
+    st.check_state()
+
+
+def test_compact_leaves_an_entry_outside_the_pool():
+    need_gpu()
+    say("compact, a table entry outside the pool")
+    st = Setup([70, 48, 5, 96], 16, 1, 64, seed=103, spare=9, columns=6)
+    ops.paged_cache_free(st.cache, i32([2, 0]))
+    st.state.free([2, 0])
+    for at, value in ((1, 1), len(st.state.refs)), ((3, 2), -9):
+        st.table[at] = value
+    ops.paged_cache_compact(st.cache)
+    assert ops.device_errors() == _lib.DEVERR_PAGED
+    st.state.compact()
+    st.state.table[1][1], st.state.table[3][2] = len(st.state.refs), -9
+    st.check_state()
