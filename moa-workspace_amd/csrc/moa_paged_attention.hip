@@ -176,7 +176,6 @@ __device__ bool token_block(const PagedView& c, const PagedAttentionCall& a, con
 // each and 167 whole.) The last tiles of a sequence, which see the most, come first.
 constexpr int kChunkRows = 128;
 constexpr int kChunkUnit = 64;
-constexpr int kChunkMinUnits = 4;
 struct ChunkPlan {
     int items;        // per KV head: workgroups that the device holds; records
     int most;         // no call has more items than this
@@ -217,11 +216,7 @@ __device__ ChunkWalk chunk_walk(const PagedView& c, const PagedAttentionCall& a,
     bad |= tiles > p.most - p.items;
     raise_bad(c, bad);
     if (tiles == 0 || tiles > p.most - p.items) return {0, 0, 0, 0};
-    // The float sum is rounded the same in every wave, and short by at most 1024 + 8 roundings of 2^-24: a part in ten
-    // thousand more covers them.
-    units = wave_sum(units);
-    const int per = (int)fminf(2.0001f * units / (float)p.items + 1.0f, 1e9f);
-    return {__builtin_amdgcn_readfirstlane(max(kChunkMinUnits, per)), 0, 0, 0};
+    return {__builtin_amdgcn_readfirstlane(chunk_part_units(wave_sum(units), p.items)), 0, 0, 0};  // the same in every wave
 }
 
 // Piece `want`, not before an earlier call's. False: there are not that many. have: the only 64 sequences' lanes, or nullptr.

@@ -6,4 +6,5 @@ int rows_in_range(int row0, int end, int rows, int max_rows) { return moa::rows_
 unsigned join_turn() { return moa::kJoinTurn; }
 unsigned join_share(int first, int parts) { return moa::join_share(first != 0, parts); }
 int join_last(unsigned before, unsigned share) { return moa::join_last(before, share); }
+int chunk_part_units(float total, int items) { return moa::chunk_part_units(total, items); }
 }

@@ -68,3 +68,17 @@ def test_counters_heal_after_calls_that_overlapped(plan):
         order = [(i == 0, parts) for i in range(parts)]
         rng.shuffle(order)
         assert arrive(plan, counter, order)[1] == [parts - 1]
+
+
+def test_the_parts_of_split_tiles_fit_their_records(plan):
+    """As many records are there as items. The total comes as short as f32 sums can make it: 1031 roundings of 2^-24."""
+    plan.chunk_part_units.argtypes, plan.chunk_part_units.restype = [C.c_float, C.c_int], C.c_int
+    rng = random.Random(5)
+    for _ in range(20000):
+        items = rng.choice([1, 2, 3, 5, 64, 270, 512, rng.randrange(1, 600)])
+        tiles, units = int(2 ** rng.uniform(0, 24)), int(2 ** rng.uniform(0, 24))
+        for n, u in ((tiles, units), (1, units), (items, units), (max(1, items // 2), units)):
+            total = n * u
+            part = plan.chunk_part_units(total * (1 - 2.0 ** -24) ** 1031, items)
+            parts = -(-u // part)
+            assert parts == 1 or (n * parts <= items and part * items >= 2 * total), (items, n, u, part)
