@@ -6,7 +6,8 @@
  * meaning of the reference's `#[device] fn` in FO/src/ops.rs, with the `device` handle
  * replaced by a trailing (M, stream) pair:
  *   - every tensor is a caller-owned device pointer (hipMalloc'd); the library never
- *     allocates per call (one per-device scratch block is made on first use or by moa_init);
+ *     allocates per call (one per-device scratch block is made on first use or by moa_init, the
+ *     paged calls' own, 98 MB, by the first of them);
  *   - `&mut` tensors of the reference (k_cache, v_cache, q_out, residual) are written in place;
  *   - bf16 tensors are raw uint16 bit patterns; E4M3FN/E2M1/E8M0 are uint8 codes;
  *   - M is the number of token rows (the reference processes exactly one, M = 1);
@@ -313,7 +314,7 @@ int moa_test_take_overs(uint32_t* count);
 
 /* Test support: which scratch exists on the current device, without creating either: bit 0 the
  * hipMalloc'd scratch of the ordinary entry points, bit 1 the static scratch of
- * moa_decoder_feedforward_fp8_noalloc. Touches no device memory. */
+ * moa_decoder_feedforward_fp8_noalloc, bit 2 the paged calls' scratch. Touches no device memory. */
 int moa_test_scratch_state(uint32_t* state);
 
 /* Test only: trips the state of `device` as a MOA_DEVERR_SPIN_TIMEOUT read by moa_device_errors

@@ -90,10 +90,6 @@ DevCtx* device_context(hipError_t* err) {
     const size_t t_rflag = carve(sizeof(uint64_t) * kRowsFlagWords);
     const size_t t_attn = carve(sizeof(float) * kAttnPartFloats);
     const size_t t_fattn = carve(sizeof(float) * kFattnPartFloats);
-    const size_t t_plist = carve(sizeof(int32_t) * (2 * (size_t)kPagedMaxPages + 16));
-    const size_t t_ptok = carve(sizeof(float) * kPagedTokenFloats);
-    const size_t t_pchunk = carve(sizeof(float) * kPagedChunkFloats);
-    const size_t t_ptick = carve(sizeof(uint32_t) * kPagedTickets);
     int cus = 0;
     *err = hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev);
     if (*err != hipSuccess) return nullptr;
@@ -123,10 +119,6 @@ DevCtx* device_context(hipError_t* err) {
     c.rows_flag = reinterpret_cast<uint64_t*>(b + t_rflag);
     c.attn_part = reinterpret_cast<float*>(b + t_attn);
     c.fattn_part = reinterpret_cast<float*>(b + t_fattn);
-    c.paged_list = reinterpret_cast<int32_t*>(b + t_plist);
-    c.paged_tokens = reinterpret_cast<float*>(b + t_ptok);
-    c.paged_chunks = reinterpret_cast<float*>(b + t_pchunk);
-    c.paged_tickets = reinterpret_cast<uint32_t*>(b + t_ptick);
     c.base = base;
     return &c;
 }
@@ -208,6 +200,50 @@ DevCtx* call_context(int* code) {
     DevCtx* c = device_context(&e);
     if (!c) *code = hip_fail(e, "allocating the per-device scratch");
     return c;
+}
+
+namespace {
+// The paged calls' scratch of the current device, 98 MB that a program without them does not pay for. A call may come while a stream is
+// captured (moa_init has been called, no paged call yet): the thread's capture mode is relaxed meanwhile and the counters
+// are cleared on a stream of their own, so that nothing of this enters the graph.
+hipError_t allocate_paged(DevCtx* c) {
+    size_t off = 0;
+    auto carve = [&](size_t bytes) { size_t at = off; off = align_up(off + bytes, 256); return at; };
+    const size_t t_list = carve(sizeof(int32_t) * (2 * (size_t)kPagedMaxPages + 16));
+    const size_t t_tok = carve(sizeof(float) * kPagedTokenFloats);
+    const size_t t_chunk = carve(sizeof(float) * kPagedChunkFloats);
+    const size_t t_tick = carve(sizeof(uint32_t) * kPagedTickets);
+    hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
+    hipError_t e = hipThreadExchangeStreamCaptureMode(&mode);
+    if (e != hipSuccess) return e;
+    void* base = nullptr;
+    hipStream_t s = nullptr;
+    e = hipMalloc(&base, off);
+    char* b = static_cast<char*>(base);
+    if (e == hipSuccess) e = hipStreamCreateWithFlags(&s, hipStreamNonBlocking);
+    if (e == hipSuccess) e = hipMemsetAsync(b + t_tick, 0, sizeof(uint32_t) * kPagedTickets, s);
+    if (e == hipSuccess) e = hipStreamSynchronize(s);
+    if (s) (void)hipStreamDestroy(s);
+    if (e != hipSuccess && base) (void)hipFree(base);
+    (void)hipThreadExchangeStreamCaptureMode(&mode);
+    if (e != hipSuccess) return e;
+    c->paged_tokens = reinterpret_cast<float*>(b + t_tok);
+    c->paged_chunks = reinterpret_cast<float*>(b + t_chunk);
+    c->paged_tickets = reinterpret_cast<uint32_t*>(b + t_tick);
+    c->paged_list = reinterpret_cast<int32_t*>(b + t_list);
+    return hipSuccess;
+}
+}  // namespace
+
+DevCtx* paged_context(int* code) {
+    DevCtx* c = call_context(code);
+    if (!c) return nullptr;
+    std::lock_guard<std::mutex> lock(g_ctx_mutex);
+    if (c->paged_list) return c;
+    const hipError_t e = allocate_paged(c);
+    if (e == hipSuccess) return c;
+    *code = hip_fail(e, "allocating the paged calls' scratch");
+    return nullptr;
 }
 
 int call_result(hipError_t e, const char* what) {
@@ -773,7 +809,8 @@ int moa_test_scratch_state(uint32_t* state) {
     hipError_t e = hipGetDevice(&dev);
     if (e != hipSuccess) return hip_fail(e, "hipGetDevice");
     if (dev < 0 || dev >= kMaxDevices) return fail(MOA_ERROR_NO_DEVICE, "device index out of range");
-    uint32_t v = existing_context(dev) ? 1u : 0u;
+    uint32_t v = 0;
+    if (const DevCtx* c = existing_context(dev)) v = c->paged_list ? 5u : 1u;
     {
         std::lock_guard<std::mutex> lock(g_na_mutex);
         if (g_na_ctx[dev].base) v |= 2u;

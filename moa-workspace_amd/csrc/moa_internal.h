@@ -103,7 +103,7 @@ struct DevCtx {
     uint64_t* rows_flag = nullptr; // tagged flags of the one-launch rows FFN (kRowsFlagWords)
     float* attn_part = nullptr;   // sliding_attention split partials (kAttnPartFloats)
     float* fattn_part = nullptr;  // full-attention page partials (kFattnPartFloats)
-    int32_t* paged_list = nullptr;  // 2 * kPagedMaxPages + 16: page lists of a cache call, its result word
+    int32_t* paged_list = nullptr;  // 2 * kPagedMaxPages + 16: page lists of a cache call, its result word (paged_context)
     float* paged_tokens = nullptr;  // paged attention's split records (kPagedTokenFloats, kPagedChunkFloats)
     float* paged_chunks = nullptr;
     uint32_t* paged_tickets = nullptr;  // kPagedTickets
@@ -124,6 +124,8 @@ DevCtx* device_context(hipError_t* err);
 // The context of the current device for a call that computes on it; nullptr, with *code set and the
 // error recorded, where there is none or its state is tripped.
 DevCtx* call_context(int* code);
+// The same with the paged calls' scratch, which the first of them allocates.
+DevCtx* paged_context(int* code);
 // MOA_SUCCESS, or MOA_ERROR_HIP with the reason recorded.
 int call_result(hipError_t e, const char* what);
 

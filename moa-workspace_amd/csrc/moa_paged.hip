@@ -603,7 +603,7 @@ int moa_paged_cache_reserve(const moa_paged_cache* cache, const int32_t* new_tok
     PagedView v;
     int e;
     if ((e = cache_view(cache, 0, &v)) || (e = check_ptr(new_tokens, "new_tokens", 4))) return e;
-    DevCtx* ctx = call_context(&e);
+    DevCtx* ctx = paged_context(&e);
     if (!ctx) return e;
     v.err = ctx->err;
     hipLaunchKernelGGL(paged_reserve_kernel, dim3(1), dim3(kPlanBlock), 0, static_cast<hipStream_t>(stream), v, new_tokens,
@@ -637,7 +637,7 @@ int moa_paged_cache_fork(const moa_paged_cache* cache, const int32_t* parents, c
     if ((e = cache_view(cache, 0, &v)) || (e = check_range(count, 0, kPagedMaxSequences, "count"))) return e;
     if (count == 0) return MOA_SUCCESS;
     if ((e = check_ptr(parents, "parents", 4)) || (e = check_ptr(children, "children", 4))) return e;
-    DevCtx* ctx = call_context(&e);
+    DevCtx* ctx = paged_context(&e);
     if (!ctx) return e;
     v.err = ctx->err;
     int32_t *src = ctx->paged_list, *dst = src + kPagedMaxPages, *result = dst + kPagedMaxPages;
@@ -669,7 +669,7 @@ int moa_paged_cache_compact(const moa_paged_cache* cache, void* stream) {
     PagedView v;
     int e;
     if ((e = cache_view(cache, 0, &v))) return e;
-    DevCtx* ctx = call_context(&e);
+    DevCtx* ctx = paged_context(&e);
     if (!ctx) return e;
     v.err = ctx->err;
     // at most half of the pages move: their sources and targets share the second list
@@ -704,7 +704,7 @@ int moa_paged_attention(const uint16_t* q, int64_t q_row_stride, const moa_paged
     for (const int64_t st : {q_row_stride, out_row_stride})
         if (rows > 1 && (st < width || st % 8 || st > (int64_t(1) << 40)))
             return bad_value("q and out row strides must be multiples of 8 elements and at least q_heads * head_dim, got " + std::to_string(st));
-    DevCtx* ctx = call_context(&e);
+    DevCtx* ctx = paged_context(&e);
     if (!ctx) return e;
     v.err = ctx->err;
     const PagedAttentionCall a{q, out, q_row_stride, out_row_stride, row_starts, rows, q_heads, q_heads / v.kv_heads,
