@@ -280,10 +280,6 @@ struct Check {
     }
 };
 
-DevCtx* ctx_or_fail(int* code) { return call_context(code); }
-
-int finish(hipError_t e, const char* what) { return call_result(e, what); }
-
 int qkv_common(const QkvParams& p, int M, void* stream) {
     Check c;
     c.ptr(p.x, "x").ptr(p.qw, "q_weight").ptr(p.kw, "k_weight").ptr(p.vw, "v_weight");
@@ -294,12 +290,12 @@ int qkv_common(const QkvParams& p, int M, void* stream) {
     c.ptr(p.k_cache, "k_cache").ptr(p.v_cache, "v_cache").ptr(p.q_out, "q_out").rows(M);
     if (c.code) return c.code;
     int code = MOA_SUCCESS;
-    DevCtx* ctx = ctx_or_fail(&code);
+    DevCtx* ctx = call_context(&code);
     if (!ctx) return code;
     hipStream_t s = static_cast<hipStream_t>(stream);
-    if (M <= kMaxDecodeM) return finish(launch_qkv_decode(p, M, s, ctx), "sliding_project_qkv launch");
+    if (M <= kMaxDecodeM) return call_result(launch_qkv_decode(p, M, s, ctx), "sliding_project_qkv launch");
     for (int m0 = 0; m0 < M; m0 += kMaxChunkM) {
-        const int e = finish(launch_qkv_chunk(p, m0, M - m0 < kMaxChunkM ? M - m0 : kMaxChunkM, s, ctx),
+        const int e = call_result(launch_qkv_chunk(p, m0, M - m0 < kMaxChunkM ? M - m0 : kMaxChunkM, s, ctx),
                              "sliding_project_qkv launch");
         if (e) return e;
     }
@@ -314,9 +310,9 @@ int o_check(const OParams& p, int M) {
 }
 
 int o_launch(const OParams& p, int M, hipStream_t s, DevCtx* ctx) {
-    if (M <= kMaxDecodeM) return finish(launch_o_decode(p, M, s, ctx), "sliding_attention_output launch");
+    if (M <= kMaxDecodeM) return call_result(launch_o_decode(p, M, s, ctx), "sliding_attention_output launch");
     for (int m0 = 0; m0 < M; m0 += kMaxChunkM) {
-        const int e = finish(launch_o_chunk(p, m0, M - m0 < kMaxChunkM ? M - m0 : kMaxChunkM, s, ctx),
+        const int e = call_result(launch_o_chunk(p, m0, M - m0 < kMaxChunkM ? M - m0 : kMaxChunkM, s, ctx),
                              "sliding_attention_output launch");
         if (e) return e;
     }
@@ -326,7 +322,7 @@ int o_launch(const OParams& p, int M, hipStream_t s, DevCtx* ctx) {
 int o_common(const OParams& p, int M, void* stream) {
     if (const int bad = o_check(p, M)) return bad;
     int code = MOA_SUCCESS;
-    DevCtx* ctx = ctx_or_fail(&code);
+    DevCtx* ctx = call_context(&code);
     if (!ctx) return code;
     return o_launch(p, M, static_cast<hipStream_t>(stream), ctx);
 }
@@ -354,9 +350,9 @@ int ffn_check(const FfnParams& p, int M) {
 
 int ffn_launch(const FfnParams& p, int M, hipStream_t s, DevCtx* ctx) {
     // More than kMaxDecodeM rows take the MFMA path (every weight format).
-    if (M <= kMaxDecodeM) return finish(launch_ffn_decode(p, M, s, ctx), "decoder_feedforward launch");
+    if (M <= kMaxDecodeM) return call_result(launch_ffn_decode(p, M, s, ctx), "decoder_feedforward launch");
     for (int m0 = 0; m0 < M; m0 += kMaxChunkM) {
-        const int e = finish(launch_ffn_chunk(p, m0, M - m0 < kMaxChunkM ? M - m0 : kMaxChunkM, s, ctx),
+        const int e = call_result(launch_ffn_chunk(p, m0, M - m0 < kMaxChunkM ? M - m0 : kMaxChunkM, s, ctx),
                              "decoder_feedforward launch");
         if (e) return e;
     }
@@ -366,7 +362,7 @@ int ffn_launch(const FfnParams& p, int M, hipStream_t s, DevCtx* ctx) {
 int ffn_common(const FfnParams& p, int M, void* stream) {
     if (const int bad = ffn_check(p, M)) return bad;
     int code = MOA_SUCCESS;
-    DevCtx* ctx = ctx_or_fail(&code);
+    DevCtx* ctx = call_context(&code);
     if (!ctx) return code;
     return ffn_launch(p, M, static_cast<hipStream_t>(stream), ctx);
 }
@@ -379,22 +375,22 @@ int o_ffn_common(const OParams& o, const FfnParams& p, int M, void* stream) {
     if (const int bad = o_check(o, M)) return bad;
     if (const int bad = ffn_check(p, M)) return bad;
     int code = MOA_SUCCESS;
-    DevCtx* ctx = ctx_or_fail(&code);
+    DevCtx* ctx = call_context(&code);
     if (!ctx) return code;
     hipStream_t s = static_cast<hipStream_t>(stream);
     hipError_t e = hipSuccess;
     if (M == 1 && launch_o_ffn_fused(o, p, s, ctx, &e))
-        return finish(e, "sliding_attention_output_feedforward launch");
+        return call_result(e, "sliding_attention_output_feedforward launch");
     if (M > kMaxDecodeM) {  // the MFMA path: O's post rows write the FFN's normalised input too
         for (int m0 = 0; m0 < M; m0 += kMaxChunkM) {
-            const int bad = finish(launch_o_ffn_chunk(o, p, m0, M - m0 < kMaxChunkM ? M - m0 : kMaxChunkM, s, ctx),
+            const int bad = call_result(launch_o_ffn_chunk(o, p, m0, M - m0 < kMaxChunkM ? M - m0 : kMaxChunkM, s, ctx),
                                    "sliding_attention_output_feedforward launch");
             if (bad) return bad;
         }
         return MOA_SUCCESS;
     }
     if (M >= kRowsProjMinM)  // the rows path: O's post rows write the FFN's normalised input too
-        return finish(launch_o_ffn_rows(o, p, 0, M, s, ctx), "sliding_attention_output_feedforward launch");
+        return call_result(launch_o_ffn_rows(o, p, 0, M, s, ctx), "sliding_attention_output_feedforward launch");
     if (const int bad = o_launch(o, M, s, ctx)) return bad;
     return ffn_launch(p, M, s, ctx);
 }
@@ -416,7 +412,7 @@ int moa_init(int device) {
     e = hipSetDevice(device);
     if (e != hipSuccess) return hip_fail(e, "hipSetDevice");
     int code = MOA_SUCCESS;
-    if (!ctx_or_fail(&code)) return code;
+    if (!call_context(&code)) return code;
     return noalloc_context(&code) ? MOA_SUCCESS : code;
 }
 
@@ -534,7 +530,7 @@ int moa_decoder_feedforward_fp8_noalloc(uint16_t* residual, const uint16_t* pre_
     int code = MOA_SUCCESS;
     DevCtx* ctx = noalloc_context(&code);
     if (!ctx) return code;
-    return finish(launch_ffn_decode(p, M, static_cast<hipStream_t>(stream), ctx), "decoder_feedforward_fp8_noalloc launch");
+    return call_result(launch_ffn_decode(p, M, static_cast<hipStream_t>(stream), ctx), "decoder_feedforward_fp8_noalloc launch");
 }
 
 int moa_decoder_feedforward_mxfp4(uint16_t* residual, const uint16_t* pre_ff_rms_weight,
@@ -595,9 +591,9 @@ int moa_sliding_attention(const uint16_t* q, const uint16_t* k, const uint16_t* 
     c.ptr(q, "q").ptr(k, "k").ptr(v, "v").ptr(mask, "mask", 4).ptr(out, "out").rows(M);
     if (c.code) return c.code;
     int code = MOA_SUCCESS;
-    DevCtx* ctx = ctx_or_fail(&code);
+    DevCtx* ctx = call_context(&code);
     if (!ctx) return code;
-    return finish(launch_sliding_attention(q, k, v, mask, out, M, static_cast<hipStream_t>(stream), ctx),
+    return call_result(launch_sliding_attention(q, k, v, mask, out, M, static_cast<hipStream_t>(stream), ctx),
                   "sliding_attention launch");
 }
 
@@ -614,14 +610,14 @@ int moa_full_project_qkv(const uint16_t* x, const uint8_t* q_weight, const uint8
     c.ptr(k_cache, "k_cache").ptr(v_cache, "v_cache").ptr(q_out, "q_out").rows(M);
     if (c.code) return c.code;
     int code = MOA_SUCCESS;
-    DevCtx* ctx = ctx_or_fail(&code);
+    DevCtx* ctx = call_context(&code);
     if (!ctx) return code;
     QkvParams p{x, q_weight, k_weight, nullptr, q_weight_scale, k_weight_scale, nullptr, ScaleKind::BF16,
                 input_rms_weight, q_rms_weight, k_rms_weight, kv_offset, rope_offset, cos, sin, k_cache, v_cache, q_out};
     hipStream_t s = static_cast<hipStream_t>(stream);
-    if (M <= kMaxDecodeM) return finish(launch_full_qkv(p, M, s, ctx), "full_project_qkv launch");
+    if (M <= kMaxDecodeM) return call_result(launch_full_qkv(p, M, s, ctx), "full_project_qkv launch");
     for (int m0 = 0; m0 < M; m0 += kMaxFullQkvM) {
-        const int e = finish(launch_full_qkv_chunk(p, m0, M - m0 < kMaxFullQkvM ? M - m0 : kMaxFullQkvM, s, ctx),
+        const int e = call_result(launch_full_qkv_chunk(p, m0, M - m0 < kMaxFullQkvM ? M - m0 : kMaxFullQkvM, s, ctx),
                              "full_project_qkv launch");
         if (e) return e;
     }
@@ -635,9 +631,9 @@ static int full_page(const uint16_t* q, const uint16_t* k, const uint16_t* v, co
     c.ptr(running_sum, "running_sum", 4).ptr(out, "out").rows(M);
     if (c.code) return c.code;
     int code = MOA_SUCCESS;
-    DevCtx* ctx = ctx_or_fail(&code);
+    DevCtx* ctx = call_context(&code);
     if (!ctx) return code;
-    return finish(launch_full_attention_page(q, k, v, mask, running_max, running_sum, out, M, first,
+    return call_result(launch_full_attention_page(q, k, v, mask, running_max, running_sum, out, M, first,
                                              static_cast<hipStream_t>(stream), ctx),
                   first ? "full_attention_first_page launch" : "full_attention_page launch");
 }
@@ -660,9 +656,9 @@ int moa_full_attention(const uint16_t* q, const uint16_t* k_pages, const uint16_
     if (c.code) return c.code;
     if (P < 1 || P > kCf) return fail(MOA_ERROR_INVALID_VALUE, "P must be in [1, 64], got " + std::to_string(P));
     int code = MOA_SUCCESS;
-    DevCtx* ctx = ctx_or_fail(&code);
+    DevCtx* ctx = call_context(&code);
     if (!ctx) return code;
-    return finish(launch_full_attention(q, k_pages, v_pages, masks, P, running_max, running_sum, out, M,
+    return call_result(launch_full_attention(q, k_pages, v_pages, masks, P, running_max, running_sum, out, M,
                                         static_cast<hipStream_t>(stream), ctx),
                   "full_attention launch");
 }
@@ -675,13 +671,13 @@ int moa_full_attention_output(const uint16_t* x, const float* running_sum, const
     c.ptr(o_weight, "o_weight").ptr(o_weight_scale, "o_weight_scale", 2).ptr(residual, "residual").rows(M);
     if (c.code) return c.code;
     int code = MOA_SUCCESS;
-    DevCtx* ctx = ctx_or_fail(&code);
+    DevCtx* ctx = call_context(&code);
     if (!ctx) return code;
     OParams p{x, post_attn_rms_weight, o_weight, o_weight_scale, ScaleKind::BF16, residual, running_sum};
     hipStream_t s = static_cast<hipStream_t>(stream);
-    if (M <= kMaxDecodeM) return finish(launch_full_o(p, M, s, ctx), "full_attention_output launch");
+    if (M <= kMaxDecodeM) return call_result(launch_full_o(p, M, s, ctx), "full_attention_output launch");
     for (int m0 = 0; m0 < M; m0 += kMaxChunkM) {
-        const int e = finish(launch_o_chunk(p, m0, M - m0 < kMaxChunkM ? M - m0 : kMaxChunkM, s, ctx),
+        const int e = call_result(launch_o_chunk(p, m0, M - m0 < kMaxChunkM ? M - m0 : kMaxChunkM, s, ctx),
                              "full_attention_output launch");
         if (e) return e;
     }
@@ -694,7 +690,7 @@ int moa_final_norm_and_logits(const uint16_t* input, const uint16_t* rms_weight,
     c.ptr(input, "input").ptr(rms_weight, "rms_weight").ptr(lm_head_weight, "lm_head_weight").ptr(out, "out").rows(M);
     if (c.code) return c.code;
     if (g_tripped[current_device_or_0()].load()) return tripped_fail(current_device_or_0());
-    return finish(launch_final_norm_and_logits(input, rms_weight, lm_head_weight, out, M, static_cast<hipStream_t>(stream)),
+    return call_result(launch_final_norm_and_logits(input, rms_weight, lm_head_weight, out, M, static_cast<hipStream_t>(stream)),
                   "final_norm_and_logits launch");
 }
 
@@ -707,7 +703,7 @@ int moa_fp8_scaled_projection(const uint16_t* x, const uint8_t* w, const float* 
     if (M > 65535) return fail(MOA_ERROR_INVALID_VALUE, "M must be <= 65535 for the projection");
     if (g_tripped[current_device_or_0()].load()) return tripped_fail(current_device_or_0());
     ProjParams p{x, w, scale, ScaleKind::F32, out, N, K};
-    return finish(launch_proj_decode(p, M, static_cast<hipStream_t>(stream)), "fp8_scaled_projection launch");
+    return call_result(launch_proj_decode(p, M, static_cast<hipStream_t>(stream)), "fp8_scaled_projection launch");
 }
 
 int moa_test_epoch_layout(int kernel, int* counters, int* per) {
@@ -734,7 +730,7 @@ int moa_test_epoch_tag(int kernel, uint64_t old, uint32_t* tag) {
 
 int moa_test_preset_epochs(uint64_t launches) {
     int code = MOA_SUCCESS;
-    DevCtx* ctx = ctx_or_fail(&code);
+    DevCtx* ctx = call_context(&code);
     if (!ctx) return code;
     hipError_t e = hipDeviceSynchronize();
     auto put64 = [&](int first, int n, uint64_t v) {
@@ -748,7 +744,7 @@ int moa_test_preset_epochs(uint64_t launches) {
     const uint32_t at = (uint32_t)(launches * 32u);
     for (int i = 0; i < kMaxDecodeM * kNs && e == hipSuccess; ++i)
         e = hipMemcpy(ctx->tickets + (size_t)(kTicketAttn + i) * kTicketStride, &at, sizeof at, hipMemcpyHostToDevice);
-    return finish(e, "presetting the epoch counters");
+    return call_result(e, "presetting the epoch counters");
 }
 
 int moa_test_set_stall(uint32_t steal_ticks, uint32_t hold_ticks, const int32_t* hold) {
@@ -792,7 +788,7 @@ int moa_test_take_overs(uint32_t* count) {
         total += n;
     }
     if (e == hipSuccess) *count = total;
-    return finish(e, "reading the take-over count");
+    return call_result(e, "reading the take-over count");
 }
 
 int moa_test_trip_device_state(int device) {
@@ -823,7 +819,7 @@ int moa_format_selftest(uint32_t* out, void* stream) {
     Check c;
     c.ptr(out, "out", 4);
     if (c.code) return c.code;
-    return finish(launch_format_selftest(out, static_cast<hipStream_t>(stream)), "format selftest launch");
+    return call_result(launch_format_selftest(out, static_cast<hipStream_t>(stream)), "format selftest launch");
 }
 
 }  // extern "C"
