@@ -816,9 +816,9 @@ __device__ __forceinline__ void chunk_part(const PagedView& c, const PagedAttent
     const int l32 = lane & 31, hf = lane >> 5;
     const int rg = wave & 3, half = wave >> 2;  // rows 32 rg .., dims half * kMine ..
     // x = factor (q . k): a negative factor's sign goes to q, so that the largest product is the largest x; and a factor of
-    // zero stays above it, so that a product of -inf (a position that a row does not see) stays -inf
+    // zero stays above it, so that a product of -inf (a position that a row does not see) stays -inf (a NaN stays one)
     const float signed_factor = E4M3 ? c.k_scale[kvh] * a.scale_log2 : a.scale_log2;
-    const float factor = fmaxf(fabsf(signed_factor), 1.2e-38f);
+    const float factor = fabsf(signed_factor) < 1.2e-38f ? 1.2e-38f : fabsf(signed_factor);
     const uint32_t flip = signed_factor < 0.0f ? 0x80008000u : 0u;
     // LDS byte addresses of a lane: K rows lane % 32, chunk 2 s + lane / 32; V's transposing reads, dim tile 0
     auto k_address = [&] {

@@ -1281,3 +1281,21 @@ def test_compact_leaves_an_entry_outside_the_pool():
     st.state.compact()
     st.state.table[1][1], st.state.table[3][2] = len(st.state.refs), -9
     st.check_state()
+
+
+@pytest.mark.parametrize("n,group,dim", [(1, 4, 128), (1, 2, 256), (40, 4, 128), (40, 2, 256), (30, 4, 512)])
+@pytest.mark.parametrize("which", ["k_scale", "v_scale"])
+def test_a_scale_that_is_nan_shows_in_its_heads(which, n, group, dim):
+    """E4M3 pages: the query heads of that KV head are NaN, in single tokens and in chunks; the others are unharmed."""
+    need_gpu()
+    say(f"paged attention, a NaN {which}, {n} rows of {dim}")
+    st = Setup([300], 16, 2, dim, "e4m3", seed=104)
+    sc = st.k_scale[0].clone(), st.v_scale[0].clone()
+    getattr(st, which)[0, 1] = float("nan")
+    q = queries(n, 2 * group, dim, 105)
+    out = torch.zeros_like(q)
+    ops.paged_attention(q, st.cache, i32([0, n]), out)
+    assert ops.device_errors() == 0
+    want, a, d = pm.attention(q, *st.values(), st.state.table, [300], [0, n], 16, 0, 1.0, *sc)
+    assert torch.isnan(out[:, group:].float()).all()
+    check_rows(out[:, :group], want[:, :group], a[:, :group], d[:, :group], dim)
