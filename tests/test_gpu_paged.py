@@ -1299,3 +1299,43 @@ def test_a_scale_that_is_nan_shows_in_its_heads(which, n, group, dim):
     want, a, d = pm.attention(q, *st.values(), st.state.table, [300], [0, n], 16, 0, 1.0, *sc)
     assert torch.isnan(out[:, group:].float()).all()
     check_rows(out[:, :group], want[:, :group], a[:, :group], d[:, :group], dim)
+
+
+def test_calls_wait_for_the_current_streams_work():
+    """New keys, values and queries are made by work that is still running on the side stream when the calls are issued: nothing between it
+    and the calls waits, so a call on another stream would read the zeros that were there before."""
+    need_gpu()
+    say("paged calls behind running work of a side stream")
+    st = Setup([100, 40], 16, 2, 128, seed=106, spare=10, columns=20)
+    lens, rows = [101, 70], [1, 30]
+    side = torch.cuda.Stream()
+    new, starts = i32(rows), i32(starts_of(rows))
+    nk, nv, q = (torch.zeros((31, h, 128), dtype=torch.bfloat16, device=DEV) for h in (2, 2, 8))
+    made = queries(31, 2, 128, 1, 11.0), queries(31, 2, 128, 2, 11.0), queries(31, 8, 128, 3)
+    out = torch.full_like(q, 123.0)
+    big = torch.randn((4096, 4096), device=DEV)
+    before = [t.float().clone() for t in (st.k[0], st.v[0])]
+    for warm in (True, False):  # the first turn loads what the second one needs, so that it runs without a pause
+        with torch.cuda.stream(side):
+            x = big
+            for _ in range(1 if warm else 20):
+                x = x @ big
+                x = x / x.norm()
+            zero = (x[0, 0] * 0).to(torch.bfloat16)
+            for t, m in zip((nk, nv, q), made):
+                t.copy_(m + zero if not warm else t)
+            if not warm:
+                busy = not side.query()
+                ops.paged_cache_reserve(st.cache, new)
+                ops.paged_cache_append(st.cache, nk, nv, starts)
+                ops.paged_attention(q, st.cache, starts, out, max_rows=30)
+        torch.cuda.synchronize()
+    assert busy, "the side stream had finished before the calls were issued: the test shows nothing"
+    assert ops.device_errors() == 0 and st.state.reserve(rows)
+    st.check_state()
+    for t, old, m in zip((st.k[0], st.v[0]), before, made):
+        for i, s, pos in pm.positions(starts_of(rows), lens):
+            old[st.state.table[s][pos // 16], pos % 16] = m[i].float()
+        assert torch.equal(t.float(), old)
+    want, a, d = pm.attention(made[2], *before, st.state.table, lens, starts_of(rows), 16, 0, 1.0)
+    check_rows(out, want, a, d, 128)
