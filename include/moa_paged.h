@@ -104,8 +104,9 @@ int moa_paged_cache_compact(const moa_paged_cache* cache, void* stream);
  * query heads per KV head. max_rows: the most rows a sequence has in this call (it chooses the kernel
  * and its grid; rows itself is always right). Rows that belong to no sequence are left as they were.
  * A sequence whose rows or length are out of range, or that has more than max_rows rows, is left out; so
- * is at least every row that sees a page outside the pool, and row starts that descend may leave out all
- * (MOA_DEVERR_PAGED). The result is deterministic; how the positions are split, and with it the order of f32 sums,
+ * is at least every row that sees a page outside the pool, and row starts that descend may leave out all; rows that two sequences
+ * claim by such starts get either's result (MOA_DEVERR_PAGED for each). The entries of positions before a window have to
+ * name pages of the pool too: tiles begin up to 63 positions before it. The result is deterministic; how the positions are split, and with it the order of f32 sums,
  * follows the whole batch, so a row's last bits may differ between calls of other batches. Scores, maxima, sums and outputs are
  * f32; a weight enters the product with V as two bf16 numbers, which hold it to 2^-16 of itself, in every row of every call; the
  * result is rounded once. rows may be 0. */

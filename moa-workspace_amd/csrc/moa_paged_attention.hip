@@ -29,7 +29,7 @@ __device__ __forceinline__ bf16x8 as_bf16x8(const uint4& v) { return __builtin_b
 
 // Two weights as two pairs of bf16, high parts and rests: what is lost is at most 2^-16 of a weight. (One part alone loses 2^-8,
 // which is more than what is left where values nearly cancel; a third, for the last 8 bits of f32, takes the chunk kernel another 24 %
-// and moves the result by less than the f32 rounding of its scores does.)
+// and is below what the f32 rounding of the scores can move.)
 constexpr int kParts = 2;
 __device__ __forceinline__ void split_weights(float p0, float p1, uint32_t (&w)[kParts]) {
     w[0] = pk_bf16(p0, p1);
@@ -735,10 +735,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(TokenShape<
 // row are what it supplies as B of V^T times P^T when V's transposing LDS reads fetch the same positions: P moves
 // between no lanes, and a row's maximum, sum and rescaling stay in its lane. P enters as two bf16 parts, which share V's
 // fragments, and up to 256 dims 16 positions are weighed beside the products of the 16 before them. (Four prompts of 1100 to 4100
-// tokens, 32 heads of 128 over 8: 301 us, 0.59 PFLOP/s of the products' own work; 318 with all weights first, 250 with one part.)
+// tokens, 32 heads of 128 over 8: 298 to 310 us from card to card, 0.59 PFLOP/s of the formula's work; 318 with all weights first,
+// 250 with one part. The same over E4M3 pages: 294.)
 // 512 dims: a row's Q and out do not fit beside each other in a wave's registers, so two waves share 32 rows, each with
 // half of the dims: they add the halves of the scores through LDS, and each weighs half of the positions for both (1000 rows of
-// 16 heads over 15800 positions: 810 us; 677 with one part).
+// 16 heads over 15800 positions: 810 to 860 us from card to card, 677 with one part; over E4M3 pages 1020).
 template <int D, bool E4M3>
 struct ChunkShape {
     static constexpr int kTile = D >= 256 ? 32 : 64;
@@ -785,7 +786,10 @@ __device__ __forceinline__ int in_loop(int v) {
     return v;
 }
 // The lane, computed where it is used: registers that the chunk kernel's loop reloaded from scratch memory would wait for every
-// load into LDS before them (512 dims, 1000 rows over 15800 positions: 758 us with three such reloads a tile, 734 without).
+// load into LDS before them (512 dims, 1000 rows over 15800 positions: three such reloads a tile cost 24 us). What the chunk kernels
+// still spill (32 and 46 registers at 256 dims, bf16 and E4M3, 24 and 52 at 512) lies outside that loop, but for one reload a tile before
+// each of the products at 256 dims and, with E4M3 pages, for five at 256 dims and three at 512; seen positions computed in the loop instead
+// of held took one away: 148 us for 152 there, 1 % more elsewhere, and were left out.
 __device__ __forceinline__ int lane_here() {
     int v;
     __asm__ volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(v));
@@ -1076,7 +1080,7 @@ __device__ __forceinline__ void chunk_part(const PagedView& c, const PagedAttent
             }
             {
                 // step n: 16 positions n / kDims, dim tile n % kDims (the next 16 positions weighed beside it: see above). V is read kAhead
-                // steps ahead: four took 256 and 512 dims 172 and 886 us, three 152 and 810 (registers).
+                // steps ahead: four took 256 dims (mixed chunks and tokens) 172 us and 512 dims 886, three 152 and 810 (registers).
                 constexpr int kAhead = T::kSub == 2 ? 4 : 3, kUnits = 2 * T::kSub, kN = kUnits * kDims;
                 const float mu = m_ref == -INFINITY ? 0.0f : m_ref;
                 float sum = 0.0f;  // (pairs of waves have added theirs)
@@ -1198,7 +1202,7 @@ __device__ __forceinline__ void chunk_part(const PagedView& c, const PagedAttent
         if (odd && !bad) careful_piece<E4M3>(c, a, t, kvh, r0, nr, lo, hi, [&](int, const Row& x) { return a.q + x.m * a.q_row + x.h * D; }, rec, kChunkRows);
     };
     // Few workgroups have a second item: the first takes the sequences that the walk has read (four prompts of 32 heads of 128,
-    // five items in turn on a place: 251 us, 254 with them read again; 512 dims: 683 and 675, for want of registers).
+    // five items in turn on a place: 3 us less than with them read again; 512 dims: 8 us more, for want of registers).
     int item = first;
     if constexpr (kPair == 1) {
         if (item >= plan.most || !find_piece(c, a, walk, 0, item, &seqs, &t)) return;
@@ -1214,7 +1218,7 @@ __device__ __forceinline__ void chunk_part(const PagedView& c, const PagedAttent
 // Chunks, and up to 256 dims the token rows beside them: a workgroup of either kind fits a CU next to one of the other, the
 // one bound by memory, the other by arithmetic. `stripe` groups in a row (a KV head's share of one workgroup per CU) are
 // chunks', the next tokens', until the token groups are used up. (30 single tokens and 5 chunks of 8 heads of 256, window 1024:
-// 144 us in two launches, 112 in one.)
+// 152 us, with weights of one part 118; in two launches 32 us more.)
 template <int D, bool E4M3>
 __global__ __launch_bounds__((ChunkShape<D, E4M3>::kThreads)) __attribute__((amdgpu_waves_per_eu(2))) void paged_chunk_kernel(
     PagedView c, PagedAttentionCall a, ChunkPlan plan, int token_groups, int stripe, float* token_records, float* chunk_records) {

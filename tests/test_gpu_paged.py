@@ -1339,3 +1339,41 @@ def test_calls_wait_for_the_current_streams_work():
         assert torch.equal(t.float(), old)
     want, a, d = pm.attention(made[2], *before, st.state.table, lens, starts_of(rows), 16, 0, 1.0)
     check_rows(out, want, a, d, 128)
+
+
+def test_one_scratch_ring_serves_the_projections_of_a_whole_step():
+    """Sequences at positions of their own: a QKV call each, into one ring, at the slots of their rows in the step; the rows then lie in the
+    order that one append and one attention take."""
+    need_gpu()
+    say("QKV of three sequences into one scratch ring, one append, one attention")
+    from gpu_util import dev, dev_zeros
+    from moa_amd import synth
+    before, M = [700, 31, 0], [1, 3, 20]
+    lens, starts = [b + m for b, m in zip(before, M)], starts_of(M)
+    st = Setup(before, 64, 8, 256, seed=107, spare=20, columns=12)
+    ops.paged_cache_reserve(st.cache, i32(M))
+    assert st.state.reserve(M)
+    kr, vr, q = dev_zeros(1024 * 2048), dev_zeros(1024 * 2048), dev_zeros(sum(M) * 4096)
+    apart = []
+    names = ("x", "q_weight", "k_weight", "v_weight", "q_weight_scale", "k_weight_scale", "v_weight_scale", "input_rms_weight",
+             "q_rms_weight", "k_rms_weight")
+    for s, m in enumerate(M):
+        d = synth.cfg_qkv(seed=3 + s, M=m, pos=before[s])
+        w = [dev(d[n]) for n in names]
+        cos, sin, rope = dev(d["cos"]), dev(d["sin"]), i32([512 * before[s]])
+        ops.sliding_project_qkv(*w, i32([4096 * starts[s]]), rope, cos, sin, kr, vr, q[starts[s] * 4096:starts[s + 1] * 4096])
+        own = dev_zeros(1024 * 2048), dev_zeros(1024 * 2048), dev_zeros(m * 4096)
+        ops.sliding_project_qkv(*w, i32([4096 * before[s]]), rope, cos, sin, *own)
+        apart.append([own[0].view(1024, 2048)[before[s]:lens[s]], own[1].view(1024, 2048)[before[s]:lens[s]], own[2]])
+    k, v = (t.view(torch.bfloat16).view(1024, 8, 256)[:sum(M)] for t in (kr, vr))
+    q = q.view(torch.bfloat16).view(sum(M), 16, 256)
+    for got, i in ((k, 0), (v, 1), (q, 2)):
+        assert torch.equal(raw(got).flatten(), torch.cat([a[i].flatten().view(torch.int16) for a in apart]))
+    out = torch.empty_like(q)
+    ops.paged_cache_append(st.cache, k, v, i32(starts))
+    ops.paged_attention(q, st.cache, i32(starts), out, window=1024, max_rows=max(M))
+    assert ops.device_errors() == 0
+    want, a, d = pm.attention(q, *st.values(), st.state.table, lens, starts, 64, 1024, 1.0)
+    check_rows(out, want, a, d, 256)
+    for m, s, t in pm.positions(starts, lens):
+        assert torch.equal(raw(st.k)[0, st.state.table[s][t // 64], t % 64], raw(k)[m])
