@@ -10,8 +10,8 @@
  * The cache is caller-owned device memory described by a moa_paged_cache (a host struct that the
  * caller keeps; a call reads it before it returns). Its state -- page table, lengths, reference
  * counts -- lives on the device, and every call that changes it runs there: nothing synchronises,
- * and the calls can be captured into a HIP graph (call moa_init before). The first call on a device allocates the paged calls'
- * scratch (98 MB), also while a stream is captured.
+ * and the calls can be captured into a HIP graph (call moa_init before). The first call on a device
+ * allocates the paged calls' scratch (98 MB), also while a stream is captured.
  *   - sequence s holds positions 0 .. seq_lens[s] - 1; position t lies in page
  *     page_table[s][t / slots] at slot t % slots. Table entries behind the last page in use are
  *     never read as pages.
@@ -104,12 +104,13 @@ int moa_paged_cache_compact(const moa_paged_cache* cache, void* stream);
  * query heads per KV head. max_rows: the most rows a sequence has in this call (it chooses the kernel
  * and its grid; rows itself is always right). Rows that belong to no sequence are left as they were.
  * A sequence whose rows or length are out of range, or that has more than max_rows rows, is left out; so
- * is at least every row that sees a page outside the pool, and row starts that descend may leave out all; rows that two sequences
- * claim by such starts get either's result (MOA_DEVERR_PAGED for each). The entries of positions before a window have to
- * name pages of the pool too: tiles begin up to 63 positions before it. The result is deterministic; how the positions are split, and with it the order of f32 sums,
- * follows the whole batch, so a row's last bits may differ between calls of other batches. Scores, maxima, sums and outputs are
- * f32; a weight enters the product with V as two bf16 numbers, which hold it to 2^-16 of itself, in every row of every call; the
- * result is rounded once. rows may be 0. */
+ * is at least every row that sees a page outside the pool, and row starts that descend may leave out all; rows
+ * that two sequences claim by such starts get either's result (MOA_DEVERR_PAGED for each). The entries of the
+ * positions before a window have to name pages of the pool too: tiles begin up to 63 positions before it.
+ * The result is deterministic; how the positions are split, and with it the order of f32 sums, follows the
+ * whole batch, so a row's last bits may differ between calls of other batches. Scores, maxima, sums and outputs
+ * are f32; a weight enters the product with V as two bf16 numbers, which hold it to 2^-16 of itself, in every row
+ * of every call; the result is rounded once. rows may be 0. */
 int moa_paged_attention(const uint16_t* q, int64_t q_row_stride, const moa_paged_cache* cache,
                         const int32_t* row_starts, uint16_t* out, int64_t out_row_stride, int rows, int q_heads,
                         int layer, int window, float scale, int max_rows, void* stream);

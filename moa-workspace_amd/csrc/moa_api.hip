@@ -296,7 +296,7 @@ int qkv_common(const QkvParams& p, int M, void* stream) {
     if (M <= kMaxDecodeM) return call_result(launch_qkv_decode(p, M, s, ctx), "sliding_project_qkv launch");
     for (int m0 = 0; m0 < M; m0 += kMaxChunkM) {
         const int e = call_result(launch_qkv_chunk(p, m0, M - m0 < kMaxChunkM ? M - m0 : kMaxChunkM, s, ctx),
-                             "sliding_project_qkv launch");
+                                  "sliding_project_qkv launch");
         if (e) return e;
     }
     return MOA_SUCCESS;
@@ -313,7 +313,7 @@ int o_launch(const OParams& p, int M, hipStream_t s, DevCtx* ctx) {
     if (M <= kMaxDecodeM) return call_result(launch_o_decode(p, M, s, ctx), "sliding_attention_output launch");
     for (int m0 = 0; m0 < M; m0 += kMaxChunkM) {
         const int e = call_result(launch_o_chunk(p, m0, M - m0 < kMaxChunkM ? M - m0 : kMaxChunkM, s, ctx),
-                             "sliding_attention_output launch");
+                                  "sliding_attention_output launch");
         if (e) return e;
     }
     return MOA_SUCCESS;
@@ -353,7 +353,7 @@ int ffn_launch(const FfnParams& p, int M, hipStream_t s, DevCtx* ctx) {
     if (M <= kMaxDecodeM) return call_result(launch_ffn_decode(p, M, s, ctx), "decoder_feedforward launch");
     for (int m0 = 0; m0 < M; m0 += kMaxChunkM) {
         const int e = call_result(launch_ffn_chunk(p, m0, M - m0 < kMaxChunkM ? M - m0 : kMaxChunkM, s, ctx),
-                             "decoder_feedforward launch");
+                                  "decoder_feedforward launch");
         if (e) return e;
     }
     return MOA_SUCCESS;
@@ -384,7 +384,7 @@ int o_ffn_common(const OParams& o, const FfnParams& p, int M, void* stream) {
     if (M > kMaxDecodeM) {  // the MFMA path: O's post rows write the FFN's normalised input too
         for (int m0 = 0; m0 < M; m0 += kMaxChunkM) {
             const int bad = call_result(launch_o_ffn_chunk(o, p, m0, M - m0 < kMaxChunkM ? M - m0 : kMaxChunkM, s, ctx),
-                                   "sliding_attention_output_feedforward launch");
+                                        "sliding_attention_output_feedforward launch");
             if (bad) return bad;
         }
         return MOA_SUCCESS;
@@ -594,7 +594,7 @@ int moa_sliding_attention(const uint16_t* q, const uint16_t* k, const uint16_t* 
     DevCtx* ctx = call_context(&code);
     if (!ctx) return code;
     return call_result(launch_sliding_attention(q, k, v, mask, out, M, static_cast<hipStream_t>(stream), ctx),
-                  "sliding_attention launch");
+                       "sliding_attention launch");
 }
 
 int moa_full_project_qkv(const uint16_t* x, const uint8_t* q_weight, const uint8_t* k_weight,
@@ -618,7 +618,7 @@ int moa_full_project_qkv(const uint16_t* x, const uint8_t* q_weight, const uint8
     if (M <= kMaxDecodeM) return call_result(launch_full_qkv(p, M, s, ctx), "full_project_qkv launch");
     for (int m0 = 0; m0 < M; m0 += kMaxFullQkvM) {
         const int e = call_result(launch_full_qkv_chunk(p, m0, M - m0 < kMaxFullQkvM ? M - m0 : kMaxFullQkvM, s, ctx),
-                             "full_project_qkv launch");
+                                  "full_project_qkv launch");
         if (e) return e;
     }
     return MOA_SUCCESS;
@@ -634,8 +634,8 @@ static int full_page(const uint16_t* q, const uint16_t* k, const uint16_t* v, co
     DevCtx* ctx = call_context(&code);
     if (!ctx) return code;
     return call_result(launch_full_attention_page(q, k, v, mask, running_max, running_sum, out, M, first,
-                                             static_cast<hipStream_t>(stream), ctx),
-                  first ? "full_attention_first_page launch" : "full_attention_page launch");
+                                                  static_cast<hipStream_t>(stream), ctx),
+                       first ? "full_attention_first_page launch" : "full_attention_page launch");
 }
 
 int moa_full_attention_first_page(const uint16_t* q, const uint16_t* k, const uint16_t* v, const float* mask,
@@ -659,8 +659,8 @@ int moa_full_attention(const uint16_t* q, const uint16_t* k_pages, const uint16_
     DevCtx* ctx = call_context(&code);
     if (!ctx) return code;
     return call_result(launch_full_attention(q, k_pages, v_pages, masks, P, running_max, running_sum, out, M,
-                                        static_cast<hipStream_t>(stream), ctx),
-                  "full_attention launch");
+                                             static_cast<hipStream_t>(stream), ctx),
+                       "full_attention launch");
 }
 
 int moa_full_attention_output(const uint16_t* x, const float* running_sum, const uint16_t* post_attn_rms_weight,
@@ -678,7 +678,7 @@ int moa_full_attention_output(const uint16_t* x, const float* running_sum, const
     if (M <= kMaxDecodeM) return call_result(launch_full_o(p, M, s, ctx), "full_attention_output launch");
     for (int m0 = 0; m0 < M; m0 += kMaxChunkM) {
         const int e = call_result(launch_o_chunk(p, m0, M - m0 < kMaxChunkM ? M - m0 : kMaxChunkM, s, ctx),
-                             "full_attention_output launch");
+                                  "full_attention_output launch");
         if (e) return e;
     }
     return MOA_SUCCESS;
@@ -691,7 +691,7 @@ int moa_final_norm_and_logits(const uint16_t* input, const uint16_t* rms_weight,
     if (c.code) return c.code;
     if (g_tripped[current_device_or_0()].load()) return tripped_fail(current_device_or_0());
     return call_result(launch_final_norm_and_logits(input, rms_weight, lm_head_weight, out, M, static_cast<hipStream_t>(stream)),
-                  "final_norm_and_logits launch");
+                       "final_norm_and_logits launch");
 }
 
 int moa_fp8_scaled_projection(const uint16_t* x, const uint8_t* w, const float* scale, uint16_t* out,
