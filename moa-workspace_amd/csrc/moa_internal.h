@@ -77,6 +77,8 @@ constexpr int kPagedMaxPages = 1 << 20;
 constexpr int kPagedMaxSequences = 1 << 16;
 constexpr size_t kPagedTokenFloats = (size_t)9 << 19;   // 18.9 MB
 constexpr size_t kPagedChunkFloats = (size_t)17 << 20;  // 71.3 MB
+constexpr int kTreeMaxWords = 4, kTreeMaxNodes = 64 * kTreeMaxWords;  // nodes of a drafted tree, one mask bit each
+constexpr int kMaxBeams = 64;                           // sequences of a beam search's group
 constexpr int kPagedTickets = 2048;                     // arrivals at split sequences (moa_paged_plan.h: kJoinTurn)
 
 // Device-side error bits (OR-ed by kernels; read back by moa_device_errors()).

@@ -58,6 +58,13 @@ struct PagedAttentionCall {
     float scale_log2;                     // scale * log2 e
 };
 
+// Rows that are nodes of trees: masks [rows][words], bit j % 64 of word j / 64 of a row: it sees node j of its sequence.
+struct PagedTreeCall : PagedAttentionCall {
+    const uint64_t* masks;
+    int words;
+};
+
 hipError_t launch_paged_attention(const PagedView& c, const PagedAttentionCall& a, hipStream_t s, DevCtx* ctx);
+hipError_t launch_paged_tree_attention(const PagedView& c, const PagedTreeCall& a, hipStream_t s, DevCtx* ctx);
 
 }  // namespace moa

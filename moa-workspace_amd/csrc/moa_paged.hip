@@ -4,9 +4,11 @@
 // State changes are planned by one workgroup that reads the lengths and the reference counts, checks the whole
 // call, and only then writes: that makes a call all or nothing and its result independent of any order between
 // workgroups. Pages are copied by a second launch over the plan's list of moves.
+#include <algorithm>
 #include <string>
 
 #include "../../include/moa_paged.h"
+#include "moa_checks.h"
 #include "moa_device.h"
 #include "moa_paged.h"
 
@@ -439,6 +441,276 @@ __global__ __launch_bounds__(kCopyBlock) void paged_compact_kernel(PagedView c, 
     copy_pages(c, src, dst, moves, elem, dense_k, dense_v, blockIdx.x, gridDim.x);
 }
 
+// ------------------------------------------------------------------------------------------- commit
+
+// A sequence's thread per node: the nodes that the accepted one sees, in order, become positions base, base + 1, ... of the
+// sequence, base the positions before the tree. The first of them may be there already (`still` of them); the others move:
+// nodes[s][m], the node of rank still + m. Then the state: the length, and the counts of the pages behind it, which are
+// the sequence's alone. A sequence that breaks a rule has no moves and keeps its state.
+struct Commit { int moves, base, still, unused; };
+
+__global__ __launch_bounds__(kTreeMaxNodes) void paged_commit_plan_kernel(PagedView c, const int32_t* starts, const uint64_t* masks, int words,
+                                                                          const int32_t* leaves, int rows, uint8_t* nodes, Commit* commits) {
+    const int s = blockIdx.x, i = threadIdx.x;
+    const int row0 = starts[s], end = starts[s + 1], len = c.lens[s], leaf = leaves[s];
+    if (i == 0) commits[s] = {0, 0, 0, 0};
+    if (row0 == end) return;
+    // (in this order: differences only of values that are in range)
+    if (!rows_in_range(row0, end, rows, 64 * words) || len < end - row0 || len > paged_capacity(c) || leaf < -1 || leaf >= end - row0) {
+        if (i == 0) raise(c);
+        return;
+    }
+    const int n = end - row0, base = len - n;
+    const int32_t* table = c.table + s * c.table_stride;
+    int rank = 0, kept = 0;
+    bool mine = false;
+    for (int w = 0; w < words && leaf >= 0; ++w) {
+        uint64_t m = masks[(int64_t)(row0 + leaf) * words + w];
+        const int left = n - 64 * w;
+        m &= left >= 64 ? ~0ull : (left > 0 ? (1ull << left) - 1 : 0);
+        kept += __popcll(m);
+        if (i >> 6 > w) rank += __popcll(m);
+        if (i >> 6 == w) rank += __popcll(m & ((1ull << (i & 63)) - 1)), mine = m >> (i & 63) & 1;
+    }
+    bool bad = false;
+    if (i < n) {
+        const int page = table[page_of(c, base + i)];
+        bad = page < 0 || page >= c.pages || c.refs[page] != 1;
+    }
+    if (__syncthreads_or(bad)) {
+        if (i == 0) raise(c);
+        return;
+    }
+    // (a rank is at most the node's number, and once below stays below)
+    const int still = __syncthreads_count(mine && rank == i);
+    if (mine && rank != i) nodes[s * kTreeMaxNodes + rank - still] = (uint8_t)i;
+    if (i == 0) {
+        commits[s] = {kept - still, base, still, 0};
+        c.lens[s] = base + kept;
+    }
+    for (int x = pages_of(c, base + kept) + i; x < pages_of(c, len); x += kTreeMaxNodes) c.refs[table[x]] = 0;
+}
+
+// Moves within a sequence go one after the other, eight at a time read before they are written: a target lies before its
+// source, and so before every later source. A unit of work is a sequence, a layer's K or V and 256 chunks of 16 bytes of a position.
+__host__ __device__ inline int commit_parts(const PagedView& c, int elem) {
+    return (c.kv_heads * c.head_dim * elem / 16 + kCopyBlock - 1) / kCopyBlock;
+}
+
+__global__ __launch_bounds__(kCopyBlock) void paged_commit_kernel(PagedView c, const uint8_t* nodes, const Commit* commits, int elem) {
+    static_assert(kCopyBlock == kTreeMaxNodes, "a thread per move");
+    __shared__ int4 moves[kTreeMaxNodes];  // source page and slot, target page and slot
+    const int parts = commit_parts(c, elem), per_head = c.head_dim * elem / 16, per = parts * 2 * c.layers;
+    const int64_t units = (int64_t)c.sequences * per;
+    for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
+        const int s = (int)(u / per), r = (int)(u - (int64_t)s * per), tensor = r / parts;
+        const int node = nodes[s * kTreeMaxNodes + threadIdx.x];
+        const Commit m = commits[s];
+        if (m.moves == 0) continue;
+        __syncthreads();  // the unit before has read its moves
+        if ((int)threadIdx.x < m.moves) {
+            const int32_t* table = c.table + s * c.table_stride;
+            const int from = m.base + node, to = m.base + m.still + (int)threadIdx.x;
+            const int fc = (int)page_of(c, from), tc = (int)page_of(c, to);
+            moves[threadIdx.x] = make_int4(table[fc], from - fc * (int)c.slots, table[tc], to - tc * (int)c.slots);
+        }
+        __syncthreads();
+        const int chunk = (r - tensor * parts) * kCopyBlock + (int)threadIdx.x;
+        if (chunk >= c.kv_heads * per_head) continue;
+        const bool v = tensor & 1;
+        const int h = chunk / per_head;
+        uint8_t* base = (v ? c.v + (int64_t)(tensor >> 1) * c.v_layer + h * c.v_head : c.k + (int64_t)(tensor >> 1) * c.k_layer + h * c.k_head) +
+                        (chunk - h * per_head) * 16;
+        const int64_t page = v ? c.v_page : c.k_page, slot = v ? c.v_slot : c.k_slot;
+        for (int m0 = 0; m0 < m.moves; m0 += 8) {
+            uint4 w[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int4 x = moves[min(m0 + j, m.moves - 1)];
+                w[j] = ld16(base + x.x * page + x.y * slot);
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int4 x = moves[min(m0 + j, m.moves - 1)];
+                if (m0 + j < m.moves) *reinterpret_cast<uint4*>(base + x.z * page + x.w * slot) = w[j];
+            }
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------ reorder
+
+// Scratch of a reorder, in the page lists: the lengths before it; of every sequence the copy of its parent's last page that it gets
+// (-1: none); source, target and slots in use of every copy; pages of dropped sequences and free ones behind the first kFew.
+struct ReorderLists {
+    int32_t *lens, *copy, *src, *dst, *used, *more, *result;
+    __device__ explicit ReorderLists(int32_t* list)
+        : lens(list), copy(list + kPagedMaxSequences), src(list + 2 * kPagedMaxSequences), dst(list + 3 * kPagedMaxSequences),
+          used(list + 4 * kPagedMaxSequences), more(list + 5 * kPagedMaxSequences), result(list + 2 * kPagedMaxPages) {}
+};
+static_assert(7 * kPagedMaxSequences < 2 * kPagedMaxPages, "a reorder's lists fit the page lists");
+
+// One workgroup, whole groups of beams at a time. A parent's partly filled last page stays with its keeper: the parent itself if it is its
+// own child, else its first child. Every other child gets a copy, in the order of the sequences: in the partly filled last pages of the
+// sequences that are nobody's parents, where those were theirs alone, then in the lowest free pages. result: the copies, or -1.
+struct Beam { int parent, len, parent_len, last; bool copies, dropped; };
+
+__global__ __launch_bounds__(kPlanBlock) void paged_reorder_plan_kernel(PagedView c, const int32_t* parents, int count, int beams, int32_t* list) {
+    __shared__ int lds[2 * kWave], few[kFew], par[kPlanBlock], len[kPlanBlock];
+    const ReorderLists l(list);
+    const PageList pages = {few, l.more};
+    const Counts first = counts_at(c, 0);
+    const int t = threadIdx.x, step = kPlanBlock / beams * beams;
+    // sequence base + t's part; the workgroup's lists are those of the step
+    auto beam_at = [&](int base, bool* bad) {
+        Beam b = {-1, 0, 0, -1, false, false};
+        const int s = base + t;
+        const bool in = t < step && s < count;
+        __syncthreads();  // the step before has read the lists
+        if (in) {
+            b.parent = parents[s];
+            b.len = c.lens[s];
+            const int g = s / beams * beams;
+            if (b.parent < g || b.parent >= g + beams || b.len < 0 || b.len > paged_capacity(c)) {
+                *bad = true;
+                b.parent = s;
+                b.len = 0;
+            }
+            par[t] = b.parent;
+            len[t] = b.len;
+        }
+        __syncthreads();
+        if (!in) return b;
+        const int g = t / beams * beams, p = b.parent - base;
+        bool chosen = false;
+        b.copies = b.parent != s && par[p] == b.parent;
+        for (int i = g; i < g + beams; ++i) {
+            chosen |= par[i] == s;
+            b.copies |= i < t && par[i] == b.parent && b.parent != s;
+        }
+        b.parent_len = len[p];
+        b.copies &= b.parent_len % (int)c.slots != 0;
+        b.dropped = !chosen && b.len % (int)c.slots != 0;
+        if (b.copies) {
+            b.last = c.table[b.parent * c.table_stride + b.parent_len / (int)c.slots];
+            *bad |= b.last < 0 || b.last >= c.pages;
+        }
+        return b;
+    };
+    bool bad = false;
+    int copies = 0, dropped = 0;
+    for (int base = 0; base < count; base += step) {
+        const Beam b = beam_at(base, &bad);
+        int page = -1, all = 0;
+        if (b.dropped) {
+            page = c.table[(base + t) * c.table_stride + b.len / (int)c.slots];
+            if (page < 0 || page >= c.pages || c.refs[page] != 1) page = -1;
+        }
+        const int at = dropped + block_before(page >= 0, lds, &all);
+        if (page >= 0) pages.put(at, page);
+        dropped += all;
+        (void)block_before(b.copies, lds, &all);
+        copies += all;
+        if (t < step && base + t < count) l.lens[base + t] = b.len;
+    }
+    bad = __syncthreads_or(bad);
+    const int more = copies - dropped;
+    if (bad || (more > 0 && each_page(c, first, 0, c.pages, true, more, lds, [&](int p, int rank, int) { pages.put(dropped + rank, p); }) < more)) {
+        if (t == 0) {
+            *l.result = -1;
+            raise(c);
+        }
+        return;
+    }
+    int given = 0;
+    for (int base = 0; base < count; base += step) {
+        const Beam b = beam_at(base, &bad);
+        int all = 0;
+        const int at = given + block_before(b.copies, lds, &all);
+        if (t < step && base + t < count) {
+            const int p = b.copies ? pages.get(at) : -1;
+            l.copy[base + t] = p;
+            if (b.copies) {
+                l.src[at] = b.last;
+                l.dst[at] = p;
+                l.used[at] = b.parent_len % (int)c.slots;
+            }
+            if (b.parent != base + t) c.lens[base + t] = b.parent_len;  // (the step's lengths have been read)
+        }
+        given += all;
+    }
+    if (t == 0) *l.result = copies;
+}
+
+constexpr int kReorderColumns = 64;
+
+// A workgroup takes 64 columns of a group's table rows, all of them read before any is written; a page's count follows the entries that
+// name it. All workgroups copy the slots in use of the pages that are copied.
+__global__ __launch_bounds__(kCopyBlock) void paged_reorder_kernel(PagedView c, const int32_t* parents, int count, int beams, int32_t* list, int elem) {
+    __shared__ int32_t entry[kMaxBeams][kReorderColumns];
+    __shared__ int par[kMaxBeams], len[kMaxBeams];
+    const ReorderLists l(list);
+    const int copies = *l.result;
+    if (copies < 0) return;
+    const int slices = (c.columns + kReorderColumns - 1) / kReorderColumns, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t tables = (int64_t)(count / beams) * slices;
+    for (int64_t u = blockIdx.x; u < tables; u += gridDim.x) {
+        const int g = (int)(u / slices) * beams, i = (int)(u % slices) * kReorderColumns + lane;
+        __syncthreads();
+        bool moves = false;
+        if ((int)threadIdx.x < beams) {
+            par[threadIdx.x] = parents[g + threadIdx.x] - g;
+            len[threadIdx.x] = l.lens[g + threadIdx.x];
+            moves = par[threadIdx.x] != (int)threadIdx.x;
+        }
+        if (!__syncthreads_or(moves)) continue;
+        for (int b = wave; b < beams; b += 4)
+            entry[b][lane] = i < pages_of(c, len[b]) ? c.table[(g + b) * c.table_stride + i] : -1;
+        __syncthreads();
+        for (int b = wave; b < beams; b += 4) {
+            const int p = par[b];
+            if (p == b) continue;
+            const int had = pages_of(c, len[b]), has = pages_of(c, len[p]), copy = l.copy[g + b];
+            const int old = entry[b][lane], now = copy >= 0 && i == has - 1 ? copy : entry[p][lane];
+            if (i < has) c.table[(g + b) * c.table_stride + i] = now;
+            if (i < had && i < has && old == now) continue;
+            if (i < has) {
+                if (now < 0 || now >= c.pages) raise(c);
+                else atomicAdd(c.refs + now, 1);
+            }
+            if (i < had) {
+                if (old < 0 || old >= c.pages) raise(c);
+                else if (atomicSub(c.refs + old, 1) <= 0) {  // the count was wrong: a free page stays at 0
+                    atomicAdd(c.refs + old, 1);
+                    raise(c);
+                }
+            }
+        }
+    }
+    const uint32_t per_row = (uint32_t)(c.head_dim * elem / 16), chunks = c.slots * (uint32_t)c.kv_heads * per_row;
+    const uint32_t parts = (chunks + kCopyBytes / 16 - 1) / (kCopyBytes / 16);
+    const uint64_t per_move = (uint64_t)parts * 2 * c.layers;
+    for (uint64_t u = blockIdx.x; u < per_move * copies; u += gridDim.x) {
+        const int m = (int)(u / per_move);
+        const uint32_t r = (uint32_t)(u - m * per_move), tensor = r / parts, i0 = (r - tensor * parts) * (kCopyBytes / 16) + threadIdx.x;
+        const uint32_t used = l.used[m] * (uint32_t)c.kv_heads * per_row;
+        const bool v = tensor & 1;
+        uint8_t* base = v ? c.v + (int64_t)(tensor >> 1) * c.v_layer : c.k + (int64_t)(tensor >> 1) * c.k_layer;
+        const int64_t page = v ? c.v_page : c.k_page, slot = v ? c.v_slot : c.k_slot, head = v ? c.v_head : c.k_head;
+        const uint8_t* a = base + l.src[m] * page;
+        uint8_t* b = base + l.dst[m] * page;
+        const bool dense = head == c.head_dim * elem && slot == (int64_t)c.kv_heads * head;
+        uint4 w[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (i0 + j * kCopyBlock < used) w[j] = ld16(a + chunk_at(dense, i0 + j * kCopyBlock, per_row, c.kv_heads, slot, head));
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (i0 + j * kCopyBlock < used)
+                *reinterpret_cast<uint4*>(b + chunk_at(dense, i0 + j * kCopyBlock, per_row, c.kv_heads, slot, head)) = w[j];
+    }
+}
+
 // -------------------------------------------------------------------------------------------- append
 
 // One wave per row: it finds the row's sequence, then moves K and V, 8 elements a lane and step. Bound by memory: 10500
@@ -493,20 +765,6 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedView c, const ui
 }
 
 // ------------------------------------------------------------------------------------ host: the checks
-
-int bad_value(const std::string& msg) { return set_error(MOA_ERROR_INVALID_VALUE, msg.c_str()); }
-
-int check_ptr(const void* p, const char* name, size_t align) {
-    if (!p) return bad_value(std::string(name) + " is NULL");
-    if (reinterpret_cast<uintptr_t>(p) % align)
-        return set_error(MOA_ERROR_MISALIGNED, (std::string(name) + " is not " + std::to_string(align) + "-byte aligned").c_str());
-    return MOA_SUCCESS;
-}
-
-int check_range(int v, int lo, int hi, const char* name) {
-    if (v >= lo && v <= hi) return MOA_SUCCESS;
-    return bad_value(std::string(name) + " must be in [" + std::to_string(lo) + ", " + std::to_string(hi) + "], got " + std::to_string(v));
-}
 
 int elem_bytes(const moa_paged_cache* c) { return c->element == MOA_PAGES_BF16 ? 2 : 1; }
 
@@ -591,6 +849,27 @@ int64_t copy_units(const moa_paged_cache* c, int64_t moves) {
 int copy_grid(int64_t units, int cus) {
     const int64_t most = (int64_t)cus * 8;
     return (int)(units < 1 ? 1 : (units < most ? units : most));
+}
+
+// The checks of both attention calls; of a call without rows only those of its numbers.
+int check_attention(const uint16_t* q, int64_t q_row_stride, const moa_paged_cache* cache, const int32_t* row_starts, const uint16_t* out,
+                    int64_t out_row_stride, int rows, int q_heads, int layer, int window, float scale, int max_rows, PagedView* v) {
+    int e;
+    if ((e = cache_view(cache, layer, v)) || (e = check_range(rows, 0, 1 << 20, "rows")) ||
+        (e = check_range(q_heads, 1, 1 << 15, "q_heads")) || (e = check_range(window, 0, 1 << 30, "window")))
+        return e;
+    if (q_heads % v->kv_heads || q_heads / v->kv_heads > 128)
+        return bad_value("q_heads must be kv_heads times 1 .. 128, got " + std::to_string(q_heads) + " and " + std::to_string(v->kv_heads));
+    if (!(scale > -1e30f && scale < 1e30f)) return bad_value("scale must be finite and below 1e30");
+    if (rows == 0) return MOA_SUCCESS;
+    if ((e = check_range(max_rows, 1, rows, "max_rows")) || (e = check_ptr(q, "q", 16)) || (e = check_ptr(out, "out", 16)) ||
+        (e = check_ptr(row_starts, "row_starts", 4)))
+        return e;
+    const int64_t width = (int64_t)q_heads * v->head_dim;
+    for (const int64_t st : {q_row_stride, out_row_stride})
+        if (rows > 1 && (st < width || st % 8 || st > (int64_t(1) << 40)))
+            return bad_value("q and out row strides must be multiples of 8 elements and at least q_heads * head_dim, got " + std::to_string(st));
+    return MOA_SUCCESS;
 }
 
 }  // namespace
@@ -691,26 +970,83 @@ int moa_paged_attention(const uint16_t* q, int64_t q_row_stride, const moa_paged
                         int max_rows, void* stream) {
     PagedView v;
     int e;
-    if ((e = cache_view(cache, layer, &v)) || (e = check_range(rows, 0, 1 << 20, "rows")) ||
-        (e = check_range(q_heads, 1, 1 << 15, "q_heads")) || (e = check_range(window, 0, 1 << 30, "window")))
+    if ((e = check_attention(q, q_row_stride, cache, row_starts, out, out_row_stride, rows, q_heads, layer, window, scale, max_rows, &v)))
         return e;
-    if (q_heads % v.kv_heads || q_heads / v.kv_heads > 128)
-        return bad_value("q_heads must be kv_heads times 1 .. 128, got " + std::to_string(q_heads) + " and " + std::to_string(v.kv_heads));
-    if (!(scale > -1e30f && scale < 1e30f)) return bad_value("scale must be finite and below 1e30");
     if (rows == 0) return MOA_SUCCESS;
-    if ((e = check_range(max_rows, 1, rows, "max_rows")) || (e = check_ptr(q, "q", 16)) || (e = check_ptr(out, "out", 16)) ||
-        (e = check_ptr(row_starts, "row_starts", 4)))
-        return e;
-    const int64_t width = (int64_t)q_heads * v.head_dim;
-    for (const int64_t st : {q_row_stride, out_row_stride})
-        if (rows > 1 && (st < width || st % 8 || st > (int64_t(1) << 40)))
-            return bad_value("q and out row strides must be multiples of 8 elements and at least q_heads * head_dim, got " + std::to_string(st));
     DevCtx* ctx = paged_context(&e);
     if (!ctx) return e;
     v.err = ctx->err;
     const PagedAttentionCall a{q, out, q_row_stride, out_row_stride, row_starts, rows, q_heads, q_heads / v.kv_heads,
                                window, max_rows, scale * 1.4426950408889634f};
     return call_result(launch_paged_attention(v, a, static_cast<hipStream_t>(stream), ctx), "paged_attention launch");
+}
+
+int moa_paged_tree_attention(const uint16_t* q, int64_t q_row_stride, const moa_paged_cache* cache, const int32_t* row_starts,
+                             const uint64_t* masks, int mask_words, uint16_t* out, int64_t out_row_stride, int rows, int q_heads,
+                             int layer, int window, float scale, int max_rows, void* stream) {
+    PagedView v;
+    int e;
+    if ((e = check_attention(q, q_row_stride, cache, row_starts, out, out_row_stride, rows, q_heads, layer, window, scale, max_rows, &v)) ||
+        (e = check_range(mask_words, 1, kTreeMaxWords, "mask_words")))
+        return e;
+    if (rows == 0) return MOA_SUCCESS;
+    if ((e = check_ptr(masks, "masks", 8)) || (e = check_range(max_rows, 1, 64 * mask_words, "max_rows"))) return e;
+    if (window && window < max_rows)
+        return bad_value("window must be 0 or at least max_rows, got " + std::to_string(window) + " and " + std::to_string(max_rows));
+    DevCtx* ctx = paged_context(&e);
+    if (!ctx) return e;
+    v.err = ctx->err;
+    PagedTreeCall a;
+    static_cast<PagedAttentionCall&>(a) = {q, out, q_row_stride, out_row_stride, row_starts, rows, q_heads, q_heads / v.kv_heads,
+                                           window, max_rows, scale * 1.4426950408889634f};
+    a.masks = masks, a.words = mask_words;
+    return call_result(launch_paged_tree_attention(v, a, static_cast<hipStream_t>(stream), ctx), "paged_tree_attention launch");
+}
+
+int moa_paged_tree_commit(const moa_paged_cache* cache, const int32_t* row_starts, const uint64_t* masks, int mask_words,
+                          const int32_t* leaves, int rows, void* stream) {
+    PagedView v;
+    int e;
+    if ((e = cache_view(cache, 0, &v)) || (e = check_range(rows, 0, 1 << 20, "rows")) ||
+        (e = check_range(mask_words, 1, kTreeMaxWords, "mask_words")))
+        return e;
+    if (rows == 0) return MOA_SUCCESS;
+    if ((e = check_ptr(row_starts, "row_starts", 4)) || (e = check_ptr(masks, "masks", 8)) || (e = check_ptr(leaves, "leaves", 4)))
+        return e;
+    DevCtx* ctx = paged_context(&e);
+    if (!ctx) return e;
+    v.err = ctx->err;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    uint8_t* nodes = reinterpret_cast<uint8_t*>(ctx->paged_chunks);
+    Commit* commits = reinterpret_cast<Commit*>(ctx->paged_list);
+    hipLaunchKernelGGL(paged_commit_plan_kernel, dim3(v.sequences), dim3(kTreeMaxNodes), 0, s, v, row_starts, masks, mask_words, leaves,
+                       rows, nodes, commits);
+    if ((e = call_result(hipGetLastError(), "paged_tree_commit launch"))) return e;
+    const int64_t units = (int64_t)v.sequences * v.layers * 2 * commit_parts(v, elem_bytes(cache));
+    hipLaunchKernelGGL(paged_commit_kernel, dim3(copy_grid(units, ctx->cus)), dim3(kCopyBlock), 0, s, v, nodes, commits, elem_bytes(cache));
+    return call_result(hipGetLastError(), "paged_tree_commit launch");
+}
+
+int moa_paged_cache_reorder(const moa_paged_cache* cache, const int32_t* parents, int count, int beams, void* stream) {
+    PagedView v;
+    int e;
+    if ((e = cache_view(cache, 0, &v)) || (e = check_range(count, 0, v.sequences, "count")) ||
+        (e = check_range(beams, 1, kMaxBeams, "beams")))
+        return e;
+    if (count % beams) return bad_value("count must be a multiple of beams, got " + std::to_string(count) + " and " + std::to_string(beams));
+    if (count == 0) return MOA_SUCCESS;
+    if ((e = check_ptr(parents, "parents", 4))) return e;
+    DevCtx* ctx = paged_context(&e);
+    if (!ctx) return e;
+    v.err = ctx->err;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    hipLaunchKernelGGL(paged_reorder_plan_kernel, dim3(1), dim3(kPlanBlock), 0, s, v, parents, count, beams, ctx->paged_list);
+    if ((e = call_result(hipGetLastError(), "paged_cache_reorder launch"))) return e;
+    // at least one sequence of a group keeps its pages
+    const int64_t copies = copy_units(cache, count - count / beams), tables = (int64_t)(count / beams) * ((v.columns + kReorderColumns - 1) / kReorderColumns);
+    hipLaunchKernelGGL(paged_reorder_kernel, dim3(copy_grid(std::max(copies, tables), ctx->cus)), dim3(kCopyBlock), 0, s, v, parents, count,
+                       beams, ctx->paged_list, elem_bytes(cache));
+    return call_result(hipGetLastError(), "paged_cache_reorder launch");
 }
 
 }  // extern "C"

@@ -36,6 +36,11 @@ __device__ __forceinline__ void split_weights(float p0, float p1, uint32_t (&w)[
     w[1] = pk_bf16(p0 - __uint_as_float(w[0] << 16), p1 - __uint_as_float(w[0] & 0xffff0000u));
 }
 
+// Rows that are nodes of trees see the positions before the tree and the nodes of their masks, in any order: their call's type
+// chooses the rules below at compile time.
+template <class A>
+constexpr bool kTree = std::is_same_v<A, PagedTreeCall>;
+
 // ------------------------------------------------------------------------------------ who does what
 
 // A sequence that takes part: its first row of the call, new rows and length. n = 0: it does not, or is bad.
@@ -91,7 +96,8 @@ struct TokenWalk {
     int64_t before;             // units before them
 };
 
-// First position and units of a sequence's span: from a multiple of `align` on, at least one unit.
+// First position and units of a sequence's span: from a multiple of `align` on, at least one unit. (A tree's first node stands where
+// the first token of consecutive ones does, and no node's window begins before its.)
 __device__ __forceinline__ int token_first(const PagedAttentionCall& a, const Seq& q, int align) {
     const int p0 = q.len - q.n;
     return a.window && p0 >= a.window ? (p0 - a.window + 1) / align * align : 0;
@@ -191,14 +197,16 @@ struct ChunkWalk {
 
 // Tiles of a sequence, and the units that a tile's rows see: all, or the window and the tile's tokens.
 __device__ __forceinline__ int chunk_tiles(const PagedAttentionCall& a, const Seq& q) { return (q.n * a.group + kChunkRows - 1) / kChunkRows; }
-__device__ __forceinline__ int chunk_units(const PagedAttentionCall& a, const Seq& q) {
-    const int span = min(q.n, (kChunkRows + a.group - 1) / a.group + 1);
+template <class A>
+__device__ __forceinline__ int chunk_units(const A& a, const Seq& q) {
+    const int span = kTree<A> ? q.n : min(q.n, (kChunkRows + a.group - 1) / a.group + 1);
     const int seen = a.window ? min(q.len, a.window + span - 1 + kChunkUnit) : q.len;
     return max(1, (seen + kChunkUnit - 1) / kChunkUnit);
 }
 
 // last: the last 64 sequences' lanes, the only ones of most calls.
-__device__ ChunkWalk chunk_walk(const PagedView& c, const PagedAttentionCall& a, const ChunkPlan& p, Seq* last) {
+template <class A>
+__device__ ChunkWalk chunk_walk(const PagedView& c, const A& a, const ChunkPlan& p, Seq* last) {
     int tiles = 0;
     float units = 0.0f;
     bool bad = false;
@@ -220,7 +228,8 @@ __device__ ChunkWalk chunk_walk(const PagedView& c, const PagedAttentionCall& a,
 }
 
 // Piece `want`, not before an earlier call's. False: there are not that many. have: the only 64 sequences' lanes, or nullptr.
-__device__ __forceinline__ bool find_piece(const PagedView& c, const PagedAttentionCall& a, ChunkWalk& w, int merge_rows, int want, const Seq* have,
+template <class A>
+__device__ __forceinline__ bool find_piece(const PagedView& c, const A& a, ChunkWalk& w, int merge_rows, int want, const Seq* have,
                                            Piece* out) {
     const int lane = threadIdx.x & 63;
     bool bad = false;
@@ -261,13 +270,62 @@ __device__ __forceinline__ bool find_piece(const PagedView& c, const PagedAttent
 // outside the pool has NaN maxima: its rows are not written.
 __host__ __device__ inline int64_t record_floats(int bm, int dim) { return (int64_t)bm * (2 + dim); }
 
+// Row r of a sequence: where it lies in the call, and the positions it sees (of a tree's, those before the tree).
+struct Row {
+    int64_t m;      // row of the call
+    int h, lo, hi;  // query head; positions [lo, hi)
+};
+
+// Trees: bit k of the result says whether row m of the call sees position t0 + k as a node (t0 + 63 not before the tree).
+__device__ __forceinline__ uint64_t node_bits(const PagedTreeCall& a, const Piece& t, int64_t m, int t0) {
+    const uint64_t* w = a.masks + m * a.words;
+    const int at = t0 - (t.len - t.n), left = t.n - at;  // the first position's node (may be negative); nodes from it on
+    if (left <= 0) return 0;
+    uint64_t bits;
+    if (at < 0) {
+        bits = w[0] << -at;
+    } else {
+        const int i = at >> 6, r = at & 63;  // at < n <= 64 words
+        bits = w[i] >> r;
+        if (r && i + 1 < a.words) bits |= w[i + 1] << (64 - r);
+    }
+    return left >= 64 ? bits : bits & ((1ull << left) - 1);
+}
+
+// A node's depth in its tree, itself included: the nodes it sees.
+__device__ __forceinline__ int node_depth(const PagedTreeCall& a, const Piece& t, int64_t m) {
+    int d = 0;
+    for (int i = 0; i < a.words; ++i) {
+        const int left = t.n - 64 * i;
+        if (left > 0) d += __popcll(a.masks[m * a.words + i] & (left >= 64 ? ~0ull : (1ull << left) - 1));
+    }
+    return d;
+}
+
+template <class A>
+__device__ __forceinline__ Row row_of(const A& a, const Piece& t, int kvh, int r) {
+    Row x;
+    const int i = r / a.group;
+    x.m = t.row0 + i;
+    x.h = kvh * a.group + (r - i * a.group);
+    int p = t.len - t.n + i;
+    x.hi = p + 1;
+    if constexpr (kTree<A>) {
+        const int depth = node_depth(a, t, x.m), base = t.len - t.n;
+        p = base + depth - 1;
+        x.hi = depth ? max(base, 0) : 0;
+    }
+    x.lo = a.window && p >= a.window ? p - a.window + 1 : 0;
+    return x;
+}
+
 // One row by one wave over positions [lo, hi), nothing outside them used: 64 positions at a time, a lane each for the
 // scores; then lane l holds dims l * dim / 64 .. and takes the weights in turn. The kernels fall back to it where a value that
 // their rows do not all see is infinite or NaN (zero times that is NaN). Pages are in range here.
-template <bool E4M3>
-__device__ void careful_row(const PagedView& c, const uint16_t* q, int s, int kvh, float factor, int lo, int hi, float* mx_out,
-                            float* sum_out, float (&o)[8]) {
-    const int lane = threadIdx.x & 63, d = c.head_dim, per = d / 64;
+template <bool E4M3, class A>
+__device__ void careful_row(const PagedView& c, const A& a, const Piece& piece, const Row& row, const uint16_t* q, int kvh, float factor, int lo, int hi,
+                            float* mx_out, float* sum_out, float (&o)[8]) {
+    const int lane = threadIdx.x & 63, d = c.head_dim, per = d / 64, s = piece.s;
     float mx = -INFINITY, sum = 0.0f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) o[i] = 0.0f;
@@ -290,18 +348,25 @@ __device__ void careful_row(const PagedView& c, const uint16_t* q, int s, int kv
 #pragma unroll
             for (int k = 0; k < 8; ++k) x = fmaf(e[k], f[k], x);
         }
-        x = t0 + lane < hi ? x * factor : -INFINITY;
+        uint64_t seen = 0;  // trees: which of the 64 the row sees
+        bool sees = t0 + lane < hi;
+        if constexpr (kTree<A>) {
+            sees = sees && (t < row.hi || (t0 + 63 >= piece.len - piece.n && (node_bits(a, piece, row.m, t0) >> lane & 1)));
+            seen = __ballot(sees);
+        }
+        x = sees ? x * factor : -INFINITY;
         float mn = x;
 #pragma unroll
         for (int w = 32; w > 0; w >>= 1) mn = fmaxf(mn, __shfl_xor(mn, w, kWave));
         mn = fmaxf(mn, mx);
         const float f = mx == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mx - mn);
-        const float w = t0 + lane < hi ? __builtin_amdgcn_exp2f(x - mn) : 0.0f;
+        const float w = sees ? __builtin_amdgcn_exp2f(x - mn) : 0.0f;
         mx = mn;
         sum = fmaf(sum, f, wave_sum(w));
 #pragma unroll
         for (int k = 0; k < 8; ++k) o[k] *= f;
         for (int j = 0; j < min(64, hi - t0); ++j) {
+            if (kTree<A> && !(seen >> j & 1)) continue;
             const float wj = __shfl(w, j, kWave);
             const uint8_t* vp = c.v + __shfl(page, j, kWave) * c.v_page + __shfl(slot, j, kWave) * c.v_slot + kvh * c.v_head;
 #pragma unroll
@@ -314,27 +379,13 @@ __device__ void careful_row(const PagedView& c, const uint16_t* q, int s, int kv
     *sum_out = sum;
 }
 
-// Row r of a sequence: where it lies in the call, and the positions it sees.
-struct Row {
-    int64_t m;      // row of the call
-    int h, lo, hi;  // query head; positions [lo, hi)
-};
-__device__ __forceinline__ Row row_of(const PagedAttentionCall& a, const Piece& t, int kvh, int r) {
-    Row x;
-    const int i = r / a.group, p = t.len - t.n + i;
-    x.m = t.row0 + i;
-    x.h = kvh * a.group + (r - i * a.group);
-    x.hi = p + 1;
-    x.lo = a.window && p >= a.window ? p - a.window + 1 : 0;
-    return x;
-}
-
 // The positions [lo, hi) of a tile's split: what rows r0 .. r1 of its sequence see, from a multiple of `align` on, in even
 // parts of whole units.
 struct Span { int lo, hi; };
-__device__ __forceinline__ Span span_of(const PagedAttentionCall& a, const Piece& t, int r0, int r1, int align) {
+template <class A>
+__device__ __forceinline__ Span span_of(const A& a, const Piece& t, int r0, int r1, int align) {
     constexpr int unit = kChunkUnit;
-    const int p0 = t.len - t.n + r0 / a.group, p1 = t.len - t.n + r1 / a.group;
+    const int p0 = t.len - t.n + (kTree<A> ? 0 : r0 / a.group), p1 = kTree<A> ? t.len - 1 : t.len - t.n + r1 / a.group;
     const int lo = a.window && p0 >= a.window ? (p0 - a.window + 1) / align * align : 0, hi = max(p1 + 1, lo);
     const int units = (hi - lo + unit - 1) / unit, per = (units + t.splits - 1) / t.splits;
     const int64_t from = (int64_t)t.split * per * unit, to = from + (int64_t)per * unit;
@@ -343,15 +394,15 @@ __device__ __forceinline__ Span span_of(const PagedAttentionCall& a, const Piece
 
 // The careful path for a piece's rows [r0, r0 + nr) over positions [lo, hi), waves taking rows in turn. q(r, row): where row
 // r0 + r's query lies, not in `out` once that is written (out may be q).
-template <bool E4M3, class Q>
-__device__ void careful_piece(const PagedView& c, const PagedAttentionCall& a, const Piece& t, int kvh, int r0, int nr, int lo, int hi, Q q,
+template <bool E4M3, class Q, class A>
+__device__ void careful_piece(const PagedView& c, const A& a, const Piece& t, int kvh, int r0, int nr, int lo, int hi, Q q,
                               float* rec, int bm) {
     const int lane = threadIdx.x & 63, per = c.head_dim / 64;
     for (int r = threadIdx.x >> 6; r < nr; r += blockDim.x >> 6) {
         const Row x = row_of(a, t, kvh, r0 + r);
         float o[8], mx, sum;
-        careful_row<E4M3>(c, q(r, x), t.s, kvh, E4M3 ? c.k_scale[kvh] * a.scale_log2 : a.scale_log2,
-                          max(lo, x.lo), min(hi, x.hi), &mx, &sum, o);
+        careful_row<E4M3>(c, a, t, x, q(r, x), kvh, E4M3 ? c.k_scale[kvh] * a.scale_log2 : a.scale_log2,
+                          max(lo, x.lo), kTree<A> ? hi : min(hi, x.hi), &mx, &sum, o);
         if (rec) {
             if (lane == 0) rec[r] = mx, rec[bm + r] = sum;
             for (int k = 0; k < per; ++k) rec[2 * bm + (int64_t)r * c.head_dim + lane * per + k] = o[k];
@@ -419,8 +470,8 @@ constexpr int kJoinUnits = 16;
 static_assert(kJoinUnits < (int)kJoinTurn, "a sequence's parts are fewer than a turn of its counter");
 constexpr int kJoinElements = 1024;
 
-template <int D, bool E4M3>
-__device__ __forceinline__ void join_records(const PagedView& c, const PagedAttentionCall& a, const Piece& t, int kvh, const float* base, int splits) {
+template <int D, bool E4M3, class A>
+__device__ __forceinline__ void join_records(const PagedView& c, const A& a, const Piece& t, int kvh, const float* base, int splits) {
     constexpr int kAhead = 8, kSize = kTokenRows * (2 + D) * 4;
     const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(base), 0, (uint32_t)(2 * splits * kSize), 0x00020000);
     const float vs = E4M3 ? c.v_scale[kvh] : 1.0f;
@@ -460,8 +511,8 @@ __device__ __forceinline__ void join_records(const PagedView& c, const PagedAtte
 }
 
 // kJoin: the workgroups join their records (tickets [kv_heads][groups], multiples of kJoinTurn); else the merge kernel does.
-template <int D, bool E4M3, bool kJoin = false>
-__device__ __forceinline__ void token_part(const PagedView& c, const PagedAttentionCall& a, float* part, int kvh, int group, int groups,
+template <int D, bool E4M3, bool kJoin = false, class A>
+__device__ __forceinline__ void token_part(const PagedView& c, const A& a, float* part, int kvh, int group, int groups,
                                            uint8_t* lds, uint32_t* tickets = nullptr) {
     using T = TokenShape<D, E4M3>;
     constexpr int NT = T::kSub;
@@ -575,13 +626,19 @@ __device__ __forceinline__ void token_part(const PagedView& c, const PagedAttent
             if (t0 + kStep < hi) load_k();
 
             // weights of row l16 at positions t0 + 16 i + 4 g + e
+            uint32_t nodes = 0;
+            if constexpr (kTree<A>) {
+                if (t0 + T::kTile > t.len - t.n && l16 < nr) nodes = (uint32_t)node_bits(a, t, mine.m, t0);
+            }
             float x[NT][4], mx = -INFINITY;
 #pragma unroll
             for (int i = 0; i < NT; ++i)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int p = t0 + 16 * i + 4 * g + e;
-                    x[i][e] = p >= see_lo && p < see_hi ? sc[i][e] * factor : -INFINITY;
+                    bool sees = p >= see_lo && p < see_hi;
+                    if constexpr (kTree<A>) sees = sees || (nodes >> (16 * i + 4 * g + e) & 1);
+                    x[i][e] = sees ? sc[i][e] * factor : -INFINITY;
                     mx = fmaxf(mx, x[i][e]);
                 }
             mx = fmaxf(mx, __shfl_xor(mx, 16));
@@ -711,9 +768,9 @@ __device__ __forceinline__ void token_part(const PagedView& c, const PagedAttent
     }
 }
 
-template <int D, bool E4M3, bool kJoin>
+template <int D, bool E4M3, bool kJoin, class A>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(TokenShape<D, E4M3>::kHeld))) void paged_token_kernel(
-    PagedView c, PagedAttentionCall a, float* part, uint32_t* tickets) {
+    PagedView c, A a, float* part, uint32_t* tickets) {
     __shared__ __attribute__((aligned(16))) uint8_t lds[TokenShape<D, E4M3>::kLds];
     const int groups = gridDim.x / c.kv_heads;
     int kvh = blockIdx.x % c.kv_heads, group = blockIdx.x / c.kv_heads;
@@ -797,8 +854,8 @@ __device__ __forceinline__ int lane_here() {
 }
 
 // Items first, first + stride, ... of KV head kvh. lds: T::kLds bytes at a multiple of 1024.
-template <int D, bool E4M3>
-__device__ __forceinline__ void chunk_part(const PagedView& c, const PagedAttentionCall& a, const ChunkPlan& plan, float* part, int kvh, int first,
+template <int D, bool E4M3, class A>
+__device__ __forceinline__ void chunk_part(const PagedView& c, const A& a, const ChunkPlan& plan, float* part, int kvh, int first,
                                            int stride, uint8_t* lds_base) {
     using T = ChunkShape<D, E4M3>;
     constexpr int kTile = T::kTile, kPair = T::kPair, kWaves = 4 * kPair, kMine = D / kPair;  // dims of a wave
@@ -852,6 +909,7 @@ __device__ __forceinline__ void chunk_part(const PagedView& c, const PagedAttent
         }
         all_lo = __builtin_amdgcn_readfirstlane(all_lo), all_hi = __builtin_amdgcn_readfirstlane(all_hi);
         any_lo = __builtin_amdgcn_readfirstlane(any_lo), any_hi = __builtin_amdgcn_readfirstlane(any_hi);
+        if constexpr (kTree<A>) any_hi = t.len;
         if (32 * rg >= nr) any_hi = 0;  // no rows
 
         uint4 qf[kSteps];
@@ -941,6 +999,13 @@ __device__ __forceinline__ void chunk_part(const PagedView& c, const PagedAttent
             __builtin_amdgcn_s_barrier();
             __asm__ volatile("" ::: "memory");
         };
+        // trees: the nodes among the tile's positions that the lane's row sees
+        auto nodes_seen = [&](int t0) __attribute__((always_inline)) -> uint64_t {
+            if constexpr (kTree<A>) {
+                if (t0 + kTile > t.len - t.n && wrow < nr) return node_bits(a, t, mine.m, t0);
+            }
+            return 0;
+        };
         auto compute = [&](uint32_t tile, int t0) __attribute__((always_inline)) {  // tile: the buffer's place in `tiles`
             const bool sees = t0 < any_hi && t0 + kTile > any_lo;
             if (kPair == 1 && !sees) return;
@@ -975,12 +1040,15 @@ __device__ __forceinline__ void chunk_part(const PagedView& c, const PagedAttent
             if constexpr (kPair == 1) {
                 if (t0 < all_lo || t0 + kTile > all_hi) {  // some row does not see all of it
                     const int from = in_loop(see_lo - t0 - 4 * hf), to = in_loop(see_hi - t0 - 4 * hf);
+                    const uint64_t nodes = nodes_seen(t0) >> (4 * hf);
 #pragma unroll
                     for (int b = 0; b < T::kSub; ++b)
 #pragma unroll
                         for (int e = 0; e < 16; ++e) {
                             const int p = 32 * b + 8 * (e >> 2) + (e & 3);
-                            sc[b][e] = p >= from && p < to ? sc[b][e] : -INFINITY;
+                            bool sees = p >= from && p < to;
+                            if constexpr (kTree<A>) sees = sees || (nodes >> p & 1);
+                            sc[b][e] = sees ? sc[b][e] : -INFINITY;
                         }
                 }
                 float mx = -INFINITY;
@@ -1021,10 +1089,13 @@ __device__ __forceinline__ void chunk_part(const PagedView& c, const PagedAttent
                               sc[0][4] + y1.x, sc[0][5] + y1.y, sc[0][6] + y1.z, sc[0][7] + y1.w};
                 if (t0 < all_lo || t0 + kTile > all_hi) {  // some row does not see all of it
                     const int from = in_loop(see_lo - t0 - 4 * hf - 16 * half), to = in_loop(see_hi - t0 - 4 * hf - 16 * half);
+                    const uint64_t nodes = nodes_seen(t0) >> (4 * hf + 16 * half);
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
                         const int p = 8 * (e >> 2) + (e & 3);
-                        x[e] = p >= from && p < to ? x[e] : -INFINITY;
+                        bool sees = p >= from && p < to;
+                        if constexpr (kTree<A>) sees = sees || (nodes >> p & 1);
+                        x[e] = sees ? x[e] : -INFINITY;
                     }
                 }
                 float mx = x[0];
@@ -1219,9 +1290,9 @@ __device__ __forceinline__ void chunk_part(const PagedView& c, const PagedAttent
 // one bound by memory, the other by arithmetic. `stripe` groups in a row (a KV head's share of one workgroup per CU) are
 // chunks', the next tokens', until the token groups are used up. (30 single tokens and 5 chunks of 8 heads of 256, window 1024:
 // 152 us, with weights of one part 118; in two launches 32 us more.)
-template <int D, bool E4M3>
+template <int D, bool E4M3, class A>
 __global__ __launch_bounds__((ChunkShape<D, E4M3>::kThreads)) __attribute__((amdgpu_waves_per_eu(2))) void paged_chunk_kernel(
-    PagedView c, PagedAttentionCall a, ChunkPlan plan, int token_groups, int stripe, float* token_records, float* chunk_records) {
+    PagedView c, A a, ChunkPlan plan, int token_groups, int stripe, float* token_records, float* chunk_records) {
     using T = ChunkShape<D, E4M3>;
     constexpr int kLds = T::kPair == 1 && TokenShape<D, E4M3>::kLds > T::kLds ? TokenShape<D, E4M3>::kLds : T::kLds;
     __shared__ __attribute__((aligned(1024))) uint8_t lds[kLds];
@@ -1249,8 +1320,8 @@ constexpr int kMergeDims = 128;
 constexpr int kMergeChunkRows = 8;
 
 // Row r of the tile (rec(j): the record of split j, bm rows each), row `row` of its sequence, by one wave.
-template <int D, bool E4M3, class R>
-__device__ __forceinline__ void merge_row(const PagedView& c, const PagedAttentionCall& a, const Piece& t, int kvh, R rec, int bm, int r, int row) {
+template <int D, bool E4M3, class R, class A>
+__device__ __forceinline__ void merge_row(const PagedView& c, const A& a, const Piece& t, int kvh, R rec, int bm, int r, int row) {
     constexpr int kPer = D / 64;  // dims of a lane
     const int lane = threadIdx.x & 63;
     float m = -INFINITY, l = 0.0f, v[kPer] = {};
@@ -1308,8 +1379,8 @@ __device__ __forceinline__ void merge_row(const PagedView& c, const PagedAttenti
     }
 }
 
-template <int D, bool E4M3>
-__device__ void merge_tokens(const PagedView& c, const PagedAttentionCall& a, int groups, int blocks, const float* part, int kvh,
+template <int D, bool E4M3, class A>
+__device__ void merge_tokens(const PagedView& c, const A& a, int groups, int blocks, const float* part, int kvh,
                              int first, int stride) {
     constexpr int DB = D < kMergeDims ? D : kMergeDims, kBlocks = D / DB, kCols = DB / 4, kGroups = 256 / kCols, kAhead = 4;
     __shared__ float4 ov[kGroups][kCols];
@@ -1382,8 +1453,8 @@ __device__ void merge_tokens(const PagedView& c, const PagedAttentionCall& a, in
     }
 }
 
-template <int D, bool E4M3>
-__device__ void merge_chunks(const PagedView& c, const PagedAttentionCall& a, const ChunkPlan& plan, const float* part, int kvh, int first,
+template <int D, bool E4M3, class A>
+__device__ void merge_chunks(const PagedView& c, const A& a, const ChunkPlan& plan, const float* part, int kvh, int first,
                              int stride) {
     Seq seqs;
     ChunkWalk walk = chunk_walk(c, a, plan, &seqs);
@@ -1399,8 +1470,8 @@ __device__ void merge_chunks(const PagedView& c, const PagedAttentionCall& a, co
 
 // The first token_wgs workgroups of a KV head merge tokens (dealt out to token_groups groups, at most token_blocks blocks),
 // the others chunks.
-template <int D, bool E4M3>
-__global__ __launch_bounds__(256) void paged_merge_kernel(PagedView c, PagedAttentionCall a, int token_groups, int token_blocks, int token_wgs,
+template <int D, bool E4M3, class A>
+__global__ __launch_bounds__(256) void paged_merge_kernel(PagedView c, A a, int token_groups, int token_blocks, int token_wgs,
                                                           ChunkPlan chunks, const float* token_part, const float* chunk_part) {
     const int kvh = blockIdx.x % c.kv_heads, g = blockIdx.x / c.kv_heads, wgs = gridDim.x / c.kv_heads;
     if (g < token_wgs) merge_tokens<D, E4M3>(c, a, token_groups, token_blocks, token_part, kvh, g, token_wgs);
@@ -1409,8 +1480,8 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedView c, PagedAtte
 
 int64_t clamp64(int64_t v, int64_t lo, int64_t hi) { return v < lo ? lo : (v > hi ? hi : v); }
 
-template <int D, bool E4M3>
-hipError_t launch(const PagedView& c, const PagedAttentionCall& a, hipStream_t s, DevCtx* ctx) {
+template <int D, bool E4M3, class A>
+hipError_t launch(const PagedView& c, const A& a, hipStream_t s, DevCtx* ctx) {
     using T = TokenShape<D, E4M3>;
     const int heads = c.kv_heads;
     const bool chunks_too = (int64_t)a.max_rows * a.group > kTokenRows;
@@ -1425,12 +1496,12 @@ hipError_t launch(const PagedView& c, const PagedAttentionCall& a, hipStream_t s
     hipError_t e = hipSuccess;
     const bool join = !chunks_too && units <= kJoinUnits && (int64_t)a.max_rows * a.group * D <= kJoinElements && (int64_t)groups * heads <= kPagedTickets;
     if (join) {
-        hipLaunchKernelGGL((paged_token_kernel<D, E4M3, true>), dim3((uint32_t)(groups * heads)), dim3(256), 0, s, c, a, ctx->paged_tokens,
+        hipLaunchKernelGGL((paged_token_kernel<D, E4M3, true, A>), dim3((uint32_t)(groups * heads)), dim3(256), 0, s, c, a, ctx->paged_tokens,
                            ctx->paged_tickets);
         return hipGetLastError();
     }
     if (!one_launch) {
-        hipLaunchKernelGGL((paged_token_kernel<D, E4M3, false>), dim3((uint32_t)(groups * heads)), dim3(256), 0, s, c, a, ctx->paged_tokens,
+        hipLaunchKernelGGL((paged_token_kernel<D, E4M3, false, A>), dim3((uint32_t)(groups * heads)), dim3(256), 0, s, c, a, ctx->paged_tokens,
                            ctx->paged_tickets);
         e = hipGetLastError();
         if (e != hipSuccess) return e;
@@ -1448,32 +1519,41 @@ hipError_t launch(const PagedView& c, const PagedAttentionCall& a, hipStream_t s
         // a split tile has two records at least
         chunks.most_blocks = chunks.items / 2 * (kChunkRows / kMergeChunkRows);
         const int64_t grid = std::min<int64_t>(chunks.most, std::max(1, 65536 / heads)) + (one_launch ? groups : 0);
-        hipLaunchKernelGGL((paged_chunk_kernel<D, E4M3>), dim3((uint32_t)(grid * heads)), dim3(ChunkShape<D, E4M3>::kThreads), 0, s, c, a, chunks,
+        hipLaunchKernelGGL((paged_chunk_kernel<D, E4M3, A>), dim3((uint32_t)(grid * heads)), dim3(ChunkShape<D, E4M3>::kThreads), 0, s, c, a, chunks,
                            groups, std::max(1, ctx->cus / heads), ctx->paged_tokens, ctx->paged_chunks);
         e = hipGetLastError();
         if (e != hipSuccess) return e;
         chunk_wgs = std::min<int64_t>(chunks.most_blocks, std::max(1, 2048 / heads));
     }
     if (token_wgs + chunk_wgs == 0) return e;
-    hipLaunchKernelGGL((paged_merge_kernel<D, E4M3>), dim3((uint32_t)((token_wgs + chunk_wgs) * heads)), dim3(256), 0, s, c, a, groups,
+    hipLaunchKernelGGL((paged_merge_kernel<D, E4M3, A>), dim3((uint32_t)((token_wgs + chunk_wgs) * heads)), dim3(256), 0, s, c, a, groups,
                        (int)token_blocks, (int)token_wgs, chunks, ctx->paged_tokens, ctx->paged_chunks);
     return hipGetLastError();
 }
 
-template <int D>
-hipError_t launch_type(const PagedView& c, const PagedAttentionCall& a, hipStream_t s, DevCtx* ctx) {
+template <int D, class A>
+hipError_t launch_type(const PagedView& c, const A& a, hipStream_t s, DevCtx* ctx) {
     return c.k_scale ? launch<D, true>(c, a, s, ctx) : launch<D, false>(c, a, s, ctx);
 }
 
-}  // namespace
-
-hipError_t launch_paged_attention(const PagedView& c, const PagedAttentionCall& a, hipStream_t s, DevCtx* ctx) {
+template <class A>
+hipError_t launch_dims(const PagedView& c, const A& a, hipStream_t s, DevCtx* ctx) {
     switch (c.head_dim) {
         case 64: return launch_type<64>(c, a, s, ctx);
         case 128: return launch_type<128>(c, a, s, ctx);
         case 256: return launch_type<256>(c, a, s, ctx);
         default: return launch_type<512>(c, a, s, ctx);
     }
+}
+
+}  // namespace
+
+hipError_t launch_paged_attention(const PagedView& c, const PagedAttentionCall& a, hipStream_t s, DevCtx* ctx) {
+    return launch_dims(c, a, s, ctx);
+}
+
+hipError_t launch_paged_tree_attention(const PagedView& c, const PagedTreeCall& a, hipStream_t s, DevCtx* ctx) {
+    return launch_dims(c, a, s, ctx);
 }
 
 }  // namespace moa

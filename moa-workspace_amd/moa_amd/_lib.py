@@ -1,4 +1,4 @@
-"""ctypes binding of libmoa_gfx950.so (declarations mirror include/moa_ops.h, moa_paged.h and moa_ckpt.h).
+"""ctypes binding of libmoa_gfx950.so (declarations mirror include/moa_ops.h, moa_paged.h, moa_search.h and moa_ckpt.h).
 
 Loading fails loudly when the library is missing: there is no CPU fallback.
 """
@@ -93,6 +93,12 @@ SIGNATURES = {
     "moa_paged_cache_free": [P, P, I32, P],
     "moa_paged_cache_compact": [P, P],
     "moa_paged_attention": [P, I64, P, P, P, I64, I32, I32, I32, I32, C.c_float, I32, P],
+    "moa_paged_tree_attention": [P, I64, P, P, P, I32, P, I64, I32, I32, I32, I32, C.c_float, I32, P],
+    "moa_paged_tree_commit": [P, P, P, I32, P, I32, P],
+    "moa_paged_cache_reorder": [P, P, I32, I32, P],
+    # include/moa_search.h
+    "moa_tree_verify": [P, I64, P, P, P, I32, P, P, P, I32, I32, I32, P],
+    "moa_beam_select": [P, I64, P, P, P, P, P, P, I32, I32, I32, I32, P],
     # include/moa_bench.h
     "moa_bench_stream_read": [P, U64, I32, I32, P, P],
 }

@@ -69,6 +69,7 @@ _BF16 = (torch.bfloat16, torch.int16, torch.uint16)
 _U8 = (torch.uint8, torch.float8_e4m3fn)
 _F32 = (torch.float32,)
 _I32 = (torch.int32,)
+_I64 = (torch.int64,)
 
 
 def _stream(t: torch.Tensor) -> int:
@@ -511,6 +512,105 @@ def paged_attention(q, cache, row_starts, out, layer=0, window=0, scale=1.0, max
         raise ValueError(f"out: expected {rows} rows, got {orows}")
     _call("moa_paged_attention", qp, qr, cache._struct, p, op, orow, rows, q.shape[1], layer, window, scale,
           rows if max_rows is None else max_rows, _cache_stream(cache))
+
+
+def _masks(t, rows, device_index):
+    """Address and words of the nodes' masks: int64 [rows, words], dense."""
+    p = _ptr(t, "masks", _I64)
+    if p is None:
+        raise TypeError("masks must be a torch.Tensor")
+    if t.dim() != 2 or t.shape[0] != rows:
+        raise ValueError(f"masks must be [{rows}, words], got {tuple(t.shape)}")
+    if t.get_device() != device_index:
+        raise ValueError(f"masks lives on cuda:{t.get_device()}, the call's other tensors on cuda:{device_index}")
+    return p, t.shape[1]
+
+
+def paged_tree_attention(q, cache, row_starts, masks, out, layer=0, window=0, scale=1.0, max_rows=None) -> None:
+    """Attention of drafted trees, appended as their sequences' last positions: row i of a sequence's n is node i, at position
+    seq_lens[s] - n + i, and sees the positions before the tree and the nodes of its mask (int64 [rows, words], 1 to 4 words; bit
+    j % 64 of word j // 64: node j, itself among them). A window (0, or at least max_rows) counts from a node's depth, the number of
+    nodes that it sees. A row without bits gives zeros. Otherwise as paged_attention; max_rows is at most 64 * words (default: all rows)."""
+    p = _index(row_starts, "row_starts", cache, ("sequences", 1))
+    qp, qr, rows = _row_tensor(q, "q", cache, None)
+    op, orow, orows = _row_tensor(out, "out", cache, q.shape[1])
+    if orows != rows:
+        raise ValueError(f"out: expected {rows} rows, got {orows}")
+    mp, words = _masks(masks, rows, cache.device_index)
+    _call("moa_paged_tree_attention", qp, qr, cache._struct, p, mp, words, op, orow, rows, q.shape[1], layer, window, scale,
+          rows if max_rows is None else max_rows, _cache_stream(cache))
+
+
+def paged_tree_commit(cache, row_starts, masks, leaves) -> None:
+    """Ends a speculative step: the nodes that node leaves[s] (int32 [sequences], -1: none is kept) of a sequence sees become its
+    positions behind those before the tree, in order and in every layer; the sequence ends there, and pages that it no longer
+    reaches are free. row_starts and masks as in paged_tree_attention; a sequence without rows is left alone. A sequence whose rows,
+    length or leaf are out of range, or with a node in a page that is outside the pool or not its alone, stays as it was (bit 8)."""
+    p = _index(row_starts, "row_starts", cache, ("sequences", 1))
+    leaf = _index(leaves, "leaves", cache, ("sequences", 0))
+    rows = masks.shape[0] if isinstance(masks, torch.Tensor) and masks.dim() == 2 else -1
+    mp, words = _masks(masks, rows, cache.device_index)
+    _call("moa_paged_tree_commit", cache._struct, p, mp, words, leaf, rows, _cache_stream(cache))
+
+
+def paged_cache_reorder(cache, parents, beams) -> None:
+    """Sequences 0 .. len(parents) - 1 are groups of `beams`; every sequence s of them becomes what parents[s] (int32, a sequence of its
+    group) was: full pages are shared, a partly filled last page stays with one of its children and its slots in use are copied
+    for the others, first into the last pages of sequences that are nobody's parent, then into the lowest free pages. All or
+    nothing (bit 8): see moa_paged.h."""
+    p = _index(parents, "parents", cache, None)
+    _call("moa_paged_cache_reorder", cache._struct, p, parents.numel(), beams, _cache_stream(cache))
+
+
+def _logits(t):
+    """Address, row stride, rows and columns of bf16 logits [rows, vocab] whose rows may lie apart."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError("logits must be a torch.Tensor")
+    if not t.is_cuda:
+        raise ValueError(f"logits must live on a ROCm device, got {t.device}")
+    if t.dtype not in _BF16:
+        raise TypeError(f"logits: dtype {t.dtype} not in {_BF16}")
+    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
+        raise ValueError("logits must be [rows, vocab] with dense rows")
+    rows, vocab = t.shape
+    return t.data_ptr(), (t.stride(0) if rows > 1 else vocab), rows, vocab
+
+
+def _beside(t, name, logits, dtypes, numel):
+    p = _ptr(t, name, dtypes, numel)
+    if p is None:
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if t.get_device() != logits.get_device():
+        raise ValueError(f"{name} lives on cuda:{t.get_device()}, the logits on cuda:{logits.get_device()}")
+    return p
+
+
+def tree_verify(logits, tokens, row_starts, masks, best, leaves, next_tokens) -> None:
+    """Greedy verification of drafted trees (row_starts [sequences + 1] and masks as in paged_tree_attention): best[row] is the token of
+    the row's largest logit (bf16 [rows, vocab], rows may lie apart), ties to the lowest. From node 0 of a sequence the walk goes to
+    the lowest child whose token (int32 [rows]) is its best, as long as there is one: leaves[s] is the node where it ends,
+    next_tokens[s] that node's best; -1 both for a sequence without rows or whose first row is no node."""
+    lp, stride, rows, vocab = _logits(logits)
+    n = leaves.numel() if isinstance(leaves, torch.Tensor) else None
+    mp, words = _masks(masks, rows, logits.get_device())
+    args = [_beside(tokens, "tokens", logits, _I32, rows), _beside(row_starts, "row_starts", logits, _I32, None if n is None else n + 1), mp, words,
+            _beside(best, "best", logits, _I32, rows), _beside(leaves, "leaves", logits, _I32, None),
+            _beside(next_tokens, "next_tokens", logits, _I32, n)]
+    _call("moa_tree_verify", lp, stride, *args, rows, vocab, n, _stream(logits))
+
+
+def beam_select(logits, scores, finished, out_scores, out_finished, parents, tokens, beams, eos=-1) -> None:
+    """A beam search's step over groups of `beams` rows (bf16 logits [rows, vocab], rows may lie apart): the `beams` best of a group's
+    candidates, in descending order, ties to the lowest row and token. A candidate is scores[row] + log softmax(logits[row])[token]; a
+    finished row has the one candidate eos at its score. parents: the rows that the best come from, as paged_cache_reorder takes them.
+    out_scores may be scores (f32 [rows]), out_finished may be finished (int32 [rows]). See moa_search.h for rows without candidates."""
+    lp, stride, rows, vocab = _logits(logits)
+    if not isinstance(beams, int) or beams < 1 or rows % beams:
+        raise ValueError(f"the rows must be groups of beams, got {rows} rows and {beams} beams")
+    args = [_beside(scores, "scores", logits, _F32, rows), _beside(finished, "finished", logits, _I32, rows),
+            _beside(out_scores, "out_scores", logits, _F32, rows), _beside(out_finished, "out_finished", logits, _I32, rows),
+            _beside(parents, "parents", logits, _I32, rows), _beside(tokens, "tokens", logits, _I32, rows)]
+    _call("moa_beam_select", lp, stride, *args, rows // beams, beams, vocab, eos, _stream(logits))
 
 
 def fp8_scaled_projection(x, w, scale, out) -> None:
