@@ -203,7 +203,7 @@ DevCtx* call_context(int* code) {
 }
 
 namespace {
-// The paged calls' scratch of the current device, 98 MB that a program without them does not pay for. A call may come while a stream is
+// The paged calls' scratch of the current device, 100 MB that a program without them does not pay for. A call may come while a stream is
 // captured (moa_init has been called, no paged call yet): the thread's capture mode is relaxed meanwhile and the counters
 // are cleared on a stream of their own, so that nothing of this enters the graph.
 hipError_t allocate_paged(DevCtx* c) {
@@ -213,6 +213,7 @@ hipError_t allocate_paged(DevCtx* c) {
     const size_t t_tok = carve(sizeof(float) * kPagedTokenFloats);
     const size_t t_chunk = carve(sizeof(float) * kPagedChunkFloats);
     const size_t t_tick = carve(sizeof(uint32_t) * kPagedTickets);
+    const size_t t_search = carve(sizeof(uint32_t) * 2 * kSearchRows * kTicketStride);
     hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
     hipError_t e = hipThreadExchangeStreamCaptureMode(&mode);
     if (e != hipSuccess) return e;
@@ -221,7 +222,7 @@ hipError_t allocate_paged(DevCtx* c) {
     e = hipMalloc(&base, off);
     char* b = static_cast<char*>(base);
     if (e == hipSuccess) e = hipStreamCreateWithFlags(&s, hipStreamNonBlocking);
-    if (e == hipSuccess) e = hipMemsetAsync(b + t_tick, 0, sizeof(uint32_t) * kPagedTickets, s);
+    if (e == hipSuccess) e = hipMemsetAsync(b + t_tick, 0, off - t_tick, s);
     if (e == hipSuccess) e = hipStreamSynchronize(s);
     if (s) (void)hipStreamDestroy(s);
     if (e != hipSuccess && base) (void)hipFree(base);
@@ -230,6 +231,7 @@ hipError_t allocate_paged(DevCtx* c) {
     c->paged_tokens = reinterpret_cast<float*>(b + t_tok);
     c->paged_chunks = reinterpret_cast<float*>(b + t_chunk);
     c->paged_tickets = reinterpret_cast<uint32_t*>(b + t_tick);
+    c->search_tickets = reinterpret_cast<uint32_t*>(b + t_search);
     c->paged_list = reinterpret_cast<int32_t*>(b + t_list);
     return hipSuccess;
 }

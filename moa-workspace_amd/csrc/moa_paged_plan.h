@@ -19,8 +19,8 @@ MOA_PLAN_FN bool rows_in_range(int row0, int end, int rows, int max_rows) {
 // the arrival that completes a turn is the last one, nothing is set back, and the counter stands at a multiple of kJoinTurn after
 // every launch, whatever it held: calls that overlapped against the contract spoil their own results and no later call's.
 constexpr unsigned kJoinTurn = 32;
-MOA_PLAN_FN unsigned join_share(bool first, int parts) { return first ? kJoinTurn + 1 - (unsigned)parts : 1; }
-MOA_PLAN_FN bool join_last(unsigned before, unsigned share) { return (before + share) % kJoinTurn == 0; }
+MOA_PLAN_FN unsigned join_share(bool first, int parts, unsigned turn = kJoinTurn) { return first ? turn + 1 - (unsigned)parts : 1; }
+MOA_PLAN_FN bool join_last(unsigned before, unsigned share, unsigned turn = kJoinTurn) { return (before + share) % turn == 0; }
 
 // Units of a part of a split tile, such that tiles of more units, in ceil(units / part) parts each, have at most `items` parts in all: a
 // tile has less than 2 units / part of them, so part >= 2 total / items will do. `total` is an f32 sum of one product per

@@ -6,6 +6,7 @@
 #include "moa_checks.h"
 #include "moa_device.h"
 #include "moa_paged_plan.h"
+#include "moa_sync.h"
 
 namespace moa {
 namespace {
@@ -13,7 +14,8 @@ namespace {
 constexpr int kBlock = 256;
 constexpr int kGroupLogits = 64;        // logits that share a key (their largest): 8 lanes' 16 bytes
 constexpr int kSearchMaxVocab = 1 << 20;
-constexpr int kMaxGroups = kSearchMaxVocab / kGroupLogits;
+
+constexpr unsigned kGroupTurn = 128;  // of the counters of a group's rows
 
 typedef short s16x2 __attribute__((ext_vector_type(2)));
 
@@ -68,6 +70,7 @@ __device__ __forceinline__ int wave_max(int v) {
     return v;
 }
 
+constexpr int kMaxParts = kSearchMaxVocab / (kBlock * 8 * 2);
 // A row's parts: 256 threads of kLoads chunks each.
 __host__ __device__ inline int parts_of(int vocab, int loads) { return (vocab + kBlock * 8 * loads - 1) / (kBlock * 8 * loads); }
 
@@ -179,13 +182,15 @@ __global__ __launch_bounds__(kBlock) void verify_walk_kernel(const uint64_t* par
 
 // ---------------------------------------------------------------------------------------------- select
 
-// What a selection keeps of each row: the keys of its groups of logits, its parts' maxima and sums, and its candidates.
+// What a selection keeps of each row of a launch: the keys of its groups of logits, its parts' maxima and sums, its candidates, and the
+// counters of what has arrived.
 struct SelectScratch {
-    uint16_t* keys;      // [rows][groups]: the largest logit of a group, ordered() + 32768
-    float2* parts;       // [rows][parts]: largest logit, sum of e^(logit - largest)
-    double* totals;      // [rows][beams], descending
-    int32_t* places;     // [rows][beams]
-    int groups, parts_n; // of a row
+    uint16_t* keys;        // [rows][key_stride]: the largest logit of a group, ordered() + 32768
+    float2* parts;         // [rows][parts_n]: a reference, the sum of e^(logit - reference)
+    uint64_t* totals;      // [rows][beams] f64, descending
+    uint32_t* places;      // [rows][beams]
+    uint32_t* tickets;     // a line for every group of beams
+    int groups, key_stride, parts_n;  // of a row
 };
 
 struct SelectCall {
@@ -196,41 +201,44 @@ struct SelectCall {
 };
 
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kSlack = 2.0f;  // what a logit may lie above its lane's reference: the larger, the more an exponential's argument is rounded
 
 // A beam that adds candidates from its logits.
 __device__ __forceinline__ bool grows(const SelectCall& c, int row) { return c.finished[row] == 0 && c.scores[row] > -INFINITY; }
 
-// One pass over a part of a row: the keys of its groups, and its largest logit and sum.
+// One pass over a part of a row: the keys of its groups, and its reference and sum.
 template <int kLoads>
 __global__ __launch_bounds__(kBlock) void select_scan_kernel(SelectCall c, SelectScratch k) {
+    constexpr int kGroups = kBlock * kLoads / 8;  // of a part
     __shared__ float top[4], sums[4];
-    if (!grows(c, c.row0 + blockIdx.y)) return;
-    const LogitRow row(c.logits, c.stride, c.row0 + (int)blockIdx.y, c.vocab);
+    __shared__ __attribute__((aligned(8))) uint16_t keys[kGroups];
+    const int r = blockIdx.y;
+    if (!grows(c, c.row0 + r)) return;
+    const LogitRow row(c.logits, c.stride, c.row0 + r, c.vocab);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, first = blockIdx.x * kBlock * kLoads + threadIdx.x;
     uint4 w[kLoads];
 #pragma unroll
     for (int j = 0; j < kLoads; ++j) w[j] = row.chunk(first + j * kBlock, kMinusInfinity);
-    int most = -32768;
-    uint16_t* keys = k.keys + (int64_t)blockIdx.y * k.groups;
-#pragma unroll
-    for (int j = 0; j < kLoads; ++j) {
-        const s16x2 m = __builtin_elementwise_max(__builtin_elementwise_max(ordered(w[j].x), ordered(w[j].y)),
-                                                  __builtin_elementwise_max(ordered(w[j].z), ordered(w[j].w)));
-        int g = larger(m);
-        most = max(most, g);
-#pragma unroll
-        for (int o = 1; o < 8; o *= 2) g = max(g, __shfl_xor(g, o, kWave));
-        const int at = (first + j * kBlock) / 8;
-        if ((lane & 7) == 0 && at < k.groups) keys[at] = (uint16_t)(g + 32768);
-    }
-    const float m = most >= kLowestFinite ? key_value(most) : -INFINITY, ref = m == -INFINITY ? 0.0f : m;
-    float sum = 0.0f;
+    // The lane's sum stands against a reference that follows its largest logit so far, so that its first chunks are summed while the
+    // others are on their way. A difference of two logits is exact or its exponential nothing beside the sum.
+    float m = -INFINITY, sum = 0.0f;
 #pragma unroll
     for (int j = 0; j < kLoads; ++j) {
         float x[8];
         bf16x8_to_f32(w[j], x);
+        float most = x[0];
+#pragma unroll
+        for (int i = 1; i < 8; ++i) most = fmaxf(most, x[i]);
+        if (most > m + kSlack) {
+            sum *= __builtin_amdgcn_exp2f((m - most) * kLog2e);
+            m = most;
+        }
+        const float ref = m == -INFINITY ? 0.0f : m;
 #pragma unroll
         for (int i = 0; i < 8; ++i) sum += __builtin_amdgcn_exp2f((x[i] - ref) * kLog2e);
+#pragma unroll
+        for (int o = 1; o < 8; o *= 2) most = fmaxf(most, __shfl_xor(most, o, kWave));
+        if ((lane & 7) == 0) keys[(j * kBlock + threadIdx.x) / 8] = (uint16_t)(ordered(__float_as_uint(most) >> 16)[0] + 32768);
     }
     float all = m;
 #pragma unroll
@@ -238,182 +246,224 @@ __global__ __launch_bounds__(kBlock) void select_scan_kernel(SelectCall c, Selec
     sum = wave_sum(m == -INFINITY ? sum : sum * __builtin_amdgcn_exp2f((m - all) * kLog2e));  // (a NaN in a lane without a finite logit stays)
     if (lane == 0) top[wave] = all, sums[wave] = sum;
     __syncthreads();
-    if (threadIdx.x) return;
-    const float part = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-    float total = 0.0f;
+    const int at = (int)blockIdx.x * kGroups + 4 * (int)threadIdx.x;  // four keys a thread
+    if ((int)threadIdx.x < kGroups / 4 && at < k.key_stride)
+        *reinterpret_cast<uint64_t*>(k.keys + (int64_t)r * k.key_stride + at) = reinterpret_cast<const uint64_t*>(keys)[threadIdx.x];
+    if (threadIdx.x == 0) {
+        const float part = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+        float total = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) total += top[i] == -INFINITY ? sums[i] : sums[i] * __builtin_amdgcn_exp2f((top[i] - part) * kLog2e);
-    k.parts[(int64_t)blockIdx.y * k.parts_n + blockIdx.x] = make_float2(part, total);
+        for (int i = 0; i < 4; ++i) total += top[i] == -INFINITY ? sums[i] : sums[i] * __builtin_amdgcn_exp2f((top[i] - part) * kLog2e);
+        k.parts[(int64_t)r * k.parts_n + blockIdx.x] = make_float2(part, total);
+    }
 }
 
-// The sum of v over the workgroup, in every thread. lds: 4 numbers that no earlier call may still read.
-template <class T>
-__device__ T block_total(T v, T* lds) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, kWave);
+// Whether this workgroup is the last of `parts` to arrive at a counter; what the others published before is then there to
+// collect. kTurn: a power of two above any number of parts.
+template <unsigned kTurn>
+__device__ bool arrive_last(uint32_t* ticket, bool first, int parts) {
+    __shared__ uint32_t flag;
+    __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+    if (threadIdx.x == 0) {
+        const uint32_t share = join_share(first, parts, kTurn);
+        flag = join_last(__hip_atomic_fetch_add(ticket, share, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT), share, kTurn);
+    }
     __syncthreads();
-    return lds[0] + lds[1] + lds[2] + lds[3];
+    return flag;
 }
 
-// The positions of the `want` largest of n keys in LDS that are at least `least`, ties to the lowest position, in any order;
-// returns how many there are. The smallest of them is found by halving the range of keys.
-__device__ int largest_keys(const uint16_t* keys, int n, int want, int least, int* out, int* lds) {
-    const int t = threadIdx.x, per = (n + kBlock - 1) / kBlock, from = min(t * per, n), to = min(from + per, n);
-    auto count = [&](int least) {
-        int c = 0;
-        for (int i = from; i < to; ++i) c += keys[i] >= least;
-        return block_total(c, lds);
+// The largest of the wave's values, the same in every lane: four shifts within rows of 16, then the rows' last lanes (DPP).
+__device__ __forceinline__ uint32_t wave_largest(uint32_t x) {
+    auto step = [&](uint32_t y) { x = max(x, y); };
+    step(__builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false));
+    step(__builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false));
+    step(__builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false));
+    step(__builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false));
+    step(__builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false));
+    step(__builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false));
+    return __builtin_amdgcn_readlane(x, 63);
+}
+
+// The `want` largest of the workgroup's numbers (kN a thread; different but for 0, which is none), in descending order in `out`
+// behind a barrier; returns how many there are. Each wave takes its own one after the other, and where a number stands among the
+// four waves' lists is counted. lists: [4][kMaxBeams].
+template <int kN>
+__device__ int block_largest(uint32_t (&v)[kN], int want, uint32_t (*lists)[kMaxBeams], uint32_t* out) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    uint32_t mine = 0;
+#pragma unroll
+    for (int i = 0; i < kN; ++i) mine = max(mine, v[i]);
+    uint32_t kept = 0;  // lane i: number i of the wave's
+    for (int i = 0; i < want; ++i) {
+        const uint32_t best = wave_largest(mine);
+        if (best == 0) break;
+        if (lane == i) kept = best;
+        if (mine == best) {
+            mine = 0;
+#pragma unroll
+            for (int j = 0; j < kN; ++j) {
+                v[j] = v[j] == best ? 0 : v[j];
+                mine = max(mine, v[j]);
+            }
+        }
+    }
+    __syncthreads();  // the lists of an earlier call have been read
+    lists[wave][lane] = kept;
+    __syncthreads();
+    int rank = lane, n = 0;
+#pragma unroll
+    for (int w = 0; w < 4; ++w)
+        for (int i = 0; i < want; ++i) {
+            const uint32_t y = lists[w][i];
+            n += y != 0;
+            rank += w != wave && y > kept;
+        }
+    if (kept && rank < want) out[rank] = kept;
+    __syncthreads();
+    return min(n, want);
+}
+
+// The row's candidates: of the groups that come first by key and place, as many as beams (each holds a logit that comes before all of a
+// later group's), then of their logits. Numbers order by key, then by place, the lower first.
+template <int kKeys>
+__device__ void select_row(const SelectCall& c, const SelectScratch& k, int r) {
+    __shared__ uint32_t lists[4][kMaxBeams], found[kMaxBeams];
+    __shared__ int groups[kMaxBeams];
+    __shared__ double row_lse;
+    const int row = c.row0 + r, t = threadIdx.x, lane = t & 63;
+    uint64_t* totals = k.totals + (int64_t)r * c.beams;
+    uint32_t* places = k.places + (int64_t)r * c.beams;
+    const float score_f = c.scores[row];
+    const int done = c.finished[row];
+    const double score = score_f;
+    auto put = [&](int i, double total, int place) {
+        publish64(totals + i, __builtin_bit_cast(uint64_t, total));
+        publish32(places + i, (uint32_t)place);
     };
-    int lo = least, hi = 65536;  // at least `want` keys are lo or more (or lo is `least`); fewer are hi or more
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) / 2;
-        if (count(mid) >= want) lo = mid;
-        else hi = mid;
-    }
-    int above = 0, equal = 0;
-    for (int i = from; i < to; ++i) above += keys[i] > lo, equal += keys[i] == lo;
-    // both prefix sums at once: neither passes 2^16
-    int x = above << 16 | equal, before = 0;
-    const int mine = x, lane = t & 63, wave = t >> 6;
+    constexpr int kMost = kMaxParts / kWave;
+    float2 part[kMost];  // the row's sums, in every wave
 #pragma unroll
-    for (int o = 1; o < kWave; o <<= 1) {
-        const int y = __shfl_up(x, o, kWave);
-        if (lane >= o) x += y;
+    for (int i = 0; i < kMost; ++i)
+        part[i] = i * kWave + lane < k.parts_n ? k.parts[(int64_t)r * k.parts_n + i * kWave + lane] : make_float2(-INFINITY, 0.0f);
+    constexpr uint32_t kLeast = kLowestFinite + 32768;
+    const uint16_t* keys = k.keys + (int64_t)r * k.key_stride;
+    uint64_t four[kKeys / 4];  // (of a row that adds none: of an earlier call)
+#pragma unroll
+    for (int j = 0; j < kKeys / 4; ++j) {
+        const int at = 4 * (j * kBlock + t);
+        four[j] = at < k.groups ? *reinterpret_cast<const uint64_t*>(keys + at) : 0;
     }
-    __syncthreads();
-    if (lane == 63) lds[wave] = x;
-    __syncthreads();
-    for (int i = 0; i < wave; ++i) before += lds[i];
-    const int total = lds[0] + lds[1] + lds[2] + lds[3], tops = total >> 16;
-    before += x - mine;
-    int a = before >> 16, e = tops + (before & 0xffff);
-    for (int i = from; i < to; ++i) {
-        if (keys[i] > lo) out[a++] = i;
-        else if (keys[i] == lo) {
-            if (e < want) out[e] = i;
-            ++e;
-        }
-    }
-    __syncthreads();
-    return min(want, tops + (total & 0xffff));
-}
-
-// One workgroup per row: its sum, the groups that hold its `beams` largest logits (of the groups that come first by key and place,
-// since each holds a logit that comes before all of a later group), those logits, and their totals in descending order.
-__global__ __launch_bounds__(kBlock) void select_row_kernel(SelectCall c, SelectScratch k) {
-    __shared__ uint16_t keys[kMaxGroups > kMaxBeams * kGroupLogits ? kMaxGroups : kMaxBeams * kGroupLogits];
-    __shared__ int groups[kMaxBeams], chosen[kMaxBeams], lds[4];
-    __shared__ double sums[4];
-    __shared__ float top[4];
-    const int r = blockIdx.x, row = c.row0 + r, t = threadIdx.x, lane = t & 63;
-    double* totals = k.totals + (int64_t)r * c.beams;
-    int32_t* places = k.places + (int64_t)r * c.beams;
-    const double score = c.scores[row];
-    if (!grows(c, row)) {
-        if (t < c.beams) {
-            totals[t] = t == 0 && c.eos >= 0 && score > -INFINITY ? score : -INFINITY;
-            places[t] = c.eos;
-        }
+    if (done != 0 || !(score_f > -INFINITY)) {
+        if (t < c.beams) put(t, t == 0 && c.eos >= 0 && done != 0 && score_f > -INFINITY ? score : -INFINITY, c.eos);
         return;
     }
-    float m = -INFINITY;
-    for (int i = t; i < k.parts_n; i += kBlock) m = fmaxf(m, k.parts[(int64_t)r * k.parts_n + i].x);
+    uint32_t v[kKeys];
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, kWave));
-    if (lane == 0) top[t >> 6] = m;
-    for (int i = t; i < k.groups; i += kBlock) keys[i] = k.keys[(int64_t)r * k.groups + i];
-    __syncthreads();
-    m = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-    double sum = 0.0;
-    for (int i = t; i < k.parts_n; i += kBlock) {
-        const float2 p = k.parts[(int64_t)r * k.parts_n + i];
-        sum += p.x == -INFINITY ? (double)p.y : (double)p.y * exp((double)p.x - (double)m);
-    }
-    sum = block_total(sum, sums);
-    const bool alive = sum > 0.0 && sum < INFINITY && m < INFINITY;
-    const double lse = (double)m + log(sum);
-    constexpr int kLeast = kLowestFinite + 32768;
-    const int ng = alive ? largest_keys(keys, k.groups, c.beams, kLeast, groups, lds) : 0;
-    // their logits, groups in ascending order
-    const LogitRow logits(c.logits, c.stride, row, c.vocab);
-    __syncthreads();
-    if (t < 64) {
-        const int g = lane < ng ? groups[lane] : 0x7fffffff;
+    for (int j = 0; j < kKeys / 4; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int at = 4 * (j * kBlock + t) + i;
+            const uint32_t key = (uint32_t)(four[j] >> 16 * i) & 0xffffu;
+            v[4 * j + i] = at < k.groups && key >= kLeast ? key << 16 | (0xffffu - at) : 0;
+        }
+    const int ng = block_largest<kKeys>(v, c.beams, lists, found);
+    if (t < ng) {  // in ascending order
+        const int g = 0xffff - (int)(found[t] & 0xffffu);
         int rank = 0;
-        for (int i = 0; i < ng; ++i) rank += __shfl(g, i, kWave) < g;
-        if (lane < ng) chosen[rank] = g;
+        for (int i = 0; i < ng; ++i) rank += 0xffff - (int)(found[i] & 0xffffu) < g;
+        groups[rank] = g;
     }
     __syncthreads();
-    for (int i = t; i < ng * 8; i += kBlock) {
-        const uint4 w = logits.chunk(chosen[i / 8] * 8 + i % 8, kMinusInfinity);
-        const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+    const LogitRow logits(c.logits, c.stride, row, c.vocab);
+    uint32_t e[16];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const s16x2 o = ordered(v[j]);
-            keys[8 * i + 2 * j] = (uint16_t)(o[0] + 32768), keys[8 * i + 2 * j + 1] = (uint16_t)(o[1] + 32768);
+    for (int j = 0; j < 2; ++j) {
+        const int i = j * kBlock + t;  // 16 bytes of a group
+        uint4 w = make_uint4(0, 0, 0, 0);
+        if (i < 8 * ng) w = logits.chunk(groups[i / 8] * 8 + i % 8, kMinusInfinity);
+        const uint32_t two[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+            const s16x2 o = ordered(two[h]);
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+                e[8 * j + 2 * h + x] = i < 8 * ng && o[x] >= kLowestFinite ? (uint32_t)(o[x] + 32768) << 16 | (0xffffu - (8 * i + 2 * h + x)) : 0;
         }
     }
-    __syncthreads();
-    const int n = ng ? largest_keys(keys, ng * kGroupLogits, c.beams, kLeast, groups, lds) : 0;
-    if (t >= 64) return;
-    int key = 0, at = 0x7fffffff;
-    if (lane < n) key = keys[groups[lane]], at = groups[lane];
-    int rank = 0;
-    for (int i = 0; i < n; ++i) {
-        const int y = __shfl(key, i, kWave), z = __shfl(at, i, kWave);
-        rank += y > key || (y == key && z < at);
+    if (t >= 3 * kWave) {  // the row's sum, by the wave that has no logits of up to 24 beams
+        float m = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < kMost; ++i) m = fmaxf(m, part[i].x);
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, kWave));
+        double sum = 0.0;
+#pragma unroll
+        for (int i = 0; i < kMost; ++i)
+            sum += part[i].x == -INFINITY ? (double)part[i].y : (double)part[i].y * (double)__builtin_amdgcn_exp2f((part[i].x - m) * kLog2e);
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, kWave);
+        if (lane == 0) row_lse = sum > 0.0 && sum < INFINITY && m < INFINITY ? (double)m + log(sum) : -INFINITY;
     }
-    if (lane < n) {
-        totals[rank] = score + ((double)key_value(key - 32768) - lse);
-        places[rank] = chosen[at / kGroupLogits] * kGroupLogits + at % kGroupLogits;
-    } else if (lane < c.beams) {
-        totals[lane] = -INFINITY;
-        places[lane] = -1;
+    const int n = block_largest<16>(e, c.beams, lists, found);
+    if (t >= c.beams) return;
+    if (t < n && row_lse > -INFINITY) {
+        const int at = 0xffff - (int)(found[t] & 0xffffu);
+        put(t, score + ((double)key_value((int)(found[t] >> 16) - 32768) - row_lse), groups[at / kGroupLogits] * kGroupLogits + at % kGroupLogits);
+    } else {
+        put(t, -INFINITY, -1);
     }
 }
 
-// One wave per group, a lane per row: the largest of the rows' next candidates, `beams` times.
-__global__ __launch_bounds__(kWave) void select_merge_kernel(SelectCall c, SelectScratch k) {
-    const int lane = threadIdx.x, r0 = blockIdx.x * c.beams, row = c.row0 + r0 + lane;
-    const double* totals = k.totals + (int64_t)(r0 + lane) * c.beams;
-    const int32_t* places = k.places + (int64_t)(r0 + lane) * c.beams;
+// A group's beams, a lane per row of one wave: the largest of the rows' next candidates, `beams` times. Totals are compared as 64-bit
+// numbers in their order, 0 for none: high words first, then the low words of those that are equal. The candidates come to LDS at once.
+__device__ void select_merge(const SelectCall& c, const SelectScratch& k, int r0) {
+    __shared__ uint64_t orders[kMaxBeams * kMaxBeams];
+    __shared__ uint32_t tokens[kMaxBeams * kMaxBeams];
+    for (int i = threadIdx.x; i < c.beams * c.beams; i += kBlock) {
+        const uint64_t b = collect64(k.totals + (int64_t)r0 * c.beams + i);
+        tokens[i] = __hip_atomic_load(k.places + (int64_t)r0 * c.beams + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        orders[i] = __builtin_bit_cast(double, b) > -INFINITY ? (b >> 63 ? ~b : b | 1ull << 63) : 0;
+    }
+    __syncthreads();
+    if (threadIdx.x >= kWave) return;
+    const int lane = threadIdx.x, row = c.row0 + r0 + lane;
     const bool in = lane < c.beams;
-    int next = 0, place = in ? places[0] : 0, out_parent = row, out_token = max(c.eos, 0);
-    double total = in ? totals[0] : -INFINITY, out_total = -INFINITY;
-    if (total != total) total = -INFINITY;
+    int next = 0;
+    uint64_t order = in ? orders[lane * c.beams] : 0;  // the row's next candidate
     const int done = in ? c.finished[row] != 0 : 0;
-    int out_done = 1;
+    int out_parent = row, out_token = max(c.eos, 0), out_done = 1;
+    uint64_t out = 0;
     for (int i = 0; i < c.beams; ++i) {
-        double best = total;
-        int who = lane;
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) {
-            const double y = __shfl_xor(best, o, kWave);
-            const int z = __shfl_xor(who, o, kWave);
-            if (y > best || (y == best && z < who)) best = y, who = z;
-        }
-        if (best == -INFINITY) break;
-        const int token = __shfl(place, who, kWave), was = __shfl(done, who, kWave);
+        const uint32_t hi = wave_largest((uint32_t)(order >> 32));
+        if (hi == 0) break;
+        const bool top = (uint32_t)(order >> 32) == hi;
+        const uint32_t lo = wave_largest(top ? (uint32_t)order : 0);
+        const int who = __builtin_ctzll(__ballot(top && (uint32_t)order == lo));  // the lowest row of equals
+        const int token = (int)tokens[who * c.beams + __builtin_amdgcn_readlane(next, who)], was = __builtin_amdgcn_readlane(done, who);
         if (lane == i) {
-            out_total = best;
+            out = (uint64_t)hi << 32 | lo;
             out_parent = c.row0 + r0 + who;
             out_token = token;
             out_done = was || token == c.eos;
         }
-        if (lane == who) {
-            ++next;
-            total = next < c.beams ? totals[next] : -INFINITY;
-            place = next < c.beams ? places[next] : 0;
-            if (total != total) total = -INFINITY;
-        }
+        if (lane == who) order = ++next < c.beams ? orders[lane * c.beams + next] : 0;
     }
     if (!in) return;
-    c.out_scores[row] = (float)out_total;
+    const double total = __builtin_bit_cast(double, out >> 63 ? out & ~(1ull << 63) : ~out);
+    c.out_scores[row] = out ? (float)total : -INFINITY;
     c.parents[row] = out_parent;
     c.tokens[row] = out_token;
     c.out_finished[row] = out_done;
+}
+
+// A workgroup per row; the last of a group picks its beams.
+template <int kKeys>
+__global__ __launch_bounds__(kBlock) void select_rows_kernel(SelectCall c, SelectScratch k) {
+    const int r = blockIdx.x, g = r / c.beams;
+    select_row<kKeys>(c, k, r);
+    if (!arrive_last<kGroupTurn>(k.tickets + (int64_t)g * kTicketStride, r == g * c.beams, c.beams)) return;
+    select_merge(c, k, g * c.beams);
 }
 
 int check_logits(const uint16_t* logits, int64_t stride, int rows, int vocab) {
@@ -424,9 +474,11 @@ int check_logits(const uint16_t* logits, int64_t stride, int rows, int vocab) {
     return MOA_SUCCESS;
 }
 
-// Loads of a thread: eight where two workgroups a CU are left then, else two, for more workgroups.
-int loads_of(int64_t rows, int vocab, int cus) { return rows * parts_of(vocab, 8) >= 2 * (int64_t)cus ? 8 : 2; }
+// Loads of a thread: four where two workgroups a CU are left then, else two, for more workgroups. (151 rows of 262144: 17.5 us with four, 18.7 with
+// eight.)
+int loads_of(int64_t rows, int vocab, int cus) { return rows * parts_of(vocab, 4) >= 2 * (int64_t)cus ? 4 : 2; }
 
+static_assert(kMaxBeams < (int)kGroupTurn, "arrivals are fewer than a turn");
 constexpr size_t kSearchBytes = kPagedChunkFloats * sizeof(float);
 
 }  // namespace
@@ -453,7 +505,7 @@ int moa_tree_verify(const uint16_t* logits, int64_t logit_row_stride, const int3
     const int loads = loads_of(rows, vocab, ctx->cus), parts = parts_of(vocab, loads);
     uint64_t* part = reinterpret_cast<uint64_t*>(ctx->paged_chunks);
     if (rows) {
-        auto* f = loads == 8 ? verify_scan_kernel<8> : verify_scan_kernel<2>;
+        auto* f = loads == 4 ? verify_scan_kernel<4> : verify_scan_kernel<2>;
         hipLaunchKernelGGL(f, dim3(parts, rows), dim3(kBlock), 0, s, logits, logit_row_stride, vocab, part);
         if ((e = call_result(hipGetLastError(), "tree_verify launch"))) return e;
     }
@@ -481,23 +533,25 @@ int moa_beam_select(const uint16_t* logits, int64_t logit_row_stride, const floa
     const int loads = loads_of(rows, vocab, ctx->cus);
     SelectScratch k;
     k.groups = (vocab + kGroupLogits - 1) / kGroupLogits;
+    k.key_stride = (k.groups + 3) / 4 * 4;
     k.parts_n = parts_of(vocab, loads);
-    // the groups of rows that the scratch holds at once (all but always: it holds 2000 rows of the largest vocabulary)
-    const size_t row_bytes = (size_t)beams * 12 + (size_t)k.parts_n * 8 + (size_t)k.groups * 2;
-    const int most = (int)std::min<size_t>(groups, kSearchBytes / (row_bytes * beams));
+    // the groups of rows that the scratch and its counters hold at once
+    const size_t row_bytes = (size_t)beams * 12 + (size_t)k.parts_n * 8 + (size_t)k.key_stride * 2;
+    const int most = (int)std::min<size_t>(groups, std::min<size_t>(kSearchBytes / (row_bytes * beams), kSearchRows / beams));
     uint8_t* at = reinterpret_cast<uint8_t*>(ctx->paged_chunks);
     const size_t held = (size_t)most * beams;
-    k.totals = reinterpret_cast<double*>(at);
+    k.totals = reinterpret_cast<uint64_t*>(at);
     k.parts = reinterpret_cast<float2*>(at + held * beams * 8);
-    k.places = reinterpret_cast<int32_t*>(at + held * (beams * 8 + k.parts_n * 8));
-    k.keys = reinterpret_cast<uint16_t*>(at + held * (beams * 12 + k.parts_n * 8));
+    k.keys = reinterpret_cast<uint16_t*>(at + held * (beams * 8 + k.parts_n * 8));
+    k.places = reinterpret_cast<uint32_t*>(at + held * (beams * 8 + k.parts_n * 8 + k.key_stride * 2));
+    k.tickets = ctx->search_tickets;
+    auto* scan = loads == 4 ? select_scan_kernel<4> : select_scan_kernel<2>;
+    auto* pick = k.groups > 16 * kBlock ? select_rows_kernel<64> : select_rows_kernel<16>;
     for (int g = 0; g < groups; g += most) {
-        const int here = std::min(most, groups - g), n = here * beams;
+        const int here = std::min(most, groups - g);
         const SelectCall c{logits, logit_row_stride, scores, finished, out_scores, out_finished, parents, tokens, beams, vocab, eos, g * beams};
-        auto* f = loads == 8 ? select_scan_kernel<8> : select_scan_kernel<2>;
-        hipLaunchKernelGGL(f, dim3(k.parts_n, n), dim3(kBlock), 0, s, c, k);
-        hipLaunchKernelGGL(select_row_kernel, dim3(n), dim3(kBlock), 0, s, c, k);
-        hipLaunchKernelGGL(select_merge_kernel, dim3(here), dim3(kWave), 0, s, c, k);
+        hipLaunchKernelGGL(scan, dim3(k.parts_n, here * beams), dim3(kBlock), 0, s, c, k);
+        hipLaunchKernelGGL(pick, dim3(here * beams), dim3(kBlock), 0, s, c, k);
         if ((e = call_result(hipGetLastError(), "beam_select launch"))) return e;
     }
     return MOA_SUCCESS;
