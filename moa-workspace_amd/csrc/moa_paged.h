@@ -66,5 +66,7 @@ struct PagedTreeCall : PagedAttentionCall {
 
 hipError_t launch_paged_attention(const PagedView& c, const PagedAttentionCall& a, hipStream_t s, DevCtx* ctx);
 hipError_t launch_paged_tree_attention(const PagedView& c, const PagedTreeCall& a, hipStream_t s, DevCtx* ctx);
+// The kernels of few and of many rows a sequence, for trees.
+hipError_t launch_paged_tree_rows(const PagedView& c, const PagedTreeCall& a, hipStream_t s, DevCtx* ctx);
 
 }  // namespace moa

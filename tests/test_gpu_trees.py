@@ -160,6 +160,33 @@ def test_values_that_a_node_does_not_see_never_reach_it(n, heads, group, dim, fm
         assert all(out[i].isnan().all() for i in range(n) if masks[i] >> victim & 1)
 
 
+@pytest.mark.parametrize("fmt", ["bf16", "e4m3"])
+@pytest.mark.parametrize("n,heads,group,dim", [(6, 2, 2, 128), (20, 1, 1, 256), (12, 2, 4, 64), (50, 2, 1, 256), (25, 1, 4, 128), (40, 1, 16, 512), (200, 1, 1, 64)])
+@pytest.mark.parametrize("rise", [0.05, 1.0, 40.0])
+def test_scores_that_rise_along_the_sequence(rise, n, heads, group, dim, fmt):
+    """The largest score grows by 700 rise over the positions, so that a reference taken early is far below it."""
+    need_gpu()
+    st = Setup([700 + n, 3 + n], 16, heads, dim, fmt)
+    step = torch.arange(700 + n, device=DEV).float() * rise / dim
+    page = torch.tensor(st.state.table[0], device=DEV)[torch.arange(700 + n, device=DEV) // 16]
+    rows = step[:, None, None].expand(-1, heads, dim)
+    if fmt == "bf16":
+        st.k[0, page, torch.arange(700 + n, device=DEV) % 16] = rows.to(torch.bfloat16)
+    else:
+        codes = (rows / st.k_scale[0][:, None]).clamp(-448, 448).to(torch.float8_e4m3fn)
+        st.k.view(torch.uint8)[0, page, torch.arange(700 + n, device=DEV) % 16] = codes.view(torch.uint8)
+    masks = trees([n, n], 3)
+    q = torch.ones((2 * n, heads * group, dim), dtype=torch.bfloat16, device=DEV)
+    q[::2] = -1.0
+    out = torch.empty_like(q)
+    ops.paged_tree_attention(q, st.cache, i32([0, n, 2 * n]), cm.mask_tensor(masks, cm.words_of(n), DEV), out, max_rows=n)
+    assert ops.device_errors() == 0
+    k, v = st.values()
+    sc = (None, None) if st.k_scale is None else (st.k_scale[0], st.v_scale[0])
+    want, a, d = cm.attention(q, k, v, st.state.table, st.state.lens, [0, n, 2 * n], masks, 16, 0, 1.0, *sc)
+    check(out, want, a, d, dim)
+
+
 @pytest.mark.parametrize("n", [2, 60])
 @pytest.mark.parametrize("bad", ["page", "length", "rows", "descend"])
 def test_bad_sequences_are_left_out(bad, n):
