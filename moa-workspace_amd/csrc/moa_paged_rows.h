@@ -248,6 +248,28 @@ __device__ __forceinline__ uint32_t bf16_pair_of_fp8(uint32_t two) {
     return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(two, 1.0f, false));
 }
 
+// 16-byte chunk c of LDS row r lies in chunk c ^ swizzle(r): sixteen rows' reads of one chunk, and four rows' reads of four
+// chunks, then meet on no bank. Rows of 128 bytes (64 dims) pair up: two rows span the banks.
+template <int D>
+__host__ __device__ constexpr int chunk_swizzle(int r) {
+    return D == 64 ? ((r >> 1 & 1) << 2 | (r >> 2 & 3)) : ((r & 3) << 2 | (r >> 2 & 3));
+}
+
+typedef __attribute__((address_space(3))) void lds_void;
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+
+// 16 bytes per lane from global memory into LDS, lane l's at lds + 16 l. In asm, since the compiler would let no LDS read
+// pass before all such loads are done; `ready` waits for them. (One wait state between the
+// write of m0 and its use, five between a vector instruction's write of a scalar register and its use.)
+__device__ __forceinline__ void load_to_lds(const void* from, uint32_t lds) {
+    __asm__ volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "{m0}"(lds) : "memory");
+}
+__device__ __forceinline__ void load_to_lds(const void* base, uint32_t offset, uint32_t lds) {
+    __asm__ volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(base), "{m0}"(lds) : "memory");
+}
+
 // Row r of the tile (rec(j): the record of split j, bm rows each), row `row` of its sequence, by one wave.
 template <int D, bool E4M3, class R, class A>
 __device__ __forceinline__ void merge_row(const PagedView& c, const A& a, const Piece& t, int kvh, R rec, int bm, int r, int row) {

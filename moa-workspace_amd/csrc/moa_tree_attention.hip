@@ -1,9 +1,8 @@
 // moa_tree_attention.hip -- attention of drafted trees over the paged cache (include/moa_paged.h) for sequences of a few dozen rows.
 //
-// Every row of a tree sees the positions before it, so K and V of a sequence are read once for up to 16 RB rows, and the
-// kernel is bound by their bytes: they go from memory to registers and never through LDS, each of four waves taking tiles of 16 or 32
-// positions in turn, as in the kernel of few rows (moa_paged_attention.hip), whose lane layouts these are. What a wave
-// has of K and V it uses for RB blocks of 16 rows, whose queries are in LDS and whose outputs in registers.
+// Every row of a tree sees the positions before it, so one pass over K and V serves all rows of a sequence: up to 64 or 128 of them in a
+// workgroup, 16 for each of its waves. K and V go through LDS, in a ring of tiles of 16 KB: the matrix cores and LDS have a third of the
+// time that memory takes, so what counts is that loads never pause.
 #include <algorithm>
 
 #include "moa_paged_rows.h"
@@ -11,22 +10,25 @@
 namespace moa {
 namespace {
 
+constexpr int kTreeRows = 64;       // of a tile: 16 for each of four waves
 constexpr int kTreeMaxRows = 128;  // of a sequence: two passes over its K and V
 
-template <int D, bool E4M3, int RB>  // RB: 2 or 4
+template <int D, bool E4M3>
 struct TreeShape {
-    static constexpr int kElem = E4M3 ? 1 : 2;
-    static constexpr int kRows = 16 * RB;                                       // of a tile
-    static constexpr int kSub = D * kElem >= 512 ? 1 : 2;                       // 16 positions each
-    static constexpr int kTile = 16 * kSub;
-    static constexpr int kHeld = RB * D <= 256 ? 2 : 1;                         // workgroups on a CU: waves per SIMD
-    static constexpr int kKLoads = D * kElem / 64;                              // 16-byte loads of a K row per lane
-    static constexpr int kVD = (E4M3 ? 16 : 8) < D / 16 ? (E4M3 ? 16 : 8) : D / 16;  // dims per V load
-    static constexpr int kVB = D / (16 * kVD);                                  // V loads of a row per lane
-    static constexpr int kVWords = kVD * kElem / 4;
-    static constexpr int kQStride = D + 8;                                      // LDS row of Q: 16 rows start on 16 bank groups
-    static constexpr int kQBytes = kRows * kQStride * 2;
-    static constexpr int kLds = kQBytes + 4 * 16 * D * 4 + 2 * 4 * 16 * 4;
+    static constexpr int kTile = D == 64 ? 64 : 32;          // positions: 16 KB of K and V as bf16, 32 KB of 256 dims
+    static constexpr int kSub = kTile / 16;
+    static constexpr int kRowBytes = 2 * D;                  // LDS row of a position
+    static constexpr int kStage = 2 * kTile * kRowBytes;
+    // Two workgroups share a CU's 160 KB. bf16: tiles on their way or there. E4M3: two tiles as bf16, and kAhead tiles of codes on their way
+    // in registers, 32 of them.
+    static constexpr int kStages = E4M3 ? 2 : 80 * 1024 / kStage;
+    static constexpr int kLds = kStages * kStage;
+    static constexpr int kAhead = D == 256 ? 2 : 4;
+    static constexpr int kWaveRows = kTile / 4;              // positions of a tile that a wave loads
+    static constexpr int kRowsPerLoad = 1024 / kRowBytes;    // positions that a load of 16 bytes a lane covers
+    static constexpr int kLoads = kWaveRows / kRowsPerLoad;  // of K, and of V, per wave and tile
+    static constexpr int kCodeLoads = kTile * D / 16 / 256;  // E4M3: the same per thread
+    static constexpr int kGroup = 64 / kWaveRows;            // tiles whose positions a wave's lanes look up at once
 };
 
 // The units of kTokenUnit positions of all sequences' tiles, a sequence's tiles behind each other, are one row of U, dealt out evenly: group
@@ -37,7 +39,11 @@ struct TreeWalk {
     int64_t units, q;  // U, q
     int base;          // the 64 sequences looked at
     int64_t before;    // units before them
+    Seq last;          // the last 64 sequences' lanes, the only ones of most calls
 };
+
+// A split tile, for the merge: its sequence's rows, its number there, its parts. A group begins one at most: its last.
+struct TreeSplit { int row0, n, tile, parts; };
 
 // Inclusive sums of numbers below 2^50: the low 20 bits and the others apart.
 __device__ __forceinline__ int64_t scan_sum64(int64_t x) { return ((int64_t)scan_sum((int)(x >> 20)) << 20) + scan_sum((int)(x & 0xfffff)); }
@@ -48,16 +54,14 @@ __device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {  // of numbe
     return (a | b) >> 31 ? a / b : (int64_t)((uint32_t)a / (uint32_t)b);
 }
 
-template <int R>
-__device__ __forceinline__ int tree_tiles(const PagedTreeCall& a, const Seq& q) { return (q.n * a.group + R - 1) / R; }
+__device__ __forceinline__ int tree_tiles(const PagedTreeCall& a, const Seq& q) { return (q.n * a.group + kTreeRows - 1) / kTreeRows; }
 
-template <int R>
 __device__ TreeWalk tree_walk(const PagedView& c, const PagedTreeCall& a, int groups, int align) {
-    TreeWalk w = {0, 1, 0, 0};
+    TreeWalk w = {0, 1, 0, 0, {0, 0, 0}};
     bool bad = false;
     for (int base = 0; base < c.sequences; base += 64) {
-        const Seq q = seq_of<true>(c, a, base + (threadIdx.x & 63), true, &bad);
-        w.units += (int64_t)tree_tiles<R>(a, q) * token_units(a, q, align);
+        w.last = seq_of<true>(c, a, base + (threadIdx.x & 63), true, &bad);
+        w.units += (int64_t)tree_tiles(a, w.last) * token_units(a, w.last, align);
     }
     raise_bad(c, bad);
     w.units = lane64(scan_sum64(w.units), 63);
@@ -67,14 +71,14 @@ __device__ TreeWalk tree_walk(const PagedView& c, const PagedTreeCall& a, int gr
 }
 
 // The tile that unit u (not before an earlier call's) belongs to, its units and the first of them. u < w.units.
-template <int R>
 __device__ void tree_at(const PagedView& c, const PagedTreeCall& a, TreeWalk& w, int align, int64_t u, Piece* out, int* units, int64_t* first) {
     const int lane = threadIdx.x & 63;
     bool bad = false;
     for (;; w.base += 64) {
-        const Seq q = seq_of<true>(c, a, w.base + lane, true, &bad);
+        Seq q = w.last;
+        if (c.sequences > 64) q = seq_of<true>(c, a, w.base + lane, true, &bad);
         const int n = token_units(a, q, align);
-        const int64_t all = (int64_t)tree_tiles<R>(a, q) * n, x = scan_sum64(all), end = lane64(x, 63);
+        const int64_t all = (int64_t)tree_tiles(a, q) * n, x = scan_sum64(all), end = lane64(x, 63);
         if (w.base + 64 >= c.sequences || u - w.before < end) {
             const int l = __builtin_ctzll(__ballot(x > u - w.before) | 1ull << 63);
             auto get = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
@@ -89,24 +93,23 @@ __device__ void tree_at(const PagedView& c, const PagedTreeCall& a, TreeWalk& w,
     }
 }
 
-// A row's weights are 2^(x - reference), the reference its largest x in the first tile where it sees anything: outputs are never rescaled,
-// since a branch that does, however rarely, has the compiler move all of them between the matrix cores' and the vector registers in every
-// step (64 rows of 256 dims: 476 moves). Weights may be large: f32 sums and pairs of bf16 keep their relative precision up to 2^kRise
-// (times values of 2^60; beyond, the sums are infinite, and the careful path takes the rows). A wave that meets a larger x starts its part
-// again with the largest x so far.
-constexpr float kRise = 64.0f;
+// Up to kRows rows of a sequence over a part of its positions, rows 16 w .. of them by wave w. Scores are K times Q^T (16 x 16 x 32 MFMAs):
+// lane (c = lane % 16, g = lane / 16) holds, for row c, positions 4 g .. 4 g + 3 of 16, which are just what it supplies as B of
+// V^T times P^T, 32 positions at a time, when V's transposing LDS reads fetch the same positions: P moves between no lanes, and a
+// row's maximum, sum and outputs are its lanes'. P enters as two bf16 parts, which share V's fragments.
+// The largest of a row's values, over the four lanes that hold it: 16 and 32 lanes apart, in vector registers.
+__device__ __forceinline__ float rows_max(float x) {
+    auto pair = [](auto y) { return fmaxf(__uint_as_float(y[0]), __uint_as_float(y[1])); };
+    x = pair(__builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false));
+    return pair(__builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false));
+}
 
-// Up to kRows rows of a sequence over a part of its positions.
-template <int D, bool E4M3, int RB>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(TreeShape<D, E4M3, RB>::kHeld))) void paged_tree_kernel(
-    PagedView c, PagedTreeCall a, float* part) {
-    using T = TreeShape<D, E4M3, RB>;
-    constexpr int NT = T::kSub;
-    __shared__ __attribute__((aligned(16))) uint8_t lds[T::kLds];
-    uint16_t* qs = reinterpret_cast<uint16_t*>(lds);                   // [kRows][kQStride]
-    float* os = reinterpret_cast<float*>(lds + T::kQBytes);            // [4 waves][16][D]
-    float(*ms)[16] = reinterpret_cast<float(*)[16]>(os + 4 * 16 * D);
-    float(*ls)[16] = ms + 4;
+template <int D, bool E4M3>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void paged_tree_kernel(
+    PagedView c, PagedTreeCall a, float* part, TreeSplit* split) {
+    using T = TreeShape<D, E4M3>;
+    constexpr int kTile = T::kTile, kSteps = D / 32, kDims = D / 16;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[T::kLds];
     const int groups = gridDim.x / c.kv_heads, kvh = blockIdx.x % c.kv_heads, group = blockIdx.x / c.kv_heads;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l16 = lane & 15, g = lane >> 4;
     // x = factor (q . k): a negative factor's sign goes to q, so that the largest product is the largest x; and a factor of
@@ -114,353 +117,353 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(TreeShape<D
     const float signed_factor = E4M3 ? c.k_scale[kvh] * a.scale_log2 : a.scale_log2;
     const float factor = fabsf(signed_factor) < 1.2e-38f ? 1.2e-38f : fabsf(signed_factor);
     const uint32_t flip = signed_factor < 0.0f ? 0x80008000u : 0u;
-    TreeWalk walk = tree_walk<T::kRows>(c, a, groups, T::kTile);
+    // LDS byte addresses of a lane: K row l16, chunk 4 j + g; V's transposing reads, rows 4 g + ln / 4 % 4, chunk 2 d + ln / 2 % 2
+    const int k_at = l16 * T::kRowBytes + ((g ^ chunk_swizzle<D>(l16)) * 16);
+    const int v_row = 4 * g + (lane >> 2 & 3), v_at = v_row * T::kRowBytes + (((lane >> 1 & 1) ^ chunk_swizzle<D>(v_row)) * 16) + (lane & 1) * 8;
+    const uint32_t lds_at = (uint32_t)(uintptr_t)(lds_void*)lds;
+    TreeWalk walk = tree_walk(c, a, groups, kTile);
     const int64_t end = min(walk.units, (group + 1) * walk.q);
+    TreeSplit begun = {0, 0, 0, 0};
     for (int64_t unit = group * walk.q; unit < end;) {
         Piece t;
         int units;
         int64_t first;
-        tree_at<T::kRows>(c, a, walk, T::kTile, unit, &t, &units, &first);
+        tree_at(c, a, walk, kTile, unit, &t, &units, &first);
         const int off = (int)(unit - first), take = (int)min((int64_t)(units - off), end - unit);
         const bool whole = off == 0 && take == units;
         unit += take;
-        const int r0 = t.tile * T::kRows, nr = min(T::kRows, t.n * a.group - r0), from = token_first(a, Seq{t.row0, t.n, t.len}, T::kTile);
+        if (off == 0 && !whole) {  // at most one of a group's parts
+            const int64_t last = quotient(first + units - 1, walk.q);
+            begun = {t.row0, t.n, t.tile, (int)(last - group) + 1};
+        }
+        const int r0 = t.tile * kTreeRows, nr = min(kTreeRows, t.n * a.group - r0), from = token_first(a, Seq{t.row0, t.n, t.len}, kTile);
         const int lo = from + off * kTokenUnit, hi = (int)min((int64_t)lo + (int64_t)take * kTokenUnit, (int64_t)t.len), tree0 = t.len - t.n;
-        // as many blocks of 16 rows as there are
-        auto run = [&](auto blocks) __attribute__((always_inline)) {
-            constexpr int NB = decltype(blocks)::value;
-            __syncthreads();  // the part before has been written out
-            for (int i = threadIdx.x; i < 16 * NB * D / 8; i += 256) {
-                const int r = i / (D / 8), j = i - r * (D / 8), row = r0 + min(r, nr - 1), node = row / a.group;
-                const uint4 w = ld16(a.q + (int64_t)(t.row0 + node) * a.q_row + (kvh * a.group + row - node * a.group) * D + 8 * j);
-                *reinterpret_cast<uint4*>(qs + r * T::kQStride + 8 * j) = make_uint4(w.x ^ flip, w.y ^ flip, w.z ^ flip, w.w ^ flip);
-            }
-            int see_lo[NB], see_hi[NB], mask_row[NB];  // of row 16 b + l16; -1: no row
-            int all_lo = 0, all_hi = t.len;            // positions that all rows see
+        // the lane's row: where it lies, its query, and the positions that it, and all rows of the wave, see
+        const int wrow = 16 * wave + l16;
+        const bool is = wrow < nr, rows = 16 * wave < nr;
+        const int row = r0 + min(wrow, nr - 1), node = row / a.group, m_row = t.row0 + node, head = kvh * a.group + row - node * a.group;
+        uint4 qf[kSteps];
+        int see_lo = 0, see_hi = 0, all_lo = 0, all_hi = 0;
+        f32x4 o[kDims];
 #pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                const bool is = 16 * b + l16 < nr;
-                const Row x = row_of(a, t, kvh, r0 + min(16 * b + l16, nr - 1));
-                see_lo[b] = is ? x.lo : 0, see_hi[b] = is ? x.hi : 0, mask_row[b] = is ? (int)x.m : -1;
-                all_lo = max(all_lo, x.lo), all_hi = min(all_hi, x.hi);
-            }
-#pragma unroll
-            for (int b = 8; b > 0; b >>= 1) all_lo = max(all_lo, __shfl_xor(all_lo, b)), all_hi = min(all_hi, __shfl_xor(all_hi, b));
-            all_lo = __builtin_amdgcn_readfirstlane(all_lo), all_hi = __builtin_amdgcn_readfirstlane(all_hi);
-            __syncthreads();
+        for (int d = 0; d < kDims; ++d) o[d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        float m_run = -INFINITY, m_ref = -INFINITY, l_run = 0.0f;
+        bool bad = false;
 
-            f32x4 o[NB][T::kVB][T::kVD];
-            float m_run[NB], m_ref[NB], l_run[NB];
-#pragma unroll
-            for (int r = 0; r < NB; ++r) m_run[r] = -INFINITY;
-            bool bad = false;
-
-            const int32_t* table = c.table + t.s * c.table_stride;
-            // lane l looks after position t0 + l % kTile: its page (the next tile's is asked for a tile ahead)
-            auto page_at = [&](int t0) { return t0 < hi ? table[page_of(c, min(t0 + lane % T::kTile, hi - 1))] : 0; };
-            uint4 kf[NT][T::kKLoads];
-            Words<T::kVWords> vf[T::kVB][4 * NT];
-            int64_t koff = 0, voff = 0;
-            auto place = [&](int page, int t0) {  // offsets of the lane's position; a bad page becomes page 0, and is remembered
-                if (t0 >= hi) return;
-                const int p = min(t0 + lane % T::kTile, hi - 1);
-                const bool in = page >= 0 && page < c.pages;
-                bad |= !in;
-                page = in ? page : 0;
-                const uint32_t slot = p - page_of(c, p) * c.slots;
-                koff = page * c.k_page + slot * c.k_slot;
-                voff = page * c.v_page + slot * c.v_slot;
-            };
-            const uint8_t* kbase = c.k + kvh * c.k_head + 16 * g;
-            const uint8_t* vbase = c.v + kvh * c.v_head + l16 * T::kVD * T::kElem;
-            auto load_k = [&] {
-#pragma unroll
-                for (int i = 0; i < NT; ++i) {
-                    const uint8_t* p = kbase + __shfl(koff, 16 * i + l16, kWave);
-#pragma unroll
-                    for (int j = 0; j < T::kKLoads; ++j) kf[i][j] = ld16(p + 64 * j);
-                }
-            };
-            auto load_v = [&] {
-#pragma unroll
-                for (int i = 0; i < 4 * NT; ++i) {
-                    const uint8_t* p = vbase + __shfl(voff, 16 * (i >> 2) + 4 * g + (i & 3), kWave);
-#pragma unroll
-                    for (int b = 0; b < T::kVB; ++b) vf[b][i] = ld_words<T::kVWords>(p + 16 * T::kVD * T::kElem * b);
-                }
-            };
-
-            constexpr int kStep = 4 * T::kTile;
-            bool over = false;
-            do {
-                int t0 = lo + wave * T::kTile;
-                int page = page_at(t0), page1 = page_at(t0 + kStep);
-                place(page, t0);
-                if (t0 < hi) load_k();
-#pragma unroll
-                for (int r = 0; r < NB; ++r) {
-                    m_ref[r] = m_run[r], l_run[r] = 0.0f;
-#pragma unroll
-                    for (int b = 0; b < T::kVB; ++b)
-#pragma unroll
-                        for (int d = 0; d < T::kVD; ++d) o[r][b][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-                }
-                over = false;
-                for (; t0 < hi && !over; t0 += kStep) {
-                    load_v();
-                    if constexpr (NB * D > 256) __asm__ volatile("" ::: "memory");  // Q is read from LDS again: no registers for it
-                    f32x4 sc[NB][NT];
-#pragma unroll
-                    for (int r = 0; r < NB; ++r)
-#pragma unroll
-                        for (int i = 0; i < NT; ++i) sc[r][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-                    // Q's dims follow the order K's 16-byte loads have: bf16 dims 32 j + 8 g, E4M3 dims 64 j + 16 g, two steps a load
-#pragma unroll
-                    for (int j = 0; j < T::kKLoads; ++j)
-#pragma unroll
-                        for (int h = 0; h < (E4M3 ? 2 : 1); ++h) {
-                            bf16x8 kb[NT];
-#pragma unroll
-                            for (int i = 0; i < NT; ++i) {
-                                if constexpr (E4M3) {
-                                    const uint32_t w0 = h ? kf[i][j].z : kf[i][j].x, w1 = h ? kf[i][j].w : kf[i][j].y;
-                                    kb[i] = as_bf16x8(make_uint4(bf16_pair_of_fp8(w0), bf16_pair_of_fp8(w0 >> 16), bf16_pair_of_fp8(w1), bf16_pair_of_fp8(w1 >> 16)));
-                                } else {
-                                    kb[i] = as_bf16x8(kf[i][j]);
-                                }
-                            }
-#pragma unroll
-                            for (int r = 0; r < NB; ++r) {
-                                const bf16x8 qf = as_bf16x8(ld16(qs + (16 * r + l16) * T::kQStride + (E4M3 ? 64 * j + 16 * g + 8 * h : 32 * j + 8 * g)));
-#pragma unroll
-                                for (int i = 0; i < NT; ++i) sc[r][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kb[i], qf, sc[r][i], 0, 0, 0);
-                            }
-                        }
-                    // the next tile's K
-                    page = page1;
-                    page1 = page_at(t0 + 2 * kStep);
-                    place(page, t0 + kStep);
-                    if (t0 + kStep < hi) load_k();
-
-                    const bool some = t0 < all_lo || t0 + T::kTile > all_hi;  // some row does not see all of it
-                    uint32_t pw[NB][2 * NT][kParts];
-#pragma unroll
-                    for (int r = 0; r < NB; ++r) {
-                        // weights of row 16 r + l16 at positions t0 + 16 i + 4 g + e
-                        if (some) {
-                            const uint32_t nodes = t0 + T::kTile > tree0 && mask_row[r] >= 0 ? (uint32_t)node_bits(a, t, mask_row[r], t0) : 0;
-#pragma unroll
-                            for (int i = 0; i < NT; ++i)
-#pragma unroll
-                                for (int e = 0; e < 4; ++e) {
-                                    const int p = t0 + 16 * i + 4 * g + e;
-                                    const bool sees = (p >= see_lo[r] && p < see_hi[r]) || (nodes >> (16 * i + 4 * g + e) & 1);
-                                    sc[r][i][e] = sees ? sc[r][i][e] : -INFINITY;
-                                }
-                        }
-                        float mx = sc[r][0][0];
-#pragma unroll
-                        for (int i = 0; i < NT; ++i)
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) mx = fmaxf(mx, sc[r][i][e]);
-                        mx = fmaxf(mx, __shfl_xor(mx, 16));
-                        mx = fmaxf(mx, __shfl_xor(mx, 32));
-                        m_run[r] = fmaxf(m_run[r], mx * factor);
-                        m_ref[r] = m_ref[r] == -INFINITY ? m_run[r] : m_ref[r];
-                        over |= __any(m_run[r] > m_ref[r] + kRise);
-                        const float mu = m_ref[r] == -INFINITY ? 0.0f : m_ref[r];
-                        float sum = 0.0f;
-#pragma unroll
-                        for (int i = 0; i < NT; ++i)
-#pragma unroll
-                            for (int e = 0; e < 4; e += 2) {
-                                const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[r][i][e], factor, -mu)), p1 = __builtin_amdgcn_exp2f(fmaf(sc[r][i][e + 1], factor, -mu));
-                                sum += p0 + p1;
-                                split_weights(p0, p1, pw[r][2 * i + e / 2]);
-                            }
-                        l_run[r] += sum;
-                    }
-#pragma unroll
-                    for (int b = 0; b < T::kVB; ++b)
-#pragma unroll
-                        for (int d = 0; d < T::kVD; ++d) {
-                            uint32_t w[2 * NT];
-#pragma unroll
-                            for (int i = 0; i < 2 * NT; ++i) {
-                                if constexpr (E4M3)
-                                    w[i] = bf16_pair_of_fp8(__builtin_amdgcn_perm(vf[b][2 * i + 1].w[d / 4], vf[b][2 * i].w[d / 4],
-                                                                                  0x0c0c0000u | (4 + d % 4) << 8 | d % 4));
-                                else
-                                    w[i] = __builtin_amdgcn_perm(vf[b][2 * i + 1].w[d / 2], vf[b][2 * i].w[d / 2], d & 1 ? 0x07060302u : 0x05040100u);
-                            }
-#pragma unroll
-                            for (int r = 0; r < NB; ++r) {
-                                if constexpr (NT == 1) {
-                                    o[r][b][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(make_uint4(pw[r][0][0], pw[r][1][0], pw[r][0][1], pw[r][1][1])),
-                                                                                         as_bf16x8(make_uint4(w[0], w[1], w[0], w[1])), o[r][b][d], 0, 0, 0);
-                                } else {
-#pragma unroll
-                                    for (int p = 0; p < kParts; ++p)
-                                        o[r][b][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(make_uint4(pw[r][0][p], pw[r][1][p], pw[r][2][p], pw[r][3][p])),
-                                                                                             as_bf16x8(make_uint4(w[0], w[1], w[2], w[3])), o[r][b][d], 0, 0, 0);
-                                }
-                            }
-                        }
-                }
-            } while (over);
-
-            // the four waves' states into one, 16 rows at a time
-            bad = __syncthreads_or(bad);
-            float* rec = whole ? nullptr : part + ((int64_t)kvh * 2 * groups + 2 * group + (off == 0)) * record_floats(T::kRows, D);
-            bool odd = false;
-            const float vs = E4M3 ? c.v_scale[kvh] : 1.0f;
-#pragma unroll
-            for (int r = 0; r < NB; ++r) {
-                if (16 * r >= nr) continue;
-                if (r) __syncthreads();  // the rows before have been read
-                l_run[r] += __shfl_xor(l_run[r], 16);
-                l_run[r] += __shfl_xor(l_run[r], 32);
-                if (g == 0) ms[wave][l16] = m_ref[r], ls[wave][l16] = l_run[r];
-#pragma unroll
-                for (int b = 0; b < T::kVB; ++b)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-#pragma unroll
-                        for (int d = 0; d < T::kVD; d += 4)
-                            *reinterpret_cast<float4*>(os + ((wave * 16 + 4 * g + e) * D + 16 * T::kVD * b + T::kVD * l16 + d)) =
-                                make_float4(o[r][b][d][e], o[r][b][d + 1][e], o[r][b][d + 2][e], o[r][b][d + 3][e]);
-                __syncthreads();
-                const int here = min(16, nr - 16 * r);
-                for (int i = threadIdx.x; i < here * (D / 4); i += 256) {
-                    const int y = i / (D / 4), d = 4 * (i - y * (D / 4));
-                    const float m = fmaxf(fmaxf(ms[0][y], ms[1][y]), fmaxf(ms[2][y], ms[3][y]));
-                    float l = 0.0f, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                    for (int w = 0; w < 4; ++w) {
-                        const float f = ms[w][y] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ms[w][y] - m);
-                        const float4 z = *reinterpret_cast<const float4*>(os + (w * 16 + y) * D + d);
-                        l = fmaf(f, ls[w][y], l);
-                        v[0] = fmaf(f, z.x, v[0]), v[1] = fmaf(f, z.y, v[1]), v[2] = fmaf(f, z.z, v[2]), v[3] = fmaf(f, z.w, v[3]);
-                    }
-                    odd |= !(fabsf(v[0]) + fabsf(v[1]) + fabsf(v[2]) + fabsf(v[3]) < INFINITY);
-                    const int row = 16 * r + y;
-                    if (rec) {
-                        if (d == 0) rec[row] = bad ? NAN : m, rec[T::kRows + row] = l;
-                        *reinterpret_cast<float4*>(rec + 2 * T::kRows + row * D + d) = make_float4(v[0], v[1], v[2], v[3]);
-                    } else if (!bad) {
-                        const int node = (r0 + row) / a.group;
-                        const float inv = l == 0.0f ? 0.0f : vs / l;
-                        *reinterpret_cast<uint2*>(a.out + (int64_t)(t.row0 + node) * a.out_row + (kvh * a.group + r0 + row - node * a.group) * D + d) =
-                            make_uint2(pk_bf16(v[0] * inv, v[1] * inv), pk_bf16(v[2] * inv, v[3] * inv));
-                    }
-                }
-            }
-            odd = __syncthreads_or(odd);
-            if (bad && threadIdx.x == 0) atomicOr(c.err, kErrPaged);
-            if (odd && !bad && flip) {  // q as it was
-                for (int i = threadIdx.x; i < 16 * NB * D / 2; i += 256) reinterpret_cast<uint32_t*>(qs)[i / (D / 2) * (T::kQStride / 2) + i % (D / 2)] ^= flip;
-                __syncthreads();
-            }
-            if (odd && !bad)
-                careful_piece<E4M3>(c, a, t, kvh, r0, nr, lo, hi, [&](int r, const Row&) { return qs + r * T::kQStride; }, rec, T::kRows);
+        const int32_t* table = c.table + t.s * c.table_stride;
+        const uint8_t *kbase = c.k + kvh * c.k_head, *vbase = c.v + kvh * c.v_head;
+        // Lane l looks after position l % kWaveRows of the wave's part of tile l / kWaveRows, kGroup tiles at once; the next
+        // group's pages are asked for a group ahead.
+        const int own = lane / T::kWaveRows * kTile + wave * T::kWaveRows + lane % T::kWaveRows;
+        auto page_at = [&](int t0) { return t0 < hi ? table[page_of(c, min(t0 + own, hi - 1))] : 0; };
+        int64_t koff = 0, voff = 0;
+        auto place = [&](int page, int t0) {  // a bad page becomes page 0, and is remembered
+            const int p = min(t0 + own, hi - 1);
+            const bool in = page >= 0 && page < c.pages;
+            bad |= !in;
+            page = in ? page : 0;
+            const uint32_t slot = p - page_of(c, p) * c.slots;
+            koff = page * c.k_page + slot * c.k_slot;
+            voff = page * c.v_page + slot * c.v_slot;
         };
-        const int blocks = (nr + 15) / 16;
-        if (blocks == 1) run(std::integral_constant<int, 1>{});
-        if (blocks == 2) run(std::integral_constant<int, 2>{});
-        if constexpr (RB == 4) {
-            if (blocks == 3) run(std::integral_constant<int, 3>{});
-            if (blocks == 4) run(std::integral_constant<int, 4>{});
-        }
-    }
-}
-
-// Rows of split tiles, four in a workgroup, a wave each.
-constexpr int kTreeMergeRows = 4;
-
-// Block `want` of the rows of the tiles that are split: its sequence, tile, parts, first record and first row in the tile. False: there are
-// not that many.
-template <int R>
-__device__ bool tree_block(const PagedView& c, const PagedTreeCall& a, const TreeWalk& w, int align, int want, Piece* out) {
-    const int lane = threadIdx.x & 63;
-    bool bad = false;
-    int64_t before = 0;
-    for (int base = 0; base < c.sequences; base += 64) {
-        const Seq q = seq_of<true>(c, a, base + lane, true, &bad);
-        const int n = token_units(a, q, align), tiles = tree_tiles<R>(a, q), rows = q.n * a.group;
-        const int64_t all = (int64_t)tiles * n, x = scan_sum64(all), first = before + x - all;
-        // a sequence's tiles are split but for those that a group has whole; each is looked at below
-        int blocks = 0;
-        for (int i = 0; i < tiles; ++i) {
-            const int64_t u = first + (int64_t)i * n;
-            if (quotient(u, w.q) != quotient(u + n - 1, w.q)) blocks += (min(R, rows - i * R) + kTreeMergeRows - 1) / kTreeMergeRows;
-        }
-        const int xb = scan_sum(blocks);
-        const uint64_t hit = __ballot(xb > want);
-        if (hit) {
-            const int l = __builtin_ctzll(hit);
-            auto get = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
-            int left = want - get(xb - blocks);
-            const int64_t u0 = lane64(first, l);
-            const int un = get(n), ur = get(rows);
-            for (int i = 0;; ++i) {
-                const int64_t u = u0 + (int64_t)i * un, w0 = quotient(u, w.q), w1 = quotient(u + un - 1, w.q);
-                if (w0 == w1) continue;
-                const int here = (min(R, ur - i * R) + kTreeMergeRows - 1) / kTreeMergeRows;
-                if (left < here) {
-                    *out = {base + l, get(q.row0), get(q.n), get(q.len), i, 0, (int)(w1 - w0) + 1, (int)(2 * w0), left * kTreeMergeRows};
-                    return true;
+        int page = 0, ti = 0, look = lo;  // the next group's pages; the next tile's place in its group, and its first position
+        auto look_up = [&] {             // before each tile's loads
+            if (ti == T::kGroup) {
+                ti = 0;
+                place(page, look);
+                page = page_at(look + T::kGroup * kTile);
+            }
+        };
+        // bf16: the wave's part of the next tile, straight into LDS
+        auto load_tile = [&](uint32_t stage) __attribute__((always_inline)) {
+            look_up();
+            constexpr int kLanes = 64 / T::kRowsPerLoad;  // lanes of a row
+            const int src0 = ti * T::kWaveRows + lane / kLanes;
+#pragma unroll
+            for (int i = 0; i < T::kLoads; ++i) {
+                const int row = wave * T::kWaveRows + i * T::kRowsPerLoad;
+                const int at = ((lane % kLanes) ^ chunk_swizzle<D>(row + lane / kLanes)) * 16, src = src0 + i * T::kRowsPerLoad;
+                const uint32_t kd = lds_at + stage + row * T::kRowBytes, vd = kd + T::kStage / 2;
+                if (c.near) {
+                    const uint32_t ko = (uint32_t)__shfl((int)koff, src, kWave);
+                    const uint32_t vo = c.alike ? ko : (uint32_t)__shfl((int)voff, src, kWave);
+                    load_to_lds(kbase, ko + at, kd);
+                    load_to_lds(vbase, vo + at, vd);
+                } else {
+                    load_to_lds(kbase + __shfl(koff, src, kWave) + at, kd);
+                    load_to_lds(vbase + __shfl(voff, src, kWave) + at, vd);
                 }
-                left -= here;
+            }
+            ++ti, look += kTile;
+        };
+        // E4M3: the same positions' codes into registers, 16 a load, and from there into LDS as bf16
+        struct Codes { uint4 k[T::kCodeLoads], v[T::kCodeLoads]; };
+        constexpr int kCodeLanes = D / 16, kCodeRows = 64 / kCodeLanes;  // lanes of a row, rows of a load
+        auto load_codes = [&](Codes& x) __attribute__((always_inline)) {
+            look_up();
+#pragma unroll
+            for (int j = 0; j < T::kCodeLoads; ++j) {
+                const int src = ti * T::kWaveRows + j * kCodeRows + lane / kCodeLanes, at = lane % kCodeLanes * 16;
+                x.k[j] = ld16(kbase + __shfl(koff, src, kWave) + at);
+                x.v[j] = ld16(vbase + __shfl(voff, src, kWave) + at);
+            }
+            ++ti, look += kTile;
+        };
+        auto store_codes = [&](const Codes& x, uint8_t* kd) __attribute__((always_inline)) {
+            auto put = [&](uint8_t* d, const uint4& w, int row, int col) {
+                *reinterpret_cast<uint4*>(d + row * T::kRowBytes + ((2 * col) ^ chunk_swizzle<D>(row)) * 16) =
+                    make_uint4(bf16_pair_of_fp8(w.x), bf16_pair_of_fp8(w.x >> 16), bf16_pair_of_fp8(w.y), bf16_pair_of_fp8(w.y >> 16));
+                *reinterpret_cast<uint4*>(d + row * T::kRowBytes + ((2 * col + 1) ^ chunk_swizzle<D>(row)) * 16) =
+                    make_uint4(bf16_pair_of_fp8(w.z), bf16_pair_of_fp8(w.z >> 16), bf16_pair_of_fp8(w.w), bf16_pair_of_fp8(w.w >> 16));
+            };
+#pragma unroll
+            for (int j = 0; j < T::kCodeLoads; ++j) {
+                const int row = wave * T::kWaveRows + j * kCodeRows + lane / kCodeLanes, col = lane % kCodeLanes;
+                put(kd, x.k[j], row, col);
+                put(kd + T::kStage / 2, x.v[j], row, col);
+            }
+        };
+
+        // the tile of positions t0 .. in LDS at `tile`, 16 positions at a time
+        auto compute = [&](const uint8_t* tile, int t0) __attribute__((always_inline)) {
+            if (!rows) return;
+            // fragments are read kAhead steps before their MFMAs, in an order that the compiler keeps (left to it, each is waited for at once)
+            f32x4 sc[T::kSub];
+            {
+                constexpr int kAhead = 2;
+                bf16x8 kf[kAhead][T::kSub];
+                auto read_k = [&](int s) __attribute__((always_inline)) {
+#pragma unroll
+                    for (int b = 0; b < T::kSub; ++b)
+                        kf[s % kAhead][b] = *reinterpret_cast<const bf16x8*>(tile + (k_at ^ (64 * (s & (D == 64 ? 1 : 3)))) + (D == 64 ? 0 : 256 * (s >> 2)) +
+                                                                             16 * b * T::kRowBytes);
+                };
+#pragma unroll
+                for (int b = 0; b < T::kSub; ++b) sc[b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int s = 0; s < kAhead; ++s) read_k(s);
+#pragma unroll
+                for (int s = 0; s < kSteps; ++s) {
+#pragma unroll
+                    for (int b = 0; b < T::kSub; ++b) sc[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[s % kAhead][b], as_bf16x8(qf[s]), sc[b], 0, 0, 0);
+                    if (s + kAhead < kSteps) read_k(s + kAhead);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+            if (t0 < all_lo || t0 + kTile > all_hi) {  // some row does not see all of it
+                const uint64_t nodes = t0 + kTile > tree0 && t0 < hi && is ? node_bits(a, t, m_row, t0) : 0;
+#pragma unroll
+                for (int b = 0; b < T::kSub; ++b)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int at = 16 * b + 4 * g + e, p = t0 + at;
+                        const bool sees = (p >= see_lo && p < see_hi) || (nodes >> at & 1);
+                        sc[b][e] = sees ? sc[b][e] : -INFINITY;
+                    }
+            }
+            float mx = -INFINITY;
+#pragma unroll
+            for (int b = 0; b < T::kSub; ++b)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) mx = fmaxf(mx, sc[b][e]);
+            mx = rows_max(mx);
+            m_run = fmaxf(m_run, mx * factor);
+            float scale = 1.0f;
+            if (m_run > m_ref + kSlack) {
+                scale = m_ref == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m_ref - m_run);  // -inf: sum and out are zero
+                m_ref = m_run;
+            }
+            if (__any(scale != 1.0f)) {
+#pragma unroll
+                for (int d = 0; d < kDims; ++d)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[d][e] *= scale;
+            }
+            const float mu = m_ref == -INFINITY ? 0.0f : m_ref;
+            float sum = 0.0f;
+            // step n: positions 32 (n / kDims) .., dims 16 (n % kDims) ..; the first V fragments are read beside the weights
+            constexpr int kAhead = 4, kN = T::kSub / 2 * kDims;
+            s16x4 vr[kAhead][2];
+            auto read_v = [&](int n) __attribute__((always_inline)) {
+                const int d = n % kDims, u = n / kDims;
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    vr[n % kAhead][i] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(tile + T::kStage / 2 + (v_at ^ (32 * (d & (D == 64 ? 3 : 7)))) +
+                                                                                              (D == 64 ? 0 : 256 * (d >> 3)) + 16 * (2 * u + i) * T::kRowBytes));
+            };
+#pragma unroll
+            for (int n = 0; n < kAhead; ++n) read_v(n);
+            __builtin_amdgcn_sched_barrier(0);
+            uint32_t pw[T::kSub][2][kParts];
+#pragma unroll
+            for (int b = 0; b < T::kSub; ++b)
+#pragma unroll
+                for (int e = 0; e < 4; e += 2) {
+                    const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[b][e], factor, -mu)), p1 = __builtin_amdgcn_exp2f(fmaf(sc[b][e + 1], factor, -mu));
+                    sum += p0 + p1;
+                    split_weights(p0, p1, pw[b][e / 2]);
+                }
+#pragma unroll
+            for (int n = 0; n < kN; ++n) {
+                const int d = n % kDims, b = 2 * (n / kDims);
+                const bf16x8 vf = __builtin_bit_cast(bf16x8, __builtin_shufflevector(vr[n % kAhead][0], vr[n % kAhead][1], 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+                for (int p = 0; p < kParts; ++p)
+                    o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, as_bf16x8(make_uint4(pw[b][0][p], pw[b][1][p], pw[b + 1][0][p], pw[b + 1][1][p])), o[d],
+                                                                   0, 0, 0);
+                if (n + kAhead < kN) read_v(n + kAhead);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            l_run = fmaf(l_run, scale, sum);
+        };
+
+        const int tiles = (hi - lo + kTile - 1) / kTile;
+        // what the part reads of its rows is asked for ahead of its tiles, and looked at when those are on their way
+        uint64_t mask[kTreeMaxWords];
+        {
+            const uint16_t* qp = a.q + (int64_t)m_row * a.q_row + head * D + 8 * g;
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s) qf[s] = ld16(qp + 32 * s);
+#pragma unroll
+            for (int w = 0; w < kTreeMaxWords; ++w) mask[w] = w < a.words ? a.masks[(int64_t)m_row * a.words + w] : 0;
+        }
+        if (tiles > 0) {
+            place(page_at(lo), lo);
+            page = page_at(lo + T::kGroup * kTile);
+        }
+        __syncthreads();  // the part before has read its flags
+        Codes codes[E4M3 ? T::kAhead : 1];
+        constexpr int kFlight = T::kStages - 2;  // bf16: tiles whose loads may be on their way while a tile is used
+        if (tiles > 0) {
+            if constexpr (E4M3) {
+#pragma unroll
+                for (int s = 0; s < T::kAhead; ++s) load_codes(codes[s]);
+            } else {
+                for (int s = 0; s <= kFlight && s < tiles; ++s) load_tile(s * T::kStage);
             }
         }
-        want -= __builtin_amdgcn_readlane(xb, 63);
-        before += lane64(x, 63);
+        {
+            int depth = 0;
+#pragma unroll
+            for (int w = 0; w < kTreeMaxWords; ++w) {
+                const int left = t.n - 64 * w;
+                if (left > 0) depth += __popcll(mask[w] & (left >= 64 ? ~0ull : (1ull << left) - 1));
+            }
+            const int place = tree0 + depth - 1, from_here = a.window && place >= a.window ? place - a.window + 1 : 0;
+            see_lo = all_lo = from_here, see_hi = all_hi = depth ? min(max(tree0, 0), hi) : 0;
+            if (!is) see_lo = see_hi = 0;
+#pragma unroll
+            for (int x = 8; x > 0; x >>= 1) all_lo = max(all_lo, __shfl_xor(all_lo, x)), all_hi = min(all_hi, __shfl_xor(all_hi, x));
+            all_lo = __builtin_amdgcn_readfirstlane(all_lo), all_hi = __builtin_amdgcn_readfirstlane(all_hi);
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s) qf[s] = make_uint4(qf[s].x ^ flip, qf[s].y ^ flip, qf[s].z ^ flip, qf[s].w ^ flip);
+        }
+        if constexpr (E4M3) {
+            // kAhead tiles a turn, the last of them perhaps behind the part
+            for (int i = 0; i < tiles; i += T::kAhead) {
+#pragma unroll
+                for (int s = 0; s < T::kAhead; ++s) {
+                    uint8_t* tile = lds + (s & 1) * T::kStage;  // read by all two tiles ago
+                    store_codes(codes[s], tile);
+                    load_codes(codes[s]);
+                    __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                    __builtin_amdgcn_s_barrier();
+                    __asm__ volatile("" ::: "memory");
+                    if (i + s < tiles) compute(tile, lo + (i + s) * kTile);
+                }
+            }
+        } else {
+            uint32_t at = 0, into = (T::kStages - 1) * T::kStage;
+            for (int i = 0; i < tiles; ++i) {
+                // this wave's loads of the tile are done, and then everybody's; and everybody has read the tile before it
+                if (i + kFlight < tiles) __asm__ volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(kFlight * 2 * T::kLoads) : "memory");
+                else __asm__ volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+                __builtin_amdgcn_s_barrier();
+                __asm__ volatile("" ::: "memory");
+                if (i + T::kStages - 1 < tiles) load_tile(into);
+                compute(lds + at, lo + i * kTile);
+                into = at;
+                at = at + T::kStage == T::kStages * T::kStage ? 0 : at + T::kStage;
+            }
+        }
+
+        l_run += __shfl_xor(l_run, 16);
+        l_run += __shfl_xor(l_run, 32);
+        float most = 0.0f;
+#pragma unroll
+        for (int d = 0; d < kDims; ++d)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) most += fabsf(o[d][e]);
+        uint32_t* flags = reinterpret_cast<uint32_t*>(lds);
+        const uint32_t wave_flags = (__any(bad) ? 1u : 0u) | (__any(is && !(most < INFINITY)) ? 2u : 0u);
+        __syncthreads();  // the last tile has been read
+        if (lane == 0) flags[wave] = wave_flags;
+        __syncthreads();
+        uint32_t all = 0;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) all |= flags[w];
+        bad = all & 1;
+        const bool odd = all & 2;  // the careful path writes, and reads q, which may be out
+        float* rec = whole ? nullptr : part + ((int64_t)kvh * 2 * groups + 2 * group + (off == 0)) * record_floats(kTreeRows, D);
+        if (is && (bad || !odd)) {
+            if (rec) {
+                float* to = rec + 2 * kTreeRows + wrow * D + 4 * g;
+#pragma unroll
+                for (int d = 0; d < kDims; ++d) *reinterpret_cast<float4*>(to + 16 * d) = make_float4(o[d][0], o[d][1], o[d][2], o[d][3]);
+                if (g == 0) rec[wrow] = bad ? NAN : m_ref, rec[kTreeRows + wrow] = l_run;
+            } else if (!bad) {
+                const float inv = l_run == 0.0f ? 0.0f : (E4M3 ? c.v_scale[kvh] : 1.0f) / l_run;
+                uint16_t* to = a.out + (int64_t)m_row * a.out_row + head * D + 4 * g;
+#pragma unroll
+                for (int d = 0; d < kDims; ++d)
+                    *reinterpret_cast<uint2*>(to + 16 * d) = make_uint2(pk_bf16(o[d][0] * inv, o[d][1] * inv), pk_bf16(o[d][2] * inv, o[d][3] * inv));
+            }
+        }
+        if (bad && threadIdx.x == 0) atomicOr(c.err, kErrPaged);
+        if (odd && !bad)
+            careful_piece<E4M3>(c, a, t, kvh, r0, nr, lo, hi, [&](int, const Row& x) { return a.q + x.m * a.q_row + x.h * D; }, rec, kTreeRows);
     }
-    return false;
+    if (threadIdx.x == 0) split[kvh * groups + group] = begun;
 }
 
-template <int D, bool E4M3, int RB>
-__global__ __launch_bounds__(256) void paged_tree_merge_kernel(PagedView c, PagedTreeCall a, int groups, const float* part) {
-    using T = TreeShape<D, E4M3, RB>;
-    const int kvh = blockIdx.x % c.kv_heads;
-    const TreeWalk walk = tree_walk<T::kRows>(c, a, groups, T::kTile);
-    const int64_t size = record_floats(T::kRows, D);
-    Piece t;
-    for (int u = blockIdx.x / c.kv_heads; tree_block<T::kRows>(c, a, walk, T::kTile, u, &t); u += gridDim.x / c.kv_heads) {
-        const float* base = part + ((int64_t)kvh * 2 * groups + t.record) * size;
-        auto rec = [&](int j) { return base + (2 * j + (j == 0)) * size; };
-        const int r = t.row + (threadIdx.x >> 6), row = t.tile * T::kRows + r;
-        if (r < T::kRows && row < t.n * a.group) merge_row<D, E4M3>(c, a, t, kvh, rec, T::kRows, r, row);
+// Rows of split tiles, eight in a workgroup, two for each wave.
+constexpr int kTreeMergeRows = 8;
+
+template <int D, bool E4M3>
+__global__ __launch_bounds__(256) void paged_tree_merge_kernel(PagedView c, PagedTreeCall a, int groups, const float* part, const TreeSplit* split) {
+    const int kvh = blockIdx.x % c.kv_heads, u = blockIdx.x / c.kv_heads, group = u / (kTreeRows / kTreeMergeRows);
+    const TreeSplit s = split[kvh * groups + group];
+    const int64_t size = record_floats(kTreeRows, D);
+    const float* base = part + ((int64_t)kvh * 2 * groups + 2 * group) * size;
+    auto rec = [&](int j) { return base + (2 * j + (j == 0)) * size; };
+    const Piece t = {0, s.row0, s.n, 0, s.tile, 0, s.parts, 0, 0};
+    for (int i = threadIdx.x >> 6; i < kTreeMergeRows; i += 4) {
+        const int r = u % (kTreeRows / kTreeMergeRows) * kTreeMergeRows + i, row = s.tile * kTreeRows + r;
+        if (s.parts > 1 && row < s.n * a.group) merge_row<D, E4M3>(c, a, t, kvh, rec, kTreeRows, r, row);
     }
 }
 
-template <int D, bool E4M3, int RB>
+template <int D, bool E4M3>
 hipError_t launch_tree(const PagedView& c, const PagedTreeCall& a, hipStream_t s, DevCtx* ctx) {
-    using T = TreeShape<D, E4M3, RB>;
+    using T = TreeShape<D, E4M3>;
     const int heads = c.kv_heads;
     const int64_t capacity = (int64_t)c.columns * c.slots, sequences = std::min(c.sequences, a.rows);
     const int64_t units = (a.window ? std::min<int64_t>(capacity, (int64_t)a.window + a.max_rows + kTokenUnit) : capacity) / kTokenUnit + 1;
-    const int64_t tiles = (int64_t)a.rows * a.group / T::kRows + sequences;
-    const int64_t most = (int64_t)kPagedChunkFloats / record_floats(T::kRows, D) / heads / 2;
-    const int groups = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>((int64_t)ctx->cus * T::kHeld / heads, tiles * units), most));
-    hipLaunchKernelGGL((paged_tree_kernel<D, E4M3, RB>), dim3((uint32_t)(groups * heads)), dim3(256), 0, s, c, a, ctx->paged_chunks);
+    const int64_t tiles = (int64_t)a.rows * a.group / kTreeRows + sequences;
+    const int64_t most = (int64_t)kPagedChunkFloats / record_floats(kTreeRows, D) / heads / 2;
+    const int groups = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>((int64_t)ctx->cus * 2 / heads, tiles * units), most));
+    TreeSplit* split = reinterpret_cast<TreeSplit*>(ctx->paged_tokens);
+    hipLaunchKernelGGL((paged_tree_kernel<D, E4M3>), dim3((uint32_t)(groups * heads)), dim3(256), 0, s, c, a, ctx->paged_chunks, split);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || groups == 1) return e;
-    // a split tile has a cut between two groups
-    const int64_t blocks = std::min<int64_t>((int64_t)(groups - 1) * (T::kRows / kTreeMergeRows), (int64_t)a.rows * a.group / kTreeMergeRows + tiles);
-    const int64_t wgs = std::min<int64_t>(blocks, std::max(1, 2048 / heads));
-    hipLaunchKernelGGL((paged_tree_merge_kernel<D, E4M3, RB>), dim3((uint32_t)(wgs * heads)), dim3(256), 0, s, c, a, groups, ctx->paged_chunks);
+    hipLaunchKernelGGL((paged_tree_merge_kernel<D, E4M3>), dim3((uint32_t)(groups * (kTreeRows / kTreeMergeRows) * heads)), dim3(256), 0, s, c, a, groups,
+                       ctx->paged_chunks, split);
     return hipGetLastError();
 }
 
-template <int D, int RB>
-hipError_t launch_type(const PagedView& c, const PagedTreeCall& a, hipStream_t s, DevCtx* ctx) {
-    return c.k_scale ? launch_tree<D, true, RB>(c, a, s, ctx) : launch_tree<D, false, RB>(c, a, s, ctx);
-}
-
 template <int D>
-hipError_t launch_rows(const PagedView& c, const PagedTreeCall& a, hipStream_t s, DevCtx* ctx) {
-    return a.max_rows * a.group <= 32 ? launch_type<D, 2>(c, a, s, ctx) : launch_type<D, 4>(c, a, s, ctx);
+hipError_t launch_type(const PagedView& c, const PagedTreeCall& a, hipStream_t s, DevCtx* ctx) {
+    return c.k_scale ? launch_tree<D, true>(c, a, s, ctx) : launch_tree<D, false>(c, a, s, ctx);
 }
 
 }  // namespace
@@ -469,9 +472,9 @@ hipError_t launch_paged_tree_attention(const PagedView& c, const PagedTreeCall& 
     const int rows = a.max_rows * a.group;
     if (rows <= kTokenRows || rows > kTreeMaxRows || c.head_dim > 256) return launch_paged_tree_rows(c, a, s, ctx);
     switch (c.head_dim) {
-        case 64: return launch_rows<64>(c, a, s, ctx);
-        case 128: return launch_rows<128>(c, a, s, ctx);
-        default: return launch_rows<256>(c, a, s, ctx);
+        case 64: return launch_type<64>(c, a, s, ctx);
+        case 128: return launch_type<128>(c, a, s, ctx);
+        default: return launch_type<256>(c, a, s, ctx);
     }
 }
 
