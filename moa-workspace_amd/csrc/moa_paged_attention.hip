@@ -123,6 +123,47 @@ __device__ __forceinline__ int chunk_units(const A& a, const Seq& q) {
     return max(1, (seen + kChunkUnit - 1) / kChunkUnit);
 }
 
+// Trees: a sequence's tiles all see its whole length, so few sizes of tiles are many, and an even share of the work, rounded up for each of
+// them, leaves workgroups idle (12 sequences of 5 to 8 tiles over 900 to 16000 positions of 512 dims: parts of two even shares, 580 us).
+// Lane j tries parts as long as the longest tile's j + 1-th: those whose workgroups run at once take a part's time, others their sum's share and half a
+// part's more; a part costs kTreePartUnits besides (its start, its record, the merge). The best that leaves few enough records is taken.
+constexpr float kTreePartUnits = 6.0f;
+__device__ int tree_part_units(const PagedView& c, const PagedTreeCall& a, const ChunkPlan& p, const Seq& last) {
+    const int lane = threadIdx.x & 63;
+    bool bad = false;
+    int longest = 0;
+    float sum = 0.0f;
+    auto lanes_of = [&](int base) { return c.sequences <= 64 ? last : seq_of(c, a, base + lane, false, &bad); };
+    for (int base = 0; base < c.sequences; base += 64) {
+        const Seq q = lanes_of(base);
+        const int tiles = chunk_tiles(a, q);
+        if (tiles) longest = max(longest, chunk_units(a, q));
+        sum += tiles ? (float)tiles * (float)chunk_units(a, q) : 0.0f;
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) longest = max(longest, __shfl_xor(longest, o, kWave));
+    sum = wave_sum(sum);
+    const int part = max((longest + lane) / (lane + 1), kChunkMinUnits);
+    float items = 0.0f, records = 0.0f;  // whole numbers; those beyond 2^24 are too many
+    for (int base = 0; base < c.sequences; base += 64) {
+        const Seq q = lanes_of(base);
+        const int tiles = chunk_tiles(a, q), units = tiles ? chunk_units(a, q) : 0;
+        for (uint64_t left = __ballot(tiles > 0); left; left &= left - 1) {
+            const int l = __builtin_ctzll(left), n = __builtin_amdgcn_readlane(tiles, l), u = __builtin_amdgcn_readlane(units, l);
+            const int splits = (int)((uint32_t)(u + part - 1) / (uint32_t)part);
+            items += (float)n * (float)splits;
+            if (splits > 1) records += (float)n * (float)splits;
+        }
+    }
+    const float slots = (float)p.items;
+    float cost = items <= slots ? (float)part + kTreePartUnits : sum / slots + 0.5f * (float)part + kTreePartUnits * items / slots;
+    if (records > slots) cost = INFINITY;  // (lane 0 splits nothing)
+    float best = cost;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) best = fminf(best, __shfl_xor(best, o, kWave));
+    return __builtin_amdgcn_readlane(part, __builtin_ctzll(__ballot(cost == best)));
+}
+
 // last: the last 64 sequences' lanes, the only ones of most calls.
 template <class A>
 __device__ ChunkWalk chunk_walk(const PagedView& c, const A& a, const ChunkPlan& p, Seq* last) {
@@ -143,6 +184,7 @@ __device__ ChunkWalk chunk_walk(const PagedView& c, const A& a, const ChunkPlan&
     bad |= tiles > p.most - p.items;
     raise_bad(c, bad);
     if (tiles == 0 || tiles > p.most - p.items) return {0, 0, 0, 0};
+    if constexpr (kTree<A>) return {tree_part_units(c, a, p, *last), 0, 0, 0};
     return {__builtin_amdgcn_readfirstlane(chunk_part_units(wave_sum(units), p.items)), 0, 0, 0};  // the same in every wave
 }
 
