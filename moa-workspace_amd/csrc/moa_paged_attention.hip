@@ -125,8 +125,8 @@ __device__ __forceinline__ int chunk_units(const A& a, const Seq& q) {
 
 // Trees: a sequence's tiles all see its whole length, so few sizes of tiles are many, and an even share of the work, rounded up for each of
 // them, leaves workgroups idle (12 sequences of 5 to 8 tiles over 900 to 16000 positions of 512 dims: parts of two even shares, 580 us).
-// Lane j tries parts as long as the longest tile's j + 1-th: those whose workgroups run at once take a part's time, others their sum's share and half a
-// part's more; a part costs kTreePartUnits besides (its start, its record, the merge). The best that leaves few enough records is taken.
+// Each lane tries a fraction of the longest tile, 1 to 1/8.75 in fine steps and on to 1/258: parts that run all at once take one part's time, others their
+// sum's share and half a part's more; a part costs kTreePartUnits besides (its start, its record, the merge). The best that leaves few enough records is taken.
 constexpr float kTreePartUnits = 6.0f;
 __device__ int tree_part_units(const PagedView& c, const PagedTreeCall& a, const ChunkPlan& p, const Seq& last) {
     const int lane = threadIdx.x & 63;
@@ -143,7 +143,8 @@ __device__ int tree_part_units(const PagedView& c, const PagedTreeCall& a, const
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) longest = max(longest, __shfl_xor(longest, o, kWave));
     sum = wave_sum(sum);
-    const int part = max((longest + lane) / (lane + 1), kChunkMinUnits);
+    const float in = lane < 32 ? 1.0f + 0.25f * (float)lane : 9.0f * __builtin_amdgcn_exp2f((float)(lane - 32) * 0.15625f);
+    const int part = max((int)ceilf((float)longest / in), kChunkMinUnits);  // lane 0: all (units have 24 bits)
     float items = 0.0f, records = 0.0f;  // whole numbers; those beyond 2^24 are too many
     for (int base = 0; base < c.sequences; base += 64) {
         const Seq q = lanes_of(base);
