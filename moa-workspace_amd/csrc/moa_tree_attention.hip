@@ -23,8 +23,9 @@ struct TreeWalk {
     Seq last;          // the last 64 sequences' lanes, the only ones of most calls
 };
 
-// A split tile, for the merge: its sequence's rows, its number there, its parts. A group begins one at most: its last.
-struct TreeSplit { int row0, n, tile, parts; };
+// A split tile, for the merge: its sequence's rows, its number there, its parts and the group that begins it. A group is in two at
+// most: the one that its first part goes on with, and the one that its last part begins.
+struct TreeSplit { int row0, n, tile, parts, first, unused[3]; };
 
 // Inclusive sums of numbers below 2^50: the low 20 bits and the others apart.
 __device__ __forceinline__ int64_t scan_sum64(int64_t x) { return ((int64_t)scan_sum((int)(x >> 20)) << 20) + scan_sum((int)(x & 0xfffff)); }
@@ -81,7 +82,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void p
     const int groups = gridDim.x / c.kv_heads, kvh = blockIdx.x % c.kv_heads, group = blockIdx.x / c.kv_heads;
     TreeWalk walk = tree_walk(c, a, groups, T::kTile);
     const int64_t end = min(walk.units, (group + 1) * walk.q);
-    TreeSplit begun = {0, 0, 0, 0};
+    TreeSplit begun = {0, 0, 0, 0, 0, {}}, inside = begun;
     for (int64_t unit = group * walk.q; unit < end;) {
         Piece t;
         int units;
@@ -90,30 +91,93 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void p
         const int off = (int)(unit - first), take = (int)min((int64_t)(units - off), end - unit);
         const bool whole = off == 0 && take == units;
         unit += take;
-        if (off == 0 && !whole) begun = {t.row0, t.n, t.tile, (int)(quotient(first + units - 1, walk.q) - group) + 1};  // at most once
+        if (!whole) {
+            const int w0 = (int)quotient(first, walk.q);
+            (off == 0 ? begun : inside) = {t.row0, t.n, t.tile, (int)quotient(first + units - 1, walk.q) - w0 + 1, w0, {}};
+        }
         const int lo = token_first(a, Seq{t.row0, t.n, t.len}, T::kTile) + off * kTokenUnit;
         const int hi = (int)min((int64_t)lo + (int64_t)take * kTokenUnit, (int64_t)t.len);
         float* rec = whole ? nullptr : part + ((int64_t)kvh * 2 * groups + 2 * group + (off == 0)) * record_floats(T::kRows, D);
         tree_rows<D, E4M3>(c, a, t, kvh, lo, hi, rec, lds);
     }
-    if (threadIdx.x == 0) split[kvh * groups + group] = begun;
+    if (threadIdx.x == 0) split[2 * (kvh * groups + group)] = begun, split[2 * (kvh * groups + group) + 1] = inside;
 }
 
-// Rows of split tiles, eight in a workgroup, two for each wave.
-constexpr int kTreeMergeRows = 8;
+// The rows of a split tile are dealt out to kTreeMergeBlocks workgroups for each of its parts. Few parts: a wave takes a row. More: the four
+// waves take a row's records in turn, eight at once, and join what they have in LDS.
+constexpr int kTreeMergeBlocks = 8;
+
+template <int D, bool E4M3>
+__device__ __forceinline__ void tree_merge(const PagedView& c, const PagedTreeCall& a, const TreeSplit& s, int kvh, const float* base, int block) {
+    constexpr int kPer = D / 64;  // dims of a lane
+    __shared__ float vs[4][D], ms[4], ls[4];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, blocks = kTreeMergeBlocks * s.parts, rows = min(kTreeRows, s.n * a.group - s.tile * kTreeRows);
+    auto rec = [&](int j) { return base + (2 * j + (j == 0)) * record_floats(kTreeRows, D); };
+    const Piece t = {0, s.row0, s.n, 0, s.tile, 0, s.parts, 0, 0};
+    if (s.parts <= 4) {
+        for (int r = block + wave * blocks; r < rows; r += 4 * blocks) merge_row<D, E4M3>(c, a, t, kvh, rec, kTreeRows, r, s.tile * kTreeRows + r);
+        return;
+    }
+    for (int r = block; r < rows; r += blocks) {
+        float m = -INFINITY, l = 0.0f, v[kPer] = {};
+        bool bad = false;
+        constexpr int K = 8;
+        for (int j0 = wave; j0 < s.parts; j0 += 4 * K) {
+            float x[K], y[K], w[K][kPer], most = m;
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                const float* at = rec(min(j0 + 4 * k, s.parts - 1));
+                x[k] = j0 + 4 * k < s.parts ? at[r] : -INFINITY;
+                y[k] = at[kTreeRows + r];
+#pragma unroll
+                for (int i = 0; i < kPer; ++i) w[k][i] = at[2 * kTreeRows + r * D + lane * kPer + i];
+            }
+#pragma unroll
+            for (int k = 0; k < K; ++k) bad |= x[k] != x[k], most = fmaxf(most, x[k]);
+            const float g = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - most);
+            m = most, l *= g;
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) v[i] *= g;
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                if (j0 + 4 * k >= s.parts) continue;
+                // (a record of no weight counts too: sums that are NaN for a row's own values make the row NaN)
+                const float f = x[k] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x[k] - m);
+                l = fmaf(f, y[k], l);
+#pragma unroll
+                for (int i = 0; i < kPer; ++i) v[i] = fmaf(f, w[k][i], v[i]);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) vs[wave][lane * kPer + i] = v[i];
+        if (lane == 0) ms[wave] = bad ? NAN : m, ls[wave] = l;
+        __syncthreads();
+        bad = false, m = -INFINITY, l = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) bad |= ms[w] != ms[w], m = fmaxf(m, ms[w]);
+        if (!bad && (int)threadIdx.x < D) {
+            float o = 0.0f;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const float f = ms[w] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ms[w] - m);
+                l = fmaf(f, ls[w], l);
+                o = fmaf(f, vs[w][threadIdx.x], o);
+            }
+            const int row = s.tile * kTreeRows + r, node = row / a.group;
+            a.out[(int64_t)(s.row0 + node) * a.out_row + (kvh * a.group + row - node * a.group) * D + threadIdx.x] =
+                (uint16_t)f2bf(l == 0.0f ? 0.0f : o * ((E4M3 ? c.v_scale[kvh] : 1.0f) / l));
+        }
+        __syncthreads();  // the next row's
+    }
+}
 
 template <int D, bool E4M3>
 __global__ __launch_bounds__(256) void paged_tree_merge_kernel(PagedView c, PagedTreeCall a, int groups, const float* part, const TreeSplit* split) {
-    const int kvh = blockIdx.x % c.kv_heads, u = blockIdx.x / c.kv_heads, group = u / (kTreeRows / kTreeMergeRows);
-    const TreeSplit s = split[kvh * groups + group];
-    const int64_t size = record_floats(kTreeRows, D);
-    const float* base = part + ((int64_t)kvh * 2 * groups + 2 * group) * size;
-    auto rec = [&](int j) { return base + (2 * j + (j == 0)) * size; };
-    const Piece t = {0, s.row0, s.n, 0, s.tile, 0, s.parts, 0, 0};
-    for (int i = threadIdx.x >> 6; i < kTreeMergeRows; i += 4) {
-        const int r = u % (kTreeRows / kTreeMergeRows) * kTreeMergeRows + i, row = s.tile * kTreeRows + r;
-        if (s.parts > 1 && row < s.n * a.group) merge_row<D, E4M3>(c, a, t, kvh, rec, kTreeRows, r, row);
-    }
+    const int kvh = blockIdx.x % c.kv_heads, u = blockIdx.x / c.kv_heads, group = u / kTreeMergeBlocks;
+    const float* records = part + (int64_t)kvh * 2 * groups * record_floats(kTreeRows, D);
+    const TreeSplit mine[2] = {split[2 * (kvh * groups + group)], split[2 * (kvh * groups + group) + 1]};
+    for (const TreeSplit& s : mine)
+        if (s.parts) tree_merge<D, E4M3>(c, a, s, kvh, records + 2 * (int64_t)s.first * record_floats(kTreeRows, D), (group - s.first) * kTreeMergeBlocks + u % kTreeMergeBlocks);
 }
 
 template <int D, bool E4M3>
@@ -128,7 +192,7 @@ hipError_t launch_tree(const PagedView& c, const PagedTreeCall& a, hipStream_t s
     hipLaunchKernelGGL((paged_tree_kernel<D, E4M3>), dim3((uint32_t)(groups * heads)), dim3(256), 0, s, c, a, ctx->paged_chunks, split);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || groups == 1) return e;
-    hipLaunchKernelGGL((paged_tree_merge_kernel<D, E4M3>), dim3((uint32_t)(groups * (kTreeRows / kTreeMergeRows) * heads)), dim3(256), 0, s, c, a, groups,
+    hipLaunchKernelGGL((paged_tree_merge_kernel<D, E4M3>), dim3((uint32_t)(groups * kTreeMergeBlocks * heads)), dim3(256), 0, s, c, a, groups,
                        ctx->paged_chunks, split);
     return hipGetLastError();
 }
