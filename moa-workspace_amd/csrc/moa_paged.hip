@@ -599,8 +599,9 @@ __global__ __launch_bounds__(kPlanBlock) void paged_reorder_plan_kernel(PagedVie
     };
     bool bad = false;
     int copies = 0, dropped = 0;
+    Beam b = {-1, 0, 0, -1, false, false};
     for (int base = 0; base < count; base += step) {
-        const Beam b = beam_at(base, &bad);
+        b = beam_at(base, &bad);
         int page = -1, all = 0;
         if (b.dropped) {
             page = c.table[(base + t) * c.table_stride + b.len / (int)c.slots];
@@ -624,7 +625,7 @@ __global__ __launch_bounds__(kPlanBlock) void paged_reorder_plan_kernel(PagedVie
     }
     int given = 0;
     for (int base = 0; base < count; base += step) {
-        const Beam b = beam_at(base, &bad);
+        if (count > step) b = beam_at(base, &bad);  // (the only step's are still here)
         int all = 0;
         const int at = given + block_before(b.copies, lds, &all);
         if (t < step && base + t < count) {

@@ -15,7 +15,7 @@ constexpr int kBlock = 256;
 constexpr int kGroupLogits = 64;        // logits that share a key (their largest): 8 lanes' 16 bytes
 constexpr int kSearchMaxVocab = 1 << 20;
 
-constexpr unsigned kGroupTurn = 128;  // of the counters of a group's rows
+constexpr unsigned kGroupTurn = 128, kRowTurn = 512;  // of the counters of a group's rows, and of a row's parts and a call's rows
 
 typedef short s16x2 __attribute__((ext_vector_type(2)));
 
@@ -76,9 +76,24 @@ __host__ __device__ inline int parts_of(int vocab, int loads) { return (vocab + 
 
 // ---------------------------------------------------------------------------------------------- verify
 
-// The largest logit of a part of a row and its first place, as one number that orders by both.
+// Whether this workgroup is the last of `parts` to arrive at a counter; what the others published before is then there to
+// collect. kTurn: a power of two above any number of parts.
+template <unsigned kTurn>
+__device__ bool arrive_last(uint32_t* ticket, bool first, int parts) {
+    __shared__ uint32_t flag;
+    __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        const uint32_t share = join_share(first, parts, kTurn);
+        flag = join_last(__hip_atomic_fetch_add(ticket, share, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT), share, kTurn);
+    }
+    __syncthreads();
+    return flag;
+}
+
+// The largest logit of this workgroup's part of row blockIdx.y and its first place, as one number that orders by both, in thread 0.
 template <int kLoads>
-__global__ __launch_bounds__(kBlock) void verify_scan_kernel(const uint16_t* logits, int64_t stride, int vocab, uint64_t* best) {
+__device__ uint64_t verify_scan(const uint16_t* logits, int64_t stride, int vocab) {
     __shared__ int top[4];
     __shared__ uint32_t at[4];
     const LogitRow row(logits, stride, blockIdx.y, vocab);
@@ -107,53 +122,49 @@ __global__ __launch_bounds__(kBlock) void verify_scan_kernel(const uint16_t* log
     for (int k = 32; k > 0; k >>= 1) place = min(place, (uint32_t)__shfl_xor((int)place, k, kWave));
     if ((threadIdx.x & 63) == 0) at[wave] = place;
     __syncthreads();
-    if (threadIdx.x == 0)
-        best[(int64_t)blockIdx.y * gridDim.x + blockIdx.x] = (uint64_t)(uint32_t)(most + 32768) << 32 | ~min(min(at[0], at[1]), min(at[2], at[3]));
+    return (uint64_t)(uint32_t)(most + 32768) << 32 | ~min(min(at[0], at[1]), min(at[2], at[3]));
 }
 
-// One workgroup per sequence: its rows' parts into tokens, then the walk by one wave, four nodes a lane.
-__global__ __launch_bounds__(kBlock) void verify_walk_kernel(const uint64_t* part, int parts, const int32_t* tokens, const int32_t* starts,
-                                                             const uint64_t* masks, int words, int32_t* best, int32_t* leaves,
-                                                             int32_t* next, int rows, uint32_t* err) {
-    __shared__ int32_t named[kTreeMaxNodes];
-    const int s = blockIdx.x, t = threadIdx.x, lane = t & 63;
-    const int row0 = starts[s], end = starts[s + 1];
-    const bool out = !rows_in_range(row0, end, rows, 64 * words);
-    if (out || row0 == end) {
-        if (t == 0) {
-            leaves[s] = next[s] = -1;
-            if (out && row0 != end) atomicOr(err, kErrPaged);
-        }
-        return;
+struct VerifyCall {
+    const uint16_t* logits; int64_t stride;
+    const int32_t* tokens; const int32_t* starts; const uint64_t* masks;
+    int32_t* best; int32_t* leaves; int32_t* next;
+    int words, rows, vocab, sequences;
+    uint32_t* err;
+};
+
+// The rows of sequence s: false, with the sequence's outputs written, where it has none.
+__device__ __forceinline__ bool verify_rows(const VerifyCall& c, int s, bool first, int* row0, int* n) {
+    const int begin = c.starts[s], end = c.starts[s + 1];
+    const bool out = !rows_in_range(begin, end, c.rows, 64 * c.words);
+    *row0 = begin, *n = out ? 0 : end - begin;
+    if (*n == 0 && first) {
+        c.leaves[s] = c.next[s] = -1;
+        if (out && begin != end) atomicOr(c.err, kErrPaged);
     }
-    const int n = end - row0;
-    int lanes = 1;  // that share a row
-    while (lanes < 64 && lanes < parts) lanes *= 2;
-    for (int r = t / lanes; r < n; r += kBlock / lanes) {
-        uint64_t key = 0;
-        for (int i = t % lanes; i < parts; i += lanes) key = max(key, part[(int64_t)(row0 + r) * parts + i]);
-        for (int o = lanes / 2; o > 0; o >>= 1) key = max(key, (uint64_t)__shfl_xor((long long)key, o, kWave));
-        if (t % lanes == 0) best[row0 + r] = named[r] = (int32_t) ~(uint32_t)key;
-    }
-    __syncthreads();
-    if (t >= 64) return;
+    return *n > 0;
+}
+
+// The walk of a sequence of n rows by one wave, four nodes a lane; named: the rows' tokens.
+__device__ void verify_walk(const VerifyCall& c, int s, int row0, int n, const int32_t* named) {
+    const int lane = threadIdx.x & 63;
     uint64_t mask[4][kTreeMaxWords];
     int32_t token[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
         const int i = 64 * k + lane;
-        token[k] = i < n ? tokens[row0 + i] : 0;
+        token[k] = i < n ? c.tokens[row0 + i] : 0;
 #pragma unroll
         for (int w = 0; w < kTreeMaxWords; ++w) {
             const int left = n - 64 * w;
-            mask[k][w] = i < n && w < words && left > 0 ? masks[(int64_t)(row0 + i) * words + w] & (left >= 64 ? ~0ull : (1ull << left) - 1) : 0;
+            mask[k][w] = i < n && w < c.words && left > 0 ? c.masks[(int64_t)(row0 + i) * c.words + w] & (left >= 64 ? ~0ull : (1ull << left) - 1) : 0;
         }
     }
     auto of = [&](uint64_t v, int l) {
         return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)v, l) | (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), l) << 32;
     };
     if (!(of(mask[0][0], 0) & 1)) {  // node 0 is none
-        if (lane == 0) leaves[s] = next[s] = -1;
+        if (lane == 0) c.leaves[s] = c.next[s] = -1;
         return;
     }
     int cur = 0;
@@ -177,7 +188,57 @@ __global__ __launch_bounds__(kBlock) void verify_walk_kernel(const uint64_t* par
         if (child < 0) break;
         cur = child;
     }
-    if (lane == 0) leaves[s] = cur, next[s] = named[cur];
+    if (lane == 0) c.leaves[s] = cur, c.next[s] = named[cur];
+}
+
+template <int kLoads>
+__global__ __launch_bounds__(kBlock) void verify_scan_kernel(VerifyCall c, uint64_t* part) {
+    const uint64_t best = verify_scan<kLoads>(c.logits, c.stride, c.vocab);
+    if (threadIdx.x == 0) part[(int64_t)blockIdx.y * gridDim.x + blockIdx.x] = best;
+}
+
+// One workgroup per sequence: its rows' parts into tokens, then the walk.
+__global__ __launch_bounds__(kBlock) void verify_walk_kernel(VerifyCall c, const uint64_t* part, int parts) {
+    __shared__ int32_t named[kTreeMaxNodes];
+    const int s = blockIdx.x, t = threadIdx.x;
+    int row0, n;
+    if (!verify_rows(c, s, t == 0, &row0, &n)) return;
+    int lanes = 1;  // that share a row
+    while (lanes < 64 && lanes < parts) lanes *= 2;
+    for (int r = t / lanes; r < n; r += kBlock / lanes) {
+        uint64_t key = 0;
+        for (int i = t % lanes; i < parts; i += lanes) key = max(key, part[(int64_t)(row0 + r) * parts + i]);
+        for (int o = lanes / 2; o > 0; o >>= 1) key = max(key, (uint64_t)__shfl_xor((long long)key, o, kWave));
+        if (t % lanes == 0) c.best[row0 + r] = named[r] = (int32_t) ~(uint32_t)key;
+    }
+    __syncthreads();
+    if (t < kWave) verify_walk(c, s, row0, n, named);
+}
+
+// Few rows and sequences in one launch: the last part of a row to arrive names its token, the last row's workgroup walks, a wave per
+// sequence. (8 rows of 262144 logits, one sequence: scan and walk as two launches 13.6 us a call, 11.0 so.)
+constexpr int kFewSequences = 4;
+__global__ __launch_bounds__(kBlock) void verify_few_kernel(VerifyCall c, uint64_t* part, uint32_t* row_best, uint32_t* tickets) {
+    __shared__ int32_t named[kTreeMaxNodes];
+    const int t = threadIdx.x, parts = gridDim.x, row = blockIdx.y;
+    const uint64_t best = verify_scan<2>(c.logits, c.stride, c.vocab);
+    if (t == 0) publish64(part + (int64_t)row * parts + blockIdx.x, best);
+    if (!arrive_last<kRowTurn>(tickets + (int64_t)row * kTicketStride, blockIdx.x == 0, parts)) return;
+    if (t < kWave) {
+        uint64_t key = 0;
+        for (int i = t; i < parts; i += kWave) key = max(key, collect64(part + (int64_t)row * parts + i));
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) key = max(key, (uint64_t)__shfl_xor((long long)key, o, kWave));
+        if (t == 0) publish32(row_best + row, ~(uint32_t)key);
+    }
+    if (!arrive_last<kRowTurn>(tickets + (int64_t)kTreeMaxNodes * kTicketStride, row == 0, c.rows)) return;
+    if (t < c.rows) named[t] = (int32_t)__hip_atomic_load(row_best + t, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    const int s = t >> 6, lane = t & 63;
+    int row0, n;
+    if (s >= c.sequences || !verify_rows(c, s, lane == 0, &row0, &n)) return;
+    for (int i = lane; i < n; i += kWave) c.best[row0 + i] = named[row0 + i];
+    verify_walk(c, s, row0, n, named + row0);
 }
 
 // ---------------------------------------------------------------------------------------------- select
@@ -256,21 +317,6 @@ __global__ __launch_bounds__(kBlock) void select_scan_kernel(SelectCall c, Selec
         for (int i = 0; i < 4; ++i) total += top[i] == -INFINITY ? sums[i] : sums[i] * __builtin_amdgcn_exp2f((top[i] - part) * kLog2e);
         k.parts[(int64_t)r * k.parts_n + blockIdx.x] = make_float2(part, total);
     }
-}
-
-// Whether this workgroup is the last of `parts` to arrive at a counter; what the others published before is then there to
-// collect. kTurn: a power of two above any number of parts.
-template <unsigned kTurn>
-__device__ bool arrive_last(uint32_t* ticket, bool first, int parts) {
-    __shared__ uint32_t flag;
-    __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        const uint32_t share = join_share(first, parts, kTurn);
-        flag = join_last(__hip_atomic_fetch_add(ticket, share, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT), share, kTurn);
-    }
-    __syncthreads();
-    return flag;
 }
 
 // The largest of the wave's values, the same in every lane: four shifts within rows of 16, then the rows' last lanes (DPP).
@@ -478,7 +524,7 @@ int check_logits(const uint16_t* logits, int64_t stride, int rows, int vocab) {
 // eight.)
 int loads_of(int64_t rows, int vocab, int cus) { return rows * parts_of(vocab, 4) >= 2 * (int64_t)cus ? 4 : 2; }
 
-static_assert(kMaxBeams < (int)kGroupTurn, "arrivals are fewer than a turn");
+static_assert(kMaxParts < (int)kRowTurn && kTreeMaxNodes < (int)kRowTurn && kTreeMaxNodes < kSearchRows && kMaxBeams < (int)kGroupTurn, "arrivals are fewer than a turn");
 constexpr size_t kSearchBytes = kPagedChunkFloats * sizeof(float);
 
 }  // namespace
@@ -502,15 +548,21 @@ int moa_tree_verify(const uint16_t* logits, int64_t logit_row_stride, const int3
     DevCtx* ctx = paged_context(&e);
     if (!ctx) return e;
     hipStream_t s = static_cast<hipStream_t>(stream);
-    const int loads = loads_of(rows, vocab, ctx->cus), parts = parts_of(vocab, loads);
+    const VerifyCall c{logits, logit_row_stride, tokens, row_starts, masks, best, leaves, next_tokens, mask_words, rows, vocab, sequences, ctx->err};
     uint64_t* part = reinterpret_cast<uint64_t*>(ctx->paged_chunks);
+    if (rows && rows <= kTreeMaxNodes && sequences <= kFewSequences) {
+        const int parts = parts_of(vocab, 2);
+        hipLaunchKernelGGL(verify_few_kernel, dim3(parts, rows), dim3(kBlock), 0, s, c, part, reinterpret_cast<uint32_t*>(part + (size_t)rows * parts),
+                           ctx->search_tickets + (size_t)kSearchRows * kTicketStride);
+        return call_result(hipGetLastError(), "tree_verify launch");
+    }
+    const int loads = loads_of(rows, vocab, ctx->cus), parts = parts_of(vocab, loads);
     if (rows) {
         auto* f = loads == 4 ? verify_scan_kernel<4> : verify_scan_kernel<2>;
-        hipLaunchKernelGGL(f, dim3(parts, rows), dim3(kBlock), 0, s, logits, logit_row_stride, vocab, part);
+        hipLaunchKernelGGL(f, dim3(parts, rows), dim3(kBlock), 0, s, c, part);
         if ((e = call_result(hipGetLastError(), "tree_verify launch"))) return e;
     }
-    hipLaunchKernelGGL(verify_walk_kernel, dim3(sequences), dim3(kBlock), 0, s, part, parts, tokens, row_starts, masks, mask_words, best,
-                       leaves, next_tokens, rows, ctx->err);
+    hipLaunchKernelGGL(verify_walk_kernel, dim3(sequences), dim3(kBlock), 0, s, c, part, parts);
     return call_result(hipGetLastError(), "tree_verify launch");
 }
 
