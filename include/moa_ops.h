@@ -7,7 +7,7 @@
  * replaced by a trailing (M, stream) pair:
  *   - every tensor is a caller-owned device pointer (hipMalloc'd); the library never
  *     allocates per call (one per-device scratch block is made on first use or by moa_init, the
- *     paged calls' own, 98 MB, by the first of them);
+ *     paged calls' own, 100 MB, by the first of them);
  *   - `&mut` tensors of the reference (k_cache, v_cache, q_out, residual) are written in place;
  *   - bf16 tensors are raw uint16 bit patterns; E4M3FN/E2M1/E8M0 are uint8 codes;
  *   - M is the number of token rows (the reference processes exactly one, M = 1);

@@ -11,7 +11,7 @@
  * caller keeps; a call reads it before it returns). Its state -- page table, lengths, reference
  * counts -- lives on the device, and every call that changes it runs there: nothing synchronises,
  * and the calls can be captured into a HIP graph (call moa_init before). The first call on a device
- * allocates the paged calls' scratch (98 MB), also while a stream is captured.
+ * allocates the paged calls' scratch (100 MB), also while a stream is captured.
  *   - sequence s holds positions 0 .. seq_lens[s] - 1; position t lies in page
  *     page_table[s][t / slots] at slot t % slots. Table entries behind the last page in use are
  *     never read as pages.

@@ -35,6 +35,7 @@
 
 #include "moa_ops.h"
 #include "moa_paged.h"
+#include "moa_search.h"
 
 namespace moa {
 
@@ -199,6 +200,11 @@ inline const uint16_t* opt_u16(const HbmTensor<bf16>* t) { return t ? u16(*t) : 
 inline int int_of(size_t n) {
     if (n > static_cast<size_t>(std::numeric_limits<int>::max())) throw Error(MOA_ERROR_INVALID_VALUE, "a size past 2^31 - 1");
     return static_cast<int>(n);
+}
+// Words of the masks [rows, words] of a call's rows.
+inline int mask_words(const HbmTensor<uint64_t>& masks, size_t rows) {
+    if (masks.shape().size() != 2 || masks.shape()[0] != rows) throw Error(MOA_ERROR_INVALID_VALUE, "masks must be [rows, words]");
+    return int_of(masks.shape()[1]);
 }
 }  // namespace detail
 
@@ -594,6 +600,80 @@ inline void paged_attention(const Device& device, const HbmTensor<bf16>& q, cons
     check(moa_paged_attention(u16(q), width, cache.get(), row_starts.data(), u16(out), width, M, heads, layer, window, scale,
                               max_rows ? max_rows : M, device.stream()),
           "paged_attention");
+}
+
+// Drafted trees over the paged cache. masks [rows, words], 1 to 4 words a row: bit j of a node's row stands for node j of its sequence.
+// q, out [rows, q_heads, head_dim] (out may be q); max_rows: the most rows a sequence has, 0: all (at most 64 * words).
+template <class T>
+inline void paged_tree_attention(const Device& device, const HbmTensor<bf16>& q, const PagedCache<T>& cache,
+                                 const HbmTensor<int32_t>& row_starts, const HbmTensor<uint64_t>& masks, HbmTensor<bf16>& out,
+                                 int layer = 0, int window = 0, float scale = 1.0f, int max_rows = 0) {
+    using namespace detail;
+    if (q.shape().size() != 3 || q.shape()[2] != cache.head_dim() || q.size() == 0)
+        throw Error(MOA_ERROR_INVALID_VALUE, "q must be [rows, q_heads, head_dim]");
+    const int M = int_of(q.shape()[0]), heads = int_of(q.shape()[1]);
+    const int64_t width = static_cast<int64_t>(heads) * static_cast<int64_t>(cache.head_dim());
+    const int words = mask_words(masks, q.shape()[0]);
+    want(out, q.size(), "out"); want(row_starts, cache.sequences() + 1, "row_starts");
+    device.make_current();
+    check(moa_paged_tree_attention(u16(q), width, cache.get(), row_starts.data(), masks.data(), words, u16(out), width, M, heads, layer,
+                                   window, scale, max_rows ? max_rows : M, device.stream()),
+          "paged_tree_attention");
+}
+
+// leaves [sequences]: the node whose path each sequence keeps, -1: none.
+template <class T>
+inline void paged_tree_commit(const Device& device, PagedCache<T>& cache, const HbmTensor<int32_t>& row_starts,
+                              const HbmTensor<uint64_t>& masks, const HbmTensor<int32_t>& leaves) {
+    using namespace detail;
+    const size_t M = masks.shape().empty() ? 0 : masks.shape()[0];
+    const int words = mask_words(masks, M);
+    want(row_starts, cache.sequences() + 1, "row_starts"); want(leaves, cache.sequences(), "leaves");
+    device.make_current();
+    check(moa_paged_tree_commit(cache.get(), row_starts.data(), masks.data(), words, leaves.data(), int_of(M), device.stream()),
+          "paged_tree_commit");
+}
+
+// parents [count]: sequences 0 .. count - 1 are groups of `beams`, each becomes what its parent was.
+template <class T>
+inline void paged_cache_reorder(const Device& device, PagedCache<T>& cache, const HbmTensor<int32_t>& parents, int beams) {
+    device.make_current();
+    check(moa_paged_cache_reorder(cache.get(), parents.data(), detail::int_of(parents.size()), beams, device.stream()),
+          "paged_cache_reorder");
+}
+
+// Tokens from logits (include/moa_search.h). logits [rows, vocab]; tokens, best [rows]; row_starts [sequences + 1], masks [rows,
+// words]; leaves, next_tokens [sequences].
+inline void tree_verify(const Device& device, const HbmTensor<bf16>& logits, const HbmTensor<int32_t>& tokens,
+                        const HbmTensor<int32_t>& row_starts, const HbmTensor<uint64_t>& masks, HbmTensor<int32_t>& best,
+                        HbmTensor<int32_t>& leaves, HbmTensor<int32_t>& next_tokens) {
+    using namespace detail;
+    const std::vector<size_t>& n = logits.shape();
+    if (n.size() != 2) throw Error(MOA_ERROR_INVALID_VALUE, "logits must be [rows, vocab]");
+    const int words = mask_words(masks, n[0]);
+    want(tokens, n[0], "tokens"); want(best, n[0], "best"); want(row_starts, leaves.size() + 1, "row_starts");
+    want(next_tokens, leaves.size(), "next_tokens");
+    device.make_current();
+    check(moa_tree_verify(u16(logits), static_cast<int64_t>(n[1]), tokens.data(), row_starts.data(), masks.data(), words, best.data(),
+                          leaves.data(), next_tokens.data(), int_of(n[0]), int_of(n[1]), int_of(leaves.size()), device.stream()),
+          "tree_verify");
+}
+
+// logits [groups * beams, vocab], the others [groups * beams]; out_scores may be scores and out_finished may be finished. eos: -1 where
+// no token ends a beam.
+inline void beam_select(const Device& device, const HbmTensor<bf16>& logits, const HbmTensor<float>& scores,
+                        const HbmTensor<int32_t>& finished, HbmTensor<float>& out_scores, HbmTensor<int32_t>& out_finished,
+                        HbmTensor<int32_t>& parents, HbmTensor<int32_t>& tokens, int beams, int eos = -1) {
+    using namespace detail;
+    const std::vector<size_t>& n = logits.shape();
+    if (n.size() != 2 || beams < 1 || n[0] % static_cast<size_t>(beams))
+        throw Error(MOA_ERROR_INVALID_VALUE, "logits must be [groups * beams, vocab]");
+    want(scores, n[0], "scores"); want(finished, n[0], "finished"); want(out_scores, n[0], "out_scores");
+    want(out_finished, n[0], "out_finished"); want(parents, n[0], "parents"); want(tokens, n[0], "tokens");
+    device.make_current();
+    check(moa_beam_select(u16(logits), static_cast<int64_t>(n[1]), scores.data(), finished.data(), out_scores.data(), out_finished.data(),
+                          parents.data(), tokens.data(), int_of(n[0]) / beams, beams, int_of(n[1]), eos, device.stream()),
+          "beam_select");
 }
 
 }  // namespace ops
