@@ -145,51 +145,62 @@ __device__ __forceinline__ bool verify_rows(const VerifyCall& c, int s, bool fir
     return *n > 0;
 }
 
-// The walk of a sequence of n rows by one wave, four nodes a lane; named: the rows' tokens.
-__device__ void verify_walk(const VerifyCall& c, int s, int row0, int n, const int32_t* named) {
-    const int lane = threadIdx.x & 63;
-    uint64_t mask[4][kTreeMaxWords];
-    int32_t token[4];
+// The walk of a sequence of n rows by one wave, kWords nodes a lane: what it needs of the rows, asked for ahead of their tokens, and the
+// walk along `named`, the rows' tokens. (Trees of up to 64 nodes have one word: the compares of four are most of a step.)
+template <int kWords>
+struct VerifyWalk {
+    uint64_t mask[kWords][kWords];
+    int32_t token[kWords];
+
+    __device__ __forceinline__ void load(const VerifyCall& c, int row0, int n) {
+        const int lane = threadIdx.x & 63;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        const int i = 64 * k + lane;
-        token[k] = i < n ? c.tokens[row0 + i] : 0;
+        for (int k = 0; k < kWords; ++k) {
+            const int i = 64 * k + lane;
+            token[k] = i < n ? c.tokens[row0 + i] : 0;
 #pragma unroll
-        for (int w = 0; w < kTreeMaxWords; ++w) {
-            const int left = n - 64 * w;
-            mask[k][w] = i < n && w < c.words && left > 0 ? c.masks[(int64_t)(row0 + i) * c.words + w] & (left >= 64 ? ~0ull : (1ull << left) - 1) : 0;
+            for (int w = 0; w < kWords; ++w) {
+                const int left = n - 64 * w;
+                mask[k][w] = i < n && w < c.words && left > 0 ? c.masks[(int64_t)(row0 + i) * c.words + w] & (left >= 64 ? ~0ull : (1ull << left) - 1) : 0;
+            }
         }
     }
-    auto of = [&](uint64_t v, int l) {
-        return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)v, l) | (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), l) << 32;
-    };
-    if (!(of(mask[0][0], 0) & 1)) {  // node 0 is none
-        if (lane == 0) c.leaves[s] = c.next[s] = -1;
-        return;
-    }
-    int cur = 0;
-    for (int step = 0; step < n; ++step) {
-        const int want = named[cur];
-        uint64_t sees[kTreeMaxWords];
-#pragma unroll
-        for (int w = 0; w < kTreeMaxWords; ++w) {
-            const uint64_t x = cur < 64 ? mask[0][w] : cur < 128 ? mask[1][w] : cur < 192 ? mask[2][w] : mask[3][w];
-            sees[w] = of(x, cur & 63);
+
+    __device__ __forceinline__ void walk(const VerifyCall& c, int s, int n, const int32_t* named) {
+        const int lane = threadIdx.x & 63;
+        auto of = [&](uint64_t v, int l) {
+            return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)v, l) | (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), l) << 32;
+        };
+        if (!(of(mask[0][0], 0) & 1)) {  // node 0 is none
+            if (lane == 0) c.leaves[s] = c.next[s] = -1;
+            return;
         }
-        int child = -1;
+        int cur = 0;
+        for (int step = 0; step < n; ++step) {
+            const int want = named[cur];
+            uint64_t sees[kWords];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            bool is = token[k] == want && (mask[k][k] >> lane & 1) && 64 * k + lane < n && !(sees[k] >> lane & 1);
+            for (int w = 0; w < kWords; ++w) {
+                uint64_t x = mask[0][w];
 #pragma unroll
-            for (int w = 0; w < kTreeMaxWords; ++w) is = is && (mask[k][w] & ~(w == k ? 1ull << lane : 0ull)) == sees[w];
-            const uint64_t hit = __ballot(is);
-            if (child < 0 && hit) child = 64 * k + __builtin_ctzll(hit);
+                for (int k = 1; k < kWords; ++k) x = cur >= 64 * k ? mask[k][w] : x;
+                sees[w] = of(x, cur & 63);
+            }
+            int child = -1;
+#pragma unroll
+            for (int k = 0; k < kWords; ++k) {
+                bool is = token[k] == want && (mask[k][k] >> lane & 1) && 64 * k + lane < n && !(sees[k] >> lane & 1);
+#pragma unroll
+                for (int w = 0; w < kWords; ++w) is = is && (mask[k][w] & ~(w == k ? 1ull << lane : 0ull)) == sees[w];
+                const uint64_t hit = __ballot(is);
+                if (child < 0 && hit) child = 64 * k + __builtin_ctzll(hit);
+            }
+            if (child < 0) break;
+            cur = child;
         }
-        if (child < 0) break;
-        cur = child;
+        if (lane == 0) c.leaves[s] = cur, c.next[s] = named[cur];
     }
-    if (lane == 0) c.leaves[s] = cur, c.next[s] = named[cur];
-}
+};
 
 template <int kLoads>
 __global__ __launch_bounds__(kBlock) void verify_scan_kernel(VerifyCall c, uint64_t* part) {
@@ -198,11 +209,14 @@ __global__ __launch_bounds__(kBlock) void verify_scan_kernel(VerifyCall c, uint6
 }
 
 // One workgroup per sequence: its rows' parts into tokens, then the walk.
+template <int kWords>
 __global__ __launch_bounds__(kBlock) void verify_walk_kernel(VerifyCall c, const uint64_t* part, int parts) {
     __shared__ int32_t named[kTreeMaxNodes];
     const int s = blockIdx.x, t = threadIdx.x;
     int row0, n;
     if (!verify_rows(c, s, t == 0, &row0, &n)) return;
+    VerifyWalk<kWords> tree;
+    if (t < kWave) tree.load(c, row0, n);
     int lanes = 1;  // that share a row
     while (lanes < 64 && lanes < parts) lanes *= 2;
     for (int r = t / lanes; r < n; r += kBlock / lanes) {
@@ -212,12 +226,13 @@ __global__ __launch_bounds__(kBlock) void verify_walk_kernel(VerifyCall c, const
         if (t % lanes == 0) c.best[row0 + r] = named[r] = (int32_t) ~(uint32_t)key;
     }
     __syncthreads();
-    if (t < kWave) verify_walk(c, s, row0, n, named);
+    if (t < kWave) tree.walk(c, s, n, named);
 }
 
 // Few rows and sequences in one launch: the last part of a row to arrive names its token, the last row's workgroup walks, a wave per
 // sequence. (8 rows of 262144 logits, one sequence: scan and walk as two launches 13.6 us a call, 11.0 so.)
 constexpr int kFewSequences = 4;
+template <int kWords>
 __global__ __launch_bounds__(kBlock) void verify_few_kernel(VerifyCall c, uint64_t* part, uint32_t* row_best, uint32_t* tickets) {
     __shared__ int32_t named[kTreeMaxNodes];
     const int t = threadIdx.x, parts = gridDim.x, row = blockIdx.y;
@@ -237,8 +252,10 @@ __global__ __launch_bounds__(kBlock) void verify_few_kernel(VerifyCall c, uint64
     const int s = t >> 6, lane = t & 63;
     int row0, n;
     if (s >= c.sequences || !verify_rows(c, s, lane == 0, &row0, &n)) return;
+    VerifyWalk<kWords> tree;
+    tree.load(c, row0, n);
     for (int i = lane; i < n; i += kWave) c.best[row0 + i] = named[row0 + i];
-    verify_walk(c, s, row0, n, named + row0);
+    tree.walk(c, s, n, named + row0);
 }
 
 // ---------------------------------------------------------------------------------------------- select
@@ -552,7 +569,7 @@ int moa_tree_verify(const uint16_t* logits, int64_t logit_row_stride, const int3
     uint64_t* part = reinterpret_cast<uint64_t*>(ctx->paged_chunks);
     if (rows && rows <= kTreeMaxNodes && sequences <= kFewSequences) {
         const int parts = parts_of(vocab, 2);
-        hipLaunchKernelGGL(verify_few_kernel, dim3(parts, rows), dim3(kBlock), 0, s, c, part, reinterpret_cast<uint32_t*>(part + (size_t)rows * parts),
+        hipLaunchKernelGGL(mask_words == 1 ? verify_few_kernel<1> : verify_few_kernel<kTreeMaxWords>, dim3(parts, rows), dim3(kBlock), 0, s, c, part, reinterpret_cast<uint32_t*>(part + (size_t)rows * parts),
                            ctx->search_tickets + (size_t)kSearchRows * kTicketStride);
         return call_result(hipGetLastError(), "tree_verify launch");
     }
@@ -562,7 +579,7 @@ int moa_tree_verify(const uint16_t* logits, int64_t logit_row_stride, const int3
         hipLaunchKernelGGL(f, dim3(parts, rows), dim3(kBlock), 0, s, c, part);
         if ((e = call_result(hipGetLastError(), "tree_verify launch"))) return e;
     }
-    hipLaunchKernelGGL(verify_walk_kernel, dim3(sequences), dim3(kBlock), 0, s, c, part, parts);
+    hipLaunchKernelGGL(mask_words == 1 ? verify_walk_kernel<1> : verify_walk_kernel<kTreeMaxWords>, dim3(sequences), dim3(kBlock), 0, s, c, part, parts);
     return call_result(hipGetLastError(), "tree_verify launch");
 }
 

@@ -11,7 +11,7 @@ constexpr int kTreeMaxRows = 128;  // of a sequence up to 256 dims: two passes o
 template <int D, bool E4M3>
 struct TreeShape {
     static constexpr int kRows = 64;                         // of a tile: 16 for each of four waves
-    static constexpr int kTile = D == 64 ? 64 : 32;          // positions: 16 KB of K and V as bf16, 32 KB of 256 dims
+    static constexpr int kTile = D == 64 || (D == 128 && E4M3) ? 64 : 32;          // positions: 16 KB of K and V as bf16, 32 KB of 256 dims
     static constexpr int kSub = kTile / 16;
     static constexpr int kRowBytes = 2 * D;                  // LDS row of a position
     static constexpr int kStage = 2 * kTile * kRowBytes;
@@ -19,7 +19,7 @@ struct TreeShape {
     // in registers, 32 of them.
     static constexpr int kStages = E4M3 ? 2 : 80 * 1024 / kStage;
     static constexpr int kLds = kStages * kStage;
-    static constexpr int kAhead = D == 256 ? 2 : 4;
+    static constexpr int kAhead = kTile * D == 32 * 128 || D == 64 ? 4 : 2;
     static constexpr int kWaveRows = kTile / 4;              // positions of a tile that a wave loads
     static constexpr int kRowsPerLoad = 1024 / kRowBytes;    // positions that a load of 16 bytes a lane covers
     static constexpr int kLoads = kWaveRows / kRowsPerLoad;  // of K, and of V, per wave and tile

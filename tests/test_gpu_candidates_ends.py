@@ -451,3 +451,37 @@ def test_commit_of_the_most_sequences():
     assert torch.equal(k.view(S, 2, 64)[:, 0], want) and torch.equal(v.view(S, 2, 64)[:, 0], -want)
     st = Setup([5, 40], 16, 2, 64)
     run_commit(st, [5, 4], trees([5, 4], 2), [2, 3])
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "e4m3"])
+@pytest.mark.parametrize("n,group,heads,dim", KINDS)
+def test_sequences_shorter_than_their_trees(n, group, heads, dim, fmt):
+    """The nodes that would stand before the first position are not there; a row that sees no other gives zeros."""
+    need_gpu()
+    say(f"{n} nodes of {heads} x {group} x {dim} {fmt} over fewer positions")
+    lens = [0, n // 2, n - 1]
+    st = Setup(lens, 16, heads, dim, fmt, seed=3)
+    starts, masks = [0, n, 2 * n, 3 * n], trees([n] * 3, 5)
+    scale = 1 / math.sqrt(dim)
+    q = queries(3 * n, heads * group, dim, 4, 2.0 / scale)
+    out = torch.full_like(q, 7.0)
+    call(st, q, starts, masks, out, n, scale=scale)
+    assert ops.device_errors() == 0
+    # the same as trees of the nodes that are there, each at its position
+    short = [[masks[s * n + i] >> (n - lens[s]) for i in range(n)] for s in range(3)]
+    for s in range(3):
+        rows = [i for i in range(n) if short[s][i]]
+        assert (out[[s * n + i for i in range(n) if not short[s][i]]] == 0).all()
+        if not rows:
+            continue
+        k, v = st.values()
+        sc = (None, None) if st.k_scale is None else (st.k_scale[0], st.v_scale[0])
+        for i in rows:
+            pos = [p for p in range(lens[s]) if short[s][i] >> p & 1]
+            page, slot = torch.tensor([st.state.table[s][p // 16] for p in pos], device=DEV), torch.tensor([p % 16 for p in pos], device=DEV)
+            kr, vr = (t[page, slot].double() * (1 if x is None else x.double()[:, None]) for t, x in zip((k, v), sc))
+            qh = q[s * n + i].double().view(heads, group, dim)
+            kr, vr = kr.permute(1, 2, 0).contiguous(), vr.permute(1, 0, 2).contiguous()
+            w = torch.softmax(torch.matmul(qh, kr) * scale, -1)
+            check(out[s * n + i], torch.matmul(w, vr).reshape(heads * group, dim), torch.matmul(w, vr.abs()).reshape(heads * group, dim),
+                  (torch.matmul(qh.abs(), kr.abs()) * scale).amax(-1).reshape(heads * group), dim)
