@@ -187,7 +187,7 @@ hipError_t launch_tree(const PagedView& c, const PagedTreeCall& a, hipStream_t s
     const int64_t units = (a.window ? std::min<int64_t>(capacity, (int64_t)a.window + a.max_rows + kTokenUnit) : capacity) / kTokenUnit + 1;
     const int64_t tiles = (int64_t)a.rows * a.group / kTreeRows + sequences;
     const int64_t most = (int64_t)kPagedChunkFloats / record_floats(kTreeRows, D) / heads / 2;
-    const int groups = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>((int64_t)ctx->cus * 2 / heads, tiles * units), most));
+    const int groups = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>((int64_t)ctx->cus * TreeShape<D, E4M3>::kPerCu / heads, tiles * units), most));
     TreeSplit* split = reinterpret_cast<TreeSplit*>(ctx->paged_tokens);
     hipLaunchKernelGGL((paged_tree_kernel<D, E4M3>), dim3((uint32_t)(groups * heads)), dim3(256), 0, s, c, a, ctx->paged_chunks, split);
     hipError_t e = hipGetLastError();

@@ -19,7 +19,8 @@ struct TreeShape {
     // in registers, 32 of them.
     static constexpr int kStages = E4M3 ? 2 : 80 * 1024 / kStage;
     static constexpr int kLds = kStages * kStage;
-    static constexpr int kAhead = kTile * D == 32 * 128 || D == 64 ? 4 : 2;
+    static constexpr int kAhead = D == 64 ? 4 : 2;
+    static constexpr int kPerCu = 2;
     static constexpr int kWaveRows = kTile / 4;              // positions of a tile that a wave loads
     static constexpr int kRowsPerLoad = 1024 / kRowBytes;    // positions that a load of 16 bytes a lane covers
     static constexpr int kLoads = kWaveRows / kRowsPerLoad;  // of K, and of V, per wave and tile
@@ -112,31 +113,45 @@ __device__ __forceinline__ void tree_rows(const PagedView& c, const PagedTreeCal
         }
         ++ti, look += kTile;
     };
-    // E4M3: the same positions' codes into registers, 16 a load, and from there into LDS as bf16
+    // E4M3: the same positions' codes into registers, 16 a load, and from there into LDS as bf16, two chunks of a row. Eight lanes take half as
+    // many columns of two rows four apart, whose swizzles differ in their lowest bit: so their writes fall on all banks.
     struct Codes { uint4 k[T::kCodeLoads], v[T::kCodeLoads]; };
     constexpr int kCodeLanes = D / 16, kCodeRows = 64 / kCodeLanes;  // lanes of a row, rows of a load
+    const int code_col = (lane & 3) + (lane >> 3) % (kCodeLanes / 4) * 4;
+    auto code_row = [&](int j) {
+        const int x = (lane >> 3) / (kCodeLanes / 4) + j * (kCodeRows / 2);
+        return (x & 3) + (lane >> 2 & 1) * 4 + (x >> 2) * 8;
+    };
     auto load_codes = [&](Codes& x) __attribute__((always_inline)) {
         look_up();
 #pragma unroll
         for (int j = 0; j < T::kCodeLoads; ++j) {
-            const int src = ti * T::kWaveRows + j * kCodeRows + lane / kCodeLanes, at = lane % kCodeLanes * 16;
-            x.k[j] = ld16(kbase + __shfl(koff, src, kWave) + at);
-            x.v[j] = ld16(vbase + __shfl(voff, src, kWave) + at);
+            const int src = ti * T::kWaveRows + code_row(j), at = code_col * 16;
+            if (c.near) {
+                const uint32_t ko = (uint32_t)__shfl((int)koff, src, kWave), vo = c.alike ? ko : (uint32_t)__shfl((int)voff, src, kWave);
+                x.k[j] = ld16(kbase + (ko + at));
+                x.v[j] = ld16(vbase + (vo + at));
+            } else {
+                x.k[j] = ld16(kbase + __shfl(koff, src, kWave) + at);
+                x.v[j] = ld16(vbase + __shfl(voff, src, kWave) + at);
+            }
         }
         ++ti, look += kTile;
     };
     auto store_codes = [&](const Codes& x, uint8_t* kd) __attribute__((always_inline)) {
-        auto put = [&](uint8_t* d, const uint4& w, int row, int col) {
-            *reinterpret_cast<uint4*>(d + row * T::kRowBytes + ((2 * col) ^ chunk_swizzle<D>(row)) * 16) =
-                make_uint4(bf16_pair_of_fp8(w.x), bf16_pair_of_fp8(w.x >> 16), bf16_pair_of_fp8(w.y), bf16_pair_of_fp8(w.y >> 16));
-            *reinterpret_cast<uint4*>(d + row * T::kRowBytes + ((2 * col + 1) ^ chunk_swizzle<D>(row)) * 16) =
-                make_uint4(bf16_pair_of_fp8(w.z), bf16_pair_of_fp8(w.z >> 16), bf16_pair_of_fp8(w.w), bf16_pair_of_fp8(w.w >> 16));
+        auto low = [](uint32_t w) { return bf16_pair_of_fp8(w); };
+        auto high = [](uint32_t w) { return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, true)); };
+        auto put = [&](uint8_t* d, const uint4& w, int row) {
+            *reinterpret_cast<uint4*>(d + row * T::kRowBytes + ((2 * code_col) ^ chunk_swizzle<D>(row)) * 16) =
+                make_uint4(low(w.x), high(w.x), low(w.y), high(w.y));
+            *reinterpret_cast<uint4*>(d + row * T::kRowBytes + ((2 * code_col + 1) ^ chunk_swizzle<D>(row)) * 16) =
+                make_uint4(low(w.z), high(w.z), low(w.w), high(w.w));
         };
 #pragma unroll
         for (int j = 0; j < T::kCodeLoads; ++j) {
-            const int row = wave * T::kWaveRows + j * kCodeRows + lane / kCodeLanes, col = lane % kCodeLanes;
-            put(kd, x.k[j], row, col);
-            put(kd + T::kStage / 2, x.v[j], row, col);
+            const int row = wave * T::kWaveRows + code_row(j);
+            put(kd, x.k[j], row);
+            put(kd + T::kStage / 2, x.v[j], row);
         }
     };
 
