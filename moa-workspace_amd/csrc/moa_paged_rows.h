@@ -261,7 +261,7 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
 // 16 bytes per lane from global memory into LDS, lane l's at lds + 16 l. In asm, since the compiler would let no LDS read
-// pass before all such loads are done; `ready` waits for them. (One wait state between the
+// pass before all such loads are done; the kernels wait for them by count. (One wait state between the
 // write of m0 and its use, five between a vector instruction's write of a scalar register and its use.)
 __device__ __forceinline__ void load_to_lds(const void* from, uint32_t lds) {
     __asm__ volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "{m0}"(lds) : "memory");

@@ -1,5 +1,6 @@
 // moa_search.hip -- tokens from logits (include/moa_search.h): the greedy verification of drafted trees, and the selection of
-// beams. Both read every row of bf16 logits once; what is left of a row then fits a workgroup.
+// beams. Both read every row of bf16 logits once, at the rate of memory (524 rows of 262144, 275 MB: 43 us, 6.4 TB/s; the 151 live rows of a
+// selection, with exponentials beside, 79 MB: 17 us, 4.6 TB/s); what is left of a row then fits a workgroup.
 #include <algorithm>
 
 #include "../../include/moa_search.h"
@@ -208,7 +209,8 @@ __global__ __launch_bounds__(kBlock) void verify_scan_kernel(VerifyCall c, uint6
     if (threadIdx.x == 0) part[(int64_t)blockIdx.y * gridDim.x + blockIdx.x] = best;
 }
 
-// One workgroup per sequence: its rows' parts into tokens, then the walk.
+// One workgroup per sequence: its rows' parts into tokens, then the walk. (24 trees of 5 to 33 nodes: 6 us; 9.6 with four words of masks that are
+// asked for behind the tokens.)
 template <int kWords>
 __global__ __launch_bounds__(kBlock) void verify_walk_kernel(VerifyCall c, const uint64_t* part, int parts) {
     __shared__ int32_t named[kTreeMaxNodes];
@@ -520,7 +522,8 @@ __device__ void select_merge(const SelectCall& c, const SelectScratch& k, int r0
     c.out_finished[row] = out_done;
 }
 
-// A workgroup per row; the last of a group picks its beams.
+// A workgroup per row; the last of a group picks its beams. Latency bounds it (keys, logits of the groups found, arrival, candidates: 10.4 us for
+// one group of 4, 12.2 for 20 of 8); one row of a group after the other in one workgroup would take its steps in turn.
 template <int kKeys>
 __global__ __launch_bounds__(kBlock) void select_rows_kernel(SelectCall c, SelectScratch k) {
     const int r = blockIdx.x, g = r / c.beams;

@@ -1,16 +1,19 @@
 // moa_tree_attention.hip -- attention of drafted trees over the paged cache (include/moa_paged.h) for sequences of a few dozen rows.
 //
-// Every row of a tree sees the positions before it, so one pass over K and V serves all rows of a sequence: up to 64 or 128 of them in a
-// workgroup, 16 for each of its waves. K and V go through LDS, in a ring of tiles of 16 KB: the matrix cores and LDS have a third of the
-// time that memory takes, so what counts is that loads never pause.
+// Every row of a tree sees the positions before it, so one pass over K and V serves a tile of 64 rows of a sequence, 16 for each of a
+// workgroup's waves, and two tiles the 65 to 128 rows that still come here. K and V go through LDS (moa_tree_rows.h says how). The positions are dealt
+// out evenly over as many workgroups as the device holds, and the rows of tiles that were split so are joined by a second launch.
+//
+// Measured, 40 trees of 9 to 33 nodes with 2 x 256 dims a KV head, bf16: 318 MB of K and V in 67 us, 4.7 TB/s, and 8 us of the merge. 32 trees of
+// 5 to 16 nodes with 4 x 128 dims over E4M3 pages: 265 MB in 85 us and 10; loads, widening and the stores to LDS alone take 50, the products and
+// the softmax, of three to four waves behind one barrier a tile, the rest. Dealing by (KV head, positions) in the other order, other
+// places of the row groups among the waves, and twice the workgroups on a CU (tiles of 32 positions) changed nothing or were slower.
 #include <algorithm>
 
 #include "moa_tree_rows.h"
 
 namespace moa {
 namespace {
-
-constexpr int kTreeRows = 64;  // of a tile up to 256 dims
 
 // The units of kTokenUnit positions of all sequences' tiles, a sequence's tiles behind each other, are one row of U, dealt out evenly: group
 // w of `groups` takes units [w q, (w + 1) q), q = ceil(U / groups), crossing from tile to tile. A part that is not its whole tile leaves a
@@ -97,7 +100,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void p
         }
         const int lo = token_first(a, Seq{t.row0, t.n, t.len}, T::kTile) + off * kTokenUnit;
         const int hi = (int)min((int64_t)lo + (int64_t)take * kTokenUnit, (int64_t)t.len);
-        float* rec = whole ? nullptr : part + ((int64_t)kvh * 2 * groups + 2 * group + (off == 0)) * record_floats(T::kRows, D);
+        float* rec = whole ? nullptr : part + ((int64_t)kvh * 2 * groups + 2 * group + (off == 0)) * record_floats(kTreeRows, D);
         tree_rows<D, E4M3>(c, a, t, kvh, lo, hi, rec, lds);
     }
     if (threadIdx.x == 0) split[2 * (kvh * groups + group)] = begun, split[2 * (kvh * groups + group) + 1] = inside;
@@ -187,7 +190,7 @@ hipError_t launch_tree(const PagedView& c, const PagedTreeCall& a, hipStream_t s
     const int64_t units = (a.window ? std::min<int64_t>(capacity, (int64_t)a.window + a.max_rows + kTokenUnit) : capacity) / kTokenUnit + 1;
     const int64_t tiles = (int64_t)a.rows * a.group / kTreeRows + sequences;
     const int64_t most = (int64_t)kPagedChunkFloats / record_floats(kTreeRows, D) / heads / 2;
-    const int groups = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>((int64_t)ctx->cus * TreeShape<D, E4M3>::kPerCu / heads, tiles * units), most));
+    const int groups = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>((int64_t)ctx->cus * 2 / heads, tiles * units), most));
     TreeSplit* split = reinterpret_cast<TreeSplit*>(ctx->paged_tokens);
     hipLaunchKernelGGL((paged_tree_kernel<D, E4M3>), dim3((uint32_t)(groups * heads)), dim3(256), 0, s, c, a, ctx->paged_chunks, split);
     hipError_t e = hipGetLastError();

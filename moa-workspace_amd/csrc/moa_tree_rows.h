@@ -6,12 +6,21 @@
 namespace moa {
 namespace {
 
-constexpr int kTreeMaxRows = 128;  // of a sequence up to 256 dims: two passes over its K and V
+constexpr int kTreeRows = 64;      // of a tile: 16 for each of four waves
+
+// Rows of a sequence that come here, up to 256 dims: from 17 on, since the token kernel reads K and V without LDS for all 16 that one MFMA takes
+// (one sequence of 12000 positions, 16 rows of 256 dims: 22 us there, 51 here), to two tiles, as many rows as the chunk kernel shares a tile of
+// K and V among. Against that kernel, 16 sequences of 1000 to 9000 positions, us here / there at 24, 64, 100 and 128 rows: 256 dims bf16
+// 145 / 207, 200 / 261, 225 / 240, 266 / 266; 256 dims E4M3 105 / 185, 154 / 247, 171 / 213, 262 / 260; 128 dims bf16 81 / 89, 95 / 100, 146 / 134,
+// 164 / 167; 128 dims E4M3 61 / 77, 79 / 98, 121 / 128, 160 / 157. One sequence of 4000 positions, 100 rows: 27 / 46 (256 dims), 22 / 27 (128).
+// Rows of 512 dims took 590 us here and 376 there (12 sequences of up to 16000 positions): half the registers of a wave hold its output.
+constexpr int kTreeMaxRows = 128;
 
 template <int D, bool E4M3>
 struct TreeShape {
-    static constexpr int kRows = 64;                         // of a tile: 16 for each of four waves
-    static constexpr int kTile = D == 64 || (D == 128 && E4M3) ? 64 : 32;          // positions: 16 KB of K and V as bf16, 32 KB of 256 dims
+    // Positions of a tile: 16 KB of K and V as bf16, 32 KB of 256 dims; and of E4M3 of 128 dims, where only two tiles are in LDS and more of
+    // the work lies between barriers then (32 trees, 265 MB: 87 us, 94 with 32 positions).
+    static constexpr int kTile = D == 64 || (D == 128 && E4M3) ? 64 : 32;
     static constexpr int kSub = kTile / 16;
     static constexpr int kRowBytes = 2 * D;                  // LDS row of a position
     static constexpr int kStage = 2 * kTile * kRowBytes;
@@ -20,7 +29,6 @@ struct TreeShape {
     static constexpr int kStages = E4M3 ? 2 : 80 * 1024 / kStage;
     static constexpr int kLds = kStages * kStage;
     static constexpr int kAhead = D == 64 ? 4 : 2;
-    static constexpr int kPerCu = 2;
     static constexpr int kWaveRows = kTile / 4;              // positions of a tile that a wave loads
     static constexpr int kRowsPerLoad = 1024 / kRowBytes;    // positions that a load of 16 bytes a lane covers
     static constexpr int kLoads = kWaveRows / kRowsPerLoad;  // of K, and of V, per wave and tile
@@ -35,17 +43,22 @@ __device__ __forceinline__ float rows_max(float x) {
     return pair(__builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false));
 }
 
-// Up to kRows rows of a sequence, those of tile t.tile, over positions [lo, hi) of it, from a multiple of kTile on: rows 16 w .. of them by wave w
-// of the workgroup. rec: the record that they leave, or nullptr: they are all positions, and the rows are written. lds: kLds bytes at a multiple of 1024. Scores are K times Q^T (16 x 16 x 32 MFMAs):
-// lane (c = lane % 16, g = lane / 16) holds, for row c, positions 4 g .. 4 g + 3 of 16, which are just what it supplies as B of
-// V^T times P^T, 32 positions at a time, when V's transposing LDS reads fetch the same positions: P moves between no lanes, and a
-// row's maximum, sum and outputs are its lanes'. P enters as two bf16 parts, which share V's fragments.
+// Up to kTreeRows rows of a sequence, those of tile t.tile, over positions [lo, hi) of it, lo a multiple of kTile: rows 16 w .. of them by
+// wave w of the workgroup. rec: the record that they leave, or nullptr where [lo, hi) is all they see: then their results are written. lds: kLds
+// bytes at a multiple of 1024.
+//
+// Scores are K times Q^T (16 x 16 x 32 MFMAs): lane (c = lane % 16, g = lane / 16) holds, for row c, positions 4 g .. 4 g + 3 of 16, which
+// are just what it supplies as B of V^T times P^T, 32 positions at a time, when V's transposing LDS reads fetch the same positions: P moves
+// between no lanes, and a row's maximum, sum and outputs are its lanes'. P enters as two bf16 parts, which share V's fragments.
+//
+// bf16 tiles go from memory to LDS directly, into a ring of stages with one barrier a tile: the matrix cores and LDS have a third of the time that
+// memory takes, so what counts is that loads never pause. E4M3 codes wait in registers and are widened on their way to LDS.
 template <int D, bool E4M3>
 __device__ __forceinline__ void tree_rows(const PagedView& c, const PagedTreeCall& a, const Piece& t, int kvh, int lo, int hi, float* rec, uint8_t* lds) {
     using T = TreeShape<D, E4M3>;
     constexpr int kTile = T::kTile, kSteps = D / 32, kDims = D / 16;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l16 = lane & 15, g = lane >> 4;
-    const int r0 = t.tile * T::kRows, nr = min(T::kRows, t.n * a.group - r0), tree0 = t.len - t.n;
+    const int r0 = t.tile * kTreeRows, nr = min(kTreeRows, t.n * a.group - r0), tree0 = t.len - t.n;
     // x = factor (q . k): a negative factor's sign goes to q, so that the largest product is the largest x; and a factor of
     // zero stays above it, so that a product of -inf (a position that a row does not see) stays -inf (a NaN stays one)
     const float signed_factor = E4M3 ? c.k_scale[kvh] * a.scale_log2 : a.scale_log2;
@@ -337,10 +350,10 @@ __device__ __forceinline__ void tree_rows(const PagedView& c, const PagedTreeCal
     const bool odd = all & 2;  // the careful path writes, and reads q, which may be out
     if (is && (bad || !odd)) {
         if (rec) {
-            float* to = rec + 2 * T::kRows + wrow * D + 4 * g;
+            float* to = rec + 2 * kTreeRows + wrow * D + 4 * g;
 #pragma unroll
             for (int d = 0; d < kDims; ++d) *reinterpret_cast<float4*>(to + 16 * d) = make_float4(o[d][0], o[d][1], o[d][2], o[d][3]);
-            if (g == 0) rec[wrow] = bad ? NAN : m_ref, rec[T::kRows + wrow] = l_run;
+            if (g == 0) rec[wrow] = bad ? NAN : m_ref, rec[kTreeRows + wrow] = l_run;
         } else if (!bad) {
             const float inv = l_run == 0.0f ? 0.0f : (E4M3 ? c.v_scale[kvh] : 1.0f) / l_run;
             uint16_t* to = a.out + (int64_t)m_row * a.out_row + head * D + 4 * g;
@@ -351,7 +364,7 @@ __device__ __forceinline__ void tree_rows(const PagedView& c, const PagedTreeCal
     }
     if (bad && threadIdx.x == 0) atomicOr(c.err, kErrPaged);
     if (odd && !bad)
-        careful_piece<E4M3>(c, a, t, kvh, r0, nr, lo, hi, [&](int, const Row& x) { return a.q + x.m * a.q_row + x.h * D; }, rec, T::kRows);
+        careful_piece<E4M3>(c, a, t, kvh, r0, nr, lo, hi, [&](int, const Row& x) { return a.q + x.m * a.q_row + x.h * D; }, rec, kTreeRows);
 }
 
 }  // namespace
