@@ -36,6 +36,21 @@ struct TreeShape {
     static constexpr int kGroup = 64 / kWaveRows;            // tiles whose positions a wave's lanes look up at once
 };
 
+// 16-byte chunk c of LDS row r lies in chunk c ^ swizzle(r). What has to fall on all banks: K's reads, which take one chunk of four quads of rows
+// beside each other, the quads of lanes l and l + 16 from different ones (any four different low bits do, where the lane's step leaves them alone);
+// V's, two chunks of eight rows (bit 1 differs between quads 0 and 1, and 2 and 3); and the writes of widened codes, every other chunk of a
+// row and of the row four behind (bit 0 differs there). Rows of 128 bytes (64 dims) pair up: two rows span the banks.
+template <int D>
+__host__ __device__ constexpr int tree_swizzle(int r) {
+    const int quad = (r >> 2 & 1) * 3 ^ (r >> 3 & 1);
+    return D == 64 ? (r >> 1 & 1) << 2 | quad : (r & 3) << 2 | quad;
+}
+// The chunk of a row that lane group g multiplies in step s. (Any order of the dims will do that Q has too.)
+template <int D>
+__host__ __device__ constexpr int tree_chunk(int s, int g) {
+    return D == 64 ? 4 * (g & 1) + (g >> 1) + 2 * s : 16 * (s >> 2) + 4 * g + (s & 3);
+}
+
 // The largest of a row's values, over the four lanes that hold it: 16 and 32 lanes apart, in vector registers.
 __device__ __forceinline__ float rows_max(float x) {
     auto pair = [](auto y) { return fmaxf(__uint_as_float(y[0]), __uint_as_float(y[1])); };
@@ -64,9 +79,9 @@ __device__ __forceinline__ void tree_rows(const PagedView& c, const PagedTreeCal
     const float signed_factor = E4M3 ? c.k_scale[kvh] * a.scale_log2 : a.scale_log2;
     const float factor = fabsf(signed_factor) < 1.2e-38f ? 1.2e-38f : fabsf(signed_factor);
     const uint32_t flip = signed_factor < 0.0f ? 0x80008000u : 0u;
-    // LDS byte addresses of a lane: K row l16, chunk 4 j + g; V's transposing reads, rows 4 g + ln / 4 % 4, chunk 2 d + ln / 2 % 2
-    const int k_at = l16 * T::kRowBytes + ((g ^ chunk_swizzle<D>(l16)) * 16);
-    const int v_row = 4 * g + (lane >> 2 & 3), v_at = v_row * T::kRowBytes + (((lane >> 1 & 1) ^ chunk_swizzle<D>(v_row)) * 16) + (lane & 1) * 8;
+    // LDS byte addresses of a lane: K row l16, chunk tree_chunk; V's transposing reads, rows 4 g + ln / 4 % 4, chunk 2 d + ln / 2 % 2
+    const int k_at = l16 * T::kRowBytes + ((tree_chunk<D>(0, g) ^ tree_swizzle<D>(l16)) * 16);
+    const int v_row = 4 * g + (lane >> 2 & 3), v_at = v_row * T::kRowBytes + (((lane >> 1 & 1) ^ tree_swizzle<D>(v_row)) * 16) + (lane & 1) * 8;
     const uint32_t lds_at = (uint32_t)(uintptr_t)(lds_void*)lds;
     // the lane's row: where it lies, its query, and the positions that it, and all rows of the wave, see
     const int wrow = 16 * wave + l16;
@@ -112,7 +127,7 @@ __device__ __forceinline__ void tree_rows(const PagedView& c, const PagedTreeCal
 #pragma unroll
         for (int i = 0; i < T::kLoads; ++i) {
             const int row = wave * T::kWaveRows + i * T::kRowsPerLoad;
-            const int at = ((lane % kLanes) ^ chunk_swizzle<D>(row + lane / kLanes)) * 16, src = src0 + i * T::kRowsPerLoad;
+            const int at = ((lane % kLanes) ^ tree_swizzle<D>(row + lane / kLanes)) * 16, src = src0 + i * T::kRowsPerLoad;
             const uint32_t kd = lds_at + stage + row * T::kRowBytes, vd = kd + T::kStage / 2;
             if (c.near) {
                 const uint32_t ko = (uint32_t)__shfl((int)koff, src, kWave);
@@ -155,9 +170,9 @@ __device__ __forceinline__ void tree_rows(const PagedView& c, const PagedTreeCal
         auto low = [](uint32_t w) { return bf16_pair_of_fp8(w); };
         auto high = [](uint32_t w) { return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, true)); };
         auto put = [&](uint8_t* d, const uint4& w, int row) {
-            *reinterpret_cast<uint4*>(d + row * T::kRowBytes + ((2 * code_col) ^ chunk_swizzle<D>(row)) * 16) =
+            *reinterpret_cast<uint4*>(d + row * T::kRowBytes + ((2 * code_col) ^ tree_swizzle<D>(row)) * 16) =
                 make_uint4(low(w.x), high(w.x), low(w.y), high(w.y));
-            *reinterpret_cast<uint4*>(d + row * T::kRowBytes + ((2 * code_col + 1) ^ chunk_swizzle<D>(row)) * 16) =
+            *reinterpret_cast<uint4*>(d + row * T::kRowBytes + ((2 * code_col + 1) ^ tree_swizzle<D>(row)) * 16) =
                 make_uint4(low(w.z), high(w.z), low(w.w), high(w.w));
         };
 #pragma unroll
@@ -179,7 +194,7 @@ __device__ __forceinline__ void tree_rows(const PagedView& c, const PagedTreeCal
             auto read_k = [&](int s) __attribute__((always_inline)) {
 #pragma unroll
                 for (int b = 0; b < T::kSub; ++b)
-                    kf[s % kAhead][b] = *reinterpret_cast<const bf16x8*>(tile + (k_at ^ (64 * (s & (D == 64 ? 1 : 3)))) + (D == 64 ? 0 : 256 * (s >> 2)) +
+                    kf[s % kAhead][b] = *reinterpret_cast<const bf16x8*>(tile + (k_at ^ (D == 64 ? 32 * s : 16 * (s & 3))) + (D == 64 ? 0 : 256 * (s >> 2)) +
                                                                          16 * b * T::kRowBytes);
             };
 #pragma unroll
@@ -265,9 +280,9 @@ __device__ __forceinline__ void tree_rows(const PagedView& c, const PagedTreeCal
     // what the part reads of its rows is asked for ahead of its tiles, and looked at when those are on their way
     uint64_t mask[kTreeMaxWords];
     {
-        const uint16_t* qp = a.q + (int64_t)m_row * a.q_row + head * D + 8 * g;
+        const uint16_t* qp = a.q + (int64_t)m_row * a.q_row + head * D;
 #pragma unroll
-        for (int s = 0; s < kSteps; ++s) qf[s] = ld16(qp + 32 * s);
+        for (int s = 0; s < kSteps; ++s) qf[s] = ld16(qp + 8 * tree_chunk<D>(s, g));
 #pragma unroll
         for (int w = 0; w < kTreeMaxWords; ++w) mask[w] = w < a.words ? a.masks[(int64_t)m_row * a.words + w] : 0;
     }
