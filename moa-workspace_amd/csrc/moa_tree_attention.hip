@@ -5,7 +5,7 @@
 // out evenly over as many workgroups as the device holds, and the rows of tiles that were split so are joined by a second launch.
 //
 // Measured, 40 trees of 9 to 33 nodes with 2 x 256 dims a KV head, bf16: 318 MB of K and V in 67 us, 4.7 TB/s, and 8 us of the merge. 32 trees of
-// 5 to 16 nodes with 4 x 128 dims over E4M3 pages: 265 MB in 85 us and 10; loads, widening and the stores to LDS alone take 50, the products and
+// 5 to 16 nodes with 4 x 128 dims over E4M3 pages: 265 MB in 83 us and 10; loads, widening and the stores to LDS alone take 50, the products and
 // the softmax, of three to four waves behind one barrier a tile, the rest. Dealing by (KV head, positions) in the other order, other
 // places of the row groups among the waves, and twice the workgroups on a CU (tiles of 32 positions) changed nothing or were slower.
 #include <algorithm>
