@@ -403,7 +403,7 @@ __device__ void select_row(const SelectCall& c, const SelectScratch& k, int r) {
     const int done = c.finished[row];
     const double score = score_f;
     auto put = [&](int i, double total, int place) {
-        publish64(totals + i, __builtin_bit_cast(uint64_t, total));
+        publish64(totals + i, __builtin_bit_cast(uint64_t, total + 0.0));  // (-0 ties with 0)
         publish32(places + i, (uint32_t)place);
     };
     constexpr int kMost = kMaxParts / kWave;

@@ -408,3 +408,9 @@ def test_the_front_end_refuses():
         with pytest.raises(error):
             call()
     assert ops.device_errors() == 0
+
+
+@pytest.mark.parametrize("scores", [[-0.0, 0.0, -0.0], [0.0, -0.0, 0.0]])
+def test_select_of_zeros_of_both_signs(scores):
+    need_gpu()
+    run_select(logits_of(3, 20), scores, [1, 1, 1], 3, 4)
