@@ -115,38 +115,41 @@ int moa_paged_attention(const uint16_t* q, int64_t q_row_stride, const moa_paged
                         const int32_t* row_starts, uint16_t* out, int64_t out_row_stride, int rows, int q_heads,
                         int layer, int window, float scale, int max_rows, void* stream);
 
-/* Drafted trees. A step of speculative decoding appends a tree of drafted tokens to a sequence as its last n positions, n at
- * most 256: node i of sequence s is row row_starts[s] + i of the call and position seq_lens[s] - n + i. masks (device
- * uint64 [rows][mask_words], 1 to 4 words) says what a node sees: bit j % 64 of word j / 64 of a node's row stands for node j of the same
- * sequence, the node itself and its ancestors in a tree (any set is allowed; bits from n on are ignored). A row without
- * bits is no node. A node's depth is the number of nodes that it sees, so it stands depth - 1 positions behind the
- * first node; a node without ancestors stands at position seq_lens[s] - n. */
+/* Drafted trees. A step of speculative decoding appends a tree of drafted tokens to a sequence as its last n positions,
+ * n at most 256: node i of sequence s is row row_starts[s] + i of the call and position seq_lens[s] - n + i. masks
+ * (device uint64 [rows][mask_words], 1 to 4 words) says what a node sees: bit j % 64 of word j / 64 of a node's row
+ * stands for node j of the same sequence, the node itself and its ancestors in a tree (any set is allowed; bits from n
+ * on are ignored). A row without bits is no node. A node's depth is the number of nodes that it sees, so it stands depth
+ * - 1 positions behind the first node; a node without ancestors stands at position seq_lens[s] - n. */
 
 /* Attention of the nodes: node i sees the positions before the tree (with a window, those less than `window` before its
  * own place as above) and the nodes of its mask. Everything else is as in moa_paged_attention, whose last bits a chain's
- * rows need not have. A row without bits gives zeros. Sequences without a tree take part with trees of one node. max_rows is
- * at most 64 * mask_words; window is 0 or at least max_rows. */
+ * rows need not have. A row without bits gives zeros; nodes that would stand before position 0 are not there. Sequences
+ * without a tree take part with trees of one node. max_rows is at most 64 * mask_words; window is 0 or at least
+ * max_rows. */
 int moa_paged_tree_attention(const uint16_t* q, int64_t q_row_stride, const moa_paged_cache* cache,
                              const int32_t* row_starts, const uint64_t* masks, int mask_words, uint16_t* out,
                              int64_t out_row_stride, int rows, int q_heads, int layer, int window, float scale, int max_rows,
                              void* stream);
 
-/* Ends a speculative step: of each sequence that has rows, the nodes that node leaves[s] (device int32 [sequences]) sees become, in
- * ascending order and in every layer, the positions behind those before the tree; the sequence ends behind them, and
- * pages that it no longer reaches are free. -1 keeps no node. Positions behind the new length keep what they held or were
- * moved from. A sequence whose rows, length or leaf are out of range, that is shorter than its rows, or one of whose
- * nodes lies in a page outside the pool or in one with a reference count other than 1, stays as it was (MOA_DEVERR_PAGED). rows may be 0. */
+/* Ends a speculative step: of each sequence that has rows, the nodes that node leaves[s] (device int32 [sequences]) sees
+ * become, in ascending order and in every layer, the positions behind those before the tree; the sequence ends behind
+ * them, and pages that it no longer reaches are free. -1 keeps no node. Positions behind the new length keep what they
+ * held or were moved from. A sequence whose rows, length or leaf are out of range, that is shorter than its rows, or one
+ * of whose nodes lies in a page outside the pool or in one with a reference count other than 1, stays as it was
+ * (MOA_DEVERR_PAGED). rows may be 0. */
 int moa_paged_tree_commit(const moa_paged_cache* cache, const int32_t* row_starts, const uint64_t* masks, int mask_words,
                           const int32_t* leaves, int rows, void* stream);
 
-/* A beam search's step back: sequences 0 .. count - 1 are groups of `beams` (1 to 64; count a multiple of it), and every sequence s of
- * them becomes what parents[s] (device int32 [count], a sequence of its group) was before the call, in every layer. Full pages are
- * shared, reference counts follow. A partly filled last page stays with its parent, if that is its own child, else with the
- * parent's first child; the other children get copies of the slots in use: in ascending order, in the partly filled last pages of the sequences that
- * are nobody's parent (where their reference count is 1), in ascending order, then in the lowest free pages. Pages that no
- * sequence names any more are free. All or nothing: a parent outside the group, a length out of range, a page to copy outside the pool or
- * too few free pages leave the state as it was; another table entry outside the pool moves with its row and is not
- * counted (MOA_DEVERR_PAGED for all). count may be 0. */
+/* A beam search's step back: sequences 0 .. count - 1 are groups of `beams` (1 to 64; count a multiple of it), and every
+ * sequence s of them becomes what parents[s] (device int32 [count], a sequence of its group) was before the call, in
+ * every layer. Full pages are shared, reference counts follow. A partly filled last page stays with its parent, if that
+ * is its own child, else with the parent's first child; the other children get copies of the slots in use: in ascending
+ * order, in the partly filled last pages of the sequences that are nobody's parent (where their reference count is 1),
+ * in ascending order, then in the lowest free pages. Pages that no sequence names any more are free. All or nothing: a
+ * parent outside the group, a length out of range, a page to copy outside the pool or too few free pages leave the state
+ * as it was; another table entry outside the pool moves with its row and is not counted (MOA_DEVERR_PAGED for all).
+ * count may be 0. */
 int moa_paged_cache_reorder(const moa_paged_cache* cache, const int32_t* parents, int count, int beams, void* stream);
 
 #ifdef __cplusplus
