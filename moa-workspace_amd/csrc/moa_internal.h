@@ -80,7 +80,7 @@ constexpr size_t kPagedChunkFloats = (size_t)17 << 20;  // 71.3 MB
 constexpr int kTreeMaxWords = 4, kTreeMaxNodes = 64 * kTreeMaxWords;  // nodes of a drafted tree, one mask bit each
 constexpr int kMaxBeams = 64;                           // sequences of a beam search's group
 constexpr int kPagedTickets = 2048;                     // arrivals at split sequences (moa_paged_plan.h: kJoinTurn)
-constexpr int kSearchRows = 4096;                       // rows of logits of a selection's launch; a counter for each, and for each group of beams
+constexpr int kSearchRows = 4096;                       // rows of logits of a selection's launch, sequences of a commit's
 
 // Device-side error bits (OR-ed by kernels; read back by moa_device_errors()).
 constexpr uint32_t kErrRopeOffset = 1u;
@@ -110,7 +110,7 @@ struct DevCtx {
     float* paged_tokens = nullptr;  // paged attention's split records (kPagedTokenFloats, kPagedChunkFloats)
     float* paged_chunks = nullptr;
     uint32_t* paged_tickets = nullptr;  // kPagedTickets
-    uint32_t* search_tickets = nullptr;  // 2 * kSearchRows counters, kTicketStride apart
+    uint32_t* search_tickets = nullptr;  // kSearchRows counters of groups of beams, then as many of kRowTurn's; kTicketStride apart
     void* base = nullptr;
     int cus = 0;                  // compute units of the device
     int8_t ffn_fused[6] = {-1, -1, -1, -1, -1, -1};  // per (format, scale kind): grid fits resident? (-1 unknown)

@@ -1,13 +1,14 @@
 // moa_paged.hip -- the paged KV cache (include/moa_paged.h): argument checks, the calls that change its
-// state (reserve, fork, free, compact), the append of new rows, and the copies of pages.
+// state (reserve, fork, free, compact, a tree's commit, reorder), the append of new rows, and the copies of pages.
 //
-// State changes are planned by one workgroup that reads the lengths and the reference counts, checks the whole
+// State changes that are all or nothing are planned by one workgroup that reads the lengths and the reference counts, checks the whole
 // call, and only then writes: that makes a call all or nothing and its result independent of any order between
 // workgroups. Pages are copied by a second launch over the plan's list of moves.
 #include <algorithm>
 #include <string>
 
 #include "../../include/moa_paged.h"
+#include "moa_arrive.h"
 #include "moa_checks.h"
 #include "moa_device.h"
 #include "moa_paged.h"
@@ -443,28 +444,35 @@ __global__ __launch_bounds__(kCopyBlock) void paged_compact_kernel(PagedView c, 
 
 // ------------------------------------------------------------------------------------------- commit
 
-// A sequence's thread per node: the nodes that the accepted one sees, in order, become positions base, base + 1, ... of the
-// sequence, base the positions before the tree. The first of them may be there already (`still` of them); the others move:
-// nodes[s][m], the node of rank still + m. Then the state: the length, and the counts of the pages behind it, which are
-// the sequence's alone. A sequence that breaks a rule has no moves and keeps its state. Latency bounds it: starts, then the leaf's mask and
-// the pages, then their counts, 3.3 us for one sequence and 4 for 60, beside launches that the host sends 7 us apart.
-struct Commit { int moves, base, still, unused; };
+// A workgroup has a thread per node of its sequence: the nodes that the accepted one sees, in order, become positions base, base + 1, ... of the
+// sequence, base the positions before the tree. The first of them may be there already (`still` of them); the others move, one after the
+// other and eight at a time read before they are written: a target lies before its source, and so before every later source. A unit of
+// work is a layer's K or V and 256 chunks of 16 bytes of a position: its chunks of all moves are the same lanes', so no lane waits for another.
+// Every workgroup of a sequence finds the moves for itself; the last of them to arrive, when all have read the state, writes it: the length,
+// and the counts of the pages behind it, which are the sequence's alone. A sequence that breaks a rule has no moves and keeps its state.
+// Latency bounds it: starts, then the leaf's mask and the pages, their counts, the moves, the arrival. 8 layers of one path 5.6 us, 60 paths of 10
+// layers, 20 MB read and written, 8.8; a plan and the moves as two launches 3.3 + 4.0 and 4.0 + 6.3, and 15.5 us a call for 12.5 by the host.
+__host__ __device__ inline int commit_units(const PagedView& c, int elem) {
+    return 2 * c.layers * ((c.kv_heads * c.head_dim * elem / 16 + kCopyBlock - 1) / kCopyBlock);
+}
 
-__global__ __launch_bounds__(kTreeMaxNodes) void paged_commit_plan_kernel(PagedView c, const int32_t* starts, const uint64_t* masks, int words,
-                                                                          const int32_t* leaves, int rows, uint8_t* nodes, Commit* commits) {
-    const int s = blockIdx.x, i = threadIdx.x;
+__global__ __launch_bounds__(kCopyBlock) void paged_commit_kernel(PagedView c, const int32_t* starts, const uint64_t* masks, int words,
+                                                                  const int32_t* leaves, int rows, int first, uint32_t* tickets, int elem) {
+    static_assert(kCopyBlock == kTreeMaxNodes, "a thread per node");
+    __shared__ int2 place[kTreeMaxNodes];  // page and slot of every node
+    __shared__ uint8_t from[kTreeMaxNodes];  // the nodes that move
+    const int s = first + blockIdx.y, i = threadIdx.x;
     const int row0 = starts[s], end = starts[s + 1], len = c.lens[s], leaf = leaves[s];
-    if (i == 0) commits[s] = {0, 0, 0, 0};
     if (row0 == end) return;
     // (in this order: differences only of values that are in range)
     if (!rows_in_range(row0, end, rows, 64 * words) || len < end - row0 || len > paged_capacity(c) || leaf < -1 || leaf >= end - row0) {
-        if (i == 0) raise(c);
+        if (i == 0 && blockIdx.x == 0) raise(c);
         return;
     }
     const int n = end - row0, base = len - n;
     const int32_t* table = c.table + s * c.table_stride;
     int rank = 0, kept = 0;
-    bool mine = false;
+    bool mine = false, bad = false;
     for (int w = 0; w < words && leaf >= 0; ++w) {
         uint64_t m = masks[(int64_t)(row0 + leaf) * words + w];
         const int left = n - 64 * w;
@@ -473,71 +481,46 @@ __global__ __launch_bounds__(kTreeMaxNodes) void paged_commit_plan_kernel(PagedV
         if (i >> 6 > w) rank += __popcll(m);
         if (i >> 6 == w) rank += __popcll(m & ((1ull << (i & 63)) - 1)), mine = m >> (i & 63) & 1;
     }
-    bool bad = false;
     if (i < n) {
-        const int page = table[page_of(c, base + i)];
+        const int column = (int)page_of(c, base + i), page = table[column];
         bad = page < 0 || page >= c.pages || c.refs[page] != 1;
+        place[i] = make_int2(page, base + i - column * (int)c.slots);
     }
-    if (__syncthreads_or(bad)) {
-        if (i == 0) raise(c);
-        return;
-    }
+    bad = __syncthreads_or(bad);
     // (a rank is at most the node's number, and once below stays below)
-    const int still = __syncthreads_count(mine && rank == i);
-    if (mine && rank != i) nodes[s * kTreeMaxNodes + rank - still] = (uint8_t)i;
-    if (i == 0) {
-        commits[s] = {kept - still, base, still, 0};
-        c.lens[s] = base + kept;
-    }
-    for (int x = pages_of(c, base + kept) + i; x < pages_of(c, len); x += kTreeMaxNodes) c.refs[table[x]] = 0;
-}
-
-// Moves within a sequence go one after the other, eight at a time read before they are written: a target lies before its
-// source, and so before every later source. A unit of work is a sequence, a layer's K or V and 256 chunks of 16 bytes of a position: its chunks
-// of all moves are the same lanes', so no lane waits for another. (3.9 us for 8 layers of one path; 60 paths of 10 layers, 20 MB, 6.2.)
-__host__ __device__ inline int commit_parts(const PagedView& c, int elem) {
-    return (c.kv_heads * c.head_dim * elem / 16 + kCopyBlock - 1) / kCopyBlock;
-}
-
-__global__ __launch_bounds__(kCopyBlock) void paged_commit_kernel(PagedView c, const uint8_t* nodes, const Commit* commits, int elem) {
-    static_assert(kCopyBlock == kTreeMaxNodes, "a thread per move");
-    __shared__ int4 moves[kTreeMaxNodes];  // source page and slot, target page and slot
-    const int parts = commit_parts(c, elem), per_head = c.head_dim * elem / 16, per = parts * 2 * c.layers;
-    const int64_t units = (int64_t)c.sequences * per;
-    for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
-        const int s = (int)(u / per), r = (int)(u - (int64_t)s * per), tensor = r / parts;
-        const int node = nodes[s * kTreeMaxNodes + threadIdx.x];
-        const Commit m = commits[s];
-        if (m.moves == 0) continue;
-        __syncthreads();  // the unit before has read its moves
-        if ((int)threadIdx.x < m.moves) {
-            const int32_t* table = c.table + s * c.table_stride;
-            const int from = m.base + node, to = m.base + m.still + (int)threadIdx.x;
-            const int fc = (int)page_of(c, from), tc = (int)page_of(c, to);
-            moves[threadIdx.x] = make_int4(table[fc], from - fc * (int)c.slots, table[tc], to - tc * (int)c.slots);
-        }
-        __syncthreads();
-        const int chunk = (r - tensor * parts) * kCopyBlock + (int)threadIdx.x;
+    const int still = __syncthreads_count(mine && rank == i), moves = bad ? 0 : kept - still;
+    if (mine && rank != i) from[rank - still] = (uint8_t)i;
+    __syncthreads();
+    const int units = commit_units(c, elem), parts = units / (2 * c.layers), per_head = c.head_dim * elem / 16;
+    for (int u = blockIdx.x; u < units && moves; u += gridDim.x) {
+        const int tensor = u / parts, chunk = (u - tensor * parts) * kCopyBlock + i;
         if (chunk >= c.kv_heads * per_head) continue;
         const bool v = tensor & 1;
         const int h = chunk / per_head;
-        uint8_t* base = (v ? c.v + (int64_t)(tensor >> 1) * c.v_layer + h * c.v_head : c.k + (int64_t)(tensor >> 1) * c.k_layer + h * c.k_head) +
-                        (chunk - h * per_head) * 16;
+        uint8_t* at = (v ? c.v + (int64_t)(tensor >> 1) * c.v_layer + h * c.v_head : c.k + (int64_t)(tensor >> 1) * c.k_layer + h * c.k_head) +
+                      (chunk - h * per_head) * 16;
         const int64_t page = v ? c.v_page : c.k_page, slot = v ? c.v_slot : c.k_slot;
-        for (int m0 = 0; m0 < m.moves; m0 += 8) {
+        for (int m0 = 0; m0 < moves; m0 += 8) {
             uint4 w[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const int4 x = moves[min(m0 + j, m.moves - 1)];
-                w[j] = ld16(base + x.x * page + x.y * slot);
+                const int2 x = place[from[min(m0 + j, moves - 1)]];
+                w[j] = ld16(at + x.x * page + x.y * slot);
             }
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const int4 x = moves[min(m0 + j, m.moves - 1)];
-                if (m0 + j < m.moves) *reinterpret_cast<uint4*>(base + x.z * page + x.w * slot) = w[j];
+                const int2 x = place[still + min(m0 + j, moves - 1)];
+                if (m0 + j < moves) *reinterpret_cast<uint4*>(at + x.x * page + x.y * slot) = w[j];
             }
         }
     }
+    if (!arrive_last<kRowTurn>(tickets + (int64_t)blockIdx.y * kTicketStride, blockIdx.x == 0, gridDim.x)) return;
+    if (bad) {
+        if (i == 0) raise(c);
+        return;
+    }
+    if (i == 0) c.lens[s] = base + kept;
+    for (int x = pages_of(c, base + kept) + i; x < pages_of(c, len); x += kTreeMaxNodes) c.refs[table[x]] = 0;
 }
 
 // ------------------------------------------------------------------------------------------ reorder
@@ -1023,14 +1006,14 @@ int moa_paged_tree_commit(const moa_paged_cache* cache, const int32_t* row_start
     if (!ctx) return e;
     v.err = ctx->err;
     hipStream_t s = static_cast<hipStream_t>(stream);
-    uint8_t* nodes = reinterpret_cast<uint8_t*>(ctx->paged_chunks);
-    Commit* commits = reinterpret_cast<Commit*>(ctx->paged_list);
-    hipLaunchKernelGGL(paged_commit_plan_kernel, dim3(v.sequences), dim3(kTreeMaxNodes), 0, s, v, row_starts, masks, mask_words, leaves,
-                       rows, nodes, commits);
-    if ((e = call_result(hipGetLastError(), "paged_tree_commit launch"))) return e;
-    const int64_t units = (int64_t)v.sequences * v.layers * 2 * commit_parts(v, elem_bytes(cache));
-    hipLaunchKernelGGL(paged_commit_kernel, dim3(copy_grid(units, ctx->cus)), dim3(kCopyBlock), 0, s, v, nodes, commits, elem_bytes(cache));
-    return call_result(hipGetLastError(), "paged_tree_commit launch");
+    // a counter for each of a launch's sequences; of few sequences, as many workgroups as there are units, below a turn
+    for (int first = 0; first < v.sequences; first += kSearchRows) {
+        const int here = std::min(kSearchRows, v.sequences - first), most = std::min(commit_units(v, elem_bytes(cache)), (int)kRowTurn / 2);
+        hipLaunchKernelGGL(paged_commit_kernel, dim3(std::max(1, std::min(most, 8 * ctx->cus / here)), here), dim3(kCopyBlock), 0, s, v, row_starts, masks,
+                           mask_words, leaves, rows, first, ctx->search_tickets + (size_t)kSearchRows * kTicketStride, elem_bytes(cache));
+        if ((e = call_result(hipGetLastError(), "paged_tree_commit launch"))) return e;
+    }
+    return MOA_SUCCESS;
 }
 
 int moa_paged_cache_reorder(const moa_paged_cache* cache, const int32_t* parents, int count, int beams, void* stream) {

@@ -4,9 +4,9 @@
 #include <algorithm>
 
 #include "../../include/moa_search.h"
+#include "moa_arrive.h"
 #include "moa_checks.h"
 #include "moa_device.h"
-#include "moa_paged_plan.h"
 #include "moa_sync.h"
 
 namespace moa {
@@ -16,7 +16,7 @@ constexpr int kBlock = 256;
 constexpr int kGroupLogits = 64;        // logits that share a key (their largest): 8 lanes' 16 bytes
 constexpr int kSearchMaxVocab = 1 << 20;
 
-constexpr unsigned kGroupTurn = 128, kRowTurn = 512;  // of the counters of a group's rows, and of a row's parts and a call's rows
+constexpr unsigned kGroupTurn = 128;  // of the counters of a group's rows
 
 typedef short s16x2 __attribute__((ext_vector_type(2)));
 
@@ -76,21 +76,6 @@ constexpr int kMaxParts = kSearchMaxVocab / (kBlock * 8 * 2);
 __host__ __device__ inline int parts_of(int vocab, int loads) { return (vocab + kBlock * 8 * loads - 1) / (kBlock * 8 * loads); }
 
 // ---------------------------------------------------------------------------------------------- verify
-
-// Whether this workgroup is the last of `parts` to arrive at a counter; what the others published before is then there to
-// collect. kTurn: a power of two above any number of parts.
-template <unsigned kTurn>
-__device__ bool arrive_last(uint32_t* ticket, bool first, int parts) {
-    __shared__ uint32_t flag;
-    __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        const uint32_t share = join_share(first, parts, kTurn);
-        flag = join_last(__hip_atomic_fetch_add(ticket, share, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT), share, kTurn);
-    }
-    __syncthreads();
-    return flag;
-}
 
 // The largest logit of this workgroup's part of row blockIdx.y and its first place, as one number that orders by both, in thread 0.
 template <int kLoads>

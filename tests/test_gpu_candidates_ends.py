@@ -485,3 +485,10 @@ def test_sequences_shorter_than_their_trees(n, group, heads, dim, fmt):
             w = torch.softmax(torch.matmul(qh, kr) * scale, -1)
             check(out[s * n + i], torch.matmul(w, vr).reshape(heads * group, dim), torch.matmul(w, vr.abs()).reshape(heads * group, dim),
                   (torch.matmul(qh.abs(), kr.abs()) * scale).amax(-1).reshape(heads * group), dim)
+
+
+def test_commit_of_more_work_than_a_sequences_workgroups():
+    need_gpu()
+    say("commit of 20 layers of 33 heads of 512 dims")
+    st = Setup([12 + 20, 7], 4, 33, 512, layers=20)
+    run_commit(st, [20, 3], trees([20, 3], 2), [17, 2])
