@@ -125,8 +125,8 @@ int moa_paged_attention(const uint16_t* q, int64_t q_row_stride, const moa_paged
 /* Attention of the nodes: node i sees the positions before the tree (with a window, those less than `window` before its
  * own place as above) and the nodes of its mask. Everything else is as in moa_paged_attention, whose last bits a chain's
  * rows need not have. A row without bits gives zeros; nodes that would stand before position 0 are not there. Sequences
- * without a tree take part with trees of one node. max_rows is at most 64 * mask_words; window is 0 or at least
- * max_rows. */
+ * without a tree take part with trees of one node. max_rows is at most 64 * mask_words (the lesser of that and rows is
+ * always right); window is 0 or at least max_rows. */
 int moa_paged_tree_attention(const uint16_t* q, int64_t q_row_stride, const moa_paged_cache* cache,
                              const int32_t* row_starts, const uint64_t* masks, int mask_words, uint16_t* out,
                              int64_t out_row_stride, int rows, int q_heads, int layer, int window, float scale, int max_rows,

@@ -23,6 +23,7 @@
 
 #include <hip/hip_runtime_api.h>
 
+#include <algorithm>
 #include <cstddef>
 #include <cstdint>
 #include <limits>
@@ -603,7 +604,7 @@ inline void paged_attention(const Device& device, const HbmTensor<bf16>& q, cons
 }
 
 // Drafted trees over the paged cache. masks [rows, words], 1 to 4 words a row: bit j of a node's row stands for node j of its sequence.
-// q, out [rows, q_heads, head_dim] (out may be q); max_rows: the most rows a sequence has, 0: all (at most 64 * words).
+// q, out [rows, q_heads, head_dim] (out may be q); max_rows: the most rows a sequence has, at most 64 * words and all rows, 0: that many.
 template <class T>
 inline void paged_tree_attention(const Device& device, const HbmTensor<bf16>& q, const PagedCache<T>& cache,
                                  const HbmTensor<int32_t>& row_starts, const HbmTensor<uint64_t>& masks, HbmTensor<bf16>& out,
@@ -617,7 +618,7 @@ inline void paged_tree_attention(const Device& device, const HbmTensor<bf16>& q,
     want(out, q.size(), "out"); want(row_starts, cache.sequences() + 1, "row_starts");
     device.make_current();
     check(moa_paged_tree_attention(u16(q), width, cache.get(), row_starts.data(), masks.data(), words, u16(out), width, M, heads, layer,
-                                   window, scale, max_rows ? max_rows : M, device.stream()),
+                                   window, scale, max_rows ? max_rows : std::min(M, 64 * std::clamp(words, 1, 4)), device.stream()),
           "paged_tree_attention");
 }
 

@@ -530,7 +530,8 @@ def paged_tree_attention(q, cache, row_starts, masks, out, layer=0, window=0, sc
     """Attention of drafted trees, appended as their sequences' last positions: row i of a sequence's n is node i, at position
     seq_lens[s] - n + i, and sees the positions before the tree and the nodes of its mask (int64 [rows, words], 1 to 4 words; bit
     j % 64 of word j // 64: node j, itself among them). A window (0, or at least max_rows) counts from a node's depth, the number of
-    nodes that it sees. A row without bits gives zeros. Otherwise as paged_attention; max_rows is at most 64 * words (default: all rows)."""
+    nodes that it sees. A row without bits gives zeros. Otherwise as paged_attention; max_rows, the most rows a sequence has, is at most
+    64 * words and the rows of the call, the default where it is not said (so a smaller window asks for a max_rows of its own)."""
     p = _index(row_starts, "row_starts", cache, ("sequences", 1))
     qp, qr, rows = _row_tensor(q, "q", cache, None)
     op, orow, orows = _row_tensor(out, "out", cache, q.shape[1])
@@ -538,7 +539,7 @@ def paged_tree_attention(q, cache, row_starts, masks, out, layer=0, window=0, sc
         raise ValueError(f"out: expected {rows} rows, got {orows}")
     mp, words = _masks(masks, rows, cache.device_index)
     _call("moa_paged_tree_attention", qp, qr, cache._struct, p, mp, words, op, orow, rows, q.shape[1], layer, window, scale,
-          rows if max_rows is None else max_rows, _cache_stream(cache))
+          min(rows, 64 * max(words, 1)) if max_rows is None else max_rows, _cache_stream(cache))
 
 
 def paged_tree_commit(cache, row_starts, masks, leaves) -> None:
