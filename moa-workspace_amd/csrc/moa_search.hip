@@ -249,9 +249,10 @@ __global__ __launch_bounds__(kBlock) void verify_few_kernel(VerifyCall c, uint64
 
 // What a selection keeps of each row of a launch: the keys of its groups of logits, its parts' maxima and sums, its candidates, and the
 // counters of what has arrived.
+struct PartSum { double sum; float ref; };  // the sum of e^(logit - ref)
 struct SelectScratch {
     uint16_t* keys;        // [rows][key_stride]: the largest logit of a group, ordered() + 32768
-    float2* parts;         // [rows][parts_n]: a reference, the sum of e^(logit - reference)
+    PartSum* parts;        // [rows][parts_n]
     uint64_t* totals;      // [rows][beams] f64, descending
     uint32_t* places;      // [rows][beams]
     uint32_t* tickets;     // a line for every group of beams
@@ -275,7 +276,8 @@ __device__ __forceinline__ bool grows(const SelectCall& c, int row) { return c.f
 template <int kLoads>
 __global__ __launch_bounds__(kBlock) void select_scan_kernel(SelectCall c, SelectScratch k) {
     constexpr int kGroups = kBlock * kLoads / 8;  // of a part
-    __shared__ float top[4], sums[4];
+    __shared__ double sums[4];
+    __shared__ float top[4];
     __shared__ __attribute__((aligned(8))) uint16_t keys[kGroups];
     const int r = blockIdx.y;
     if (!grows(c, c.row0 + r)) return;
@@ -285,8 +287,11 @@ __global__ __launch_bounds__(kBlock) void select_scan_kernel(SelectCall c, Selec
 #pragma unroll
     for (int j = 0; j < kLoads; ++j) w[j] = row.chunk(first + j * kBlock, kMinusInfinity);
     // The lane's sum stands against a reference that follows its largest logit so far, so that its first chunks are summed while the
-    // others are on their way. A difference of two logits is exact or its exponential nothing beside the sum.
-    float m = -INFINITY, sum = 0.0f;
+    // others are on their way. It is f64 from the first exponential on: beside a logit that stands out every other one can be below f32's
+    // last bit, and a beam whose total differs by their sum would come in the wrong place. (151 rows of 262144: 1 us more a call than f32
+    // sums, 0.6 with exponentials added in pairs first.)
+    float m = -INFINITY;
+    double sum = 0.0;
 #pragma unroll
     for (int j = 0; j < kLoads; ++j) {
         float x[8];
@@ -295,12 +300,12 @@ __global__ __launch_bounds__(kBlock) void select_scan_kernel(SelectCall c, Selec
 #pragma unroll
         for (int i = 1; i < 8; ++i) most = fmaxf(most, x[i]);
         if (most > m + kSlack) {
-            sum *= __builtin_amdgcn_exp2f((m - most) * kLog2e);
+            sum *= (double)__builtin_amdgcn_exp2f((m - most) * kLog2e);
             m = most;
         }
         const float ref = m == -INFINITY ? 0.0f : m;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sum += __builtin_amdgcn_exp2f((x[i] - ref) * kLog2e);
+        for (int i = 0; i < 8; ++i) sum += (double)__builtin_amdgcn_exp2f((x[i] - ref) * kLog2e);
 #pragma unroll
         for (int o = 1; o < 8; o *= 2) most = fmaxf(most, __shfl_xor(most, o, kWave));
         if ((lane & 7) == 0) keys[(j * kBlock + threadIdx.x) / 8] = (uint16_t)(ordered(__float_as_uint(most) >> 16)[0] + 32768);
@@ -308,7 +313,9 @@ __global__ __launch_bounds__(kBlock) void select_scan_kernel(SelectCall c, Selec
     float all = m;
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) all = fmaxf(all, __shfl_xor(all, o, kWave));
-    sum = wave_sum(m == -INFINITY ? sum : sum * __builtin_amdgcn_exp2f((m - all) * kLog2e));  // (a NaN in a lane without a finite logit stays)
+    if (m > -INFINITY) sum *= (double)__builtin_amdgcn_exp2f((m - all) * kLog2e);  // (a NaN in a lane without a finite logit stays)
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, kWave);
     if (lane == 0) top[wave] = all, sums[wave] = sum;
     __syncthreads();
     const int at = (int)blockIdx.x * kGroups + 4 * (int)threadIdx.x;  // four keys a thread
@@ -316,10 +323,10 @@ __global__ __launch_bounds__(kBlock) void select_scan_kernel(SelectCall c, Selec
         *reinterpret_cast<uint64_t*>(k.keys + (int64_t)r * k.key_stride + at) = reinterpret_cast<const uint64_t*>(keys)[threadIdx.x];
     if (threadIdx.x == 0) {
         const float part = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-        float total = 0.0f;
+        double total = 0.0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) total += top[i] == -INFINITY ? sums[i] : sums[i] * __builtin_amdgcn_exp2f((top[i] - part) * kLog2e);
-        k.parts[(int64_t)r * k.parts_n + blockIdx.x] = make_float2(part, total);
+        for (int i = 0; i < 4; ++i) total += top[i] == -INFINITY ? sums[i] : sums[i] * (double)__builtin_amdgcn_exp2f((top[i] - part) * kLog2e);
+        k.parts[(int64_t)r * k.parts_n + blockIdx.x] = {total, part};
     }
 }
 
@@ -392,10 +399,10 @@ __device__ void select_row(const SelectCall& c, const SelectScratch& k, int r) {
         publish32(places + i, (uint32_t)place);
     };
     constexpr int kMost = kMaxParts / kWave;
-    float2 part[kMost];  // the row's sums, in every wave
+    PartSum part[kMost];  // the row's sums, in every wave
 #pragma unroll
     for (int i = 0; i < kMost; ++i)
-        part[i] = i * kWave + lane < k.parts_n ? k.parts[(int64_t)r * k.parts_n + i * kWave + lane] : make_float2(-INFINITY, 0.0f);
+        part[i] = i * kWave + lane < k.parts_n ? k.parts[(int64_t)r * k.parts_n + i * kWave + lane] : PartSum{0.0, -INFINITY};
     constexpr uint32_t kLeast = kLowestFinite + 32768;
     const uint16_t* keys = k.keys + (int64_t)r * k.key_stride;
     uint64_t four[kKeys / 4];  // (of a row that adds none: of an earlier call)
@@ -444,13 +451,13 @@ __device__ void select_row(const SelectCall& c, const SelectScratch& k, int r) {
     if (t >= 3 * kWave) {  // the row's sum, by the wave that has no logits of up to 24 beams
         float m = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < kMost; ++i) m = fmaxf(m, part[i].x);
+        for (int i = 0; i < kMost; ++i) m = fmaxf(m, part[i].ref);
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, kWave));
         double sum = 0.0;
 #pragma unroll
         for (int i = 0; i < kMost; ++i)
-            sum += part[i].x == -INFINITY ? (double)part[i].y : (double)part[i].y * (double)__builtin_amdgcn_exp2f((part[i].x - m) * kLog2e);
+            sum += part[i].ref == -INFINITY ? part[i].sum : part[i].sum * (double)__builtin_amdgcn_exp2f((part[i].ref - m) * kLog2e);
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, kWave);
         if (lane == 0) row_lse = sum > 0.0 && sum < INFINITY && m < INFINITY ? (double)m + log(sum) : -INFINITY;
@@ -593,14 +600,14 @@ int moa_beam_select(const uint16_t* logits, int64_t logit_row_stride, const floa
     k.key_stride = (k.groups + 3) / 4 * 4;
     k.parts_n = parts_of(vocab, loads);
     // the groups of rows that the scratch and its counters hold at once
-    const size_t row_bytes = (size_t)beams * 12 + (size_t)k.parts_n * 8 + (size_t)k.key_stride * 2;
+    const size_t row_bytes = (size_t)beams * 12 + (size_t)k.parts_n * sizeof(PartSum) + (size_t)k.key_stride * 2;
     const int most = (int)std::min<size_t>(groups, std::min<size_t>(kSearchBytes / (row_bytes * beams), kSearchRows / beams));
     uint8_t* at = reinterpret_cast<uint8_t*>(ctx->paged_chunks);
     const size_t held = (size_t)most * beams;
     k.totals = reinterpret_cast<uint64_t*>(at);
-    k.parts = reinterpret_cast<float2*>(at + held * beams * 8);
-    k.keys = reinterpret_cast<uint16_t*>(at + held * (beams * 8 + k.parts_n * 8));
-    k.places = reinterpret_cast<uint32_t*>(at + held * (beams * 8 + k.parts_n * 8 + k.key_stride * 2));
+    k.parts = reinterpret_cast<PartSum*>(at + held * beams * 8);
+    k.keys = reinterpret_cast<uint16_t*>(at + held * (beams * 8 + k.parts_n * sizeof(PartSum)));
+    k.places = reinterpret_cast<uint32_t*>(at + held * (beams * 8 + k.parts_n * sizeof(PartSum) + k.key_stride * 2));
     k.tickets = ctx->search_tickets;
     auto* scan = loads == 4 ? select_scan_kernel<4> : select_scan_kernel<2>;
     auto* pick = k.groups > 16 * kBlock ? select_rows_kernel<64> : select_rows_kernel<16>;
