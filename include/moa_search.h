@@ -34,14 +34,15 @@ int moa_tree_verify(const uint16_t* logits, int64_t logit_row_stride, const int3
  * log sum_t e^logits[t]; a finished beam (finished[row] not 0) has the one candidate `eos` at its score, and its logits
  * are not read. The `beams` best of a group, ties to the lowest row and then the lowest token, become its rows in
  * descending order: out_scores, parents (the row that it comes from, as moa_paged_cache_reorder takes it), tokens, and
- * out_finished (1 where the parent is finished or the token is eos, else 0). Candidates at -infinity or NaN are none (so
- * is every one of a row that holds a NaN or +infinity, or no finite logit): a row that is left without one is finished,
- * its own parent, at -infinity, with token max(eos, 0). eos: below vocab, or -1 where no token ends a beam (then no beam
- * may be finished: it has no candidate). out_scores may be scores and out_finished may be finished. f32 arrays and int32
- * arrays are [groups * beams]. Sums and totals are f64, and the scores are rounded once. Exponentials are f32: that of
- * a logit d below its row's largest is off by at most (d + 6) 2^-22 of itself, the logarithm of their sum by less than
- * 2^-17, so totals of two rows that lie closer can change places; equal rows have equal sums. Where a row's totals are
- * equal, since its score leaves no bit to its logits, the larger logit comes first. groups may be 0. */
+ * out_finished (1 where the parent is finished or the token is eos, else 0). Candidates at -infinity (a total that rounds
+ * to it as a score among them) or NaN are none (so is every one of a row that holds a NaN or +infinity, or no finite
+ * logit): a row that is left without one is finished, its own parent, at -infinity, with token max(eos, 0). eos: below
+ * vocab, or -1 where no token ends a beam (then no beam may be finished: it has no candidate). out_scores may be scores and
+ * out_finished may be finished. f32 arrays and int32 arrays are [groups * beams]. Sums and totals are f64, and the scores
+ * are rounded once. Exponentials are f32: that of a logit d below its row's largest is off by at most (d + 6) 2^-22 of
+ * itself, the logarithm of their sum by less than 2^-17, so totals of two rows that lie closer can change places; equal
+ * rows have equal sums. Where a row's totals are equal, since its score leaves no bit to its logits, the larger logit
+ * comes first. groups may be 0. */
 int moa_beam_select(const uint16_t* logits, int64_t logit_row_stride, const float* scores, const int32_t* finished,
                     float* out_scores, int32_t* out_finished, int32_t* parents, int32_t* tokens, int groups, int beams,
                     int vocab, int eos, void* stream);

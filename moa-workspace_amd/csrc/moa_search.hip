@@ -480,7 +480,8 @@ __device__ void select_merge(const SelectCall& c, const SelectScratch& k, int r0
     for (int i = threadIdx.x; i < c.beams * c.beams; i += kBlock) {
         const uint64_t b = collect64(k.totals + (int64_t)r0 * c.beams + i);
         tokens[i] = __hip_atomic_load(k.places + (int64_t)r0 * c.beams + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        orders[i] = __builtin_bit_cast(double, b) > -INFINITY ? (b >> 63 ? ~b : b | 1ull << 63) : 0;
+        // (a total below f32's range would be a score of -infinity)
+        orders[i] = (float)__builtin_bit_cast(double, b) > -INFINITY ? (b >> 63 ? ~b : b | 1ull << 63) : 0;
     }
     __syncthreads();
     if (threadIdx.x >= kWave) return;
