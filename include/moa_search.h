@@ -5,7 +5,7 @@
  * No counterpart in the reference, which copies one row of logits to the host and samples there
  * (FO/src/host/generate.rs:129-134). logits are bf16 [rows][vocab], rows logit_row_stride elements apart (at least
  * vocab); vocab may be any number up to 2^20, rows at most 65535. Results are deterministic. The calls share the paged
- * calls' scratch: one stream at a time.
+ * calls' scratch (moa_paged.h; the first call of either kind allocates its 100 MB): one stream at a time.
  */
 #ifndef MOA_SEARCH_H
 #define MOA_SEARCH_H

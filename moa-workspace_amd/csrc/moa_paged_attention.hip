@@ -130,6 +130,7 @@ __device__ __forceinline__ int chunk_units(const A& a, const Seq& q) {
 // them, leaves workgroups idle (12 sequences of 5 to 8 tiles over 900 to 16000 positions of 512 dims: parts of two even shares, 580 us).
 // Each lane tries a fraction of the longest tile, 1 to 1/8.75 in fine steps and on to 1/258: parts that run all at once take one part's time, others their
 // sum's share and half a part's more; a part costs kTreePartUnits besides (its start, its record, the merge). The best that leaves few enough records is taken.
+// (The model and its constant were set by that one batch alone: 365 us.)
 constexpr float kTreePartUnits = 6.0f;
 __device__ int tree_part_units(const PagedView& c, const PagedTreeCall& a, const ChunkPlan& p, const Seq& last) {
     const int lane = threadIdx.x & 63;
@@ -633,7 +634,9 @@ __device__ __forceinline__ int in_loop(int v) {
 // load into LDS before them (512 dims, 1000 rows over 15800 positions: three such reloads a tile cost 24 us). What the chunk kernels
 // still spill (32 and 46 registers at 256 dims, bf16 and E4M3, 24 and 52 at 512) lies outside that loop, but for one reload a tile before
 // each of the products at 256 dims and, with E4M3 pages, for five at 256 dims and three at 512; seen positions computed in the loop instead
-// of held took one away: 148 us for 152 there, 1 % more elsewhere, and were left out.
+// of held took one away: 148 us for 152 there, 1 % more elsewhere, and were left out. Those are the calls without trees. The kernels of trees spill 36
+// and 57 at 256 dims, 35 and 55 at 512, and read some of them in the branch for tiles that a row does not see whole; a row without bits sends
+// every tile of its wave there.
 __device__ __forceinline__ int lane_here() {
     int v;
     __asm__ volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(v));

@@ -1,6 +1,6 @@
 // moa_search.hip -- tokens from logits (include/moa_search.h): the greedy verification of drafted trees, and the selection of
-// beams. Both read every row of bf16 logits once, at the rate of memory (524 rows of 262144, 275 MB: 43 us, 6.4 TB/s; the 151 live rows of a
-// selection, with exponentials beside, 79 MB: 17 us, 4.6 TB/s); what is left of a row then fits a workgroup.
+// beams. Both read every row of bf16 logits once, at the rate of memory (524 rows of 262144, 275 MB: 45 us, 6.1 TB/s; the 151 live rows of a
+// selection, with exponentials and their f64 sums beside, 79 MB: 19 us, 4.2 TB/s); what is left of a row then fits a workgroup.
 #include <algorithm>
 
 #include "../../include/moa_search.h"
@@ -217,7 +217,9 @@ __global__ __launch_bounds__(kBlock) void verify_walk_kernel(VerifyCall c, const
 }
 
 // Few rows and sequences in one launch: the last part of a row to arrive names its token, the last row's workgroup walks, a wave per
-// sequence. (8 rows of 262144 logits, one sequence: scan and walk as two launches 13.6 us a call, 11.0 so.)
+// sequence. Against scan and walk as two launches, one sequence, us a call here / there at 8, 33, 64, 128 and 256 rows: 262144 logits 8.6 / 11.3,
+// 9.1 / 11.4, 12.9 / 16.3, 20.6 / 27.6, 34.5 / 49.3; 32000 logits 8.8 / 11.5 up to 128 rows, 11.6 / 11.4 at 256. As a graph's nodes,
+// where a second launch costs little, up to 8 rows are level at 262144 (6.8 both) and 32000 logits 0.6 to 0.9 slower (7.1 / 6.4 at 64).
 constexpr int kFewSequences = 4;
 template <int kWords>
 __global__ __launch_bounds__(kBlock) void verify_few_kernel(VerifyCall c, uint64_t* part, uint32_t* row_best, uint32_t* tickets) {
@@ -515,8 +517,8 @@ __device__ void select_merge(const SelectCall& c, const SelectScratch& k, int r0
     c.out_finished[row] = out_done;
 }
 
-// A workgroup per row; the last of a group picks its beams. Latency bounds it (keys, logits of the groups found, arrival, candidates: 10.4 us for
-// one group of 4, 12.2 for 20 of 8); one row of a group after the other in one workgroup would take its steps in turn.
+// A workgroup per row; the last of a group picks its beams. Latency bounds it (keys, logits of the groups found, arrival, candidates: 10.3 us for
+// one group of 4, 12.6 for 20 of 8); one row of a group after the other in one workgroup would take its steps in turn.
 template <int kKeys>
 __global__ __launch_bounds__(kBlock) void select_rows_kernel(SelectCall c, SelectScratch k) {
     const int r = blockIdx.x, g = r / c.beams;
@@ -533,8 +535,8 @@ int check_logits(const uint16_t* logits, int64_t stride, int rows, int vocab) {
     return MOA_SUCCESS;
 }
 
-// Loads of a thread: four where two workgroups a CU are left then, else two, for more workgroups. (151 rows of 262144: 17.5 us with four, 18.7 with
-// eight.)
+// Loads of a thread: four where two workgroups a CU are left then, else two, for more workgroups. (Selection of 20 groups of 8 beams of 262144, us a
+// call: 29.7 with four, 31.0 with two, 31.3 with eight; of one group of 4: 13.5 with two, 15.5 with eight.)
 int loads_of(int64_t rows, int vocab, int cus) { return rows * parts_of(vocab, 4) >= 2 * (int64_t)cus ? 4 : 2; }
 
 static_assert(kMaxParts < (int)kRowTurn && kTreeMaxNodes < (int)kRowTurn && kTreeMaxNodes < kSearchRows && kMaxBeams < (int)kGroupTurn, "arrivals are fewer than a turn");

@@ -4,9 +4,9 @@
 // workgroup's waves, and two tiles the 65 to 128 rows that still come here. K and V go through LDS (moa_tree_rows.h says how). The positions are dealt
 // out evenly over as many workgroups as the device holds, and the rows of tiles that were split so are joined by a second launch.
 //
-// Measured, 40 trees of 9 to 33 nodes with 2 x 256 dims a KV head, bf16: 318 MB of K and V in 67 us, 4.7 TB/s, and 8 us of the merge. 32 trees of
-// 5 to 16 nodes with 4 x 128 dims over E4M3 pages: 265 MB in 83 us and 10; loads, widening and the stores to LDS alone take 50, the products and
-// the softmax, of three to four waves behind one barrier a tile, the rest. Dealing by (KV head, positions) in the other order, other
+// Measured, 40 trees of 9 to 33 nodes with 2 x 256 dims a KV head, bf16: 318 MB of K and V in 72 us, 4.4 TB/s, and 7 us of the merge. 32 trees of
+// 5 to 16 nodes with 4 x 128 dims over E4M3 pages: 265 MB in 79 us and 10; loads, widening and the stores to LDS alone took 50 of 85, the products
+// and the softmax, of two to four waves behind one barrier a tile, the rest. Dealing by (KV head, positions) in the other order, other
 // places of the row groups among the waves, and twice the workgroups on a CU (tiles of 32 positions) changed nothing or were slower.
 #include <algorithm>
 

@@ -14,6 +14,8 @@ constexpr int kTreeRows = 64;      // of a tile: 16 for each of four waves
 // 145 / 207, 200 / 261, 225 / 240, 266 / 266; 256 dims E4M3 105 / 185, 154 / 247, 171 / 213, 262 / 260; 128 dims bf16 81 / 89, 95 / 100, 146 / 134,
 // 164 / 167; 128 dims E4M3 61 / 77, 79 / 98, 121 / 128, 160 / 157. One sequence of 4000 positions, 100 rows: 27 / 46 (256 dims), 22 / 27 (128).
 // Rows of 512 dims took 590 us here and 376 there (12 sequences of up to 16000 positions): half the registers of a wave hold its output.
+// One bound for all types and dims, though 128 dims bf16 change sides between 64 and 100 rows (9 % at 100) and E4M3 at 128 (2 %). It is compared
+// with the call's max_rows: a batch with one larger tree goes to the chunk kernel whole.
 constexpr int kTreeMaxRows = 128;
 
 template <int D, bool E4M3>
@@ -24,8 +26,8 @@ struct TreeShape {
     static constexpr int kSub = kTile / 16;
     static constexpr int kRowBytes = 2 * D;                  // LDS row of a position
     static constexpr int kStage = 2 * kTile * kRowBytes;
-    // Two workgroups share a CU's 160 KB. bf16: tiles on their way or there. E4M3: two tiles as bf16, and kAhead tiles of codes on their way
-    // in registers, 32 of them.
+    // Two workgroups share a CU's 160 KB. bf16: the tile in use and those on their way, five of 16 KB up to 128 dims, two of 32 KB at 256.
+    // E4M3: two tiles as bf16, and kAhead tiles of codes on their way in registers, 32 of them (at 256 dims 18 registers spill, 44 bytes a lane).
     static constexpr int kStages = E4M3 ? 2 : 80 * 1024 / kStage;
     static constexpr int kLds = kStages * kStage;
     static constexpr int kAhead = D == 64 ? 4 : 2;
@@ -67,7 +69,9 @@ __device__ __forceinline__ float rows_max(float x) {
 // between no lanes, and a row's maximum, sum and outputs are its lanes'. P enters as two bf16 parts, which share V's fragments.
 //
 // bf16 tiles go from memory to LDS directly, into a ring of stages with one barrier a tile: the matrix cores and LDS have a third of the time that
-// memory takes, so what counts is that loads never pause. E4M3 codes wait in registers and are widened on their way to LDS.
+// memory takes, so what counts is that loads pause as little as can be. At 64 and 128 dims three tiles stay on their way while a wave waits
+// for one; at 256 dims, two stages, the next tile is asked for behind the wait and the barrier, and in between only the CU's other workgroup's loads
+// are. E4M3 codes wait in registers and are widened on their way to LDS.
 template <int D, bool E4M3>
 __device__ __forceinline__ void tree_rows(const PagedView& c, const PagedTreeCall& a, const Piece& t, int kvh, int lo, int hi, float* rec, uint8_t* lds) {
     using T = TreeShape<D, E4M3>;
