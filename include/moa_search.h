@@ -40,9 +40,9 @@ int moa_tree_verify(const uint16_t* logits, int64_t logit_row_stride, const int3
  * vocab, or -1 where no token ends a beam (then no beam may be finished: it has no candidate). out_scores may be scores and
  * out_finished may be finished. f32 arrays and int32 arrays are [groups * beams]. Sums and totals are f64, and the scores
  * are rounded once. Exponentials are f32: that of a logit d below its row's largest is off by at most (d + 6) 2^-22 of
- * itself, the logarithm of their sum by less than 2^-17, so totals of two rows that lie closer can change places; equal
- * rows have equal sums. Where a row's totals are equal, since its score leaves no bit to its logits, the larger logit
- * comes first. groups may be 0. */
+ * itself (below 2^-126 it may be 0), the logarithm of their sum by less than 2^-17, so totals of two rows that lie closer
+ * can change places; equal rows have equal sums. Where a row's totals are equal, since its score leaves no bit to its
+ * logits, the larger logit comes first. groups may be 0. */
 int moa_beam_select(const uint16_t* logits, int64_t logit_row_stride, const float* scores, const int32_t* finished,
                     float* out_scores, int32_t* out_finished, int32_t* parents, int32_t* tokens, int groups, int beams,
                     int vocab, int eos, void* stream);

@@ -249,9 +249,11 @@ __global__ __launch_bounds__(kBlock) void verify_few_kernel(VerifyCall c, uint64
 
 // ---------------------------------------------------------------------------------------------- select
 
-// What a selection keeps of each row of a launch: the keys of its groups of logits, its parts' maxima and sums, its candidates, and the
-// counters of what has arrived.
-struct PartSum { double sum; float ref; };  // the sum of e^(logit - ref)
+// Of a part of a row: the sum of e^(logit - ref), ref its lanes' largest reference.
+struct PartSum { double sum; float ref; };
+
+// What a selection keeps of each row of a launch: the keys of its groups of logits, its parts' sums, its candidates, and the counters of
+// what has arrived.
 struct SelectScratch {
     uint16_t* keys;        // [rows][key_stride]: the largest logit of a group, ordered() + 32768
     PartSum* parts;        // [rows][parts_n]
